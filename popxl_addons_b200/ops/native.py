@@ -1824,3 +1824,4 @@ def _register_late():
 _register_late()
 
 from . import native_sequence  # noqa: E402,F401  (kernels of the sequence-model ops)
+from . import native_serving  # noqa: E402,F401  (kernels of the serving ops)

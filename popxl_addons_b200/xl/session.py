@@ -299,6 +299,15 @@ class Session:
                                      f"{var.shape_on_host} ({var})")
             self._write_var(var, host)
 
+    def device_tensor(self, var: Variable) -> torch.Tensor:
+        """The tensor that holds `var` on the session's device: a view, not a copy. It stays where it is for the life of the
+        session, so it can be read and written between runs, in stream order. One local replica only."""
+        if var.remote_buffer is not None or self.num_local != 1:
+            raise ValueError(f"{var} has no single tensor on the device (remote, or simulated on several replicas)")
+        if var not in self._vars:
+            raise KeyError(f"{var} is not held by this process")
+        return self._vars[var][0]
+
     # popxl names
     def weights_to_host(self):
         pass
@@ -1009,9 +1018,10 @@ class Session:
         return out
 
     def run_program(self, program, inputs: Optional[Mapping[HostToDeviceStream, Any]] = None,
-                    fetch: bool = True) -> Dict[DeviceToHostStream, np.ndarray]:
+                    fetch: bool = True, copy: bool = True) -> Dict[DeviceToHostStream, np.ndarray]:
         """Execute a `Program` once; inputs, outputs and `fetch` as in `run`. The first run is eager (lazy
-        initialisation); a capturable program is captured into a CUDA graph at its second run and replayed from then on."""
+        initialisation); a capturable program is captured into a CUDA graph at its second run and replayed from then on.
+        With `fetch=False, copy=False` the outputs may be the program's own buffers, which its next run overwrites."""
         self._outputs = {}
         state = self._programs.get(program)
         capturable = (program.capture and self.device.type == "cuda" and self.num_local == 1 and self.profile is None
@@ -1027,7 +1037,7 @@ class Session:
                 state["graph"].replay()
                 _native.count_replay(state["kernels"])
                 # outputs that are read before anything else can replay the program need no copy of their own
-                self._after_replay(state, copy=not fetch)
+                self._after_replay(state, copy=copy and not fetch)
             else:
                 vals = [self._value(t, {}) for t in program.bindings.values()]
                 with _read_ahead.following(self._launch_order(program.graph)):
