@@ -1,13 +1,18 @@
 """CUDA implementations of the serving ops (`xl/ops/serving.py`)."""
+import ctypes
+
 import torch
 
 from ..xl.opdef import native
 from .native import _CODE, _c_f, _c_int, _c_ll, _c_p, _check, _count, _ok, _sig, _stream, counters
 from .native_sequence import _clamped_glu, _f32, _i32, _ptr, stream_rms
 
+_c_d = ctypes.c_double
 _shape_logits = _sig("xl_shape_logits", *[_c_p] * 10, *[_c_int] * 7, _c_p)
 _take_shaped = _sig("xl_take_shaped", *[_c_p] * 13, *[_c_int] * 11, _c_p)
 _append_tokens = _sig("xl_append_tokens", _c_p, _c_p, _c_p, _c_p, _c_int, _c_int, _c_int, _c_p)
+_q8_append = _sig("xl_q8_append", _c_p, _c_ll, *[_c_p] * 13, *[_c_int] * 7, _c_d, _c_int, _c_p)
+_q8_general = _sig("xl_q8_attn_general", *[_c_p] * 8, _c_ll, _c_p, _c_ll, _c_p, _c_p, *[_c_int] * 9, _c_f, _c_f, _c_int, _c_p)
 
 
 def _launched(rc, name) -> bool:
@@ -75,3 +80,30 @@ def append_tokens_cuda(history, tokens, pos, count, T):
     rc = _append_tokens(history.data_ptr(), tokens.data_ptr(), pos.data_ptr(), count.data_ptr(), history.shape[0], T, history.shape[1],
                         _stream())
     return history if _launched(rc, "append_tokens") else NotImplemented
+
+
+@native("window_attention_q8_")
+def window_attention_q8_cuda(proj, q_norm, k_norm, k, v, k_scale, v_scale, k_tail, v_tail, pos, count, joint, T, heads, window,
+                             keep_first, scale, sink, eps):
+    B, G, blocks, _, dim = k.shape
+    vdim, dt, dev = v.shape[-1], proj.dtype, proj.device
+    plain = (heads + G) * dim + G * vdim
+    if not _ok(k_tail, v_tail, joint, q_norm, k_norm) or not _f32(q_norm, k_norm, k_scale, v_scale) or not _i32(pos, count):
+        return NotImplemented
+    if not (dt == k_tail.dtype == v_tail.dtype == joint.dtype) or proj.stride(1) != 1 or proj.shape[0] != B * T or not proj.is_cuda:
+        return NotImplemented
+    if any(not t.is_contiguous() for t in (k, v, k_scale, v_scale)):
+        return NotImplemented
+    code, s, ld, ldo = _CODE[dt], _stream(), proj.stride(0), joint.stride(0)
+    sink = float("-inf") if sink is None else sink
+    gate = proj.data_ptr() + plain * proj.element_size() if proj.shape[1] > plain else None
+    cache = tuple(t.data_ptr() for t in (k, v, k_scale, v_scale))
+    q = torch.empty((B, G, T, heads // G, dim), dtype=torch.float32, device=dev)
+    raw = [torch.empty((B, G, T + 64, width), dtype=dt, device=dev) for width in (dim, vdim)]
+    rc = _q8_append(proj.data_ptr(), ld, q_norm.data_ptr(), k_norm.data_ptr(), q.data_ptr(), raw[0].data_ptr(), raw[1].data_ptr(), *cache,
+                    k_tail.data_ptr(), v_tail.data_ptr(), pos.data_ptr(), count.data_ptr(), B, T, heads, G, dim, vdim, blocks, eps, code, s)
+    if not _launched(rc, "q8_append"):
+        return NotImplemented
+    rc = _q8_general(q.data_ptr(), raw[0].data_ptr(), raw[1].data_ptr(), *cache, gate, ld, joint.data_ptr(), ldo, pos.data_ptr(),
+                     count.data_ptr(), B, T, heads, G, dim, vdim, blocks, window, keep_first, scale, sink, code, s)
+    return joint if _launched(rc, "q8_attn_general") else NotImplemented

@@ -33,19 +33,19 @@ def q8_attention(rows, q_norm, k_norm, heads, G, dim, vdim, window, keep, scale,
             for held, x in ((kq, k), (vq, v)):
                 codes, step = block_codes(x[lo:lo + BLOCK, g])
                 held[lo:lo + BLOCK, g] = codes * step.double()
-    out = torch.zeros(n, heads, vdim, dtype=torch.float64)
+    out = torch.zeros(n, G, R, vdim, dtype=torch.float64)
     for i in range(n):
         j = torch.arange(i + 1)
         if window:
             j = j[(i - j < window) | (j < keep)]
-        own = j >= i // BLOCK * BLOCK
-        for h in range(heads):
-            g = h // R
-            keys, vals = (torch.where(own[:, None], a[j, g], b[j, g]) for a, b in ((k, kq), (v, vq)))
-            s = keys @ q[i, h] * scale
-            top = s.max() if sink is None else torch.maximum(s.max(), torch.tensor(float(sink), dtype=torch.float64))
-            e = torch.exp(s - top)
-            out[i, h] = (e @ vals) / (e.sum() + (0.0 if sink is None else torch.exp(sink - top)))
+        own = (j >= i // BLOCK * BLOCK)[:, None, None]
+        keys, vals = (torch.where(own, a[j], b[j]).transpose(0, 1) for a, b in ((k, kq), (v, vq)))
+        s = q[i].reshape(G, R, dim) @ keys.transpose(1, 2) * scale
+        top = s.amax(-1, keepdim=True)
+        if sink is not None:
+            top = top.clamp(min=sink)
+        e = torch.exp(s - top)
+        out[i] = (e @ vals) / (e.sum(-1, keepdim=True) + (0.0 if sink is None else torch.exp(sink - top)))
     out = out.reshape(n, heads * vdim)
     return (out * torch.sigmoid(gate) if gate.shape[1] else out), k, v
 

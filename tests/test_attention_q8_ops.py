@@ -1,0 +1,181 @@
+"""Attention against a cache of 8 bits: whole sequences of the plain oracle against the op run in portions that are cut anywhere,
+inside blocks, at their ends and across several of them. Codes, scales and tails are compared bit for bit: they depend on nothing but
+the tokens. CPU backend, and marked `gpu` the kernels (32-bit and bf16)."""
+import pytest
+import torch
+
+import plain_serving as plain
+from test_dunelix_ops import backend, close, i32, op, rnd  # noqa: F401  (fixture and helpers)
+from popxl_addons_b200 import xl
+from popxl_addons_b200.xl import ops
+
+BLOCK = plain.BLOCK
+# heads, key / value heads, dim, vdim
+SHAPES = {"grouped": (4, 2, 16, 24), "wide": (20, 1, 64, 32), "plain": (3, 3, 32, 16), "odd": (2, 1, 10, 7), "full": (8, 2, 128, 128),
+          "long": (1, 1, 200, 264), "group_of_three": (6, 2, 96, 80)}
+
+
+def empty_cache(backend, B, G, blocks, dim, vdim, junk=True):  # noqa: F811
+    """What an earlier request may have left: anything finite in the codes, anything at all in the tails."""
+    g = torch.Generator().manual_seed(99)
+    t = [torch.randint(-127, 128, (B, G, blocks, BLOCK, w), generator=g).to(torch.int8) for w in (dim, vdim)]
+    t += [torch.rand(B, G, blocks, generator=g) * 100 for _ in range(2)]
+    t += [torch.full((B, G, BLOCK, w), float("nan")).to(backend[1]) for w in (dim, vdim)]
+    return [x.to(backend[0]) for x in t]
+
+
+def bound(backend, dim):  # noqa: F811
+    """Largest difference over the largest output. 32 bits: scores of up to 8 from sums of `dim` roundings of 2^-24 relative to
+    |q||k|, about 2^-18 of a weight, and as much again for sums over keys. bf16: the output's own rounding is 2^-9 of the value at
+    most (half a step of 2^-8), a gate's input has none; queries are held to 2^-12 where products take 16 bits, which moves a score of up to
+    8 by 2^-9 at most, values times codes to 2^-9: four times 2^-9 in all."""
+    return 2e-5 if backend[1] == torch.float32 else 4 * 2.0 ** -9
+
+
+def run_portions(backend, rows, cuts, start, T, shape, window, keep, sink, gated, cache, eps=1e-5):  # noqa: F811
+    """Portions of `rows (n, columns)` of the middle one of three slots, `cuts` their lengths; the last slot is idle, the first would
+    not fit. Returns the outputs and what is left of the other rows."""
+    H, G, d, dv = shape
+    dev, outs = backend[0], []
+    (qn, _), (kn, _) = norms(backend, d)
+    p = start
+    blocks = cache[0].shape[2]
+    for n in cuts:
+        T_now = max(T, n) if T else n
+        proj = torch.full((3, T_now, rows.shape[1]), 3.0, dtype=backend[1])
+        proj[1, :n] = rows[p:p + n]
+        joint = torch.full((3 * T_now, H * dv + 5), -7.0, dtype=backend[1], device=dev)
+        got = op("window_attention_q8_", backend, proj.reshape(3 * T_now, -1).to(dev), qn, kn, *cache, i32(backend, blocks * BLOCK - n + 1, p, 3),
+                 i32(backend, n, n, 0), joint, T=T_now, heads=H, window=window, keep_first=keep, scale=d ** -0.5, sink=sink, eps=eps)
+        got = got.reshape(3, T_now, -1)
+        assert (got[0] == -7).all() and (got[2] == -7).all() and (got[1, n:] == -7).all() and (got[1, :, H * dv:] == -7).all()
+        outs.append(got[1, :n, :H * dv])
+        p += n
+    return torch.cat(outs)
+
+
+def norms(backend, d):  # noqa: F811
+    f32 = (backend[0], torch.float32)
+    (q, q64), (k, k64) = rnd(f32, d, std=0.3, seed=21), rnd(f32, d, std=0.3, seed=22)
+    return (q + 1.5, (q.cpu() + 1.5).double()), (k + 1.2, (k.cpu() + 1.2).double())
+
+
+# portions that are cut inside blocks, at their ends and across several of them
+CUTS = {"ones": [1] * 3, "even": [64, 64, 2], "ragged": [5, 59, 1, 63, 64, 65, 1], "two": [200, 1, 1], "edges": [63, 1, 1, 127, 1],
+        "whole": [130], "growing": [2, 3, 4, 8, 16, 33, 100, 40]}
+# window, kept first tokens, sink, gate
+MASKS = {"all": (0, 0, None, True), "window": (70, 4, 0.0, True), "narrow": (3, 1, 0.5, False), "kept": (40, 90, 0.0, True)}
+MIXED = [("grouped", c, m) for c in CUTS for m in ("window", "narrow")] + [
+    ("full", c, m) for c, m in zip(CUTS, ("all", "window", "kept", "narrow", "all", "window", "kept"))] + [
+    ("wide", "growing", "window"), ("wide", "edges", "all"), ("plain", "ragged", "kept"), ("plain", "two", "all"), ("odd", "ragged", "kept"),
+    ("odd", "edges", "all"), ("long", "two", "window"), ("long", "edges", "kept"), ("group_of_three", "growing", "all"),
+    ("group_of_three", "edges", "narrow")]
+
+
+@pytest.mark.parametrize("shape,cut,mask", MIXED)
+def test_portions_against_whole_sequences(backend, shape, cut, mask):  # noqa: F811
+    cuts, (window, keep, sink, gated) = CUTS[cut], MASKS[mask]
+    H, G, d, dv = SHAPES[shape]
+    eps, n = 1e-5, sum(cuts)
+    blocks = n // BLOCK + 1
+    cols = (H + G) * d + G * dv + (H * dv if gated else 0)
+    rows = torch.randn(n, cols, generator=torch.Generator().manual_seed(1))
+    rows[n // 3] *= 30.0  # a token whose block has a scale of its own
+    rows = rows.to(backend[1])
+    cache = empty_cache(backend, 3, G, blocks, d, dv)
+    before = [x.clone() for x in cache]
+    got = run_portions(backend, rows, cuts, 0, 0, SHAPES[shape], window, keep, sink, gated, cache, eps)
+    (_, qn), (_, kn) = norms(backend, d)
+    want, k, v = plain.q8_attention(rows.double(), qn, kn, H, G, d, dv, window, keep, d ** -0.5, sink, eps, backend[1])
+    for i in range(n):  # row by row: a single wrong position would drown among larger ones
+        close(got[i], want[i], backend, bound(backend, d), bound(backend, d))
+    full = n // BLOCK
+    for held, scale, tail, x in ((cache[0], cache[2], cache[4], k), (cache[1], cache[3], cache[5], v)):
+        for j in range(full):
+            for g in range(G):
+                codes, step = plain.block_codes(x[j * BLOCK:(j + 1) * BLOCK, g])
+                assert torch.equal(held[1, g, j].cpu().double(), codes) and scale[1, g, j].item() == step.item()
+        assert torch.equal(tail[1, :, :n % BLOCK].cpu().double(), x[full * BLOCK:].transpose(0, 1))
+    for now, was in zip(cache, before):  # the other slots, blocks that are not complete, places of the tail that are not in use
+        assert torch.equal(now[[0, 2]].nan_to_num(5.0), was[[0, 2]].nan_to_num(5.0))
+    for now, was in zip(cache[:4], before[:4]):
+        assert torch.equal(now[:, :, full:], was[:, :, full:])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_codes_do_not_depend_on_the_kernel(dtype):
+    """Every division of a prompt into portions, and the CPU, come to the same bits of codes, scales and tails."""
+    H, G, d, dv = SHAPES["full"]
+    rows = (torch.randn(321, (H + G) * d + (G + H) * dv, generator=torch.Generator().manual_seed(4)) * 3).to(dtype)
+    held = []
+    for dev, cuts in (("cpu", [321]), ("cuda", [321]), ("cuda", [1] * 321), ("cuda", [7, 200, 1, 50, 63])):
+        cache = empty_cache((dev, dtype), 3, G, 6, d, dv)
+        run_portions((dev, dtype), rows, cuts, 0, 0, SHAPES["full"], 100, 4, 0.0, True, cache)
+        held.append([x.cpu()[1] for x in cache])
+        held[-1][4], held[-1][5] = (x[:, :321 % BLOCK] for x in held[-1][4:])
+    for other in held[1:]:
+        assert all(torch.equal(x, y) for x, y in zip(held[0], other))
+
+
+def test_blocks_of_zeros_and_of_one_large_value(backend):  # noqa: F811
+    """A scale of zero, and a value next to which the others vanish: their code is zero."""
+    H, G, d, dv = 2, 1, 16, 16
+    rows = torch.zeros(70, (H + G) * d + G * dv, dtype=backend[1])
+    rows[5, -1], rows[6, -2] = 1e6, 1.0
+    rows[:, :H * d] = 1.0
+    cache = empty_cache(backend, 3, G, 2, d, dv)
+    got = run_portions(backend, rows, [64, 6], 0, 0, (H, G, d, dv), 0, 0, None, False, cache)
+    assert cache[2][1, 0, 0] == 0 and (cache[0][1, 0, 0] == 0).all()
+    assert cache[1][1, 0, 0].abs().sum() == 127 and cache[1][1, 0, 0, 5, -1] == 127
+    close(got[5, dv - 1:dv], torch.tensor([float(rows[5, -1]) / 6]), backend, 1e-5, 2.0 ** -8)      # its own block: as computed
+    close(got[69, dv - 2:dv], torch.tensor([0.0, float(rows[5, -1]) / 70]), backend, 1e-5, 2.0 ** -8)
+
+
+@pytest.mark.parametrize("T", [1, 40])
+def test_repeated_passes_and_padding(backend, T):  # noqa: F811
+    """The same pass twice gives the same state; padded rows and idle sequences touch nothing."""
+    H, G, d, dv = SHAPES["grouped"]
+    rows = torch.randn(150, (H + G) * d + (G + H) * dv, generator=torch.Generator().manual_seed(2)).to(backend[1])
+    cache = empty_cache(backend, 3, G, 3, d, dv)
+    run_portions(backend, rows, [127], 0, 0, SHAPES["grouped"], 30, 2, 0.0, True, cache)
+    first = run_portions(backend, rows, [1], 127, T, SHAPES["grouped"], 30, 2, 0.0, True, cache)
+    state = [x.clone() for x in cache]
+    again = run_portions(backend, rows, [1], 127, T, SHAPES["grouped"], 30, 2, 0.0, True, cache)
+    # the block that the first pass completed is whole: the second computes it from the tail, which it left alone
+    assert torch.equal(first, again)
+    assert all(torch.equal(a.nan_to_num(5.0), b.nan_to_num(5.0)) for a, b in zip(state, cache))
+
+
+def test_refusals():
+    ir = xl.Ir()
+    with ir.main_graph:
+        def var(shape, dt):
+            return xl.variable(xl.LazyInit(shape, kind="zeros"), dt)
+
+        def cache(dt=xl.bfloat16, **kw):
+            spec = ops.cache8_spec(2, 2, 100, 16, 24, dt)
+            t = {k: var(*kw.get(k, s)) for k, s in spec.items()}
+            return ops.Cache8(**t)
+
+        f32, i32_ = xl.float32, xl.int32
+        proj = var((6, (4 + 2) * 16 + (2 + 4) * 24), xl.bfloat16)
+        rest = (var((2,), i32_), var((2,), i32_))
+        joint = var((6, 4 * 24), xl.bfloat16)
+        norm = var((16,), f32)
+        out = ops.window_attention_q8_(proj, norm, norm, cache(), *rest, joint, 3, 4, 0.25)
+        assert out.shape == joint.shape
+        with pytest.raises(ValueError, match="cache.k_scale"):
+            ops.window_attention_q8_(proj, norm, norm, cache(k_scale=((2, 2, 1), f32)), *rest, joint, 3, 4, 0.25)
+        with pytest.raises(ValueError, match="cache.v_tail"):
+            ops.window_attention_q8_(proj, norm, norm, cache(v_tail=((2, 2, 64, 24), f32)), *rest, joint, 3, 4, 0.25)
+        with pytest.raises(ValueError, match="multiple of the cache's"):
+            ops.window_attention_q8_(proj, norm, norm, cache(), *rest, joint, 3, 3, 0.25)
+        with pytest.raises(ValueError, match="projections"):
+            ops.window_attention_q8_(proj, norm, norm, cache(), *rest, joint, 4, 4, 0.25)
+        with pytest.raises(ValueError, match="joint buffer"):
+            ops.window_attention_q8_(proj, norm, norm, cache(), *rest, var((6, 95), xl.bfloat16), 3, 4, 0.25)
+        with pytest.raises(ValueError, match="q_norm"):
+            ops.window_attention_q8_(proj, var((17,), f32), norm, cache(), *rest, joint, 3, 4, 0.25)
+        with pytest.raises(ValueError, match="positive"):
+            ops.window_attention_q8_(proj, norm, norm, cache(), *rest, joint, 3, 4, 0.0)
