@@ -4,7 +4,10 @@
 //
 //   xl_q8_append          queries to their buffer, keys and values to `raw`; complete blocks to codes, the rest to the tails
 //   xl_q8_attn_general    any sizes and types, scores and weights in fp32 on the CUDA cores: one warp per row and head
+//   xl_q8_attn_few        few rows per sequence, bf16, on mma.sync; of a single token norms, append and codes in the same launch
+#include "attention_decode.cuh"
 #include "attention_q8.cuh"
+#include "tcgen05.cuh"
 
 #include <math.h>
 
@@ -326,6 +329,678 @@ __global__ void __launch_bounds__(SPLIT == 1 ? 128 : SPLIT * 32) q8_attn_general
   }
 }
 
+// ---- few query rows per key / value head: mma.sync -----------------------------------------------------------------------
+// Grid (splits, G * row chunks, B). A CTA takes up to 8 RT rows (token-major, the query heads of one key / value head) and a share of
+// the keys that any of them sees: codes in items of 32 keys, then (the last split) its raw rows in tiles of 16. Its four warps walk
+// their items independently, each through a ring of its own (the codes by TMA, swizzled so that 16-byte reads by rows and ldmatrix
+// by columns meet few bank conflicts), with online softmax state in registers.
+//
+//   scores   A: queries as fp16 (divided by a power of two above the norm's factors), B: codes as fp16, which is exact; the scale of
+//            the block multiplies the fp32 result
+//   output   A: weights times value scale over the warp's largest, as fp16 (2^-12 relative); B: codes as fp16, exact
+//   raw rows keys as fp16 likewise, values in bf16 with weights as sums of two bf16 numbers
+//
+// A code c becomes fp16 by two instructions for two of them: the byte c + 128 is the low byte of 1024 + (c + 128) under the high byte
+// 0x64, from which 1152 is taken. The value product needs keys in pairs: ldmatrix transposes pairs of bytes, that is two features of
+// two keys, and the same byte selection takes even and odd features apart, whose results go to tiles of their own.
+//
+// FUSED (T = 1): norms, the new key and value, and a block that they complete in the same launch.
+constexpr int QD_WARPS = 4;
+constexpr int QD_KEYS = 32, QD_RAW = 16;
+constexpr int QD_MAX_SPLITS = 64;
+enum { ERR_Q8_CODES = 91 };
+
+struct Q8FewParams {
+  const __nv_bfloat16* proj;
+  long long ld;
+  const float *wq, *wk;
+  const float* q;                       // not FUSED: (B, G, T, H/G, dim), and raw rows
+  const __nv_bfloat16 *raw_k, *raw_v;
+  int8_t *kc, *vc;
+  float *ks, *vs;
+  __nv_bfloat16 *kt, *vt, *out;
+  long long ldo;
+  const int *pos, *count;
+  int T, H, G, dim, vdim, blocks, window, keep_first, gated;
+  float scale, sink;
+  double eps;
+  float* part;             // [B * G * chunks][splits][rows per CTA][vdim], then the same with [2]: maximum, sum
+  unsigned int* counters;  // [B * G * chunks], zero between launches
+  int stages, read_ahead;
+  int* err;
+};
+
+__device__ __forceinline__ void q8_mma_f16(float (&c)[4], const uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// eight rows in use: the upper eight are zero
+__device__ __forceinline__ void q8_mma_f16(float (&c)[2], const uint32_t a0, uint32_t, uint32_t a2, uint32_t, uint32_t b0, uint32_t b1) {
+  float unused0, unused1;
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%12};"
+               : "=f"(c[0]), "=f"(c[1]), "=f"(unused0), "=f"(unused1)
+               : "r"(a0), "r"(0u), "r"(a2), "r"(0u), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(0.f));
+}
+__device__ __forceinline__ void q8_mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  dd_mma(c, a0, a1, a2, a3, b0, b1);
+}
+__device__ __forceinline__ void q8_mma_bf16(float (&c)[2], uint32_t a0, uint32_t, uint32_t a2, uint32_t, uint32_t b0, uint32_t b1) {
+  float unused0, unused1;
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%12};"
+               : "=f"(c[0]), "=f"(c[1]), "=f"(unused0), "=f"(unused1)
+               : "r"(a0), "r"(0u), "r"(a2), "r"(0u), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(0.f));
+}
+__device__ __forceinline__ uint32_t q8_pack_f16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// two codes of a word (selected bytes, biased by 128) -> fp16 pair
+template <int SEL> __device__ __forceinline__ uint32_t q8_pair(uint32_t biased) {
+  const uint32_t w = __byte_perm(biased, 0x64646464u, SEL);
+  uint32_t r;
+  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(w), "r"(0xe480e480u));  // - 1152
+  return r;
+}
+
+template <int DK, int DV> __host__ __device__ constexpr int q8_stage_bytes() { return QD_KEYS * (DK + DV); }
+
+// DK, DV: 64 or 128, features of a key and of a value rounded up
+template <int DK, int DV, int RT, bool FUSED>
+__global__ void __launch_bounds__(QD_WARPS * 32, 2)
+    q8_few_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const Q8FewParams p) {
+  using namespace xl_tc;
+  constexpr int ROWS = 8 * RT, STAGE = q8_stage_bytes<DK, DV>(), KG = DK / 64, VT = DV / 16;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  __shared__ __align__(16) __half sq[ROWS][DK];
+  __shared__ __align__(16) __nv_bfloat16 new_k[DK], new_v[DV];
+  __shared__ uint64_t bars[QD_WARPS][4];
+  __shared__ float tops[2][QD_WARPS];
+  __shared__ float sm[QD_WARPS][ROWS], sl[QD_WARPS][ROWS], fw[QD_WARPS][ROWS], fl[ROWS];
+  __shared__ float wt[QD_MAX_SPLITS * ROWS], wl[QD_MAX_SPLITS * ROWS];
+  __shared__ unsigned int is_last;
+  __shared__ volatile int abort_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = lane >> 2, j = lane & 3;
+  const int R = p.H / p.G, chunks = (p.T * R + ROWS - 1) / ROWS;
+  const int split = blockIdx.x, splits = gridDim.x, g = blockIdx.y / chunks, chunk = blockIdx.y % chunks, b = blockIdx.z;
+  if (threadIdx.x == 0) {
+    for (int w = 0; w < QD_WARPS; ++w)
+      for (int i = 0; i < 4; ++i) mbar_init(&bars[w][i], 1);
+    abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncthreads();
+  if (!p.read_ahead) xl_grid_dependency_wait();
+  const int pos = p.pos[b], n_tok = min(p.count[b], p.T), nh = min(ROWS, n_tok * R - chunk * ROWS);
+  if (nh <= 0 || pos < 0 || (long long)pos + n_tok > (long long)p.blocks * Q8_BLOCK) {
+    xl_grid_dependency_wait();  // no kernel of a chain ends before its predecessor
+    return;
+  }
+  const int p_lo = pos + chunk * ROWS / R, p_hi = pos + (chunk * ROWS + nh - 1) / R;
+  const int base = pos / Q8_BLOCK * Q8_BLOCK, own_lo = p_lo / Q8_BLOCK * Q8_BLOCK, own_hi = p_hi / Q8_BLOCK * Q8_BLOCK;
+  const long long head = (long long)b * p.G + g;
+  // ---- this CTA's items -----------------------------------------------------------------------------------------------------
+  const int w0 = p.window ? max(0, p_lo - p.window + 1) / QD_KEYS * QD_KEYS : 0;
+  const int kept = min(min(p.keep_first, w0), own_hi), kept_items = (kept + QD_KEYS - 1) / QD_KEYS;
+  const int items = kept_items + max(0, own_hi - w0) / QD_KEYS;
+  const int raw0 = own_lo - base, raw_end = p_hi - base + 1, raw_tiles = (raw_end - raw0 + QD_RAW - 1) / QD_RAW;
+  const long long all = (long long)items + raw_tiles;
+  const int it0 = min(items, (int)(split * all / splits)), it1 = min(items, (int)((split + 1) * all / splits));
+  const bool has_raw = split == splits - 1;
+  auto first_key = [&](int it) { return it < kept_items ? it * QD_KEYS : w0 + (it - kept_items) * QD_KEYS; };
+  const int n_raw = has_raw ? max(0, (raw_tiles - warp + QD_WARPS - 1) / QD_WARPS) : 0;
+  const int n_code = max(0, (it1 - it0 - warp + QD_WARPS - 1) / QD_WARPS), n_all = n_raw + n_code;
+  const int fill = pos - base;  // FUSED: the new token's row
+  uint8_t* ring = smem + warp * p.stages * STAGE;
+  const int row_base = (int)(head * p.blocks) * Q8_BLOCK;
+  const __nv_bfloat16* raw_k = FUSED ? p.kt + head * Q8_BLOCK * p.dim : p.raw_k + head * (p.T + Q8_BLOCK) * p.dim;
+  const __nv_bfloat16* raw_v = FUSED ? p.vt + head * Q8_BLOCK * p.vdim : p.raw_v + head * (p.T + Q8_BLOCK) * p.vdim;
+  auto prefetch = [&](int n) {
+    if (n >= n_all) return;
+    const int slot = n % p.stages;
+    uint8_t* st = ring + slot * STAGE;
+    if (n < n_raw) {
+      const int r0 = raw0 + (warp + n * QD_WARPS) * QD_RAW, valid = FUSED ? fill : raw_end;
+      for (int i = lane; i < QD_RAW * (DK / 8); i += 32) {
+        const int r = i / (DK / 8), c = i % (DK / 8);
+        const bool on = r0 + r < valid && c * 8 < p.dim;
+        dd_cp16_zfill(st + r * (DK * 2) + ((c ^ (r & 7)) * 16), on ? raw_k + (long long)(r0 + r) * p.dim + c * 8 : raw_k, on);
+      }
+      for (int i = lane; i < QD_RAW * (DV / 8); i += 32) {
+        const int r = i / (DV / 8), c = i % (DV / 8);
+        const bool on = r0 + r < valid && c * 8 < p.vdim;
+        dd_cp16_zfill(st + QD_RAW * DK * 2 + r * (DV * 2) + ((c ^ (r & 6)) * 16), on ? raw_v + (long long)(r0 + r) * p.vdim + c * 8 : raw_v, on);
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    } else if (lane == 0) {
+      const int row = row_base + first_key(it0 + warp + (n - n_raw) * QD_WARPS);
+      mbar_expect_tx(&bars[warp][slot], STAGE);
+      tma_load_2d(st, &map_k, &bars[warp][slot], 0, row);
+      tma_load_2d(st + QD_KEYS * DK, &map_v, &bars[warp][slot], 0, row);
+    }
+  };
+  for (int n = 0; n < p.stages; ++n) prefetch(n);
+  // the largest value scale of this warp's items: the unit of its output
+  float ref = 0.f;
+  for (int i = lane; i < n_code; i += 32) ref = fmaxf(ref, p.vs[head * p.blocks + first_key(it0 + warp + i * QD_WARPS) / Q8_BLOCK]);
+  ref = n_code ? fmaxf(xl_warp_max(ref), 1e-20f) : 1.f;
+  const float unit_q = q8_norm_unit(p.wq, p.dim, lane), unit_k = q8_norm_unit(p.wk, p.dim, lane);
+  if (p.read_ahead) xl_grid_dependency_wait();  // the new projections
+  xl_grid_launch_dependents();
+  // ---- queries (fp16, in units) to shared memory; the new key and value -----------------------------------------------------
+  const int plain = (p.H + p.G) * p.dim + p.G * p.vdim;
+  for (int r = warp; r < ROWS; r += QD_WARPS) {
+    const int at = chunk * ROWS + r, t = at / R, hh = at % R;
+    float x[DK / 32];
+    if (FUSED) {
+      const __nv_bfloat16* src = p.proj + (long long)b * p.ld + (long long)(g * R + hh) * p.dim;
+      float sum = 0.f;
+#pragma unroll
+      for (int u = 0; u < DK / 64; ++u) {
+        const int e = 2 * lane + 64 * u;
+        const uint32_t w = r < nh && e < p.dim ? *reinterpret_cast<const uint32_t*>(src + e) : 0u;
+        x[2 * u] = dd_lo(w);
+        x[2 * u + 1] = dd_hi(w);
+        sum += x[2 * u] * x[2 * u] + x[2 * u + 1] * x[2 * u + 1];
+      }
+      const float f = 1.f / (sqrtf(xl_warp_sum(sum) / p.dim + (float)p.eps) * unit_q);
+#pragma unroll
+      for (int u = 0; u < DK / 64; ++u) {
+        const int e = 2 * lane + 64 * u;
+        const bool on = r < nh && e < p.dim;
+        x[2 * u] = on ? x[2 * u] * f * p.wq[e] : 0.f;
+        x[2 * u + 1] = on ? x[2 * u + 1] * f * p.wq[e + 1] : 0.f;
+      }
+    } else {
+      const float* src = p.q + ((head * p.T + t) * R + hh) * p.dim;
+#pragma unroll
+      for (int u = 0; u < DK / 64; ++u) {
+        const int e = 2 * lane + 64 * u;
+        const bool on = r < nh && e < p.dim;
+        x[2 * u] = on ? src[e] / unit_q : 0.f;
+        x[2 * u + 1] = on ? src[e + 1] / unit_q : 0.f;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < DK / 64; ++u) *reinterpret_cast<uint32_t*>(&sq[r][2 * lane + 64 * u]) = q8_pack_f16(x[2 * u], x[2 * u + 1]);
+  }
+  const bool writes = FUSED && has_raw && chunk == 0, completes = writes && fill == Q8_BLOCK - 1;
+  if (FUSED && has_raw && warp == QD_WARPS - 1) {
+    const __nv_bfloat16* src = p.proj + (long long)b * p.ld + (long long)(p.H + g) * p.dim;
+    const __nv_bfloat16* vsrc = p.proj + (long long)b * p.ld + (long long)(p.H + p.G) * p.dim + (long long)g * p.vdim;
+    float x[DK / 32];
+    double sum = 0.0;
+#pragma unroll
+    for (int u = 0; u < DK / 64; ++u) {
+      const int e = 2 * lane + 64 * u;
+      const uint32_t w = e < p.dim ? *reinterpret_cast<const uint32_t*>(src + e) : 0u;
+      x[2 * u] = dd_lo(w);
+      x[2 * u + 1] = dd_hi(w);
+      sum += (double)x[2 * u] * x[2 * u] + (double)x[2 * u + 1] * x[2 * u + 1];
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    const double f = 1.0 / sqrt(sum / p.dim + p.eps);
+#pragma unroll
+    for (int u = 0; u < DK / 64; ++u) {
+      const int e = 2 * lane + 64 * u;
+      const bool on = e < p.dim;
+      const uint32_t w = on ? dd_pack((float)((double)x[2 * u] * f * (double)p.wk[e]), (float)((double)x[2 * u + 1] * f * (double)p.wk[e + 1])) : 0u;
+      *reinterpret_cast<uint32_t*>(new_k + e) = w;
+      if (on && writes && !completes) *reinterpret_cast<uint32_t*>(p.kt + (head * Q8_BLOCK + fill) * p.dim + e) = w;
+    }
+#pragma unroll
+    for (int u = 0; u < DV / 64; ++u) {
+      const int e = 2 * lane + 64 * u;
+      const uint32_t w = e < p.vdim ? *reinterpret_cast<const uint32_t*>(vsrc + e) : 0u;
+      *reinterpret_cast<uint32_t*>(new_v + e) = w;
+      if (e < p.vdim && writes && !completes) *reinterpret_cast<uint32_t*>(p.vt + (head * Q8_BLOCK + fill) * p.vdim + e) = w;
+    }
+  }
+  __syncthreads();
+  uint32_t q[RT][KG][8];  // rows quad (+ 8), features 64 i + 16 j .. + 15
+#pragma unroll
+  for (int m = 0; m < RT; ++m)
+#pragma unroll
+    for (int i = 0; i < KG; ++i)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const uint4 w = *reinterpret_cast<const uint4*>(&sq[quad + 8 * m][64 * i + 16 * j + 8 * u]);
+        q[m][i][4 * u] = w.x; q[m][i][4 * u + 1] = w.y; q[m][i][4 * u + 2] = w.z; q[m][i][4 * u + 3] = w.w;
+      }
+  int qpos[RT], lo[RT], own[RT];
+#pragma unroll
+  for (int m = 0; m < RT; ++m) {
+    qpos[m] = min(p_hi, pos + (chunk * ROWS + quad + 8 * m) / R);
+    lo[m] = p.window ? qpos[m] - p.window + 1 : 0;
+    own[m] = qpos[m] / Q8_BLOCK * Q8_BLOCK;
+  }
+  const int lo_max = p.window ? p_hi - p.window + 1 : 0;
+  float o[VT][2][2 * RT];  // even and odd features of a tile of 16
+#pragma unroll
+  for (int t = 0; t < VT; ++t)
+#pragma unroll
+    for (int e = 0; e < 2 * RT; ++e) o[t][0][e] = o[t][1][e] = 0.f;
+  float mx[RT], l[RT];
+#pragma unroll
+  for (int m = 0; m < RT; ++m) {
+    mx[m] = -INFINITY;
+    l[m] = 0.f;
+  }
+  const float c_unit = p.scale * 1.4426950408889634f * unit_q;
+  // scores of NT tiles of eight keys -> weights (in place); rescales the output where a maximum moved
+  auto softmax = [&](auto& s) {
+    constexpr int NT = sizeof(s) / sizeof(s[0]);
+    float alpha[RT];
+    bool moved = false;
+#pragma unroll
+    for (int m = 0; m < RT; ++m) {
+      float v = -INFINITY;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) v = fmaxf(v, fmaxf(s[t][2 * m], s[t][2 * m + 1]));
+      v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
+      v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+      const float m_new = fmaxf(mx[m], v), m_use = m_new == -INFINITY ? 0.f : m_new;  // a row may see none of these keys
+      alpha[m] = exp2f(mx[m] - m_use);
+      mx[m] = m_new;
+      float sum = 0.f;
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          s[t][2 * m + e] = exp2f(s[t][2 * m + e] - m_use);
+          sum += s[t][2 * m + e];
+        }
+      l[m] = l[m] * alpha[m] + sum;  // this lane's share of the row sum
+      moved |= alpha[m] != 1.f;
+    }
+    if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+      for (int t = 0; t < VT; ++t)
+#pragma unroll
+        for (int e = 0; e < 2 * RT; ++e) {
+          o[t][0][e] *= alpha[e >> 1];
+          o[t][1][e] *= alpha[e >> 1];
+        }
+    }
+  };
+  bool ok = true;
+  int given_up = 0;
+  // ---- raw tiles -------------------------------------------------------------------------------------------------------------
+  for (int n = 0; n < n_raw; ++n) {
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncwarp();
+    uint8_t* st = ring + (n % p.stages) * STAGE;
+    uint8_t* sv = st + QD_RAW * DK * 2;
+    const int r0 = raw0 + (warp + n * QD_WARPS) * QD_RAW, key0 = base + r0;
+    if (FUSED && fill >= r0 && fill < r0 + QD_RAW) {  // the new key and value take their place
+      const int r = fill - r0;
+      if (lane < DK / 8) *reinterpret_cast<uint4*>(st + r * (DK * 2) + ((lane ^ (r & 7)) * 16)) = *reinterpret_cast<const uint4*>(new_k + lane * 8);
+      if (lane < DV / 8) *reinterpret_cast<uint4*>(sv + r * (DV * 2) + ((lane ^ (r & 6)) * 16)) = *reinterpret_cast<const uint4*>(new_v + lane * 8);
+      __syncwarp();
+    }
+    if (completes) {  // every warp of the CTA has one tile: together the whole block
+      float top[2] = {0.f, 0.f};
+      auto largest = [&](const uint4& w, float& m) {
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) m = fmaxf(m, fmaxf(fabsf(dd_lo(u[e])), fabsf(dd_hi(u[e]))));
+      };
+      for (int i = lane; i < QD_RAW * (DK / 8); i += 32) largest(*reinterpret_cast<const uint4*>(st + i * 16), top[0]);
+      for (int i = lane; i < QD_RAW * (DV / 8); i += 32) largest(*reinterpret_cast<const uint4*>(sv + i * 16), top[1]);
+#pragma unroll
+      for (int kind = 0; kind < 2; ++kind) {
+        const float m = xl_warp_max(top[kind]);
+        if (lane == 0) tops[kind][warp] = m;
+      }
+      __syncthreads();
+      const long long blk = head * p.blocks + pos / Q8_BLOCK;
+      float scale[2];
+#pragma unroll
+      for (int kind = 0; kind < 2; ++kind) {
+        float m = tops[kind][0];
+        for (int w = 1; w < QD_WARPS; ++w) m = fmaxf(m, tops[kind][w]);
+        scale[kind] = __fdiv_rn(m, 127.f);
+        if (threadIdx.x == 0) (kind ? p.vs : p.ks)[blk] = scale[kind];
+      }
+      auto write = [&](const uint4& w, int8_t* dst, float step) {
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+        uint32_t c[2] = {0u, 0u};
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          c[e >> 2] |= (uint32_t)(q8_code(e & 1 ? dd_hi(u[e >> 1]) : dd_lo(u[e >> 1]), step) & 0xff) << (8 * (e & 3));
+        *reinterpret_cast<uint2*>(dst) = make_uint2(c[0], c[1]);
+      };
+      for (int i = lane; i < QD_RAW * (DK / 8); i += 32) {
+        const int r = i / (DK / 8), c = i % (DK / 8);
+        if (c * 8 < p.dim)
+          write(*reinterpret_cast<const uint4*>(st + r * (DK * 2) + ((c ^ (r & 7)) * 16)), p.kc + (blk * Q8_BLOCK + r0 + r) * p.dim + c * 8, scale[0]);
+      }
+      for (int i = lane; i < QD_RAW * (DV / 8); i += 32) {
+        const int r = i / (DV / 8), c = i % (DV / 8);
+        if (c * 8 < p.vdim)
+          write(*reinterpret_cast<const uint4*>(sv + r * (DV * 2) + ((c ^ (r & 6)) * 16)), p.vc + (blk * Q8_BLOCK + r0 + r) * p.vdim + c * 8, scale[1]);
+      }
+    }
+    float s[QD_RAW / 8][2 * RT];
+#pragma unroll
+    for (int t = 0; t < QD_RAW / 8; ++t) {
+#pragma unroll
+      for (int e = 0; e < 2 * RT; ++e) s[t][e] = 0.f;
+      const int r = 8 * t + quad;
+      const float inv = 1.f / unit_k;
+#pragma unroll
+      for (int i = 0; i < KG; ++i)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const uint4 w = *reinterpret_cast<const uint4*>(st + r * (DK * 2) + (((8 * i + 2 * j + u) ^ (r & 7)) * 16));
+          uint32_t k[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) k[e] = q8_pack_f16(dd_lo(k[e]) * inv, dd_hi(k[e]) * inv);
+          q8_mma_f16(s[t], q[0][i][4 * u], q[RT - 1][i][4 * u], q[0][i][4 * u + 1], q[RT - 1][i][4 * u + 1], k[0], k[1]);
+          q8_mma_f16(s[t], q[0][i][4 * u + 2], q[RT - 1][i][4 * u + 2], q[0][i][4 * u + 3], q[RT - 1][i][4 * u + 3], k[2], k[3]);
+        }
+      const float c = c_unit * unit_k;
+#pragma unroll
+      for (int e = 0; e < 2 * RT; ++e) {
+        const int key = key0 + 8 * t + 2 * j + (e & 1), m = e >> 1;
+        s[t][e] = key >= own[m] && key <= qpos[m] && (key >= lo[m] || key < p.keep_first) ? s[t][e] * c : -INFINITY;
+      }
+    }
+    softmax(s);
+    uint32_t ph[2][RT], pl[2][RT];  // weights in units of `ref` as operands of the second product, and their rounding errors
+    const float inv_ref = 1.f / ref;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int m = 0; m < RT; ++m) {
+        const float x = s[t][2 * m] * inv_ref, y = s[t][2 * m + 1] * inv_ref;
+        ph[t][m] = dd_pack(x, y);
+        pl[t][m] = dd_pack(x - dd_lo(ph[t][m]), y - dd_hi(ph[t][m]));
+      }
+    bool seen[4];  // rows 2 j, 2 j + 1, 2 j + 8, 2 j + 9 of the tile: one that no row sees may hold anything
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int key = key0 + 2 * j + (e & 1) + 8 * (e >> 1);
+      seen[e] = key <= p_hi && (!p.window || key >= p_lo - p.window + 1 || key < p.keep_first);
+    }
+#pragma unroll
+    for (int t = 0; t < VT; ++t) {
+      uint32_t w[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = 2 * j + (e & 1) + 8 * (e >> 1), c = 2 * t + (quad >> 2);
+        w[e] = seen[e] ? *reinterpret_cast<const uint32_t*>(sv + r * (DV * 2) + ((c ^ (r & 6)) * 16) + (quad & 3) * 4) : 0u;
+      }
+#pragma unroll
+      for (int odd = 0; odd < 2; ++odd) {
+        const uint32_t b0 = __byte_perm(w[0], w[1], odd ? 0x7632 : 0x5410), b1 = __byte_perm(w[2], w[3], odd ? 0x7632 : 0x5410);
+        q8_mma_bf16(o[t][odd], ph[0][0], ph[0][RT - 1], ph[1][0], ph[1][RT - 1], b0, b1);
+        q8_mma_bf16(o[t][odd], pl[0][0], pl[0][RT - 1], pl[1][0], pl[1][RT - 1], b0, b1);
+      }
+    }
+    fence_proxy_async_smem();  // ordinary accesses to the stage before TMA fills it
+    __threadfence_block();
+    __syncwarp();
+    prefetch(n + p.stages);
+  }
+  // ---- codes -----------------------------------------------------------------------------------------------------------------
+  float my_ks = 0.f, my_vs = 0.f;  // scales of the next 32 items, one per lane
+  for (int i = 0; i < n_code; ++i) {
+    const int n = n_raw + i, slot = n % p.stages, key0 = first_key(it0 + warp + i * QD_WARPS);
+    if ((i & 31) == 0 && i + lane < n_code) {
+      const long long blk = head * p.blocks + first_key(it0 + warp + (i + lane) * QD_WARPS) / Q8_BLOCK;
+      my_ks = p.ks[blk];
+      my_vs = p.vs[blk];
+    }
+    const float c = c_unit * __shfl_sync(0xffffffffu, my_ks, i & 31), rel = __shfl_sync(0xffffffffu, my_vs, i & 31) / ref;
+    ok = mbar_wait_warp(&bars[warp][slot], (uint32_t)(i / p.stages) & 1u, &abort_flag, p.err, ERR_Q8_CODES);
+    if (!ok) {
+      given_up = i;
+      break;
+    }
+    const uint8_t* st = ring + slot * STAGE;
+    float s[QD_KEYS / 8][2 * RT];
+#pragma unroll
+    for (int t = 0; t < QD_KEYS / 8; ++t) {
+#pragma unroll
+      for (int e = 0; e < 2 * RT; ++e) s[t][e] = 0.f;
+      const int r = 8 * t + quad;
+#pragma unroll
+      for (int i2 = 0; i2 < KG; ++i2) {
+        const int ch = DK == 128 ? (4 * i2 + j) ^ (r & 7) : j ^ ((r >> 1) & 3);
+        const uint4 w = *reinterpret_cast<const uint4*>(st + r * DK + ch * 16);
+        const uint32_t k[4] = {w.x ^ 0x80808080u, w.y ^ 0x80808080u, w.z ^ 0x80808080u, w.w ^ 0x80808080u};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          q8_mma_f16(s[t], q[0][i2][2 * e], q[RT - 1][i2][2 * e], q[0][i2][2 * e + 1], q[RT - 1][i2][2 * e + 1], q8_pair<0x4140>(k[e]),
+                     q8_pair<0x4342>(k[e]));
+      }
+    }
+    const bool full = key0 + QD_KEYS <= own_lo && (key0 >= lo_max || key0 + QD_KEYS <= p.keep_first);
+    if (full) {
+#pragma unroll
+      for (int t = 0; t < QD_KEYS / 8; ++t)
+#pragma unroll
+        for (int e = 0; e < 2 * RT; ++e) s[t][e] *= c;
+    } else {
+#pragma unroll
+      for (int t = 0; t < QD_KEYS / 8; ++t)
+#pragma unroll
+        for (int e = 0; e < 2 * RT; ++e) {
+          const int key = key0 + 8 * t + 2 * j + (e & 1), m = e >> 1;
+          s[t][e] = key < own[m] && (key >= lo[m] || key < p.keep_first) ? s[t][e] * c : -INFINITY;
+        }
+    }
+    softmax(s);
+    uint32_t ph[QD_KEYS / 8][RT];
+#pragma unroll
+    for (int t = 0; t < QD_KEYS / 8; ++t)
+#pragma unroll
+      for (int m = 0; m < RT; ++m) ph[t][m] = q8_pack_f16(s[t][2 * m] * rel, s[t][2 * m + 1] * rel);
+    const uint32_t sv = smem_u32(st + QD_KEYS * DK) + lane * DV;
+#pragma unroll
+    for (int t = 0; t < VT; ++t) {
+      if (t * 16 < p.vdim) {
+        uint32_t w[4];  // keys 8 e + 2 j, + 1: features 16 t + 2 quad, + 1 of each
+        const int ch = DV == 128 ? t ^ (lane & 7) : t ^ ((lane >> 1) & 3);
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                     : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                     : "r"(sv + ch * 16));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] ^= 0x80808080u;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          q8_mma_f16(o[t][0], ph[2 * k][0], ph[2 * k][RT - 1], ph[2 * k + 1][0], ph[2 * k + 1][RT - 1], q8_pair<0x4240>(w[2 * k]),
+                     q8_pair<0x4240>(w[2 * k + 1]));
+          q8_mma_f16(o[t][1], ph[2 * k][0], ph[2 * k][RT - 1], ph[2 * k + 1][0], ph[2 * k + 1][RT - 1], q8_pair<0x4341>(w[2 * k]),
+                     q8_pair<0x4341>(w[2 * k + 1]));
+        }
+      }
+    }
+    __threadfence_block();  // the reads of all lanes have taken place before the stage is filled again
+    __syncwarp();
+    prefetch(n + p.stages);
+  }
+  if (!ok) {  // loads in flight target this CTA's shared memory: give them a bounded time to land before the CTA ends
+    for (int i = given_up; i < min(n_code, given_up + p.stages); ++i)
+      for (uint32_t w = 0; w < MBAR_SPIN_LIMIT && !mbar_try_wait(&bars[warp][(n_raw + i) % p.stages], (uint32_t)(i / p.stages) & 1u); ++w) {}
+  }
+  // From here on one warp per row; features c of a lane: (lane + 32 u) * 4 .. The gates are asked for before they are needed.
+  constexpr int CH = (DV + 127) / 128, MINE = ROWS / QD_WARPS;
+  uint2 gates[MINE][CH];
+#pragma unroll
+  for (int i = 0; i < MINE; ++i)
+#pragma unroll
+    for (int u = 0; u < CH; ++u) {
+      const int r = warp + i * QD_WARPS, at = chunk * ROWS + r, c = (lane + 32 * u) * 4;
+      gates[i][u] = make_uint2(0u, 0u);
+      if (p.gated && r < nh && c < p.vdim)
+        gates[i][u] = *reinterpret_cast<const uint2*>(p.proj + ((long long)b * p.T + at / R) * p.ld + plain + (long long)(g * R + at % R) * p.vdim + c);
+    }
+#pragma unroll
+  for (int m = 0; m < RT; ++m) {
+    l[m] += __shfl_xor_sync(0xffffffffu, l[m], 1);
+    l[m] += __shfl_xor_sync(0xffffffffu, l[m], 2);
+    if (j == 0) {
+      sm[warp][quad + 8 * m] = mx[m];
+      sl[warp][quad + 8 * m] = l[m];
+    }
+  }
+  __syncthreads();  // all rings are idle: their memory holds the warps' outputs from here on
+  float* so = reinterpret_cast<float*>(smem);  // [QD_WARPS][ROWS][vdim + 8]
+  const int old = p.vdim + 8;                  // the padding keeps the quads' stores in different banks
+#pragma unroll
+  for (int t = 0; t < VT; ++t) {
+    if (t * 16 < p.vdim) {
+#pragma unroll
+      for (int m = 0; m < RT; ++m)
+        *reinterpret_cast<float4*>(so + (warp * ROWS + quad + 8 * m) * old + t * 16 + 4 * j) =
+            make_float4(o[t][0][2 * m] * ref, o[t][1][2 * m] * ref, o[t][0][2 * m + 1] * ref, o[t][1][2 * m + 1] * ref);
+    }
+  }
+  // ---- merge of the warps: their weights, and the sums of the weights --------------------------------------------------------
+  const long long units = (long long)gridDim.z * gridDim.y, unit = (long long)b * gridDim.y + blockIdx.y;
+  const float sink = p.sink * 1.4426950408889634f;
+  float2* stats = reinterpret_cast<float2*>(p.part + units * splits * ROWS * p.vdim);
+  if (threadIdx.x < ROWS) {
+    const int r = threadIdx.x;
+    float m = splits > 1 ? -INFINITY : sink;
+#pragma unroll
+    for (int w = 0; w < QD_WARPS; ++w) m = fmaxf(m, sm[w][r]);
+    float ll = splits > 1 || sink == -INFINITY ? 0.f : exp2f(sink - m);
+#pragma unroll
+    for (int w = 0; w < QD_WARPS; ++w) {
+      const float f = sm[w][r] == -INFINITY ? 0.f : exp2f(sm[w][r] - m);
+      fw[w][r] = f;
+      ll += sm[w][r] == -INFINITY ? 0.f : sl[w][r] * f;
+    }
+    fl[r] = ll;
+    if (splits > 1) __stcg(stats + (unit * splits + split) * ROWS + r, make_float2(m, ll));
+  }
+  __syncthreads();
+  auto merged = [&](int r, int c) {  // row r, features c .. c + 3, over this CTA's warps
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < QD_WARPS; ++w) {
+      const float f = fw[w][r];
+      const float4 x = *reinterpret_cast<const float4*>(so + (w * ROWS + r) * old + c);
+      if (sm[w][r] != -INFINITY) a = make_float4(a.x + x.x * f, a.y + x.y * f, a.z + x.z * f, a.w + x.w * f);
+    }
+    return a;
+  };
+  if (splits > 1) {
+    for (int r = warp; r < nh; r += QD_WARPS)
+#pragma unroll
+      for (int u = 0; u < CH; ++u) {
+        const int c = (lane + 32 * u) * 4;
+        if (c < p.vdim) __stcg(reinterpret_cast<float4*>(p.part + ((unit * splits + split) * ROWS + r) * p.vdim + c), merged(r, c));
+      }
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) is_last = atomicAdd(p.counters + unit, 1u) == (unsigned int)splits - 1;
+    __syncthreads();
+    if (!is_last) return;
+    __threadfence();
+    for (int i = threadIdx.x; i < splits * ROWS; i += blockDim.x) {
+      const float2 v = __ldcg(stats + unit * splits * ROWS + i);
+      wt[i] = v.x;
+      wl[i] = v.y;
+    }
+    __syncthreads();
+    if (threadIdx.x < ROWS) {
+      float m = sink;
+      for (int k = 0; k < splits; ++k) m = fmaxf(m, wt[k * ROWS + threadIdx.x]);
+      float ll = sink == -INFINITY ? 0.f : exp2f(sink - m);
+      for (int k = 0; k < splits; ++k) {
+        float& w = wt[k * ROWS + threadIdx.x];
+        w = w == -INFINITY ? 0.f : exp2f(w - m);
+        ll += w * wl[k * ROWS + threadIdx.x];
+      }
+      fl[threadIdx.x] = ll;
+    }
+    if (threadIdx.x == 0) p.counters[unit] = 0;
+    __syncthreads();
+  }
+#pragma unroll
+  for (int i = 0; i < MINE; ++i) {
+    const int r = warp + i * QD_WARPS;
+    if (r >= nh) break;
+    const int at = chunk * ROWS + r;
+    const float sum = fl[r];
+    __nv_bfloat16* out = p.out + ((long long)b * p.T + at / R) * p.ldo + (long long)(g * R + at % R) * p.vdim;
+#pragma unroll
+    for (int u = 0; u < CH; ++u) {
+      const int c = (lane + 32 * u) * 4;
+      if (c >= p.vdim) continue;
+      float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (splits > 1) {
+        const float* src = p.part + (unit * splits * ROWS + r) * p.vdim + c;
+#pragma unroll 4
+        for (int k = 0; k < splits; ++k) {
+          const float f = wt[k * ROWS + r];
+          const float4 x = __ldcg(reinterpret_cast<const float4*>(src + (long long)k * ROWS * p.vdim));
+          if (f != 0.f) a = make_float4(a.x + x.x * f, a.y + x.y * f, a.z + x.z * f, a.w + x.w * f);
+        }
+      } else {
+        a = merged(r, c);
+      }
+      float v[4] = {a.x / sum, a.y / sum, a.z / sum, a.w / sum};
+      if (p.gated) {
+        const uint2 gt = gates[i][u];
+        v[0] *= 1.f / (1.f + expf(-dd_lo(gt.x)));
+        v[1] *= 1.f / (1.f + expf(-dd_hi(gt.x)));
+        v[2] *= 1.f / (1.f + expf(-dd_lo(gt.y)));
+        v[3] *= 1.f / (1.f + expf(-dd_hi(gt.y)));
+      }
+      dd_store4(out + c, v[0], v[1], v[2], v[3], ((uintptr_t)out & 3) == 0);
+    }
+  }
+}
+
+// 2-D map over rows of `cols` codes, boxes of {width, QD_KEYS}: columns past the row are filled with zeros
+int q8_make_map(CUtensorMap* map, const void* ptr, long long rows, int cols, int width) {
+  xl_tc::EncodeTiledFn fn = xl_tc::get_encode_fn();
+  if (!fn) return -2;
+  cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)cols};
+  cuuint32_t box[2] = {(cuuint32_t)width, QD_KEYS};
+  cuuint32_t estr[2] = {1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, (void*)ptr, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        width == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : -3;
+}
+
+constexpr int QD_RING_LIMIT = 100 * 1024;  // two CTAs per SM
+
+template <int DK, int DV, int RT, bool FUSED> int q8_few_launch(Q8FewParams p, int B, int splits, cudaStream_t s) {
+  constexpr int STAGE = q8_stage_bytes<DK, DV>() * QD_WARPS;
+  p.stages = 4 * STAGE <= QD_RING_LIMIT ? 4 : 3;
+  static_assert(3 * STAGE <= QD_RING_LIMIT, "ring");
+  constexpr int merge = QD_WARPS * 8 * RT * (DV + 8) * 4;
+  const int ring = p.stages * STAGE, bytes = (ring > merge ? ring : merge) + 1024;
+  CUtensorMap mk, mv;
+  const long long rows = (long long)B * p.G * p.blocks * Q8_BLOCK;
+  int r = q8_make_map(&mk, p.kc, rows, p.dim, DK);
+  if (!r) r = q8_make_map(&mv, p.vc, rows, p.vdim, DV);
+  if (r) return r;
+  static XlPerDevice smem;
+  XL_TRY(xl_allow_smem(q8_few_rows_kernel<DK, DV, RT, FUSED>, bytes, smem));
+  const int chunks = (p.T * (p.H / p.G) + 8 * RT - 1) / (8 * RT);
+  const cudaError_t e = xl_launch_overlapped(q8_few_rows_kernel<DK, DV, RT, FUSED>, dim3(splits, p.G * chunks, B), dim3(QD_WARPS * 32),
+                                             (size_t)bytes, s, mk, mv, p);
+  return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
+}
+
+template <int DK, int DV> int q8_few_sizes(const Q8FewParams& p, int B, int splits, cudaStream_t s) {
+  const bool one = p.T * (p.H / p.G) <= 8;
+  if (p.T == 1) return one ? q8_few_launch<DK, DV, 1, true>(p, B, splits, s) : q8_few_launch<DK, DV, 2, true>(p, B, splits, s);
+  return one ? q8_few_launch<DK, DV, 1, false>(p, B, splits, s) : q8_few_launch<DK, DV, 2, false>(p, B, splits, s);
+}
+
 bool q8_sizes_ok(int B, int T, int H, int G, int dim, int vdim, int blocks) {
   return B >= 1 && B <= 65535 && T >= 1 && T <= (1 << 24) && G >= 1 && G <= 65535 && H >= 1 && H <= 65535 && H % G == 0 && dim >= 1 &&
          dim <= Q8_MAX_DIM && vdim >= 1 && vdim <= Q8_MAX_DIM && blocks >= 1 && blocks <= (1 << 24);
@@ -367,4 +1042,32 @@ XL_API int xl_q8_attn_general(const float* q, const void* raw_k, const void* raw
     XL_TRY(xl_launch_overlapped(kernel, grid, block, (size_t)0, s, p));
   });
   return (int)cudaGetLastError();
+}
+
+// Few rows per sequence, bf16: dim, vdim multiples of 16 up to 128, ld, ldo and all pointers as the 16-byte accesses need them.
+// T = 1: the kernel normalises, appends and completes blocks itself (q and raw rows are null). T > 1: after xl_q8_append, on its q and
+// raw rows, with read_ahead 0. part: B * G * ceil(T H/G / 8 RT) * splits * 8 RT * (vdim + 2) floats with RT = 1 where T H/G <= 8, else
+// 2; counters: B * G * ceil(...) zero-initialised words (left zeroed). read_ahead: positions, counts and the cache were complete before the
+// previous launch. err: device int for the code of a wait that gave up.
+XL_API int xl_q8_attn_few(const void* proj, long long ld, const float* wq, const float* wk, const float* q, const void* raw_k,
+                          const void* raw_v, void* kc, void* vc, float* ks, float* vs, void* kt, void* vt, void* out, long long ldo,
+                          const int* pos, const int* count, int B, int T, int H, int G, int dim, int vdim, int blocks, int window,
+                          int keep_first, int gated, float scale, float sink, double eps, int splits, float* part, unsigned int* counters,
+                          int read_ahead, int* err, cudaStream_t s) {
+  if (!q8_sizes_ok(B, T, H, G, dim, vdim, blocks) || window < 0 || keep_first < 0 || !(scale > 0.f) || !wq || !wk) return -1;
+  if (dim % 16 || vdim % 16 || dim > 128 || vdim > 128 || ld % 8 || ldo < (long long)H * vdim || splits < 1 || splits > QD_MAX_SPLITS ||
+      ld < (long long)(H + G) * dim + (long long)G * vdim + (gated ? (long long)H * vdim : 0) || (T > 1 && (read_ahead || !q || !raw_k || !raw_v)))
+    return -1;
+  const uintptr_t at = (uintptr_t)proj | (uintptr_t)raw_k | (uintptr_t)raw_v | (uintptr_t)kc | (uintptr_t)vc | (uintptr_t)kt | (uintptr_t)vt;
+  if ((at & 15) || (splits > 1 && (!part || ((uintptr_t)part & 15) || !counters)) || !err) return -1;
+  const long long chunks = ((long long)T * (H / G) + 7) / 8;
+  if ((long long)B * G * blocks * Q8_BLOCK > 0x7fffff00LL || G * chunks > 65535) return -1;
+  Q8FewParams p = {};
+  p.proj = (const __nv_bfloat16*)proj; p.ld = ld; p.wq = wq; p.wk = wk; p.q = q; p.raw_k = (const __nv_bfloat16*)raw_k;
+  p.raw_v = (const __nv_bfloat16*)raw_v; p.kc = (int8_t*)kc; p.vc = (int8_t*)vc; p.ks = ks; p.vs = vs; p.kt = (__nv_bfloat16*)kt;
+  p.vt = (__nv_bfloat16*)vt; p.out = (__nv_bfloat16*)out; p.ldo = ldo; p.pos = pos; p.count = count; p.T = T; p.H = H; p.G = G;
+  p.dim = dim; p.vdim = vdim; p.blocks = blocks; p.window = window; p.keep_first = keep_first; p.gated = gated; p.scale = scale;
+  p.sink = sink; p.eps = eps; p.part = part; p.counters = counters; p.read_ahead = read_ahead; p.err = err;
+  if (dim <= 64) return vdim <= 64 ? q8_few_sizes<64, 64>(p, B, splits, s) : q8_few_sizes<64, 128>(p, B, splits, s);
+  return vdim <= 64 ? q8_few_sizes<128, 64>(p, B, splits, s) : q8_few_sizes<128, 128>(p, B, splits, s);
 }

@@ -294,7 +294,8 @@ def check_gemm_errors():
                      61: "int4 product: codes or tokens never arrived", 62: "int4 product: shared-memory stage was never released (codes)",
                      63: "int4 product: shared-memory stage was never released (tokens)",
                      64: "decode attention: keys and values never arrived",
-                     65: "decode attention: shared-memory stage was never released"}
+                     65: "decode attention: shared-memory stage was never released",
+                     91: "attention over an 8-bit cache: codes never arrived"}
             raise RuntimeError(f"tcgen05 GEMM on cuda:{idx} gave up waiting: {names.get(code, code)}")
 
 

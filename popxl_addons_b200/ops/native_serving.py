@@ -3,9 +3,10 @@ import ctypes
 
 import torch
 
+from ..xl import read_ahead
 from ..xl.opdef import native
-from .native import _CODE, _c_f, _c_int, _c_ll, _c_p, _check, _count, _ok, _sig, _stream, counters
-from .native_sequence import _clamped_glu, _f32, _i32, _ptr, stream_rms
+from .native import _CODE, _c_f, _c_int, _c_ll, _c_p, _check, _count, _ok, _sig, _stream, counters, gemm_error_flag
+from .native_sequence import _clamped_glu, _decode_slices, _f32, _i32, _ptr, stream_rms
 
 _c_d = ctypes.c_double
 _shape_logits = _sig("xl_shape_logits", *[_c_p] * 10, *[_c_int] * 7, _c_p)
@@ -13,6 +14,8 @@ _take_shaped = _sig("xl_take_shaped", *[_c_p] * 13, *[_c_int] * 11, _c_p)
 _append_tokens = _sig("xl_append_tokens", _c_p, _c_p, _c_p, _c_p, _c_int, _c_int, _c_int, _c_p)
 _q8_append = _sig("xl_q8_append", _c_p, _c_ll, *[_c_p] * 13, *[_c_int] * 7, _c_d, _c_int, _c_p)
 _q8_general = _sig("xl_q8_attn_general", *[_c_p] * 8, _c_ll, _c_p, _c_ll, _c_p, _c_p, *[_c_int] * 9, _c_f, _c_f, _c_int, _c_p)
+_q8_few = _sig("xl_q8_attn_few", _c_p, _c_ll, *[_c_p] * 12, _c_ll, _c_p, _c_p, *[_c_int] * 10, _c_f, _c_f, _c_d, _c_int, _c_p, _c_p, _c_int,
+               _c_p, _c_p)
 
 
 def _launched(rc, name) -> bool:
@@ -98,12 +101,33 @@ def window_attention_q8_cuda(proj, q_norm, k_norm, k, v, k_scale, v_scale, k_tai
     sink = float("-inf") if sink is None else sink
     gate = proj.data_ptr() + plain * proj.element_size() if proj.shape[1] > plain else None
     cache = tuple(t.data_ptr() for t in (k, v, k_scale, v_scale))
+    sizes = (B, T, heads, G, dim, vdim, blocks, window, keep_first)
+
+    def few(q, raw, ahead):
+        rows = T * (heads // G)
+        per = 8 if rows <= 8 else 16  # rows of a CTA
+        units = B * G * -(-rows // per)
+        if units > 1 << 16:
+            return False
+        longest = min(blocks * 64, window + keep_first + T) if window else blocks * 64
+        splits = _decode_slices(units, longest, 320, dev)
+        done = counters(units, dev, "counters sequence", 1 << 16)
+        part = torch.empty(units * splits * per * (vdim + 2), dtype=torch.float32, device=dev) if splits > 1 else None
+        rc = _q8_few(proj.data_ptr(), ld, q_norm.data_ptr(), k_norm.data_ptr(), _ptr(q), _ptr(raw[0]), _ptr(raw[1]), *cache, k_tail.data_ptr(),
+                     v_tail.data_ptr(), joint.data_ptr(), ldo, pos.data_ptr(), count.data_ptr(), *sizes, int(gate is not None), scale, sink,
+                     eps, splits, _ptr(part), done.data_ptr(), int(ahead), gemm_error_flag(dev).data_ptr(), s)
+        return _launched(rc, "q8_attn_few")
+
+    if T == 1 and dt == torch.bfloat16 and few(None, (None, None), read_ahead.allowed(pos, count, k, v, k_scale, v_scale, k_tail, v_tail)):
+        return joint
     q = torch.empty((B, G, T, heads // G, dim), dtype=torch.float32, device=dev)
     raw = [torch.empty((B, G, T + 64, width), dtype=dt, device=dev) for width in (dim, vdim)]
     rc = _q8_append(proj.data_ptr(), ld, q_norm.data_ptr(), k_norm.data_ptr(), q.data_ptr(), raw[0].data_ptr(), raw[1].data_ptr(), *cache,
                     k_tail.data_ptr(), v_tail.data_ptr(), pos.data_ptr(), count.data_ptr(), B, T, heads, G, dim, vdim, blocks, eps, code, s)
     if not _launched(rc, "q8_append"):
         return NotImplemented
+    if dt == torch.bfloat16 and T * (heads // G) <= 64 and few(q, raw, False):
+        return joint
     rc = _q8_general(q.data_ptr(), raw[0].data_ptr(), raw[1].data_ptr(), *cache, gate, ld, joint.data_ptr(), ldo, pos.data_ptr(),
                      count.data_ptr(), B, T, heads, G, dim, vdim, blocks, window, keep_first, scale, sink, code, s)
     return joint if _launched(rc, "q8_attn_general") else NotImplemented
