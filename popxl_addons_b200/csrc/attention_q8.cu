@@ -335,10 +335,13 @@ __global__ void __launch_bounds__(SPLIT == 1 ? 128 : SPLIT * 32) q8_attn_general
 // their items independently, each through a ring of its own (the codes by TMA, swizzled so that 16-byte reads by rows and ldmatrix
 // by columns meet few bank conflicts), with online softmax state in registers.
 //
-//   scores   A: queries as fp16 (divided by a power of two above the norm's factors), B: codes as fp16, which is exact; the scale of
-//            the block multiplies the fp32 result
-//   output   A: weights times value scale over the warp's largest, as fp16 (2^-12 relative); B: codes as fp16, exact
-//   raw rows keys as fp16 likewise, values in bf16 with weights as sums of two bf16 numbers
+// The products are taken transposed, so that the few query rows are the eight columns of the instruction and its sixteen rows are
+// keys and features (with queries as rows, eight heads fill half of every instruction and every accumulator):
+//   S^T = K Q^T   A: codes as fp16, which is exact; B: queries as fp16, divided by a power of two above the norm's factors. The
+//                 scale of the block multiplies the fp32 result.
+//   O^T = V^T P^T A: codes as fp16; B: weights times value scale over the warp's largest, as fp16 (2^-12 relative), transposed between
+//                 the lanes by movmatrix
+//   raw rows      keys as fp16 likewise, values in bf16 with weights as sums of two bf16 numbers
 //
 // A code c becomes fp16 by two instructions for two of them: the byte c + 128 is the low byte of 1024 + (c + 128) under the high byte
 // 0x64, from which 1152 is taken. The value product needs keys in pairs: ldmatrix transposes pairs of bytes, that is two features of
@@ -370,26 +373,21 @@ struct Q8FewParams {
   int* err;
 };
 
-__device__ __forceinline__ void q8_mma_f16(float (&c)[4], const uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-// eight rows in use: the upper eight are zero
-__device__ __forceinline__ void q8_mma_f16(float (&c)[2], const uint32_t a0, uint32_t, uint32_t a2, uint32_t, uint32_t b0, uint32_t b1) {
-  float unused0, unused1;
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%12};"
-               : "=f"(c[0]), "=f"(c[1]), "=f"(unused0), "=f"(unused1)
-               : "r"(a0), "r"(0u), "r"(a2), "r"(0u), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(0.f));
+__device__ __forceinline__ void q8_mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void q8_mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  dd_mma(c, a0, a1, a2, a3, b0, b1);
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void q8_mma_bf16(float (&c)[2], uint32_t a0, uint32_t, uint32_t a2, uint32_t, uint32_t b0, uint32_t b1) {
-  float unused0, unused1;
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%12};"
-               : "=f"(c[0]), "=f"(c[1]), "=f"(unused0), "=f"(unused1)
-               : "r"(a0), "r"(0u), "r"(a2), "r"(0u), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(0.f));
+// transpose of an 8 x 8 matrix of 16-bit values: lane 4 r + c holds elements (r, 2 c), (r, 2 c + 1) before and (2 c, r), (2 c + 1, r) after
+__device__ __forceinline__ uint32_t q8_transpose(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
 }
 __device__ __forceinline__ uint32_t q8_pack_f16(float lo, float hi) {
   uint32_t r;
@@ -408,7 +406,7 @@ template <int DK, int DV> __host__ __device__ constexpr int q8_stage_bytes() { r
 
 // DK, DV: 64 or 128, features of a key and of a value rounded up
 template <int DK, int DV, int RT, bool FUSED>
-__global__ void __launch_bounds__(QD_WARPS * 32, 2)
+__global__ void __launch_bounds__(QD_WARPS * 32, RT == 1 ? 3 : 2)
     q8_few_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const Q8FewParams p) {
   using namespace xl_tc;
   constexpr int ROWS = 8 * RT, STAGE = q8_stage_bytes<DK, DV>(), KG = DK / 64, VT = DV / 16;
@@ -560,7 +558,7 @@ __global__ void __launch_bounds__(QD_WARPS * 32, 2)
     }
   }
   __syncthreads();
-  uint32_t q[RT][KG][8];  // rows quad (+ 8), features 64 i + 16 j .. + 15
+  uint32_t q[RT][KG][8];  // rows quad + 8 m, features 64 i + 16 j .. + 15
 #pragma unroll
   for (int m = 0; m < RT; ++m)
 #pragma unroll
@@ -570,60 +568,67 @@ __global__ void __launch_bounds__(QD_WARPS * 32, 2)
         const uint4 w = *reinterpret_cast<const uint4*>(&sq[quad + 8 * m][64 * i + 16 * j + 8 * u]);
         q[m][i][4 * u] = w.x; q[m][i][4 * u + 1] = w.y; q[m][i][4 * u + 2] = w.z; q[m][i][4 * u + 3] = w.w;
       }
-  int qpos[RT], lo[RT], own[RT];
+  int qpos[RT][2];  // positions of this lane's rows of the scores: 8 m + 2 j + e
 #pragma unroll
-  for (int m = 0; m < RT; ++m) {
-    qpos[m] = min(p_hi, pos + (chunk * ROWS + quad + 8 * m) / R);
-    lo[m] = p.window ? qpos[m] - p.window + 1 : 0;
-    own[m] = qpos[m] / Q8_BLOCK * Q8_BLOCK;
-  }
+  for (int m = 0; m < RT; ++m)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) qpos[m][e] = FUSED ? pos : min(p_hi, pos + (chunk * ROWS + 8 * m + 2 * j + e) / R);
   const int lo_max = p.window ? p_hi - p.window + 1 : 0;
-  float o[VT][2][2 * RT];  // even and odd features of a tile of 16
+  auto sees = [&](int at, int key, bool raw) {
+    const int own = at / Q8_BLOCK * Q8_BLOCK;
+    return (raw ? key >= own && key <= at : key < own) && (!p.window || key > at - p.window || key < p.keep_first);
+  };
+  float o[VT][RT][4];  // features 16 t + 2 quad + (e >> 1), rows 8 m + 2 j + (e & 1)
 #pragma unroll
   for (int t = 0; t < VT; ++t)
 #pragma unroll
-    for (int e = 0; e < 2 * RT; ++e) o[t][0][e] = o[t][1][e] = 0.f;
-  float mx[RT], l[RT];
+    for (int m = 0; m < RT; ++m)
 #pragma unroll
-  for (int m = 0; m < RT; ++m) {
-    mx[m] = -INFINITY;
-    l[m] = 0.f;
-  }
+      for (int e = 0; e < 4; ++e) o[t][m][e] = 0.f;
+  float mx[RT][2], l[RT][2];
+#pragma unroll
+  for (int m = 0; m < RT; ++m)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      mx[m][e] = -INFINITY;
+      l[m][e] = 0.f;
+    }
   const float c_unit = p.scale * 1.4426950408889634f * unit_q;
-  // scores of NT tiles of eight keys -> weights (in place); rescales the output where a maximum moved
+  // scores of NT tiles of 16 keys (keys 16 t + quad + 8 (e >> 1)) -> weights (in place); rescales the output where a maximum moved
   auto softmax = [&](auto& s) {
     constexpr int NT = sizeof(s) / sizeof(s[0]);
-    float alpha[RT];
     bool moved = false;
+    float alpha[RT][2];
 #pragma unroll
-    for (int m = 0; m < RT; ++m) {
-      float v = -INFINITY;
+    for (int m = 0; m < RT; ++m)
 #pragma unroll
-      for (int t = 0; t < NT; ++t) v = fmaxf(v, fmaxf(s[t][2 * m], s[t][2 * m + 1]));
-      v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
-      v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
-      const float m_new = fmaxf(mx[m], v), m_use = m_new == -INFINITY ? 0.f : m_new;  // a row may see none of these keys
-      alpha[m] = exp2f(mx[m] - m_use);
-      mx[m] = m_new;
-      float sum = 0.f;
+      for (int e = 0; e < 2; ++e) {
+        float v = -INFINITY;
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
+        for (int t = 0; t < NT; ++t) v = fmaxf(v, fmaxf(s[t][m][e], s[t][m][e + 2]));
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          s[t][2 * m + e] = exp2f(s[t][2 * m + e] - m_use);
-          sum += s[t][2 * m + e];
-        }
-      l[m] = l[m] * alpha[m] + sum;  // this lane's share of the row sum
-      moved |= alpha[m] != 1.f;
-    }
+        for (int d = 4; d < 32; d *= 2) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
+        const float m_new = fmaxf(mx[m][e], v), m_use = m_new == -INFINITY ? 0.f : m_new;  // a row may see none of these keys
+        alpha[m][e] = xl_tc::fast_exp2(mx[m][e] - m_use);
+        moved |= m_new != mx[m][e];
+        mx[m][e] = m_new;
+        float sum = 0.f;
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int u = 0; u < 4; u += 2) {
+            s[t][m][e + u] = xl_tc::fast_exp2(s[t][m][e + u] - m_use);
+            sum += s[t][m][e + u];
+          }
+        l[m][e] = l[m][e] * alpha[m][e] + sum;  // this lane's share of the row sum
+      }
     if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
       for (int t = 0; t < VT; ++t)
 #pragma unroll
-        for (int e = 0; e < 2 * RT; ++e) {
-          o[t][0][e] *= alpha[e >> 1];
-          o[t][1][e] *= alpha[e >> 1];
-        }
+        for (int m = 0; m < RT; ++m)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[t][m][e] *= alpha[m][e & 1];
     }
   };
   bool ok = true;
@@ -684,41 +689,46 @@ __global__ void __launch_bounds__(QD_WARPS * 32, 2)
           write(*reinterpret_cast<const uint4*>(sv + r * (DV * 2) + ((c ^ (r & 6)) * 16)), p.vc + (blk * Q8_BLOCK + r0 + r) * p.vdim + c * 8, scale[1]);
       }
     }
-    float s[QD_RAW / 8][2 * RT];
+    float s[1][RT][4];
 #pragma unroll
-    for (int t = 0; t < QD_RAW / 8; ++t) {
+    for (int m = 0; m < RT; ++m)
 #pragma unroll
-      for (int e = 0; e < 2 * RT; ++e) s[t][e] = 0.f;
-      const int r = 8 * t + quad;
-      const float inv = 1.f / unit_k;
+      for (int e = 0; e < 4; ++e) s[0][m][e] = 0.f;
+    const float inv = 1.f / unit_k;
 #pragma unroll
-      for (int i = 0; i < KG; ++i)
+    for (int i = 0; i < KG; ++i)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const uint4 w = *reinterpret_cast<const uint4*>(st + r * (DK * 2) + (((8 * i + 2 * j + u) ^ (r & 7)) * 16));
-          uint32_t k[4] = {w.x, w.y, w.z, w.w};
+      for (int u = 0; u < 2; ++u) {
+        uint32_t k[2][4];  // keys quad, quad + 8
 #pragma unroll
-          for (int e = 0; e < 4; ++e) k[e] = q8_pack_f16(dd_lo(k[e]) * inv, dd_hi(k[e]) * inv);
-          q8_mma_f16(s[t], q[0][i][4 * u], q[RT - 1][i][4 * u], q[0][i][4 * u + 1], q[RT - 1][i][4 * u + 1], k[0], k[1]);
-          q8_mma_f16(s[t], q[0][i][4 * u + 2], q[RT - 1][i][4 * u + 2], q[0][i][4 * u + 3], q[RT - 1][i][4 * u + 3], k[2], k[3]);
+        for (int h = 0; h < 2; ++h) {
+          const uint4 w = *reinterpret_cast<const uint4*>(st + (quad + 8 * h) * (DK * 2) + (((8 * i + 2 * j + u) ^ quad) * 16));
+          const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) k[h][e] = q8_pack_f16(dd_lo(x[e]) * inv, dd_hi(x[e]) * inv);
         }
-      const float c = c_unit * unit_k;
 #pragma unroll
-      for (int e = 0; e < 2 * RT; ++e) {
-        const int key = key0 + 8 * t + 2 * j + (e & 1), m = e >> 1;
-        s[t][e] = key >= own[m] && key <= qpos[m] && (key >= lo[m] || key < p.keep_first) ? s[t][e] * c : -INFINITY;
+        for (int e = 0; e < 4; e += 2)
+#pragma unroll
+          for (int m = 0; m < RT; ++m)
+            q8_mma_f16(s[0][m], k[0][e], k[1][e], k[0][e + 1], k[1][e + 1], q[m][i][4 * u + e], q[m][i][4 * u + e + 1]);
       }
-    }
+    const float c = c_unit * unit_k;
+#pragma unroll
+    for (int m = 0; m < RT; ++m)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[0][m][e] = sees(qpos[m][e & 1], key0 + quad + 8 * (e >> 1), true) ? s[0][m][e] * c : -INFINITY;
     softmax(s);
-    uint32_t ph[2][RT], pl[2][RT];  // weights in units of `ref` as operands of the second product, and their rounding errors
+    uint32_t ph[RT][2], pl[RT][2];  // weights in units of `ref` as operands of the second product, and their rounding errors
     const float inv_ref = 1.f / ref;
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int m = 0; m < RT; ++m)
 #pragma unroll
-      for (int m = 0; m < RT; ++m) {
-        const float x = s[t][2 * m] * inv_ref, y = s[t][2 * m + 1] * inv_ref;
-        ph[t][m] = dd_pack(x, y);
-        pl[t][m] = dd_pack(x - dd_lo(ph[t][m]), y - dd_hi(ph[t][m]));
+      for (int u = 0; u < 2; ++u) {
+        const float x = s[0][m][2 * u] * inv_ref, y = s[0][m][2 * u + 1] * inv_ref;
+        const uint32_t w = dd_pack(x, y);
+        ph[m][u] = q8_transpose(w);
+        pl[m][u] = q8_transpose(dd_pack(x - dd_lo(w), y - dd_hi(w)));
       }
     bool seen[4];  // rows 2 j, 2 j + 1, 2 j + 8, 2 j + 9 of the tile: one that no row sees may hold anything
 #pragma unroll
@@ -731,14 +741,15 @@ __global__ void __launch_bounds__(QD_WARPS * 32, 2)
       uint32_t w[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int r = 2 * j + (e & 1) + 8 * (e >> 1), c = 2 * t + (quad >> 2);
-        w[e] = seen[e] ? *reinterpret_cast<const uint32_t*>(sv + r * (DV * 2) + ((c ^ (r & 6)) * 16) + (quad & 3) * 4) : 0u;
+        const int r = 2 * j + (e & 1) + 8 * (e >> 1), c2 = 2 * t + (quad >> 2);
+        w[e] = seen[e] ? *reinterpret_cast<const uint32_t*>(sv + r * (DV * 2) + ((c2 ^ (r & 6)) * 16) + (quad & 3) * 4) : 0u;
       }
+      const uint32_t a0 = __byte_perm(w[0], w[1], 0x5410), a1 = __byte_perm(w[0], w[1], 0x7632), a2 = __byte_perm(w[2], w[3], 0x5410),
+                     a3 = __byte_perm(w[2], w[3], 0x7632);
 #pragma unroll
-      for (int odd = 0; odd < 2; ++odd) {
-        const uint32_t b0 = __byte_perm(w[0], w[1], odd ? 0x7632 : 0x5410), b1 = __byte_perm(w[2], w[3], odd ? 0x7632 : 0x5410);
-        q8_mma_bf16(o[t][odd], ph[0][0], ph[0][RT - 1], ph[1][0], ph[1][RT - 1], b0, b1);
-        q8_mma_bf16(o[t][odd], pl[0][0], pl[0][RT - 1], pl[1][0], pl[1][RT - 1], b0, b1);
+      for (int m = 0; m < RT; ++m) {
+        q8_mma_bf16(o[t][m], a0, a1, a2, a3, ph[m][0], ph[m][1]);
+        q8_mma_bf16(o[t][m], a0, a1, a2, a3, pl[m][0], pl[m][1]);
       }
     }
     fence_proxy_async_smem();  // ordinary accesses to the stage before TMA fills it
@@ -762,44 +773,59 @@ __global__ void __launch_bounds__(QD_WARPS * 32, 2)
       break;
     }
     const uint8_t* st = ring + slot * STAGE;
-    float s[QD_KEYS / 8][2 * RT];
+    constexpr int NT = QD_KEYS / 16;
+    float s[NT][RT][4];
 #pragma unroll
-    for (int t = 0; t < QD_KEYS / 8; ++t) {
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int e = 0; e < 2 * RT; ++e) s[t][e] = 0.f;
-      const int r = 8 * t + quad;
+      for (int m = 0; m < RT; ++m)
 #pragma unroll
-      for (int i2 = 0; i2 < KG; ++i2) {
-        const int ch = DK == 128 ? (4 * i2 + j) ^ (r & 7) : j ^ ((r >> 1) & 3);
-        const uint4 w = *reinterpret_cast<const uint4*>(st + r * DK + ch * 16);
-        const uint32_t k[4] = {w.x ^ 0x80808080u, w.y ^ 0x80808080u, w.z ^ 0x80808080u, w.w ^ 0x80808080u};
+        for (int e = 0; e < 4; ++e) s[t][m][e] = 0.f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          q8_mma_f16(s[t], q[0][i2][2 * e], q[RT - 1][i2][2 * e], q[0][i2][2 * e + 1], q[RT - 1][i2][2 * e + 1], q8_pair<0x4140>(k[e]),
-                     q8_pair<0x4342>(k[e]));
-      }
-    }
-    const bool full = key0 + QD_KEYS <= own_lo && (key0 >= lo_max || key0 + QD_KEYS <= p.keep_first);
-    if (full) {
+    for (int i2 = 0; i2 < KG; ++i2) {
+      uint32_t k[NT][2][4];
 #pragma unroll
-      for (int t = 0; t < QD_KEYS / 8; ++t)
+      for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int e = 0; e < 2 * RT; ++e) s[t][e] *= c;
-    } else {
+        for (int h = 0; h < 2; ++h) {
+          const int r = 16 * t + 8 * h + quad, ch = DK == 128 ? (4 * i2 + j) ^ quad : j ^ ((r >> 1) & 3);
+          const uint4 w = *reinterpret_cast<const uint4*>(st + r * DK + ch * 16);
+          k[t][h][0] = w.x ^ 0x80808080u; k[t][h][1] = w.y ^ 0x80808080u; k[t][h][2] = w.z ^ 0x80808080u; k[t][h][3] = w.w ^ 0x80808080u;
+        }
 #pragma unroll
-      for (int t = 0; t < QD_KEYS / 8; ++t)
+      for (int e = 0; e < 4; ++e)  // the tiles' products side by side
 #pragma unroll
-        for (int e = 0; e < 2 * RT; ++e) {
-          const int key = key0 + 8 * t + 2 * j + (e & 1), m = e >> 1;
-          s[t][e] = key < own[m] && (key >= lo[m] || key < p.keep_first) ? s[t][e] * c : -INFINITY;
+        for (int t = 0; t < NT; ++t) {
+          const uint32_t a0 = q8_pair<0x4140>(k[t][0][e]), a1 = q8_pair<0x4140>(k[t][1][e]), a2 = q8_pair<0x4342>(k[t][0][e]),
+                         a3 = q8_pair<0x4342>(k[t][1][e]);
+#pragma unroll
+          for (int m = 0; m < RT; ++m) q8_mma_f16(s[t][m], a0, a1, a2, a3, q[m][i2][2 * e], q[m][i2][2 * e + 1]);
         }
     }
+    const bool full = key0 + QD_KEYS <= own_lo && (key0 >= lo_max || key0 + QD_KEYS <= p.keep_first);
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int m = 0; m < RT; ++m)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[t][m][e] *= c;
+    if (!full) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int m = 0; m < RT; ++m)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (!sees(qpos[m][e & 1], key0 + 16 * t + quad + 8 * (e >> 1), false)) s[t][m][e] = -INFINITY;
+    }
     softmax(s);
-    uint32_t ph[QD_KEYS / 8][RT];
+    uint32_t ph[NT][RT][2];
 #pragma unroll
-    for (int t = 0; t < QD_KEYS / 8; ++t)
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int m = 0; m < RT; ++m) ph[t][m] = q8_pack_f16(s[t][2 * m] * rel, s[t][2 * m + 1] * rel);
+      for (int m = 0; m < RT; ++m)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) ph[t][m][u] = q8_transpose(q8_pack_f16(s[t][m][2 * u] * rel, s[t][m][2 * u + 1] * rel));
     const uint32_t sv = smem_u32(st + QD_KEYS * DK) + lane * DV;
 #pragma unroll
     for (int t = 0; t < VT; ++t) {
@@ -812,11 +838,11 @@ __global__ void __launch_bounds__(QD_WARPS * 32, 2)
 #pragma unroll
         for (int e = 0; e < 4; ++e) w[e] ^= 0x80808080u;
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          q8_mma_f16(o[t][0], ph[2 * k][0], ph[2 * k][RT - 1], ph[2 * k + 1][0], ph[2 * k + 1][RT - 1], q8_pair<0x4240>(w[2 * k]),
-                     q8_pair<0x4240>(w[2 * k + 1]));
-          q8_mma_f16(o[t][1], ph[2 * k][0], ph[2 * k][RT - 1], ph[2 * k + 1][0], ph[2 * k + 1][RT - 1], q8_pair<0x4341>(w[2 * k]),
-                     q8_pair<0x4341>(w[2 * k + 1]));
+        for (int k = 0; k < NT; ++k) {
+          const uint32_t a0 = q8_pair<0x4240>(w[2 * k]), a1 = q8_pair<0x4341>(w[2 * k]), a2 = q8_pair<0x4240>(w[2 * k + 1]),
+                         a3 = q8_pair<0x4341>(w[2 * k + 1]);
+#pragma unroll
+          for (int m = 0; m < RT; ++m) q8_mma_f16(o[t][m], a0, a1, a2, a3, ph[k][m][0], ph[k][m][1]);
         }
       }
     }
@@ -841,24 +867,28 @@ __global__ void __launch_bounds__(QD_WARPS * 32, 2)
         gates[i][u] = *reinterpret_cast<const uint2*>(p.proj + ((long long)b * p.T + at / R) * p.ld + plain + (long long)(g * R + at % R) * p.vdim + c);
     }
 #pragma unroll
-  for (int m = 0; m < RT; ++m) {
-    l[m] += __shfl_xor_sync(0xffffffffu, l[m], 1);
-    l[m] += __shfl_xor_sync(0xffffffffu, l[m], 2);
-    if (j == 0) {
-      sm[warp][quad + 8 * m] = mx[m];
-      sl[warp][quad + 8 * m] = l[m];
+  for (int m = 0; m < RT; ++m)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+#pragma unroll
+      for (int d = 4; d < 32; d *= 2) l[m][e] += __shfl_xor_sync(0xffffffffu, l[m][e], d);
+      if (quad == 0) {
+        sm[warp][8 * m + 2 * j + e] = mx[m][e];
+        sl[warp][8 * m + 2 * j + e] = l[m][e];
+      }
     }
-  }
   __syncthreads();  // all rings are idle: their memory holds the warps' outputs from here on
   float* so = reinterpret_cast<float*>(smem);  // [QD_WARPS][ROWS][vdim + 8]
-  const int old = p.vdim + 8;                  // the padding keeps the quads' stores in different banks
+  const int old = p.vdim + 8;                  // the padding keeps the stores of different rows in different banks
 #pragma unroll
   for (int t = 0; t < VT; ++t) {
     if (t * 16 < p.vdim) {
 #pragma unroll
       for (int m = 0; m < RT; ++m)
-        *reinterpret_cast<float4*>(so + (warp * ROWS + quad + 8 * m) * old + t * 16 + 4 * j) =
-            make_float4(o[t][0][2 * m] * ref, o[t][1][2 * m] * ref, o[t][0][2 * m + 1] * ref, o[t][1][2 * m + 1] * ref);
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          *reinterpret_cast<float2*>(so + (warp * ROWS + 8 * m + 2 * j + e) * old + t * 16 + 2 * quad) =
+              make_float2(o[t][m][e] * ref, o[t][m][e + 2] * ref);
     }
   }
   // ---- merge of the warps: their weights, and the sums of the weights --------------------------------------------------------
@@ -870,10 +900,10 @@ __global__ void __launch_bounds__(QD_WARPS * 32, 2)
     float m = splits > 1 ? -INFINITY : sink;
 #pragma unroll
     for (int w = 0; w < QD_WARPS; ++w) m = fmaxf(m, sm[w][r]);
-    float ll = splits > 1 || sink == -INFINITY ? 0.f : exp2f(sink - m);
+    float ll = splits > 1 || sink == -INFINITY ? 0.f : xl_tc::fast_exp2(sink - m);
 #pragma unroll
     for (int w = 0; w < QD_WARPS; ++w) {
-      const float f = sm[w][r] == -INFINITY ? 0.f : exp2f(sm[w][r] - m);
+      const float f = sm[w][r] == -INFINITY ? 0.f : xl_tc::fast_exp2(sm[w][r] - m);
       fw[w][r] = f;
       ll += sm[w][r] == -INFINITY ? 0.f : sl[w][r] * f;
     }
@@ -913,10 +943,10 @@ __global__ void __launch_bounds__(QD_WARPS * 32, 2)
     if (threadIdx.x < ROWS) {
       float m = sink;
       for (int k = 0; k < splits; ++k) m = fmaxf(m, wt[k * ROWS + threadIdx.x]);
-      float ll = sink == -INFINITY ? 0.f : exp2f(sink - m);
+      float ll = sink == -INFINITY ? 0.f : xl_tc::fast_exp2(sink - m);
       for (int k = 0; k < splits; ++k) {
         float& w = wt[k * ROWS + threadIdx.x];
-        w = w == -INFINITY ? 0.f : exp2f(w - m);
+        w = w == -INFINITY ? 0.f : xl_tc::fast_exp2(w - m);
         ll += w * wl[k * ROWS + threadIdx.x];
       }
       fl[threadIdx.x] = ll;
@@ -974,12 +1004,12 @@ int q8_make_map(CUtensorMap* map, const void* ptr, long long rows, int cols, int
   return r == CUDA_SUCCESS ? 0 : -3;
 }
 
-constexpr int QD_RING_LIMIT = 100 * 1024;  // two CTAs per SM
+constexpr int q8_ring_limit(int rt) { return (rt == 1 ? 65 : 100) * 1024; }  // three CTAs per SM, two
 
 template <int DK, int DV, int RT, bool FUSED> int q8_few_launch(Q8FewParams p, int B, int splits, cudaStream_t s) {
   constexpr int STAGE = q8_stage_bytes<DK, DV>() * QD_WARPS;
-  p.stages = 4 * STAGE <= QD_RING_LIMIT ? 4 : 3;
-  static_assert(3 * STAGE <= QD_RING_LIMIT, "ring");
+  p.stages = 4 * STAGE <= q8_ring_limit(RT) ? 4 : (3 * STAGE <= q8_ring_limit(RT) ? 3 : 2);
+  static_assert(2 * STAGE <= q8_ring_limit(RT), "ring");
   constexpr int merge = QD_WARPS * 8 * RT * (DV + 8) * 4;
   const int ring = p.stages * STAGE, bytes = (ring > merge ? ring : merge) + 1024;
   CUtensorMap mk, mv;

@@ -5,8 +5,8 @@ import torch
 
 from ..xl import read_ahead
 from ..xl.opdef import native
-from .native import _CODE, _c_f, _c_int, _c_ll, _c_p, _check, _count, _ok, _sig, _stream, counters, gemm_error_flag
-from .native_sequence import _clamped_glu, _decode_slices, _f32, _i32, _ptr, stream_rms
+from .native import _CODE, _c_f, _c_int, _c_ll, _c_p, _check, _count, _ok, _sig, _sms, _stream, counters, gemm_error_flag
+from .native_sequence import _clamped_glu, _f32, _i32, _ptr, stream_rms
 
 _c_d = ctypes.c_double
 _shape_logits = _sig("xl_shape_logits", *[_c_p] * 10, *[_c_int] * 7, _c_p)
@@ -85,6 +85,14 @@ def append_tokens_cuda(history, tokens, pos, count, T):
     return history if _launched(rc, "append_tokens") else NotImplemented
 
 
+def _q8_slices(units, longest, per_sm, device) -> int:
+    """Into how many CTAs the keys of one unit (sequence, key head, chunk of rows) are cut, at up to `longest` keys."""
+    most = per_sm * _sms(device) // units
+    if longest <= 320 or most < 2:
+        return 1
+    return min(most, (longest + 127) // 128, 64)
+
+
 @native("window_attention_q8_")
 def window_attention_q8_cuda(proj, q_norm, k_norm, k, v, k_scale, v_scale, k_tail, v_tail, pos, count, joint, T, heads, window,
                              keep_first, scale, sink, eps):
@@ -110,7 +118,7 @@ def window_attention_q8_cuda(proj, q_norm, k_norm, k, v, k_scale, v_scale, k_tai
         if units > 1 << 16:
             return False
         longest = min(blocks * 64, window + keep_first + T) if window else blocks * 64
-        splits = _decode_slices(units, longest, 320, dev)
+        splits = _q8_slices(units, longest, 3 if per == 8 else 2, dev)
         done = counters(units, dev, "counters sequence", 1 << 16)
         part = torch.empty(units * splits * per * (vdim + 2), dtype=torch.float32, device=dev) if splits > 1 else None
         rc = _q8_few(proj.data_ptr(), ld, q_norm.data_ptr(), k_norm.data_ptr(), _ptr(q), _ptr(raw[0]), _ptr(raw[1]), *cache, k_tail.data_ptr(),
