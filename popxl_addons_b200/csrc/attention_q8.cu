@@ -172,12 +172,12 @@ __global__ void __launch_bounds__(256) q8_append_kernel(const Q8AppendParams p) 
     for (int kind = 0; kind < 2; ++kind) {
       const T* src = raw[kind] + (long long)r0 * width[kind];
       int8_t* dst = (kind ? p.vc : p.kc) + at * Q8_BLOCK * width[kind];
-      const float scale = scales[kind];
+      const Q8Step step(scales[kind]);
       for (int i = threadIdx.x * V; i < Q8_BLOCK * width[kind]; i += 256 * V) {
         const Q8Piece<T, V> piece = *reinterpret_cast<const Q8Piece<T, V>*>(src + i);
         Q8Piece<int8_t, V> code;
 #pragma unroll
-        for (int e = 0; e < V; ++e) code.v[e] = (int8_t)q8_code(xl_to_float(piece.v[e]), scale);
+        for (int e = 0; e < V; ++e) code.v[e] = (int8_t)step.code(xl_to_float(piece.v[e]));
         *reinterpret_cast<Q8Piece<int8_t, V>*>(dst + i) = code;
       }
     }
@@ -351,6 +351,7 @@ __global__ void __launch_bounds__(SPLIT == 1 ? 128 : SPLIT * 32) q8_attn_general
 constexpr int QD_WARPS = 4;
 constexpr int QD_KEYS = 32, QD_RAW = 16;
 constexpr int QD_MAX_SPLITS = 64;
+constexpr int QD_TABLE = 128;  // items of a CTA whose scales wait in shared memory; those of more are read when they are needed
 enum { ERR_Q8_CODES = 91 };
 
 struct Q8FewParams {
@@ -366,7 +367,7 @@ struct Q8FewParams {
   const int *pos, *count;
   int T, H, G, dim, vdim, blocks, window, keep_first, gated;
   float scale, sink;
-  double eps;
+  double eps, inv_dim;
   float* part;             // [B * G * chunks][splits][rows per CTA][vdim], then the same with [2]: maximum, sum
   unsigned int* counters;  // [B * G * chunks], zero between launches
   int stages, read_ahead;
@@ -415,7 +416,8 @@ __global__ void __launch_bounds__(QD_WARPS * 32, RT == 1 ? 3 : 2)
   __shared__ __align__(16) __half sq[ROWS][DK];
   __shared__ __align__(16) __nv_bfloat16 new_k[DK], new_v[DV];
   __shared__ uint64_t bars[QD_WARPS][4];
-  __shared__ float tops[2][QD_WARPS];
+  __shared__ float tops[3][QD_WARPS];  // value scales of the items; the block that the token completes
+  __shared__ float2 table[QD_TABLE];
   __shared__ float sm[QD_WARPS][ROWS], sl[QD_WARPS][ROWS], fw[QD_WARPS][ROWS], fl[ROWS];
   __shared__ float wt[QD_MAX_SPLITS * ROWS], wl[QD_MAX_SPLITS * ROWS];
   __shared__ unsigned int is_last;
@@ -480,84 +482,114 @@ __global__ void __launch_bounds__(QD_WARPS * 32, RT == 1 ? 3 : 2)
     }
   };
   for (int n = 0; n < p.stages; ++n) prefetch(n);
-  // the largest value scale of this warp's items: the unit of its output
-  float ref = 0.f;
-  for (int i = lane; i < n_code; i += 32) ref = fmaxf(ref, p.vs[head * p.blocks + first_key(it0 + warp + i * QD_WARPS) / Q8_BLOCK]);
-  ref = n_code ? fmaxf(xl_warp_max(ref), 1e-20f) : 1.f;
-  const float unit_q = q8_norm_unit(p.wq, p.dim, lane), unit_k = q8_norm_unit(p.wk, p.dim, lane);
+  // ---- scales of the items (read once, by all threads), factors of the norms, and the largest value scale: the unit of the output --
+  auto item_block = [&](int it) { return head * p.blocks + first_key(it) / Q8_BLOCK; };
+  const int tabled = min(it1 - it0, QD_TABLE);
+  float top_v = 0.f;
+  for (int i = threadIdx.x; i < it1 - it0; i += QD_WARPS * 32) {
+    const long long blk = item_block(it0 + i);
+    const float2 x = make_float2(p.ks[blk], p.vs[blk]);
+    if (i < QD_TABLE) table[i] = x;
+    top_v = fmaxf(top_v, x.y);
+  }
+  float2 wq[DK / 64], wk[DK / 64];
+  float top_q = 0.f, top_k = 0.f;
+#pragma unroll
+  for (int u = 0; u < DK / 64; ++u) {
+    const int e = 2 * lane + 64 * u;
+    const bool on = e < p.dim;
+    wq[u] = on ? *reinterpret_cast<const float2*>(p.wq + e) : make_float2(0.f, 0.f);
+    wk[u] = on ? *reinterpret_cast<const float2*>(p.wk + e) : make_float2(0.f, 0.f);
+    top_q = fmaxf(top_q, fmaxf(fabsf(wq[u].x), fabsf(wq[u].y)));
+    top_k = fmaxf(top_k, fmaxf(fabsf(wk[u].x), fabsf(wk[u].y)));
+  }
   if (p.read_ahead) xl_grid_dependency_wait();  // the new projections
   xl_grid_launch_dependents();
-  // ---- queries (fp16, in units) to shared memory; the new key and value -----------------------------------------------------
+  // ---- queries (fp16, in units) to shared memory; the new key and value (the last warp) --------------------------------------------
   const int plain = (p.H + p.G) * p.dim + p.G * p.vdim;
-  for (int r = warp; r < ROWS; r += QD_WARPS) {
-    const int at = chunk * ROWS + r, t = at / R, hh = at % R;
-    float x[DK / 32];
+  constexpr int Q_WARPS = FUSED ? QD_WARPS - 1 : QD_WARPS, MINE_Q = (ROWS + Q_WARPS - 1) / Q_WARPS;
+  float unit_q;
+  if (!FUSED || warp < Q_WARPS) {
+    float2 x[MINE_Q][DK / 64];
+#pragma unroll
+    for (int i = 0; i < MINE_Q; ++i)
+#pragma unroll
+      for (int u = 0; u < DK / 64; ++u) {
+        const int r = warp + i * Q_WARPS, at = chunk * ROWS + r, e = 2 * lane + 64 * u;
+        x[i][u] = make_float2(0.f, 0.f);
+        if (r < nh && e < p.dim) {
+          if (FUSED) {
+            const uint32_t w = *reinterpret_cast<const uint32_t*>(p.proj + (long long)b * p.ld + (long long)(g * R + at) * p.dim + e);
+            x[i][u] = make_float2(dd_lo(w), dd_hi(w));
+          } else {
+            x[i][u] = *reinterpret_cast<const float2*>(p.q + ((head * p.T + at / R) * R + at % R) * p.dim + e);
+          }
+        }
+      }
+    unit_q = q8_norm_unit(top_q);
+    float f[MINE_Q];
+#pragma unroll
+    for (int i = 0; i < MINE_Q; ++i) {
+      f[i] = 0.f;
+#pragma unroll
+      for (int u = 0; u < DK / 64; ++u) f[i] += x[i][u].x * x[i][u].x + x[i][u].y * x[i][u].y;
+    }
     if (FUSED) {
-      const __nv_bfloat16* src = p.proj + (long long)b * p.ld + (long long)(g * R + hh) * p.dim;
-      float sum = 0.f;
 #pragma unroll
-      for (int u = 0; u < DK / 64; ++u) {
-        const int e = 2 * lane + 64 * u;
-        const uint32_t w = r < nh && e < p.dim ? *reinterpret_cast<const uint32_t*>(src + e) : 0u;
-        x[2 * u] = dd_lo(w);
-        x[2 * u + 1] = dd_hi(w);
-        sum += x[2 * u] * x[2 * u] + x[2 * u + 1] * x[2 * u + 1];
-      }
-      const float f = 1.f / (sqrtf(xl_warp_sum(sum) / p.dim + (float)p.eps) * unit_q);
+      for (int d = 16; d > 0; d >>= 1)  // the rows' sums side by side
 #pragma unroll
-      for (int u = 0; u < DK / 64; ++u) {
-        const int e = 2 * lane + 64 * u;
-        const bool on = r < nh && e < p.dim;
-        x[2 * u] = on ? x[2 * u] * f * p.wq[e] : 0.f;
-        x[2 * u + 1] = on ? x[2 * u + 1] * f * p.wq[e + 1] : 0.f;
-      }
-    } else {
-      const float* src = p.q + ((head * p.T + t) * R + hh) * p.dim;
-#pragma unroll
-      for (int u = 0; u < DK / 64; ++u) {
-        const int e = 2 * lane + 64 * u;
-        const bool on = r < nh && e < p.dim;
-        x[2 * u] = on ? src[e] / unit_q : 0.f;
-        x[2 * u + 1] = on ? src[e + 1] / unit_q : 0.f;
-      }
+        for (int i = 0; i < MINE_Q; ++i) f[i] += __shfl_xor_sync(0xffffffffu, f[i], d);
     }
 #pragma unroll
-    for (int u = 0; u < DK / 64; ++u) *reinterpret_cast<uint32_t*>(&sq[r][2 * lane + 64 * u]) = q8_pack_f16(x[2 * u], x[2 * u + 1]);
+    for (int i = 0; i < MINE_Q; ++i) {
+      const int r = warp + i * Q_WARPS;
+      f[i] = FUSED ? 1.f / (sqrtf(f[i] / p.dim + (float)p.eps) * unit_q) : 1.f / unit_q;
+      if (r < ROWS) {
+#pragma unroll
+        for (int u = 0; u < DK / 64; ++u)
+          *reinterpret_cast<uint32_t*>(&sq[r][2 * lane + 64 * u]) =
+              FUSED ? q8_pack_f16(x[i][u].x * f[i] * wq[u].x, x[i][u].y * f[i] * wq[u].y) : q8_pack_f16(x[i][u].x * f[i], x[i][u].y * f[i]);
+      }
+    }
+  } else {
+    unit_q = q8_norm_unit(top_q);
+  }
+  const float unit_k = q8_norm_unit(top_k);
+  {
+    const float m = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top_v)));
+    if (lane == 0) tops[0][warp] = m;
   }
   const bool writes = FUSED && has_raw && chunk == 0, completes = writes && fill == Q8_BLOCK - 1;
   if (FUSED && has_raw && warp == QD_WARPS - 1) {
     const __nv_bfloat16* src = p.proj + (long long)b * p.ld + (long long)(p.H + g) * p.dim;
     const __nv_bfloat16* vsrc = p.proj + (long long)b * p.ld + (long long)(p.H + p.G) * p.dim + (long long)g * p.vdim;
-    float x[DK / 32];
+    uint32_t w[DK / 64], vw[DV / 64];
     double sum = 0.0;
 #pragma unroll
-    for (int u = 0; u < DK / 64; ++u) {
-      const int e = 2 * lane + 64 * u;
-      const uint32_t w = e < p.dim ? *reinterpret_cast<const uint32_t*>(src + e) : 0u;
-      x[2 * u] = dd_lo(w);
-      x[2 * u + 1] = dd_hi(w);
-      sum += (double)x[2 * u] * x[2 * u] + (double)x[2 * u + 1] * x[2 * u + 1];
-    }
+    for (int u = 0; u < DK / 64; ++u) w[u] = 2 * lane + 64 * u < p.dim ? *reinterpret_cast<const uint32_t*>(src + 2 * lane + 64 * u) : 0u;
+#pragma unroll
+    for (int u = 0; u < DV / 64; ++u) vw[u] = 2 * lane + 64 * u < p.vdim ? *reinterpret_cast<const uint32_t*>(vsrc + 2 * lane + 64 * u) : 0u;
+#pragma unroll
+    for (int u = 0; u < DK / 64; ++u) sum += (double)dd_lo(w[u]) * dd_lo(w[u]) + (double)dd_hi(w[u]) * dd_hi(w[u]);
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    const double f = 1.0 / sqrt(sum / p.dim + p.eps);
+    const double f = rsqrt(sum * p.inv_dim + p.eps);
 #pragma unroll
     for (int u = 0; u < DK / 64; ++u) {
       const int e = 2 * lane + 64 * u;
-      const bool on = e < p.dim;
-      const uint32_t w = on ? dd_pack((float)((double)x[2 * u] * f * (double)p.wk[e]), (float)((double)x[2 * u + 1] * f * (double)p.wk[e + 1])) : 0u;
-      *reinterpret_cast<uint32_t*>(new_k + e) = w;
-      if (on && writes && !completes) *reinterpret_cast<uint32_t*>(p.kt + (head * Q8_BLOCK + fill) * p.dim + e) = w;
+      const uint32_t y = dd_pack((float)(dd_lo(w[u]) * f * (double)wk[u].x), (float)(dd_hi(w[u]) * f * (double)wk[u].y));
+      *reinterpret_cast<uint32_t*>(new_k + e) = y;
+      if (e < p.dim && writes && !completes) *reinterpret_cast<uint32_t*>(p.kt + (head * Q8_BLOCK + fill) * p.dim + e) = y;
     }
 #pragma unroll
     for (int u = 0; u < DV / 64; ++u) {
       const int e = 2 * lane + 64 * u;
-      const uint32_t w = e < p.vdim ? *reinterpret_cast<const uint32_t*>(vsrc + e) : 0u;
-      *reinterpret_cast<uint32_t*>(new_v + e) = w;
-      if (e < p.vdim && writes && !completes) *reinterpret_cast<uint32_t*>(p.vt + (head * Q8_BLOCK + fill) * p.vdim + e) = w;
+      *reinterpret_cast<uint32_t*>(new_v + e) = vw[u];
+      if (e < p.vdim && writes && !completes) *reinterpret_cast<uint32_t*>(p.vt + (head * Q8_BLOCK + fill) * p.vdim + e) = vw[u];
     }
   }
   __syncthreads();
+  const float ref = it1 > it0 ? fmaxf(fmaxf(fmaxf(tops[0][0], tops[0][1]), fmaxf(tops[0][2], tops[0][3])), 1e-20f) : 1.f;
   uint32_t q[RT][KG][8];  // rows quad + 8 m, features 64 i + 16 j .. + 15
 #pragma unroll
   for (int m = 0; m < RT; ++m)
@@ -593,7 +625,7 @@ __global__ void __launch_bounds__(QD_WARPS * 32, RT == 1 ? 3 : 2)
       mx[m][e] = -INFINITY;
       l[m][e] = 0.f;
     }
-  const float c_unit = p.scale * 1.4426950408889634f * unit_q;
+  const float c_unit = p.scale * 1.4426950408889634f * unit_q, inv_ref = 1.f / ref;
   // scores of NT tiles of 16 keys (keys 16 t + quad + 8 (e >> 1)) -> weights (in place); rescales the output where a maximum moved
   auto softmax = [&](auto& s) {
     constexpr int NT = sizeof(s) / sizeof(s[0]);
@@ -658,35 +690,36 @@ __global__ void __launch_bounds__(QD_WARPS * 32, RT == 1 ? 3 : 2)
 #pragma unroll
       for (int kind = 0; kind < 2; ++kind) {
         const float m = xl_warp_max(top[kind]);
-        if (lane == 0) tops[kind][warp] = m;
+        if (lane == 0) tops[1 + kind][warp] = m;
       }
       __syncthreads();
       const long long blk = head * p.blocks + pos / Q8_BLOCK;
       float scale[2];
 #pragma unroll
       for (int kind = 0; kind < 2; ++kind) {
-        float m = tops[kind][0];
-        for (int w = 1; w < QD_WARPS; ++w) m = fmaxf(m, tops[kind][w]);
+        float m = tops[1 + kind][0];
+        for (int w = 1; w < QD_WARPS; ++w) m = fmaxf(m, tops[1 + kind][w]);
         scale[kind] = __fdiv_rn(m, 127.f);
         if (threadIdx.x == 0) (kind ? p.vs : p.ks)[blk] = scale[kind];
       }
-      auto write = [&](const uint4& w, int8_t* dst, float step) {
+      const Q8Step step_k(scale[0]), step_v(scale[1]);
+      auto write = [&](const uint4& w, int8_t* dst, const Q8Step& step) {
         const uint32_t u[4] = {w.x, w.y, w.z, w.w};
         uint32_t c[2] = {0u, 0u};
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          c[e >> 2] |= (uint32_t)(q8_code(e & 1 ? dd_hi(u[e >> 1]) : dd_lo(u[e >> 1]), step) & 0xff) << (8 * (e & 3));
+          c[e >> 2] |= (uint32_t)(step.code(e & 1 ? dd_hi(u[e >> 1]) : dd_lo(u[e >> 1])) & 0xff) << (8 * (e & 3));
         *reinterpret_cast<uint2*>(dst) = make_uint2(c[0], c[1]);
       };
       for (int i = lane; i < QD_RAW * (DK / 8); i += 32) {
         const int r = i / (DK / 8), c = i % (DK / 8);
         if (c * 8 < p.dim)
-          write(*reinterpret_cast<const uint4*>(st + r * (DK * 2) + ((c ^ (r & 7)) * 16)), p.kc + (blk * Q8_BLOCK + r0 + r) * p.dim + c * 8, scale[0]);
+          write(*reinterpret_cast<const uint4*>(st + r * (DK * 2) + ((c ^ (r & 7)) * 16)), p.kc + (blk * Q8_BLOCK + r0 + r) * p.dim + c * 8, step_k);
       }
       for (int i = lane; i < QD_RAW * (DV / 8); i += 32) {
         const int r = i / (DV / 8), c = i % (DV / 8);
         if (c * 8 < p.vdim)
-          write(*reinterpret_cast<const uint4*>(sv + r * (DV * 2) + ((c ^ (r & 6)) * 16)), p.vc + (blk * Q8_BLOCK + r0 + r) * p.vdim + c * 8, scale[1]);
+          write(*reinterpret_cast<const uint4*>(sv + r * (DV * 2) + ((c ^ (r & 6)) * 16)), p.vc + (blk * Q8_BLOCK + r0 + r) * p.vdim + c * 8, step_v);
       }
     }
     float s[1][RT][4];
@@ -720,7 +753,6 @@ __global__ void __launch_bounds__(QD_WARPS * 32, RT == 1 ? 3 : 2)
       for (int e = 0; e < 4; ++e) s[0][m][e] = sees(qpos[m][e & 1], key0 + quad + 8 * (e >> 1), true) ? s[0][m][e] * c : -INFINITY;
     softmax(s);
     uint32_t ph[RT][2], pl[RT][2];  // weights in units of `ref` as operands of the second product, and their rounding errors
-    const float inv_ref = 1.f / ref;
 #pragma unroll
     for (int m = 0; m < RT; ++m)
 #pragma unroll
@@ -758,15 +790,12 @@ __global__ void __launch_bounds__(QD_WARPS * 32, RT == 1 ? 3 : 2)
     prefetch(n + p.stages);
   }
   // ---- codes -----------------------------------------------------------------------------------------------------------------
-  float my_ks = 0.f, my_vs = 0.f;  // scales of the next 32 items, one per lane
   for (int i = 0; i < n_code; ++i) {
     const int n = n_raw + i, slot = n % p.stages, key0 = first_key(it0 + warp + i * QD_WARPS);
-    if ((i & 31) == 0 && i + lane < n_code) {
-      const long long blk = head * p.blocks + first_key(it0 + warp + (i + lane) * QD_WARPS) / Q8_BLOCK;
-      my_ks = p.ks[blk];
-      my_vs = p.vs[blk];
-    }
-    const float c = c_unit * __shfl_sync(0xffffffffu, my_ks, i & 31), rel = __shfl_sync(0xffffffffu, my_vs, i & 31) / ref;
+    const int it = warp + i * QD_WARPS;
+    float2 scale = it < tabled ? table[it] : make_float2(0.f, 0.f);
+    if (it >= tabled) scale = make_float2(p.ks[item_block(it0 + it)], p.vs[item_block(it0 + it)]);
+    const float c = c_unit * scale.x, rel = scale.y * inv_ref;
     ok = mbar_wait_warp(&bars[warp][slot], (uint32_t)(i / p.stages) & 1u, &abort_flag, p.err, ERR_Q8_CODES);
     if (!ok) {
       given_up = i;
@@ -1097,7 +1126,7 @@ XL_API int xl_q8_attn_few(const void* proj, long long ld, const float* wq, const
   p.raw_v = (const __nv_bfloat16*)raw_v; p.kc = (int8_t*)kc; p.vc = (int8_t*)vc; p.ks = ks; p.vs = vs; p.kt = (__nv_bfloat16*)kt;
   p.vt = (__nv_bfloat16*)vt; p.out = (__nv_bfloat16*)out; p.ldo = ldo; p.pos = pos; p.count = count; p.T = T; p.H = H; p.G = G;
   p.dim = dim; p.vdim = vdim; p.blocks = blocks; p.window = window; p.keep_first = keep_first; p.gated = gated; p.scale = scale;
-  p.sink = sink; p.eps = eps; p.part = part; p.counters = counters; p.read_ahead = read_ahead; p.err = err;
+  p.sink = sink; p.eps = eps; p.inv_dim = 1.0 / dim; p.part = part; p.counters = counters; p.read_ahead = read_ahead; p.err = err;
   if (dim <= 64) return vdim <= 64 ? q8_few_sizes<64, 64>(p, B, splits, s) : q8_few_sizes<64, 128>(p, B, splits, s);
   return vdim <= 64 ? q8_few_sizes<128, 64>(p, B, splits, s) : q8_few_sizes<128, 128>(p, B, splits, s);
 }

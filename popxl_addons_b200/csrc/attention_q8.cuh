@@ -11,14 +11,27 @@
 
 constexpr int Q8_BLOCK = 64;
 
-// exponent e with 2^e above every factor, so that normalised rows divided by 2^e are at most sqrt(features) and fit 16-bit floats
+// A power of two above every factor of a norm: normalised rows divided by it are at most sqrt(features) and fit 16-bit floats. `top`: the
+// largest absolute factor that the lane has seen; the result is that of the warp.
+__device__ __forceinline__ float q8_norm_unit(float top) {
+  const uint32_t e = __reduce_max_sync(0xffffffffu, __float_as_uint(top)) >> 23;  // floats above zero are ordered like their bits
+  return e > 0 && e < 250 ? __uint_as_float((e + 1) << 23) : 1.f;
+}
 __device__ __forceinline__ float q8_norm_unit(const float* w, int dim, int lane) {
   float top = 0.f;
   for (int d = lane; d < dim; d += 32) top = fmaxf(top, fabsf(w[d]));
-  top = xl_warp_max(top);
-  return top > 0.f && top < 1e30f ? exp2f((float)(ilogbf(top) + 1)) : 1.f;
+  return q8_norm_unit(top);
 }
 
-__device__ __forceinline__ int q8_code(float x, float scale) {
-  return scale > 0.f ? max(-127, min(127, __float2int_rn(__fdiv_rn(x, scale)))) : 0;
-}
+// Codes of a block: x / scale rounded to the nearest whole number. A product with the reciprocal is off by less than 2^-15 there, so
+// only next to the middle between two codes does it take the division to know (which costs 20 times as much).
+struct Q8Step {
+  float scale, inv;
+  __device__ __forceinline__ explicit Q8Step(float s) : scale(s), inv(s > 1e-30f ? 1.f / s : 0.f) {}
+  __device__ __forceinline__ int code(float x) const {
+    const float y = x * inv;
+    float r = rintf(y);
+    if (fabsf(y - r) > 0.4999f || (inv == 0.f && scale > 0.f)) r = rintf(__fdiv_rn(x, scale));
+    return max(-127, min(127, __float2int_rn(r)));
+  }
+};
