@@ -175,9 +175,14 @@ __global__ void __launch_bounds__(256) q8_append_kernel(const Q8AppendParams p) 
       const Q8Step step(scales[kind]);
       for (int i = threadIdx.x * V; i < Q8_BLOCK * width[kind]; i += 256 * V) {
         const Q8Piece<T, V> piece = *reinterpret_cast<const Q8Piece<T, V>*>(src + i);
+        float x[V];
+        uint32_t word[1];
+#pragma unroll
+        for (int e = 0; e < V; ++e) x[e] = xl_to_float(piece.v[e]);
+        step.codes(x, word);
         Q8Piece<int8_t, V> code;
 #pragma unroll
-        for (int e = 0; e < V; ++e) code.v[e] = (int8_t)step.code(xl_to_float(piece.v[e]));
+        for (int e = 0; e < V; ++e) code.v[e] = (int8_t)(word[0] >> (8 * e));
         *reinterpret_cast<Q8Piece<int8_t, V>*>(dst + i) = code;
       }
     }
@@ -370,7 +375,7 @@ struct Q8FewParams {
   double eps, inv_dim;
   float* part;             // [B * G * chunks][splits][rows per CTA][vdim], then the same with [2]: maximum, sum
   unsigned int* counters;  // [B * G * chunks], zero between launches
-  int stages, read_ahead;
+  int stages, read_ahead, R, chunks;
   int* err;
 };
 
@@ -423,8 +428,8 @@ __global__ void __launch_bounds__(QD_WARPS * 32, RT == 1 ? 3 : 2)
   __shared__ unsigned int is_last;
   __shared__ volatile int abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = lane >> 2, j = lane & 3;
-  const int R = p.H / p.G, chunks = (p.T * R + ROWS - 1) / ROWS;
-  const int split = blockIdx.x, splits = gridDim.x, g = blockIdx.y / chunks, chunk = blockIdx.y % chunks, b = blockIdx.z;
+  const int R = p.R, chunks = p.chunks;
+  const int split = blockIdx.x, splits = gridDim.x, g = chunks == 1 ? blockIdx.y : blockIdx.y / chunks, chunk = blockIdx.y - g * chunks, b = blockIdx.z;
   if (threadIdx.x == 0) {
     for (int w = 0; w < QD_WARPS; ++w)
       for (int i = 0; i < 4; ++i) mbar_init(&bars[w][i], 1);
@@ -438,7 +443,7 @@ __global__ void __launch_bounds__(QD_WARPS * 32, RT == 1 ? 3 : 2)
     xl_grid_dependency_wait();  // no kernel of a chain ends before its predecessor
     return;
   }
-  const int p_lo = pos + chunk * ROWS / R, p_hi = pos + (chunk * ROWS + nh - 1) / R;
+  const int p_lo = FUSED ? pos : pos + chunk * ROWS / R, p_hi = FUSED ? pos : pos + (chunk * ROWS + nh - 1) / R;
   const int base = pos / Q8_BLOCK * Q8_BLOCK, own_lo = p_lo / Q8_BLOCK * Q8_BLOCK, own_hi = p_hi / Q8_BLOCK * Q8_BLOCK;
   const long long head = (long long)b * p.G + g;
   // ---- this CTA's items -----------------------------------------------------------------------------------------------------
@@ -446,8 +451,9 @@ __global__ void __launch_bounds__(QD_WARPS * 32, RT == 1 ? 3 : 2)
   const int kept = min(min(p.keep_first, w0), own_hi), kept_items = (kept + QD_KEYS - 1) / QD_KEYS;
   const int items = kept_items + max(0, own_hi - w0) / QD_KEYS;
   const int raw0 = own_lo - base, raw_end = p_hi - base + 1, raw_tiles = (raw_end - raw0 + QD_RAW - 1) / QD_RAW;
-  const long long all = (long long)items + raw_tiles;
-  const int it0 = min(items, (int)(split * all / splits)), it1 = min(items, (int)((split + 1) * all / splits));
+  const unsigned all = items + raw_tiles;  // at most 2^25 items, 2^6 splits
+  const int it0 = splits == 1 ? 0 : min(items, (int)(split * all / splits));
+  const int it1 = splits == 1 ? items : min(items, (int)((split + 1) * all / splits));
   const bool has_raw = split == splits - 1;
   auto first_key = [&](int it) { return it < kept_items ? it * QD_KEYS : w0 + (it - kept_items) * QD_KEYS; };
   const int n_raw = has_raw ? max(0, (raw_tiles - warp + QD_WARPS - 1) / QD_WARPS) : 0;
@@ -481,7 +487,7 @@ __global__ void __launch_bounds__(QD_WARPS * 32, RT == 1 ? 3 : 2)
       tma_load_2d(st + QD_KEYS * DK, &map_v, &bars[warp][slot], 0, row);
     }
   };
-  for (int n = 0; n < p.stages; ++n) prefetch(n);
+  for (int n = p.stages - 1; n >= 0; --n) prefetch(n);  // codes come from further away than the raw rows
   // ---- scales of the items (read once, by all threads), factors of the norms, and the largest value scale: the unit of the output --
   auto item_block = [&](int it) { return head * p.blocks + first_key(it) / Q8_BLOCK; };
   const int tabled = min(it1 - it0, QD_TABLE);
@@ -704,13 +710,12 @@ __global__ void __launch_bounds__(QD_WARPS * 32, RT == 1 ? 3 : 2)
       }
       const Q8Step step_k(scale[0]), step_v(scale[1]);
       auto write = [&](const uint4& w, int8_t* dst, const Q8Step& step) {
-        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-        uint32_t c[2] = {0u, 0u};
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          c[e >> 2] |= (uint32_t)(step.code(e & 1 ? dd_hi(u[e >> 1]) : dd_lo(u[e >> 1])) & 0xff) << (8 * (e & 3));
+        const float x[8] = {dd_lo(w.x), dd_hi(w.x), dd_lo(w.y), dd_hi(w.y), dd_lo(w.z), dd_hi(w.z), dd_lo(w.w), dd_hi(w.w)};
+        uint32_t c[2];
+        step.codes(x, c);
         *reinterpret_cast<uint2*>(dst) = make_uint2(c[0], c[1]);
       };
+#pragma unroll
       for (int i = lane; i < QD_RAW * (DK / 8); i += 32) {
         const int r = i / (DK / 8), c = i % (DK / 8);
         if (c * 8 < p.dim)
@@ -893,7 +898,7 @@ __global__ void __launch_bounds__(QD_WARPS * 32, RT == 1 ? 3 : 2)
       const int r = warp + i * QD_WARPS, at = chunk * ROWS + r, c = (lane + 32 * u) * 4;
       gates[i][u] = make_uint2(0u, 0u);
       if (p.gated && r < nh && c < p.vdim)
-        gates[i][u] = *reinterpret_cast<const uint2*>(p.proj + ((long long)b * p.T + at / R) * p.ld + plain + (long long)(g * R + at % R) * p.vdim + c);
+        gates[i][u] = *reinterpret_cast<const uint2*>(p.proj + ((long long)b * p.T + (FUSED ? 0 : at / R)) * p.ld + plain + (long long)(g * R + (FUSED ? at : at % R)) * p.vdim + c);
     }
 #pragma unroll
   for (int m = 0; m < RT; ++m)
@@ -989,7 +994,7 @@ __global__ void __launch_bounds__(QD_WARPS * 32, RT == 1 ? 3 : 2)
     if (r >= nh) break;
     const int at = chunk * ROWS + r;
     const float sum = fl[r];
-    __nv_bfloat16* out = p.out + ((long long)b * p.T + at / R) * p.ldo + (long long)(g * R + at % R) * p.vdim;
+    __nv_bfloat16* out = p.out + ((long long)b * p.T + (FUSED ? 0 : at / R)) * p.ldo + (long long)(g * R + (FUSED ? at : at % R)) * p.vdim;
 #pragma unroll
     for (int u = 0; u < CH; ++u) {
       const int c = (lane + 32 * u) * 4;
@@ -1048,8 +1053,9 @@ template <int DK, int DV, int RT, bool FUSED> int q8_few_launch(Q8FewParams p, i
   if (r) return r;
   static XlPerDevice smem;
   XL_TRY(xl_allow_smem(q8_few_rows_kernel<DK, DV, RT, FUSED>, bytes, smem));
-  const int chunks = (p.T * (p.H / p.G) + 8 * RT - 1) / (8 * RT);
-  const cudaError_t e = xl_launch_overlapped(q8_few_rows_kernel<DK, DV, RT, FUSED>, dim3(splits, p.G * chunks, B), dim3(QD_WARPS * 32),
+  p.R = p.H / p.G;
+  p.chunks = (p.T * p.R + 8 * RT - 1) / (8 * RT);
+  const cudaError_t e = xl_launch_overlapped(q8_few_rows_kernel<DK, DV, RT, FUSED>, dim3(splits, p.G * p.chunks, B), dim3(QD_WARPS * 32),
                                              (size_t)bytes, s, mk, mv, p);
   return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
 }

@@ -86,11 +86,14 @@ def append_tokens_cuda(history, tokens, pos, count, T):
 
 
 def _q8_slices(units, longest, per_sm, device) -> int:
-    """Into how many CTAs the keys of one unit (sequence, key head, chunk of rows) are cut, at up to `longest` keys."""
+    """Into how many CTAs the keys of one unit (sequence, key head, chunk of rows) are cut, at up to `longest` keys: one wave of
+    `per_sm` CTAs per SM, three 32-key items for each of a CTA's four warps (32 heads on 8 of 128: one sequence of 8000 keys 22.7, 16.5 and
+    18.6 us in 8, 16 and 24 slices, 4 of 4000 17.6, 16.5 and 22.7 in 8, 12 and 16, 16 of 8000 65.7, 54.3 and 66.0 in 2, 3 and 4). Up to
+    640 keys the merge costs what it saves (160 units of 600 keys: 16.6 us in 1 and 2 slices, in a window of 256 14.5 and 14.5)."""
     most = per_sm * _sms(device) // units
-    if longest <= 320 or most < 2:
+    if longest <= 640 or most < 2:
         return 1
-    return min(most, (longest + 127) // 128, 64)
+    return min(most, (longest + 383) // 384, 64)
 
 
 @native("window_attention_q8_")
