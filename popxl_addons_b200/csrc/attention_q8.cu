@@ -4,6 +4,7 @@
 //
 //   xl_q8_append          queries to their buffer, keys and values to `raw`; complete blocks to codes, the rest to the tails
 //   xl_q8_attn_general    any sizes and types, scores and weights in fp32 on the CUDA cores: one warp per row and head
+//   xl_q8_append_expand   the same, laid out for the tensor cores (xl_q8_attn_tcgen05 in attention_window_tcgen05.cu)
 //   xl_q8_attn_few        few rows per sequence, bf16, on mma.sync; of a single token norms, append and codes in the same launch
 #include "attention_decode.cuh"
 #include "attention_q8.cuh"
@@ -194,6 +195,250 @@ __global__ void __launch_bounds__(256) q8_append_kernel(const Q8AppendParams p) 
       float x[NP][V];
       fresh(i & 1, last + (i >> 1) - fill, x);
       store(tail[i & 1] + (long long)(i >> 1) * width[i & 1], width[i & 1], x);
+    }
+  }
+}
+
+__device__ __forceinline__ uint32_t q8_pack_f16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// two codes of a word (selected bytes, biased by 128) -> fp16 pair
+template <int SEL> __device__ __forceinline__ uint32_t q8_pair(uint32_t biased) {
+  const uint32_t w = __byte_perm(biased, 0x64646464u, SEL);
+  uint32_t r;
+  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(w), "r"(0xe480e480u));  // - 1152
+  return r;
+}
+
+// ---- append for the tensor cores ----------------------------------------------------------------------------------------------
+// What attention_window_tcgen05.cu reads: queries and raw keys as fp16 in units of a power of two, raw values, and the codes of
+// complete blocks as fp16 keys and bf16 values. bf16 projections, dim and vdim multiples of 8 up to 128. Sixteen lanes share a row, 16 bytes
+// each; a CTA has the rows of one block of one key / value head, two rows of each half warp in flight. Value rows that a tile of 128 keys
+// may read beyond the last key are zeros: a weight of zero times what memory happened to hold could be NaN.
+struct Q8ExpandParams {
+  const __nv_bfloat16* proj;
+  long long ld;
+  const float *wq, *wk;
+  __half* q;                        // (B, G, T, H/G, dim)
+  __half* raw_k;                    // (B, G, raw_rows, dim)
+  __nv_bfloat16* raw_v;             // (B, G, raw_rows, vdim)
+  __half* kx;                       // (B, G, blocks * 64, dim)
+  __nv_bfloat16* vx;                // (B, G, blocks * 64, vdim)
+  int8_t *kc, *vc;
+  float *ks, *vs;
+  __nv_bfloat16 *kt, *vt;
+  const int *pos, *count;
+  int T, H, G, dim, vdim, blocks, raw_rows, window, keep_first;
+  double eps, inv_dim;
+};
+
+__device__ __forceinline__ void q8_unpack(const uint4& w, float (&x)[8]) {
+  x[0] = dd_lo(w.x); x[1] = dd_hi(w.x); x[2] = dd_lo(w.y); x[3] = dd_hi(w.y);
+  x[4] = dd_lo(w.z); x[5] = dd_hi(w.z); x[6] = dd_lo(w.w); x[7] = dd_hi(w.w);
+}
+__device__ __forceinline__ uint4 q8_halves(const float (&x)[8]) {
+  return make_uint4(q8_pack_f16(x[0], x[1]), q8_pack_f16(x[2], x[3]), q8_pack_f16(x[4], x[5]), q8_pack_f16(x[6], x[7]));
+}
+// eight codes as fp16, and as bf16 times the scale
+__device__ __forceinline__ uint4 q8_code_halves(const uint2& c) {
+  const uint32_t a = c.x ^ 0x80808080u, b = c.y ^ 0x80808080u;
+  return make_uint4(q8_pair<0x4140>(a), q8_pair<0x4342>(a), q8_pair<0x4140>(b), q8_pair<0x4342>(b));
+}
+__device__ __forceinline__ uint4 q8_code_values(const uint2& c, float scale) {
+  float x[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = (float)(int8_t)((e < 4 ? c.x : c.y) >> (8 * (e & 3))) * scale;
+  return make_uint4(dd_pack(x[0], x[1]), dd_pack(x[2], x[3]), dd_pack(x[4], x[5]), dd_pack(x[6], x[7]));
+}
+
+__global__ void __launch_bounds__(256, 3) q8_append_expand_kernel(const Q8ExpandParams p) {
+  constexpr int HALVES = 16;  // half warps
+  __shared__ __align__(16) uint4 tile[2][Q8_BLOCK][16];
+  __shared__ float tops[2][HALVES], scales[2];
+  xl_grid_dependency_wait();
+  xl_grid_launch_dependents();
+  const int blk = blockIdx.x, g = blockIdx.y, b = blockIdx.z, half = threadIdx.x >> 4, l = threadIdx.x & 15, lane = threadIdx.x & 31;
+  const int pos = p.pos[b], n = min(p.count[b], p.T), R = p.H / p.G;
+  if (n <= 0 || pos < 0 || (long long)pos + n > (long long)p.blocks * Q8_BLOCK) return;
+  const int fill = pos % Q8_BLOCK, end = fill + n, r0 = blk * Q8_BLOCK, r1 = min(r0 + Q8_BLOCK, end);
+  if (r0 >= end) return;
+  const long long head = (long long)b * p.G + g, at = head * p.blocks + pos / Q8_BLOCK + blk;
+  const __nv_bfloat16* proj = p.proj + (long long)b * p.T * p.ld;
+  const bool on_k = l * 8 < p.dim, on_v = l * 8 < p.vdim;
+  float wq[8], wk[8], top_q = 0.f, top_w = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    wq[e] = on_k ? p.wq[l * 8 + e] : 0.f;
+    wk[e] = on_k ? p.wk[l * 8 + e] : 0.f;
+    top_q = fmaxf(top_q, fabsf(wq[e]));
+    top_w = fmaxf(top_w, fabsf(wk[e]));
+  }
+  const float unit_q = q8_norm_unit(top_q), inv_k = 1.f / q8_norm_unit(top_w);
+  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+  auto key_of = [&](const uint4& w) {  // the normalised key, rounded to bf16; all lanes of the warp together
+    float x[8];
+    q8_unpack(w, x);
+    double sum = 0.0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum += (double)x[e] * x[e];
+#pragma unroll
+    for (int d = 8; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    const double f = rsqrt(sum * p.inv_dim + p.eps);
+    uint32_t y[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = dd_pack((float)((double)x[2 * e] * f * wk[2 * e]), (float)((double)x[2 * e + 1] * f * wk[2 * e + 1]));
+    return make_uint4(y[0], y[1], y[2], y[3]);
+  };
+  float top[2] = {0.f, 0.f};
+  auto largest = [&](const uint4& w, float& m) {
+    float x[8];
+    q8_unpack(w, x);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(x[e]));
+  };
+  auto put_key = [&](int r, const uint4& w) {
+    float x[8];
+    q8_unpack(w, x);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] *= inv_k;
+    tile[0][r - r0][l] = w;
+    largest(w, top[0]);
+    if (on_k) *reinterpret_cast<uint4*>(p.raw_k + (head * p.raw_rows + r) * p.dim + l * 8) = q8_halves(x);
+  };
+  auto put_value = [&](int r, const uint4& w) {
+    tile[1][r - r0][l] = w;
+    largest(w, top[1]);
+    if (on_v) *reinterpret_cast<uint4*>(p.raw_v + (head * p.raw_rows + r) * p.vdim + l * 8) = w;
+  };
+  // tokens that were there before
+  for (int r = r0 + half; r < min(r1, fill); r += HALVES) {
+    put_key(r, on_k ? *reinterpret_cast<const uint4*>(p.kt + (head * Q8_BLOCK + r) * p.dim + l * 8) : zero);
+    put_value(r, on_v ? *reinterpret_cast<const uint4*>(p.vt + (head * Q8_BLOCK + r) * p.vdim + l * 8) : zero);
+  }
+  // new tokens: whole warps go through the rows, for the sums' shuffles
+  const bool to_tail = end < Q8_BLOCK;
+  const int first = max(r0, fill);
+  for (int rr = first; rr < r1; rr += HALVES) {
+    const int r = rr + half, t = r - fill;
+    const bool on = r < r1;
+    const __nv_bfloat16* row = proj + (long long)(on ? t : 0) * p.ld;
+    uint4 w = on && on_k ? *reinterpret_cast<const uint4*>(row + (long long)(p.H + g) * p.dim + l * 8) : zero;
+    const uint4 v = on && on_v ? *reinterpret_cast<const uint4*>(row + (long long)(p.H + p.G) * p.dim + (long long)g * p.vdim + l * 8) : zero;
+    w = key_of(w);
+    if (on) {
+      put_key(r, w);
+      put_value(r, v);
+      if (to_tail && on_k) *reinterpret_cast<uint4*>(p.kt + (head * Q8_BLOCK + r) * p.dim + l * 8) = w;
+      if (to_tail && on_v) *reinterpret_cast<uint4*>(p.vt + (head * Q8_BLOCK + r) * p.vdim + l * 8) = v;
+    }
+  }
+  const int queries = (r1 - first) * R;  // consecutive in `q`, heads of a token side by side in a row of the projections
+  __half* q = p.q + (head * p.T + (first - fill)) * R * p.dim;
+#pragma unroll 2
+  for (int i0 = 0; i0 < queries; i0 += HALVES) {
+    const int i = i0 + half;
+    const bool on = i < queries && on_k;
+    const int t = i / R, hh = i - t * R;
+    const uint4 w = on ? *reinterpret_cast<const uint4*>(proj + (long long)(first - fill + t) * p.ld + (long long)(g * R + hh) * p.dim + l * 8) : zero;
+    float x[8], sum = 0.f;
+    q8_unpack(w, x);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum += x[e] * x[e];
+#pragma unroll
+    for (int d = 8; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    const float f = 1.f / (sqrtf(sum / p.dim + (float)p.eps) * unit_q);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] *= f * wq[e];
+    if (on) *reinterpret_cast<uint4*>(q + (long long)i * p.dim + l * 8) = q8_halves(x);
+  }
+  if (r1 == end) {  // the last rows: zeros behind them
+    for (int r = end + half; r < end + 128; r += HALVES)
+      if (on_v) *reinterpret_cast<uint4*>(p.raw_v + (head * p.raw_rows + r) * p.vdim + l * 8) = zero;
+    if (r1 < r0 + Q8_BLOCK)
+      for (int r = half; r < Q8_BLOCK; r += HALVES)
+        if (on_v) *reinterpret_cast<uint4*>(p.vx + (at * Q8_BLOCK + r) * p.vdim + l * 8) = zero;
+  }
+  if (r1 == r0 + Q8_BLOCK) {
+#pragma unroll
+    for (int kind = 0; kind < 2; ++kind) {
+      const float m = xl_warp_max(top[kind]);
+      if (lane == 0) tops[kind][threadIdx.x >> 5] = m;
+    }
+    __syncthreads();
+    if (threadIdx.x < 2) {
+      float m = 0.f;
+      for (int w = 0; w < 8; ++w) m = fmaxf(m, tops[threadIdx.x][w]);
+      scales[threadIdx.x] = __fdiv_rn(m, 127.f);
+      (threadIdx.x ? p.vs : p.ks)[at] = scales[threadIdx.x];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int kind = 0; kind < 2; ++kind) {
+      const Q8Step step(scales[kind]);
+      for (int r = half; r < Q8_BLOCK; r += HALVES) {
+        float x[8];
+        uint32_t c[2];
+        q8_unpack(tile[kind][r][l], x);
+        step.codes(x, c);
+        const uint2 word = make_uint2(c[0], c[1]);
+        const long long row = at * Q8_BLOCK + r;
+        if (kind == 0 && on_k) {
+          *reinterpret_cast<uint2*>(p.kc + row * p.dim + l * 8) = word;
+          *reinterpret_cast<uint4*>(p.kx + row * p.dim + l * 8) = q8_code_halves(word);
+        } else if (kind == 1 && on_v) {
+          *reinterpret_cast<uint2*>(p.vc + row * p.vdim + l * 8) = word;
+          *reinterpret_cast<uint4*>(p.vx + row * p.vdim + l * 8) = q8_code_values(word, step.scale);
+        }
+      }
+    }
+  }
+  if (blk == 0 && end >= Q8_BLOCK) {  // the tail is the start of a later block
+    __syncthreads();                  // its old rows have been read
+    const int last = end / Q8_BLOCK * Q8_BLOCK;
+    for (int rr = last; rr < end; rr += HALVES) {
+      const int r = rr + half, t = r - fill;
+      const bool on = r < end;
+      const __nv_bfloat16* row = proj + (long long)(on ? t : 0) * p.ld;
+      const uint4 w = key_of(on && on_k ? *reinterpret_cast<const uint4*>(row + (long long)(p.H + g) * p.dim + l * 8) : zero);
+      if (on && on_k) *reinterpret_cast<uint4*>(p.kt + (head * Q8_BLOCK + r - last) * p.dim + l * 8) = w;
+      if (on && on_v)
+        *reinterpret_cast<uint4*>(p.vt + (head * Q8_BLOCK + r - last) * p.vdim + l * 8) =
+            *reinterpret_cast<const uint4*>(row + (long long)(p.H + p.G) * p.dim + (long long)g * p.vdim + l * 8);
+    }
+  }
+}
+
+// Blocks that were complete before the portion and that its tiles read: those of the kept first tokens, whole tiles of them, and those
+// from the first window on. Grid (groups of blocks, G, B).
+constexpr int Q8_EXPAND_GROUP = 8;
+__global__ void __launch_bounds__(256) q8_expand_kernel(const Q8ExpandParams p) {
+  xl_grid_dependency_wait();
+  xl_grid_launch_dependents();
+  const int g = blockIdx.y, b = blockIdx.z, half = threadIdx.x >> 4, l = threadIdx.x & 15;
+  const int pos = p.pos[b], n = min(p.count[b], p.T);
+  if (n <= 0 || pos < 0 || (long long)pos + n > (long long)p.blocks * Q8_BLOCK) return;
+  const int done = pos / Q8_BLOCK, from = p.window ? max(0, pos - p.window + 1) / Q8_BLOCK : 0;
+  const int kept = (int)(((long long)p.keep_first + 127) / 128 * 2);
+  const long long head = (long long)b * p.G + g;
+  const bool on_k = l * 8 < p.dim, on_v = l * 8 < p.vdim;
+  for (int j = blockIdx.x * Q8_EXPAND_GROUP; j < min(done, (int)(blockIdx.x + 1) * Q8_EXPAND_GROUP); ++j) {
+    if (j < from && j >= kept) continue;
+    const long long at = head * p.blocks + j;
+    const float scale = p.vs[at];
+    uint2 k[4], v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const long long row = at * Q8_BLOCK + half + 16 * i;
+      if (on_k) k[i] = *reinterpret_cast<const uint2*>(p.kc + row * p.dim + l * 8);
+      if (on_v) v[i] = *reinterpret_cast<const uint2*>(p.vc + row * p.vdim + l * 8);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const long long row = at * Q8_BLOCK + half + 16 * i;
+      if (on_k) *reinterpret_cast<uint4*>(p.kx + row * p.dim + l * 8) = q8_code_halves(k[i]);
+      if (on_v) *reinterpret_cast<uint4*>(p.vx + row * p.vdim + l * 8) = q8_code_values(v[i], scale);
     }
   }
 }
@@ -395,19 +640,6 @@ __device__ __forceinline__ uint32_t q8_transpose(uint32_t x) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-__device__ __forceinline__ uint32_t q8_pack_f16(float lo, float hi) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-// two codes of a word (selected bytes, biased by 128) -> fp16 pair
-template <int SEL> __device__ __forceinline__ uint32_t q8_pair(uint32_t biased) {
-  const uint32_t w = __byte_perm(biased, 0x64646464u, SEL);
-  uint32_t r;
-  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(w), "r"(0xe480e480u));  // - 1152
-  return r;
-}
-
 template <int DK, int DV> __host__ __device__ constexpr int q8_stage_bytes() { return QD_KEYS * (DK + DV); }
 
 // DK, DV: 64 or 128, features of a key and of a value rounded up
@@ -1135,4 +1367,25 @@ XL_API int xl_q8_attn_few(const void* proj, long long ld, const float* wq, const
   p.sink = sink; p.eps = eps; p.inv_dim = 1.0 / dim; p.part = part; p.counters = counters; p.read_ahead = read_ahead; p.err = err;
   if (dim <= 64) return vdim <= 64 ? q8_few_sizes<64, 64>(p, B, splits, s) : q8_few_sizes<64, 128>(p, B, splits, s);
   return vdim <= 64 ? q8_few_sizes<128, 64>(p, B, splits, s) : q8_few_sizes<128, 128>(p, B, splits, s);
+}
+
+// The same as xl_q8_append for xl_q8_attn_tcgen05 (see there): q (B, G, T, H/G, dim) and raw_k (B, G, raw_rows, dim) fp16, raw_v (B, G,
+// raw_rows, vdim) bf16 with raw_rows >= T + 192, kx (B, G, blocks * 64, dim) fp16, vx (.., vdim) bf16: complete blocks that the portion
+// can see. bf16; dim, vdim multiples of 8 up to 128, ld a multiple of 8, all pointers 16-byte aligned.
+XL_API int xl_q8_append_expand(const void* proj, long long ld, const float* wq, const float* wk, void* q, void* raw_k, void* raw_v,
+                               int raw_rows, void* kx, void* vx, void* kc, void* vc, float* ks, float* vs, void* kt, void* vt,
+                               const int* pos, const int* count, int B, int T, int H, int G, int dim, int vdim, int blocks, int window,
+                               int keep_first, double eps, cudaStream_t s) {
+  if (!q8_sizes_ok(B, T, H, G, dim, vdim, blocks) || dim % 8 || vdim % 8 || dim > 128 || vdim > 128 || ld % 8 || !wq || !wk ||
+      ld < (long long)(H + G) * dim + (long long)G * vdim || raw_rows < T + Q8_BLOCK + 128 || window < 0 || keep_first < 0)
+    return -1;
+  const uintptr_t at = (uintptr_t)proj | (uintptr_t)q | (uintptr_t)raw_k | (uintptr_t)raw_v | (uintptr_t)kx | (uintptr_t)vx | (uintptr_t)kc |
+                       (uintptr_t)vc | (uintptr_t)kt | (uintptr_t)vt;
+  if (at & 15) return -1;
+  const Q8ExpandParams p{(const __nv_bfloat16*)proj, ld, wq, wk, (__half*)q, (__half*)raw_k, (__nv_bfloat16*)raw_v, (__half*)kx,
+                         (__nv_bfloat16*)vx, (int8_t*)kc, (int8_t*)vc, ks, vs, (__nv_bfloat16*)kt, (__nv_bfloat16*)vt, pos, count, T, H, G, dim,
+                         vdim, blocks, raw_rows, window, keep_first, eps, 1.0 / dim};
+  XL_TRY(xl_launch_overlapped(q8_append_expand_kernel, dim3((T + 2 * Q8_BLOCK - 2) / Q8_BLOCK, G, B), dim3(256), (size_t)0, s, p));
+  XL_TRY(xl_launch_overlapped(q8_expand_kernel, dim3((blocks + Q8_EXPAND_GROUP - 1) / Q8_EXPAND_GROUP, G, B), dim3(256), (size_t)0, s, p));
+  return (int)cudaGetLastError();
 }

@@ -16,6 +16,8 @@ _q8_append = _sig("xl_q8_append", _c_p, _c_ll, *[_c_p] * 13, *[_c_int] * 7, _c_d
 _q8_general = _sig("xl_q8_attn_general", *[_c_p] * 8, _c_ll, _c_p, _c_ll, _c_p, _c_p, *[_c_int] * 9, _c_f, _c_f, _c_int, _c_p)
 _q8_few = _sig("xl_q8_attn_few", _c_p, _c_ll, *[_c_p] * 12, _c_ll, _c_p, _c_p, *[_c_int] * 10, _c_f, _c_f, _c_d, _c_int, _c_p, _c_p, _c_int,
                _c_p, _c_p)
+_q8_append_expand = _sig("xl_q8_append_expand", _c_p, _c_ll, *[_c_p] * 5, _c_int, *[_c_p] * 10, *[_c_int] * 9, _c_d, _c_p)
+_q8_tcgen05 = _sig("xl_q8_attn_tcgen05", *[_c_p] * 5, _c_int, *[_c_p] * 4, _c_ll, _c_p, _c_ll, _c_p, _c_p, *[_c_int] * 9, _c_f, _c_f, _c_p, _c_p)
 
 
 def _launched(rc, name) -> bool:
@@ -25,6 +27,11 @@ def _launched(rc, name) -> bool:
     _check(rc, name)
     _count(name)
     return True
+
+
+def _done(rc, name):
+    _check(rc, name)
+    _count(name)
 
 
 @native("split_glu")
@@ -96,6 +103,33 @@ def _q8_slices(units, longest, per_sm, device) -> int:
     return min(most, (longest + 383) // 384, 64)
 
 
+_Q8_FEW_ROWS = 64       # rows per sequence and key head up to which portions run on mma.sync
+_Q8_EXPANDED = 2 << 30  # bytes that the codes of a portion may expand to at a time
+
+
+def _q8_portion(at, proj, q_norm, k_norm, cache, pos, count, joint, gate, T, heads, window, keep_first, scale, sink, eps, s):
+    """A portion of the sequences `at` on the tensor cores: append, codes of visible blocks as 16-bit numbers, attention."""
+    cache, pos, count = tuple(t[at] for t in cache), pos[at], count[at]
+    B, G, blocks, _, dim = cache[0].shape
+    vdim, dev, rows = cache[1].shape[-1], proj.device, T + 192
+    ld, ldo, row0 = proj.stride(0), joint.stride(0), at.start * T
+    q = torch.empty((B, G, T, heads // G, dim), dtype=torch.float16, device=dev)
+    raw_k = torch.empty((B, G, rows, dim), dtype=torch.float16, device=dev)
+    raw_v = torch.empty((B, G, rows, vdim), dtype=torch.bfloat16, device=dev)
+    kx = torch.empty((B, G, blocks * 64, dim), dtype=torch.float16, device=dev)
+    vx = torch.empty((B, G, blocks * 64, vdim), dtype=torch.bfloat16, device=dev)
+    sizes = (B, T, heads, G, dim, vdim, blocks, window, keep_first)
+    norms, where = (q_norm.data_ptr(), k_norm.data_ptr()), (pos.data_ptr(), count.data_ptr())
+    rc = _q8_append_expand(proj.data_ptr() + row0 * ld * 2, ld, *norms, q.data_ptr(), raw_k.data_ptr(), raw_v.data_ptr(), rows, kx.data_ptr(),
+                           vx.data_ptr(), *map(_ptr, cache), *where, *sizes, eps, s)
+    _done(rc, "q8_append_expand")
+    _count("q8_expand")
+    rc = _q8_tcgen05(q.data_ptr(), kx.data_ptr(), vx.data_ptr(), raw_k.data_ptr(), raw_v.data_ptr(), rows, cache[2].data_ptr(), *norms,
+                     gate + row0 * ld * 2 if gate else None, ld, joint.data_ptr() + row0 * ldo * 2, ldo, *where, *sizes, scale, sink,
+                     gemm_error_flag(dev).data_ptr(), s)
+    _done(rc, "q8_attn_tcgen05")
+
+
 @native("window_attention_q8_")
 def window_attention_q8_cuda(proj, q_norm, k_norm, k, v, k_scale, v_scale, k_tail, v_tail, pos, count, joint, T, heads, window,
                              keep_first, scale, sink, eps):
@@ -131,14 +165,24 @@ def window_attention_q8_cuda(proj, q_norm, k_norm, k, v, k_scale, v_scale, k_tai
 
     if T == 1 and dt == torch.bfloat16 and few(None, (None, None), read_ahead.allowed(pos, count, k, v, k_scale, v_scale, k_tail, v_tail)):
         return joint
+    if (dt == torch.bfloat16 and T * (heads // G) > _Q8_FEW_ROWS and dim <= 128 and vdim <= 128 and dim % 8 == vdim % 8 == ld % 8 == ldo % 8 == 0
+            and T * heads <= 1 << 22 and G * blocks * 64 * (dim + vdim) * 2 <= _Q8_EXPANDED):
+        # as many sequences at a time as expand to what is set aside for it
+        step = max(1, _Q8_EXPANDED // (G * blocks * 64 * (dim + vdim) * 2))
+        step = min(step, (1 << 30) // (G * (T + 192)) + 1, (1 << 30) // (T * heads) + 1)
+        for b in range(0, B, step):
+            _q8_portion(slice(b, min(B, b + step)), proj, q_norm, k_norm, (k, v, k_scale, v_scale, k_tail, v_tail), pos, count, joint, gate, T,
+                        heads, window, keep_first, scale, sink, eps, s)
+        return joint
     q = torch.empty((B, G, T, heads // G, dim), dtype=torch.float32, device=dev)
     raw = [torch.empty((B, G, T + 64, width), dtype=dt, device=dev) for width in (dim, vdim)]
     rc = _q8_append(proj.data_ptr(), ld, q_norm.data_ptr(), k_norm.data_ptr(), q.data_ptr(), raw[0].data_ptr(), raw[1].data_ptr(), *cache,
                     k_tail.data_ptr(), v_tail.data_ptr(), pos.data_ptr(), count.data_ptr(), B, T, heads, G, dim, vdim, blocks, eps, code, s)
     if not _launched(rc, "q8_append"):
         return NotImplemented
-    if dt == torch.bfloat16 and T * (heads // G) <= 64 and few(q, raw, False):
+    if dt == torch.bfloat16 and T * (heads // G) <= _Q8_FEW_ROWS and few(q, raw, False):
         return joint
     rc = _q8_general(q.data_ptr(), raw[0].data_ptr(), raw[1].data_ptr(), *cache, gate, ld, joint.data_ptr(), ldo, pos.data_ptr(),
                      count.data_ptr(), B, T, heads, G, dim, vdim, blocks, window, keep_first, scale, sink, code, s)
-    return joint if _launched(rc, "q8_attn_general") else NotImplemented
+    _done(rc, "q8_attn_general")  # the keys are in the cache: there is no other way from here
+    return joint
