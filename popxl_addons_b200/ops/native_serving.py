@@ -5,8 +5,8 @@ import torch
 
 from ..xl import read_ahead
 from ..xl.opdef import native
-from .native import _CODE, _c_f, _c_int, _c_ll, _c_p, _check, _count, _ok, _sig, _sms, _stream, counters, gemm_error_flag
-from .native_sequence import _clamped_glu, _f32, _i32, _ptr, stream_rms
+from .native import _CODE, _c_f, _c_int, _c_ll, _c_p, _check, _count, _ok, _sig, _sms, _stream, counters, gemm, gemm_error_flag, gemm_pays
+from .native_sequence import _clamped_glu, _f32, _i32, _ptr, _small, product, stream_rms
 
 _c_d = ctypes.c_double
 _shape_logits = _sig("xl_shape_logits", *[_c_p] * 10, *[_c_int] * 7, _c_p)
@@ -18,6 +18,10 @@ _q8_few = _sig("xl_q8_attn_few", _c_p, _c_ll, *[_c_p] * 12, _c_ll, _c_p, _c_p, *
                _c_p, _c_p)
 _q8_append_expand = _sig("xl_q8_append_expand", _c_p, _c_ll, *[_c_p] * 5, _c_int, *[_c_p] * 10, *[_c_int] * 9, _c_d, _c_p)
 _q8_tcgen05 = _sig("xl_q8_attn_tcgen05", *[_c_p] * 5, _c_int, *[_c_p] * 4, _c_ll, _c_p, _c_ll, _c_p, _c_p, *[_c_int] * 9, _c_f, _c_f, _c_p, _c_p)
+_adapter_down = _sig("xl_adapter_down", *[_c_p] * 5, _c_ll, *[_c_int] * 5, _c_p)
+_adapter_up = _sig("xl_adapter_up", *[_c_p] * 5, _c_ll, *[_c_int] * 6, _c_p)
+_adapter_down_mma = _sig("xl_adapter_down_mma", *[_c_p] * 5, _c_ll, *[_c_int] * 5, _c_p)
+_adapter_up_mma = _sig("xl_adapter_up_mma", *[_c_p] * 4, _c_ll, *[_c_int] * 5, _c_p)
 
 
 def _launched(rc, name) -> bool:
@@ -186,3 +190,34 @@ def window_attention_q8_cuda(proj, q_norm, k_norm, k, v, k_scale, v_scale, k_tai
                      count.data_ptr(), B, T, heads, G, dim, vdim, blocks, window, keep_first, scale, sink, code, s)
     _done(rc, "q8_attn_general")  # the keys are in the cache: there is no other way from here
     return joint
+
+
+@native("linear_adapted")
+def linear_adapted_cuda(x, weight, a, b, scale, slot, T, out_dtype):
+    dt, dev = x.dtype, x.device
+    (rows, K), N, (n, r, _) = x.shape, weight.shape[0], a.shape
+    if not (dt in _CODE and dt == weight.dtype == a.dtype == b.dtype and out_dtype in (dt, torch.float32)):
+        return NotImplemented
+    if not x.is_cuda or not _f32(scale) or not _i32(slot) or any(not t.is_contiguous() for t in (x, a, b, scale)) or slot.numel() * T != rows:
+        return NotImplemented
+    if r > 128:  # the kernels hold the numbers between the two products in shared memory
+        return NotImplemented
+    code, s = _CODE[dt], _stream()
+    low = torch.empty((rows, -(-r // 16) * 16), dtype=torch.float32, device=dev)
+    down = (x.data_ptr(), a.data_ptr(), scale.data_ptr(), slot.data_ptr(), low.data_ptr(), rows, T, K, n, r, code, s)
+    if not (T >= 8 and dt != torch.float32 and _launched(_adapter_down_mma(*down), "adapter_down_mma")):
+        if not _launched(_adapter_down(*down), "adapter_down"):
+            return NotImplemented
+    if dt != torch.float32 and out_dtype == dt and T >= 8 and not _small(x, weight):
+        out = torch.empty((rows, N), dtype=dt, device=dev)
+        if gemm_pays(x, weight.t(), out=out) and _launched(_adapter_up_mma(low.data_ptr(), b.data_ptr(), slot.data_ptr(), out.data_ptr(), rows, T,
+                                                                           N, n, r, code, s), "adapter_up_mma"):
+            if gemm(x, weight.t(), out=out, accumulate=1) is not NotImplemented:
+                return out
+    # 32-bit results also where the GEMM needs copies for them: the sum is rounded once
+    y = product(x, weight, torch.float32) if dt == torch.float32 or _small(x, weight) else gemm(x, weight.t(), out_dtype=torch.float32)
+    if y is NotImplemented:
+        return NotImplemented
+    out = y if out_dtype == torch.float32 else torch.empty((rows, N), dtype=out_dtype, device=dev)
+    rc = _adapter_up(low.data_ptr(), b.data_ptr(), slot.data_ptr(), y.data_ptr(), out.data_ptr(), rows, T, N, n, r, code, _CODE[out_dtype], s)
+    return out if _launched(rc, "adapter_up") else NotImplemented
