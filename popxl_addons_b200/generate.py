@@ -15,14 +15,21 @@ def main(argv=None) -> int:
     ap.add_argument("--batch", type=int, default=0, help="sequences run together (default: all prompts, at most 16)")
     ap.add_argument("--max-seq", type=int, default=0, help="positions a sequence can hold (default: what the prompts need)")
     ap.add_argument("--device", default="auto")
+    ap.add_argument("--cache", default="model", choices=("model", "int8"), help="how keys and values are held (int8: where the architecture offers it)")
+    ap.add_argument("--repetition-penalty", type=float, default=1.0)
+    ap.add_argument("--frequency-penalty", type=float, default=0.0)
+    ap.add_argument("--presence-penalty", type=float, default=0.0)
     a = ap.parse_args(argv)
     from .models.registry import load_model
+    from .models.sequence_generator import LogitShaping
 
     prompts = [[int(x) for x in p.replace(",", " ").split()] for p in a.prompt]
+    shaping = LogitShaping(a.repetition_penalty, a.frequency_penalty, a.presence_penalty)
     need = max(len(p) for p in prompts) + a.max_new_tokens
     gen = load_model(a.model, dtype=a.dtype, batch=a.batch or min(len(prompts), 16), max_seq=a.max_seq or need,
-                     max_new_tokens=a.max_new_tokens, device=a.device)
-    for out in gen.generate(prompts, a.max_new_tokens):
+                     max_new_tokens=a.max_new_tokens, device=a.device, shaping=shaping != LogitShaping(),
+                     model_options={} if a.cache == "model" else {"cache": a.cache})
+    for out in gen.generate(prompts, a.max_new_tokens, shaping if gen.shaping else None):
         print(" ".join(str(int(x)) for x in out))
     return 0
 

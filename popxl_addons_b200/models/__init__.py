@@ -4,12 +4,12 @@ a checkpoint folder by `SequenceGenerator`; the registry of architectures (`load
 from .decoder import DecoderBlock, DecoderConfig, DecoderEmbedding, DecoderHead
 
 __all__ = ["DecoderConfig", "DecoderBlock", "DecoderEmbedding", "DecoderHead", "DecoderTrainer", "PipelineTrainer",
-           "DecoderGenerator", "Dunelix", "DunelixConfig", "Zirunex", "ZirunexConfig", "SequenceGenerator", "load_model",
+           "DecoderGenerator", "Dunelix", "DunelixConfig", "Zirunex", "ZirunexConfig", "SequenceGenerator", "LogitShaping", "load_model",
            "load_config", "register_architecture", "ARCHITECTURES"]
 
 _LAZY = {"DecoderTrainer": "trainer", "PipelineTrainer": "pipeline_trainer", "DecoderGenerator": "generator",
          "Dunelix": "dunelix", "DunelixConfig": "dunelix", "Zirunex": "zirunex", "ZirunexConfig": "zirunex",
-         "SequenceGenerator": "sequence_generator", "load_model": "registry", "load_config": "registry",
+         "SequenceGenerator": "sequence_generator", "LogitShaping": "sequence_generator", "load_model": "registry", "load_config": "registry",
          "register_architecture": "registry", "ARCHITECTURES": "registry"}
 
 

@@ -13,7 +13,7 @@ __all__ = ["Architecture", "ARCHITECTURES", "register_architecture", "architectu
 class Architecture:
     name: str
     config: Callable[[Dict[str, Any]], Any]   # entries of config.json -> configuration object
-    model: Optional[Callable[..., Any]] = None  # (configuration, dtype) -> model description for SequenceGenerator
+    model: Optional[Callable[..., Any]] = None  # (configuration, dtype, **options) -> model description for SequenceGenerator
     dtypes: tuple = ("bfloat16", "float32")
 
 
@@ -45,8 +45,11 @@ def _served(name: str, module: str) -> Architecture:
     def config(d: Dict[str, Any]):
         return getattr(import_module(f"{__package__}.{module}"), f"{name}Config").from_dict(d)
 
-    def model(cfg, dtype: str = "bfloat16"):
-        return getattr(import_module(f"{__package__}.{module}"), name)(cfg, dtype)
+    def model(cfg, dtype: str = "bfloat16", **options):
+        cls = getattr(import_module(f"{__package__}.{module}"), name)
+        if set(options) - set(getattr(cls, "options", ())):
+            raise ValueError(f"{name} has no options {sorted(set(options) - set(getattr(cls, 'options', ())))}")
+        return cls(cfg, dtype, **options)
 
     return Architecture(name, config, model)
 
@@ -68,8 +71,9 @@ def load_config(folder: str):
     return arch, arch.config(d)
 
 
-def load_model(folder: str, dtype: str = "bfloat16", **generator_options):
-    """A `SequenceGenerator` with the folder's weights loaded."""
+def load_model(folder: str, dtype: str = "bfloat16", model_options: Optional[Dict[str, Any]] = None, **generator_options):
+    """A `SequenceGenerator` with the folder's weights loaded. `model_options`: what the architecture leaves to a deployment, such as
+    `{"cache": "int8"}`."""
     from ..utils.safetensors import read_safetensors
     from .sequence_generator import SequenceGenerator
 
@@ -78,5 +82,5 @@ def load_model(folder: str, dtype: str = "bfloat16", **generator_options):
         raise ValueError(f"architecture {arch.name!r} is not served from a checkpoint folder")
     if dtype not in arch.dtypes:
         raise ValueError(f"architecture {arch.name!r} runs in {arch.dtypes}, not in {dtype!r}")
-    gen = SequenceGenerator(arch.model(cfg, dtype), **generator_options)
+    gen = SequenceGenerator(arch.model(cfg, dtype, **(model_options or {})), **generator_options)
     return gen.load_checkpoint(read_safetensors(os.path.join(folder, "model.safetensors")))

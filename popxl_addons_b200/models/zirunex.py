@@ -11,7 +11,8 @@ Both sublayers read the same h and end in the same sum, so a layer is two produc
 `[o | down]` on the attention's and the feed-forward's results side by side.
 
 `Zirunex` describes the model to `SequenceGenerator`: which tensors it needs, how they are made from a checkpoint, what state
-a sequence has, and the ops of one portion of tokens.
+a sequence has, and the ops of one portion of tokens. Two of its properties belong to a deployment and not to a checkpoint: whether
+caches are held in the model's type or in 8 bits, and how many low-rank adapters stand beside the projections of every layer.
 """
 from dataclasses import dataclass
 from typing import Any, Callable, Dict, List, Mapping, Optional, Tuple
@@ -149,11 +150,19 @@ class Zirunex:
     """Weights, state and step of the model for `SequenceGenerator`."""
 
     config_class = ZirunexConfig
+    options = ("cache", "adapters", "adapter_rank")
 
-    def __init__(self, cfg: ZirunexConfig, dtype: str = "bfloat16"):
+    def __init__(self, cfg: ZirunexConfig, dtype: str = "bfloat16", cache: str = "model", adapters: int = 0, adapter_rank: int = 16):
+        """`cache`: "model" (keys and values in the model's type) or "int8" (codes of 8 bits with a scale per block of 64 tokens and
+        head). `adapters`: how many low-rank adapters the program holds, each of `adapter_rank` numbers per joint matrix of a layer."""
+        if cache not in ("model", "int8"):
+            raise ValueError(f"a cache is held as 'model' or 'int8', not {cache!r}")
+        if adapters < 0 or not 1 <= adapter_rank <= ops.MAX_RANK:
+            raise ValueError(f"cannot hold {adapters} adapters of rank {adapter_rank}")
         self.cfg = cfg
         self.dtype = xl.dtype.as_dtype(dtype)
         self.vocab, self.width = cfg.vocab, cfg.width
+        self.cache, self.adapters, self.adapter_rank = cache, adapters, adapter_rank
 
     # -- weights ---------------------------------------------------------------------------------------------------
     def checkpoint_tensors(self) -> Dict[str, Tuple[int, ...]]:
@@ -210,12 +219,68 @@ class Zirunex:
         return {name: 1.0 + normal(shape, 0.1) if len(shape) == 1 else normal(shape, shape[-1] ** -0.5)
                 for name, (shape, _) in self.weights().items()}
 
+    # -- adapters --------------------------------------------------------------------------------------------------------
+    def _joint(self, i: int) -> Dict[str, Tuple[int, int]]:
+        """Rows and columns of the two matrices of layer `i`."""
+        m, L, c = self.cfg.layers[i].mixer, self.cfg.layers[i], self.cfg
+        return {"in": (m.proj_cols + 2 * L.ff, c.width), "out": (c.width, L.joint_cols)}
+
+    def adapter_weights(self) -> Dict[str, Tuple[Tuple[int, ...], xl.dtype]]:
+        """Tensors of all adapters, by name: for every joint matrix `a (n, rank, K)`, `b (n, N, rank)` and `scale (n,)`."""
+        out, n, r = {}, self.adapters, self.adapter_rank
+        for i in self.cfg.owners() if n else ():
+            for k, (N, K) in self._joint(i).items():
+                out.update({f"l{i}.{k}.a": ((n, r, K), self.dtype), f"l{i}.{k}.b": ((n, N, r), self.dtype),
+                            f"l{i}.{k}.scale": ((n,), xl.float32)})
+        return out
+
+    def convert_adapter(self, ckpt: Mapping[str, torch.Tensor]) -> Dict[str, torch.Tensor]:
+        """Tensors of one adapter, by the name of the checkpoint matrix that it stands beside (`l0.mix.q.a (rank, inputs)`, `l0.mix.q.b
+        (outputs, rank)`), -> `a` and `b` of the joint matrices. Matrices without an adapter may be left out. A joint matrix takes the
+        ranks of its parts one after another; together they must not exceed `adapter_rank`."""
+        out, known = {}, set()
+        for i in self.cfg.owners():
+            m, ff, att, mlp = self.cfg.layers[i].mixer, self.cfg.layers[i].ff, f"l{i}.mix.", f"l{i}.mlp."
+            # (checkpoint name, first output row, output rows, first input column, input columns)
+            rows, parts = 0, {"in": [], "out": [(att + "o", 0, self.width, 0, m.out_cols)]}
+            for name, n in ((att + "q", m.heads * m.dim), (att + "k", m.kv_heads * m.dim), (att + "v", m.kv_heads * m.vdim),
+                            (att + "g", m.out_cols), (mlp + "gate", ff), (mlp + "up", ff)):
+                parts["in"].append((name, rows, n, 0, self.width))
+                rows += n
+            if ff:
+                parts["out"].append((mlp + "down", 0, self.width, m.out_cols, ff))
+            for k, (N, K) in self._joint(i).items():
+                a, b, used = torch.zeros(self.adapter_rank, K), torch.zeros(N, self.adapter_rank), 0
+                for name, row, n, col, c in parts[k]:
+                    known.update((name + ".a", name + ".b"))
+                    if not n or (name + ".a" not in ckpt and name + ".b" not in ckpt):
+                        continue
+                    if name + ".a" not in ckpt or name + ".b" not in ckpt:
+                        raise ValueError(f"the adapter of {name!r} needs both halves")
+                    down, up = ckpt[name + ".a"].float().cpu(), ckpt[name + ".b"].float().cpu()
+                    r = down.shape[0]
+                    if tuple(down.shape) != (r, c) or tuple(up.shape) != (n, r):
+                        raise ValueError(f"the adapter of {name!r} is {tuple(down.shape)} and {tuple(up.shape)}, not ({r}, {c}) and ({n}, {r})")
+                    if used + r > self.adapter_rank:
+                        raise ValueError(f"the adapters of one input, up to {name!r}, have a rank of {used + r} together; there is room for "
+                                         f"{self.adapter_rank}")
+                    a[used:used + r, col:col + c], b[row:row + n, used:used + r] = down, up
+                    used += r
+                out[f"l{i}.{k}.a"], out[f"l{i}.{k}.b"] = a, b
+        if set(ckpt) - known:
+            raise ValueError(f"unexpected adapter tensors: {sorted(set(ckpt) - known)[:8]}")
+        return out
+
     # -- state and constants -----------------------------------------------------------------------------------------
     def state(self, batch: int, max_seq: int) -> Dict[str, Tuple[Tuple[int, ...], xl.dtype]]:
         """Per-sequence caches of every layer (also of those that share weights)."""
         out = {}
         for i, L in enumerate(self.cfg.layers):
             m = L.mixer
+            if self.cache == "int8":
+                spec = ops.cache8_spec(batch, m.kv_heads, max_seq, m.dim, m.vdim, self.dtype)
+                out.update({f"l{i}.{field}": s for field, s in spec.items()})
+                continue
             out[f"l{i}.k"] = ((batch, m.kv_heads, max_seq, m.dim), self.dtype)
             out[f"l{i}.v"] = ((batch, m.kv_heads, max_seq, m.vdim), self.dtype)
         return out
@@ -228,7 +293,7 @@ class Zirunex:
         """Whether the norms inside the layers are finished by the products that read them: few rows, sizes that the small-M
         kernels take."""
         c = self.cfg
-        return (rows <= 64 and self.dtype == xl.bfloat16 and c.width % 8 == 0
+        return (rows <= 64 and not self.adapters and self.dtype == xl.bfloat16 and c.width % 8 == 0
                 and all(L.joint_cols % 8 == 0 for L in c.layers))
 
     def portion(self, T: int, t: Callable[[str], xl.Tensor], tokens: xl.Tensor, pos: xl.Tensor, count: xl.Tensor,
@@ -244,13 +309,28 @@ class Zirunex:
         for i, L in enumerate(c.layers):
             m, w = L.mixer, f"l{c.weights_index(i)}."
             h, sumsq = rows
-            proj, joint = ops.linear_split_glu(h, t(w + "in"), m.proj_cols, m.out_cols, L.mlp.limit if L.mlp else 0.0,
-                                               GLU_SLOPE, GLU_SHIFT, sumsq, c.eps)
-            joint = ops.window_attention_(proj, t(w + "q_norm"), t(w + "k_norm"), t(f"l{i}.k"), t(f"l{i}.v"), pos, count, joint,
-                                          T, m.heads, m.scale, m.window, m.keep_first, SINK_SCORE, c.eps)
+            limit = L.mlp.limit if L.mlp else 0.0
+            if self.adapters:
+                proj, joint = ops.split_glu(self._adapted(h, w + "in", t, T), m.proj_cols, m.out_cols, limit, GLU_SLOPE, GLU_SHIFT)
+            else:
+                proj, joint = ops.linear_split_glu(h, t(w + "in"), m.proj_cols, m.out_cols, limit, GLU_SLOPE, GLU_SHIFT, sumsq, c.eps)
+            if self.cache == "int8":
+                cache = ops.Cache8(*(t(f"l{i}.{field}") for field in ops.Cache8._fields))
+                joint = ops.window_attention_q8_(proj, t(w + "q_norm"), t(w + "k_norm"), cache, pos, count, joint, T, m.heads, m.scale,
+                                                 m.window, m.keep_first, SINK_SCORE, c.eps)
+            else:
+                joint = ops.window_attention_(proj, t(w + "q_norm"), t(w + "k_norm"), t(f"l{i}.k"), t(f"l{i}.v"), pos, count, joint,
+                                              T, m.heads, m.scale, m.window, m.keep_first, SINK_SCORE, c.eps)
             after = t(norms[i + 1]) if i + 1 < len(norms) else None
-            rows = ops.linear_residual_rms_(x, joint, t(w + "out"), after, c.eps, deferred=deferred)
+            if self.adapters:
+                rows = ops.residual_rms_(x, self._adapted(joint, w + "out", t, T), after, c.eps), None
+            else:
+                rows = ops.linear_residual_rms_(x, joint, t(w + "out"), after, c.eps, deferred=deferred)
         return rows if final_norm else None
+
+    def _adapted(self, h: xl.Tensor, name: str, t: Callable[[str], xl.Tensor], T: int) -> xl.Tensor:
+        """The product with matrix `name` and with the adapter of every sequence."""
+        return ops.linear_adapted(h, t(name), ops.Adapters(*(t(f"{name}.{k}") for k in ("a", "b", "scale"))), t("adapter"), T)
 
     def logits(self, t: Callable[[str], xl.Tensor], rows: Rows) -> xl.Tensor:
         h, sumsq = rows

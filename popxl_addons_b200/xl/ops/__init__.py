@@ -1401,7 +1401,7 @@ from .decode import (rotary_kv_append_, attention_decode_packed, argmax_rows, ad
 from .sequence import (embed_dyt_, linear_residual_dyt_, select_dyt, linear_rows, linear_swiglu, min_gru_,  # noqa: E402
                        diff_attention_, advance_by_, embed_rms_, linear_residual_rms_, select_rms, linear_split_glu,
                        window_attention_)
-from .serving import (Adapters, Cache8, LogitRules, CACHE8_BLOCK, append_tokens_, cache8_spec, linear_adapted, residual_rms_,  # noqa: E402
+from .serving import (Adapters, Cache8, LogitRules, CACHE8_BLOCK, MAX_BIASES, MAX_HISTORY, MAX_RANK, append_tokens_, cache8_spec, linear_adapted, residual_rms_,  # noqa: E402
                       shape_logits, split_glu, take_shaped_, window_attention_q8_)
 from .extra import *  # noqa: E402,F401,F403
 # module paths of popxl (`ops.call`, `ops.utils`): loaded here so that a later `from ...ops.call import CallSiteInfo`

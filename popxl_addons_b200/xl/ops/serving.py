@@ -23,7 +23,10 @@ from ..opdef import OpDef, emit, emit1
 from .decode import _store_row_ref
 from .sequence import _mm, _rms
 
-CACHE8_BLOCK = 64  # tokens that share a scale
+CACHE8_BLOCK = 64    # tokens that share a scale
+MAX_RANK = 128       # of an adapter
+MAX_BIASES = 1024    # entries of a slot's list
+MAX_HISTORY = (1 << 20) - 1
 
 
 class Cache8(NamedTuple):
@@ -243,6 +246,8 @@ def window_attention_q8_(proj: Tensor, q_norm: Tensor, k_norm: Tensor, cache: Ca
     vdim = cache.v.shape[-1]
     for (field, (shape, dt)), t in zip(cache8_spec(B, G, blocks * CACHE8_BLOCK, dim, vdim, proj.dtype).items(), cache):
         _expect(f"cache.{field}", t, shape, dt)
+    if max(dim, vdim) > 512:
+        raise ValueError(f"the attention kernels take dim and vdim up to 512, not {dim} and {vdim}")
     if heads < 1 or heads % G:
         raise ValueError(f"heads ({heads}) must be a multiple of the cache's {G} heads")
     plain = (heads + G) * dim + G * vdim
@@ -266,6 +271,8 @@ def linear_adapted(x: Tensor, weight: Tensor, adapters: Adapters, slot: Tensor, 
     if x.rank != 2 or weight.rank != 2 or x.shape[1] != weight.shape[1] or x.dtype != weight.dtype:
         raise ValueError(f"cannot multiply {tuple(x.shape)} {x.dtype} by the transpose of {tuple(weight.shape)} {weight.dtype}")
     n, rank = adapters.a.shape[0], adapters.a.shape[1]
+    if not 1 <= rank <= MAX_RANK:
+        raise ValueError(f"adapters have between 1 and {MAX_RANK} numbers between their products, not {rank}")
     _expect("adapters.a", adapters.a, (n, rank, x.shape[1]), x.dtype)
     _expect("adapters.b", adapters.b, (n, weight.shape[0], rank), x.dtype)
     _expect("adapters.scale", adapters.scale, (n,), float32)
@@ -288,6 +295,9 @@ def residual_rms_(x: Tensor, y: Tensor, norm: Optional[Tensor] = None, eps: floa
 
 def _check_rules(rules: LogitRules, vocab: int):
     slots = rules.history.shape[0]
+    if rules.history.shape[1] > MAX_HISTORY or rules.bias_tokens.shape[1] > MAX_BIASES:
+        raise ValueError(f"rules hold at most {MAX_HISTORY} tokens and {MAX_BIASES} biases of a slot, not {rules.history.shape[1]} and "
+                         f"{rules.bias_tokens.shape[1]}")
     for what, t, tail in (("start", rules.start, ()), ("penalties", rules.penalties, (3,)),
                           ("bias_values", rules.bias_values, rules.bias_tokens.shape[1:])):
         _expect(f"rules.{what}", t, (slots, *tail))
