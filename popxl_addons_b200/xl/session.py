@@ -430,7 +430,8 @@ class Session:
         res = {}
         for stream, items in self._outputs.items():
             if len(items) == 1 and len(items[0]) == 1:
-                stacked = items[0][0].contiguous()[None, None]
+                one = items[0][0].contiguous()
+                stacked = one.view(1, 1, *one.shape)
             else:
                 stacked = torch.stack([torch.stack(per_replica) for per_replica in items])  # (t, R_local, *shape)
             if not fetch:
@@ -1028,17 +1029,17 @@ class Session:
                       and self.ir.options.cuda_graphs)
         replayed = state is not None and capturable
         self._stage_inputs(inputs or {}, keep_on_host=replayed)
-        with torch.no_grad():
-            if replayed:
-                from ..ops import native as _native
+        if replayed:
+            from ..ops import native as _native
 
-                for stream, static in state["static_in"].items():
-                    static.copy_(self._next_host_item(stream), non_blocking=True)
-                state["graph"].replay()
-                _native.count_replay(state["kernels"])
-                # outputs that are read before anything else can replay the program need no copy of their own
-                self._after_replay(state, copy=copy and not fetch)
-            else:
+            for stream, static in state["static_in"].items():
+                static.copy_(self._next_host_item(stream), non_blocking=True)
+            state["graph"].replay()
+            _native.count_replay(state["kernels"])
+            # outputs that are read before anything else can replay the program need no copy of their own
+            self._after_replay(state, copy=copy and not fetch)
+        else:
+            with torch.no_grad():
                 vals = [self._value(t, {}) for t in program.bindings.values()]
                 with _read_ahead.following(self._launch_order(program.graph)):
                     if capturable and program in self._programs and self._capture_safe(program.graph):
