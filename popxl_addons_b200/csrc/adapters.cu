@@ -63,26 +63,33 @@ template <typename T, bool VEC> __global__ void __launch_bounds__(256) adapter_d
 }
 
 // ---- shared product + second term, rounded once -------------------------------------------------------------------------------
-// Grid (columns / 256, rows): a thread has one column, and with it one row of B[s], r numbers side by side. W: words of 16, 8 or 4 bytes
-// that its loads take, 0: single elements.
+// Grid (columns / 256, groups of eight rows): a thread has one column of every row of the group, and with it one row of each row's B[s],
+// r numbers side by side. The group's slots and numbers are fetched once, side by side: a CTA per row and 256 columns spent its time on
+// that chain of loads (40 rows x 32256: 17 us). W: bytes that a load of B takes, 0: single elements.
+constexpr int AD_ROWS = 8;
 template <typename T, typename O, int W> __global__ void __launch_bounds__(256) adapter_up_kernel(const AdapterParams p) {
-  __shared__ __align__(16) float low[AD_MAX_RANK];
+  __shared__ __align__(16) float low[AD_ROWS][AD_MAX_RANK];
+  __shared__ int slots[AD_ROWS];
   xl_grid_dependency_wait();
   xl_grid_launch_dependents();
   const int c = blockIdx.x * 256 + threadIdx.x;
-  for (long long row = blockIdx.y; row < p.rows; row += gridDim.y) {
-    const int s = adapter_of(p, row / p.T);
-    __syncthreads();
-    if ((int)threadIdx.x < p.rp) low[threadIdx.x] = p.low[row * p.rp + threadIdx.x];
-    __syncthreads();
-    if (c >= p.N) continue;
-    float v = p.y[row * p.N + c];
-    if (s >= 0) {
-      const T* b = (const T*)p.b + ((long long)s * p.N + c) * p.r;
+  const long long row0 = (long long)blockIdx.y * AD_ROWS;
+  const int rows = (int)(p.rows - row0 < AD_ROWS ? p.rows - row0 : AD_ROWS);
+  float v[AD_ROWS];
+#pragma unroll
+  for (int i = 0; i < AD_ROWS; ++i) v[i] = i < rows && c < p.N ? p.y[(row0 + i) * p.N + c] : 0.f;
+  for (int i = threadIdx.x; i < rows * p.rp; i += 256) low[i / p.rp][i % p.rp] = p.low[row0 * p.rp + i];
+  if ((int)threadIdx.x < rows) slots[threadIdx.x] = adapter_of(p, (row0 + threadIdx.x) / p.T);
+  __syncthreads();
+  if (c >= p.N) return;
+#pragma unroll
+  for (int i = 0; i < AD_ROWS; ++i) {
+    if (i < rows && slots[i] >= 0) {
+      const T* b = (const T*)p.b + ((long long)slots[i] * p.N + c) * p.r;
       float sum = 0.f;
       if (W > 0) {
         constexpr int E = W > 0 ? W / (int)sizeof(T) : 1;
-#pragma unroll 4
+#pragma unroll 2
         for (int j = 0; j < p.r; j += E) {
           uint32_t w[W > 0 ? W / 4 : 1];
           if (W == 16) *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(b + j);
@@ -90,15 +97,17 @@ template <typename T, typename O, int W> __global__ void __launch_bounds__(256) 
           else w[0] = *reinterpret_cast<const uint32_t*>(b + j);
           const T* e = reinterpret_cast<const T*>(w);
 #pragma unroll
-          for (int q = 0; q < E; ++q) sum = fmaf(low[j + q], xl_to_float(e[q]), sum);
+          for (int q = 0; q < E; ++q) sum = fmaf(low[i][j + q], xl_to_float(e[q]), sum);
         }
       } else {
-        for (int j = 0; j < p.r; ++j) sum = fmaf(low[j], xl_to_float(b[j]), sum);
+        for (int j = 0; j < p.r; ++j) sum = fmaf(low[i][j], xl_to_float(b[j]), sum);
       }
-      v += sum;
+      v[i] += sum;
     }
-    ((O*)p.out)[row * p.N + c] = xl_from_float<O>(v);
   }
+#pragma unroll
+  for (int i = 0; i < AD_ROWS; ++i)
+    if (i < rows) ((O*)p.out)[(row0 + i) * p.N + c] = xl_from_float<O>(v[i]);
 }
 
 // ---- many rows of a sequence: mma.sync ---------------------------------------------------------------------------------------
@@ -127,11 +136,11 @@ template <> __device__ __forceinline__ uint32_t ad_pack<__half>(float lo, float 
   return r;
 }
 
-// Grid (row tiles of 16, sequences). Eight warps share a tile and take eighths of K, 32 features at a time: a lane reads 16 bytes of its two
+// Grid (row tiles of 16, sequences). Sixteen warps (eight where their sums would not fit) share a tile and take parts of K, 32 features at a time: a lane reads 16 bytes of its two
 // rows of x and of each of its rows of A, which are the operands of two products (the order of features is free as long as both sides
 // agree). Their sums meet in shared memory. NT: tiles of eight numbers.
-template <typename T, int NT> __global__ void __launch_bounds__(256) adapter_down_mma_kernel(const AdapterParams p) {
-  constexpr int WARPS = 8;
+template <typename T, int NT> __global__ void __launch_bounds__(NT <= 2 ? 512 : 256) adapter_down_mma_kernel(const AdapterParams p) {
+  constexpr int WARPS = NT <= 2 ? 16 : 8, THREADS = WARPS * 32;
   __shared__ float part[WARPS][16][NT * 8 + 1];
   xl_grid_dependency_wait();
   xl_grid_launch_dependents();
@@ -141,7 +150,7 @@ template <typename T, int NT> __global__ void __launch_bounds__(256) adapter_dow
   float* low = p.low + (seq * p.T + t0) * p.rp;
   const int rows = min(16, p.T - t0);
   if (s < 0) {
-    for (int i = threadIdx.x; i < rows * p.rp; i += 256) low[i] = 0.f;
+    for (int i = threadIdx.x; i < rows * p.rp; i += THREADS) low[i] = 0.f;
     return;
   }
   const T* x = (const T*)p.x + (seq * p.T + t0) * p.K;
@@ -153,7 +162,7 @@ template <typename T, int NT> __global__ void __launch_bounds__(256) adapter_dow
     for (int e = 0; e < 4; ++e) c[n][e] = 0.f;
   const int steps = (p.K + 31) / 32;
   const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll 2
+#pragma unroll 4
   for (int i = warp; i < steps; i += WARPS) {
     const int k = i * 32 + j * 8;
     const bool on = k < p.K;
@@ -172,7 +181,7 @@ template <typename T, int NT> __global__ void __launch_bounds__(256) adapter_dow
     for (int e = 0; e < 4; ++e) part[warp][quad + 8 * (e >> 1)][n * 8 + 2 * j + (e & 1)] = c[n][e];
   __syncthreads();
   const float scale = p.scale[s];
-  for (int i = threadIdx.x; i < rows * p.rp; i += 256) {
+  for (int i = threadIdx.x; i < rows * p.rp; i += THREADS) {
     const int r = i / p.rp, q = i - r * p.rp;
     float sum = 0.f;
     if (q < NT * 8) {
@@ -183,29 +192,23 @@ template <typename T, int NT> __global__ void __launch_bounds__(256) adapter_dow
   }
 }
 
-// Grid (columns / 128, row tiles of 64, sequences): the adapters' term alone, rounded to T. A warp has 32 columns for all 64 rows; its lanes'
-// columns are chosen so that each ends up with eight neighbours, which leave in one store. `low` enters as sums of two T (value and
-// rounding error). KS: steps of 16 numbers.
+// Grid (columns / 128, row tiles of 256, sequences): the adapters' term alone, rounded to T. A warp has 32 columns for all rows of the tile,
+// whose row of B[s] it holds; its lanes' columns are chosen so that each ends up with eight neighbours, which leave in one store. `low`
+// enters as sums of two T (value and rounding error). Writing the result bounds it; tiles of 64 rows, each with its own chain of loads
+// before the first store, took 74 us for 4096 x 32256. KS: steps of 16 numbers.
+constexpr int AD_TILE = 256;
 template <typename T, int KS> __global__ void __launch_bounds__(128) adapter_up_mma_kernel(const AdapterParams p) {
-  __shared__ uint32_t hi[64][KS * 8 + 1], lo[64][KS * 8 + 1];  // pairs of numbers
   xl_grid_dependency_wait();
   xl_grid_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = lane >> 2, j = lane & 3;
   const long long seq = blockIdx.z;
-  const int t0 = blockIdx.y * 64, s = adapter_of(p, seq), rows = min(64, p.T - t0), c0 = blockIdx.x * 128 + warp * 32;
+  const int t0 = blockIdx.y * AD_TILE, s = adapter_of(p, seq), rows = min(AD_TILE, p.T - t0), c0 = blockIdx.x * 128 + warp * 32;
+  if (c0 >= p.N) return;
   T* out = (T*)p.out + (seq * p.T + t0) * p.N;
+  const float* low = p.low + (seq * p.T + t0) * p.rp;
   const bool wide = p.N % 8 == 0;
   uint32_t b[4][KS][2];
   if (s >= 0) {
-    const float* low = p.low + (seq * p.T + t0) * p.rp;
-    for (int i = threadIdx.x; i < 64 * KS * 8; i += 128) {
-      const int r = i / (KS * 8), q = i % (KS * 8);
-      const float2 v = r < rows ? *reinterpret_cast<const float2*>(low + r * p.rp + 2 * q) : make_float2(0.f, 0.f);
-      const uint32_t w = ad_pack<T>(v.x, v.y);
-      const float2 back = xl_pair_to_float2<T>(w);
-      hi[r][q] = w;
-      lo[r][q] = ad_pack<T>(v.x - back.x, v.y - back.y);
-    }
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const int c = c0 + 8 * (quad >> 1) + 2 * u + (quad & 1);
@@ -228,7 +231,7 @@ template <typename T, int KS> __global__ void __launch_bounds__(128) adapter_up_
         }
     }
   }
-  __syncthreads();
+#pragma unroll 2
   for (int m = 0; m * 16 < rows; ++m) {
     float c[4][4];
 #pragma unroll
@@ -236,16 +239,21 @@ template <typename T, int KS> __global__ void __launch_bounds__(128) adapter_up_
 #pragma unroll
       for (int e = 0; e < 4; ++e) c[u][e] = 0.f;
     if (s >= 0) {
-      const int r = m * 16 + quad;
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
-        const int q = k * 8 + j;
-        const uint32_t h0 = hi[r][q], h1 = hi[r + 8][q], h2 = hi[r][q + 4], h3 = hi[r + 8][q + 4];
-        const uint32_t l0 = lo[r][q], l1 = lo[r + 8][q], l2 = lo[r][q + 4], l3 = lo[r + 8][q + 4];
+        uint32_t h[4], e[4];  // rows quad, quad + 8; numbers 2 j, 2 j + 1, then 2 j + 8, 2 j + 9
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = m * 16 + quad + 8 * (i & 1);
+          const float2 v = r < rows ? *reinterpret_cast<const float2*>(low + r * p.rp + k * 16 + 8 * (i >> 1) + 2 * j) : make_float2(0.f, 0.f);
+          h[i] = ad_pack<T>(v.x, v.y);
+          const float2 back = xl_pair_to_float2<T>(h[i]);
+          e[i] = ad_pack<T>(v.x - back.x, v.y - back.y);
+        }
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-          ad_mma<T>(c[u], h0, h1, h2, h3, b[u][k][0], b[u][k][1]);
-          ad_mma<T>(c[u], l0, l1, l2, l3, b[u][k][0], b[u][k][1]);
+          ad_mma<T>(c[u], h[0], h[1], h[2], h[3], b[u][k][0], b[u][k][1]);
+          ad_mma<T>(c[u], e[0], e[1], e[2], e[3], b[u][k][0], b[u][k][1]);
         }
       }
     }
@@ -297,7 +305,8 @@ XL_API int xl_adapter_up(const float* low, const void* b, const int* slot, const
   AdapterParams p = {};
   p.b = b; p.slot = slot; p.low = const_cast<float*>(low); p.y = y; p.out = out; p.rows = rows; p.T = T; p.N = N; p.n = n; p.r = r;
   p.rp = (r + 15) / 16 * 16;
-  const dim3 grid((N + 255) / 256, (unsigned)(rows < 65535 ? rows : 65535));
+  if ((rows + AD_ROWS - 1) / AD_ROWS > 65535) return -1;
+  const dim3 grid((N + 255) / 256, (unsigned)((rows + AD_ROWS - 1) / AD_ROWS));
   XL_DISPATCH_DTYPE(dtype, D, {
     const int bytes = r * (int)sizeof(D);
     const uintptr_t at = (uintptr_t)b;
@@ -326,7 +335,7 @@ XL_API int xl_adapter_down_mma(const void* x, const void* a, const float* scale,
   else XL_AD(__half);
 #undef XL_AD
   if (!kernel) return -1;
-  XL_TRY(xl_launch_overlapped(kernel, grid, dim3(256), (size_t)0, s, p));
+  XL_TRY(xl_launch_overlapped(kernel, grid, dim3(r <= 16 ? 512 : 256), (size_t)0, s, p));
   return (int)cudaGetLastError();
 }
 
@@ -334,12 +343,12 @@ XL_API int xl_adapter_down_mma(const void* x, const void* a, const float* scale,
 XL_API int xl_adapter_up_mma(const float* low, const void* b, const int* slot, void* out, long long rows, int T, int N, int n, int r,
                              int dtype, cudaStream_t s) {
   if (!adapter_sizes_ok(rows, T, 1, N, n, r) || dtype == XL_F32 || (((uintptr_t)out) & 15) || (((uintptr_t)b) & 3) || rows / T > 65535 ||
-      (T + 63) / 64 > 65535)
+      (T + AD_TILE - 1) / AD_TILE > 65535)
     return -1;
   AdapterParams p = {};
   p.b = b; p.slot = slot; p.low = const_cast<float*>(low); p.out = out; p.rows = rows; p.T = T; p.N = N; p.n = n; p.r = r;
   p.rp = (r + 15) / 16 * 16;
-  const dim3 grid((N + 127) / 128, (T + 63) / 64, (unsigned)(rows / T));
+  const dim3 grid((N + 127) / 128, (T + AD_TILE - 1) / AD_TILE, (unsigned)(rows / T));
   void (*kernel)(const AdapterParams);
 #define XL_AD(D) \
   kernel = p.rp == 16 ? adapter_up_mma_kernel<D, 1> : (p.rp == 32 ? adapter_up_mma_kernel<D, 2> : (p.rp == 48 ? adapter_up_mma_kernel<D, 3> : (p.rp == 64 ? adapter_up_mma_kernel<D, 4> : nullptr)))

@@ -111,19 +111,19 @@ __global__ void __launch_bounds__(256) q8_append_kernel(const Q8AppendParams p) 
   const bool complete = r1 == r0 + Q8_BLOCK;
   float top[2] = {0.f, 0.f};
   const int first = max(r0, fill), items = R + 2;
-  for (int i = warp; i < (r1 - first) * items + 2 * (first - r0); i += WARPS) {
-    float x[NP][V];
-    const int k = i - (r1 - first) * items;
-    if (k >= 0) {  // a token that was there before
-      const int r = r0 + (k >> 1), kind = k & 1;
-      load(tail[kind] + (long long)r * width[kind], width[kind], x);
-      store(raw[kind] + (long long)r * width[kind], width[kind], x);
+  // tokens that were there before (of the first block: rows of the tail and of `raw` are consecutive)
 #pragma unroll
-      for (int u = 0; u < NP; ++u)
+  for (int kind = 0; kind < 2; ++kind) {
+#pragma unroll 4
+    for (int i = threadIdx.x * V; i < (first - r0) * width[kind]; i += 256 * V) {
+      const Q8Piece<T, V> piece = *reinterpret_cast<const Q8Piece<T, V>*>(tail[kind] + i);
+      *reinterpret_cast<Q8Piece<T, V>*>(raw[kind] + i) = piece;
 #pragma unroll
-        for (int e = 0; e < V; ++e) top[kind] = fmaxf(top[kind], fabsf(x[u][e]));
-      continue;
+      for (int e = 0; e < V; ++e) top[kind] = fmaxf(top[kind], fabsf(xl_to_float(piece.v[e])));
     }
+  }
+  for (int i = warp; i < (r1 - first) * items; i += WARPS) {
+    float x[NP][V];
     const int r = first + i / items, item = i % items, t = r - fill;
     if (item < R) {  // a query head
       load(proj + (long long)t * p.ld + (long long)(g * R + item) * p.dim, p.dim, x);
@@ -253,7 +253,7 @@ __device__ __forceinline__ uint4 q8_code_values(const uint2& c, float scale) {
   return make_uint4(dd_pack(x[0], x[1]), dd_pack(x[2], x[3]), dd_pack(x[4], x[5]), dd_pack(x[6], x[7]));
 }
 
-__global__ void __launch_bounds__(256, 3) q8_append_expand_kernel(const Q8ExpandParams p) {
+__global__ void __launch_bounds__(256, 4) q8_append_expand_kernel(const Q8ExpandParams p) {
   constexpr int HALVES = 16;  // half warps
   __shared__ __align__(16) uint4 tile[2][Q8_BLOCK][16];
   __shared__ float tops[2][HALVES], scales[2];
@@ -320,38 +320,54 @@ __global__ void __launch_bounds__(256, 3) q8_append_expand_kernel(const Q8Expand
   // new tokens: whole warps go through the rows, for the sums' shuffles
   const bool to_tail = end < Q8_BLOCK;
   const int first = max(r0, fill);
-  for (int rr = first; rr < r1; rr += HALVES) {
-    const int r = rr + half, t = r - fill;
-    const bool on = r < r1;
-    const __nv_bfloat16* row = proj + (long long)(on ? t : 0) * p.ld;
-    uint4 w = on && on_k ? *reinterpret_cast<const uint4*>(row + (long long)(p.H + g) * p.dim + l * 8) : zero;
-    const uint4 v = on && on_v ? *reinterpret_cast<const uint4*>(row + (long long)(p.H + p.G) * p.dim + (long long)g * p.vdim + l * 8) : zero;
-    w = key_of(w);
-    if (on) {
-      put_key(r, w);
-      put_value(r, v);
-      if (to_tail && on_k) *reinterpret_cast<uint4*>(p.kt + (head * Q8_BLOCK + r) * p.dim + l * 8) = w;
-      if (to_tail && on_v) *reinterpret_cast<uint4*>(p.vt + (head * Q8_BLOCK + r) * p.vdim + l * 8) = v;
+  {
+    constexpr int ROWS = Q8_BLOCK / HALVES;
+    uint4 w[ROWS], v[ROWS];  // every load of this block before the first use
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      const int r = first + i * HALVES + half;
+      const __nv_bfloat16* row = proj + (long long)(r - fill) * p.ld;
+      w[i] = r < r1 && on_k ? *reinterpret_cast<const uint4*>(row + (long long)(p.H + g) * p.dim + l * 8) : zero;
+      v[i] = r < r1 && on_v ? *reinterpret_cast<const uint4*>(row + (long long)(p.H + p.G) * p.dim + (long long)g * p.vdim + l * 8) : zero;
+    }
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      const int r = first + i * HALVES + half;
+      if (first + i * HALVES >= r1) break;
+      const uint4 y = key_of(w[i]);
+      if (r < r1) {
+        put_key(r, y);
+        put_value(r, v[i]);
+        if (to_tail && on_k) *reinterpret_cast<uint4*>(p.kt + (head * Q8_BLOCK + r) * p.dim + l * 8) = y;
+        if (to_tail && on_v) *reinterpret_cast<uint4*>(p.vt + (head * Q8_BLOCK + r) * p.vdim + l * 8) = v[i];
+      }
     }
   }
   const int queries = (r1 - first) * R;  // consecutive in `q`, heads of a token side by side in a row of the projections
   __half* q = p.q + (head * p.T + (first - fill)) * R * p.dim;
-#pragma unroll 2
-  for (int i0 = 0; i0 < queries; i0 += HALVES) {
-    const int i = i0 + half;
-    const bool on = i < queries && on_k;
-    const int t = i / R, hh = i - t * R;
-    const uint4 w = on ? *reinterpret_cast<const uint4*>(proj + (long long)(first - fill + t) * p.ld + (long long)(g * R + hh) * p.dim + l * 8) : zero;
-    float x[8], sum = 0.f;
-    q8_unpack(w, x);
+  constexpr int BATCH = 4;
+  for (int i0 = 0; i0 < queries; i0 += HALVES * BATCH) {
+    uint4 w[BATCH];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) sum += x[e] * x[e];
+    for (int k = 0; k < BATCH; ++k) {
+      const int i = i0 + k * HALVES + half, t = i / R, hh = i - t * R;
+      w[k] = i < queries && on_k ? *reinterpret_cast<const uint4*>(proj + (long long)(first - fill + t) * p.ld + (long long)(g * R + hh) * p.dim + l * 8)
+                                 : zero;
+    }
 #pragma unroll
-    for (int d = 8; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    const float f = 1.f / (sqrtf(sum / p.dim + (float)p.eps) * unit_q);
+    for (int k = 0; k < BATCH; ++k) {
+      const int i = i0 + k * HALVES + half;
+      float x[8], sum = 0.f;
+      q8_unpack(w[k], x);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] *= f * wq[e];
-    if (on) *reinterpret_cast<uint4*>(q + (long long)i * p.dim + l * 8) = q8_halves(x);
+      for (int e = 0; e < 8; ++e) sum += x[e] * x[e];
+#pragma unroll
+      for (int d = 8; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+      const float f = 1.f / (sqrtf(sum / p.dim + (float)p.eps) * unit_q);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] *= f * wq[e];
+      if (i < queries && on_k) *reinterpret_cast<uint4*>(q + (long long)i * p.dim + l * 8) = q8_halves(x);
+    }
   }
   if (r1 == end) {  // the last rows: zeros behind them
     for (int r = end + half; r < end + 128; r += HALVES)
@@ -529,7 +545,7 @@ __global__ void __launch_bounds__(SPLIT == 1 ? 128 : SPLIT * 32) q8_attn_general
       for (int e = 0; e < VPL; ++e) o[e] *= corr;
       const float wv = RAW ? w : w * (j < end ? vs[j / Q8_BLOCK] : 0.f);
       const int m = min(32, end - j0);
-#pragma unroll 4
+#pragma unroll 8
       for (int k = 0; k < m; ++k) {
         const float wk = __shfl_sync(0xffffffffu, wv, k);
 #pragma unroll
