@@ -139,7 +139,7 @@ template <> __device__ __forceinline__ uint32_t ad_pack<__half>(float lo, float 
 // Grid (row tiles of 16, sequences). Sixteen warps (eight where their sums would not fit) share a tile and take parts of K, 32 features at a time: a lane reads 16 bytes of its two
 // rows of x and of each of its rows of A, which are the operands of two products (the order of features is free as long as both sides
 // agree). Their sums meet in shared memory. NT: tiles of eight numbers.
-template <typename T, int NT> __global__ void __launch_bounds__(NT <= 2 ? 512 : 256) adapter_down_mma_kernel(const AdapterParams p) {
+template <typename T, int NT> __global__ void __launch_bounds__(NT <= 2 ? 512 : 256, 2) adapter_down_mma_kernel(const AdapterParams p) {
   constexpr int WARPS = NT <= 2 ? 16 : 8, THREADS = WARPS * 32;
   __shared__ float part[WARPS][16][NT * 8 + 1];
   xl_grid_dependency_wait();
@@ -162,7 +162,7 @@ template <typename T, int NT> __global__ void __launch_bounds__(NT <= 2 ? 512 : 
     for (int e = 0; e < 4; ++e) c[n][e] = 0.f;
   const int steps = (p.K + 31) / 32;
   const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll 4
+#pragma unroll 2
   for (int i = warp; i < steps; i += WARPS) {
     const int k = i * 32 + j * 8;
     const bool on = k < p.K;

@@ -4,7 +4,7 @@
 //
 //   xl_q8_append          queries to their buffer, keys and values to `raw`; complete blocks to codes, the rest to the tails
 //   xl_q8_attn_general    any sizes and types, scores and weights in fp32 on the CUDA cores: one warp per row and head
-//   xl_q8_append_expand   the same, laid out for the tensor cores (xl_q8_attn_tcgen05 in attention_window_tcgen05.cu)
+//   xl_q8_append_expand   the same, laid out for the tensor cores (xl_q8_attn_tcgen05 in attention_q8_tcgen05.cu)
 //   xl_q8_attn_few        few rows per sequence, bf16, on mma.sync; of a single token norms, append and codes in the same launch
 #include "attention_decode.cuh"
 #include "attention_q8.cuh"
@@ -213,10 +213,10 @@ template <int SEL> __device__ __forceinline__ uint32_t q8_pair(uint32_t biased) 
 }
 
 // ---- append for the tensor cores ----------------------------------------------------------------------------------------------
-// What attention_window_tcgen05.cu reads: queries and raw keys as fp16 in units of a power of two, raw values, and the codes of
-// complete blocks as fp16 keys and bf16 values. bf16 projections, dim and vdim multiples of 8 up to 128. Sixteen lanes share a row, 16 bytes
-// each; a CTA has the rows of one block of one key / value head, two rows of each half warp in flight. Value rows that a tile of 128 keys
-// may read beyond the last key are zeros: a weight of zero times what memory happened to hold could be NaN.
+// What attention_q8_tcgen05.cu reads: queries and raw keys as fp16 in units of a power of two, raw values, and the codes of
+// complete blocks as fp16 (keys) and bf16 (values). bf16 projections, dim and vdim multiples of 8 up to 128. Sixteen lanes share a row, 16 bytes
+// each; a CTA has the rows of one block of one key / value head. Raw value rows that the last block's keys do not fill are zeros: a weight of
+// zero times what memory happened to hold could be NaN.
 struct Q8ExpandParams {
   const __nv_bfloat16* proj;
   long long ld;
@@ -241,15 +241,15 @@ __device__ __forceinline__ void q8_unpack(const uint4& w, float (&x)[8]) {
 __device__ __forceinline__ uint4 q8_halves(const float (&x)[8]) {
   return make_uint4(q8_pack_f16(x[0], x[1]), q8_pack_f16(x[2], x[3]), q8_pack_f16(x[4], x[5]), q8_pack_f16(x[6], x[7]));
 }
-// eight codes as fp16, and as bf16 times the scale
+// eight codes as fp16, and as bf16
 __device__ __forceinline__ uint4 q8_code_halves(const uint2& c) {
   const uint32_t a = c.x ^ 0x80808080u, b = c.y ^ 0x80808080u;
   return make_uint4(q8_pair<0x4140>(a), q8_pair<0x4342>(a), q8_pair<0x4140>(b), q8_pair<0x4342>(b));
 }
-__device__ __forceinline__ uint4 q8_code_values(const uint2& c, float scale) {
+__device__ __forceinline__ uint4 q8_code_values(const uint2& c) {
   float x[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) x[e] = (float)(int8_t)((e < 4 ? c.x : c.y) >> (8 * (e & 3))) * scale;
+  for (int e = 0; e < 8; ++e) x[e] = (float)(int8_t)((e < 4 ? c.x : c.y) >> (8 * (e & 3)));
   return make_uint4(dd_pack(x[0], x[1]), dd_pack(x[2], x[3]), dd_pack(x[4], x[5]), dd_pack(x[6], x[7]));
 }
 
@@ -369,13 +369,8 @@ __global__ void __launch_bounds__(256, 4) q8_append_expand_kernel(const Q8Expand
       if (i < queries && on_k) *reinterpret_cast<uint4*>(q + (long long)i * p.dim + l * 8) = q8_halves(x);
     }
   }
-  if (r1 == end) {  // the last rows: zeros behind them
-    for (int r = end + half; r < end + 128; r += HALVES)
-      if (on_v) *reinterpret_cast<uint4*>(p.raw_v + (head * p.raw_rows + r) * p.vdim + l * 8) = zero;
-    if (r1 < r0 + Q8_BLOCK)
-      for (int r = half; r < Q8_BLOCK; r += HALVES)
-        if (on_v) *reinterpret_cast<uint4*>(p.vx + (at * Q8_BLOCK + r) * p.vdim + l * 8) = zero;
-  }
+  for (int r = r1 + half; r < r0 + Q8_BLOCK; r += HALVES)
+    if (on_v) *reinterpret_cast<uint4*>(p.raw_v + (head * p.raw_rows + r) * p.vdim + l * 8) = zero;
   if (r1 == r0 + Q8_BLOCK) {
 #pragma unroll
     for (int kind = 0; kind < 2; ++kind) {
@@ -405,7 +400,7 @@ __global__ void __launch_bounds__(256, 4) q8_append_expand_kernel(const Q8Expand
           *reinterpret_cast<uint4*>(p.kx + row * p.dim + l * 8) = q8_code_halves(word);
         } else if (kind == 1 && on_v) {
           *reinterpret_cast<uint2*>(p.vc + row * p.vdim + l * 8) = word;
-          *reinterpret_cast<uint4*>(p.vx + row * p.vdim + l * 8) = q8_code_values(word, step.scale);
+          *reinterpret_cast<uint4*>(p.vx + row * p.vdim + l * 8) = q8_code_values(word);
         }
       }
     }
@@ -426,8 +421,8 @@ __global__ void __launch_bounds__(256, 4) q8_append_expand_kernel(const Q8Expand
   }
 }
 
-// Blocks that were complete before the portion and that its tiles read: those of the kept first tokens, whole tiles of them, and those
-// from the first window on. Grid (groups of blocks, G, B).
+// Blocks that were complete before the portion and that its queries see: those of the kept first tokens and those from the first window
+// on. Grid (groups of blocks, G, B).
 constexpr int Q8_EXPAND_GROUP = 8;
 __global__ void __launch_bounds__(256) q8_expand_kernel(const Q8ExpandParams p) {
   xl_grid_dependency_wait();
@@ -436,13 +431,12 @@ __global__ void __launch_bounds__(256) q8_expand_kernel(const Q8ExpandParams p) 
   const int pos = p.pos[b], n = min(p.count[b], p.T);
   if (n <= 0 || pos < 0 || (long long)pos + n > (long long)p.blocks * Q8_BLOCK) return;
   const int done = pos / Q8_BLOCK, from = p.window ? max(0, pos - p.window + 1) / Q8_BLOCK : 0;
-  const int kept = (int)(((long long)p.keep_first + 127) / 128 * 2);
+  const int kept = (int)(((long long)p.keep_first + Q8_BLOCK - 1) / Q8_BLOCK);
   const long long head = (long long)b * p.G + g;
   const bool on_k = l * 8 < p.dim, on_v = l * 8 < p.vdim;
   for (int j = blockIdx.x * Q8_EXPAND_GROUP; j < min(done, (int)(blockIdx.x + 1) * Q8_EXPAND_GROUP); ++j) {
     if (j < from && j >= kept) continue;
     const long long at = head * p.blocks + j;
-    const float scale = p.vs[at];
     uint2 k[4], v[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -454,7 +448,7 @@ __global__ void __launch_bounds__(256) q8_expand_kernel(const Q8ExpandParams p) 
     for (int i = 0; i < 4; ++i) {
       const long long row = at * Q8_BLOCK + half + 16 * i;
       if (on_k) *reinterpret_cast<uint4*>(p.kx + row * p.dim + l * 8) = q8_code_halves(k[i]);
-      if (on_v) *reinterpret_cast<uint4*>(p.vx + row * p.vdim + l * 8) = q8_code_values(v[i], scale);
+      if (on_v) *reinterpret_cast<uint4*>(p.vx + row * p.vdim + l * 8) = q8_code_values(v[i]);
     }
   }
 }
@@ -1386,14 +1380,14 @@ XL_API int xl_q8_attn_few(const void* proj, long long ld, const float* wq, const
 }
 
 // The same as xl_q8_append for xl_q8_attn_tcgen05 (see there): q (B, G, T, H/G, dim) and raw_k (B, G, raw_rows, dim) fp16, raw_v (B, G,
-// raw_rows, vdim) bf16 with raw_rows >= T + 192, kx (B, G, blocks * 64, dim) fp16, vx (.., vdim) bf16: complete blocks that the portion
+// raw_rows, vdim) bf16 with raw_rows >= T + 128, kx (B, G, blocks * 64, dim) fp16, vx (.., vdim) bf16: complete blocks that the portion
 // can see. bf16; dim, vdim multiples of 8 up to 128, ld a multiple of 8, all pointers 16-byte aligned.
 XL_API int xl_q8_append_expand(const void* proj, long long ld, const float* wq, const float* wk, void* q, void* raw_k, void* raw_v,
                                int raw_rows, void* kx, void* vx, void* kc, void* vc, float* ks, float* vs, void* kt, void* vt,
                                const int* pos, const int* count, int B, int T, int H, int G, int dim, int vdim, int blocks, int window,
                                int keep_first, double eps, cudaStream_t s) {
   if (!q8_sizes_ok(B, T, H, G, dim, vdim, blocks) || dim % 8 || vdim % 8 || dim > 128 || vdim > 128 || ld % 8 || !wq || !wk ||
-      ld < (long long)(H + G) * dim + (long long)G * vdim || raw_rows < T + Q8_BLOCK + 128 || window < 0 || keep_first < 0)
+      ld < (long long)(H + G) * dim + (long long)G * vdim || raw_rows < T + 2 * Q8_BLOCK || window < 0 || keep_first < 0)
     return -1;
   const uintptr_t at = (uintptr_t)proj | (uintptr_t)q | (uintptr_t)raw_k | (uintptr_t)raw_v | (uintptr_t)kx | (uintptr_t)vx | (uintptr_t)kc |
                        (uintptr_t)vc | (uintptr_t)kt | (uintptr_t)vt;

@@ -1,4 +1,4 @@
-// Layout of attention against a key / value cache of 8 bits (attention_q8.cu, attention_window_tcgen05.cu).
+// Layout of attention against a key / value cache of 8 bits (attention_q8.cu, attention_q8_tcgen05.cu).
 //
 //   k codes (B, G, blocks, 64, dim) int8, v codes (B, G, blocks, 64, vdim) int8, scales (B, G, blocks) fp32:
 //     value = code * scale, scale = max |x| / 127 over the block, code = x / scale rounded to the nearest whole number

@@ -12,16 +12,9 @@
 //                               sink, lazy rescaling of O_m in TMEM
 // P replaces S in TMEM as two bf16 numbers per weight (value and rounding error), so the weights keep more than 16 bits.
 //
-// Against a cache of 8 bits (Q8; layouts in attention_q8.cuh) the keys are two lists, one behind the other: the codes of complete
-// blocks, and the raw rows of the portion from the start of the block in progress. A query sees raw rows of its own block and codes of
-// earlier blocks; which is which is a mask like any other. Codes come as fp16 (exact; the block's scale multiplies the score, which
-// costs a second factor per tile of two blocks), their values as bf16 products with the scale; queries and raw keys as fp16 in units of a
-// power of two above their norm's factors. Expanding codes outside this kernel moves five bytes per code once per portion, where each
-// CTA of 256 rows would convert every tile again next to a softmax that already fills the issue slots.
-//
 // TMEM columns: [0, 128) S_0 / P_0, [128, 256) S_1 / P_1 (the upper half of each holds the rounding errors),
 // [256, 256 + VD) O_0, [256 + VD, 256 + 2 VD) O_1. One CTA per SM. Every wait is bounded (see tcgen05.cuh).
-#include "attention_q8.cuh"
+#include "attention_window.cuh"
 #include "tcgen05.cuh"
 
 namespace {
@@ -43,9 +36,6 @@ struct WindowParams {
   int T, H, G, dim, vdim, Smax, window, keep_first;
   float scale, sink;
   int* err;
-  // Q8 only: scales of the key blocks (B, G, blocks), factors of the norms, rows of a head in the raw lists
-  const float *ks, *wq, *wk;
-  int blocks, raw_rows;
 };
 
 using namespace xl_tc;
@@ -64,11 +54,10 @@ template <int DK, int VD> struct WindowSmem {
   static constexpr int TOTAL = NEEDED > 120 * 1024 ? NEEDED : 120 * 1024;
 };
 
-template <int DK, int VD, bool Q8>
+template <int DK, int VD>
 __global__ void __launch_bounds__(NUM_THREADS, 1)
     window_attn_tcgen05_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-                               const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_raw_k,
-                               const __grid_constant__ CUtensorMap map_raw_v, const WindowParams p) {
+                               const __grid_constant__ CUtensorMap map_v, const WindowParams p) {
   using L = WindowSmem<DK, VD>;
   static_assert(L::TOTAL <= 227 * 1024, "shared memory");
   extern __shared__ uint8_t smem_raw[];
@@ -99,18 +88,12 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   // key blocks: those of the kept tokens that lie before every window of this CTA, then everything from there on; or, where
   // that takes no more blocks, simply all keys
   WindowRange seen = window_range(p_first, p.window, p.keep_first);
-  const int base = pos / Q8_BLOCK * Q8_BLOCK;  // Q8: position of the first raw row
-  if (Q8) seen.first = seen.first / Q8_BLOCK * Q8_BLOCK;
-  const int code_end = Q8 ? p_last / Q8_BLOCK * Q8_BLOCK : 0, raw0 = Q8 ? p_first / Q8_BLOCK * Q8_BLOCK - base : 0;
-  if (Q8) seen.kept = min(min(seen.kept, seen.first), code_end);
   int kept_blocks = (seen.kept + BKV - 1) / BKV;
-  const int last = Q8 ? code_end - 1 : p_last;  // last key of the first list, if it has any
-  if (kept_blocks + (last - seen.first) / BKV >= last / BKV && last >= seen.first) {
+  if (kept_blocks + (p_last - seen.first) / BKV >= p_last / BKV) {
     seen = {0, 0};
     kept_blocks = 0;
   }
-  const int n_code = kept_blocks + (last >= seen.first ? (last - seen.first) / BKV + 1 : 0);
-  const int n_kv = Q8 ? n_code + (p_last - base - raw0) / BKV + 1 : n_code;
+  const int n_kv = kept_blocks + (p_last - seen.first) / BKV + 1;
   auto first_key = [&](int j) { return j < kept_blocks ? j * BKV : seen.first + (j - kept_blocks) * BKV; };
 
   if (threadIdx.x == 0) {
@@ -157,8 +140,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       bool ok = true;
       int issued = 0;
       for (int j = 0; j < n_kv && ok; ++j) {
-        const bool raw = Q8 && j >= n_code;
-        const int st = j % stages, row = raw ? (b * p.G + g) * p.raw_rows + raw0 + (j - n_code) * BKV : (b * p.G + g) * p.Smax + first_key(j);
+        const int st = j % stages, row = (b * p.G + g) * p.Smax + first_key(j);
         if (j >= stages) {
           ok = mbar_wait(&empty[st], (uint32_t)(j / stages - 1) & 1u, abort_flag, p.err, ERR_KV_EMPTY);
           if (!ok) break;
@@ -167,15 +149,14 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           mbar_expect_tx(&full[st], L::K_BYTES);
 #pragma unroll
           for (int kb = 0; kb < DK / 64; ++kb)
-            tma_load_2d(sK + st * L::K_BYTES + kb * (BKV * 128), raw ? &map_raw_k : &map_k, &full[st], kb * 64, row);
+            tma_load_2d(sK + st * L::K_BYTES + kb * (BKV * 128), &map_k, &full[st], kb * 64, row);
         } else {
           mbar_expect_tx(&full[st], L::V_BYTES);
 #pragma unroll
           for (int kk = 0; kk < BKV / 64; ++kk)
 #pragma unroll
             for (int jn = 0; jn < VD / 64; ++jn)
-              tma_load_2d(sV + st * L::V_BYTES + (kk * (VD / 64) + jn) * 8192, raw ? &map_raw_v : &map_v, &full[st],
-                          jn * 64, row + kk * 64);
+              tma_load_2d(sV + st * L::V_BYTES + (kk * (VD / 64) + jn) * 8192, &map_v, &full[st], jn * 64, row + kk * 64);
         }
         issued = j + 1;
       }
@@ -190,8 +171,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   } else if (warp == 1) {
     if (elect_one()) {
       // bf16 operands, fp32 accumulators. S: both K-major, N = BKV. O: A (P) from TMEM, B (V) MN-major (bit 16), N = VD.
-      // Q8: queries and keys are fp16.
-      const uint32_t idesc_s = (1u << 4) | (Q8 ? 0u : (1u << 7) | (1u << 10)) | ((uint32_t)(BKV >> 3) << 17) | ((uint32_t)(TILE_M >> 4) << 24);
+      const uint32_t idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BKV >> 3) << 17) | ((uint32_t)(TILE_M >> 4) << 24);
       const uint32_t idesc_o = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(VD >> 3) << 17) |
                                ((uint32_t)(TILE_M >> 4) << 24);
       bool ok = mbar_wait(q_full, 0, abort_flag, p.err, ERR_Q);
@@ -246,22 +226,10 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     const uint32_t lane_base = (uint32_t)(qtr * 32) << 16;
     const uint32_t tmem_s = tmem_base + lane_base + m * BKV;
     const uint32_t tmem_o = tmem_base + lane_base + 2 * BKV + m * VD;
-    // Q8: scores differ in their factors, so the maximum is held in units of the exponent, else in units of the products
-    const float unit_q = Q8 ? q8_norm_unit(p.wq, p.dim, lane) : 1.f, unit_k = Q8 ? q8_norm_unit(p.wk, p.dim, lane) : 1.f;
-    const float c = p.scale * 1.4426950408889634f * unit_q;
-    const int own = Q8 ? qpos / Q8_BLOCK * Q8_BLOCK : 0;
-    float mx = Q8 ? p.sink * 1.4426950408889634f : p.sink / p.scale, l = p.sink == -INFINITY ? 0.f : 1.f;
+    const float c = p.scale * 1.4426950408889634f;
+    float mx = p.sink / p.scale, l = p.sink == -INFINITY ? 0.f : 1.f;
     bool ok = true;
     for (int j = 0; j < n_kv && ok; ++j) {
-      const bool raw = Q8 && j >= n_code;
-      float ch[2] = {c, c};  // factors of the tile's two halves
-      if (Q8) {
-        const long long blk = (long long)(b * p.G + g) * p.blocks;
-        const int at = raw ? 0 : first_key(j) / Q8_BLOCK;
-        // never zero, the scale of a block of zeros: minus infinity, a masked score, has to stay what it is
-        ch[0] = fmaxf(c * (raw ? unit_k : p.ks[blk + at]), 1e-37f);
-        ch[1] = fmaxf(c * (raw ? unit_k : p.ks[blk + min(at + 1, p.blocks - 1)]), 1e-37f);
-      }
       ok = __all_sync(0xffffffffu, mbar_wait(&s_full[m], (uint32_t)j & 1u, abort_flag, p.err, ERR_S));
       if (!ok) break;
       tcgen05_fence_after();
@@ -274,31 +242,25 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
 #pragma unroll
         for (int i = 0; i < 32; ++i) s[ch * 32 + i] = __uint_as_float(raw[i]);
       }
-      const int col0 = raw ? base + raw0 + (j - n_code) * BKV : first_key(j);
-      const int hi = j < kept_blocks ? (Q8 ? min(seen.kept, own) : seen.kept) - 1 : (Q8 && !raw ? own - 1 : qpos);
-      const int from = raw ? max(lo, own) : lo, keep = raw && own >= p.keep_first ? 0 : p.keep_first;
-      if (col0 + BKV - 1 > hi || (col0 < from && col0 + BKV > keep) || (raw && col0 < own)) {
+      const int col0 = first_key(j), hi = j < kept_blocks ? seen.kept - 1 : qpos;
+      if (col0 + BKV - 1 > hi || (col0 < lo && col0 + BKV > p.keep_first)) {
 #pragma unroll
         for (int i = 0; i < BKV; ++i)
-          if (col0 + i > hi || (col0 + i < from && (col0 + i >= keep || (raw && col0 + i < own)))) s[i] = -INFINITY;
+          if (col0 + i > hi || (col0 + i < lo && col0 + i >= p.keep_first)) s[i] = -INFINITY;
       }
-      float m_half[2] = {-INFINITY, -INFINITY};
+      float m_blk = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < BKV; ++i) m_half[Q8 ? i / Q8_BLOCK : 0] = fmaxf(m_half[Q8 ? i / Q8_BLOCK : 0], s[i]);
-      // a half without visible keys has no maximum, whatever its factor
-      const float m_blk = Q8 ? fmaxf(m_half[0] == -INFINITY ? -INFINITY : m_half[0] * ch[0], m_half[1] == -INFINITY ? -INFINITY : m_half[1] * ch[1])
-                             : m_half[0];
-      const float unit = Q8 ? 1.f : c;
+      for (int i = 0; i < BKV; ++i) m_blk = fmaxf(m_blk, s[i]);
       // the reference maximum moves (and O, l are rescaled) only when the exponent would exceed 2^8
-      const bool move = m_blk > -INFINITY && (mx == -INFINITY || (m_blk - mx) * unit > 8.f);
+      const bool move = m_blk > -INFINITY && (mx == -INFINITY || (m_blk - mx) * c > 8.f);
       const float m_new = move ? m_blk : mx;
       const float m_use = m_new == -INFINITY ? 0.f : m_new;  // a row without a visible key yet keeps weight 0
-      const float alpha = (move && mx != -INFINITY) ? fast_exp2((mx - m_use) * unit) : 1.f;
-      const float mc = m_use * unit;
+      const float alpha = (move && mx != -INFINITY) ? fast_exp2((mx - m_use) * c) : 1.f;
+      const float mc = m_use * c;
       float sum = 0.f;
 #pragma unroll
       for (int i = 0; i < BKV; ++i) {
-        s[i] = fast_exp2(fmaf(s[i], ch[Q8 ? i / Q8_BLOCK : 0], -mc));
+        s[i] = fast_exp2(fmaf(s[i], c, -mc));
         sum += s[i];
       }
       l = l * alpha + sum;
@@ -365,51 +327,22 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   }
 }
 
-// What Q8 adds: raw lists (B, G, raw_rows, dim | vdim)
-struct WindowRaw { const void *k, *v; };
-
-template <int DK, int VD, bool Q8>
-int launch(const void* qn, const void* kc, const void* vc, const WindowRaw& raw, const WindowParams& p, int B, cudaStream_t s) {
+template <int DK, int VD>
+int launch(const void* qn, const void* kc, const void* vc, const WindowParams& p, int B, cudaStream_t s) {
   using L = WindowSmem<DK, VD>;
-  CUtensorMap mq, mk, mv, mrk, mrv;
+  CUtensorMap mq, mk, mv;
   int r = make_map_bf16(&mq, qn, (long long)B * p.T * p.H, p.dim, p.dim, TILE_M);
   if (r) return r;
   r = make_map_bf16(&mk, kc, (long long)B * p.G * p.Smax, p.dim, p.dim, BKV);
   if (r) return r;
   r = make_map_bf16(&mv, vc, (long long)B * p.G * p.Smax, p.vdim, p.vdim, 64);
   if (r) return r;
-  mrk = mk;
-  mrv = mv;
-  if (Q8) {
-    r = make_map_bf16(&mrk, raw.k, (long long)B * p.G * p.raw_rows, p.dim, p.dim, BKV);
-    if (r) return r;
-    r = make_map_bf16(&mrv, raw.v, (long long)B * p.G * p.raw_rows, p.vdim, p.vdim, 64);
-    if (r) return r;
-  }
   static XlPerDevice smem;
-  XL_TRY(xl_allow_smem(window_attn_tcgen05_kernel<DK, VD, Q8>, L::TOTAL, smem));
+  XL_TRY(xl_allow_smem(window_attn_tcgen05_kernel<DK, VD>, L::TOTAL, smem));
   const long long rows = (long long)p.T * (p.H / p.G);
   const dim3 grid(p.G, (unsigned)((rows + 2 * TILE_M - 1) / (2 * TILE_M)), B);
-  window_attn_tcgen05_kernel<DK, VD, Q8><<<grid, NUM_THREADS, L::TOTAL, s>>>(mq, mk, mv, mrk, mrv, p);
+  window_attn_tcgen05_kernel<DK, VD><<<grid, NUM_THREADS, L::TOTAL, s>>>(mq, mk, mv, p);
   return (int)cudaGetLastError();
-}
-
-// arguments that the kernel takes; Smax: rows of a head in the lists of keys and values
-bool takes(const void* qn, const void* kc, const void* vc, const void* gate, long long ldg, const void* out, long long ldo, int B, int T,
-           int H, int G, int dim, int vdim, long long Smax, int window, int keep_first, float scale) {
-  if (B < 1 || B > 65535 || T < 1 || G < 1 || H < 1 || H % G || Smax < 1 || window < 0 || keep_first < 0) return false;
-  if (dim < 8 || dim > 128 || dim % 8 || vdim < 8 || vdim > 128 || vdim % 8 || ldo % 8 || ldo < (long long)H * vdim ||
-      (gate && (ldg % 8 || ldg < (long long)H * vdim)))
-    return false;
-  if ((((uintptr_t)qn) | ((uintptr_t)kc) | ((uintptr_t)vc) | ((uintptr_t)gate) | ((uintptr_t)out)) & 15) return false;
-  return scale > 0.f && (long long)B * G * Smax <= 0x7fffffffLL - 2 * BKV && (long long)B * T * H <= 0x7fffffffLL - 4 * TILE_M &&
-         ((long long)T * (H / G) + 2 * TILE_M - 1) / (2 * TILE_M) <= 65535;
-}
-
-template <bool Q8>
-int launch_sizes(const void* qn, const void* kc, const void* vc, const WindowRaw& raw, const WindowParams& p, int B, cudaStream_t s) {
-  if (p.dim <= 64) return p.vdim <= 64 ? launch<64, 64, Q8>(qn, kc, vc, raw, p, B, s) : launch<64, 128, Q8>(qn, kc, vc, raw, p, B, s);
-  return p.vdim <= 64 ? launch<128, 64, Q8>(qn, kc, vc, raw, p, B, s) : launch<128, 128, Q8>(qn, kc, vc, raw, p, B, s);
 }
 
 }  // namespace
@@ -421,27 +354,18 @@ int launch_sizes(const void* qn, const void* kc, const void* vc, const WindowRaw
 XL_API int xl_window_attn_tcgen05(const void* qn, const void* kc, const void* vc, const void* gate, long long ldg, void* out,
                                   long long ldo, const int* pos, const int* count, int B, int T, int H, int G, int dim, int vdim,
                                   int Smax, int window, int keep_first, float scale, float sink, int* err, cudaStream_t s) {
-  if (!takes(qn, kc, vc, gate, ldg, out, ldo, B, T, H, G, dim, vdim, Smax, window, keep_first, scale)) return -1;
-  WindowParams p = {};
+  if (B < 1 || B > 65535 || T < 1 || G < 1 || H < 1 || H % G || Smax < 1 || window < 0 || keep_first < 0) return -1;
+  if (dim < 8 || dim > 128 || dim % 8 || vdim < 8 || vdim > 128 || vdim % 8 || ldo % 8 || ldo < (long long)H * vdim ||
+      (gate && (ldg % 8 || ldg < (long long)H * vdim)))
+    return -1;
+  if ((((uintptr_t)qn) | ((uintptr_t)kc) | ((uintptr_t)vc) | ((uintptr_t)gate) | ((uintptr_t)out)) & 15) return -1;
+  if (!(scale > 0.f) || (long long)B * G * Smax > 0x7fffffffLL - 2 * BKV || (long long)B * T * H > 0x7fffffffLL - 4 * TILE_M ||
+      ((long long)T * (H / G) + 2 * TILE_M - 1) / (2 * TILE_M) > 65535)
+    return -1;
+  WindowParams p;
   p.pos = pos; p.count = count; p.gate = (const __nv_bfloat16*)gate; p.ldg = ldg; p.out = (__nv_bfloat16*)out; p.ldo = ldo;
   p.T = T; p.H = H; p.G = G; p.dim = dim; p.vdim = vdim; p.Smax = Smax; p.window = window; p.keep_first = keep_first;
   p.scale = scale; p.sink = sink; p.err = err;
-  return launch_sizes<false>(qn, kc, vc, {}, p, B, s);
-}
-
-// The same against a cache of 8 bits, after xl_q8_append_expand: q16 (B, G, T, H/G, dim) fp16, codes as fp16 kx (B, G, blocks * 64, dim) and
-// values as bf16 vx (.., vdim), raw rows as fp16 raw_k and bf16 raw_v (B, G, raw_rows, dim | vdim); ks (B, G, blocks) the key scales, wq
-// and wk the factors of the norms.
-XL_API int xl_q8_attn_tcgen05(const void* q16, const void* kx, const void* vx, const void* raw_k, const void* raw_v, int raw_rows,
-                              const float* ks, const float* wq, const float* wk, const void* gate, long long ldg, void* out,
-                              long long ldo, const int* pos, const int* count, int B, int T, int H, int G, int dim, int vdim,
-                              int blocks, int window, int keep_first, float scale, float sink, int* err, cudaStream_t s) {
-  const long long rows = (long long)blocks * Q8_BLOCK;
-  if (blocks < 1 || blocks > (1 << 24) || !takes(q16, kx, vx, gate, ldg, out, ldo, B, T, H, G, dim, vdim, rows, window, keep_first, scale)) return -1;
-  if (raw_rows < T + Q8_BLOCK + BKV || (long long)B * G * raw_rows > 0x7fffffffLL - 2 * BKV || (((uintptr_t)raw_k | (uintptr_t)raw_v) & 15)) return -1;
-  WindowParams p = {};
-  p.pos = pos; p.count = count; p.gate = (const __nv_bfloat16*)gate; p.ldg = ldg; p.out = (__nv_bfloat16*)out; p.ldo = ldo;
-  p.T = T; p.H = H; p.G = G; p.dim = dim; p.vdim = vdim; p.Smax = (int)rows; p.window = window; p.keep_first = keep_first;
-  p.scale = scale; p.sink = sink; p.err = err; p.ks = ks; p.wq = wq; p.wk = wk; p.blocks = blocks; p.raw_rows = raw_rows;
-  return launch_sizes<true>(q16, kx, vx, {raw_k, raw_v}, p, B, s);
+  if (dim <= 64) return vdim <= 64 ? launch<64, 64>(qn, kc, vc, p, B, s) : launch<64, 128>(qn, kc, vc, p, B, s);
+  return vdim <= 64 ? launch<128, 64>(qn, kc, vc, p, B, s) : launch<128, 128>(qn, kc, vc, p, B, s);
 }

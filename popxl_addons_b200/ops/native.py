@@ -295,7 +295,13 @@ def check_gemm_errors():
                      63: "int4 product: shared-memory stage was never released (tokens)",
                      64: "decode attention: keys and values never arrived",
                      65: "decode attention: shared-memory stage was never released",
-                     91: "attention over an 8-bit cache: codes never arrived"}
+                     91: "attention over an 8-bit cache: codes never arrived",
+                     92: "attention over an 8-bit cache: query tiles never arrived",
+                     93: "attention over an 8-bit cache: key / value block never arrived",
+                     94: "attention over an 8-bit cache: key / value stage was never released",
+                     95: "attention over an 8-bit cache: scores never completed",
+                     96: "attention over an 8-bit cache: weights never arrived",
+                     97: "attention over an 8-bit cache: output accumulation never completed"}
             raise RuntimeError(f"tcgen05 GEMM on cuda:{idx} gave up waiting: {names.get(code, code)}")
 
 

@@ -17,7 +17,7 @@ _q8_general = _sig("xl_q8_attn_general", *[_c_p] * 8, _c_ll, _c_p, _c_ll, _c_p, 
 _q8_few = _sig("xl_q8_attn_few", _c_p, _c_ll, *[_c_p] * 12, _c_ll, _c_p, _c_p, *[_c_int] * 10, _c_f, _c_f, _c_d, _c_int, _c_p, _c_p, _c_int,
                _c_p, _c_p)
 _q8_append_expand = _sig("xl_q8_append_expand", _c_p, _c_ll, *[_c_p] * 5, _c_int, *[_c_p] * 10, *[_c_int] * 9, _c_d, _c_p)
-_q8_tcgen05 = _sig("xl_q8_attn_tcgen05", *[_c_p] * 5, _c_int, *[_c_p] * 4, _c_ll, _c_p, _c_ll, _c_p, _c_p, *[_c_int] * 9, _c_f, _c_f, _c_p, _c_p)
+_q8_tcgen05 = _sig("xl_q8_attn_tcgen05", *[_c_p] * 5, _c_int, *[_c_p] * 5, _c_ll, _c_p, _c_ll, _c_p, _c_p, *[_c_int] * 9, _c_f, _c_f, _c_p, _c_p)
 _adapter_down = _sig("xl_adapter_down", *[_c_p] * 5, _c_ll, *[_c_int] * 5, _c_p)
 _adapter_up = _sig("xl_adapter_up", *[_c_p] * 5, _c_ll, *[_c_int] * 6, _c_p)
 _adapter_down_mma = _sig("xl_adapter_down_mma", *[_c_p] * 5, _c_ll, *[_c_int] * 5, _c_p)
@@ -115,7 +115,7 @@ def _q8_portion(at, proj, q_norm, k_norm, cache, pos, count, joint, gate, T, hea
     """A portion of the sequences `at` on the tensor cores: append, codes of visible blocks as 16-bit numbers, attention."""
     cache, pos, count = tuple(t[at] for t in cache), pos[at], count[at]
     B, G, blocks, _, dim = cache[0].shape
-    vdim, dev, rows = cache[1].shape[-1], proj.device, T + 192
+    vdim, dev, rows = cache[1].shape[-1], proj.device, T + 128
     ld, ldo, row0 = proj.stride(0), joint.stride(0), at.start * T
     q = torch.empty((B, G, T, heads // G, dim), dtype=torch.float16, device=dev)
     raw_k = torch.empty((B, G, rows, dim), dtype=torch.float16, device=dev)
@@ -128,7 +128,7 @@ def _q8_portion(at, proj, q_norm, k_norm, cache, pos, count, joint, gate, T, hea
                            vx.data_ptr(), *map(_ptr, cache), *where, *sizes, eps, s)
     _done(rc, "q8_append_expand")
     _count("q8_expand")
-    rc = _q8_tcgen05(q.data_ptr(), kx.data_ptr(), vx.data_ptr(), raw_k.data_ptr(), raw_v.data_ptr(), rows, cache[2].data_ptr(), *norms,
+    rc = _q8_tcgen05(q.data_ptr(), kx.data_ptr(), vx.data_ptr(), raw_k.data_ptr(), raw_v.data_ptr(), rows, cache[2].data_ptr(), cache[3].data_ptr(), *norms,
                      gate + row0 * ld * 2 if gate else None, ld, joint.data_ptr() + row0 * ldo * 2, ldo, *where, *sizes, scale, sink,
                      gemm_error_flag(dev).data_ptr(), s)
     _done(rc, "q8_attn_tcgen05")
@@ -173,7 +173,7 @@ def window_attention_q8_cuda(proj, q_norm, k_norm, k, v, k_scale, v_scale, k_tai
             and T * heads <= 1 << 22 and G * blocks * 64 * (dim + vdim) * 2 <= _Q8_EXPANDED):
         # as many sequences at a time as expand to what is set aside for it
         step = max(1, _Q8_EXPANDED // (G * blocks * 64 * (dim + vdim) * 2))
-        step = min(step, (1 << 30) // (G * (T + 192)) + 1, (1 << 30) // (T * heads) + 1)
+        step = min(step, (1 << 30) // (G * (T + 128)) + 1, (1 << 30) // (T * heads) + 1)
         for b in range(0, B, step):
             _q8_portion(slice(b, min(B, b + step)), proj, q_norm, k_norm, (k, v, k_scale, v_scale, k_tail, v_tail), pos, count, joint, gate, T,
                         heads, window, keep_first, scale, sink, eps, s)
