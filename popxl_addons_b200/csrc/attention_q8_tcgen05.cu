@@ -71,6 +71,29 @@ __device__ __forceinline__ uint64_t pair_add(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
+// Descriptors of 128-byte-swizzled tiles (see make_smem_desc) in two words: the upper one is the same for all of them, in the lower one
+// an offset inside a tile is an addition. Building each of a block's 24 descriptors from its address kept the one issuing thread busy
+// for longer than the softmax takes.
+constexpr uint32_t DESC_HI = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t lbo_bytes) { return ((addr & 0x3FFFFu) >> 4) | ((lbo_bytes >> 4) << 16); }
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}"
+      ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(DESC_HI), "r"(idesc), "r"((uint32_t)accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "mov.b64 b, {%2, %3};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}"
+      ::"r"(d), "r"(a), "r"(b_lo), "r"(DESC_HI), "r"(idesc), "r"((uint32_t)accumulate)
+      : "memory");
+}
 // whether the barrier has flipped, without waiting
 __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
@@ -224,28 +247,28 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       // Whatever can go next goes next: the scores of a tile once the product two blocks before has taken the weights from their buffer, a
       // product once its weights are there. Issued in a fixed order, with a wait for that product before the scores, two tiles took 3000
       // cycles per block, of which the softmax warps worked 1500.
+      const uint32_t q_desc = desc_lo(smem_u32(sQ), 16), k_desc = desc_lo(smem_u32(sK), 16), v_desc = desc_lo(smem_u32(sV), BKV * 128);
       int scored[2] = {0, 0}, taken[2] = {0, 0};  // blocks whose scores, whose products have been issued
       auto issue_scores = [&](int m) {
         const int j = scored[m]++, st = j % L::K_STAGES, buf = 2 * m + (j & 1);
         tcgen05_fence_after();
-        const uint32_t q_addr = smem_u32(sQ + m * L::Q_BYTES), k_addr = smem_u32(sK + st * L::K_BYTES);
+        const uint32_t q_lo = q_desc + m * (L::Q_BYTES >> 4), k_lo = k_desc + st * (L::K_BYTES >> 4);
 #pragma unroll
         for (int kb = 0; kb < DK / 64; ++kb)
 #pragma unroll
           for (int k = 0; k < 64 / UMMA_K; ++k)
-            tcgen05_mma_f16(tmem_base + buf * BKV, make_smem_desc(q_addr + kb * (TILE_M * 128) + k * (UMMA_K * 2), 16),
-                            make_smem_desc(k_addr + kb * (BKV * 128) + k * (UMMA_K * 2), 16), idesc_s, (kb | k) ? 1u : 0u);
+            mma_ss(tmem_base + buf * BKV, q_lo + ((kb * (TILE_M * 128) + k * (UMMA_K * 2)) >> 4),
+                   k_lo + ((kb * (BKV * 128) + k * (UMMA_K * 2)) >> 4), idesc_s, (kb | k) != 0);
         if (tiles == 1 || scored[1 - m] > j) tcgen05_commit(&k_empty[st]);  // the last reader of the block
         tcgen05_commit(&s_full[buf]);
       };
       auto issue_product = [&](int m) {
         const int j = taken[m]++, st = j % L::V_STAGES, buf = 2 * m + (j & 1);
         tcgen05_fence_after();
-        const uint32_t v_addr = smem_u32(sV + st * L::V_BYTES);
+        const uint32_t v_lo = v_desc + st * (L::V_BYTES >> 4);
 #pragma unroll
         for (int k = 0; k < BKV / UMMA_K; ++k)
-          tcgen05_mma_f16_ts(tmem_base + 4 * BKV + m * VD, tmem_base + buf * BKV + k * (UMMA_K / 2),
-                             make_smem_desc(v_addr + k * (UMMA_K * 128), BKV * 128), idesc_o, (j | k) ? 1u : 0u);
+          mma_ts(tmem_base + 4 * BKV + m * VD, tmem_base + buf * BKV + k * (UMMA_K / 2), v_lo + ((k * (UMMA_K * 128)) >> 4), idesc_o, (j | k) != 0);
         if (tiles == 1 || taken[1 - m] > j) tcgen05_commit(&v_empty[st]);
         tcgen05_commit(&pv_done[buf]);
       };
