@@ -6,7 +6,7 @@
 // of the windows, then the raw rows of the portion from the start of the block in progress. A query sees raw rows of its own block and
 // codes of earlier blocks; which is which is a mask like any other.
 //   warp 0       TMA producer : both query tiles once, key blocks (lane 0) and value blocks (lane 1) through rings
-//   warp 1       MMA issuer   : S_m = Q_m K^T into TMEM, then O_m += P_m V
+//   warps 1, 10  MMA issuers  : of a tile each, S_m = Q_m K^T into TMEM, O_m += P_m V
 //   warps 2..5   softmax of tile 0, warps 6..9 of tile 1: one thread per row; running maximum and sum in fp32 start with the
 //                               sink, lazy rescaling of O_m in TMEM
 // Codes are fp16 keys and bf16 values, both exact: the scale of a block multiplies the scores, that of its values the weights, which are
@@ -14,8 +14,9 @@
 // units of a power of two above their norm's factors.
 //
 // What bounds it is the chain of a tile: scores, softmax, weights, product. A tile has two buffers of scores of 64 keys each, so that the next
-// scores are there when a softmax ends; with one buffer of 128 keys a tile's warps waited 1700 of 4500 cycles per 128 keys for the tensor
-// core's answer (clock stamps; 2 x 515 tokens after 6000, 32 heads on 8: 171 us). The softmax takes a block's scores into registers at
+// scores are there when a softmax ends, and an issuer of its own, so that no tile's products wait behind what holds up the other's: with one
+// buffer of 128 keys a tile's warps waited 1700 of 4500 cycles per 128 keys for the tensor core's answer, with one issuer for both tiles, in
+// a fixed order or going by what is ready, 1500 of 3000 cycles per 64 keys (clock stamps; 2 x 515 tokens after 6000, 32 heads on 8). The softmax takes a block's scores into registers at
 // once and works on pairs of fp32 numbers (fma.rn.f32x2); its exponentials alone occupy the special-function unit half of the time.
 // Expanding codes outside this kernel moves five bytes per code once per portion, where every CTA would convert every block again next to a
 // softmax that fills the issue slots.
@@ -30,7 +31,7 @@ namespace {
 constexpr int TILE_M = 128;
 constexpr int BKV = Q8_BLOCK;
 constexpr int UMMA_K = 16;
-constexpr int NUM_THREADS = 64 + 2 * 128;
+constexpr int NUM_THREADS = 96 + 2 * 128;
 constexpr uint32_t TMEM_COLS = 512;
 
 enum { ERR_Q = 92, ERR_KV_FULL = 93, ERR_KV_EMPTY = 94, ERR_S = 95, ERR_P = 96, ERR_PV = 97 };
@@ -93,18 +94,6 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b_lo, ui
       "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}"
       ::"r"(d), "r"(a), "r"(b_lo), "r"(DESC_HI), "r"(idesc), "r"((uint32_t)accumulate)
       : "memory");
-}
-// whether the barrier has flipped, without waiting
-__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return ok != 0;
 }
 // bits a .. b - 1 of a word, whatever lies outside it
 __device__ __forceinline__ uint32_t bits_of(int a, int b) {
@@ -170,9 +159,9 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     mbar_init(q_full, 1);
     for (int s = 0; s < 6; ++s) {
       mbar_init(&k_full[s], 1);
-      mbar_init(&k_empty[s], 1);
+      mbar_init(&k_empty[s], tiles);
       mbar_init(&v_full[s], 1);
-      mbar_init(&v_empty[s], 1);
+      mbar_init(&v_empty[s], tiles);
     }
     for (int s = 0; s < 4; ++s) {
       mbar_init(&s_full[s], 1);
@@ -238,65 +227,47 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           for (uint32_t i = 0; i < MBAR_SPIN_LIMIT && !mbar_try_wait(&full[j % stages], (uint32_t)(j / stages) & 1u); ++i) {}
       }
     }
-  } else if (warp == 1) {
-    if (elect_one()) {
+  } else if (warp == 1 || warp == 10) {
+    const int m = warp == 1 ? 0 : 1;  // row tile whose products this warp issues
+    if (m < tiles && elect_one()) {
       // fp32 accumulators. S: fp16, both K-major, N = BKV. O: bf16, A (P) from TMEM, B (V) MN-major (bit 16), N = VD.
       const uint32_t idesc_s = (1u << 4) | ((uint32_t)(BKV >> 3) << 17) | ((uint32_t)(TILE_M >> 4) << 24);
       const uint32_t idesc_o = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(VD >> 3) << 17) |
                                ((uint32_t)(TILE_M >> 4) << 24);
-      // Whatever can go next goes next: the scores of a tile once the product two blocks before has taken the weights from their buffer, a
-      // product once its weights are there. Issued in a fixed order, with a wait for that product before the scores, two tiles took 3000
-      // cycles per block, of which the softmax warps worked 1500.
-      const uint32_t q_desc = desc_lo(smem_u32(sQ), 16), k_desc = desc_lo(smem_u32(sK), 16), v_desc = desc_lo(smem_u32(sV), BKV * 128);
-      int scored[2] = {0, 0}, taken[2] = {0, 0};  // blocks whose scores, whose products have been issued
-      auto issue_scores = [&](int m) {
-        const int j = scored[m]++, st = j % L::K_STAGES, buf = 2 * m + (j & 1);
+      const uint32_t q_lo = desc_lo(smem_u32(sQ + m * L::Q_BYTES), 16), k_desc = desc_lo(smem_u32(sK), 16),
+                     v_desc = desc_lo(smem_u32(sV), BKV * 128);
+      bool ok = mbar_wait(q_full, 0, abort_flag, p.err, ERR_Q);
+      auto issue_scores = [&](int j) -> bool {
+        const int st = j % L::K_STAGES, buf = 2 * m + (j & 1);
+        if (!mbar_wait(&k_full[st], (uint32_t)(j / L::K_STAGES) & 1u, abort_flag, p.err, ERR_KV_FULL)) return false;
+        // the buffer still holds P of the block before the last one until its product has been taken
+        if (j > 1 && !mbar_wait(&pv_done[buf], (uint32_t)((j - 2) >> 1) & 1u, abort_flag, p.err, ERR_PV)) return false;
         tcgen05_fence_after();
-        const uint32_t q_lo = q_desc + m * (L::Q_BYTES >> 4), k_lo = k_desc + st * (L::K_BYTES >> 4);
+        const uint32_t k_lo = k_desc + st * (L::K_BYTES >> 4);
 #pragma unroll
         for (int kb = 0; kb < DK / 64; ++kb)
 #pragma unroll
           for (int k = 0; k < 64 / UMMA_K; ++k)
             mma_ss(tmem_base + buf * BKV, q_lo + ((kb * (TILE_M * 128) + k * (UMMA_K * 2)) >> 4),
                    k_lo + ((kb * (BKV * 128) + k * (UMMA_K * 2)) >> 4), idesc_s, (kb | k) != 0);
-        if (tiles == 1 || scored[1 - m] > j) tcgen05_commit(&k_empty[st]);  // the last reader of the block
+        tcgen05_commit(&k_empty[st]);
         tcgen05_commit(&s_full[buf]);
+        return true;
       };
-      auto issue_product = [&](int m) {
-        const int j = taken[m]++, st = j % L::V_STAGES, buf = 2 * m + (j & 1);
+      for (int j = 0; j < min(2, n_kv) && ok; ++j) ok = issue_scores(j);
+      for (int j = 0; j < n_kv && ok; ++j) {
+        const int st = j % L::V_STAGES, buf = 2 * m + (j & 1);
+        ok = mbar_wait(&v_full[st], (uint32_t)(j / L::V_STAGES) & 1u, abort_flag, p.err, ERR_KV_FULL) &&
+             mbar_wait(&p_full[buf], (uint32_t)(j >> 1) & 1u, abort_flag, p.err, ERR_P);
+        if (!ok) break;
         tcgen05_fence_after();
         const uint32_t v_lo = v_desc + st * (L::V_BYTES >> 4);
 #pragma unroll
         for (int k = 0; k < BKV / UMMA_K; ++k)
           mma_ts(tmem_base + 4 * BKV + m * VD, tmem_base + buf * BKV + k * (UMMA_K / 2), v_lo + ((k * (UMMA_K * 128)) >> 4), idesc_o, (j | k) != 0);
-        if (tiles == 1 || taken[1 - m] > j) tcgen05_commit(&v_empty[st]);
+        tcgen05_commit(&v_empty[st]);
         tcgen05_commit(&pv_done[buf]);
-      };
-      bool ok = mbar_wait(q_full, 0, abort_flag, p.err, ERR_Q);
-      uint32_t idle = 0;  // rounds since something was issued
-      while (ok && (taken[0] < n_kv || (tiles == 2 && taken[1] < n_kv))) {
-        ++idle;
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {
-          if (m >= tiles) break;
-          int j = taken[m];
-          if (j < scored[m] && mbar_test(&p_full[2 * m + (j & 1)], (uint32_t)(j >> 1) & 1u) &&
-              mbar_test(&v_full[j % L::V_STAGES], (uint32_t)(j / L::V_STAGES) & 1u)) {
-            issue_product(m);
-            idle = 0;
-          }
-          j = scored[m];
-          if (j < n_kv && (j < 2 || (taken[m] > j - 2 && mbar_test(&pv_done[2 * m + (j & 1)], (uint32_t)((j - 2) >> 1) & 1u))) &&
-              mbar_test(&k_full[j % L::K_STAGES], (uint32_t)(j / L::K_STAGES) & 1u)) {
-            issue_scores(m);
-            idle = 0;
-          }
-        }
-        if (idle >= MBAR_SPIN_LIMIT || ((idle & 1023u) == 1023u && *abort_flag)) {
-          ok = false;
-          *abort_flag = 1;
-          if (p.err) atomicCAS(p.err, 0, ERR_P);
-        }
+        if (j + 2 < n_kv) ok = issue_scores(j + 2);
       }
     }
   } else if ((warp < 6 ? 0 : 1) < tiles) {
