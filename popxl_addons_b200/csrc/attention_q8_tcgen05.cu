@@ -9,8 +9,9 @@
 //   warps 1, 10  MMA issuers  : of a tile each, S_m = Q_m K^T into TMEM, O_m += P_m V
 //   warps 2..5   softmax of tile 0, warps 6..9 of tile 1: one thread per row; running maximum and sum in fp32 start with the
 //                               sink, lazy rescaling of O_m in TMEM
-// Codes are fp16 keys and bf16 values, both exact: the scale of a block multiplies the scores, that of its values the weights, which are
-// then rounded once to bf16 (2^-9 of each at most, in no common direction) and replace S in TMEM. Queries and raw keys are fp16 in
+// Codes are fp16 keys and bf16 values, both exact: the scale of a block multiplies the scores, that of its values the weights, which
+// replace S in TMEM as two bf16 numbers each (value and rounding error): rounded once to bf16 they would add as much error as the
+// rounding of the result does. Queries and raw keys are fp16 in
 // units of a power of two above their norm's factors.
 //
 // What bounds it is the chain of a tile: scores, softmax, weights, product. A tile has two buffers of scores of 64 keys each, so that the next
@@ -263,8 +264,11 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         tcgen05_fence_after();
         const uint32_t v_lo = v_desc + st * (L::V_BYTES >> 4);
 #pragma unroll
-        for (int k = 0; k < BKV / UMMA_K; ++k)
-          mma_ts(tmem_base + 4 * BKV + m * VD, tmem_base + buf * BKV + k * (UMMA_K / 2), v_lo + ((k * (UMMA_K * 128)) >> 4), idesc_o, (j | k) != 0);
+        for (int part = 0; part < 2; ++part)  // rounded weights, then their rounding errors
+#pragma unroll
+          for (int k = 0; k < BKV / UMMA_K; ++k)
+            mma_ts(tmem_base + 4 * BKV + m * VD, tmem_base + buf * BKV + part * (BKV / 2) + k * (UMMA_K / 2),
+                   v_lo + ((k * (UMMA_K * 128)) >> 4), idesc_o, (j | part | k) != 0);
         tcgen05_commit(&v_empty[st]);
         tcgen05_commit(&pv_done[buf]);
         if (j + 2 < n_kv) ok = issue_scores(j + 2);
@@ -277,7 +281,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     const long long f = f0 + m * TILE_M + r;  // (token, head of the group)
     const int t = (int)(f / R), hh = (int)(f - (long long)t * R);
     const int qpos = pos + t, own = qpos / BKV * BKV;
-    const int lo = window_range(qpos, p.window, 0).first;
+    const int lo = window_range(qpos, p.window, 0).first, lo_last = window_range(p_last, p.window, 0).first;
     const uint32_t lane_base = (uint32_t)(qtr * 32) << 16;
     const uint32_t tmem_o = tmem_base + lane_base + 4 * BKV + m * VD;
     const float unit_q = q8_norm_unit(p.wq, p.dim, lane), unit_k = q8_norm_unit(p.wk, p.dim, lane);
@@ -305,12 +309,15 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       const float fs = fmaxf(c * ch, 1e-37f), fv = fminf(vh, 1e37f);
       if (j + 1 < n_kv) ask(j + 1);
       // keys that the row sees: of a raw block its own, of codes the earlier ones; its window, and the kept first tokens
-      const int col0 = block_of(j) * BKV, first = raw ? own : 0, end = raw ? qpos + 1 : own, from = max(lo, first);
-      uint32_t vis[2];
+      const int blk = block_of(j), col0 = blk * BKV;
+      uint32_t vis[2] = {0xffffffffu, 0xffffffffu};
+      if (raw || blk >= own_first || (col0 < lo_last && col0 + BKV > p.keep_first)) {  // else every row of this CTA sees all of it
+        const int first = raw ? own : 0, end = raw ? qpos + 1 : own, from = max(lo, first);
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const int at = col0 + k * 32;
-        vis[k] = bits_of(from - at, end - at) | bits_of(first - at, min(p.keep_first, end) - at);
+        for (int k = 0; k < 2; ++k) {
+          const int at = col0 + k * 32;
+          vis[k] = bits_of(from - at, end - at) | bits_of(first - at, min(p.keep_first, end) - at);
+        }
       }
       const uint32_t tmem_s = tmem_base + lane_base + buf * BKV;
       ok = mbar_wait_warp(&s_full[buf], (uint32_t)(j >> 1) & 1u, abort_flag, p.err, ERR_S);
@@ -338,20 +345,24 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       const float m_use = m_new == -INFINITY ? 0.f : m_new;  // a row without a visible key yet keeps weight 0
       const float alpha = (move && mx != -INFINITY) ? fast_exp2(mx - m_use) : 1.f;
       uint64_t sums[2] = {0, 0};
-      const uint64_t f2 = pair_of(fs, fs), v2 = pair_of(fv, fv), m2 = pair_of(-m_use, -m_use);
+      const uint64_t f2 = pair_of(fs, fs), v2 = pair_of(fv, fv), m2 = pair_of(-m_use, -m_use), minus_one = pair_of(-1.f, -1.f);
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        uint32_t w[16];
+        uint32_t w[16], err[16];  // rounded weights, their rounding errors
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           float x, y;
           halves_of(pair_fma(pair_of(__uint_as_float(s[k][2 * i]), __uint_as_float(s[k][2 * i + 1])), f2, m2), x, y);
           const uint64_t e2 = pair_of(fast_exp2(x), fast_exp2(y));
           sums[i & 1] = pair_add(sums[i & 1], e2);
-          halves_of(pair_mul(e2, v2), x, y);
+          const uint64_t x2 = pair_mul(e2, v2);
+          halves_of(x2, x, y);
           asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[i]) : "f"(y), "f"(x));
+          halves_of(pair_fma(pair_of(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u)), minus_one, x2), x, y);
+          asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(err[i]) : "f"(y), "f"(x));
         }
         tmem_st_32x32b_x16(tmem_s + k * 16, w);
+        tmem_st_32x32b_x16(tmem_s + BKV / 2 + k * 16, err);
       }
       float x, y;
       halves_of(pair_add(sums[0], sums[1]), x, y);

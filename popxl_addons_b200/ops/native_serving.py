@@ -107,8 +107,14 @@ def _q8_slices(units, longest, per_sm, device) -> int:
     return min(most, (longest + 383) // 384, 64)
 
 
-_Q8_FEW_ROWS = 64       # rows per sequence and key head up to which portions run on mma.sync
 _Q8_EXPANDED = 2 << 30  # bytes that the codes of a portion may expand to at a time
+
+
+def _q8_few_rows(rows: int, positions: int) -> bool:
+    """Whether a portion of `rows` rows per sequence and key head, against a cache of `positions`, runs on mma.sync, which cuts the keys among
+    CTAs and reads codes once, and not on the tensor cores, whose keys expand first (2 sequences x 8 key heads of 128 after 6000: 16 rows
+    107 us there, 35 here, 64 rows 113 and 58, 128 rows 117 and 83; 6 x 4 heads after 500: 64 rows 37 and 35, 128 rows 39 and 45)."""
+    return rows <= 64 or (rows <= 128 and positions >= 4096)
 
 
 def _q8_portion(at, proj, q_norm, k_norm, cache, pos, count, joint, gate, T, heads, window, keep_first, scale, sink, eps, s):
@@ -167,9 +173,10 @@ def window_attention_q8_cuda(proj, q_norm, k_norm, k, v, k_scale, v_scale, k_tai
                      eps, splits, _ptr(part), done.data_ptr(), int(ahead), gemm_error_flag(dev).data_ptr(), s)
         return _launched(rc, "q8_attn_few")
 
+    is_few = _q8_few_rows(T * (heads // G), blocks * 64)
     if T == 1 and dt == torch.bfloat16 and few(None, (None, None), read_ahead.allowed(pos, count, k, v, k_scale, v_scale, k_tail, v_tail)):
         return joint
-    if (dt == torch.bfloat16 and T * (heads // G) > _Q8_FEW_ROWS and dim <= 128 and vdim <= 128 and dim % 8 == vdim % 8 == ld % 8 == ldo % 8 == 0
+    if (dt == torch.bfloat16 and not is_few and dim <= 128 and vdim <= 128 and dim % 8 == vdim % 8 == ld % 8 == ldo % 8 == 0
             and T * heads <= 1 << 22 and G * blocks * 64 * (dim + vdim) * 2 <= _Q8_EXPANDED):
         # as many sequences at a time as expand to what is set aside for it
         step = max(1, _Q8_EXPANDED // (G * blocks * 64 * (dim + vdim) * 2))
@@ -184,7 +191,7 @@ def window_attention_q8_cuda(proj, q_norm, k_norm, k, v, k_scale, v_scale, k_tai
                     k_tail.data_ptr(), v_tail.data_ptr(), pos.data_ptr(), count.data_ptr(), B, T, heads, G, dim, vdim, blocks, eps, code, s)
     if not _launched(rc, "q8_append"):
         return NotImplemented
-    if dt == torch.bfloat16 and T * (heads // G) <= _Q8_FEW_ROWS and few(q, raw, False):
+    if dt == torch.bfloat16 and is_few and few(q, raw, False):
         return joint
     rc = _q8_general(q.data_ptr(), raw[0].data_ptr(), raw[1].data_ptr(), *cache, gate, ld, joint.data_ptr(), ldo, pos.data_ptr(),
                      count.data_ptr(), B, T, heads, G, dim, vdim, blocks, window, keep_first, scale, sink, code, s)
