@@ -460,18 +460,30 @@ __device__ __forceinline__ Q8Ranges q8_ranges(int p, int window, int keep_first)
   return {seen.kept, seen.first, p / Q8_BLOCK * Q8_BLOCK};
 }
 
+// four codes of a word as fp32: the byte c + 128 under 2^23, less 2^23 + 128 (a conversion instruction runs at a quarter of this rate)
+__device__ __forceinline__ void q8_floats(uint32_t w, float (&x)[4]) {
+  w ^= 0x80808080u;
+  x[0] = __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7540)) - 8388736.f;
+  x[1] = __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7541)) - 8388736.f;
+  x[2] = __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7542)) - 8388736.f;
+  x[3] = __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7543)) - 8388736.f;
+}
 // dot product of n values in shared memory with a row of codes
 __device__ __forceinline__ float q8_row_dot(const float* a, const int8_t* row, int n) {
   float s = 0.f;
   if ((n & 3) == 0 && (((uintptr_t)row) & 3) == 0) {
+    float t[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
     for (int d = 0; d < n; d += 4) {
-      const char4 c = *reinterpret_cast<const char4*>(row + d);
-      s = fmaf(a[d], (float)c.x, s);
-      s = fmaf(a[d + 1], (float)c.y, s);
-      s = fmaf(a[d + 2], (float)c.z, s);
-      s = fmaf(a[d + 3], (float)c.w, s);
+      float x[4];
+      q8_floats(*reinterpret_cast<const uint32_t*>(row + d), x);
+      const float4 q = *reinterpret_cast<const float4*>(a + d);
+      t[0] = fmaf(q.x, x[0], t[0]);
+      t[1] = fmaf(q.y, x[1], t[1]);
+      t[2] = fmaf(q.z, x[2], t[2]);
+      t[3] = fmaf(q.w, x[3], t[3]);
     }
+    s = (t[0] + t[1]) + (t[2] + t[3]);
   } else {
     for (int d = 0; d < n; ++d) s = fmaf(a[d], (float)row[d], s);
   }
@@ -494,7 +506,8 @@ struct Q8AttnParams {
 
 // SPLIT 1: a warp per query row, four of them per CTA. SPLIT 8: a CTA per query row whose warps take its blocks of 32 keys in turn
 // and merge their parts of the softmax in shared memory, for the few rows of a decoding step.
-template <typename T, int VPL, int SPLIT>  // VPL: value features per lane
+// VPL: value features per lane. WIDE: four neighbours at a time, for value rows of whole words; else one of each 32.
+template <typename T, int VPL, int SPLIT, bool WIDE>
 __global__ void __launch_bounds__(SPLIT == 1 ? 128 : SPLIT * 32) q8_attn_general_kernel(const Q8AttnParams p) {
   constexpr int ROWS = SPLIT == 1 ? 4 : 1;
   __shared__ __align__(16) float sq[ROWS][Q8_MAX_DIM];
@@ -518,12 +531,16 @@ __global__ void __launch_bounds__(SPLIT == 1 ? 128 : SPLIT * 32) q8_attn_general
   const float *ks = p.ks + head * p.blocks, *vs = p.vs + head * p.blocks;
   const T* kr = (const T*)p.raw_k + head * (p.T + Q8_BLOCK) * p.dim;
   const T* vr = (const T*)p.raw_v + head * (p.T + Q8_BLOCK) * p.vdim;
+  auto feature = [&](int e) { return WIDE ? (e / 4 * 32 + lane) * 4 + (e & 3) : lane + 32 * e; };
   float o[VPL], mx = part ? -INFINITY : p.sink, l = part || p.sink == -INFINITY ? 0.f : 1.f;  // the sink is the first part's
 #pragma unroll
   for (int e = 0; e < VPL; ++e) o[e] = 0.f;
+  int groups = 0;
   auto walk = [&](int begin, int end, auto is_raw) {
     constexpr bool RAW = decltype(is_raw)::value;
-    for (int j0 = begin + part * 32; j0 < end; j0 += 32 * SPLIT) {
+    const int mine = (part - groups % SPLIT + SPLIT) % SPLIT;  // the warps take the groups of all ranges in turn
+    groups += max(0, (end - begin + 31) / 32);
+    for (int j0 = begin + mine * 32; j0 < end; j0 += 32 * SPLIT) {
       const int j = j0 + lane;
       float s = -INFINITY;
       if (j < end) {
@@ -542,12 +559,31 @@ __global__ void __launch_bounds__(SPLIT == 1 ? 128 : SPLIT * 32) q8_attn_general
 #pragma unroll 8
       for (int k = 0; k < m; ++k) {
         const float wk = __shfl_sync(0xffffffffu, wv, k);
+        const T* row_r = vr + (long long)(j0 + k - base) * p.vdim;
+        const int8_t* row_c = vc + (long long)(j0 + k) * p.vdim;
+        if (WIDE) {
 #pragma unroll
-        for (int e = 0; e < VPL; ++e) {
-          const int c = lane + 32 * e;
-          if (c < p.vdim)
-            o[e] = fmaf(wk, RAW ? xl_to_float(vr[(long long)(j0 + k - base) * p.vdim + c]) : (float)vc[(long long)(j0 + k) * p.vdim + c],
-                        o[e]);
+          for (int e = 0; e < VPL; e += 4) {
+            const int c = feature(e);
+            if (c < p.vdim) {
+              float x[4];
+              if (RAW) {
+                const Q8Piece<T, 4> piece = *reinterpret_cast<const Q8Piece<T, 4>*>(row_r + c);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[i] = xl_to_float(piece.v[i]);
+              } else {
+                q8_floats(*reinterpret_cast<const uint32_t*>(row_c + c), x);
+              }
+#pragma unroll
+              for (int i = 0; i < 4; ++i) o[e + i] = fmaf(wk, x[i], o[e + i]);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < VPL; ++e) {
+            const int c = feature(e);
+            if (c < p.vdim) o[e] = fmaf(wk, RAW ? xl_to_float(row_r[c]) : (float)row_c[c], o[e]);
+          }
         }
       }
     }
@@ -580,7 +616,7 @@ __global__ void __launch_bounds__(SPLIT == 1 ? 128 : SPLIT * 32) q8_attn_general
   const T* gr = p.gate ? (const T*)p.gate + row * p.ldg + (long long)h * p.vdim : nullptr;
 #pragma unroll
   for (int e = 0; e < VPL; ++e) {
-    const int c = lane + 32 * e;
+    const int c = feature(e);
     if (c < p.vdim) {
       float v = o[e] / l;
       if (gr) v *= 1.f / (1.f + expf(-xl_to_float(gr[c])));
@@ -599,7 +635,7 @@ __global__ void __launch_bounds__(SPLIT == 1 ? 128 : SPLIT * 32) q8_attn_general
 // keys and features (with queries as rows, eight heads fill half of every instruction and every accumulator):
 //   S^T = K Q^T   A: codes as fp16, which is exact; B: queries as fp16, divided by a power of two above the norm's factors. The
 //                 scale of the block multiplies the fp32 result.
-//   O^T = V^T P^T A: codes as fp16; B: weights times value scale over the warp's largest, as fp16 (2^-12 relative), transposed between
+//   O^T = V^T P^T A: codes as fp16; B: weights times value scale over the largest of the CTA's, as fp16 (2^-11 relative), transposed between
 //                 the lanes by movmatrix
 //   raw rows      keys as fp16 likewise, values in bf16 with weights as sums of two bf16 numbers
 //
@@ -1344,8 +1380,14 @@ XL_API int xl_q8_attn_general(const float* q, const void* raw_k, const void* raw
   const bool split = (long long)T * H * B <= 2 * 148;
   const dim3 grid(split ? T : (T + 3) / 4, H, B), block(split ? 256 : 128);
   XL_DISPATCH_DTYPE(dtype, D, {
-    void (*kernel)(const Q8AttnParams) = vdim <= 128 ? (split ? q8_attn_general_kernel<D, 4, 8> : q8_attn_general_kernel<D, 4, 1>)
-                                                     : (split ? q8_attn_general_kernel<D, 16, 8> : q8_attn_general_kernel<D, 16, 1>);
+    const bool wide = vdim % 4 == 0 && (((uintptr_t)raw_v | (uintptr_t)vc) & 15) == 0;
+    void (*kernel)(const Q8AttnParams);
+    if (wide)
+      kernel = vdim <= 128 ? (split ? q8_attn_general_kernel<D, 4, 8, true> : q8_attn_general_kernel<D, 4, 1, true>)
+                           : (split ? q8_attn_general_kernel<D, 16, 8, true> : q8_attn_general_kernel<D, 16, 1, true>);
+    else
+      kernel = vdim <= 128 ? (split ? q8_attn_general_kernel<D, 4, 8, false> : q8_attn_general_kernel<D, 4, 1, false>)
+                           : (split ? q8_attn_general_kernel<D, 16, 8, false> : q8_attn_general_kernel<D, 16, 1, false>);
     XL_TRY(xl_launch_overlapped(kernel, grid, block, (size_t)0, s, p));
   });
   return (int)cudaGetLastError();
