@@ -28,7 +28,7 @@ def host_load(h2d_stream, name: Optional[str] = None) -> Tensor:
 
 
 def _special_host_store(ex, op, env):
-    ex.host_store(op.attrs["stream"], env[op.inputs[0]])
+    ex.host_store(op.attrs["stream"], env[op.inputs[0]], lambda: ex.held_by_nothing_else(op.inputs[0], op, env))
 
 
 OpDef("host_store", special=_special_host_store, infer=lambda op: [])

@@ -419,9 +419,10 @@ class Session:
         self._cursor[stream] = i + 1
         return [data[i, r] for r in range(self.num_local)]
 
-    def host_store(self, stream: DeviceToHostStream, vals: List[torch.Tensor]):
+    def host_store(self, stream: DeviceToHostStream, vals: List[torch.Tensor], unshared=lambda: False):
+        """`unshared`: whether nothing else holds the values, so that a captured graph can hand them out as they are."""
         if getattr(self, "_capture_outputs", None) is not None:
-            self._capture_outputs.append((stream, [v.detach().clone() for v in vals]))
+            self._capture_outputs.append((stream, [v.detach() for v in vals] if unshared() else [v.detach().clone() for v in vals]))
             return
         self._outputs.setdefault(stream, []).append([v.detach().clone() for v in vals])
 
@@ -445,6 +446,18 @@ class Session:
                 arr = arr[0]
             res[stream] = arr
         return res
+
+    def held_by_nothing_else(self, t: Tensor, op, env) -> bool:
+        """Whether the value of `t` is memory of its own that `op` is the last to use: no view, not among the values of other tensors
+        (inputs and variables of the graph are some of them), not a static input of the captured graph."""
+        if t.producer is None or any(t in later.inputs for later in op.graph.ops[op.graph.ops.index(op) + 1:]):
+            return False
+        mine = env[t]
+        held = {v.untyped_storage().data_ptr() for k, vals in env.items() if k is not t for v in vals or () if isinstance(v, torch.Tensor)}
+        held.update(v.untyped_storage().data_ptr() for v in (self._capture_inputs or {}).values())
+        held.update(v.untyped_storage().data_ptr() for vals in self._vars.values() for v in vals)
+        return all(v.is_contiguous() and v.untyped_storage().nbytes() == v.numel() * v.element_size()
+                   and v.untyped_storage().data_ptr() not in held for v in mine)
 
     # ------------------------------------------------------------------------------------------------------
     # remote buffers / device copies
