@@ -11,6 +11,8 @@
 //       moving the whole result in 32 bits (4 bytes more per value written and read again; 4096 x 32256: 160 us).
 #include "common.cuh"
 
+#include <type_traits>
+
 namespace {
 
 constexpr int AD_MAX_RANK = 128;
@@ -238,17 +240,41 @@ template <typename T, int KS> __global__ void __launch_bounds__(128) adapter_up_
     for (int u = 0; u < 4; ++u)
 #pragma unroll
       for (int e = 0; e < 4; ++e) c[u][e] = 0.f;
+    float up[2] = {1.f, 1.f};  // rows quad, quad + 8
     if (s >= 0) {
+      float down[2] = {1.f, 1.f};
+      if constexpr (std::is_same<T, __half>::value) {  // fp16 ends at 65504: rows of larger numbers are scaled by a power of two on the way
+        float top[2] = {0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < KS * 4; ++i) {
+          const int r = m * 16 + quad + 8 * (i & 1);
+          if (r < rows) {
+            const float2 v = *reinterpret_cast<const float2*>(low + r * p.rp + 8 * (i >> 1) + 2 * j);
+            top[i & 1] = fmaxf(top[i & 1], fmaxf(fabsf(v.x), fabsf(v.y)));
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
+          top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
+          if (top[i] > 32768.f && top[i] < INFINITY) {
+            const int by = ilogbf(top[i]) - 14;
+            down[i] = ldexpf(1.f, -by);
+            up[i] = ldexpf(1.f, by);
+          }
+        }
+      }
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
         uint32_t h[4], e[4];  // rows quad, quad + 8; numbers 2 j, 2 j + 1, then 2 j + 8, 2 j + 9
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int r = m * 16 + quad + 8 * (i & 1);
-          const float2 v = r < rows ? *reinterpret_cast<const float2*>(low + r * p.rp + k * 16 + 8 * (i >> 1) + 2 * j) : make_float2(0.f, 0.f);
+          float2 v = r < rows ? *reinterpret_cast<const float2*>(low + r * p.rp + k * 16 + 8 * (i >> 1) + 2 * j) : make_float2(0.f, 0.f);
+          if constexpr (std::is_same<T, __half>::value) v = make_float2(v.x * down[i & 1], v.y * down[i & 1]);
           h[i] = ad_pack<T>(v.x, v.y);
-          const float2 back = xl_pair_to_float2<T>(h[i]);
-          e[i] = ad_pack<T>(v.x - back.x, v.y - back.y);
+          const float2 back = xl_pair_to_float2<T>(h[i]);  // infinite: there is no rest
+          e[i] = ad_pack<T>(fabsf(back.x) < INFINITY ? v.x - back.x : 0.f, fabsf(back.y) < INFINITY ? v.y - back.y : 0.f);
         }
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
@@ -264,7 +290,10 @@ template <typename T, int KS> __global__ void __launch_bounds__(128) adapter_up_
       T* dst = out + (long long)r * p.N + c1;
       uint32_t w[4];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) w[u] = ad_pack<T>(c[u][2 * h], c[u][2 * h + 1]);
+      for (int u = 0; u < 4; ++u) {
+        if constexpr (std::is_same<T, __half>::value) w[u] = ad_pack<T>(c[u][2 * h] * up[h], c[u][2 * h + 1] * up[h]);
+        else w[u] = ad_pack<T>(c[u][2 * h], c[u][2 * h + 1]);
+      }
       if (wide) {
         if (c1 < p.N) *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
       } else {

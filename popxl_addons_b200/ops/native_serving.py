@@ -57,6 +57,12 @@ def residual_rms_cuda(x, y, *norm, mult, eps):
     return stream_rms(x, y, mult, None, None, norm[0] if norm else None, eps, y.dtype)
 
 
+def _rows16(t):
+    """The same numbers in rows one after the other from a 16-byte boundary, as the kernels read them; a copy where they lie elsewhere."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 def _rules_ok(history, start, penalties, bias_tokens, bias_values, allowed) -> bool:
     return (_i32(history, start, bias_tokens, allowed) and _f32(penalties, bias_values)
             and all(t.is_cuda and t.is_contiguous() for t in (penalties, bias_values)))
@@ -64,6 +70,7 @@ def _rules_ok(history, start, penalties, bias_tokens, bias_values, allowed) -> b
 
 @native("shape_logits")
 def shape_logits_cuda(logits, slot, length, *rules):
+    logits = _rows16(logits)
     if not _ok(logits) or logits.dim() != 2 or not _i32(slot, length) or not _rules_ok(*rules):
         return NotImplemented
     (rows, V), (slots, L) = logits.shape, rules[0].shape
@@ -75,6 +82,7 @@ def shape_logits_cuda(logits, slot, length, *rules):
 
 @native("take_shaped_")
 def take_shaped_cuda(current, logits, buf, pos, length, count, *rules, valid, base, ahead, advance):
+    logits = _rows16(logits)
     if not _ok(logits) or logits.dim() != 2 or not _i32(current, buf, pos, length, count) or not _rules_ok(*rules):
         return NotImplemented
     rows, V = logits.shape
@@ -176,7 +184,8 @@ def window_attention_q8_cuda(proj, q_norm, k_norm, k, v, k_scale, v_scale, k_tai
     is_few = _q8_few_rows(T * (heads // G), blocks * 64)
     if T == 1 and dt == torch.bfloat16 and few(None, (None, None), read_ahead.allowed(pos, count, k, v, k_scale, v_scale, k_tail, v_tail)):
         return joint
-    if (dt == torch.bfloat16 and not is_few and dim <= 128 and vdim <= 128 and dim % 8 == vdim % 8 == ld % 8 == ldo % 8 == 0
+    aligned = all(t.data_ptr() % 16 == 0 for t in (proj, joint, k, v, k_tail, v_tail))
+    if (dt == torch.bfloat16 and not is_few and aligned and dim <= 128 and vdim <= 128 and dim % 8 == vdim % 8 == ld % 8 == ldo % 8 == 0
             and T * heads <= 1 << 22 and G * blocks * 64 * (dim + vdim) * 2 <= _Q8_EXPANDED):
         # as many sequences at a time as expand to what is set aside for it
         step = max(1, _Q8_EXPANDED // (G * blocks * 64 * (dim + vdim) * 2))
@@ -201,6 +210,7 @@ def window_attention_q8_cuda(proj, q_norm, k_norm, k, v, k_scale, v_scale, k_tai
 
 @native("linear_adapted")
 def linear_adapted_cuda(x, weight, a, b, scale, slot, T, out_dtype):
+    x = x.contiguous()
     dt, dev = x.dtype, x.device
     (rows, K), N, (n, r, _) = x.shape, weight.shape[0], a.shape
     if not (dt in _CODE and dt == weight.dtype == a.dtype == b.dtype and out_dtype in (dt, torch.float32)):

@@ -18,7 +18,7 @@ from typing import Dict, NamedTuple, Optional, Tuple
 import torch
 
 from ..core import Tensor
-from ..dtypes import dtype as _dtype, float32, int8
+from ..dtypes import dtype as _dtype, float32, int32, int8
 from ..opdef import OpDef, emit, emit1
 from .decode import _store_row_ref
 from .sequence import _mm, _rms
@@ -239,7 +239,8 @@ def window_attention_q8_(proj: Tensor, q_norm: Tensor, k_norm: Tensor, cache: Ca
     """`window_attention_` against a cache of 8 bits: `proj` rows are `[q: heads x dim | k: G x dim | v: G x vdim | gate: heads x
     vdim]` (the gate may be absent), every query and key head gets an RMS norm, keys and values join the cache, and the gated
     attention goes to the first `heads * vdim` columns of `joint`. A sequence that would not fit the cache is left out, rows past
-    `count[b]` are left as they are."""
+    `count[b]` are left as they are. A key or value that is not finite has no code: it spoils the positions that read its block, of
+    the portion that brings it from the block's first one on."""
     if cache.k.rank != 5 or cache.v.rank != 5:
         raise ValueError("the codes of a cache are (batch, heads, blocks, tokens, features)")
     B, G, blocks, _, dim = cache.k.shape
@@ -258,6 +259,8 @@ def window_attention_q8_(proj: Tensor, q_norm: Tensor, k_norm: Tensor, cache: Ca
         raise ValueError(f"the joint buffer needs {B * T} rows of {heads * vdim} columns or more in {proj.dtype}")
     for what, t, n in (("q_norm", q_norm, dim), ("k_norm", k_norm, dim)):
         _expect(what, t, (n,), float32)
+    _expect("pos", pos, (B,), int32)
+    _expect("count", count, (B,), int32)
     if not scale > 0 or window < 0 or keep_first < 0:
         raise ValueError(f"scale ({scale}) must be positive, window ({window}) and keep_first ({keep_first}) not negative")
     return emit1("window_attention_q8_", [proj, q_norm, k_norm, *cache, pos, count, joint],
@@ -276,8 +279,8 @@ def linear_adapted(x: Tensor, weight: Tensor, adapters: Adapters, slot: Tensor, 
     _expect("adapters.a", adapters.a, (n, rank, x.shape[1]), x.dtype)
     _expect("adapters.b", adapters.b, (n, weight.shape[0], rank), x.dtype)
     _expect("adapters.scale", adapters.scale, (n,), float32)
-    if T < 1 or x.shape[0] != slot.shape[0] * T:
-        raise ValueError(f"{slot.shape[0]} sequences of {T} tokens do not make {x.shape[0]} rows")
+    if T < 1 or slot.rank != 1 or slot.dtype != int32 or x.shape[0] != slot.shape[0] * T:
+        raise ValueError(f"sequences of {T} tokens with slots {tuple(slot.shape)} {slot.dtype} do not make {x.shape[0]} rows")
     return emit1("linear_adapted", [x, weight, *adapters, slot], dict(T=int(T), out_dtype=(dtype or x.dtype).as_torch()))
 
 
@@ -295,6 +298,9 @@ def residual_rms_(x: Tensor, y: Tensor, norm: Optional[Tensor] = None, eps: floa
 
 def _check_rules(rules: LogitRules, vocab: int):
     slots = rules.history.shape[0]
+    for what, t, dt in zip(rules._fields, rules, (int32, int32, float32, int32, float32, int32)):
+        if t.dtype != dt or t.rank != (1 if what == "start" else 2):
+            raise ValueError(f"rules.{what} must be {'one row' if what == 'start' else 'rows'} of {dt}, not {tuple(t.shape)} {t.dtype}")
     if rules.history.shape[1] > MAX_HISTORY or rules.bias_tokens.shape[1] > MAX_BIASES:
         raise ValueError(f"rules hold at most {MAX_HISTORY} tokens and {MAX_BIASES} biases of a slot, not {rules.history.shape[1]} and "
                          f"{rules.bias_tokens.shape[1]}")
@@ -311,8 +317,9 @@ def shape_logits(logits: Tensor, slot: Tensor, length: Tensor, rules: LogitRules
     the frequency penalty is subtracted for every time a token occurred since the prompt, the presence penalty once; biases are
     added; what is not allowed becomes minus infinity. A row that allows nothing is minus infinity throughout."""
     _check_rules(rules, logits.shape[1])
-    if slot.shape != (logits.shape[0],) or length.shape != (logits.shape[0],):
-        raise ValueError(f"{logits.shape[0]} rows of logits need as many slots and lengths")
+    if any(t.shape != (logits.shape[0],) or t.dtype != int32 for t in (slot, length)):
+        raise ValueError(f"{logits.shape[0]} rows of logits need as many slots and lengths in int32, not {tuple(slot.shape)} {slot.dtype} and "
+                         f"{tuple(length.shape)} {length.dtype}")
     return emit1("shape_logits", [logits, slot, length, *rules])
 
 
@@ -323,8 +330,13 @@ def take_shaped_(current: Tensor, logits: Tensor, buf: Tensor, pos: Tensor, leng
     Of equal logits the lowest index is chosen (index 0 where nothing is allowed)."""
     valid = int(valid or logits.shape[-1])
     _check_rules(rules, valid)
-    if not rules.history.shape[0] == logits.shape[0] == length.shape[0] == count.shape[0]:
-        raise ValueError(f"{logits.shape[0]} rows of logits need as many slots, lengths and counts")
+    rows = logits.shape[0]
+    if rules.history.shape[0] != rows or any(t.shape != (rows,) or t.dtype != int32 for t in (length, count)):
+        raise ValueError(f"{rows} rows of logits need as many slots, lengths and counts in int32")
+    if not 1 <= valid <= logits.shape[1]:
+        raise ValueError(f"a choice among {valid} entries from rows of {logits.shape[1]}")
+    if current.dtype != int32 or pos.dtype != int32 or buf.dtype != int32 or buf.rank != 2 or not current.nelms == buf.shape[1] == rows:
+        raise ValueError(f"{rows} choices go to as many int32 numbers and rows of a buffer, not {tuple(current.shape)} and {tuple(buf.shape)}")
     return emit1("take_shaped_", [current, logits, buf, pos, length, count, *rules],
                  dict(valid=valid, base=int(base), ahead=int(ahead), advance=bool(advance)))
 
@@ -332,4 +344,8 @@ def take_shaped_(current: Tensor, logits: Tensor, buf: Tensor, pos: Tensor, leng
 def append_tokens_(history: Tensor, tokens: Tensor, pos: Tensor, count: Tensor, T: int) -> Tensor:
     """The real tokens of a portion, `tokens (batch * T,)`, take their places in `history (batch, length)`; places past its end are
     dropped."""
+    if T < 1 or history.rank != 2 or tokens.nelms != history.shape[0] * T:
+        raise ValueError(f"{tuple(tokens.shape)} tokens are not portions of {T} for {history.shape[0]} sequences")
+    for what, t in (("pos", pos), ("count", count)):
+        _expect(what, t, (history.shape[0],), int32)
     return emit1("append_tokens_", [history, tokens, pos, count], dict(T=int(T)))

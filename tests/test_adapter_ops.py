@@ -27,8 +27,10 @@ def test_adapted_products(backend, B, T, K, N, n, r):  # noqa: F811
         y = op("linear_adapted", backend, x, w, a, b, scale.to(backend[0]), i32(backend, *slot), T=T, out_dtype=out)
         assert y.dtype == out
         # fp32: sums of K + r products, each off by 2^-24 of terms below the largest result: 2e-5 covers 4096 of them many times.
-        # 16-bit results: one rounding of the sum (2^-9 of the largest at most), with many rows one more of the adapters' term
-        close(y, want, (backend[0], out), 2e-5, 2 * 2.0 ** -9 + 1e-4)
+        # bf16 results: one rounding of the sum, half a step, 2^-8 of the value at most
+        # where rows are many (T >= 8) the adapters' term is rounded ahead of it: no more than 2^-8 of a term that here is smaller than
+        # the largest result
+        close(y, want, (backend[0], out), 2e-5, (1 if T < 8 else 2) * 2.0 ** -8 + 1e-4)
 
 
 @pytest.mark.parametrize("T", [1, 64])
@@ -44,6 +46,35 @@ def test_rows_without_an_adapter_are_the_shared_product(backend, T):  # noqa: F8
     assert not torch.isfinite(y[T:2 * T]).any()
 
 
+@pytest.mark.parametrize("T", [1, 40])
+def test_strided_rows(backend, T):  # noqa: F811
+    x, x64 = rnd(backend, 2 * T, 72, seed=1)
+    w, w64 = rnd(backend, 136, 40, std=0.15, seed=2)
+    a, a64 = rnd(backend, 3, 8, 40, std=0.15, seed=3)
+    b, b64 = rnd(backend, 3, 136, 8, std=0.3, seed=4)
+    scale = torch.ones(3)
+    y = op("linear_adapted", backend, x[:, 3:43], w, a, b, scale.to(backend[0]), i32(backend, 2, 2), T=T, out_dtype=backend[1])
+    close(y, plain.adapted(x64[:, 3:43], w64, a64, b64, scale.double(), [2, 2], T), backend, 2e-5, 2 * 2.0 ** -8 + 1e-4)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("r", [8, 40])
+def test_fp16_numbers_past_its_range(r):
+    """What stands between the products may be larger than fp16 holds (65504), next to rows of ordinary size."""
+    backend, T = ("cuda", torch.float16), 50  # noqa: F811
+    x, x64 = rnd(backend, T, 256, seed=1)
+    x[::3] *= 40.0  # exact powers are not needed: both sides read the rounded values
+    x64 = x.double().cpu()
+    w, w64 = rnd(backend, 256, 256, std=1e-3, seed=2)
+    a, a64 = rnd(backend, 1, r, 256, std=200.0, seed=3)
+    b, b64 = rnd(backend, 1, 256, r, std=2e-4, seed=4)
+    assert (x64 @ a64[0].T).abs().max() > 65504
+    y = op("linear_adapted", backend, x, w, a, b, torch.ones(1, device="cuda"), i32(backend, 0), T=T, out_dtype=torch.float16)
+    want = plain.adapted(x64, w64, a64, b64, torch.ones(1).double(), [0], T)
+    for i in range(T):  # two roundings of half a step of fp16, 2^-11 each, and sums in 32 bits
+        close(y[i], want[i], backend, 0, 2 * 2.0 ** -11 + 1e-4)
+
+
 def test_refusals():
     ir = xl.Ir()
     with ir.main_graph:
@@ -57,6 +88,8 @@ def test_refusals():
         assert ops.linear_adapted(x, w, adapters(), slot, 2).shape == (6, 24)
         with pytest.raises(ValueError, match="sequences of"):
             ops.linear_adapted(x, w, adapters(), slot, 3)
+        with pytest.raises(ValueError, match="sequences of"):
+            ops.linear_adapted(x, w, adapters(), var((3,), xl.float32), 2)
         with pytest.raises(ValueError, match="adapters.a"):
             ops.linear_adapted(x, w, adapters(K=8), slot, 2)
         with pytest.raises(ValueError, match="adapters.b"):

@@ -8,6 +8,7 @@ import plain_serving as plain
 from test_dunelix_ops import backend, close, i32, op, rnd  # noqa: F401  (fixture and helpers)
 from popxl_addons_b200 import xl
 from popxl_addons_b200.xl import ops
+from popxl_addons_b200.xl.opdef import OPS
 
 BLOCK = plain.BLOCK
 # heads, key / value heads, dim, vdim
@@ -26,10 +27,11 @@ def empty_cache(backend, B, G, blocks, dim, vdim, junk=True):  # noqa: F811
 
 def bound(backend, dim):  # noqa: F811
     """Largest difference over the largest output. 32 bits: scores of up to 8 from sums of `dim` roundings of 2^-24 relative to
-    |q||k|, about 2^-18 of a weight, and as much again for sums over keys. bf16: the output's own rounding is 2^-9 of the value at
-    most (half a step of 2^-8), a gate's input has none; queries are held to 2^-12 where products take 16 bits, which moves a score of up to
-    8 by 2^-9 at most, values times codes to 2^-9: four times 2^-9 in all."""
-    return 2e-5 if backend[1] == torch.float32 else 4 * 2.0 ** -9
+    |q||k|, about 2^-18 of a weight, and as much again for sums over keys. bf16: the output's own rounding is 2^-8 of the value at
+    most (half a step of 2^-7), a gate's input has none; queries, held to 2^-11 where products take 16 bits, move a score of up to 8 by
+    the sum of `dim` independent roundings, about 2^-11 * 8 / sqrt(dim) and 2^-10 at most for widths of 16 and more; weights
+    times scales in 16 bits add 2^-11: below 2 * 2^-8 in all."""
+    return 2e-5 if backend[1] == torch.float32 else 2 * 2.0 ** -8
 
 
 def run_portions(backend, rows, cuts, start, T, shape, window, keep, sink, gated, cache, eps=1e-5):  # noqa: F811
@@ -147,6 +149,58 @@ def test_repeated_passes_and_padding(backend, T):  # noqa: F811
     assert all(torch.equal(a.nan_to_num(5.0), b.nan_to_num(5.0)) for a, b in zip(state, cache))
 
 
+@pytest.mark.parametrize("offset", [0, 1])
+@pytest.mark.parametrize("T", [1, 20, 130])
+def test_projections_inside_wider_rows(backend, T, offset):  # noqa: F811
+    """Columns of a wider buffer, whose rows start where 16-byte accesses can and where they cannot."""
+    H, G, d, dv = SHAPES["full"]
+    cols, n, (qn, qn64), (kn, kn64) = (H + G) * d + (G + H) * dv, 70 + T, *norms(backend, d)
+    rows = torch.randn(n, cols, generator=torch.Generator().manual_seed(5)).to(backend[1])
+    cache = empty_cache(backend, 1, G, 4, d, dv)
+    want, _, _ = plain.q8_attention(rows.double(), qn64, kn64, H, G, d, dv, 100, 4, d ** -0.5, 0.0, 1e-5, backend[1])
+    for p, T_now in ((0, 70), (70, T)):
+        wide = torch.full((T_now, cols + 8), float("nan"), dtype=backend[1], device=backend[0])
+        wide[:, offset:offset + cols] = rows[p:p + T_now].to(backend[0])
+        joint = torch.zeros(T_now, H * dv, dtype=backend[1], device=backend[0])
+        op("window_attention_q8_", backend, wide[:, offset:offset + cols], qn, kn, *cache, i32(backend, p), i32(backend, T_now), joint, T=T_now,
+           heads=H, window=100, keep_first=4, scale=d ** -0.5, sink=0.0, eps=1e-5)
+        for i in range(T_now):
+            close(joint[i], want[p + i], backend, bound(backend, d), bound(backend, d))
+
+
+@pytest.mark.gpu
+def test_two_streams():
+    """Single tokens whose keys are cut among CTAs, few rows, and portions, side by side on two streams: what each leaves alone."""
+    from popxl_addons_b200.ops.native import check_gemm_errors
+
+    backend, (H, G, d, dv) = ("cuda", torch.bfloat16), SHAPES["full"]
+    (qn, _), (kn, _) = norms(backend, d)
+    runs = []
+    for seed, T in ((1, 1), (2, 1), (3, 12), (4, 300)):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        cache = [t.nan_to_num(1.0) for t in empty_cache(backend, 2, G, 80, d, dv)]
+        proj = torch.randn(2 * T, (H + G) * d + (G + H) * dv, generator=g, device="cuda").bfloat16()
+        where = (torch.tensor([4000 + 64 * seed, 700], dtype=torch.int32, device="cuda"), torch.tensor([T, T], dtype=torch.int32, device="cuda"))
+
+        def run(T=T, cache=cache, proj=proj, where=where):
+            joint = torch.zeros(2 * T, H * dv, dtype=torch.bfloat16, device="cuda")
+            assert OPS["window_attention_q8_"].native["cuda"](proj, qn, kn, *cache, *where, joint, T=T, heads=H, window=0, keep_first=0, scale=d ** -0.5,
+                                                              sink=None, eps=1e-5) is joint
+            return joint
+
+        runs.append(run)
+    want = [run() for run in runs]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], []
+    for i in range(40):  # a cache stays with its stream
+        with torch.cuda.stream(streams[i % 2]):
+            got.append((i % 2, [runs[k]() for k in (i % 2, 2 + i % 2)]))
+    torch.cuda.synchronize()
+    check_gemm_errors()
+    for at, pair in got:
+        assert torch.equal(pair[0], want[at]) and torch.equal(pair[1], want[2 + at])
+
+
 def test_refusals():
     ir = xl.Ir()
     with ir.main_graph:
@@ -175,6 +229,9 @@ def test_refusals():
             ops.window_attention_q8_(proj, norm, norm, cache(), *rest, joint, 4, 4, 0.25)
         with pytest.raises(ValueError, match="joint buffer"):
             ops.window_attention_q8_(proj, norm, norm, cache(), *rest, var((6, 95), xl.bfloat16), 3, 4, 0.25)
+        for bad in ((var((1,), i32_), rest[1]), (rest[0], var((2,), f32))):
+            with pytest.raises(ValueError, match="pos|count"):
+                ops.window_attention_q8_(proj, norm, norm, cache(), *bad, joint, 3, 4, 0.25)
         with pytest.raises(ValueError, match="q_norm"):
             ops.window_attention_q8_(proj, var((17,), f32), norm, cache(), *rest, joint, 3, 4, 0.25)
         with pytest.raises(ValueError, match="positive"):

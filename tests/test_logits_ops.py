@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import plain_serving as plain
-from test_dunelix_ops import backend, i32, op  # noqa: F401  (fixture and helpers)
+from test_dunelix_ops import backend, i32, op, rnd  # noqa: F401  (fixture and helpers)
 from popxl_addons_b200 import xl
 from popxl_addons_b200.xl import ops
 from popxl_addons_b200.xl.opdef import OPS
@@ -145,6 +145,18 @@ def test_infinite_and_undefined_logits(backend):  # noqa: F811
     assert current.tolist() == [6, 3]
 
 
+@pytest.mark.parametrize("offset", [0, 1])
+def test_logits_inside_wider_rows(backend, offset):  # noqa: F811
+    """A slice of a padded vocabulary, and two rows under the rules of one slot."""
+    r, _ = rules(2, 77, 9, 3)
+    wide, _ = rnd(backend, 3, 90, seed=8)
+    d = [x.to(backend[0]) for x in r]
+    got = op("shape_logits", backend, wide[:, offset:offset + 77], i32(backend, 1, 1, 0), i32(backend, 9, 4, 9), *d)
+    alone = [op("shape_logits", backend, wide[i:i + 1, offset:offset + 77].contiguous(), i32(backend, s), i32(backend, n), *d)
+             for i, (s, n) in enumerate(((1, 9), (1, 4), (0, 9)))]
+    assert torch.equal(got, torch.cat(alone))
+
+
 def test_append_tokens(backend):  # noqa: F811
     dev, T = backend[0], 5
     history = torch.full((4, 8), -1, dtype=torch.int32, device=dev)
@@ -172,3 +184,14 @@ def test_refusals():
             ops.shape_logits(logits, var((3,)), var((2,)), rules_of())
         with pytest.raises(ValueError, match="slots, lengths and counts"):
             ops.take_shaped_(var((2,)), logits, var((4, 2)), var((1,)), var((2,)), var((2,)), rules_of(slots=3, biases=(3, 3)))
+        with pytest.raises(ValueError, match="slots, lengths and counts"):
+            ops.take_shaped_(var((2,)), logits, var((4, 2)), var((1,)), var((1,)), var((2,)), rules_of())
+        with pytest.raises(ValueError, match="choices go to"):
+            ops.take_shaped_(var((2,)), logits, var((4, 3)), var((1,)), var((2,)), var((2,)), rules_of())
+        with pytest.raises(ValueError, match="among 51"):
+            ops.take_shaped_(var((2,)), logits, var((4, 2)), var((1,)), var((2,)), var((2,)), rules_of(), valid=51)
+        with pytest.raises(ValueError, match="rules.penalties"):
+            ops.shape_logits(logits, var((2,)), var((2,)), rules_of()._replace(penalties=var((2, 3))))
+        for bad in ((var((4, 6)), var((9,)), 2), (var((2, 6)), var((2, 2)), 2)):
+            with pytest.raises(ValueError, match="portions|pos"):
+                ops.append_tokens_(bad[0], var((4,)), bad[1], var((2,)), bad[2])
