@@ -449,8 +449,8 @@ class Session:
 
     def held_by_nothing_else(self, t: Tensor, op, env) -> bool:
         """Whether the value of `t` is memory of its own that `op` is the last to use: no view, not among the values of other tensors
-        (inputs and variables of the graph are some of them), not a static input of the captured graph."""
-        if t.producer is None or any(t in later.inputs for later in op.graph.ops[op.graph.ops.index(op) + 1:]):
+        (inputs and variables of the graph are some of them), not handed to a caller, not a static input of the captured graph."""
+        if t.producer is None or t in op.graph.outputs or any(t in later.inputs for later in op.graph.ops[op.graph.ops.index(op) + 1:]):
             return False
         mine = env[t]
         held = {v.untyped_storage().data_ptr() for k, vals in env.items() if k is not t for v in vals or () if isinstance(v, torch.Tensor)}

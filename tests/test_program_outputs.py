@@ -55,6 +55,31 @@ def test_values_changed_after_they_were_stored(device):
         assert (got[early] == i).all() and (got[late] == i + 1).all()
 
 
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_a_called_graph_stores_what_it_returns(device):
+    """The caller changes in place what the called graph stored."""
+    ir = xl.Ir()
+    with ir.main_graph:
+        stream = xl.h2d_stream((4,), xl.float32, "x")
+    p = xl.Program(ir, "p")
+    with p:
+        early, late = (xl.d2h_stream((4,), xl.float32, n) for n in ("early", "late"))
+
+        def body(t):
+            y = t * 2.0
+            ops.host_store(early, y)
+            return y
+
+        x = ops.host_load(stream)
+        y, = ops.call(ir.create_graph(body, x), x)
+        ops.var_updates.accumulate_(y, x)
+        ops.host_store(late, y)
+    session = xl.Session(ir, device)
+    for i in range(1, 5):
+        got = session.run_program(p, {stream: np.full(4, float(i), np.float32)})
+        assert (got[early] == 2 * i).all() and (got[late] == 3 * i).all()
+
+
 @pytest.mark.gpu
 def test_outputs_without_copies():
     """Copies stay as they are when the program runs again; without copies the buffers are the program's own."""
