@@ -11,14 +11,16 @@
 //                               sink, lazy rescaling of O_m in TMEM
 // Codes are fp16 keys and bf16 values, both exact: the scale of a block multiplies the scores, that of its values the weights, which
 // replace S in TMEM as two bf16 numbers each (value and rounding error): rounded once to bf16 they would add as much error as the
-// rounding of the result does. Queries and raw keys are fp16 in
-// units of a power of two above their norm's factors.
+// rounding of the result does, and save 7 % of the time. Queries and raw keys are fp16 in units of a power of two above their norm's
+// factors.
 //
-// What bounds it is the chain of a tile: scores, softmax, weights, product. A tile has two buffers of scores of 64 keys each, so that the next
-// scores are there when a softmax ends, and an issuer of its own, so that no tile's products wait behind what holds up the other's: with one
-// buffer of 128 keys a tile's warps waited 1700 of 4500 cycles per 128 keys for the tensor core's answer, with one issuer for both tiles, in
-// a fixed order or going by what is ready, 1500 of 3000 cycles per 64 keys (clock stamps; 2 x 515 tokens after 6000, 32 heads on 8). The softmax takes a block's scores into registers at
-// once and works on pairs of fp32 numbers (fma.rn.f32x2); its exponentials alone occupy the special-function unit half of the time.
+// 32 heads on 8 of 128 features: 2 x 4096 tokens, window 1024, 261 us; 2 x 515 tokens after 6000, 161 us (632 TFLOP/s of visible keys,
+// the tensor pipe 48 % busy). What bounds it is the chain of a tile: scores, softmax, weights, product. A tile has two buffers of scores
+// of 64 keys each, so that the next scores are there when a softmax ends, and an issuer of its own, so that no tile's products wait
+// behind what holds up the other's: with one buffer of 128 keys a tile's warps waited 1700 of 4500 cycles per 128 keys for the tensor
+// core's answer, with one issuer for both tiles, in a fixed order or going by what is ready, 1500 of 3000 cycles per 64 keys (clock stamps
+// of the second call). The softmax takes a block's scores into registers at once and works on pairs of fp32 numbers (fma.rn.f32x2); its
+// exponentials alone occupy the special-function unit half of the time.
 // Expanding codes outside this kernel moves five bytes per code once per portion, where every CTA would convert every block again next to a
 // softmax that fills the issue slots.
 //

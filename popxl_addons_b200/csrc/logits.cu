@@ -64,7 +64,8 @@ struct ShapedTake {
 // CHOOSE: the parts of a row are a cluster, whose winners meet in the first CTA.
 // What bounds it is latency: a row's scalars, its tokens, the count, the logits. The logits go to shared memory by asynchronous copies
 // that are asked for first, and the first eight tokens of every thread at once with the scalars that say how many there are. With
-// the logits in registers four CTAs fitted an SM and 96 rows of 50400 took two waves.
+// the logits in registers four CTAs fitted an SM and 96 rows of 50400 took two waves. 96 rows of 50400 fp32 logits, 2048 tokens, 64 biases:
+// 16.5 us (the bytes alone: 6); the choice from 48 rows in bf16: 12.4; one row of 32000: 4.1.
 template <typename T, bool CHOOSE>
 __global__ void __launch_bounds__(LG_THREADS)
     logits_kernel(const T* logits, float* out, const int* slot_of, const int* length_of, const LogitRulesArgs r, int V, int valid,
