@@ -637,8 +637,8 @@ __global__ void __launch_bounds__(SPLIT == 1 ? 128 : SPLIT * 32) q8_attn_general
 // keys and features (with queries as rows, eight heads fill half of every instruction and every accumulator):
 //   S^T = K Q^T   A: codes as fp16, which is exact; B: queries as fp16, divided by a power of two above the norm's factors. The
 //                 scale of the block multiplies the fp32 result.
-//   O^T = V^T P^T A: codes as fp16; B: weights times value scale over the largest of the CTA's, as fp16 (2^-11 relative), transposed between
-//                 the lanes by movmatrix
+//   O^T = V^T P^T A: codes as fp16; B: weights times value scale over a 2^15th of the largest of the CTA's, as fp16 (2^-11 relative),
+//                 transposed between the lanes by movmatrix
 //   raw rows      keys as fp16 likewise, values in bf16 with weights as sums of two bf16 numbers
 //
 // A code c becomes fp16 by two instructions for two of them: the byte c + 128 is the low byte of 1024 + (c + 128) under the high byte
@@ -879,7 +879,8 @@ __global__ void __launch_bounds__(QD_WARPS * 32, RT == 1 ? 3 : 2)
     }
   }
   __syncthreads();
-  const float ref = it1 > it0 ? fmaxf(fmaxf(fmaxf(tops[0][0], tops[0][1]), fmaxf(tops[0][2], tops[0][3])), 1e-20f) : 1.f;
+  // weights of 1 under the largest scale are 2^15, so that those under a scale a million times smaller are still normal numbers of fp16
+  const float ref = it1 > it0 ? fmaxf(fmaxf(fmaxf(tops[0][0], tops[0][1]), fmaxf(tops[0][2], tops[0][3])), 1e-20f) * (1.f / 32768.f) : 1.f;
   uint32_t q[RT][KG][8];  // rows quad + 8 m, features 64 i + 16 j .. + 15
 #pragma unroll
   for (int m = 0; m < RT; ++m)

@@ -134,6 +134,24 @@ def test_blocks_of_zeros_and_of_one_large_value(backend):  # noqa: F811
     close(got[69, dv - 2:dv], torch.tensor([0.0, float(rows[5, -1]) / 70]), backend, 1e-5, 2.0 ** -8)
 
 
+@pytest.mark.parametrize("T", [1, 5, 130])
+def test_values_of_very_different_size(backend, T):  # noqa: F811
+    """A block with one value of a million, next to blocks of values around 1: what the others add up to keeps its precision."""
+    H, G, d, dv = SHAPES["full"]
+    n, (qn, qn64), (kn, kn64) = 200 + T, *norms(backend, d)
+    g = torch.Generator().manual_seed(6)
+    rows = torch.randn(n, (H + G) * d + G * dv, generator=g)
+    rows[:, (H + G) * d:] = 0.5 + torch.rand(n, G * dv, generator=g)  # positive: nothing cancels
+    rows[10, (H + G) * d], rows[10, (H + G) * d + dv] = 1e6, 1e6
+    rows = rows.to(backend[1])
+    cache = empty_cache(backend, 3, G, 6, d, dv)
+    got = run_portions(backend, rows, [200, T], 0, 0, SHAPES["full"], 0, 0, None, False, cache)
+    want, _, _ = plain.q8_attention(rows.double(), qn64, kn64, H, G, d, dv, 0, 0, d ** -0.5, None, 1e-5, backend[1])
+    for i in range(200, n):  # value by value; bf16: half a step of the result, and as much again for what `bound` counts
+        x, y = (t.reshape(H, dv)[:, 1:].double().cpu() for t in (got[i], want[i]))
+        assert ((x - y).abs() / y).max().item() < (5e-5 if backend[1] == torch.float32 else 2 * 2.0 ** -8)
+
+
 @pytest.mark.parametrize("T", [1, 40])
 def test_repeated_passes_and_padding(backend, T):  # noqa: F811
     """The same pass twice gives the same state; padded rows and idle sequences touch nothing."""
