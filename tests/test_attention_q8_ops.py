@@ -187,6 +187,41 @@ def test_projections_inside_wider_rows(backend, T, offset):  # noqa: F811
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("seed", range(40))
+def test_drawn_calls(seed):
+    """Sizes, positions, counts and masks drawn at random, idle and misplaced sequences among them: the kernels against the CPU reference, bit
+    for bit in the cache."""
+    import random
+
+    r, g = random.Random(seed), torch.Generator().manual_seed(seed)
+    dtype = r.choice([torch.bfloat16] * 4 + [torch.float32, torch.float16])
+    d, dv = r.choice([(128, 128), (128, 64), (64, 128), (96, 80), (16, 16), (40, 24), (7, 10), (200, 264)])
+    G, R, B, blocks = r.choice([1, 2, 3]), r.choice([1, 3, 4, 8, 20]), r.choice([1, 2, 5]), r.choice([1, 8, 70])
+    T = min(r.choice([1, 1, 3, 17, 64, 129, 300]), blocks * BLOCK)
+    H, end = G * R, blocks * BLOCK
+    count = [r.choice([0, 1, T, T, -1]) for _ in range(B)]
+    pos = [r.choice([0, 63, r.randint(0, end), end - max(n, 0), end, -1]) for n in count]
+    proj = torch.randn(B * T, (H + G) * d + G * dv + r.choice([0, H * dv]), generator=g).to(dtype)
+    cache = [t.nan_to_num(0.5) for t in empty_cache(("cpu", dtype), B, G, blocks, d, dv)]
+    cache[2:4] = [t * 3e-4 for t in cache[2:4]]  # keys and values of ordinary size
+    qn, kn = norms(("cpu", dtype), d)[0][0], norms(("cpu", dtype), d)[1][0]
+    how = dict(T=T, heads=H, window=r.choice([0, 1, 65, 1000]), keep_first=r.choice([0, 4, 64, 300]), scale=d ** -0.5,
+               sink=r.choice([None, 0.0]), eps=1e-5)
+    held = []
+    for backend in (("cpu", dtype), ("cuda", dtype)):  # noqa: F811
+        state = [t.clone().to(backend[0]) for t in cache]
+        joint = torch.full((B * T, H * dv + 8), -7.0, dtype=dtype, device=backend[0])
+        op("window_attention_q8_", backend, proj.to(backend[0]), qn.to(backend[0]), kn.to(backend[0]), *state, i32(backend, *pos), i32(backend, *count),
+           joint, **how)
+        held.append([joint.cpu()] + [t.cpu() for t in state])
+    assert all(torch.equal(x, y) for x, y in zip(held[0][1:], held[1][1:]))
+    # both sides are rounded: twice what `bound` allows one of them (fp16: its half step is an eighth of that of bf16)
+    tol = 2 * bound(("", dtype), d) / (8 if dtype == torch.float16 else 1)
+    for x, y in zip(held[0][0].double(), held[1][0].double()):
+        assert (x - y).abs().max() <= tol * x.abs().max()
+
+
+@pytest.mark.gpu
 def test_two_streams():
     """Single tokens whose keys are cut among CTAs, few rows, and portions, side by side on two streams: what each leaves alone."""
     from popxl_addons_b200.ops.native import check_gemm_errors
