@@ -1403,8 +1403,8 @@ XL_API int xl_q8_attn_general(const float* q, const void* raw_k, const void* raw
 // Few rows per sequence, bf16: dim, vdim multiples of 16 up to 128, ld, ldo and all pointers as the 16-byte accesses need them.
 // T = 1: the kernel normalises, appends and completes blocks itself (q and raw rows are null). T > 1: after xl_q8_append, on its q and
 // raw rows, with read_ahead 0. part: B * G * ceil(T H/G / 8 RT) * splits * 8 RT * (vdim + 2) floats with RT = 1 where T H/G <= 8, else
-// 2; counters: B * G * ceil(...) zero-initialised words (left zeroed). read_ahead: positions, counts and the cache were complete before the
-// previous launch. err: device int for the code of a wait that gave up.
+// 2; counters: B * G * ceil(...) zero-initialised words (left zeroed). read_ahead: positions, counts, the cache and the factors of both norms
+// were complete before the previous launch. err: device int for the code of a wait that gave up.
 XL_API int xl_q8_attn_few(const void* proj, long long ld, const float* wq, const float* wk, const float* q, const void* raw_k,
                           const void* raw_v, void* kc, void* vc, float* ks, float* vs, void* kt, void* vt, void* out, long long ldo,
                           const int* pos, const int* count, int B, int T, int H, int G, int dim, int vdim, int blocks, int window,

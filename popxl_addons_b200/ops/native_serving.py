@@ -182,8 +182,10 @@ def window_attention_q8_cuda(proj, q_norm, k_norm, k, v, k_scale, v_scale, k_tai
         return _launched(rc, "q8_attn_few")
 
     is_few = _q8_few_rows(T * (heads // G), blocks * 64)
-    if T == 1 and dt == torch.bfloat16 and few(None, (None, None), read_ahead.allowed(pos, count, k, v, k_scale, v_scale, k_tail, v_tail)):
-        return joint
+    if T == 1 and dt == torch.bfloat16:
+        ahead = read_ahead.allowed(q_norm, k_norm, k, v, k_scale, v_scale, k_tail, v_tail, pos, count)
+        if few(None, (None, None), ahead):
+            return joint
     aligned = all(t.data_ptr() % 16 == 0 for t in (proj, joint, k, v, k_tail, v_tail))
     if (dt == torch.bfloat16 and not is_few and aligned and dim <= 128 and vdim <= 128 and dim % 8 == vdim % 8 == ld % 8 == ldo % 8 == 0
             and T * heads <= 1 << 22 and G * blocks * 64 * (dim + vdim) * 2 <= _Q8_EXPANDED):
