@@ -18,7 +18,7 @@ from typing import Dict, NamedTuple, Optional, Tuple
 import torch
 
 from ..core import Tensor
-from ..dtypes import dtype as _dtype, float32, int32, int8
+from ..dtypes import bfloat16, dtype as _dtype, float16, float32, int32, int8
 from ..opdef import OpDef, emit, emit1
 from .decode import _store_row_ref
 from .sequence import _mm, _rms
@@ -286,25 +286,35 @@ def linear_adapted(x: Tensor, weight: Tensor, adapters: Adapters, slot: Tensor, 
 
 def split_glu(y: Tensor, cols: int, lead: int, limit: float, slope: float = 1.0, shift: float = 0.0) -> Tuple[Tensor, Tensor]:
     """The second half of `linear_split_glu`, for a product `y (n, cols + 2 F)` that is there already."""
+    if y.rank != 2 or cols < 0 or lead < 0 or y.shape[1] < cols or (y.shape[1] - cols) % 2:
+        raise ValueError(f"rows of {cols} columns with as many of gate and up behind them, and {lead} columns in front of the unit, do not "
+                         f"make {tuple(y.shape)}")
     return tuple(emit("split_glu", [y], dict(cols=int(cols), lead=int(lead), limit=float(limit), slope=float(slope), shift=float(shift))))
 
 
 def residual_rms_(x: Tensor, y: Tensor, norm: Optional[Tensor] = None, eps: float = 1e-6, mult: float = 1.0) -> Optional[Tensor]:
     """The second half of `linear_residual_rms_`: `x += mult * y` on the fp32 residual stream; with `norm`, returns the RMS norm of
     the updated rows in the type of `y`."""
+    if x.rank != 2 or y.rank != 2 or x.dtype != float32 or x.shape[1] != y.shape[1] or y.shape[0] > x.shape[0]:
+        raise ValueError(f"{tuple(y.shape)} cannot be added to the first rows of the residual stream {tuple(x.shape)} {x.dtype} (float32)")
+    if norm is not None:
+        _expect("norm", norm, (x.shape[1],), float32)
     out = emit("residual_rms_", [x, y] + ([norm] if norm is not None else []), dict(mult=float(mult), eps=float(eps)))
     return out[0] if norm is not None else None
 
 
-def _check_rules(rules: LogitRules, vocab: int):
-    slots = rules.history.shape[0]
+def _check_rules(rules: LogitRules, logits: Tensor, vocab: Optional[int] = None):
+    if logits.rank != 2 or logits.dtype not in (float32, float16, bfloat16):
+        raise ValueError(f"logits are rows of floating-point numbers, not {tuple(logits.shape)} {logits.dtype}")
+    vocab = vocab or logits.shape[1]
     for what, t, dt in zip(rules._fields, rules, (int32, int32, float32, int32, float32, int32)):
         if t.dtype != dt or t.rank != (1 if what == "start" else 2):
             raise ValueError(f"rules.{what} must be {'one row' if what == 'start' else 'rows'} of {dt}, not {tuple(t.shape)} {t.dtype}")
     if rules.history.shape[1] > MAX_HISTORY or rules.bias_tokens.shape[1] > MAX_BIASES:
         raise ValueError(f"rules hold at most {MAX_HISTORY} tokens and {MAX_BIASES} biases of a slot, not {rules.history.shape[1]} and "
                          f"{rules.bias_tokens.shape[1]}")
-    for what, t, tail in (("start", rules.start, ()), ("penalties", rules.penalties, (3,)),
+    slots = rules.history.shape[0]
+    for what, t, tail in (("start", rules.start, ()), ("penalties", rules.penalties, (3,)), ("bias_tokens", rules.bias_tokens, rules.bias_tokens.shape[1:]),
                           ("bias_values", rules.bias_values, rules.bias_tokens.shape[1:])):
         _expect(f"rules.{what}", t, (slots, *tail))
     if rules.allowed.shape[0] != slots or rules.allowed.shape[1] * 32 < vocab:
@@ -316,7 +326,7 @@ def shape_logits(logits: Tensor, slot: Tensor, length: Tensor, rules: LogitRules
     they are). In this order: tokens that occurred are divided by the repetition penalty where positive, else multiplied by it;
     the frequency penalty is subtracted for every time a token occurred since the prompt, the presence penalty once; biases are
     added; what is not allowed becomes minus infinity. A row that allows nothing is minus infinity throughout."""
-    _check_rules(rules, logits.shape[1])
+    _check_rules(rules, logits)
     if any(t.shape != (logits.shape[0],) or t.dtype != int32 for t in (slot, length)):
         raise ValueError(f"{logits.shape[0]} rows of logits need as many slots and lengths in int32, not {tuple(slot.shape)} {slot.dtype} and "
                          f"{tuple(length.shape)} {length.dtype}")
@@ -329,7 +339,7 @@ def take_shaped_(current: Tensor, logits: Tensor, buf: Tensor, pos: Tensor, leng
     `current[b]`, row `pos + ahead - base` of `buf` and token `length[b]` of the history. Rows with `count[b] <= 0` are left out.
     Of equal logits the lowest index is chosen (index 0 where nothing is allowed)."""
     valid = int(valid or logits.shape[-1])
-    _check_rules(rules, valid)
+    _check_rules(rules, logits, valid)
     rows = logits.shape[0]
     if rules.history.shape[0] != rows or any(t.shape != (rows,) or t.dtype != int32 for t in (length, count)):
         raise ValueError(f"{rows} rows of logits need as many slots, lengths and counts in int32")
@@ -337,6 +347,8 @@ def take_shaped_(current: Tensor, logits: Tensor, buf: Tensor, pos: Tensor, leng
         raise ValueError(f"a choice among {valid} entries from rows of {logits.shape[1]}")
     if current.dtype != int32 or pos.dtype != int32 or buf.dtype != int32 or buf.rank != 2 or not current.nelms == buf.shape[1] == rows:
         raise ValueError(f"{rows} choices go to as many int32 numbers and rows of a buffer, not {tuple(current.shape)} and {tuple(buf.shape)}")
+    if pos.nelms != 1:
+        raise ValueError(f"the choices of a step have one position, not {tuple(pos.shape)}")
     return emit1("take_shaped_", [current, logits, buf, pos, length, count, *rules],
                  dict(valid=valid, base=int(base), ahead=int(ahead), advance=bool(advance)))
 
@@ -346,6 +358,8 @@ def append_tokens_(history: Tensor, tokens: Tensor, pos: Tensor, count: Tensor, 
     dropped."""
     if T < 1 or history.rank != 2 or tokens.nelms != history.shape[0] * T:
         raise ValueError(f"{tuple(tokens.shape)} tokens are not portions of {T} for {history.shape[0]} sequences")
+    if history.dtype != int32 or tokens.dtype != int32:
+        raise ValueError(f"tokens are held in int32, not in {tokens.dtype} and {history.dtype}")
     for what, t in (("pos", pos), ("count", count)):
         _expect(what, t, (history.shape[0],), int32)
     return emit1("append_tokens_", [history, tokens, pos, count], dict(T=int(T)))
