@@ -161,6 +161,7 @@ def window_attention_q8_cuda(proj, q_norm, k_norm, k, v, k_scale, v_scale, k_tai
     if any(not t.is_contiguous() for t in (k, v, k_scale, v_scale)):
         return NotImplemented
     code, s, ld, ldo = _CODE[dt], _stream(), proj.stride(0), joint.stride(0)
+    window, keep_first = min(window, blocks * 64), min(keep_first, blocks * 64)  # no key is further back, and the kernels count in 32 bits
     sink = float("-inf") if sink is None else sink
     gate = proj.data_ptr() + plain * proj.element_size() if proj.shape[1] > plain else None
     cache = tuple(t.data_ptr() for t in (k, v, k_scale, v_scale))

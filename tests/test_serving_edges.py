@@ -5,6 +5,7 @@ import torch
 
 from popxl_addons_b200 import xl
 from popxl_addons_b200.xl import ops
+from test_serving_order import OnDevice
 
 
 def test_shapes_that_do_not_fit_are_refused():
@@ -52,3 +53,43 @@ def test_shapes_that_do_not_fit_are_refused():
         for history, tokens in ((var((2, 6), f32), var((4,))), (var((2, 6)), var((4,), f32))):
             with pytest.raises(ValueError, match="int32"):
                 ops.append_tokens_(history, tokens, slot, slot, 2)
+
+
+@pytest.fixture
+def launches(monkeypatch):
+    """What the binding of attention over 8-bit codes hands to its kernels, without a GPU: a list of (name, arguments)."""
+    from popxl_addons_b200.ops import native_serving as ns
+
+    seen = []
+    for name, fake in (("_ok", lambda *t: True), ("_i32", lambda *t: True), ("_stream", lambda: 0), ("_sms", lambda device: 148),
+                       ("_count", lambda name: None), ("counters", lambda n, *a: torch.zeros(n, dtype=torch.int32)),
+                       ("gemm_error_flag", lambda device: torch.zeros(1, dtype=torch.int32))):
+        monkeypatch.setattr(ns, name, fake)
+    for name in ("_q8_few", "_q8_append", "_q8_general", "_q8_append_expand", "_q8_tcgen05"):
+        monkeypatch.setattr(ns, name, lambda *a, name=name: seen.append((name, a)) or 0)
+    return seen
+
+
+def call_of_attention(B=1, T=1, H=2, G=1, dim=16, vdim=16, blocks=2, dtype=torch.bfloat16, **kw):
+    """The binding on tensors of the CPU (see `launches`)."""
+    from popxl_addons_b200.ops import native_serving as ns
+
+    cache = [torch.zeros(B, G, blocks, 64, w, dtype=torch.int8) for w in (dim, vdim)] + [torch.zeros(B, G, blocks) for _ in range(2)]
+    cache += [torch.zeros(B, G, 64, w, dtype=dtype) for w in (dim, vdim)]
+    rows = [torch.zeros(B * T, n, dtype=dtype) for n in ((H + G) * dim + G * vdim, H * vdim)]
+    where = [torch.zeros(B, dtype=torch.int32), torch.ones(B, dtype=torch.int32)]
+    proj, *cache, pos, count, joint = (t.as_subclass(OnDevice) for t in (rows[0], *cache, *where, rows[1]))
+    how = dict(T=T, heads=H, window=0, keep_first=0, scale=0.25, sink=None, eps=1e-6)
+    return ns.window_attention_q8_cuda(proj, torch.ones(dim), torch.ones(dim), *cache, pos, count, joint, **{**how, **kw})
+
+
+@pytest.mark.parametrize("T,dtype,kernel", [(1, torch.bfloat16, "_q8_few"), (3, torch.bfloat16, "_q8_few"), (100, torch.bfloat16, "_q8_append_expand"),
+                                            (100, torch.bfloat16, "_q8_tcgen05"), (2, torch.float32, "_q8_general")])
+def test_windows_wider_than_an_int(launches, T, dtype, kernel):
+    """A window or a number of kept tokens past 2^31 arrives as one that hides nothing, not as its low 32 bits."""
+    call_of_attention(T=T, dtype=dtype, window=(1 << 32) + 5, keep_first=(1 << 33) + 1)
+    args = dict(launches)[kernel]
+    sizes = [a for a in args if isinstance(a, int)]
+    assert (1 << 32) + 5 not in sizes and (1 << 33) + 1 not in sizes
+    at = max(i for i in range(len(args) - 2) if args[i] == 2 and i > 8)  # blocks, window, keep_first
+    assert args[at + 1] >= 128 and args[at + 2] >= 128 and max(args[at + 1:at + 3]) < 1 << 31
