@@ -154,11 +154,13 @@ def window_attention_q8_cuda(proj, q_norm, k_norm, k, v, k_scale, v_scale, k_tai
     B, G, blocks, _, dim = k.shape
     vdim, dt, dev = v.shape[-1], proj.dtype, proj.device
     plain = (heads + G) * dim + G * vdim
-    if not _ok(k_tail, v_tail, joint, q_norm, k_norm) or not _f32(q_norm, k_norm, k_scale, v_scale) or not _i32(pos, count):
+    proj = proj if proj.stride(1) == 1 else proj.contiguous()
+    given, (q_norm, k_norm) = (q_norm, k_norm), (_rows16(q_norm), _rows16(k_norm))
+    if not _ok(q_norm, k_norm) or not _f32(q_norm, k_norm, k_scale, v_scale) or not _i32(pos, count) or dt not in _CODE:
         return NotImplemented
-    if not (dt == k_tail.dtype == v_tail.dtype == joint.dtype) or proj.stride(1) != 1 or proj.shape[0] != B * T or not proj.is_cuda:
+    if not (dt == k_tail.dtype == v_tail.dtype == joint.dtype) or joint.stride(1) != 1 or proj.shape[0] != B * T:
         return NotImplemented
-    if any(not t.is_contiguous() for t in (k, v, k_scale, v_scale)):
+    if any(not t.is_contiguous() for t in (k, v, k_scale, v_scale, k_tail, v_tail)) or not (proj.is_cuda and k_tail.is_cuda and joint.is_cuda):
         return NotImplemented
     code, s, ld, ldo = _CODE[dt], _stream(), proj.stride(0), joint.stride(0)
     window, keep_first = min(window, blocks * 64), min(keep_first, blocks * 64)  # no key is further back, and the kernels count in 32 bits
@@ -184,7 +186,8 @@ def window_attention_q8_cuda(proj, q_norm, k_norm, k, v, k_scale, v_scale, k_tai
 
     is_few = _q8_few_rows(T * (heads // G), blocks * 64)
     if T == 1 and dt == torch.bfloat16:
-        ahead = read_ahead.allowed(q_norm, k_norm, k, v, k_scale, v_scale, k_tail, v_tail, pos, count)
+        # (a copy of the factors was written just now)
+        ahead = given[0] is q_norm and given[1] is k_norm and read_ahead.allowed(q_norm, k_norm, k, v, k_scale, v_scale, k_tail, v_tail, pos, count)
         if few(None, (None, None), ahead):
             return joint
     aligned = all(t.data_ptr() % 16 == 0 for t in (proj, joint, k, v, k_tail, v_tail))

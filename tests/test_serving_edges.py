@@ -5,6 +5,7 @@ import torch
 
 from popxl_addons_b200 import xl
 from popxl_addons_b200.xl import ops
+from test_dunelix_ops import backend, i32, op  # noqa: F401  (fixture and helpers)
 from test_serving_order import OnDevice
 
 
@@ -93,3 +94,50 @@ def test_windows_wider_than_an_int(launches, T, dtype, kernel):
     assert (1 << 32) + 5 not in sizes and (1 << 33) + 1 not in sizes
     at = max(i for i in range(len(args) - 2) if args[i] == 2 and i > 8)  # blocks, window, keep_first
     assert args[at + 1] >= 128 and args[at + 2] >= 128 and max(args[at + 1:at + 3]) < 1 << 31
+
+
+def shifted(t, by=1):
+    """The same numbers, `by` elements behind a 16-byte boundary."""
+    flat = torch.empty(t.numel() + 16, dtype=t.dtype, device=t.device)
+    assert flat.data_ptr() % 16 == 0
+    flat[by:by + t.numel()] = t.reshape(-1)
+    return flat[by:by + t.numel()].view(t.shape)
+
+
+@pytest.mark.parametrize("T", [1, 5, 130])
+@pytest.mark.parametrize("which", ["norms", "tails", "joint"])
+def test_operands_off_a_16_byte_boundary(backend, which, T):  # noqa: F811
+    """Factors of norms out of a table of odd rows, tails and results inside a larger buffer: taken by the kernels, and with them by a
+    captured program, with the results of operands on such a boundary."""
+    B, (H, G, d, dv), dev, dt = 2, (8, 2, 64, 64), *backend
+    g = torch.Generator().manual_seed(4)
+    cache = [torch.randint(-127, 128, (B, G, 4, 64, w), generator=g).to(torch.int8) for w in (d, dv)] + [torch.full((B, G, 4), 0.02) for _ in range(2)]
+    cache += [torch.randn(B, G, 64, w, generator=g).to(dt) for w in (d, dv)]
+    qn, kn = (1 + 0.3 * torch.randn(d, generator=g) for _ in range(2))
+    proj, joint = torch.randn(B * T, (H + G) * d + G * dv, generator=g).to(dt).to(dev), torch.zeros(B * T, H * dv + 3, dtype=dt)
+    cache, qn, kn, joint = [t.to(dev) for t in cache], qn.to(dev), kn.to(dev), joint.to(dev)
+    how = dict(T=T, heads=H, window=0, keep_first=0, scale=d ** -0.5, sink=None, eps=1e-5)
+    where = (i32(backend, 100, 40), i32(backend, T, T))
+    want_cache = [t.clone() for t in cache]
+    want = op("window_attention_q8_", backend, proj, qn, kn, *want_cache, *where, joint.clone(), **how)
+    if which == "norms":
+        qn, kn = shifted(qn), shifted(kn, 3)
+    elif which == "tails":
+        cache[4:] = [shifted(t) for t in cache[4:]]
+    else:
+        joint = shifted(joint)
+    got = op("window_attention_q8_", backend, proj, qn, kn, *cache, *where, joint, **how)
+    assert all(torch.equal(a, b) for a, b in zip(cache, want_cache))
+    # other kernels may take it: each side is off by two half steps of bf16 at most, 2 * 2^-8, and by 2e-5 in 32 bits
+    assert (got.double() - want.double()).abs().max() <= (4e-5 if dt == torch.float32 else 4 * 2.0 ** -8) * want.double().abs().max()
+
+
+def test_copied_factors_are_not_read_ahead(launches, monkeypatch):
+    """Factors that had to be copied were written by the launch before."""
+    from popxl_addons_b200.ops import native_serving as ns
+
+    monkeypatch.setattr(ns.read_ahead, "allowed", lambda *t: True)
+    call_of_attention()
+    monkeypatch.setattr(ns, "_rows16", lambda t: t.clone())
+    call_of_attention()
+    assert [(name, args[-3]) for name, args in launches] == [("_q8_few", 1), ("_q8_few", 0)]
