@@ -118,11 +118,14 @@ def _q8_slices(units, longest, per_sm, device) -> int:
 _Q8_EXPANDED = 2 << 30  # bytes that the codes of a portion may expand to at a time
 
 
-def _q8_few_rows(rows: int, positions: int) -> bool:
+def _q8_few_rows(rows: int, positions: int, dim: int, vdim: int) -> bool:
     """Whether a portion of `rows` rows per sequence and key head, against a cache of `positions`, runs on mma.sync, which cuts the keys among
     CTAs and reads codes once, and not on the tensor cores, whose keys expand first (2 sequences x 8 key heads of 128 after 6000: 16 rows
-    107 us there, 35 here, 64 rows 113 and 58, 128 rows 117 and 83; 6 x 4 heads after 500: 64 rows 37 and 35, 128 rows 39 and 45)."""
-    return rows <= 64 or (rows <= 128 and positions >= 4096)
+    107 us there, 35 here, 64 rows 113 and 58, 128 rows 117 and 83; 6 x 4 heads after 500: 64 rows 37 and 35, 128 rows 39 and 45).
+    Features that 16 does not divide have no rows that TMA can take: on the tensor cores, which take multiples of 8, they are faster than on the
+    CUDA cores for one token already (2 x 8 key heads of 40 and 24 after 6000: 4 rows 166 -> 107 us, 64 rows 1241 -> 109; 16 x 8 heads of
+    72 after 8000: 4 rows 3354 -> 211; 60 x 4 heads after 100: 33 -> 27), all but a few rows against short caches (6 x 4 heads after 500: 24.6 -> 28.7)."""
+    return dim % 16 == 0 and vdim % 16 == 0 and (rows <= 64 or (rows <= 128 and positions >= 4096))
 
 
 def _q8_portion(at, proj, q_norm, k_norm, cache, pos, count, joint, gate, T, heads, window, keep_first, scale, sink, eps, s):
@@ -173,7 +176,7 @@ def window_attention_q8_cuda(proj, q_norm, k_norm, k, v, k_scale, v_scale, k_tai
         rows = T * (heads // G)
         per = 8 if rows <= 8 else 16  # rows of a CTA
         units = B * G * -(-rows // per)
-        if units > 1 << 16:
+        if dim % 16 or vdim % 16 or units > 1 << 16:
             return False
         longest = min(blocks * 64, window + keep_first + T) if window else blocks * 64
         splits = _q8_slices(units, longest, 3 if per == 8 else 2, dev)
@@ -184,7 +187,7 @@ def window_attention_q8_cuda(proj, q_norm, k_norm, k, v, k_scale, v_scale, k_tai
                      eps, splits, _ptr(part), done.data_ptr(), int(ahead), gemm_error_flag(dev).data_ptr(), s)
         return _launched(rc, "q8_attn_few")
 
-    is_few = _q8_few_rows(T * (heads // G), blocks * 64)
+    is_few = _q8_few_rows(T * (heads // G), blocks * 64, dim, vdim)
     if T == 1 and dt == torch.bfloat16:
         # (a copy of the factors was written just now)
         ahead = given[0] is q_norm and given[1] is k_norm and read_ahead.allowed(q_norm, k_norm, k, v, k_scale, v_scale, k_tail, v_tail, pos, count)

@@ -141,3 +141,12 @@ def test_copied_factors_are_not_read_ahead(launches, monkeypatch):
     monkeypatch.setattr(ns, "_rows16", lambda t: t.clone())
     call_of_attention()
     assert [(name, args[-3]) for name, args in launches] == [("_q8_few", 1), ("_q8_few", 0)]
+
+
+@pytest.mark.parametrize("T", [1, 4, 32])
+@pytest.mark.parametrize("dim,vdim,kernels", [(48, 32, {"_q8_few"}), (40, 24, {"_q8_append_expand", "_q8_tcgen05"}),
+                                              (48, 24, {"_q8_append_expand", "_q8_tcgen05"}), (40, 21, {"_q8_append", "_q8_general"})])
+def test_which_kernel_takes_few_rows(launches, T, dim, vdim, kernels):
+    """No size is kept for a kernel that does not take it: features in multiples of 8, but not of 16, go to the tensor cores."""
+    call_of_attention(T=T, dim=dim, vdim=vdim)
+    assert {name for name, _ in launches} - {"_q8_append"} == kernels - {"_q8_append"}
