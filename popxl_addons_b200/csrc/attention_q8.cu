@@ -119,7 +119,7 @@ __global__ void __launch_bounds__(256) q8_append_kernel(const Q8AppendParams p) 
       const Q8Piece<T, V> piece = *reinterpret_cast<const Q8Piece<T, V>*>(tail[kind] + i);
       *reinterpret_cast<Q8Piece<T, V>*>(raw[kind] + i) = piece;
 #pragma unroll
-      for (int e = 0; e < V; ++e) top[kind] = fmaxf(top[kind], fabsf(xl_to_float(piece.v[e])));
+      for (int e = 0; e < V; ++e) top[kind] = q8_max(top[kind], fabsf(xl_to_float(piece.v[e])));
     }
   }
   for (int i = warp; i < (r1 - first) * items; i += WARPS) {
@@ -151,12 +151,12 @@ __global__ void __launch_bounds__(256) q8_append_kernel(const Q8AppendParams p) 
 #pragma unroll
     for (int u = 0; u < NP; ++u)
 #pragma unroll
-      for (int e = 0; e < V; ++e) top[kind] = fmaxf(top[kind], fabsf(x[u][e]));
+      for (int e = 0; e < V; ++e) top[kind] = q8_max(top[kind], fabsf(x[u][e]));
   }
   if (complete) {
 #pragma unroll
     for (int kind = 0; kind < 2; ++kind) {
-      const float m = xl_warp_max(top[kind]);
+      const float m = q8_warp_max(top[kind]);
       if (lane == 0) tops[kind][warp] = m;
     }
     __syncthreads();  // the raw rows of this block are written
@@ -164,8 +164,8 @@ __global__ void __launch_bounds__(256) q8_append_kernel(const Q8AppendParams p) 
     if (threadIdx.x < 2) {
       const int kind = threadIdx.x;
       float m = 0.f;
-      for (int w = 0; w < WARPS; ++w) m = fmaxf(m, tops[kind][w]);
-      scales[kind] = __fdiv_rn(m, 127.f);
+      for (int w = 0; w < WARPS; ++w) m = q8_max(m, tops[kind][w]);
+      scales[kind] = q8_scale_of(m);
       (kind ? p.vs : p.ks)[at] = scales[kind];
     }
     __syncthreads();
@@ -217,7 +217,8 @@ template <int SEL> __device__ __forceinline__ uint32_t q8_pair(uint32_t biased) 
 // complete blocks as fp16 (keys) and bf16 (values). bf16 projections, dim and vdim multiples of 8 up to 128. Sixteen lanes share a row, 16 bytes
 // each; a CTA has the rows of one block of one key / value head. 2 x 4096 tokens of 32 heads on 8 of 128: 65 us; the fp64 sums of the keys' norms
 // and five layouts of results bound it. Raw value rows that the last block's keys do not fill are zeros: a weight of
-// zero times what memory happened to hold could be NaN.
+// zero times what memory happened to hold could be NaN. For the same reason a raw value that is not finite becomes zero, and its block's
+// `raw_unit` NaN instead of 1: the rows that read the block become NaN by that, and no other row of their tile.
 struct Q8ExpandParams {
   const __nv_bfloat16* proj;
   long long ld;
@@ -225,6 +226,7 @@ struct Q8ExpandParams {
   __half* q;                        // (B, G, T, H/G, dim)
   __half* raw_k;                    // (B, G, raw_rows, dim)
   __nv_bfloat16* raw_v;             // (B, G, raw_rows, vdim)
+  float* raw_unit;                  // (B, G, q8_touched(T))
   __half* kx;                       // (B, G, blocks * 64, dim)
   __nv_bfloat16* vx;                // (B, G, blocks * 64, vdim)
   int8_t *kc, *vc;
@@ -242,6 +244,10 @@ __device__ __forceinline__ void q8_unpack(const uint4& w, float (&x)[8]) {
 __device__ __forceinline__ uint4 q8_halves(const float (&x)[8]) {
   return make_uint4(q8_pack_f16(x[0], x[1]), q8_pack_f16(x[2], x[3]), q8_pack_f16(x[4], x[5]), q8_pack_f16(x[6], x[7]));
 }
+// two bf16 numbers, zero in the place of one that is not finite
+__device__ __forceinline__ uint32_t q8_finite_pair(uint32_t w) {
+  return ((w & 0x7f80u) == 0x7f80u ? 0u : w & 0xffffu) | ((w & 0x7f800000u) == 0x7f800000u ? 0u : w & 0xffff0000u);
+}
 // eight codes as fp16, and as bf16
 __device__ __forceinline__ uint4 q8_code_halves(const uint2& c) {
   const uint32_t a = c.x ^ 0x80808080u, b = c.y ^ 0x80808080u;
@@ -257,7 +263,7 @@ __device__ __forceinline__ uint4 q8_code_values(const uint2& c) {
 __global__ void __launch_bounds__(256, 4) q8_append_expand_kernel(const Q8ExpandParams p) {
   constexpr int HALVES = 16;  // half warps
   __shared__ __align__(16) uint4 tile[2][Q8_BLOCK][16];
-  __shared__ float tops[2][HALVES], scales[2];
+  __shared__ float tops[2][HALVES / 2], scales[2];
   xl_grid_dependency_wait();
   xl_grid_launch_dependents();
   const int blk = blockIdx.x, g = blockIdx.y, b = blockIdx.z, half = threadIdx.x >> 4, l = threadIdx.x & 15, lane = threadIdx.x & 31;
@@ -293,11 +299,13 @@ __global__ void __launch_bounds__(256, 4) q8_append_expand_kernel(const Q8Expand
     return make_uint4(y[0], y[1], y[2], y[3]);
   };
   float top[2] = {0.f, 0.f};
-  auto largest = [&](const uint4& w, float& m) {
+  auto largest = [&](const uint4& w) {
     float x[8];
     q8_unpack(w, x);
+    float m = 0.f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(x[e]));
+    for (int e = 0; e < 8; ++e) m = q8_max(m, fabsf(x[e]));
+    return m;
   };
   auto put_key = [&](int r, const uint4& w) {
     float x[8];
@@ -305,12 +313,14 @@ __global__ void __launch_bounds__(256, 4) q8_append_expand_kernel(const Q8Expand
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] *= inv_k;
     tile[0][r - r0][l] = w;
-    largest(w, top[0]);
+    top[0] = q8_max(top[0], largest(w));
     if (on_k) *reinterpret_cast<uint4*>(p.raw_k + (head * p.raw_rows + r) * p.dim + l * 8) = q8_halves(x);
   };
-  auto put_value = [&](int r, const uint4& w) {
+  auto put_value = [&](int r, uint4 w) {
     tile[1][r - r0][l] = w;
-    largest(w, top[1]);
+    const float m = largest(w);
+    top[1] = q8_max(top[1], m);
+    if (!(m < INFINITY)) w = make_uint4(q8_finite_pair(w.x), q8_finite_pair(w.y), q8_finite_pair(w.z), q8_finite_pair(w.w));
     if (on_v) *reinterpret_cast<uint4*>(p.raw_v + (head * p.raw_rows + r) * p.vdim + l * 8) = w;
   };
   // tokens that were there before
@@ -372,19 +382,21 @@ __global__ void __launch_bounds__(256, 4) q8_append_expand_kernel(const Q8Expand
   }
   for (int r = r1 + half; r < r0 + Q8_BLOCK; r += HALVES)
     if (on_v) *reinterpret_cast<uint4*>(p.raw_v + (head * p.raw_rows + r) * p.vdim + l * 8) = zero;
-  if (r1 == r0 + Q8_BLOCK) {
 #pragma unroll
-    for (int kind = 0; kind < 2; ++kind) {
-      const float m = xl_warp_max(top[kind]);
-      if (lane == 0) tops[kind][threadIdx.x >> 5] = m;
-    }
-    __syncthreads();
-    if (threadIdx.x < 2) {
-      float m = 0.f;
-      for (int w = 0; w < 8; ++w) m = fmaxf(m, tops[threadIdx.x][w]);
-      scales[threadIdx.x] = __fdiv_rn(m, 127.f);
-      (threadIdx.x ? p.vs : p.ks)[at] = scales[threadIdx.x];
-    }
+  for (int kind = 0; kind < 2; ++kind) {
+    const float m = q8_warp_max(top[kind]);
+    if (lane == 0) tops[kind][threadIdx.x >> 5] = m;
+  }
+  __syncthreads();
+  const bool complete = r1 == r0 + Q8_BLOCK;
+  if (threadIdx.x < 2) {
+    float m = 0.f;
+    for (int w = 0; w < HALVES / 2; ++w) m = q8_max(m, tops[threadIdx.x][w]);
+    scales[threadIdx.x] = q8_scale_of(m);
+    if (complete) (threadIdx.x ? p.vs : p.ks)[at] = scales[threadIdx.x];
+    if (threadIdx.x == 1) p.raw_unit[head * gridDim.x + blk] = m < INFINITY ? 1.f : scales[1];
+  }
+  if (complete) {
     __syncthreads();
 #pragma unroll
     for (int kind = 0; kind < 2; ++kind) {
@@ -774,11 +786,16 @@ __global__ void __launch_bounds__(QD_WARPS * 32, RT == 1 ? 3 : 2)
   for (int n = p.stages - 1; n >= 0; --n) prefetch(n);  // codes come from further away than the raw rows
   // ---- scales of the items (read once, by all threads), factors of the norms, and the largest value scale: the unit of the output --
   auto item_block = [&](int it) { return head * p.blocks + first_key(it) / Q8_BLOCK; };
+  // scales of a block; where either is NaN, that of the keys is: the scores that a row sees become NaN, and its weights by them
+  auto factors = [&](long long blk) {
+    const float k = p.ks[blk], v = p.vs[blk];
+    return make_float2(fmaf(v, 0.f, k), fmaxf(v, 0.f));
+  };
   const int tabled = min(it1 - it0, QD_TABLE);
   float top_v = 0.f;
   for (int i = threadIdx.x; i < it1 - it0; i += QD_WARPS * 32) {
     const long long blk = item_block(it0 + i);
-    const float2 x = make_float2(p.ks[blk], p.vs[blk]);
+    const float2 x = factors(blk);
     if (i < QD_TABLE) table[i] = x;
     top_v = fmaxf(top_v, x.y);
   }
@@ -974,13 +991,13 @@ __global__ void __launch_bounds__(QD_WARPS * 32, RT == 1 ? 3 : 2)
       auto largest = [&](const uint4& w, float& m) {
         const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) m = fmaxf(m, fmaxf(fabsf(dd_lo(u[e])), fabsf(dd_hi(u[e]))));
+        for (int e = 0; e < 4; ++e) m = q8_max(m, q8_max(fabsf(dd_lo(u[e])), fabsf(dd_hi(u[e]))));
       };
       for (int i = lane; i < QD_RAW * (DK / 8); i += 32) largest(*reinterpret_cast<const uint4*>(st + i * 16), top[0]);
       for (int i = lane; i < QD_RAW * (DV / 8); i += 32) largest(*reinterpret_cast<const uint4*>(sv + i * 16), top[1]);
 #pragma unroll
       for (int kind = 0; kind < 2; ++kind) {
-        const float m = xl_warp_max(top[kind]);
+        const float m = q8_warp_max(top[kind]);
         if (lane == 0) tops[1 + kind][warp] = m;
       }
       __syncthreads();
@@ -989,8 +1006,8 @@ __global__ void __launch_bounds__(QD_WARPS * 32, RT == 1 ? 3 : 2)
 #pragma unroll
       for (int kind = 0; kind < 2; ++kind) {
         float m = tops[1 + kind][0];
-        for (int w = 1; w < QD_WARPS; ++w) m = fmaxf(m, tops[1 + kind][w]);
-        scale[kind] = __fdiv_rn(m, 127.f);
+        for (int w = 1; w < QD_WARPS; ++w) m = q8_max(m, tops[1 + kind][w]);
+        scale[kind] = q8_scale_of(m);
         if (threadIdx.x == 0) (kind ? p.vs : p.ks)[blk] = scale[kind];
       }
       const Q8Step step_k(scale[0]), step_v(scale[1]);
@@ -1012,6 +1029,22 @@ __global__ void __launch_bounds__(QD_WARPS * 32, RT == 1 ? 3 : 2)
           write(*reinterpret_cast<const uint4*>(sv + r * (DV * 2) + ((c ^ (r & 6)) * 16)), p.vc + (blk * Q8_BLOCK + r0 + r) * p.vdim + c * 8, step_v);
       }
     }
+    // Rows of different positions share a product, where a weight of zero times a value that is not finite would reach positions that do
+    // not see it: such a key's values become zero, its scores NaN. (Of a single token every row sees the same keys.)
+    uint32_t bad = 0u;  // bits 2 r, 2 r + 1: row r of the tile
+    if (!FUSED) {
+      bool any = false;
+      const int r = lane >> 1;
+#pragma unroll
+      for (int c8 = lane & 1; c8 < DV / 8; c8 += 2) {
+        const uint4 w = *reinterpret_cast<const uint4*>(sv + r * (DV * 2) + ((c8 ^ (r & 6)) * 16));
+        const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) any |= q8_finite_pair(x[e]) != x[e];
+      }
+      bad = __ballot_sync(0xffffffffu, any);
+    }
+    auto is_bad = [&](int r) { return (bad >> (2 * r) & 3u) != 0u; };
     float s[1][RT][4];
 #pragma unroll
     for (int m = 0; m < RT; ++m)
@@ -1040,7 +1073,10 @@ __global__ void __launch_bounds__(QD_WARPS * 32, RT == 1 ? 3 : 2)
 #pragma unroll
     for (int m = 0; m < RT; ++m)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[0][m][e] = sees(qpos[m][e & 1], key0 + quad + 8 * (e >> 1), true) ? s[0][m][e] * c : -INFINITY;
+      for (int e = 0; e < 4; ++e) {
+        if (!FUSED && bad && is_bad(quad + 8 * (e >> 1))) s[0][m][e] = __uint_as_float(0x7fc00000u);
+        s[0][m][e] = sees(qpos[m][e & 1], key0 + quad + 8 * (e >> 1), true) ? s[0][m][e] * c : -INFINITY;
+      }
     softmax(s);
     uint32_t ph[RT][2], pl[RT][2];  // weights in units of `ref` as operands of the second product, and their rounding errors
 #pragma unroll
@@ -1055,8 +1091,8 @@ __global__ void __launch_bounds__(QD_WARPS * 32, RT == 1 ? 3 : 2)
     bool seen[4];  // rows 2 j, 2 j + 1, 2 j + 8, 2 j + 9 of the tile: one that no row sees may hold anything
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const int key = key0 + 2 * j + (e & 1) + 8 * (e >> 1);
-      seen[e] = key <= p_hi && (!p.window || key >= p_lo - p.window + 1 || key < p.keep_first);
+      const int r = 2 * j + (e & 1) + 8 * (e >> 1), key = key0 + r;
+      seen[e] = key <= p_hi && (!p.window || key >= p_lo - p.window + 1 || key < p.keep_first) && (FUSED || !is_bad(r));
     }
 #pragma unroll
     for (int t = 0; t < VT; ++t) {
@@ -1084,7 +1120,7 @@ __global__ void __launch_bounds__(QD_WARPS * 32, RT == 1 ? 3 : 2)
     const int n = n_raw + i, slot = n % p.stages, key0 = first_key(it0 + warp + i * QD_WARPS);
     const int it = warp + i * QD_WARPS;
     float2 scale = it < tabled ? table[it] : make_float2(0.f, 0.f);
-    if (it >= tabled) scale = make_float2(p.ks[item_block(it0 + it)], p.vs[item_block(it0 + it)]);
+    if (it >= tabled) scale = factors(item_block(it0 + it));
     const float c = c_unit * scale.x, rel = scale.y * inv_ref;
     ok = mbar_wait_warp(&bars[warp][slot], (uint32_t)(i / p.stages) & 1u, &abort_flag, p.err, ERR_Q8_CODES);
     if (!ok) {
@@ -1224,7 +1260,7 @@ __global__ void __launch_bounds__(QD_WARPS * 32, RT == 1 ? 3 : 2)
     for (int w = 0; w < QD_WARPS; ++w) {
       const float f = sm[w][r] == -INFINITY ? 0.f : xl_tc::fast_exp2(sm[w][r] - m);
       fw[w][r] = f;
-      ll += sm[w][r] == -INFINITY ? 0.f : sl[w][r] * f;
+      ll += sl[w][r] * f;  // NaN where the warp's only visible keys were no numbers, and its maximum says nothing of them
     }
     fl[r] = ll;
     if (splits > 1) __stcg(stats + (unit * splits + split) * ROWS + r, make_float2(m, ll));
@@ -1291,7 +1327,7 @@ __global__ void __launch_bounds__(QD_WARPS * 32, RT == 1 ? 3 : 2)
         for (int k = 0; k < splits; ++k) {
           const float f = wt[k * ROWS + r];
           const float4 x = __ldcg(reinterpret_cast<const float4*>(src + (long long)k * ROWS * p.vdim));
-          if (f != 0.f) a = make_float4(a.x + x.x * f, a.y + x.y * f, a.z + x.z * f, a.w + x.w * f);
+          a = make_float4(a.x + x.x * f, a.y + x.y * f, a.z + x.z * f, a.w + x.w * f);
         }
       } else {
         a = merged(r, c);
@@ -1366,7 +1402,7 @@ XL_API int xl_q8_append(const void* proj, long long ld, const float* wq, const f
   if (!q8_sizes_ok(B, T, H, G, dim, vdim, blocks) || ld < (long long)(H + G) * dim + (long long)G * vdim || !wq || !wk) return -1;
   const Q8AppendParams p{proj, ld, wq, wk, q, raw_k, raw_v, (int8_t*)kc, (int8_t*)vc, ks, vs, kt, vt, pos, count, T, H, G, dim, vdim,
                          blocks, eps};
-  const dim3 grid((T + 2 * Q8_BLOCK - 2) / Q8_BLOCK, G, B);
+  const dim3 grid(q8_touched(T), G, B);
   XL_DISPATCH_DTYPE(dtype, D, {
     const uintptr_t at = (uintptr_t)proj | (uintptr_t)raw_k | (uintptr_t)raw_v | (uintptr_t)kc | (uintptr_t)vc | (uintptr_t)kt | (uintptr_t)vt;
     const bool four = dim % 4 == 0 && vdim % 4 == 0 && ld % 4 == 0 && (at & 15) == 0;
@@ -1429,22 +1465,22 @@ XL_API int xl_q8_attn_few(const void* proj, long long ld, const float* wq, const
 }
 
 // The same as xl_q8_append for xl_q8_attn_tcgen05 (see there): q (B, G, T, H/G, dim) and raw_k (B, G, raw_rows, dim) fp16, raw_v (B, G,
-// raw_rows, vdim) bf16 with raw_rows >= T + 128, kx (B, G, blocks * 64, dim) fp16, vx (.., vdim) bf16: complete blocks that the portion
-// can see. bf16; dim, vdim multiples of 8 up to 128, ld a multiple of 8, all pointers 16-byte aligned.
+// raw_rows, vdim) bf16 with raw_rows >= T + 128, raw_unit (B, G, (T + 126) / 64) fp32, kx (B, G, blocks * 64, dim)
+// fp16, vx (.., vdim) bf16: complete blocks that the portion can see. bf16; dim, vdim multiples of 8 up to 128, ld a multiple of 8, all pointers 16-byte aligned.
 XL_API int xl_q8_append_expand(const void* proj, long long ld, const float* wq, const float* wk, void* q, void* raw_k, void* raw_v,
-                               int raw_rows, void* kx, void* vx, void* kc, void* vc, float* ks, float* vs, void* kt, void* vt,
+                               int raw_rows, float* raw_unit, void* kx, void* vx, void* kc, void* vc, float* ks, float* vs, void* kt, void* vt,
                                const int* pos, const int* count, int B, int T, int H, int G, int dim, int vdim, int blocks, int window,
                                int keep_first, double eps, cudaStream_t s) {
-  if (!q8_sizes_ok(B, T, H, G, dim, vdim, blocks) || dim % 8 || vdim % 8 || dim > 128 || vdim > 128 || ld % 8 || !wq || !wk ||
+  if (!q8_sizes_ok(B, T, H, G, dim, vdim, blocks) || dim % 8 || vdim % 8 || dim > 128 || vdim > 128 || ld % 8 || !wq || !wk || !raw_unit ||
       ld < (long long)(H + G) * dim + (long long)G * vdim || raw_rows < T + 2 * Q8_BLOCK || window < 0 || keep_first < 0)
     return -1;
   const uintptr_t at = (uintptr_t)proj | (uintptr_t)q | (uintptr_t)raw_k | (uintptr_t)raw_v | (uintptr_t)kx | (uintptr_t)vx | (uintptr_t)kc |
                        (uintptr_t)vc | (uintptr_t)kt | (uintptr_t)vt;
   if (at & 15) return -1;
-  const Q8ExpandParams p{(const __nv_bfloat16*)proj, ld, wq, wk, (__half*)q, (__half*)raw_k, (__nv_bfloat16*)raw_v, (__half*)kx,
+  const Q8ExpandParams p{(const __nv_bfloat16*)proj, ld, wq, wk, (__half*)q, (__half*)raw_k, (__nv_bfloat16*)raw_v, raw_unit, (__half*)kx,
                          (__nv_bfloat16*)vx, (int8_t*)kc, (int8_t*)vc, ks, vs, (__nv_bfloat16*)kt, (__nv_bfloat16*)vt, pos, count, T, H, G, dim,
                          vdim, blocks, raw_rows, window, keep_first, eps, 1.0 / dim};
-  XL_TRY(xl_launch_overlapped(q8_append_expand_kernel, dim3((T + 2 * Q8_BLOCK - 2) / Q8_BLOCK, G, B), dim3(256), (size_t)0, s, p));
+  XL_TRY(xl_launch_overlapped(q8_append_expand_kernel, dim3(q8_touched(T), G, B), dim3(256), (size_t)0, s, p));
   XL_TRY(xl_launch_overlapped(q8_expand_kernel, dim3((blocks + Q8_EXPAND_GROUP - 1) / Q8_EXPAND_GROUP, G, B), dim3(256), (size_t)0, s, p));
   return (int)cudaGetLastError();
 }

@@ -1,7 +1,8 @@
 // Layout of attention against a key / value cache of 8 bits (attention_q8.cu, attention_q8_tcgen05.cu).
 //
 //   k codes (B, G, blocks, 64, dim) int8, v codes (B, G, blocks, 64, vdim) int8, scales (B, G, blocks) fp32:
-//     value = code * scale, scale = max |x| / 127 over the block, code = x / scale rounded to the nearest whole number
+//     value = code * scale, scale = max |x| / 127 over the block, code = x / scale rounded to the nearest whole number;
+//     a block that holds a number that is not finite: scale NaN, codes 0
 //   tails (B, G, 64, dim | vdim): the block in progress, as it was computed
 //
 // A position reads its own block as it was computed and earlier blocks from the codes. For a portion of T tokens the rows of the
@@ -10,6 +11,8 @@
 #include "attention_window.cuh"
 
 constexpr int Q8_BLOCK = 64;
+// blocks that a portion of T tokens can touch, wherever it begins
+__host__ __device__ constexpr int q8_touched(int T) { return (T + 2 * Q8_BLOCK - 2) / Q8_BLOCK; }
 
 // A power of two above every factor of a norm: normalised rows divided by it are at most sqrt(features) and fit 16-bit floats. `top`: the
 // largest absolute factor that the lane has seen; the result is that of the warp.
@@ -23,10 +26,25 @@ __device__ __forceinline__ float q8_norm_unit(const float* w, int dim, int lane)
   return q8_norm_unit(top);
 }
 
+// The larger of two numbers, NaN where either is one (fmaxf drops a NaN); of a warp; and the scale of a block from its largest absolute value.
+__device__ __forceinline__ float q8_max(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float q8_warp_max(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = q8_max(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+__device__ __forceinline__ float q8_scale_of(float top) { return top < INFINITY ? __fdiv_rn(top, 127.f) : __uint_as_float(0x7fc00000u); }
+// Whether positions that read a block of such scales (of its keys, of its values) become NaN
+__device__ __forceinline__ bool q8_spoiled(float k_scale, float v_scale) { return !(k_scale + v_scale < INFINITY); }
+
 // Codes of a block: x / scale rounded to the nearest whole number. A product with the reciprocal is off by less than 2^-15 (three roundings of
 // numbers below 128), so
 // only next to the middle between two codes does it take the division to know. Added to 1.5 * 2^23, a number of at most 127 leaves its
-// nearest whole number in the low bits of the sum.
+// nearest whole number in the low bits of the sum. A scale that is NaN makes every code zero.
 struct Q8Step {
   float scale, inv;
   __device__ __forceinline__ explicit Q8Step(float s) : scale(s), inv(s > 1e-30f ? 1.f / s : 0.f) {}

@@ -48,6 +48,7 @@ struct Q8PortionParams {
   int T, H, G, dim, vdim, blocks, raw_rows, window, keep_first;
   float scale, sink;
   const float *ks, *vs, *wq, *wk;  // scales of the blocks (B, G, blocks), factors of the norms
+  const float* raw_unit;           // (B, G, q8_touched(T)): 1, or NaN for a raw block with a value that is not finite
   int* err;
 };
 
@@ -289,8 +290,11 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     const float unit_q = q8_norm_unit(p.wq, p.dim, lane), unit_k = q8_norm_unit(p.wk, p.dim, lane);
     const float c = p.scale * 1.4426950408889634f * unit_q;
     const float *ks = p.ks + (long long)(b * p.G + g) * p.blocks, *vs = p.vs + (long long)(b * p.G + g) * p.blocks;
+    const float* raw_unit = p.raw_unit + (long long)(b * p.G + g) * q8_touched(p.T);
     // Scores differ in their factors: the maximum is held in units of the exponent. A factor is never zero (the scale of a block of zeros):
-    // minus infinity, a masked score, has to stay what it is; the values' scale is finite: a weight of zero has to stay zero.
+    // minus infinity, a masked score, has to stay what it is; the values' factor is finite: a weight of zero has to stay zero. Where the
+    // scale is NaN (a block that held a number that is not finite; its codes are zero) the sum of every row that reads the block becomes NaN,
+    // and no other.
     float mx = p.sink * 1.4426950408889634f, l = p.sink == -INFINITY ? 0.f : 1.f;
     float ch = 0.f, vh = 0.f;  // factors of the next block
     auto ask = [&](int j) {
@@ -300,7 +304,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         vh = vs[blk];
       } else {
         ch = unit_k;
-        vh = 1.f;
+        vh = raw_unit[block_of(j) - base];
       }
     };
     ask(0);
@@ -309,6 +313,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       const int buf = 2 * m + (j & 1);
       const bool raw = j >= n_code;
       const float fs = fmaxf(c * ch, 1e-37f), fv = fminf(vh, 1e37f);
+      const bool spoiled = q8_spoiled(ch, vh);
       if (j + 1 < n_kv) ask(j + 1);
       // keys that the row sees: of a raw block its own, of codes the earlier ones; its window, and the kept first tokens
       const int blk = block_of(j), col0 = blk * BKV;
@@ -321,6 +326,7 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           vis[k] = bits_of(from - at, end - at) | bits_of(first - at, min(p.keep_first, end) - at);
         }
       }
+      if (spoiled && (vis[0] | vis[1])) l = __uint_as_float(0x7fc00000u);
       const uint32_t tmem_s = tmem_base + lane_base + buf * BKV;
       ok = mbar_wait_warp(&s_full[buf], (uint32_t)(j >> 1) & 1u, abort_flag, p.err, ERR_S);
       if (!ok) break;
@@ -462,18 +468,18 @@ int launch(const void* q, const void* kx, const void* vx, const void* raw_k, con
 }  // namespace
 
 // After xl_q8_append_expand: q16 (B, G, T, H/G, dim) fp16, codes as fp16 kx (B, G, blocks * 64, dim) and bf16 vx (.., vdim), raw rows as
-// fp16 raw_k and bf16 raw_v (B, G, raw_rows, dim | vdim); ks, vs (B, G, blocks) the scales, wq and wk the factors of the norms; gate:
-// first gate column of the projections (row stride ldg), or null; out (B*T, ldo). dim, vdim multiples of 8 and at most 128; ldg, ldo
-// multiples of 8; all pointers 16-byte aligned. Rows past count[b] are not written. err: device int for the code of a wait that gave up.
+// fp16 raw_k and bf16 raw_v (B, G, raw_rows, dim | vdim), raw_unit (B, G, (T + 126) / 64); ks, vs (B, G, blocks) the scales, wq and wk
+// the factors of the norms; gate: first gate column of the projections (row stride ldg), or null; out (B*T, ldo). dim, vdim multiples of
+// 8 and at most 128; ldg, ldo multiples of 8; all pointers but those of fp32 numbers 16-byte aligned. Rows past count[b] are not written. err: device int for the code of a wait that gave up.
 // Returns 0, a CUDA error code, or a negative value for arguments this kernel does not take.
 XL_API int xl_q8_attn_tcgen05(const void* q16, const void* kx, const void* vx, const void* raw_k, const void* raw_v, int raw_rows,
-                              const float* ks, const float* vs, const float* wq, const float* wk, const void* gate, long long ldg,
-                              void* out, long long ldo, const int* pos, const int* count, int B, int T, int H, int G, int dim, int vdim,
+                              const float* raw_unit, const float* ks, const float* vs, const float* wq, const float* wk, const void* gate,
+                              long long ldg, void* out, long long ldo, const int* pos, const int* count, int B, int T, int H, int G, int dim, int vdim,
                               int blocks, int window, int keep_first, float scale, float sink, int* err, cudaStream_t s) {
   if (B < 1 || B > 65535 || T < 1 || G < 1 || H < 1 || H % G || blocks < 1 || blocks > (1 << 24) || window < 0 || keep_first < 0 || !(scale > 0.f))
     return -1;
   if (dim < 8 || dim > 128 || dim % 8 || vdim < 8 || vdim > 128 || vdim % 8 || ldo % 8 || ldo < (long long)H * vdim ||
-      (gate && (ldg % 8 || ldg < (long long)H * vdim)) || raw_rows < T + 2 * Q8_BLOCK)
+      (gate && (ldg % 8 || ldg < (long long)H * vdim)) || raw_rows < T + 2 * Q8_BLOCK || !raw_unit)
     return -1;
   if (((uintptr_t)q16 | (uintptr_t)kx | (uintptr_t)vx | (uintptr_t)raw_k | (uintptr_t)raw_v | (uintptr_t)gate | (uintptr_t)out) & 15) return -1;
   const long long limit = 0x7fffffffLL - 4 * TILE_M;
@@ -483,7 +489,7 @@ XL_API int xl_q8_attn_tcgen05(const void* q16, const void* kx, const void* vx, c
   Q8PortionParams p = {};
   p.pos = pos; p.count = count; p.gate = (const __nv_bfloat16*)gate; p.ldg = ldg; p.out = (__nv_bfloat16*)out; p.ldo = ldo;
   p.T = T; p.H = H; p.G = G; p.dim = dim; p.vdim = vdim; p.blocks = blocks; p.raw_rows = raw_rows; p.window = window;
-  p.keep_first = keep_first; p.scale = scale; p.sink = sink; p.ks = ks; p.vs = vs; p.wq = wq; p.wk = wk; p.err = err;
+  p.keep_first = keep_first; p.scale = scale; p.sink = sink; p.ks = ks; p.vs = vs; p.wq = wq; p.wk = wk; p.raw_unit = raw_unit; p.err = err;
   if (dim <= 64) return vdim <= 64 ? launch<64, 64>(q16, kx, vx, raw_k, raw_v, p, B, s) : launch<64, 128>(q16, kx, vx, raw_k, raw_v, p, B, s);
   return vdim <= 64 ? launch<128, 64>(q16, kx, vx, raw_k, raw_v, p, B, s) : launch<128, 128>(q16, kx, vx, raw_k, raw_v, p, B, s);
 }

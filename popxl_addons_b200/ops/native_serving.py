@@ -16,8 +16,8 @@ _q8_append = _sig("xl_q8_append", _c_p, _c_ll, *[_c_p] * 13, *[_c_int] * 7, _c_d
 _q8_general = _sig("xl_q8_attn_general", *[_c_p] * 8, _c_ll, _c_p, _c_ll, _c_p, _c_p, *[_c_int] * 9, _c_f, _c_f, _c_int, _c_p)
 _q8_few = _sig("xl_q8_attn_few", _c_p, _c_ll, *[_c_p] * 12, _c_ll, _c_p, _c_p, *[_c_int] * 10, _c_f, _c_f, _c_d, _c_int, _c_p, _c_p, _c_int,
                _c_p, _c_p)
-_q8_append_expand = _sig("xl_q8_append_expand", _c_p, _c_ll, *[_c_p] * 5, _c_int, *[_c_p] * 10, *[_c_int] * 9, _c_d, _c_p)
-_q8_tcgen05 = _sig("xl_q8_attn_tcgen05", *[_c_p] * 5, _c_int, *[_c_p] * 5, _c_ll, _c_p, _c_ll, _c_p, _c_p, *[_c_int] * 9, _c_f, _c_f, _c_p, _c_p)
+_q8_append_expand = _sig("xl_q8_append_expand", _c_p, _c_ll, *[_c_p] * 5, _c_int, *[_c_p] * 11, *[_c_int] * 9, _c_d, _c_p)
+_q8_tcgen05 = _sig("xl_q8_attn_tcgen05", *[_c_p] * 5, _c_int, *[_c_p] * 6, _c_ll, _c_p, _c_ll, _c_p, _c_p, *[_c_int] * 9, _c_f, _c_f, _c_p, _c_p)
 _adapter_down = _sig("xl_adapter_down", *[_c_p] * 5, _c_ll, *[_c_int] * 5, _c_p)
 _adapter_up = _sig("xl_adapter_up", *[_c_p] * 5, _c_ll, *[_c_int] * 6, _c_p)
 _adapter_down_mma = _sig("xl_adapter_down_mma", *[_c_p] * 5, _c_ll, *[_c_int] * 5, _c_p)
@@ -137,16 +137,17 @@ def _q8_portion(at, proj, q_norm, k_norm, cache, pos, count, joint, gate, T, hea
     q = torch.empty((B, G, T, heads // G, dim), dtype=torch.float16, device=dev)
     raw_k = torch.empty((B, G, rows, dim), dtype=torch.float16, device=dev)
     raw_v = torch.empty((B, G, rows, vdim), dtype=torch.bfloat16, device=dev)
+    raw_unit = torch.empty((B, G, (T + 126) // 64), dtype=torch.float32, device=dev)
     kx = torch.empty((B, G, blocks * 64, dim), dtype=torch.float16, device=dev)
     vx = torch.empty((B, G, blocks * 64, vdim), dtype=torch.bfloat16, device=dev)
     sizes = (B, T, heads, G, dim, vdim, blocks, window, keep_first)
     norms, where = (q_norm.data_ptr(), k_norm.data_ptr()), (pos.data_ptr(), count.data_ptr())
-    rc = _q8_append_expand(proj.data_ptr() + row0 * ld * 2, ld, *norms, q.data_ptr(), raw_k.data_ptr(), raw_v.data_ptr(), rows, kx.data_ptr(),
-                           vx.data_ptr(), *map(_ptr, cache), *where, *sizes, eps, s)
+    rc = _q8_append_expand(proj.data_ptr() + row0 * ld * 2, ld, *norms, q.data_ptr(), raw_k.data_ptr(), raw_v.data_ptr(), rows, raw_unit.data_ptr(),
+                           kx.data_ptr(), vx.data_ptr(), *map(_ptr, cache), *where, *sizes, eps, s)
     _done(rc, "q8_append_expand")
     _count("q8_expand")
-    rc = _q8_tcgen05(q.data_ptr(), kx.data_ptr(), vx.data_ptr(), raw_k.data_ptr(), raw_v.data_ptr(), rows, cache[2].data_ptr(), cache[3].data_ptr(), *norms,
-                     gate + row0 * ld * 2 if gate else None, ld, joint.data_ptr() + row0 * ldo * 2, ldo, *where, *sizes, scale, sink,
+    rc = _q8_tcgen05(q.data_ptr(), kx.data_ptr(), vx.data_ptr(), raw_k.data_ptr(), raw_v.data_ptr(), rows, raw_unit.data_ptr(), cache[2].data_ptr(),
+                     cache[3].data_ptr(), *norms, gate + row0 * ld * 2 if gate else None, ld, joint.data_ptr() + row0 * ldo * 2, ldo, *where, *sizes, scale, sink,
                      gemm_error_flag(dev).data_ptr(), s)
     _done(rc, "q8_attn_tcgen05")
 

@@ -6,9 +6,10 @@ Portions, `pos` and `count` are those of the sequence ops (`sequence.py`): `batc
 
 The cache (`Cache8`) holds keys and values in blocks of `CACHE8_BLOCK` tokens. A block that is complete is held as codes of 8
 bits with one scale per block and head: `value = code * scale`, `scale` a 127th of the block's largest absolute value, `code` the
-nearest whole number. The block in progress is held as it was computed, in the tail. A position sees its own block as it was
-computed and earlier blocks as the cache holds them, whatever portions a prompt is cut into, and a code depends on nothing but the
-block: norms of keys are taken in 64 bits and rounded once, so that every kernel, and the CPU, comes to the same codes.
+nearest whole number (of a block that is not finite throughout: scale NaN, codes zero). The block in progress is held as it was
+computed, in the tail. A position sees its own block as it was computed and earlier blocks as the cache holds them, whatever portions
+a prompt is cut into, and a code depends on nothing but the block: norms of keys are taken in 64 bits and rounded once, so that
+every kernel, and the CPU, comes to the same codes.
 Positions only move forward: a sequence may go back to a multiple of `CACHE8_BLOCK`, but not into a block that is complete.
 
 No counterpart in the reference (it ships no cache or generation loop).
@@ -66,10 +67,10 @@ class LogitRules(NamedTuple):
 
 def quantize_block(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """Codes and scales of complete blocks `(..., CACHE8_BLOCK, width)`. Divisions are true divisions: a product with the
-    reciprocal would come to other codes next to a border."""
+    reciprocal would come to other codes next to a border. A block that holds a number that is not finite: scale NaN, codes zero."""
     x = x.float()
     top = x.abs().amax((-2, -1))
-    scale = top / torch.full_like(top, 127.0)
+    scale = torch.where(torch.isfinite(top), top / torch.full_like(top, 127.0), torch.full_like(top, float("nan")))
     code = torch.where(scale[..., None, None] > 0, (x / scale[..., None, None]).round(), torch.zeros_like(x))
     return code.clamp(-127, 127).to(torch.int8), scale
 
@@ -108,6 +109,9 @@ def _window_attention_q8_ref(proj, q_norm, k_norm, k, v, k_scale, v_scale, k_tai
             if window:
                 mask &= (qp - kp < window) | (kp < keep_first)
             s = torch.einsum("ngrd,gkd->grnk", q[i0 - p:i1 - p], keys) * scale
+            known = torch.isfinite(vals)  # a value that is not finite reaches those who see it, and not by a weight of zero
+            s = s.masked_fill(~known.all(-1)[:, None, None], float("nan"))
+            vals = vals.masked_fill(~known, 0.0)
             s = s.masked_fill(~mask, float("-inf"))
             if sink is not None:
                 s = torch.cat((s, torch.full_like(s[..., :1], sink)), dim=-1)
@@ -239,8 +243,10 @@ def window_attention_q8_(proj: Tensor, q_norm: Tensor, k_norm: Tensor, cache: Ca
     """`window_attention_` against a cache of 8 bits: `proj` rows are `[q: heads x dim | k: G x dim | v: G x vdim | gate: heads x
     vdim]` (the gate may be absent), every query and key head gets an RMS norm, keys and values join the cache, and the gated
     attention goes to the first `heads * vdim` columns of `joint`. A sequence that would not fit the cache is left out, rows past
-    `count[b]` are left as they are. A key or value that is not finite has no code: it spoils the positions that read its block, of
-    the portion that brings it from the block's first one on."""
+    `count[b]` are left as they are. A key or value that is not finite has no code: the scale of its block becomes NaN, and with it the
+    results, for the heads that share the key, of every later position that reads the block. Of the block's own positions those that see the
+    token become NaN or infinite in at least the feature concerned; the others may, in the portion that brings it. No position that does not
+    read the block is touched."""
     if cache.k.rank != 5 or cache.v.rank != 5:
         raise ValueError("the codes of a cache are (batch, heads, blocks, tokens, features)")
     B, G, blocks, _, dim = cache.k.shape
