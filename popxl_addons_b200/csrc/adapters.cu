@@ -6,9 +6,10 @@
 // with the r numbers between them in fp32, `low` (rows, rp), rp = r rounded up to 16, filled with zeros, scale included:
 //   xl_adapter_down        any type: one warp per number, which reads one row of A (40 rows x 4096, rank 16: 8 us)
 //   xl_adapter_up          any type: adds the second term to the shared product in fp32 and rounds once (40 rows x 32256: 11 us)
-//   xl_adapter_down_mma, xl_adapter_up_mma   16-bit types, many rows of a sequence: mma.sync. The second writes the adapters' term alone,
-//       rounded to the model's type, for the shared product to accumulate on: a second rounding, of the smaller part of the sum, instead of
-//       moving the whole result in 32 bits (4 bytes more per value written and read again; 4096 x 32256: 160 us).
+//   xl_adapter_down_mma, xl_adapter_up_mma   the same for 16-bit types and many rows of a sequence, on mma.sync
+// Either second half takes the shared product in 32 bits and rounds the sum once. An adapters' term in 16 bits, for the shared product to
+// accumulate on, would move 4 bytes less per value (4096 x 32256: 82 us of 845), but its rounding is half a step of the term, which
+// nothing keeps below the sum: where the two cancel it would be all there is, and in fp16 the term may be past 65504 where the sum is not.
 #include "common.cuh"
 
 #include <type_traits>
@@ -195,10 +196,10 @@ template <typename T, int NT> __global__ void __launch_bounds__(NT <= 2 ? 512 : 
   }
 }
 
-// Grid (columns / 128, row tiles of 256, sequences): the adapters' term alone, rounded to T. A warp has 32 columns for all rows of the tile,
-// whose row of B[s] it holds; its lanes' columns are chosen so that each ends up with eight neighbours, which leave in one store. `low`
-// enters as sums of two T (value and rounding error). Writing the result bounds it: 4 x 1024 rows x 32256 take 60 us (4.4 TB/s; in tiles of 64
-// rows, each with its own chain of loads before the first store, 74). KS: steps of 16 numbers.
+// Grid (columns / 128, row tiles of 256, sequences): the shared product + the adapters' term, rounded to T. A warp has 32 columns for all rows of
+// the tile, whose row of B[s] it holds; its lanes' columns are chosen so that each ends up with eight neighbours, which arrive in two loads
+// and leave in one store. `low` enters as sums of two T (value and rounding error). Moving the results bounds it: 4 x 1024 rows x 32256 take
+// 132 us (793 MB, 6.0 TB/s). KS: steps of 16 numbers.
 constexpr int AD_TILE = 256;
 template <typename T, int KS> __global__ void __launch_bounds__(128) adapter_up_mma_kernel(const AdapterParams p) {
   xl_grid_dependency_wait();
@@ -208,6 +209,7 @@ template <typename T, int KS> __global__ void __launch_bounds__(128) adapter_up_
   const int t0 = blockIdx.y * AD_TILE, s = adapter_of(p, seq), rows = min(AD_TILE, p.T - t0), c0 = blockIdx.x * 128 + warp * 32;
   if (c0 >= p.N) return;
   T* out = (T*)p.out + (seq * p.T + t0) * p.N;
+  const float* y = p.y + (seq * p.T + t0) * p.N;
   const float* low = p.low + (seq * p.T + t0) * p.rp;
   const bool wide = p.N % 8 == 0;
   uint32_t b[4][KS][2];
@@ -236,6 +238,19 @@ template <typename T, int KS> __global__ void __launch_bounds__(128) adapter_up_
   }
 #pragma unroll 2
   for (int m = 0; m * 16 < rows; ++m) {
+    float sum[2][8];  // rows quad, quad + 8: the shared product, asked for ahead of what is added to it
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = m * 16 + quad + 8 * h, c1 = c0 + 8 * j;
+      const float* src = y + (long long)r * p.N + c1;
+      if (wide && r < rows && c1 < p.N) {
+        *reinterpret_cast<float4*>(&sum[h][0]) = __ldcs(reinterpret_cast<const float4*>(src));
+        *reinterpret_cast<float4*>(&sum[h][4]) = __ldcs(reinterpret_cast<const float4*>(src + 4));
+      } else {
+#pragma unroll
+        for (int q = 0; q < 8; ++q) sum[h][q] = r < rows && c1 + q < p.N ? src[q] : 0.f;
+      }
+    }
     float c[4][4];
 #pragma unroll
     for (int u = 0; u < 4; ++u)
@@ -292,8 +307,9 @@ template <typename T, int KS> __global__ void __launch_bounds__(128) adapter_up_
       uint32_t w[4];
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        if constexpr (std::is_same<T, __half>::value) w[u] = ad_pack<T>(c[u][2 * h] * up[h], c[u][2 * h + 1] * up[h]);
-        else w[u] = ad_pack<T>(c[u][2 * h], c[u][2 * h + 1]);
+        if constexpr (std::is_same<T, __half>::value)
+          w[u] = ad_pack<T>(fmaf(c[u][2 * h], up[h], sum[h][2 * u]), fmaf(c[u][2 * h + 1], up[h], sum[h][2 * u + 1]));
+        else w[u] = ad_pack<T>(sum[h][2 * u] + c[u][2 * h], sum[h][2 * u + 1] + c[u][2 * h + 1]);
       }
       if (wide) {
         if (c1 < p.N) *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
@@ -369,14 +385,14 @@ XL_API int xl_adapter_down_mma(const void* x, const void* a, const float* scale,
   return (int)cudaGetLastError();
 }
 
-// out (rows, N) of b's type, 16-byte aligned = low b[slot]^T. 16-bit types, r <= 64; b aligned to 4 bytes.
-XL_API int xl_adapter_up_mma(const float* low, const void* b, const int* slot, void* out, long long rows, int T, int N, int n, int r,
+// out (rows, N) of b's type = y (rows, N) fp32 + low b[slot]^T. 16-bit types, r <= 64; y and out 16-byte aligned, b to 4 bytes.
+XL_API int xl_adapter_up_mma(const float* low, const void* b, const int* slot, const float* y, void* out, long long rows, int T, int N, int n, int r,
                              int dtype, cudaStream_t s) {
-  if (!adapter_sizes_ok(rows, T, 1, N, n, r) || dtype == XL_F32 || (((uintptr_t)out) & 15) || (((uintptr_t)b) & 3) || rows / T > 65535 ||
+  if (!adapter_sizes_ok(rows, T, 1, N, n, r) || dtype == XL_F32 || (((uintptr_t)y | (uintptr_t)out) & 15) || (((uintptr_t)b) & 3) || rows / T > 65535 ||
       (T + AD_TILE - 1) / AD_TILE > 65535)
     return -1;
   AdapterParams p = {};
-  p.b = b; p.slot = slot; p.low = const_cast<float*>(low); p.out = out; p.rows = rows; p.T = T; p.N = N; p.n = n; p.r = r;
+  p.b = b; p.slot = slot; p.low = const_cast<float*>(low); p.y = y; p.out = out; p.rows = rows; p.T = T; p.N = N; p.n = n; p.r = r;
   p.rp = (r + 15) / 16 * 16;
   const dim3 grid((N + 127) / 128, (T + AD_TILE - 1) / AD_TILE, (unsigned)(rows / T));
   void (*kernel)(const AdapterParams);

@@ -5,7 +5,7 @@ import torch
 
 from ..xl import read_ahead
 from ..xl.opdef import native
-from .native import _CODE, _c_f, _c_int, _c_ll, _c_p, _check, _count, _ok, _sig, _sms, _stream, counters, gemm, gemm_error_flag, gemm_pays
+from .native import _CODE, _c_f, _c_int, _c_ll, _c_p, _check, _count, _ok, _sig, _sms, _stream, counters, gemm, gemm_error_flag
 from .native_sequence import _clamped_glu, _f32, _i32, _ptr, _small, product, stream_rms
 
 _c_d = ctypes.c_double
@@ -21,7 +21,7 @@ _q8_tcgen05 = _sig("xl_q8_attn_tcgen05", *[_c_p] * 5, _c_int, *[_c_p] * 6, _c_ll
 _adapter_down = _sig("xl_adapter_down", *[_c_p] * 5, _c_ll, *[_c_int] * 5, _c_p)
 _adapter_up = _sig("xl_adapter_up", *[_c_p] * 5, _c_ll, *[_c_int] * 6, _c_p)
 _adapter_down_mma = _sig("xl_adapter_down_mma", *[_c_p] * 5, _c_ll, *[_c_int] * 5, _c_p)
-_adapter_up_mma = _sig("xl_adapter_up_mma", *[_c_p] * 4, _c_ll, *[_c_int] * 5, _c_p)
+_adapter_up_mma = _sig("xl_adapter_up_mma", *[_c_p] * 5, _c_ll, *[_c_int] * 5, _c_p)
 
 
 def _launched(rc, name) -> bool:
@@ -235,16 +235,16 @@ def linear_adapted_cuda(x, weight, a, b, scale, slot, T, out_dtype):
     if not (T >= 8 and dt != torch.float32 and _launched(_adapter_down_mma(*down), "adapter_down_mma")):
         if not _launched(_adapter_down(*down), "adapter_down"):
             return NotImplemented
-    if dt != torch.float32 and out_dtype == dt and T >= 8 and not _small(x, weight):
-        out = torch.empty((rows, N), dtype=dt, device=dev)
-        if gemm_pays(x, weight.t(), out=out) and _launched(_adapter_up_mma(low.data_ptr(), b.data_ptr(), slot.data_ptr(), out.data_ptr(), rows, T,
-                                                                           N, n, r, code, s), "adapter_up_mma"):
-            if gemm(x, weight.t(), out=out, accumulate=1) is not NotImplemented:
-                return out
-    # 32-bit results also where the GEMM needs copies for them: the sum is rounded once
+    # 32 bits also where the GEMM needs copies for them: the sum is rounded once
     y = product(x, weight, torch.float32) if dt == torch.float32 or _small(x, weight) else gemm(x, weight.t(), out_dtype=torch.float32)
     if y is NotImplemented:
         return NotImplemented
-    out = y if out_dtype == torch.float32 else torch.empty((rows, N), dtype=out_dtype, device=dev)
+    if out_dtype == torch.float32:
+        out = y
+    else:
+        out = torch.empty((rows, N), dtype=out_dtype, device=dev)
+        if T >= 8 and _launched(_adapter_up_mma(low.data_ptr(), b.data_ptr(), slot.data_ptr(), y.data_ptr(), out.data_ptr(), rows, T, N, n, r, code, s),
+                                "adapter_up_mma"):
+            return out
     rc = _adapter_up(low.data_ptr(), b.data_ptr(), slot.data_ptr(), y.data_ptr(), out.data_ptr(), rows, T, N, n, r, code, _CODE[out_dtype], s)
     return out if _launched(rc, "adapter_up") else NotImplemented

@@ -150,3 +150,47 @@ def test_which_kernel_takes_few_rows(launches, T, dim, vdim, kernels):
     """No size is kept for a kernel that does not take it: features in multiples of 8, but not of 16, go to the tensor cores."""
     call_of_attention(T=T, dim=dim, vdim=vdim)
     assert {name for name, _ in launches} - {"_q8_append"} == kernels - {"_q8_append"}
+
+
+def terms_that_cancel(dt, rows, K, N, r, seed=0):
+    """Whole numbers: `x`, a weight that is minus the adapter's product plus a small matrix, and the adapter; all exact in 16 bits."""
+    g = torch.Generator().manual_seed(seed)
+
+    def ints(*shape, most=8):
+        return torch.randint(1, most + 1, shape, generator=g) * (torch.randint(0, 2, shape, generator=g) * 2 - 1)
+
+    a, b = torch.zeros(1, r, K, dtype=torch.int64), torch.zeros(1, N, r, dtype=torch.int64)
+    a[0, 0], b[0, :, 0] = ints(K), ints(N)
+    w = torch.randint(-1, 2, (N, K), generator=g) - b[0] @ a[0]
+    x = torch.randn(rows, K, generator=g).to(dt)
+    return x, w.to(dt), a.to(dt), b.to(dt)
+
+
+@pytest.mark.parametrize("N", [128, 264, 131])
+@pytest.mark.parametrize("T,r", [(1, 1), (7, 16), (8, 1), (8, 16), (40, 24), (300, 16), (8, 100)])
+def test_adapters_that_cancel_the_shared_product(backend, T, r, N):  # noqa: F811
+    """The sum of both products is rounded once, whatever they are by themselves, and however a prompt is cut into portions."""
+    dev, K, seqs = backend[0], 200, 1 if T == 300 else 140 // T
+    for dt in (backend[1],) if backend[1] == torch.float32 else (torch.bfloat16, torch.float16):
+        x, w, a, b = (t.to(dev) for t in terms_that_cancel(dt, seqs * T, K, N, r))
+        y = op("linear_adapted", backend, x, w, a, b, torch.ones(1, device=dev), i32(backend, *[0] * seqs), T=T, out_dtype=dt)
+        term = x.double() @ a[0].double().T @ b[0].double().T
+        want = x.double() @ w.double().T + term
+        assert term.abs().mean() > 15 * want.abs().mean()
+        # half a step of the result; sums of K + r products in 32 bits, 2^-24 each of at most the sum of K absolute terms (some 20 times the
+        # largest); the numbers between the products as two of 8 bits or more, 2^-16 of a term
+        step = 0.0 if dt == torch.float32 else torch.finfo(dt).eps / 2
+        assert ((y.double() - want).abs() <= step * want.abs() + (2.0 ** -15 if dt == torch.bfloat16 else 2.0 ** -18) * term.abs().max()).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [1, 7, 8, 64])
+def test_fp16_adapters_whose_product_alone_is_past_its_range(T):
+    """70000 and -60000 are 10000, although fp16 ends at 65504."""
+    K, N, seqs, dt = 16, 256, 140 // T, torch.float16
+    x = torch.ones(seqs * T, K, dtype=dt, device="cuda")
+    a, b = torch.zeros(1, 8, K, dtype=dt, device="cuda"), torch.zeros(1, N, 8, dtype=dt, device="cuda")
+    a[0, 0, :7], b[0, :, 0] = 1.0, 10000.0
+    w = torch.full((N, K), -3750.0, dtype=dt, device="cuda")
+    y = op("linear_adapted", ("cuda", dt), x, w, a, b, torch.ones(1, device="cuda"), i32(("cuda",), *[0] * seqs), T=T, out_dtype=dt)
+    assert (y == 10000.0).all()
