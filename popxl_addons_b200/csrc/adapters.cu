@@ -259,7 +259,8 @@ template <typename T, int KS> __global__ void __launch_bounds__(128) adapter_up_
     float up[2] = {1.f, 1.f};  // rows quad, quad + 8
     if (s >= 0) {
       float down[2] = {1.f, 1.f};
-      if constexpr (std::is_same<T, __half>::value) {  // fp16 ends at 65504: rows of larger numbers are scaled by a power of two on the way
+      if constexpr (std::is_same<T, __half>::value) {  // fp16 ends at 65504, and keeps ever fewer bits below 2^-14: every row is brought
+                                                       // to numbers of up to 2^15 by a power of two on the way
         float top[2] = {0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < KS * 4; ++i) {
@@ -273,8 +274,8 @@ template <typename T, int KS> __global__ void __launch_bounds__(128) adapter_up_
         for (int i = 0; i < 2; ++i) {
           top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
           top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
-          if (top[i] > 32768.f && top[i] < INFINITY) {
-            const int by = ilogbf(top[i]) - 14;
+          if (top[i] > 0.f && top[i] < INFINITY) {
+            const int by = max(ilogbf(top[i]) - 14, -126);  // both powers are normal numbers
             down[i] = ldexpf(1.f, -by);
             up[i] = ldexpf(1.f, by);
           }

@@ -194,3 +194,21 @@ def test_fp16_adapters_whose_product_alone_is_past_its_range(T):
     w = torch.full((N, K), -3750.0, dtype=dt, device="cuda")
     y = op("linear_adapted", ("cuda", dt), x, w, a, b, torch.ones(1, device="cuda"), i32(("cuda",), *[0] * seqs), T=T, out_dtype=dt)
     assert (y == 10000.0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [1e-3, 1e-6, 1e-9, 1e-38])
+@pytest.mark.parametrize("r", [8, 40])
+def test_small_fp16_numbers_between_the_products(r, size):
+    """What stands between the products may be far below fp16's smallest normal number, 2^-14, in front of large rows of `b`."""
+    T, seqs, K, N, dt = 40, 4, 64, 256, torch.float16
+    g = torch.Generator().manual_seed(2)
+    x, w = torch.randn(seqs * T, K, generator=g).to(dt), torch.zeros(N, K, dtype=dt)
+    a, b = (torch.randn(2, r, K, generator=g) * 0.1).to(dt), (torch.randn(2, N, r, generator=g) * 4000).to(dt)
+    scale = torch.full((2,), size)
+    args = [t.cuda() for t in (x, w, a, b, scale)]
+    y = op("linear_adapted", ("cuda", dt), *args, i32(("cuda",), 0, 1, 1, 0), T=T, out_dtype=dt).double().cpu()
+    for i, s in enumerate((0, 1, 1, 0)):
+        want = scale.double()[s] * (x[i * T:(i + 1) * T].double() @ a[s].double().T @ b[s].double().T)
+        # half a step of the result (of its smallest step where it is below 2^-14), and 2^-18 for sums in 32 bits
+        assert ((y[i * T:(i + 1) * T] - want).abs() <= 2.0 ** -11 * want.abs() + 2.0 ** -25 + 2.0 ** -18 * want.abs().max()).all()
