@@ -187,11 +187,11 @@ __global__ void __launch_bounds__(LG_THREADS)
       }
       asm volatile("cp.async.wait_group 0;" ::: "memory");
       __syncthreads();
-      // the words that are not zero become the shaped logits; a result of zero becomes minus zero, so that it is not taken for none
+      // the words that are not zero become the shaped logits, inverted: then no number is zero (all ones is one of the NaN)
       for (int i = tid; i < changes; i += LG_THREADS) {
         const int w = changed[i];
         const uint32_t y = __float_as_uint(shaped(xl_to_float(held_logits[w]), words[w], repetition, frequency, presence, sums));
-        words[w] = y ? y : 0x80000000u;
+        words[w] = y != 0xffffffffu ? ~y : 0x80000000u;
       }
       __syncthreads();
 #pragma unroll 2
@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(LG_THREADS)
           const uint32_t word[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            x[i + k] = word[k] ? __uint_as_float(word[k]) : x[i + k];
+            x[i + k] = word[k] ? __uint_as_float(~word[k]) : x[i + k];
             x[i + k] = (bits >> (i + k)) & 1u ? x[i + k] : -INFINITY;
           }
         }

@@ -159,11 +159,12 @@ def _shaped_row(x, length, history, start, penalties, bias_tokens, bias_values, 
     repetition, frequency, presence = penalties.float()
     x = torch.where(seen > 0, torch.where(x > 0, x / repetition, x * repetition), x)
     x = torch.where(times > 0, x - frequency * times - presence, x)
-    bias = torch.zeros_like(x)
+    bias, listed = torch.zeros_like(x), torch.zeros(V, dtype=torch.bool, device=dev)
     for t, value in zip(bias_tokens.tolist(), bias_values):
         if 0 <= t < V:
             bias[t] += value
-    x = torch.where(bias != 0, x + bias, x)
+            listed[t] = True
+    x = torch.where(listed, x + bias, x)
     at = torch.arange(V, device=dev)
     return torch.where((allowed[at // 32] >> (at % 32).int()) & 1 > 0, x, torch.full_like(x, float("-inf")))
 

@@ -212,3 +212,17 @@ def test_small_fp16_numbers_between_the_products(r, size):
         want = scale.double()[s] * (x[i * T:(i + 1) * T].double() @ a[s].double().T @ b[s].double().T)
         # half a step of the result (of its smallest step where it is below 2^-14), and 2^-18 for sums in 32 bits
         assert ((y[i * T:(i + 1) * T] - want).abs() <= 2.0 ** -11 * want.abs() + 2.0 ** -25 + 2.0 ** -18 * want.abs().max()).all()
+
+
+def test_signs_of_zeros(backend):  # noqa: F811
+    """Results of zero have the sign that the formula gives them: 2 - 2 is zero, minus zero times a penalty minus zero."""
+    dev, V = backend[0], 300
+    logits = torch.zeros(1, V).to(backend[1])
+    logits[0, :8] = torch.tensor([2.0, -0.0, -0.0, 0.0, -0.0, 3.0, -0.0, 2.0])
+    history, tokens = i32(backend, 0, 1, 5, 7).reshape(1, 4), i32(backend, 2, 5, -1, 7).reshape(1, 4)
+    values = torch.tensor([[0.0, -1.0, 0.0, -0.0]], device=dev)
+    rules = (history, i32(backend, 0), torch.tensor([[1.0, 0.5, 1.5]], device=dev), tokens, values, torch.full((1, 10), -1, dtype=torch.int32, device=dev))
+    x = op("shape_logits", backend, logits.to(dev), i32(backend, 0), i32(backend, 4), *rules).cpu()[0]
+    # 2 - 0.5 - 1.5; (-0 - 0.5) - 1.5; -0 + 0; untouched ones; ((3 - 0.5) - 1.5) - 1; untouched; ((2 - 0.5) - 1.5) - 0
+    assert x[:8].tolist() == [0.0, -2.0, 0.0, 0.0, 0.0, 0.0, 0.0, 0.0]
+    assert torch.signbit(x[:8]).tolist() == [False, True, False, False, True, False, True, False] and not torch.signbit(x[8:]).any()
