@@ -227,13 +227,13 @@ struct Q8ExpandParams {
   __half* raw_k;                    // (B, G, raw_rows, dim)
   __nv_bfloat16* raw_v;             // (B, G, raw_rows, vdim)
   float* raw_unit;                  // (B, G, q8_touched(T))
-  __half* kx;                       // (B, G, blocks * 64, dim)
-  __nv_bfloat16* vx;                // (B, G, blocks * 64, vdim)
+  __half* kx;                       // (B, G, held * 64, dim)
+  __nv_bfloat16* vx;                // (B, G, held * 64, vdim)
   int8_t *kc, *vc;
   float *ks, *vs;
   __nv_bfloat16 *kt, *vt;
   const int *pos, *count;
-  int T, H, G, dim, vdim, blocks, raw_rows, window, keep_first;
+  int T, H, G, dim, vdim, blocks, held, raw_rows, window, keep_first;
   double eps, inv_dim;
 };
 
@@ -272,6 +272,7 @@ __global__ void __launch_bounds__(256, 4) q8_append_expand_kernel(const Q8Expand
   const int fill = pos % Q8_BLOCK, end = fill + n, r0 = blk * Q8_BLOCK, r1 = min(r0 + Q8_BLOCK, end);
   if (r0 >= end) return;
   const long long head = (long long)b * p.G + g, at = head * p.blocks + pos / Q8_BLOCK + blk;
+  const long long x_at = head * p.held + q8_slots(pos, p.window, p.keep_first).of(pos / Q8_BLOCK + blk);  // if it is complete
   const __nv_bfloat16* proj = p.proj + (long long)b * p.T * p.ld;
   const bool on_k = l * 8 < p.dim, on_v = l * 8 < p.vdim;
   float wq[8], wk[8], top_q = 0.f, top_w = 0.f;
@@ -407,13 +408,13 @@ __global__ void __launch_bounds__(256, 4) q8_append_expand_kernel(const Q8Expand
         q8_unpack(tile[kind][r][l], x);
         step.codes(x, c);
         const uint2 word = make_uint2(c[0], c[1]);
-        const long long row = at * Q8_BLOCK + r;
+        const long long row = at * Q8_BLOCK + r, x_row = x_at * Q8_BLOCK + r;
         if (kind == 0 && on_k) {
           *reinterpret_cast<uint2*>(p.kc + row * p.dim + l * 8) = word;
-          *reinterpret_cast<uint4*>(p.kx + row * p.dim + l * 8) = q8_code_halves(word);
+          *reinterpret_cast<uint4*>(p.kx + x_row * p.dim + l * 8) = q8_code_halves(word);
         } else if (kind == 1 && on_v) {
           *reinterpret_cast<uint2*>(p.vc + row * p.vdim + l * 8) = word;
-          *reinterpret_cast<uint4*>(p.vx + row * p.vdim + l * 8) = q8_code_values(word);
+          *reinterpret_cast<uint4*>(p.vx + x_row * p.vdim + l * 8) = q8_code_values(word);
         }
       }
     }
@@ -445,11 +446,12 @@ __global__ void __launch_bounds__(256) q8_expand_kernel(const Q8ExpandParams p) 
   if (n <= 0 || pos < 0 || (long long)pos + n > (long long)p.blocks * Q8_BLOCK) return;
   const int done = pos / Q8_BLOCK, from = p.window ? max(0, pos - p.window + 1) / Q8_BLOCK : 0;
   const int kept = (int)(((long long)p.keep_first + Q8_BLOCK - 1) / Q8_BLOCK);
+  const Q8Slots slots = q8_slots(pos, p.window, p.keep_first);
   const long long head = (long long)b * p.G + g;
   const bool on_k = l * 8 < p.dim, on_v = l * 8 < p.vdim;
   for (int j = blockIdx.x * Q8_EXPAND_GROUP; j < min(done, (int)(blockIdx.x + 1) * Q8_EXPAND_GROUP); ++j) {
     if (j < from && j >= kept) continue;
-    const long long at = head * p.blocks + j;
+    const long long at = head * p.blocks + j, x_at = head * p.held + slots.of(j);
     uint2 k[4], v[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -459,7 +461,7 @@ __global__ void __launch_bounds__(256) q8_expand_kernel(const Q8ExpandParams p) 
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const long long row = at * Q8_BLOCK + half + 16 * i;
+      const long long row = x_at * Q8_BLOCK + half + 16 * i;
       if (on_k) *reinterpret_cast<uint4*>(p.kx + row * p.dim + l * 8) = q8_code_halves(k[i]);
       if (on_v) *reinterpret_cast<uint4*>(p.vx + row * p.vdim + l * 8) = q8_code_values(v[i]);
     }
@@ -1465,21 +1467,22 @@ XL_API int xl_q8_attn_few(const void* proj, long long ld, const float* wq, const
 }
 
 // The same as xl_q8_append for xl_q8_attn_tcgen05 (see there): q (B, G, T, H/G, dim) and raw_k (B, G, raw_rows, dim) fp16, raw_v (B, G,
-// raw_rows, vdim) bf16 with raw_rows >= T + 128, raw_unit (B, G, (T + 126) / 64) fp32, kx (B, G, blocks * 64, dim)
-// fp16, vx (.., vdim) bf16: complete blocks that the portion can see. bf16; dim, vdim multiples of 8 up to 128, ld a multiple of 8, all pointers 16-byte aligned.
+// raw_rows, vdim) bf16 with raw_rows >= T + 128, raw_unit (B, G, (T + 126) / 64) fp32, kx (B, G, held * 64, dim)
+// fp16, vx (.., vdim) bf16: complete blocks that the portion can see, in `held` places (q8_held, or more). bf16; dim, vdim multiples of 8 up to 128, ld a multiple of 8, all pointers 16-byte aligned.
 XL_API int xl_q8_append_expand(const void* proj, long long ld, const float* wq, const float* wk, void* q, void* raw_k, void* raw_v,
-                               int raw_rows, float* raw_unit, void* kx, void* vx, void* kc, void* vc, float* ks, float* vs, void* kt, void* vt,
-                               const int* pos, const int* count, int B, int T, int H, int G, int dim, int vdim, int blocks, int window,
-                               int keep_first, double eps, cudaStream_t s) {
+                               int raw_rows, float* raw_unit, void* kx, void* vx, int held, void* kc, void* vc, float* ks, float* vs,
+                               void* kt, void* vt, const int* pos, const int* count, int B, int T, int H, int G, int dim, int vdim,
+                               int blocks, int window, int keep_first, double eps, cudaStream_t s) {
   if (!q8_sizes_ok(B, T, H, G, dim, vdim, blocks) || dim % 8 || vdim % 8 || dim > 128 || vdim > 128 || ld % 8 || !wq || !wk || !raw_unit ||
-      ld < (long long)(H + G) * dim + (long long)G * vdim || raw_rows < T + 2 * Q8_BLOCK || window < 0 || keep_first < 0)
+      ld < (long long)(H + G) * dim + (long long)G * vdim || raw_rows < T + 2 * Q8_BLOCK || window < 0 || keep_first < 0 ||
+      held < q8_held(T, blocks, window, keep_first))
     return -1;
   const uintptr_t at = (uintptr_t)proj | (uintptr_t)q | (uintptr_t)raw_k | (uintptr_t)raw_v | (uintptr_t)kx | (uintptr_t)vx | (uintptr_t)kc |
                        (uintptr_t)vc | (uintptr_t)kt | (uintptr_t)vt;
   if (at & 15) return -1;
   const Q8ExpandParams p{(const __nv_bfloat16*)proj, ld, wq, wk, (__half*)q, (__half*)raw_k, (__nv_bfloat16*)raw_v, raw_unit, (__half*)kx,
                          (__nv_bfloat16*)vx, (int8_t*)kc, (int8_t*)vc, ks, vs, (__nv_bfloat16*)kt, (__nv_bfloat16*)vt, pos, count, T, H, G, dim,
-                         vdim, blocks, raw_rows, window, keep_first, eps, 1.0 / dim};
+                         vdim, blocks, held, raw_rows, window, keep_first, eps, 1.0 / dim};
   XL_TRY(xl_launch_overlapped(q8_append_expand_kernel, dim3(q8_touched(T), G, B), dim3(256), (size_t)0, s, p));
   XL_TRY(xl_launch_overlapped(q8_expand_kernel, dim3((blocks + Q8_EXPAND_GROUP - 1) / Q8_EXPAND_GROUP, G, B), dim3(256), (size_t)0, s, p));
   return (int)cudaGetLastError();

@@ -14,6 +14,23 @@ constexpr int Q8_BLOCK = 64;
 // blocks that a portion of T tokens can touch, wherever it begins
 __host__ __device__ constexpr int q8_touched(int T) { return (T + 2 * Q8_BLOCK - 2) / Q8_BLOCK; }
 
+// Where the codes of a block are held as 16-bit numbers while a portion from position `pos` on is worked on: those of the kept first tokens,
+// then those from the first block that a window of the portion reaches, side by side. Blocks in between are not held.
+struct Q8Slots {
+  int kept, from;
+  __device__ __forceinline__ int of(int blk) const { return blk < kept ? blk : kept + blk - from; }
+};
+__device__ __forceinline__ Q8Slots q8_slots(int pos, int window, int keep_first) {
+  if (!window) return {0, 0};
+  const int kept = (int)(((long long)keep_first + Q8_BLOCK - 1) / Q8_BLOCK);
+  return {kept, max(kept, max(0, pos - window + 1) / Q8_BLOCK)};
+}
+// How many there are at most, for a portion of T tokens: its last complete block is less than (T + window - 1) / 64 + 1 behind `from`.
+inline long long q8_held(int T, int blocks, int window, int keep_first) {
+  const long long n = ((long long)keep_first + Q8_BLOCK - 1) / Q8_BLOCK + ((long long)T + window - 1) / Q8_BLOCK + 1;
+  return window && n < blocks ? n : blocks;
+}
+
 // A power of two above every factor of a norm: normalised rows divided by it are at most sqrt(features) and fit 16-bit floats. `top`: the
 // largest absolute factor that the lane has seen; the result is that of the warp.
 __device__ __forceinline__ float q8_norm_unit(float top) {

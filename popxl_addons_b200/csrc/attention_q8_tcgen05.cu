@@ -45,7 +45,7 @@ struct Q8PortionParams {
   long long ldg;
   __nv_bfloat16* out;
   long long ldo;
-  int T, H, G, dim, vdim, blocks, raw_rows, window, keep_first;
+  int T, H, G, dim, vdim, blocks, held, raw_rows, window, keep_first;
   float scale, sink;
   const float *ks, *vs, *wq, *wk;  // scales of the blocks (B, G, blocks), factors of the norms
   const float* raw_unit;           // (B, G, q8_touched(T)): 1, or NaN for a raw block with a value that is not finite
@@ -200,12 +200,13 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       const int stages = for_k ? L::K_STAGES : L::V_STAGES;
       uint64_t* full = for_k ? k_full : v_full;
       uint64_t* empty = for_k ? k_empty : v_empty;
+      const Q8Slots slots = q8_slots(pos, p.window, p.keep_first);
       bool ok = true;
       int issued = 0;
       for (int j = 0; j < n_kv && ok; ++j) {
         const bool raw = j >= n_code;
         const int st = j % stages, blk = block_of(j);
-        const int row = raw ? (b * p.G + g) * p.raw_rows + (blk - base) * BKV : ((b * p.G + g) * p.blocks + blk) * BKV;
+        const int row = raw ? (b * p.G + g) * p.raw_rows + (blk - base) * BKV : ((b * p.G + g) * p.held + slots.of(blk)) * BKV;
         if (j >= stages) {
           ok = mbar_wait(&empty[st], (uint32_t)(j / stages - 1) & 1u, abort_flag, p.err, ERR_KV_EMPTY);
           if (!ok) break;
@@ -452,8 +453,8 @@ int launch(const void* q, const void* kx, const void* vx, const void* raw_k, con
   CUtensorMap mq, mk, mv, mrk, mrv;  // fp16 rows travel like bf16 ones
   const long long heads = (long long)B * p.G;
   int r = make_map_bf16(&mq, q, (long long)B * p.T * p.H, p.dim, p.dim, TILE_M);
-  if (!r) r = make_map_bf16(&mk, kx, heads * p.blocks * BKV, p.dim, p.dim, BKV);
-  if (!r) r = make_map_bf16(&mv, vx, heads * p.blocks * BKV, p.vdim, p.vdim, BKV);
+  if (!r) r = make_map_bf16(&mk, kx, heads * p.held * BKV, p.dim, p.dim, BKV);
+  if (!r) r = make_map_bf16(&mv, vx, heads * p.held * BKV, p.vdim, p.vdim, BKV);
   if (!r) r = make_map_bf16(&mrk, raw_k, heads * p.raw_rows, p.dim, p.dim, BKV);
   if (!r) r = make_map_bf16(&mrv, raw_v, heads * p.raw_rows, p.vdim, p.vdim, BKV);
   if (r) return r;
@@ -467,28 +468,29 @@ int launch(const void* q, const void* kx, const void* vx, const void* raw_k, con
 
 }  // namespace
 
-// After xl_q8_append_expand: q16 (B, G, T, H/G, dim) fp16, codes as fp16 kx (B, G, blocks * 64, dim) and bf16 vx (.., vdim), raw rows as
+// After xl_q8_append_expand: q16 (B, G, T, H/G, dim) fp16, codes as fp16 kx (B, G, held * 64, dim) and bf16 vx (.., vdim), raw rows as
 // fp16 raw_k and bf16 raw_v (B, G, raw_rows, dim | vdim), raw_unit (B, G, (T + 126) / 64); ks, vs (B, G, blocks) the scales, wq and wk
 // the factors of the norms; gate: first gate column of the projections (row stride ldg), or null; out (B*T, ldo). dim, vdim multiples of
 // 8 and at most 128; ldg, ldo multiples of 8; all pointers but those of fp32 numbers 16-byte aligned. Rows past count[b] are not written. err: device int for the code of a wait that gave up.
 // Returns 0, a CUDA error code, or a negative value for arguments this kernel does not take.
-XL_API int xl_q8_attn_tcgen05(const void* q16, const void* kx, const void* vx, const void* raw_k, const void* raw_v, int raw_rows,
-                              const float* raw_unit, const float* ks, const float* vs, const float* wq, const float* wk, const void* gate,
+XL_API int xl_q8_attn_tcgen05(const void* q16, const void* kx, const void* vx, int held, const void* raw_k, const void* raw_v,
+                              int raw_rows, const float* raw_unit, const float* ks, const float* vs, const float* wq, const float* wk, const void* gate,
                               long long ldg, void* out, long long ldo, const int* pos, const int* count, int B, int T, int H, int G, int dim, int vdim,
                               int blocks, int window, int keep_first, float scale, float sink, int* err, cudaStream_t s) {
   if (B < 1 || B > 65535 || T < 1 || G < 1 || H < 1 || H % G || blocks < 1 || blocks > (1 << 24) || window < 0 || keep_first < 0 || !(scale > 0.f))
     return -1;
   if (dim < 8 || dim > 128 || dim % 8 || vdim < 8 || vdim > 128 || vdim % 8 || ldo % 8 || ldo < (long long)H * vdim ||
-      (gate && (ldg % 8 || ldg < (long long)H * vdim)) || raw_rows < T + 2 * Q8_BLOCK || !raw_unit)
+      (gate && (ldg % 8 || ldg < (long long)H * vdim)) || raw_rows < T + 2 * Q8_BLOCK || !raw_unit ||
+      held < q8_held(T, blocks, window, keep_first))
     return -1;
   if (((uintptr_t)q16 | (uintptr_t)kx | (uintptr_t)vx | (uintptr_t)raw_k | (uintptr_t)raw_v | (uintptr_t)gate | (uintptr_t)out) & 15) return -1;
   const long long limit = 0x7fffffffLL - 4 * TILE_M;
-  if ((long long)B * G * blocks * BKV > limit || (long long)B * G * raw_rows > limit || (long long)B * T * H > limit ||
+  if ((long long)B * G * held * BKV > limit || (long long)B * G * raw_rows > limit || (long long)B * T * H > limit ||
       ((long long)T * (H / G) + 2 * TILE_M - 1) / (2 * TILE_M) > 65535)
     return -1;
   Q8PortionParams p = {};
   p.pos = pos; p.count = count; p.gate = (const __nv_bfloat16*)gate; p.ldg = ldg; p.out = (__nv_bfloat16*)out; p.ldo = ldo;
-  p.T = T; p.H = H; p.G = G; p.dim = dim; p.vdim = vdim; p.blocks = blocks; p.raw_rows = raw_rows; p.window = window;
+  p.T = T; p.H = H; p.G = G; p.dim = dim; p.vdim = vdim; p.blocks = blocks; p.held = held; p.raw_rows = raw_rows; p.window = window;
   p.keep_first = keep_first; p.scale = scale; p.sink = sink; p.ks = ks; p.vs = vs; p.wq = wq; p.wk = wk; p.raw_unit = raw_unit; p.err = err;
   if (dim <= 64) return vdim <= 64 ? launch<64, 64>(q16, kx, vx, raw_k, raw_v, p, B, s) : launch<64, 128>(q16, kx, vx, raw_k, raw_v, p, B, s);
   return vdim <= 64 ? launch<128, 64>(q16, kx, vx, raw_k, raw_v, p, B, s) : launch<128, 128>(q16, kx, vx, raw_k, raw_v, p, B, s);

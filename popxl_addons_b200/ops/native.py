@@ -252,6 +252,63 @@ def capture_scratch(device):
         _CAPTURES.held = before
 
 
+class SharedScratch:
+    """Scratch memory of a session's programs: a buffer that is large, and whose contents no later launch needs, is there once and not
+    in the private memory of every captured graph. A graph keeps the buffer that it was captured with, so a larger one is another one.
+    One stream uses it at a time: `follow` orders a run, or the replay of a graph that uses it, behind what the stream before did."""
+
+    def __init__(self):
+        self._buffers: Dict[str, torch.Tensor] = {}
+        self._stream = None
+
+    def follow(self):
+        now = torch.cuda.current_stream()
+        if self._stream is not None and now != self._stream:
+            now.wait_stream(self._stream)
+            for buf in self._buffers.values():
+                buf.record_stream(now)
+        self._stream = now
+
+    def take(self, nbytes: int, device: torch.device, tag: str, most: int) -> torch.Tensor:
+        """At least `nbytes` bytes. A buffer that grows at least doubles, up to `most`: smaller ones that graphs keep are no more than it."""
+        buf, capturing = self._buffers.get(tag), torch.cuda.is_current_stream_capturing()
+        if buf is None or buf.numel() < nbytes:
+            if capturing:
+                return torch.empty(nbytes, dtype=torch.uint8, device=device)
+            buf = self._buffers[tag] = torch.empty(max(nbytes, min(2 * buf.numel(), most) if buf is not None else 0), dtype=torch.uint8, device=device)
+        if capturing:
+            _CAPTURES.held[f"shared {tag} {buf.data_ptr()}"] = buf
+        else:
+            self.follow()
+        return buf
+
+
+@contextmanager
+def sharing(scratch: SharedScratch):
+    """Ops that this thread runs take large scratch memory from `scratch`."""
+    before = getattr(_CAPTURES, "shared", None)
+    _CAPTURES.shared = scratch
+    try:
+        yield scratch
+    finally:
+        _CAPTURES.shared = before
+
+
+def uses_shared(scratch: Dict[str, torch.Tensor]) -> bool:
+    """Whether a graph with this scratch (see `capture_scratch`) uses memory that it shares with others."""
+    return any(tag.startswith("shared") for tag in scratch)
+
+
+def large_scratch(nbytes: int, device: torch.device, tag: str, most: int = 0) -> torch.Tensor:
+    """At least `nbytes` bytes for the launches of one op: of the session whose program this thread runs, on the program's own stream;
+    elsewhere new memory."""
+    shared, order = getattr(_CAPTURES, "shared", None), read_ahead.current()
+    if shared is None or order is None or order.stream != _stream() or (
+            torch.cuda.is_current_stream_capturing() and getattr(_CAPTURES, "held", None) is None):
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+    return shared.take(nbytes, device, tag, most)
+
+
 def gemm_error_flag(device: torch.device) -> torch.Tensor:
     """Device int that the GEMM kernels set when one of their bounded waits gave up."""
     idx = device.index or 0

@@ -5,7 +5,7 @@ import torch
 
 from ..xl import read_ahead
 from ..xl.opdef import native
-from .native import _CODE, _c_f, _c_int, _c_ll, _c_p, _check, _count, _ok, _sig, _sms, _stream, counters, gemm, gemm_error_flag
+from .native import _CODE, _c_f, _c_int, _c_ll, _c_p, _check, _count, _ok, _sig, _sms, _stream, counters, gemm, gemm_error_flag, large_scratch
 from .native_sequence import _clamped_glu, _f32, _i32, _ptr, _small, product, stream_rms
 
 _c_d = ctypes.c_double
@@ -16,8 +16,8 @@ _q8_append = _sig("xl_q8_append", _c_p, _c_ll, *[_c_p] * 13, *[_c_int] * 7, _c_d
 _q8_general = _sig("xl_q8_attn_general", *[_c_p] * 8, _c_ll, _c_p, _c_ll, _c_p, _c_p, *[_c_int] * 9, _c_f, _c_f, _c_int, _c_p)
 _q8_few = _sig("xl_q8_attn_few", _c_p, _c_ll, *[_c_p] * 12, _c_ll, _c_p, _c_p, *[_c_int] * 10, _c_f, _c_f, _c_d, _c_int, _c_p, _c_p, _c_int,
                _c_p, _c_p)
-_q8_append_expand = _sig("xl_q8_append_expand", _c_p, _c_ll, *[_c_p] * 5, _c_int, *[_c_p] * 11, *[_c_int] * 9, _c_d, _c_p)
-_q8_tcgen05 = _sig("xl_q8_attn_tcgen05", *[_c_p] * 5, _c_int, *[_c_p] * 6, _c_ll, _c_p, _c_ll, _c_p, _c_p, *[_c_int] * 9, _c_f, _c_f, _c_p, _c_p)
+_q8_append_expand = _sig("xl_q8_append_expand", _c_p, _c_ll, *[_c_p] * 5, _c_int, *[_c_p] * 3, _c_int, *[_c_p] * 8, *[_c_int] * 9, _c_d, _c_p)
+_q8_tcgen05 = _sig("xl_q8_attn_tcgen05", *[_c_p] * 3, _c_int, *[_c_p] * 2, _c_int, *[_c_p] * 6, _c_ll, _c_p, _c_ll, _c_p, _c_p, *[_c_int] * 9, _c_f, _c_f, _c_p, _c_p)
 _adapter_down = _sig("xl_adapter_down", *[_c_p] * 5, _c_ll, *[_c_int] * 5, _c_p)
 _adapter_up = _sig("xl_adapter_up", *[_c_p] * 5, _c_ll, *[_c_int] * 6, _c_p)
 _adapter_down_mma = _sig("xl_adapter_down_mma", *[_c_p] * 5, _c_ll, *[_c_int] * 5, _c_p)
@@ -118,6 +118,11 @@ def _q8_slices(units, longest, per_sm, device) -> int:
 _Q8_EXPANDED = 2 << 30  # bytes that the codes of a portion may expand to at a time
 
 
+def _q8_held(T: int, blocks: int, window: int, keep_first: int) -> int:
+    """Blocks of codes of one sequence that a portion of T tokens may see, wherever it begins, with its own (q8_slots in attention_q8.cuh)."""
+    return min(blocks, -(-keep_first // 64) + (T + window - 1) // 64 + 1) if window else blocks
+
+
 def _q8_few_rows(rows: int, positions: int, dim: int, vdim: int) -> bool:
     """Whether a portion of `rows` rows per sequence and key head, against a cache of `positions`, runs on mma.sync, which cuts the keys among
     CTAs and reads codes once, and not on the tensor cores, whose keys expand first (2 sequences x 8 key heads of 128 after 6000: 16 rows
@@ -128,7 +133,7 @@ def _q8_few_rows(rows: int, positions: int, dim: int, vdim: int) -> bool:
     return dim % 16 == 0 and vdim % 16 == 0 and (rows <= 64 or (rows <= 128 and positions >= 4096))
 
 
-def _q8_portion(at, proj, q_norm, k_norm, cache, pos, count, joint, gate, T, heads, window, keep_first, scale, sink, eps, s):
+def _q8_portion(at, proj, q_norm, k_norm, cache, pos, count, joint, gate, T, heads, held, window, keep_first, scale, sink, eps, s):
     """A portion of the sequences `at` on the tensor cores: append, codes of visible blocks as 16-bit numbers, attention."""
     cache, pos, count = tuple(t[at] for t in cache), pos[at], count[at]
     B, G, blocks, _, dim = cache[0].shape
@@ -138,15 +143,16 @@ def _q8_portion(at, proj, q_norm, k_norm, cache, pos, count, joint, gate, T, hea
     raw_k = torch.empty((B, G, rows, dim), dtype=torch.float16, device=dev)
     raw_v = torch.empty((B, G, rows, vdim), dtype=torch.bfloat16, device=dev)
     raw_unit = torch.empty((B, G, (T + 126) // 64), dtype=torch.float32, device=dev)
-    kx = torch.empty((B, G, blocks * 64, dim), dtype=torch.float16, device=dev)
-    vx = torch.empty((B, G, blocks * 64, vdim), dtype=torch.bfloat16, device=dev)
+    codes = large_scratch(B * G * held * 64 * (dim + vdim) * 2, dev, "q8 codes", _Q8_EXPANDED)
+    kx = codes.data_ptr()
+    vx = kx + B * G * held * 64 * dim * 2
     sizes = (B, T, heads, G, dim, vdim, blocks, window, keep_first)
     norms, where = (q_norm.data_ptr(), k_norm.data_ptr()), (pos.data_ptr(), count.data_ptr())
     rc = _q8_append_expand(proj.data_ptr() + row0 * ld * 2, ld, *norms, q.data_ptr(), raw_k.data_ptr(), raw_v.data_ptr(), rows, raw_unit.data_ptr(),
-                           kx.data_ptr(), vx.data_ptr(), *map(_ptr, cache), *where, *sizes, eps, s)
+                           kx, vx, held, *map(_ptr, cache), *where, *sizes, eps, s)
     _done(rc, "q8_append_expand")
     _count("q8_expand")
-    rc = _q8_tcgen05(q.data_ptr(), kx.data_ptr(), vx.data_ptr(), raw_k.data_ptr(), raw_v.data_ptr(), rows, raw_unit.data_ptr(), cache[2].data_ptr(),
+    rc = _q8_tcgen05(q.data_ptr(), kx, vx, held, raw_k.data_ptr(), raw_v.data_ptr(), rows, raw_unit.data_ptr(), cache[2].data_ptr(),
                      cache[3].data_ptr(), *norms, gate + row0 * ld * 2 if gate else None, ld, joint.data_ptr() + row0 * ldo * 2, ldo, *where, *sizes, scale, sink,
                      gemm_error_flag(dev).data_ptr(), s)
     _done(rc, "q8_attn_tcgen05")
@@ -195,14 +201,16 @@ def window_attention_q8_cuda(proj, q_norm, k_norm, k, v, k_scale, v_scale, k_tai
         if few(None, (None, None), ahead):
             return joint
     aligned = all(t.data_ptr() % 16 == 0 for t in (proj, joint, k, v, k_tail, v_tail))
+    held = _q8_held(T, blocks, window, keep_first)
+    expanded = G * held * 64 * (dim + vdim) * 2  # bytes of one sequence
     if (dt == torch.bfloat16 and not is_few and aligned and dim <= 128 and vdim <= 128 and dim % 8 == vdim % 8 == ld % 8 == ldo % 8 == 0
-            and T * heads <= 1 << 22 and G * blocks * 64 * (dim + vdim) * 2 <= _Q8_EXPANDED):
+            and T * heads <= 1 << 22 and expanded <= _Q8_EXPANDED):
         # as many sequences at a time as expand to what is set aside for it
-        step = max(1, _Q8_EXPANDED // (G * blocks * 64 * (dim + vdim) * 2))
+        step = max(1, _Q8_EXPANDED // expanded)
         step = min(step, (1 << 30) // (G * (T + 128)) + 1, (1 << 30) // (T * heads) + 1)
         for b in range(0, B, step):
             _q8_portion(slice(b, min(B, b + step)), proj, q_norm, k_norm, (k, v, k_scale, v_scale, k_tail, v_tail), pos, count, joint, gate, T,
-                        heads, window, keep_first, scale, sink, eps, s)
+                        heads, held, window, keep_first, scale, sink, eps, s)
         return joint
     q = torch.empty((B, G, T, heads // G, dim), dtype=torch.float32, device=dev)
     raw = [torch.empty((B, G, T + 64, width), dtype=dt, device=dev) for width in (dim, vdim)]

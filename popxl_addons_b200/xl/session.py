@@ -12,6 +12,7 @@ Parity: the `popxl.Session` surface used by popxl_addons/task_session.py:52-53,8
 import os
 import sys
 import time
+from contextlib import nullcontext
 from typing import Any, Dict, Iterable, List, Mapping, Optional
 
 import numpy as np
@@ -76,6 +77,7 @@ class Session:
         if self.use_native:
             from ..ops import native as _native  # noqa: F401  (registers the CUDA kernels; raises if not built)
 
+        self._shared_scratch = None
         self._vars: Dict[Variable, List[torch.Tensor]] = {}
         self._buffers: Dict[RemoteBuffer, List[torch.Tensor]] = {}
         self._consts: Dict[Constant, torch.Tensor] = {}
@@ -906,13 +908,9 @@ class Session:
         ptrs = tuple(v[0].data_ptr() for v in vals[n_out:])
         if ptrs != state["ptrs"]:
             raise RuntimeError("inputs of a CUDA-graph-captured loop changed address between runs")
-        from ..ops import native as _native
 
         for _ in range(it, count):
-            for stream, static in state["static_in"].items():
-                static.copy_(self._next_host_item(stream), non_blocking=True)
-            state["graph"].replay()
-            _native.count_replay(state["kernels"])
+            self._replay(state)
             self._after_replay(state)
         return [[buf[0].clone()] for buf in state["carried"]]
 
@@ -999,10 +997,23 @@ class Session:
         if os.environ.get("XL_DEBUG_CAPTURE") == "1":
             print(f"[capture rank {os.environ.get('RANK', '0')}] {graph.name}: capture ended, {len(kernels)} own kernels",
                   file=sys.stderr, flush=True)
-        g.replay()  # capture records but does not execute
-        _native.count_replay(kernels)
-        return {"graph": g, "static_in": static_in, "outputs": outs_rec, "kernels": kernels, "carried": carried, "scratch": scratch,
-                "ptrs": tuple(v[0].data_ptr() for v in vals[n_out:])}
+        state = {"graph": g, "static_in": static_in, "outputs": outs_rec, "kernels": kernels, "carried": carried, "scratch": scratch,
+                 "shared": self._shared_scratch if _native.uses_shared(scratch) else None,
+                 "ptrs": tuple(v[0].data_ptr() for v in vals[n_out:])}
+        self._replay(state, stage=False)  # capture records but does not execute
+        return state
+
+    def _replay(self, state, stage: bool = True):
+        """`stage`: the next items of the host streams that the graph reads go to their static places first."""
+        from ..ops import native as _native
+
+        if stage:
+            for stream, static in state["static_in"].items():
+                static.copy_(self._next_host_item(stream), non_blocking=True)
+        if state["shared"] is not None:
+            state["shared"].follow()
+        state["graph"].replay()
+        _native.count_replay(state["kernels"])
 
     def _after_replay(self, state, copy: bool = True):
         for stream, tensors in state["outputs"]:
@@ -1031,6 +1042,16 @@ class Session:
                 self._fused_runtime.check()
         return out
 
+    def _sharing(self):
+        """Around the ops of a program: they share large scratch memory with those of the session's other programs."""
+        if not self.use_native:
+            return nullcontext()
+        from ..ops import native as _native
+
+        if self._shared_scratch is None:
+            self._shared_scratch = _native.SharedScratch()
+        return _native.sharing(self._shared_scratch)
+
     def run_program(self, program, inputs: Optional[Mapping[HostToDeviceStream, Any]] = None,
                     fetch: bool = True, copy: bool = True) -> Dict[DeviceToHostStream, np.ndarray]:
         """Execute a `Program` once; inputs, outputs and `fetch` as in `run`. The first run is eager (lazy
@@ -1043,16 +1064,11 @@ class Session:
         replayed = state is not None and capturable
         self._stage_inputs(inputs or {}, keep_on_host=replayed)
         if replayed:
-            from ..ops import native as _native
-
-            for stream, static in state["static_in"].items():
-                static.copy_(self._next_host_item(stream), non_blocking=True)
-            state["graph"].replay()
-            _native.count_replay(state["kernels"])
+            self._replay(state)
             # outputs that are read before anything else can replay the program need no copy of their own
             self._after_replay(state, copy=copy and not fetch)
         else:
-            with torch.no_grad():
+            with torch.no_grad(), self._sharing():
                 vals = [self._value(t, {}) for t in program.bindings.values()]
                 with _read_ahead.following(self._launch_order(program.graph)):
                     if capturable and program in self._programs and self._capture_safe(program.graph):
