@@ -244,7 +244,13 @@ def linear_adapted_cuda(x, weight, a, b, scale, slot, T, out_dtype):
         if not _launched(_adapter_down(*down), "adapter_down"):
             return NotImplemented
     # 32 bits also where the GEMM needs copies for them: the sum is rounded once
-    y = product(x, weight, torch.float32) if dt == torch.float32 or _small(x, weight) else gemm(x, weight.t(), out_dtype=torch.float32)
+    if dt == torch.float32 or _small(x, weight):
+        y = product(x, weight, torch.float32)
+    elif out_dtype == torch.float32:
+        y = gemm(x, weight.t(), out_dtype=torch.float32)
+    else:  # only for the launches of this op
+        y = large_scratch(rows * N * 4, dev, "adapted", 1 << 30)[:rows * N * 4].view(torch.float32).view(rows, N)
+        y = gemm(x, weight.t(), out=y)
     if y is NotImplemented:
         return NotImplemented
     if out_dtype == torch.float32:

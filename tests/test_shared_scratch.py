@@ -220,3 +220,35 @@ def test_portions_in_slices_of_sequences(monkeypatch, window):
         outs.append([joint, *cache])
     for other in outs[1:]:
         assert all(torch.equal(a, b) for a, b in zip(outs[0], other))
+
+
+@pytest.mark.gpu
+def test_adapted_products_share_what_is_between_them():
+    """Results in 32 bits before adapters are added: one buffer, 67 MB, for eight programs, each with the results of the plain formula."""
+    K, N, r, n = 256, 8192, 16, 2
+    ir, gen = xl.Ir(), torch.Generator().manual_seed(1)
+    shapes = {"w": (N, K), "a": (n, r, K), "b": (n, N, r)}
+    values = {k: (torch.randn(s, generator=gen) * s[-1] ** -0.5).bfloat16() for k, s in shapes.items()}
+    with ir.main_graph:
+        held = {k: xl.variable(v, xl.bfloat16, k) for k, v in values.items()}
+        held["scale"], held["slot"] = xl.variable(np.ones(n, np.float32), xl.float32, "scale"), xl.variable(np.array([1, 0], np.int32), xl.int32, "slot")
+    programs = []
+    for T in (1024, 960, 896, 832, 768, 704, 640, 576):
+        p = xl.Program(ir, f"adapted_{T}")
+        with p:
+            src, dst = xl.h2d_stream((2 * T, K), xl.bfloat16, "x"), xl.d2h_stream((2,), xl.float32, "y")
+            x = ops.host_load(src)
+            y = ops.linear_adapted(x, p.use(held["w"]), ops.Adapters(*(p.use(held[k]) for k in ("a", "b", "scale"))), p.use(held["slot"]), T)
+            picked = ops.reshape(ops.cast(y, xl.float32), (2, T * N))
+            ops.host_store(dst, picked[:, T * N - 1])
+        programs.append((p, src, dst, T))
+    session = xl.Session(ir, "cuda:0")
+    for p, src, dst, T in programs:
+        x = torch.randn(2 * T, K, generator=gen).bfloat16()
+        rows = x[[T - 1, 2 * T - 1]].double()
+        want = torch.stack([row @ values["w"][-1].double() + row @ values["a"][s].double().T @ values["b"][s][-1].double() for row, s in zip(rows, (1, 0))])
+        for _ in range(3):
+            got = torch.from_numpy(np.asarray(session.run_program(p, {src: x})[dst])).double().reshape(2)
+            assert ((got - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -15).all()  # one rounding, and sums in 32 bits
+    kept = [{t.data_ptr() for tag, t in session._programs[p]["scratch"].items() if tag.startswith("shared")} for p, *_ in programs]
+    assert all(len(k) == 1 and k == kept[0] for k in kept)
