@@ -226,3 +226,44 @@ def test_signs_of_zeros(backend):  # noqa: F811
     # 2 - 0.5 - 1.5; (-0 - 0.5) - 1.5; -0 + 0; untouched ones; ((3 - 0.5) - 1.5) - 1; untouched; ((2 - 0.5) - 1.5) - 0
     assert x[:8].tolist() == [0.0, -2.0, 0.0, 0.0, 0.0, 0.0, 0.0, 0.0]
     assert torch.signbit(x[:8]).tolist() == [False, True, False, False, True, False, True, False] and not torch.signbit(x[8:]).any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("S,V", [(2, 70001), (90, 50400), (3, 200000)])
+def test_choice_from_parts_of_several_chunks(S, V, dtype):
+    """A CTA of the choice takes its part of the row 8192 entries at a time: tokens, biases and masks of every chunk."""
+    from popxl_addons_b200.xl.opdef import OPS
+    from test_logits_ops import rules
+
+    r, _ = rules(S, V, 3000, 12, seed=4)
+    g = torch.Generator().manual_seed(6)
+    r[0][:] = torch.randint(0, V, r[0].shape, generator=g)  # all over the vocabulary
+    logits = torch.randint(-6, 7, (S, V), generator=g).to(dtype)
+    for s in range(S):  # what wins without the rules lies in another chunk from row to row, and the tokens lose by the penalties
+        logits[s, (s * 8191 + 17) % V] = 9.0
+    length = torch.randint(0, 3000, (S,), generator=g).int()
+    ref = OPS["shape_logits"].impl(logits, torch.arange(S, dtype=torch.int32), length, *r)
+    want = [int((x == x.max()).int().argmax()) for x in ref]
+    d = [x.cuda() for x in r]
+    current, buf, pos = torch.full((S,), -7, dtype=torch.int32, device="cuda"), torch.zeros(1, S, dtype=torch.int32, device="cuda"), i32(("cuda",), 0)
+    op("take_shaped_", ("cuda", dtype), current, logits.cuda(), buf, pos, length.cuda(), torch.ones(S, dtype=torch.int32, device="cuda"), *d, valid=V,
+       base=0, ahead=0, advance=True)
+    assert current.tolist() == want and len(set(want)) > min(S, 3) - 2 and pos.tolist() == [1]
+
+
+@pytest.mark.gpu
+def test_shaped_logits_of_parts_of_several_chunks():
+    """Past 1024 parts of 8192 entries a CTA of the shaped row takes several chunks too."""
+    from popxl_addons_b200.xl.opdef import OPS
+    from test_logits_ops import rules
+
+    V = 1024 * 8192 + 100001
+    r, _ = rules(1, V, 5000, 2, seed=4)
+    g = torch.Generator().manual_seed(6)
+    r[0][:], r[2][:] = torch.randint(0, V, r[0].shape, generator=g), torch.tensor([1.3, 0.5, 0.25])
+    logits = torch.randn(1, V, generator=g)
+    args = (i32(("cpu",), 0), i32(("cpu",), 5000), *r)
+    want = OPS["shape_logits"].impl(logits, *args)
+    got = op("shape_logits", ("cuda", torch.float32), logits.cuda(), *[t.cuda() for t in args])
+    assert torch.equal(got.cpu(), want)
