@@ -207,7 +207,7 @@ def window_attention_q8_cuda(proj, q_norm, k_norm, k, v, k_scale, v_scale, k_tai
             and T * heads <= 1 << 22 and expanded <= _Q8_EXPANDED):
         # as many sequences at a time as expand to what is set aside for it
         step = max(1, _Q8_EXPANDED // expanded)
-        step = min(step, (1 << 30) // (G * (T + 128)) + 1, (1 << 30) // (T * heads) + 1)
+        step = min(step, (1 << 30) // (G * (T + 128)) + 1, (1 << 30) // (T * heads) + 1, 65535)
         for b in range(0, B, step):
             _q8_portion(slice(b, min(B, b + step)), proj, q_norm, k_norm, (k, v, k_scale, v_scale, k_tail, v_tail), pos, count, joint, gate, T,
                         heads, held, window, keep_first, scale, sink, eps, s)
@@ -228,7 +228,7 @@ def window_attention_q8_cuda(proj, q_norm, k_norm, k, v, k_scale, v_scale, k_tai
 
 @native("linear_adapted")
 def linear_adapted_cuda(x, weight, a, b, scale, slot, T, out_dtype):
-    x = x.contiguous()
+    x = _rows16(x)
     dt, dev = x.dtype, x.device
     (rows, K), N, (n, r, _) = x.shape, weight.shape[0], a.shape
     if not (dt in _CODE and dt == weight.dtype == a.dtype == b.dtype and out_dtype in (dt, torch.float32)):
@@ -244,7 +244,7 @@ def linear_adapted_cuda(x, weight, a, b, scale, slot, T, out_dtype):
         if not _launched(_adapter_down(*down), "adapter_down"):
             return NotImplemented
     # 32 bits also where the GEMM needs copies for them: the sum is rounded once
-    if dt == torch.float32 or _small(x, weight):
+    if dt == torch.float32 or (_small(x, weight) and weight.data_ptr() % 16 == 0):
         y = product(x, weight, torch.float32)
     elif out_dtype == torch.float32:
         y = gemm(x, weight.t(), out_dtype=torch.float32)

@@ -267,3 +267,23 @@ def test_shaped_logits_of_parts_of_several_chunks():
     want = OPS["shape_logits"].impl(logits, *args)
     got = op("shape_logits", ("cuda", torch.float32), logits.cuda(), *[t.cuda() for t in args])
     assert torch.equal(got.cpu(), want)
+
+
+@pytest.mark.parametrize("rows,K", [(1, 200), (9, 200), (40, 64), (100, 200)])
+@pytest.mark.parametrize("which", ["x", "weight", "adapters"])
+def test_adapted_operands_off_a_16_byte_boundary(backend, which, rows, K):  # noqa: F811
+    """Rows and weights inside larger buffers: the sum is rounded once all the same."""
+    dev, N, r = backend[0], 264, 8
+    for dt in (backend[1],) if backend[1] == torch.float32 else (torch.bfloat16, torch.float16):
+        x, w, a, b = (t.to(dev) for t in terms_that_cancel(dt, rows, K, N, r, seed=3))
+        term = x.double() @ a[0].double().T @ b[0].double().T
+        want = x.double() @ w.double().T + term
+        if which == "x":
+            x = shifted(x)
+        elif which == "weight":
+            w = shifted(w)
+        else:
+            a, b = shifted(a), shifted(b)
+        y = op("linear_adapted", backend, x, w, a, b, torch.ones(1, device=dev), i32(backend, *[0] * rows), T=1, out_dtype=dt)
+        step = 0.0 if dt == torch.float32 else torch.finfo(dt).eps / 2  # as above
+        assert ((y.double() - want).abs() <= step * want.abs() + (2.0 ** -15 if dt == torch.bfloat16 else 2.0 ** -18) * term.abs().max()).all()
