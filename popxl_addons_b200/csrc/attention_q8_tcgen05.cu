@@ -14,8 +14,8 @@
 // rounding of the result does, and save 7 % of the time. Queries and raw keys are fp16 in units of a power of two above their norm's
 // factors.
 //
-// 32 heads on 8 of 128 features: 2 x 4096 tokens, window 1024, 261 us; 2 x 515 tokens after 6000, 161 us (632 TFLOP/s of visible keys,
-// the tensor pipe 48 % busy). What bounds it is the chain of a tile: scores, softmax, weights, product. A tile has two buffers of scores
+// 32 heads on 8 of 128 features: 2 x 4096 tokens, window 1024, 266 us; 2 x 515 tokens after 6000, 170 us (600 TFLOP/s of visible keys,
+// the tensor pipe 46 % busy). What bounds it is the chain of a tile: scores, softmax, weights, product. A tile has two buffers of scores
 // of 64 keys each, so that the next scores are there when a softmax ends, and an issuer of its own, so that no tile's products wait
 // behind what holds up the other's: with one buffer of 128 keys a tile's warps waited 1700 of 4500 cycles per 128 keys for the tensor
 // core's answer, with one issuer for both tiles, in a fixed order or going by what is ready, 1500 of 3000 cycles per 64 keys (clock stamps
