@@ -27,6 +27,7 @@ struct AdapterParams {
   void* out;       // (rows, N)
   long long rows;
   int T, K, N, n, r, rp;
+  int tile;        // xl_adapter_up_mma: rows of a CTA
 };
 
 __device__ __forceinline__ int adapter_of(const AdapterParams& p, long long seq) {
@@ -196,17 +197,17 @@ template <typename T, int NT> __global__ void __launch_bounds__(NT <= 2 ? 512 : 
   }
 }
 
-// Grid (columns / 128, row tiles of 256, sequences): the shared product + the adapters' term, rounded to T. A warp has 32 columns for all rows of
+// Grid (columns / 128, row tiles, sequences): the shared product + the adapters' term, rounded to T. A warp has 32 columns for all rows of
 // the tile, whose row of B[s] it holds; its lanes' columns are chosen so that each ends up with eight neighbours, which arrive in two loads
 // and leave in one store. `low` enters as sums of two T (value and rounding error). Moving the results bounds it: 4 x 1024 rows x 32256 take
 // 132 us (793 MB, 6.0 TB/s). KS: steps of 16 numbers.
-constexpr int AD_TILE = 256;
+constexpr int AD_TILE = 256;  // rows of a CTA, at most
 template <typename T, int KS> __global__ void __launch_bounds__(128) adapter_up_mma_kernel(const AdapterParams p) {
   xl_grid_dependency_wait();
   xl_grid_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = lane >> 2, j = lane & 3;
   const long long seq = blockIdx.z;
-  const int t0 = blockIdx.y * AD_TILE, s = adapter_of(p, seq), rows = min(AD_TILE, p.T - t0), c0 = blockIdx.x * 128 + warp * 32;
+  const int t0 = blockIdx.y * p.tile, s = adapter_of(p, seq), rows = min(p.tile, p.T - t0), c0 = blockIdx.x * 128 + warp * 32;
   if (c0 >= p.N) return;
   T* out = (T*)p.out + (seq * p.T + t0) * p.N;
   const float* y = p.y + (seq * p.T + t0) * p.N;
@@ -390,12 +391,17 @@ XL_API int xl_adapter_down_mma(const void* x, const void* a, const float* scale,
 XL_API int xl_adapter_up_mma(const float* low, const void* b, const int* slot, const float* y, void* out, long long rows, int T, int N, int n, int r,
                              int dtype, cudaStream_t s) {
   if (!adapter_sizes_ok(rows, T, 1, N, n, r) || dtype == XL_F32 || (((uintptr_t)y | (uintptr_t)out) & 15) || (((uintptr_t)b) & 3) || rows / T > 65535 ||
-      (T + AD_TILE - 1) / AD_TILE > 65535)
+      (T + 31) / 32 > 65535)
     return -1;
   AdapterParams p = {};
   p.b = b; p.slot = slot; p.low = const_cast<float*>(low); p.y = y; p.out = out; p.rows = rows; p.T = T; p.N = N; p.n = n; p.r = r;
   p.rp = (r + 15) / 16 * 16;
-  const dim3 grid((N + 127) / 128, (T + AD_TILE - 1) / AD_TILE, (unsigned)(rows / T));
+  // Fewer rows per CTA while there are fewer than four CTAs per SM, which then wait for their loads one after another (the whole op, in tiles of
+  // 256 and by this rule: 1000 rows, 4096 x 4096, rank 64 100 and 78 us, 2048 x 2048, rank 8 33 and 23). More rows otherwise: B[s] is
+  // read once per tile.
+  p.tile = AD_TILE;
+  while (p.tile > 32 && (long long)((N + 127) / 128) * ((T + p.tile - 1) / p.tile) * (rows / T) < 4 * 148) p.tile /= 2;
+  const dim3 grid((N + 127) / 128, (T + p.tile - 1) / p.tile, (unsigned)(rows / T));
   void (*kernel)(const AdapterParams);
 #define XL_AD(D) \
   kernel = p.rp == 16 ? adapter_up_mma_kernel<D, 1> : (p.rp == 32 ? adapter_up_mma_kernel<D, 2> : (p.rp == 48 ? adapter_up_mma_kernel<D, 3> : (p.rp == 64 ? adapter_up_mma_kernel<D, 4> : nullptr)))
