@@ -1009,7 +1009,7 @@ class Session:
 
         if stage:
             for stream, static in state["static_in"].items():
-                static.copy_(self._next_host_item(stream), non_blocking=True)
+                static.copy_(self._next_host_item(stream).detach(), non_blocking=True)
         if state["shared"] is not None:
             state["shared"].follow()
         state["graph"].replay()

@@ -287,3 +287,18 @@ def test_adapted_operands_off_a_16_byte_boundary(backend, which, rows, K):  # no
         y = op("linear_adapted", backend, x, w, a, b, torch.ones(1, device=dev), i32(backend, *[0] * rows), T=1, out_dtype=dt)
         step = 0.0 if dt == torch.float32 else torch.finfo(dt).eps / 2  # as above
         assert ((y.double() - want).abs() <= step * want.abs() + (2.0 ** -15 if dt == torch.bfloat16 else 2.0 ** -18) * term.abs().max()).all()
+
+
+def test_replays_do_not_record_gradients():
+    """Inputs that require gradients leave the static inputs of a captured program without a history that grows with every replay."""
+    from types import SimpleNamespace
+
+    ir = xl.Ir()
+    with ir.main_graph:
+        stream = xl.h2d_stream((4,), xl.float32, "x")
+    session, static = xl.Session(ir, "cpu"), torch.zeros(4)
+    state = {"static_in": {stream: static}, "shared": None, "graph": SimpleNamespace(replay=lambda: None), "kernels": []}
+    for i in range(3):
+        session._stage_inputs({stream: torch.full((4,), float(i), requires_grad=True)}, keep_on_host=True)
+        session._replay(state)
+        assert static.tolist() == [i] * 4 and not static.requires_grad and static.grad_fn is None
