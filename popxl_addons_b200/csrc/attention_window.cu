@@ -11,8 +11,9 @@
 //   k cache (B, G, Smax, dim), v cache (B, G, Smax, vdim)
 //   q' (B, G, T, R, dim): the rows that read one key / value head are consecutive, so that a tile can hold several heads
 //
-//   xl_qk_norm_append        q' to its buffer, k' and v into the caches
+//   xl_qk_norm_append        q' to its buffer, k' and v into the caches (xl_qk_norm_append_fitting: of sequences that fit them)
 //   xl_window_attn_general   any sizes and types, scores and weights in fp32 on the CUDA cores: one warp per row and head
+//   xl_window_attn_shared_general   the same for sequences whose first keys are those of another slot
 //   xl_window_attn_decode    one token per sequence, bf16: norms, append, attention and gate in one launch
 #include "attention_decode.cuh"
 #include "attention_window.cuh"
@@ -34,11 +35,12 @@ __global__ void __launch_bounds__(256)
     qk_norm_append_kernel(const T* __restrict__ proj, long long ld, const float* __restrict__ wq, const float* __restrict__ wk,
                           T* __restrict__ qn, T* __restrict__ kc, T* __restrict__ vc, const int* __restrict__ pos,
                           const int* __restrict__ count, int T_len, int H, int G, int dim, int vdim, int Smax, float eps,
-                          int group) {
+                          int group, int whole) {
   xl_grid_launch_dependents();
   constexpr int NP = 16 / V;  // pieces per lane: 32 lanes cover WA_MAX_DIM features
   const int b = blockIdx.y, t = blockIdx.x, p = pos[b] + t;
   if (t >= count[b] || p < 0 || p >= Smax) return;
+  if (whole && (pos[b] < 0 || pos[b] > Smax - min(count[b], T_len))) return;  // a sequence that would not fit is left out
   const T* row = proj + ((long long)b * T_len + t) * ld;
   const int R = H / G, l = threadIdx.x & (group - 1), pieces = dim / V;
   const int heads_at_once = blockDim.x / group;
@@ -87,24 +89,25 @@ __global__ void __launch_bounds__(256)
 
 template <typename T, int V>
 int launch_append(const void* proj, long long ld, const float* wq, const float* wk, void* qn, void* kc, void* vc, const int* pos,
-                  const int* count, int B, int T_len, int H, int G, int dim, int vdim, int Smax, float eps, cudaStream_t s) {
+                  const int* count, int B, int T_len, int H, int G, int dim, int vdim, int Smax, float eps, int whole, cudaStream_t s) {
   int group = 1;
   while (group < 32 && group * V < dim) group *= 2;
   qk_norm_append_kernel<T, V><<<dim3(T_len, B), 256, 0, s>>>((const T*)proj, ld, wq, wk, (T*)qn, (T*)kc, (T*)vc, pos, count, T_len,
-                                                             H, G, dim, vdim, Smax, eps, group);
+                                                             H, G, dim, vdim, Smax, eps, group, whole);
   return (int)cudaGetLastError();
 }
 
 // ---- general kernel --------------------------------------------------------------------------------------------------
 
 // SPLIT 1: a warp per query row, four of them per CTA. SPLIT 8: a CTA per query row whose warps take its blocks of 32 keys in turn
-// and merge their parts of the softmax in shared memory, for the few rows of a decoding step.
-template <typename T, int VPL, int SPLIT>  // VPL: value features per lane
+// and merge their parts of the softmax in shared memory, for the few rows of a decoding step. SHARED: the first keys of a sequence may be
+// those of another slot.
+template <typename T, int VPL, int SPLIT, bool SHARED>  // VPL: value features per lane
 __global__ void __launch_bounds__(SPLIT == 1 ? 128 : SPLIT * 32)
     window_attn_general_kernel(const T* __restrict__ qn, const T* __restrict__ kc, const T* __restrict__ vc,
                                const T* __restrict__ gate, long long ldg, T* __restrict__ out, long long ldo,
                                const int* __restrict__ pos, const int* __restrict__ count, int T_len, int H, int G, int dim,
-                               int vdim, int Smax, int window, int keep_first, float scale, float sink) {
+                               int vdim, int Smax, int window, int keep_first, float scale, float sink, const SharedPrefix prefix) {
   xl_grid_launch_dependents();
   constexpr int ROWS = SPLIT == 1 ? 4 : 1;
   __shared__ __align__(16) float sq[ROWS][WA_MAX_DIM];
@@ -116,6 +119,11 @@ __global__ void __launch_bounds__(SPLIT == 1 ? 128 : SPLIT * 32)
   if (t >= min(count[b], T_len)) return;  // whole warps, and with SPLIT > 1 whole CTAs
   const int p = pos[b] + t;
   if (p < 0 || p >= Smax) return;
+  int lead = b, edge = 0;
+  if (SHARED) {
+    if (pos[b] < 0 || pos[b] > Smax - min(count[b], T_len)) return;
+    edge = shared_edge(prefix, pos, b, pos[b], gridDim.z, lead);
+  }
   const T* q = qn + ((((long long)b * G + g) * T_len + t) * R + h % R) * dim;
   for (int d = part * 32 + lane; d < dim; d += 32 * SPLIT) sq[slot][d] = xl_to_float(q[d]);
   if (SPLIT == 1) __syncwarp();
@@ -126,7 +134,7 @@ __global__ void __launch_bounds__(SPLIT == 1 ? 128 : SPLIT * 32)
   float o[VPL], mx = part ? -INFINITY : sink, l = part || sink == -INFINITY ? 0.f : 1.f;  // the sink is the first part's
 #pragma unroll
   for (int e = 0; e < VPL; ++e) o[e] = 0.f;
-  auto walk = [&](int begin, int end) {
+  auto walk = [&](int begin, int end, const T* kb, const T* vb) {
     for (int j0 = begin + part * 32; j0 < end; j0 += 32 * SPLIT) {
       const int j = j0 + lane;
       float s = -INFINITY;
@@ -148,8 +156,17 @@ __global__ void __launch_bounds__(SPLIT == 1 ? 128 : SPLIT * 32)
       }
     }
   };
-  walk(0, seen.kept);
-  walk(seen.first, p + 1);
+  if (SHARED) {
+    const T* kl = kc + ((long long)lead * G + g) * Smax * dim;
+    const T* vl = vc + ((long long)lead * G + g) * Smax * vdim;
+    walk(0, min(seen.kept, edge), kl, vl);
+    walk(seen.first, edge, kl, vl);
+    walk(edge, seen.kept, kb, vb);
+    walk(max(seen.first, edge), p + 1, kb, vb);
+  } else {
+    walk(0, seen.kept, kb, vb);
+    walk(seen.first, p + 1, kb, vb);
+  }
   if (SPLIT > 1) {
     if (lane == 0) { sm[warp] = mx; sl[warp] = l; }
 #pragma unroll
@@ -621,29 +638,45 @@ template <int KD, int VT> int wd_launch(const WindowDecodeParams& p, int B, int 
 
 }  // namespace
 
-// proj: (B*T_len, ld) as described above; wq, wk (dim) fp32; qn (B, G, T_len, H/G, dim). dim <= 512. Rows past count[b] are
-// left out.
-XL_API int xl_qk_norm_append(const void* proj, long long ld, const float* wq, const float* wk, void* qn, void* kc, void* vc,
-                             const int* pos, const int* count, int B, int T_len, int H, int G, int dim, int vdim, int Smax,
-                             float eps, int dtype, cudaStream_t s) {
+namespace {
+
+int norm_append(const void* proj, long long ld, const float* wq, const float* wk, void* qn, void* kc, void* vc, const int* pos, const int* count,
+                int B, int T_len, int H, int G, int dim, int vdim, int Smax, float eps, int whole, int dtype, cudaStream_t s) {
   if (B < 1 || B > 65535 || T_len < 1 || G < 1 || H < 1 || H % G || dim < 1 || dim > WA_MAX_DIM || vdim < 1 || Smax < 1 ||
       ld < (long long)(H + G) * dim + (long long)G * vdim || !wq || !wk)
     return -1;
   XL_DISPATCH_DTYPE(dtype, T, {
     constexpr int V = 16 / sizeof(T);
     if (dim % V == 0 && vdim % V == 0 && ld % V == 0 && (((uintptr_t)proj | (uintptr_t)qn | (uintptr_t)kc | (uintptr_t)vc) & 15) == 0)
-      return launch_append<T, V>(proj, ld, wq, wk, qn, kc, vc, pos, count, B, T_len, H, G, dim, vdim, Smax, eps, s);
-    return launch_append<T, 1>(proj, ld, wq, wk, qn, kc, vc, pos, count, B, T_len, H, G, dim, vdim, Smax, eps, s);
+      return launch_append<T, V>(proj, ld, wq, wk, qn, kc, vc, pos, count, B, T_len, H, G, dim, vdim, Smax, eps, whole, s);
+    return launch_append<T, 1>(proj, ld, wq, wk, qn, kc, vc, pos, count, B, T_len, H, G, dim, vdim, Smax, eps, whole, s);
   });
   return (int)cudaGetLastError();
 }
 
-// qn as above; gate: first gate column of the projections (row stride ldg), or null; out: (B*T_len, ldo). dim <= 512, vdim <= 512.
-// Rows past count[b] of a sequence are left as they are.
-XL_API int xl_window_attn_general(const void* qn, const void* kc, const void* vc, const void* gate, long long ldg, void* out,
-                                  long long ldo, const int* pos, const int* count, int B, int T_len, int H, int G, int dim,
-                                  int vdim, int Smax, int window, int keep_first, float scale, float sink, int dtype,
-                                  cudaStream_t s) {
+}  // namespace
+
+// proj: (B*T_len, ld) as described above; wq, wk (dim) fp32; qn (B, G, T_len, H/G, dim). dim <= 512. Rows past count[b] are
+// left out.
+XL_API int xl_qk_norm_append(const void* proj, long long ld, const float* wq, const float* wk, void* qn, void* kc, void* vc,
+                             const int* pos, const int* count, int B, int T_len, int H, int G, int dim, int vdim, int Smax,
+                             float eps, int dtype, cudaStream_t s) {
+  return norm_append(proj, ld, wq, wk, qn, kc, vc, pos, count, B, T_len, H, G, dim, vdim, Smax, eps, 0, dtype, s);
+}
+
+// The same, and sequences whose rows would not all fit the cache are left out.
+XL_API int xl_qk_norm_append_fitting(const void* proj, long long ld, const float* wq, const float* wk, void* qn, void* kc, void* vc,
+                                     const int* pos, const int* count, int B, int T_len, int H, int G, int dim, int vdim, int Smax,
+                                     float eps, int dtype, cudaStream_t s) {
+  return norm_append(proj, ld, wq, wk, qn, kc, vc, pos, count, B, T_len, H, G, dim, vdim, Smax, eps, 1, dtype, s);
+}
+
+namespace {
+
+template <bool SHARED>
+int window_general(const void* qn, const void* kc, const void* vc, const void* gate, long long ldg, void* out, long long ldo, const int* pos,
+                   const int* count, int B, int T_len, int H, int G, int dim, int vdim, int Smax, int window, int keep_first, float scale,
+                   float sink, const SharedPrefix& prefix, int dtype, cudaStream_t s) {
   if (B < 1 || B > 65535 || H < 1 || H > 65535 || T_len < 1 || G < 1 || H % G || dim < 1 || dim > WA_MAX_DIM || vdim < 1 ||
       vdim > 512 || Smax < 1 || window < 0 || keep_first < 0)
     return -1;
@@ -652,19 +685,42 @@ XL_API int xl_window_attn_general(const void* qn, const void* kc, const void* vc
   const dim3 grid(split ? T_len : (T_len + 3) / 4, H, B);
 #define XL_WG(VPL)                                                                                                                 \
   if (split)                                                                                                                       \
-    window_attn_general_kernel<T, VPL, 8><<<grid, 256, 0, s>>>((const T*)qn, (const T*)kc, (const T*)vc, (const T*)gate, ldg,      \
-                                                               (T*)out, ldo, pos, count, T_len, H, G, dim, vdim, Smax, window,     \
-                                                               keep_first, scale, sink);                                          \
+    window_attn_general_kernel<T, VPL, 8, SHARED><<<grid, 256, 0, s>>>((const T*)qn, (const T*)kc, (const T*)vc, (const T*)gate,   \
+                                                               ldg, (T*)out, ldo, pos, count, T_len, H, G, dim, vdim, Smax,        \
+                                                               window, keep_first, scale, sink, prefix);                          \
   else                                                                                                                             \
-    window_attn_general_kernel<T, VPL, 1><<<grid, 128, 0, s>>>((const T*)qn, (const T*)kc, (const T*)vc, (const T*)gate, ldg,      \
-                                                               (T*)out, ldo, pos, count, T_len, H, G, dim, vdim, Smax, window,     \
-                                                               keep_first, scale, sink)
+    window_attn_general_kernel<T, VPL, 1, SHARED><<<grid, 128, 0, s>>>((const T*)qn, (const T*)kc, (const T*)vc, (const T*)gate,   \
+                                                               ldg, (T*)out, ldo, pos, count, T_len, H, G, dim, vdim, Smax,        \
+                                                               window, keep_first, scale, sink, prefix)
   XL_DISPATCH_DTYPE(dtype, T, {
     if (vdim <= 128) { XL_WG(4); }
     else { XL_WG(16); }
   });
 #undef XL_WG
   return (int)cudaGetLastError();
+}
+
+}  // namespace
+
+// qn as above; gate: first gate column of the projections (row stride ldg), or null; out: (B*T_len, ldo). dim <= 512, vdim <= 512.
+// Rows past count[b] of a sequence are left as they are.
+XL_API int xl_window_attn_general(const void* qn, const void* kc, const void* vc, const void* gate, long long ldg, void* out,
+                                  long long ldo, const int* pos, const int* count, int B, int T_len, int H, int G, int dim,
+                                  int vdim, int Smax, int window, int keep_first, float scale, float sink, int dtype,
+                                  cudaStream_t s) {
+  return window_general<false>(qn, kc, vc, gate, ldg, out, ldo, pos, count, B, T_len, H, G, dim, vdim, Smax, window, keep_first, scale, sink,
+                               SharedPrefix{}, dtype, s);
+}
+
+// The same for sequences whose first min(shared[b], pos[b], pos[lead[b]]) keys and values are those of slot lead[b]. Sequences whose rows would not
+// all fit the cache are left out.
+XL_API int xl_window_attn_shared_general(const void* qn, const void* kc, const void* vc, const void* gate, long long ldg, void* out,
+                                         long long ldo, const int* pos, const int* count, const int* lead, const int* shared, int B, int T_len,
+                                         int H, int G, int dim, int vdim, int Smax, int window, int keep_first, float scale, float sink,
+                                         int dtype, cudaStream_t s) {
+  if (!lead || !shared) return -1;
+  return window_general<true>(qn, kc, vc, gate, ldg, out, ldo, pos, count, B, T_len, H, G, dim, vdim, Smax, window, keep_first, scale, sink,
+                              SharedPrefix{lead, shared}, dtype, s);
 }
 
 // One token per sequence (rows of proj = sequences), bf16. dim, vdim multiples of 8, dim <= 128, vdim <= 256, ld a multiple of

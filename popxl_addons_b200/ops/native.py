@@ -1889,3 +1889,4 @@ _register_late()
 
 from . import native_sequence  # noqa: E402,F401  (kernels of the sequence-model ops)
 from . import native_serving  # noqa: E402,F401  (kernels of the serving ops)
+from . import native_beams  # noqa: E402,F401  (kernels of the ops of sequences with a common beginning)

@@ -1,0 +1,87 @@
+"""CUDA implementations of the ops of sequences with a common beginning (`xl/ops/beams.py`)."""
+import ctypes
+
+import torch
+
+from ..xl.opdef import native
+from .native import _CODE, _c_f, _c_int, _c_ll, _c_p, _ok, _sig, _stream, counters, workspace
+from .native_sequence import _f32, _i32, _ptr
+from .native_serving import _c_d, _done, _launched, _rows16
+
+_norm_append = _sig("xl_qk_norm_append_fitting", _c_p, _c_ll, *[_c_p] * 7, *[_c_int] * 7, _c_f, _c_int, _c_p)
+_shared_general = _sig("xl_window_attn_shared_general", *[_c_p] * 4, _c_ll, _c_p, _c_ll, *[_c_p] * 4, *[_c_int] * 9, _c_f, _c_f, _c_int, _c_p)
+_take_beams = _sig("xl_take_beams", *[_c_p] * 14, *[_c_int] * 5, _c_d, *[_c_int] * 5, _c_p)
+_take_beams_parts = _sig("xl_take_beams_parts", _c_int, _c_int, _c_int)
+_reorder = _sig("xl_reorder", ctypes.POINTER(_c_ll), _c_int, *[_c_p] * 3, _c_int, _c_int, _c_p)
+
+
+@native("window_attention_shared_")
+def window_attention_shared_cuda(proj, q_norm, k_norm, kc, vc, pos, count, lead, shared, joint, T, heads, window, keep_first, scale, sink, eps):
+    B, G, smax, dim = kc.shape
+    vdim, dt, dev = vc.shape[-1], proj.dtype, proj.device
+    plain = (heads + G) * dim + G * vdim
+    proj = proj if proj.stride(1) == 1 else proj.contiguous()
+    if dt not in _CODE or not (dt == kc.dtype == vc.dtype == joint.dtype) or not _f32(q_norm, k_norm) or not _i32(pos, count, lead, shared):
+        return NotImplemented
+    if not (proj.is_cuda and joint.is_cuda and kc.is_cuda and vc.is_cuda and kc.is_contiguous() and vc.is_contiguous()) or joint.stride(1) != 1:
+        return NotImplemented
+    q_norm, k_norm = _rows16(q_norm), _rows16(k_norm)
+    gated = proj.shape[1] > plain
+    code, s, ld, ldo = _CODE[dt], _stream(), proj.stride(0), joint.stride(0)
+    window, keep_first = min(window, smax), min(keep_first, smax)  # no key is further back, and the kernels count in 32 bits
+    sink = float("-inf") if sink is None else sink
+    qn = torch.empty((B, G, T, heads // G, dim), dtype=dt, device=dev)
+    rc = _norm_append(proj.data_ptr(), ld, q_norm.data_ptr(), k_norm.data_ptr(), qn.data_ptr(), kc.data_ptr(), vc.data_ptr(), pos.data_ptr(),
+                      count.data_ptr(), B, T, heads, G, dim, vdim, smax, eps, code, s)
+    if not _launched(rc, "qk_norm_append"):
+        return NotImplemented
+    rc = _shared_general(qn.data_ptr(), kc.data_ptr(), vc.data_ptr(), proj.data_ptr() + plain * proj.element_size() if gated else None, ld,
+                         joint.data_ptr(), ldo, pos.data_ptr(), count.data_ptr(), lead.data_ptr(), shared.data_ptr(), B, T, heads, G, dim, vdim, smax,
+                         window, keep_first, scale, sink, code, s)
+    _done(rc, "window_attn_shared_general")
+    return joint
+
+
+@native("take_beams_")
+def take_beams_cuda(current, parent, logits, buf, parents, step, scores, ended, length, *into, beams, end, valid, length_penalty, base, ahead,
+                    advance):
+    to = into or (scores, ended, length)
+    rows = logits.shape[0]
+    if not logits.is_cuda or logits.dtype not in _CODE or not _i32(current, parent, buf, parents, step, ended, length, to[1], to[2]):
+        return NotImplemented
+    if not _f32(scores, to[0]) or not all(t.is_cuda and t.is_contiguous() for t in (scores, to[0])):
+        return NotImplemented
+    logits, dev = logits.contiguous(), logits.device
+    parts = _take_beams_parts(rows, beams, valid)
+    scratch = workspace(rows * parts * (16 + 8 * beams), dev, "beams")
+    done = counters(rows // beams + 1, dev, "counters beams")
+    rc = _take_beams(logits.data_ptr(), scores.data_ptr(), ended.data_ptr(), length.data_ptr(), *map(_ptr, to), current.data_ptr(), parent.data_ptr(),
+                     buf.data_ptr(), parents.data_ptr(), step.data_ptr(), scratch.data_ptr(), done.data_ptr(), rows, logits.shape[1], valid, beams,
+                     end, length_penalty, buf.shape[0], base, ahead, int(advance), _CODE[logits.dtype], _stream())
+    return current if _launched(rc, "take_beams") else NotImplemented
+
+
+def _rows_of(t, axis, per):
+    """What the kernel has to know of a state: see `xl_reorder`."""
+    size, row = t.element_size(), t.stride(0) * t.element_size()
+    if axis is None:
+        return (t.data_ptr(), row, 1, 0, 1, t[0].numel() * size, 0)
+    inner = 1
+    for n in t.shape[axis + 1:]:
+        inner *= n
+    entries, outer = t.shape[axis], t[0].numel() // (t.shape[axis] * inner)
+    return (t.data_ptr(), row, outer, entries * inner * size if outer > 1 else 0, entries, inner * size, per)
+
+
+@native("reorder_")
+def reorder_cuda(parent, begin, end, *states, beams, axes, per):
+    if not _i32(parent, begin, end) or any(not (t.is_cuda and t.is_contiguous()) for t in states):
+        return NotImplemented
+    rows = [_rows_of(*s) for s in zip(states, axes, per)]
+    if any(r[5] > 0x7fffffff for r in rows):
+        return NotImplemented
+    for lo in range(0, len(rows), 64):
+        now = [x for r in rows[lo:lo + 64] for x in r]
+        _done(_reorder((_c_ll * len(now))(*now), len(now) // 7, parent.data_ptr(), begin.data_ptr(), end.data_ptr(), parent.numel(), beams, _stream()),
+              "reorder")
+    return ()
