@@ -19,6 +19,16 @@ __device__ __forceinline__ void dd_mma(float (&c)[4], uint32_t a0, uint32_t a1, 
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// c += a b for a 16 x 8 tile of which 8 RT rows are in use; a_lo / a_hi: rows quad and quad + 8, two k pairs each.
+__device__ __forceinline__ void wd_mma(float (&c)[4], const uint2& a_lo, const uint2& a_hi, uint32_t b0, uint32_t b1) {
+  dd_mma(c, a_lo.x, a_hi.x, a_lo.y, a_hi.y, b0, b1);
+}
+__device__ __forceinline__ void wd_mma(float (&c)[2], const uint2& a_lo, const uint2&, uint32_t b0, uint32_t b1) {
+  float unused0, unused1;
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%12};"
+               : "=f"(c[0]), "=f"(c[1]), "=f"(unused0), "=f"(unused1)
+               : "r"(a_lo.x), "r"(0u), "r"(a_lo.y), "r"(0u), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(0.f));
+}
 __device__ __forceinline__ uint32_t dd_pack(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));

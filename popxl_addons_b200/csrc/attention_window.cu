@@ -11,14 +11,16 @@
 //   k cache (B, G, Smax, dim), v cache (B, G, Smax, vdim)
 //   q' (B, G, T, R, dim): the rows that read one key / value head are consecutive, so that a tile can hold several heads
 //
-//   xl_qk_norm_append        q' to its buffer, k' and v into the caches (xl_qk_norm_append_fitting: of sequences that fit them)
+//   xl_qk_norm_append        q' to its buffer, k' and v into the caches
 //   xl_window_attn_general   any sizes and types, scores and weights in fp32 on the CUDA cores: one warp per row and head
-//   xl_window_attn_shared_general   the same for sequences whose first keys are those of another slot
+//   xl_shared_attn_general   the same for sequences whose first keys are those of another slot (attention_shared.cu)
 //   xl_window_attn_decode    one token per sequence, bf16: norms, append, attention and gate in one launch
 #include "attention_decode.cuh"
 #include "attention_window.cuh"
 
 #include <math.h>
+
+#include <type_traits>
 
 namespace {
 
@@ -35,12 +37,11 @@ __global__ void __launch_bounds__(256)
     qk_norm_append_kernel(const T* __restrict__ proj, long long ld, const float* __restrict__ wq, const float* __restrict__ wk,
                           T* __restrict__ qn, T* __restrict__ kc, T* __restrict__ vc, const int* __restrict__ pos,
                           const int* __restrict__ count, int T_len, int H, int G, int dim, int vdim, int Smax, float eps,
-                          int group, int whole) {
+                          int group) {
   xl_grid_launch_dependents();
   constexpr int NP = 16 / V;  // pieces per lane: 32 lanes cover WA_MAX_DIM features
   const int b = blockIdx.y, t = blockIdx.x, p = pos[b] + t;
   if (t >= count[b] || p < 0 || p >= Smax) return;
-  if (whole && (pos[b] < 0 || pos[b] > Smax - min(count[b], T_len))) return;  // a sequence that would not fit is left out
   const T* row = proj + ((long long)b * T_len + t) * ld;
   const int R = H / G, l = threadIdx.x & (group - 1), pieces = dim / V;
   const int heads_at_once = blockDim.x / group;
@@ -89,11 +90,11 @@ __global__ void __launch_bounds__(256)
 
 template <typename T, int V>
 int launch_append(const void* proj, long long ld, const float* wq, const float* wk, void* qn, void* kc, void* vc, const int* pos,
-                  const int* count, int B, int T_len, int H, int G, int dim, int vdim, int Smax, float eps, int whole, cudaStream_t s) {
+                  const int* count, int B, int T_len, int H, int G, int dim, int vdim, int Smax, float eps, cudaStream_t s) {
   int group = 1;
   while (group < 32 && group * V < dim) group *= 2;
   qk_norm_append_kernel<T, V><<<dim3(T_len, B), 256, 0, s>>>((const T*)proj, ld, wq, wk, (T*)qn, (T*)kc, (T*)vc, pos, count, T_len,
-                                                             H, G, dim, vdim, Smax, eps, group, whole);
+                                                             H, G, dim, vdim, Smax, eps, group);
   return (int)cudaGetLastError();
 }
 
@@ -101,10 +102,10 @@ int launch_append(const void* proj, long long ld, const float* wq, const float* 
 
 // SPLIT 1: a warp per query row, four of them per CTA. SPLIT 8: a CTA per query row whose warps take its blocks of 32 keys in turn
 // and merge their parts of the softmax in shared memory, for the few rows of a decoding step. SHARED: the first keys of a sequence may be
-// those of another slot.
-template <typename T, int VPL, int SPLIT, bool SHARED>  // VPL: value features per lane
+// those of another slot. TQ: type of the queries.
+template <typename T, int VPL, int SPLIT, bool SHARED, typename TQ>  // VPL: value features per lane
 __global__ void __launch_bounds__(SPLIT == 1 ? 128 : SPLIT * 32)
-    window_attn_general_kernel(const T* __restrict__ qn, const T* __restrict__ kc, const T* __restrict__ vc,
+    window_attn_general_kernel(const TQ* __restrict__ qn, const T* __restrict__ kc, const T* __restrict__ vc,
                                const T* __restrict__ gate, long long ldg, T* __restrict__ out, long long ldo,
                                const int* __restrict__ pos, const int* __restrict__ count, int T_len, int H, int G, int dim,
                                int vdim, int Smax, int window, int keep_first, float scale, float sink, const SharedPrefix prefix) {
@@ -121,10 +122,10 @@ __global__ void __launch_bounds__(SPLIT == 1 ? 128 : SPLIT * 32)
   if (p < 0 || p >= Smax) return;
   int lead = b, edge = 0;
   if (SHARED) {
-    if (pos[b] < 0 || pos[b] > Smax - min(count[b], T_len)) return;
+    if (!window_fits(pos[b], count[b], T_len, Smax)) return;
     edge = shared_edge(prefix, pos, b, pos[b], gridDim.z, lead);
   }
-  const T* q = qn + ((((long long)b * G + g) * T_len + t) * R + h % R) * dim;
+  const TQ* q = qn + ((((long long)b * G + g) * T_len + t) * R + h % R) * dim;
   for (int d = part * 32 + lane; d < dim; d += 32 * SPLIT) sq[slot][d] = xl_to_float(q[d]);
   if (SPLIT == 1) __syncwarp();
   else __syncthreads();
@@ -235,17 +236,6 @@ struct WindowDecodeParams {
 __host__ __device__ constexpr int wd_keys(int kd, int vt) { return 4 * kd + vt <= 16 ? 32 : 16; }
 // bytes of one ring stage of one warp: the keys as KD pieces of 64 B, then the value rows of vdim + 8 elements
 __host__ __device__ constexpr int wd_stage_bytes(int keys, int kd, int vdim) { return keys * kd * 64 + keys * (vdim + 8) * 2; }
-
-// c += a b for a 16 x 8 tile of which 8 RT rows are in use; a_lo / a_hi: rows quad and quad + 8, two k pairs each.
-__device__ __forceinline__ void wd_mma(float (&c)[4], const uint2& a_lo, const uint2& a_hi, uint32_t b0, uint32_t b1) {
-  dd_mma(c, a_lo.x, a_hi.x, a_lo.y, a_hi.y, b0, b1);
-}
-__device__ __forceinline__ void wd_mma(float (&c)[2], const uint2& a_lo, const uint2&, uint32_t b0, uint32_t b1) {
-  float unused0, unused1;
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%12};"
-               : "=f"(c[0]), "=f"(c[1]), "=f"(unused0), "=f"(unused1)
-               : "r"(a_lo.x), "r"(0u), "r"(a_lo.y), "r"(0u), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(0.f));
-}
 
 // KD: 32-feature steps of a query / key row (dim <= 32 KD); VT: 8-feature tiles of a value row (vdim <= 8 VT)
 template <int KD, int VT, int RT>
@@ -638,37 +628,21 @@ template <int KD, int VT> int wd_launch(const WindowDecodeParams& p, int B, int 
 
 }  // namespace
 
-namespace {
-
-int norm_append(const void* proj, long long ld, const float* wq, const float* wk, void* qn, void* kc, void* vc, const int* pos, const int* count,
-                int B, int T_len, int H, int G, int dim, int vdim, int Smax, float eps, int whole, int dtype, cudaStream_t s) {
+// proj: (B*T_len, ld) as described above; wq, wk (dim) fp32; qn (B, G, T_len, H/G, dim). dim <= 512. Rows past count[b] are
+// left out.
+XL_API int xl_qk_norm_append(const void* proj, long long ld, const float* wq, const float* wk, void* qn, void* kc, void* vc,
+                             const int* pos, const int* count, int B, int T_len, int H, int G, int dim, int vdim, int Smax,
+                             float eps, int dtype, cudaStream_t s) {
   if (B < 1 || B > 65535 || T_len < 1 || G < 1 || H < 1 || H % G || dim < 1 || dim > WA_MAX_DIM || vdim < 1 || Smax < 1 ||
       ld < (long long)(H + G) * dim + (long long)G * vdim || !wq || !wk)
     return -1;
   XL_DISPATCH_DTYPE(dtype, T, {
     constexpr int V = 16 / sizeof(T);
     if (dim % V == 0 && vdim % V == 0 && ld % V == 0 && (((uintptr_t)proj | (uintptr_t)qn | (uintptr_t)kc | (uintptr_t)vc) & 15) == 0)
-      return launch_append<T, V>(proj, ld, wq, wk, qn, kc, vc, pos, count, B, T_len, H, G, dim, vdim, Smax, eps, whole, s);
-    return launch_append<T, 1>(proj, ld, wq, wk, qn, kc, vc, pos, count, B, T_len, H, G, dim, vdim, Smax, eps, whole, s);
+      return launch_append<T, V>(proj, ld, wq, wk, qn, kc, vc, pos, count, B, T_len, H, G, dim, vdim, Smax, eps, s);
+    return launch_append<T, 1>(proj, ld, wq, wk, qn, kc, vc, pos, count, B, T_len, H, G, dim, vdim, Smax, eps, s);
   });
   return (int)cudaGetLastError();
-}
-
-}  // namespace
-
-// proj: (B*T_len, ld) as described above; wq, wk (dim) fp32; qn (B, G, T_len, H/G, dim). dim <= 512. Rows past count[b] are
-// left out.
-XL_API int xl_qk_norm_append(const void* proj, long long ld, const float* wq, const float* wk, void* qn, void* kc, void* vc,
-                             const int* pos, const int* count, int B, int T_len, int H, int G, int dim, int vdim, int Smax,
-                             float eps, int dtype, cudaStream_t s) {
-  return norm_append(proj, ld, wq, wk, qn, kc, vc, pos, count, B, T_len, H, G, dim, vdim, Smax, eps, 0, dtype, s);
-}
-
-// The same, and sequences whose rows would not all fit the cache are left out.
-XL_API int xl_qk_norm_append_fitting(const void* proj, long long ld, const float* wq, const float* wk, void* qn, void* kc, void* vc,
-                                     const int* pos, const int* count, int B, int T_len, int H, int G, int dim, int vdim, int Smax,
-                                     float eps, int dtype, cudaStream_t s) {
-  return norm_append(proj, ld, wq, wk, qn, kc, vc, pos, count, B, T_len, H, G, dim, vdim, Smax, eps, 1, dtype, s);
 }
 
 namespace {
@@ -683,16 +657,17 @@ int window_general(const void* qn, const void* kc, const void* vc, const void* g
   // a CTA per row while that is no more than about two CTAs of eight warps per SM; longer portions fill the SMs with a warp per row
   const bool split = (long long)T_len * H * B <= 2 * 148;
   const dim3 grid(split ? T_len : (T_len + 3) / 4, H, B);
-#define XL_WG(VPL)                                                                                                                 \
-  if (split)                                                                                                                       \
-    window_attn_general_kernel<T, VPL, 8, SHARED><<<grid, 256, 0, s>>>((const T*)qn, (const T*)kc, (const T*)vc, (const T*)gate,   \
-                                                               ldg, (T*)out, ldo, pos, count, T_len, H, G, dim, vdim, Smax,        \
-                                                               window, keep_first, scale, sink, prefix);                          \
-  else                                                                                                                             \
-    window_attn_general_kernel<T, VPL, 1, SHARED><<<grid, 128, 0, s>>>((const T*)qn, (const T*)kc, (const T*)vc, (const T*)gate,   \
-                                                               ldg, (T*)out, ldo, pos, count, T_len, H, G, dim, vdim, Smax,        \
-                                                               window, keep_first, scale, sink, prefix)
+#define XL_WG(VPL)                                                                                                                  \
+  if (split)                                                                                                                        \
+    window_attn_general_kernel<T, VPL, 8, SHARED><<<grid, 256, 0, s>>>((const TQ*)qn, (const T*)kc, (const T*)vc, (const T*)gate,   \
+                                                                       ldg, (T*)out, ldo, pos, count, T_len, H, G, dim, vdim, Smax, \
+                                                                       window, keep_first, scale, sink, prefix);                    \
+  else                                                                                                                              \
+    window_attn_general_kernel<T, VPL, 1, SHARED><<<grid, 128, 0, s>>>((const TQ*)qn, (const T*)kc, (const T*)vc, (const T*)gate,   \
+                                                                       ldg, (T*)out, ldo, pos, count, T_len, H, G, dim, vdim, Smax, \
+                                                                       window, keep_first, scale, sink, prefix)
   XL_DISPATCH_DTYPE(dtype, T, {
+    using TQ = typename std::conditional<SHARED, float, T>::type;
     if (vdim <= 128) { XL_WG(4); }
     else { XL_WG(16); }
   });
@@ -712,12 +687,12 @@ XL_API int xl_window_attn_general(const void* qn, const void* kc, const void* vc
                                SharedPrefix{}, dtype, s);
 }
 
-// The same for sequences whose first min(shared[b], pos[b], pos[lead[b]]) keys and values are those of slot lead[b]. Sequences whose rows would not
-// all fit the cache are left out.
-XL_API int xl_window_attn_shared_general(const void* qn, const void* kc, const void* vc, const void* gate, long long ldg, void* out,
-                                         long long ldo, const int* pos, const int* count, const int* lead, const int* shared, int B, int T_len,
-                                         int H, int G, int dim, int vdim, int Smax, int window, int keep_first, float scale, float sink,
-                                         int dtype, cudaStream_t s) {
+// The same with queries in fp32, for sequences whose first min(shared[b], pos[b], pos[lead[b]]) keys and values are those of slot lead[b].
+// Sequences whose rows would not all fit the cache are left out.
+XL_API int xl_shared_attn_general(const float* qn, const void* kc, const void* vc, const void* gate, long long ldg, void* out, long long ldo,
+                                  const int* pos, const int* count, const int* lead, const int* shared, int B, int T_len, int H, int G,
+                                  int dim, int vdim, int Smax, int window, int keep_first, float scale, float sink, int dtype,
+                                  cudaStream_t s) {
   if (!lead || !shared) return -1;
   return window_general<true>(qn, kc, vc, gate, ldg, out, ldo, pos, count, B, T_len, H, G, dim, vdim, Smax, window, keep_first, scale, sink,
                               SharedPrefix{lead, shared}, dtype, s);

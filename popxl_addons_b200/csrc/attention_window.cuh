@@ -18,6 +18,9 @@ struct SharedPrefix {
   const int *lead, *shared;
 };
 
+// whether the real rows of a portion of T rows at position pos fit the cache
+__device__ __forceinline__ bool window_fits(int pos, int count, int T, int Smax) { return pos >= 0 && pos <= Smax - min(count, T); }
+
 // how many positions of sequence b, at position pos, are those of `lead` (which is set to b where there are none)
 __device__ __forceinline__ int shared_edge(const SharedPrefix& s, const int* pos_of, int b, int pos, int batch, int& lead) {
   lead = s.lead[b];

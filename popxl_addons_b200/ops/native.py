@@ -358,7 +358,13 @@ def check_gemm_errors():
                      94: "attention over an 8-bit cache: key / value stage was never released",
                      95: "attention over an 8-bit cache: scores never completed",
                      96: "attention over an 8-bit cache: weights never arrived",
-                     97: "attention over an 8-bit cache: output accumulation never completed"}
+                     97: "attention over an 8-bit cache: output accumulation never completed",
+                     101: "attention over shared prefixes: query tiles never arrived",
+                     102: "attention over shared prefixes: key / value tile never arrived",
+                     103: "attention over shared prefixes: key / value stage was never released",
+                     104: "attention over shared prefixes: scores never completed",
+                     105: "attention over shared prefixes: weights never arrived",
+                     106: "attention over shared prefixes: output accumulation never completed"}
             raise RuntimeError(f"tcgen05 GEMM on cuda:{idx} gave up waiting: {names.get(code, code)}")
 
 

@@ -4,12 +4,13 @@ import ctypes
 import torch
 
 from ..xl.opdef import native
-from .native import _CODE, _c_f, _c_int, _c_ll, _c_p, _ok, _sig, _stream, counters, workspace
+from .native import _CODE, _c_f, _c_int, _c_ll, _c_p, _ok, _sig, _stream, counters, gemm_error_flag, workspace
 from .native_sequence import _f32, _i32, _ptr
 from .native_serving import _c_d, _done, _launched, _rows16
 
-_norm_append = _sig("xl_qk_norm_append_fitting", _c_p, _c_ll, *[_c_p] * 7, *[_c_int] * 7, _c_f, _c_int, _c_p)
-_shared_general = _sig("xl_window_attn_shared_general", *[_c_p] * 4, _c_ll, _c_p, _c_ll, *[_c_p] * 4, *[_c_int] * 9, _c_f, _c_f, _c_int, _c_p)
+_shared_append = _sig("xl_shared_append", _c_p, _c_ll, *[_c_p] * 7, *[_c_int] * 7, _c_f, _c_int, _c_p)
+_shared_general = _sig("xl_shared_attn_general", *[_c_p] * 4, _c_ll, _c_p, _c_ll, *[_c_p] * 4, *[_c_int] * 9, _c_f, _c_f, _c_int, _c_p)
+_shared_portion = _sig("xl_shared_attn_portion", _c_p, _c_ll, *[_c_p] * 4, _c_ll, *[_c_p] * 4, *[_c_int] * 10, *[_c_f] * 3, _c_p, _c_p)
 _take_beams = _sig("xl_take_beams", *[_c_p] * 14, *[_c_int] * 5, _c_d, *[_c_int] * 5, _c_p)
 _take_beams_parts = _sig("xl_take_beams_parts", _c_int, _c_int, _c_int)
 _reorder = _sig("xl_reorder", ctypes.POINTER(_c_ll), _c_int, *[_c_p] * 3, _c_int, _c_int, _c_p)
@@ -30,15 +31,27 @@ def window_attention_shared_cuda(proj, q_norm, k_norm, kc, vc, pos, count, lead,
     code, s, ld, ldo = _CODE[dt], _stream(), proj.stride(0), joint.stride(0)
     window, keep_first = min(window, smax), min(keep_first, smax)  # no key is further back, and the kernels count in 32 bits
     sink = float("-inf") if sink is None else sink
-    qn = torch.empty((B, G, T, heads // G, dim), dtype=dt, device=dev)
-    rc = _norm_append(proj.data_ptr(), ld, q_norm.data_ptr(), k_norm.data_ptr(), qn.data_ptr(), kc.data_ptr(), vc.data_ptr(), pos.data_ptr(),
-                      count.data_ptr(), B, T, heads, G, dim, vdim, smax, eps, code, s)
-    if not _launched(rc, "qk_norm_append"):
+    norms, caches = (q_norm.data_ptr(), k_norm.data_ptr()), (kc.data_ptr(), vc.data_ptr())
+    where = tuple(t.data_ptr() for t in (pos, count, lead, shared))
+    sizes = (B, T, heads, G, dim, vdim, smax)
+
+    def append(qn):
+        return _shared_append(proj.data_ptr(), ld, *norms, _ptr(qn), *caches, *where[:2], *sizes, eps, code, s)
+
+    if (dt == torch.bfloat16 and dim <= 128 and vdim <= 128 and dim % 8 == vdim % 8 == ld % 8 == ldo % 8 == 0
+            and all(t.data_ptr() % 16 == 0 for t in (proj, joint, kc, vc))):
+        if not _launched(append(None), "shared_append"):
+            return NotImplemented
+        rc = _shared_portion(proj.data_ptr(), ld, norms[0], *caches, joint.data_ptr(), ldo, *where, *sizes, window, keep_first, int(gated), scale, sink,
+                             eps, gemm_error_flag(dev).data_ptr(), s)
+        if rc >= 0:
+            _done(rc, "shared_attn_portion")
+            return joint
+    qn = torch.empty((B, G, T, heads // G, dim), dtype=torch.float32, device=dev)
+    if not _launched(append(qn), "shared_append"):
         return NotImplemented
-    rc = _shared_general(qn.data_ptr(), kc.data_ptr(), vc.data_ptr(), proj.data_ptr() + plain * proj.element_size() if gated else None, ld,
-                         joint.data_ptr(), ldo, pos.data_ptr(), count.data_ptr(), lead.data_ptr(), shared.data_ptr(), B, T, heads, G, dim, vdim, smax,
-                         window, keep_first, scale, sink, code, s)
-    _done(rc, "window_attn_shared_general")
+    _done(_shared_general(qn.data_ptr(), *caches, proj.data_ptr() + plain * proj.element_size() if gated else None, ld, joint.data_ptr(), ldo, *where,
+                          *sizes, window, keep_first, scale, sink, code, s), "shared_attn_general")
     return joint
 
 

@@ -21,7 +21,7 @@ from .sequence import _rms
 from .serving import _expect
 
 MAX_BEAMS = 32          # of a group
-MAX_SHARED_BATCH = 4096  # sequences of one attention over shared prefixes
+MAX_SHARED_BATCH = 1024  # sequences of one attention over shared prefixes
 
 
 class BeamState(NamedTuple):
@@ -60,11 +60,12 @@ def _window_attention_shared_ref(proj, q_norm, k_norm, kc, vc, pos, count, lead,
     live = [b for b, (p, n) in enumerate(places) if n > 0 and 0 <= p and p + n <= smax]
     for b in live:
         p, n = places[b]
-        kc[b, :, p:p + n] = _rms(rows[b, :n, heads * dim:qk].reshape(n, G, dim), k_norm, eps).to(dt).transpose(0, 1)
+        k = rows[b, :n, heads * dim:qk].reshape(n, G, dim).double()
+        kc[b, :, p:p + n] = (k / torch.sqrt((k * k).mean(-1, keepdim=True) + eps) * k_norm.double()).to(dt).transpose(0, 1)
         vc[b, :, p:p + n] = rows[b, :n, qk:qk + G * vdim].reshape(n, G, vdim).transpose(0, 1)
     for b in live:
         (p, n), e, cur = places[b], edge[b], rows[b]
-        q = _rms(cur[:n, :heads * dim].reshape(n, G, heads // G, dim), q_norm, eps).to(dt).float()
+        q = _rms(cur[:n, :heads * dim].reshape(n, G, heads // G, dim), q_norm, eps)
         keys, vals = (torch.cat((c[int(lead[b]), :, :e] if e else c[b, :, :0], c[b, :, e:p + n]), 1).float() for c in (kc, vc))
         qp, kp = torch.arange(p, p + n, device=dev)[:, None], torch.arange(p + n, device=dev)[None]
         mask = kp <= qp
@@ -159,7 +160,8 @@ def window_attention_shared_(proj: Tensor, q_norm: Tensor, k_norm: Tensor, k_cac
                              keep_first: int = 0, sink: Optional[float] = None, eps: float = 1e-6) -> Tensor:
     """`window_attention_` where the first `shared[b]` positions of sequence `b` are those of slot `lead[b]` (both int32; a lead that is not
     there: none), and the others its own. Nobody shares more than both hold before the op: `min(shared[b], pos[b], pos[lead[b]])`
-    positions, which have to be in the lead's own cache. New keys and values go to the sequence's own. A sequence that would not fit the cache is
+    positions, which have to be in the lead's own cache. New keys and values go to the sequence's own; norms of keys are taken in 64 bits and rounded
+    once, queries are not rounded to the model's type. A sequence that would not fit the cache is
     left out, rows past `count[b]` are left as they are. A value that is not finite makes those results non-finite (at least in the feature
     concerned) that read its position, and may do so for the other results of its own sequence's portion; no other sequence is touched.
     On the GPU bf16 models of features up to 128 in multiples of 8 run on the tensor cores, where the keys that a group of sequences shares

@@ -10,7 +10,7 @@ def unit(x, w, eps):
 
 
 def shared_attention(proj, wq, wk, k, v, pos, count, lead, shared, T, H, window, keep, scale, sink, eps, dtype):
-    """`proj (B, T, columns)`, caches `k (B, G, S, d)`, `v` in float64, changed in place. Queries and new keys are rounded to `dtype`.
+    """`proj (B, T, columns)`, caches `k (B, G, S, d)`, `v` in float64, changed in place. New keys are rounded to `dtype`.
     Returns `{(sequence, row): (heads * vdim)}` of the real rows."""
     B, G, S, d = k.shape
     dv, R, out = v.shape[-1], H // G, {}
@@ -25,7 +25,7 @@ def shared_attention(proj, wq, wk, k, v, pos, count, lead, shared, T, H, window,
         edge = max(0, min(shared[b], p, pos[lead[b]])) if 0 <= lead[b] < B else 0
         for t in range(n):
             i, row, heads = p + t, proj[b, t], []
-            q = unit(row[:H * d].reshape(H, d), wq, eps).to(dtype).double()
+            q = unit(row[:H * d].reshape(H, d), wq, eps)
             seen = torch.tensor([j for j in range(i + 1) if not window or i - j < window or j < keep])
             theirs, own = seen[seen < edge], seen[seen >= edge]
             for h in range(H):

@@ -46,10 +46,10 @@ ROOM = 262
 def bound(backend):
     """Largest difference over the largest output. 32 bits: scores of up to 10 from sums of `dim` roundings of 2^-24 relative to |q||k|,
     about 2^-18 of a weight, and as much again for sums over keys: 2e-5. 16 bits: the rounding of the output, half a step or eps / 2 of the
-    value; weights enter as two numbers of 16 bits, which loses 2^-16; a query or key whose norm in 32 bits lies within 2^-22 of a border
-    between two numbers of the type, one in a hundred, is off by eps of one of `dim` terms of a score: eps / 4 in all."""
+    value; queries and weights enter as two numbers of 16 bits each or in 32, which loses 2^-16 of a score and of a weight, 2^-12 of the
+    result at most: eps / 16 of bf16, and of fp16, whose products are in 32 bits, less."""
     eps = torch.finfo(backend[1]).eps
-    return 2e-5 if backend[1] == torch.float32 else 0.75 * eps
+    return 2e-5 if backend[1] == torch.float32 else 0.5625 * eps
 
 
 def attention_case(backend, shape, mask, group, T, seed=0, wide=0):
@@ -80,7 +80,6 @@ def attention_case(backend, shape, mask, group, T, seed=0, wide=0):
 
 
 def check_attention(backend, args, kw, want, after):
-    before = [c.clone() for c in args[3:5]]
     got = op("window_attention_shared_", backend, *args, **kw)
     B, width, T = args[3].shape[0], kw["heads"] * args[4].shape[-1], kw["T"]
     got = got.reshape(B, T, -1).double().cpu()
@@ -92,14 +91,10 @@ def check_attention(backend, args, kw, want, after):
                 assert (got[b, t, width:] == -7).all()
             else:
                 assert (got[b, t] == -7).all(), (b, t)
-    # keys are rounded as the oracle rounds, or one step off at a border; values are taken as they are
-    for now, was, ref, steps in zip(args[3:5], before, after, (1.01, 0)):
-        now, was = now.double().cpu(), was.double().cpu()
-        same = torch.isnan(now) & torch.isnan(ref)
-        limit = ref.abs() * torch.finfo(args[3].dtype).eps * steps + 1e-6 * bool(steps)
-        assert ((now - ref).abs() <= limit)[~same].all()
-        left = (ref == was) | torch.isnan(ref)
-        assert (now[left].nan_to_num() == was[left].nan_to_num()).all()
+    # norms of keys are taken in 64 bits and rounded once: a border between two numbers within 2^-50 of one does not happen
+    for now, ref in zip(args[3:5], after):
+        now = now.double().cpu()
+        assert (now.isnan() == ref.isnan()).all() and (now.nan_to_num() == ref.nan_to_num()).all()
 
 
 @pytest.mark.parametrize("T", [1, 9])
@@ -118,14 +113,15 @@ def test_attention_of_strided_projections(backend, T):
 
 @pytest.mark.parametrize("T", [1, 9])
 def test_attention_where_nothing_is_shared_is_the_plain_one(backend, T):
-    """The results of `window_attention_`, to the rounding of its results."""
+    """The results of `window_attention_`, which rounds its queries and may round a key to the other side: eps / 2 of each of `dim` terms of a
+    score, independent ones, 0.02 of a weight at most in bf16."""
     args, kw, _, _ = attention_case(backend, "full", "window", "alone", T)
     other = [a.clone() for a in args]
     got = op("window_attention_shared_", backend, *args, **kw).double()
     ref = op("window_attention_", backend, *other[:7], other[9], **kw).double()
     live = ref != -7
     assert torch.equal(live, got != -7)
-    assert (got - ref)[live].abs().max() <= 2 * bound(backend) * ref[live].abs().max()
+    assert (got - ref)[live].abs().max() <= (2e-5 if backend[1] == torch.float32 else 3 * torch.finfo(backend[1]).eps) * ref[live].abs().max()
 
 
 @pytest.mark.parametrize("T", [1, 9])
@@ -171,7 +167,7 @@ def test_refusals_of_attention():
         for bad in (dict(cols=100), dict(heads=3), dict(scale=0.0), dict(window=-1), dict(keep_first=-1), dict(joint=var((3, 90))), dict(joint=var((2, 96))),
                     dict(norm=var((15,))), dict(norm=var((16,), xl.bfloat16)), dict(vcache=var((3, 2, 29, 24))), dict(vcache=var((3, 2, 30, 24), xl.bfloat16)),
                     dict(places=[var((3,), xl.int32)] * 3 + [var((2,), xl.int32)]), dict(places=[var((3,))] * 4), dict(d=520), dict(v=520), dict(T=0),
-                    dict(joint=var((3, 96), xl.bfloat16)), dict(B=4097)):
+                    dict(joint=var((3, 96), xl.bfloat16)), dict(B=1025)):
             with pytest.raises(ValueError):
                 call(**bad)
 
