@@ -3,10 +3,13 @@
 //
 //   xl_shared_append           new keys (norms in 64 bits, rounded once) and values into the caches; for the general kernel queries in fp32
 //   xl_shared_attn_portion     portions of tokens on the tensor cores (tcgen05), bf16
+//   xl_shared_attn_decode      one token per sequence, bf16: the keys that a group of sequences shares, once for the group (tcgen05), and each
+//                              sequence's own keys (mma.sync)
 //   xl_shared_attn_general     any sizes and types (attention_window.cu)
 //
 // Queries enter the products as two bf16 numbers, value and rounding error, as the weights do: a rounded query would move every score by
 // 2^-9 of itself, more than all other roundings together.
+#include "attention_decode.cuh"
 #include "attention_window.cuh"
 #include "tcgen05.cuh"
 
@@ -77,7 +80,7 @@ constexpr int UMMA_K = 16;
 constexpr int SA_THREADS = 64 + 2 * 128;
 constexpr uint32_t TMEM_COLS = 512;
 
-enum { ERR_Q = 101, ERR_KV_FULL = 102, ERR_KV_EMPTY = 103, ERR_S = 104, ERR_P = 105, ERR_PV = 106 };
+enum { ERR_Q = 101, ERR_KV_FULL = 102, ERR_KV_EMPTY = 103, ERR_S = 104, ERR_P = 105, ERR_PV = 106, ERR_MEET = 107 };
 
 struct SharedParams {
   const __nv_bfloat16* proj;
@@ -102,9 +105,9 @@ template <int DK, int VD> struct SharedTiles {
   static constexpr int SLOT = K_BYTES > V_BYTES ? K_BYTES : V_BYTES;
 };
 
-// Rows of a tile, normalised, to shared memory as two K-major operands of 128-byte swizzle: the 32 rows of one warp. `row(r)`: where the
-// projections have the head of row r of the tile, or null.
-template <int DK, typename F>
+// COUNT rows of a tile, normalised by one warp, to shared memory as two K-major operands of 128-byte swizzle. `row(r)`: where the projections
+// have the head of row r of the tile, or null.
+template <int DK, int COUNT, typename F>
 __device__ __forceinline__ void load_queries(uint8_t* tile, int first_row, const F& row, const float* wq, int dim, float eps) {
   constexpr int LANES = DK / 8, ROWS = 32 / LANES;  // lanes of a row, rows at a time
   const int lane = threadIdx.x & 31, chunk = lane % LANES;
@@ -113,7 +116,7 @@ __device__ __forceinline__ void load_queries(uint8_t* tile, int first_row, const
 #pragma unroll
   for (int e = 0; e < 8; ++e) w[e] = on ? wq[chunk * 8 + e] : 0.f;
 #pragma unroll 4
-  for (int i = 0; i < 32; i += ROWS) {
+  for (int i = 0; i < COUNT; i += ROWS) {
     const int r = first_row + i + lane / LANES;
     const __nv_bfloat16* src = row(r);
     float x[8], sq = 0.f;
@@ -384,7 +387,7 @@ __global__ void __launch_bounds__(SA_THREADS, 1)
     const int r = qtr * 32 + lane;            // row inside the tile
     const long long f = f0 + m * TILE_M + r;  // (token, head of the group)
     const int t = (int)(f / R), hh = (int)(f - (long long)t * R);
-    load_queries<DK>(sQ + m * L::Q_BYTES, qtr * 32, [&](int row) -> const __nv_bfloat16* {
+    load_queries<DK, 32>(sQ + m * L::Q_BYTES, qtr * 32, [&](int row) -> const __nv_bfloat16* {
       const long long at = f0 + m * TILE_M + row;
       if (at >= rows) return nullptr;
       const int tt = (int)(at / R);
@@ -493,6 +496,952 @@ template <int DK, int VD> int launch_portion(const void* kc, const void* vc, con
   return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
 }
 
+// ---- single tokens: the shared positions, once for all that share them -------------------------------------------------------------
+// The query heads of all sequences of a group (those with the same lead) that read one key / value head are the rows of tiles of 128, so a
+// group's shared keys and values are read once per tile and not once per sequence. The blocks of all tiles, groups and heads are one long
+// list, of which every CTA (one per SM) takes an equal run; a tile whose blocks belong to several CTAs leaves as many parts of its sums, and so does
+// each of the two warpgroups, which take a CTA's blocks in turn: one block's softmax runs under the other's products and loads. The kernel behind
+// this one (shared_attn_decode_kernel) adds the parts to what the sequences' own keys give.
+//
+// Every CTA makes the list by itself, from positions and leads in shared memory: counts, key ranges and offsets by slot, ranks of the members by
+// votes. CTA 0 leaves a copy for the kernel behind.
+//
+// Keys that only some rows of a tile see are masked; a value that is not finite in a block that some row does not see whole is taken out, and
+// the scores of its key become NaN for the rows that see it: a weight of zero times anything would reach the others.
+constexpr int PF_SLOTS_LARGE = 4, PF_SLOTS_SMALL = 8;
+
+struct PrefixPlan {  // where a sequence's parts are
+  int first, blocks, tiles, row;      // first block of the group, blocks of a tile, tiles of a head, the sequence's first row in the group
+  int packed, total, ctas, unused;    // rows of the groups before, blocks in all, CTAs that share them
+};
+
+struct PrefixParams {
+  SharedParams p;
+  float *main_o, *extra_o;    // parts that begin with a tile's first block: [2][G][B R][vdim]; others, by CTA: [ctas][2][TILE_M][vdim]
+  float2 *main_s, *extra_s;   // their maxima (powers of two) and sums
+  PrefixPlan* plan;           // [B]
+  int read_ahead;             // positions, counts, leads and the caches were complete before the previous launch
+};
+
+struct PrefixLists {  // by slot or by sequence
+  int *edge, *hi, *lo, *begin, *members, *run;
+  short *lead, *offset, *rank, *order;
+  __host__ __device__ static int bytes(int B) { return (B + 7) / 8 * 8 * (6 * 4 + 4 * 2); }
+  __device__ __forceinline__ PrefixLists(void* at, int B) {
+    const int n = (B + 7) / 8 * 8;
+    edge = (int*)at; hi = edge + n; lo = hi + n; begin = lo + n; members = begin + n; run = members + n;
+    lead = (short*)(run + n); offset = lead + n; rank = offset + n; order = rank + n;
+  }
+};
+
+// the blocks of a group's shared keys: those of the kept tokens, then those from `first` on
+struct PrefixBlocks {
+  int kept, first, end, kept_blocks, total;
+  __device__ __forceinline__ PrefixBlocks(int lo, int hi, int keep_first) {
+    kept = min(keep_first, lo);
+    first = lo;
+    end = hi;
+    kept_blocks = key_blocks(0, kept);
+    total = kept_blocks + key_blocks(first, hi);
+    if (total >= key_blocks(0, hi)) {  // leaving keys out saves no block
+      kept = first = kept_blocks = 0;
+      total = key_blocks(0, hi);
+    }
+  }
+};
+
+struct PrefixSegment {  // blocks [block, block + count) of one tile
+  int slot, g, tile, block, count, rows;
+  bool whole;           // begins with the tile's first block
+};
+
+template <int DK, int VD> struct PrefixSmem : SharedTiles<DK, VD> {
+  using L = SharedTiles<DK, VD>;
+  static constexpr int SLOTS = L::SLOT > 16384 ? PF_SLOTS_LARGE : PF_SLOTS_SMALL;
+  static constexpr int TILE_BYTES = L::Q_BYTES + SLOTS * L::SLOT;
+  static int total(int B) {
+    const int needed = TILE_BYTES + 1024 /*alignment*/ + 512 /*barriers*/ + PrefixLists::bytes(B);
+    // more than half of an SM's shared memory: two CTAs, each holding all of TMEM, never meet on an SM
+    return needed > 120 * 1024 ? needed : 120 * 1024;
+  }
+};
+
+// A barrier of warps whose wait is bounded: every warp arrives and waits for its phase.
+__device__ __forceinline__ bool warps_meet(uint64_t* bar, uint32_t& phase, volatile int* abort_flag, int* err) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+  const bool ok = mbar_wait_warp(bar, phase & 1u, abort_flag, err, ERR_MEET);
+  ++phase;
+  return ok;
+}
+
+template <int DK, int VD>
+__global__ void __launch_bounds__(SA_THREADS, 1)
+    shared_attn_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const PrefixParams a) {
+  using L = PrefixSmem<DK, VD>;
+  constexpr int SLOTS = L::SLOTS;
+  const SharedParams& p = a.p;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint8_t* sQ = smem;
+  uint8_t* ring = smem + L::Q_BYTES;
+  uint64_t* bars = (uint64_t*)(smem + L::TILE_BYTES);
+  uint64_t* q_full = bars;
+  uint64_t* s_full = bars + 1;   // [2] per warpgroup
+  uint64_t* p_full = bars + 3;   // [2]
+  uint64_t* pv_done = bars + 5;  // [2]
+  uint64_t* all_meet = bars + 7;  // both warpgroups
+  uint64_t* wg_meet = bars + 8;   // [2]
+  uint64_t* full = bars + 10;     // [SLOTS]
+  uint64_t* empty = bars + 10 + SLOTS;
+  uint32_t* tmem_base_slot = (uint32_t*)(bars + 10 + 2 * SLOTS);
+  volatile int* abort_flag = (volatile int*)(tmem_base_slot + 1);
+  int* least_edge = (int*)(tmem_base_slot + 2);  // [2][4] by warp: smallest edge and latest window of its rows
+  int* last_first = least_edge + 8;
+  uint32_t* unknown = (uint32_t*)(last_first + 8);  // [2][4] keys whose values are not finite
+  int* total_blocks = (int*)(unknown + 8);
+  static_assert((10 + 2 * SLOTS) * 8 + 8 + 25 * 4 <= 512, "room behind the tiles");
+  const PrefixLists list(smem + L::TILE_BYTES + 512, p.B);
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, R = p.H / p.G;
+  if (!a.read_ahead) xl_grid_dependency_wait();
+  // ---- the list of blocks ------------------------------------------------------------------------------------------------------
+  for (int b = tid; b < p.B; b += SA_THREADS) {
+    list.members[b] = list.run[b] = list.hi[b] = 0;
+    list.lo[b] = 0x7fffffff;
+  }
+  __syncthreads();
+  for (int b = tid; b < p.B; b += SA_THREADS) {
+    int lead = b, e = 0;
+    const int pos = p.pos[b];
+    if (p.count[b] > 0 && window_fits(pos, p.count[b], 1, p.Smax)) e = shared_edge(p.prefix, p.pos, b, pos, p.B, lead);
+    const int first = window_range(pos, p.window, 0).first;
+    const bool sees = e > 0 && (first < e || p.keep_first > 0);
+    list.edge[b] = e;
+    list.lead[b] = (short)(sees ? lead : -1);
+    if (sees) {
+      atomicAdd(list.members + lead, 1);
+      atomicMax(list.hi + lead, e);
+      atomicMin(list.lo + lead, min(first, e));
+    }
+  }
+  __syncthreads();
+  if (warp == 0) {  // offsets by slot
+    int rows = 0, blocks = 0;
+    for (int s0 = 0; s0 < p.B; s0 += 32) {
+      const int s = s0 + lane, n = s < p.B ? list.members[s] : 0;
+      int work = 0;
+      if (n) work = (n * R + TILE_M - 1) / TILE_M * p.G * PrefixBlocks(list.lo[s], list.hi[s], p.keep_first).total;
+      int up_n = n, up_w = work;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, up_n, d), y = __shfl_up_sync(0xffffffffu, up_w, d);
+        if (lane >= d) { up_n += x; up_w += y; }
+      }
+      if (s < p.B) {
+        list.offset[s] = (short)(rows + up_n - n);
+        list.begin[s] = blocks + up_w - work;
+      }
+      rows += __shfl_sync(0xffffffffu, up_n, 31);
+      blocks += __shfl_sync(0xffffffffu, up_w, 31);
+    }
+    if (lane == 0) *total_blocks = blocks;
+  } else if (warp == 1) {  // ranks of the members
+    for (int b0 = 0; b0 < p.B; b0 += 32) {
+      const int b = b0 + lane, s = b < p.B ? list.lead[b] : -1;
+      const unsigned int same = __match_any_sync(0xffffffffu, s);
+      const int before = __popc(same & ((1u << lane) - 1)), old = s >= 0 ? list.run[s] : 0;
+      __syncwarp();
+      if (s >= 0 && before == 0) list.run[s] = old + __popc(same);
+      __syncwarp();
+      if (b < p.B) list.rank[b] = (short)(old + before);
+    }
+  }
+  __syncthreads();
+  const int total = *total_blocks, ctas = min((int)gridDim.x, total);
+  if (blockIdx.x == 0) xl_grid_dependency_wait();  // an earlier attention may still read its plan
+  for (int b = tid; b < p.B; b += SA_THREADS) {
+    const int s = list.lead[b];
+    if (s >= 0) list.order[list.offset[s] + list.rank[b]] = (short)b;
+    if (blockIdx.x == 0) {
+      PrefixPlan x = {};
+      if (s >= 0) {
+        x.first = list.begin[s];
+        x.blocks = PrefixBlocks(list.lo[s], list.hi[s], p.keep_first).total;
+        x.tiles = (list.members[s] * R + TILE_M - 1) / TILE_M;
+        x.row = list.rank[b] * R;
+        x.packed = list.offset[s] * R;
+        x.total = total;
+        x.ctas = ctas;
+      }
+      a.plan[b] = x;
+    }
+  }
+  if ((int)blockIdx.x >= ctas) {
+    xl_grid_dependency_wait();
+    return;
+  }
+  const XlRanges ranges{total / ctas, total % ctas};
+  const int x0 = ranges.begin(blockIdx.x), x1 = ranges.begin(blockIdx.x + 1);
+  // the run of blocks from x on that belong to one tile
+  auto segment = [&](int x) {
+    int s = 0;  // the last slot whose blocks begin at x or before
+    for (int step = 512; step; step >>= 1)
+      if (s + step < p.B && list.begin[s + step] <= x) s += step;
+    const int n = PrefixBlocks(list.lo[s], list.hi[s], p.keep_first).total, rows = list.members[s] * R;
+    const int tiles = (rows + TILE_M - 1) / TILE_M, unit = (x - list.begin[s]) / n;
+    PrefixSegment g;
+    g.slot = s;
+    g.g = unit / tiles;
+    g.tile = unit % tiles;
+    g.block = (x - list.begin[s]) % n;
+    g.count = min(n - g.block, x1 - x);
+    g.rows = min(TILE_M, rows - g.tile * TILE_M);
+    g.whole = g.block == 0;
+    return g;
+  };
+
+  if (tid == 0) {
+    mbar_init(q_full, 8);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&s_full[s], 1);
+      mbar_init(&p_full[s], 4);
+      mbar_init(&pv_done[s], 1);
+      mbar_init(&wg_meet[s], 4);
+    }
+    mbar_init(all_meet, 8);
+    for (int s = 0; s < 2 * SLOTS; ++s) mbar_init(&full[s], 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_base_slot, TMEM_COLS);
+    tmem_relinquish();
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  const uint32_t tmem_base = *tmem_base_slot;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      bool ok = true;
+      int issued = 0;
+      for (int x = x0; x < x1 && ok;) {
+        const PrefixSegment sg = segment(x);
+        const PrefixBlocks keys(list.lo[sg.slot], list.hi[sg.slot], p.keep_first);
+        for (int j = sg.block; j < sg.block + sg.count && ok; ++j, ++x) {
+          const int key0 = j < keys.kept_blocks ? j * BKV : keys.first + (j - keys.kept_blocks) * BKV;
+          const int row = (sg.slot * p.G + sg.g) * p.Smax + key0;
+#pragma unroll
+          for (int kv = 0; kv < 2; ++kv) {
+            const int n = 2 * (x - x0) + kv, st = n % SLOTS;
+            if (n >= SLOTS) ok = mbar_wait(&empty[st], (uint32_t)(n / SLOTS - 1) & 1u, abort_flag, p.err, ERR_KV_EMPTY);
+            if (!ok) break;
+            uint8_t* dst = ring + st * L::SLOT;
+            if (kv) {
+              mbar_expect_tx(&full[st], L::V_BYTES);
+#pragma unroll
+              for (int kk = 0; kk < BKV / 64; ++kk)
+#pragma unroll
+                for (int jn = 0; jn < VD / 64; ++jn)
+                  tma_load_2d(dst + (kk * (VD / 64) + jn) * 8192, &map_v, &full[st], jn * 64, row + kk * 64);
+            } else {
+              mbar_expect_tx(&full[st], L::K_BYTES);
+#pragma unroll
+              for (int kb = 0; kb < DK / 64; ++kb) tma_load_2d(dst + kb * (BKV * 128), &map_k, &full[st], kb * 64, row);
+            }
+            issued = n + 1;
+          }
+        }
+      }
+      if (!ok || *abort_flag) {
+        // loads in flight target this CTA's shared memory: give them a bounded time to land before the CTA ends
+        for (int n = max(0, issued - SLOTS); n < issued; ++n)
+          for (uint32_t i = 0; i < MBAR_SPIN_LIMIT && !mbar_try_wait(&full[n % SLOTS], (uint32_t)(n / SLOTS) & 1u); ++i) {}
+      }
+    }
+  } else if (warp == 1) {
+    if (elect_one()) {
+      xl_grid_dependency_wait();    // the successor takes whatever came before this kernel as complete
+      xl_grid_launch_dependents();  // TMEM is held: a successor that allocates some on this SM cannot come first
+      auto wait_full = [&](int n) { return mbar_wait(&full[n % SLOTS], (uint32_t)(n / SLOTS) & 1u, abort_flag, p.err, ERR_KV_FULL); };
+      // block `it` of this CTA: warpgroup it & 1, its block it >> 1
+      auto issue_scores = [&](int it) -> bool {
+        const int m = it & 1, st = 2 * it % SLOTS;
+        if (!wait_full(2 * it)) return false;
+        // the buffer still holds P of the warpgroup's previous block until its product has been taken
+        if (it >= 2 && !mbar_wait(&pv_done[m], (uint32_t)((it >> 1) - 1) & 1u, abort_flag, p.err, ERR_PV)) return false;
+        tcgen05_fence_after();
+        issue_score_product<DK>(tmem_base + m * BKV, smem_u32(sQ), smem_u32(ring + st * L::SLOT));
+        tcgen05_commit(&empty[st]);
+        tcgen05_commit(&s_full[m]);
+        return true;
+      };
+      auto issue_values = [&](int it, bool add) -> bool {
+        const int m = it & 1, st = (2 * it + 1) % SLOTS;
+        if (!wait_full(2 * it + 1)) return false;
+        if (!mbar_wait(&p_full[m], (uint32_t)(it >> 1) & 1u, abort_flag, p.err, ERR_P)) return false;
+        tcgen05_fence_after();
+        issue_value_product<VD>(tmem_base + 2 * BKV + m * VD, tmem_base + m * BKV, smem_u32(ring + st * L::SLOT), add);
+        tcgen05_commit(&empty[st]);
+        tcgen05_commit(&pv_done[m]);
+        return true;
+      };
+      bool ok = true, add = false;
+      int it = 0, segments = 0;
+      for (int x = x0; x < x1 && ok; ++segments) {
+        const int count = segment(x).count;
+        if (it) ok = issue_values(it - 1, add);  // the last block of the segment before: its warpgroup ends with it
+        ok = ok && mbar_wait(q_full, (uint32_t)segments & 1u, abort_flag, p.err, ERR_Q);
+        for (int j = 0; j < count && ok; ++j, ++it) {
+          ok = issue_scores(it);
+          if (ok && j) ok = issue_values(it - 1, add);
+          add = j >= 2;  // of this block: the warpgroup has had one of this segment
+        }
+        x += count;
+      }
+      if (ok && it) issue_values(it - 1, add);
+    }
+  } else {
+    const int m = warp < 6 ? 0 : 1;  // warpgroup
+    const int qtr = warp & 3;        // TMEM lane quarter this warp may access
+    const int r = qtr * 32 + lane;   // row inside the tile
+    const uint32_t lane_base = (uint32_t)(qtr * 32) << 16;
+    const uint32_t tmem_s = tmem_base + lane_base + m * BKV;
+    const uint32_t tmem_o = tmem_base + lane_base + 2 * BKV + m * VD;
+    const float c = p.scale * 1.4426950408889634f;
+    xl_grid_dependency_wait();  // the projections
+    bool ok = true;
+    uint32_t met_all = 0, met_wg = 0;
+    for (int x = x0; x < x1 && ok;) {
+      const PrefixSegment sg = segment(x);
+      const PrefixBlocks keys(list.lo[sg.slot], list.hi[sg.slot], p.keep_first);
+      const short* members = list.order + list.offset[sg.slot];
+      ok = warps_meet(all_meet, met_all, abort_flag, p.err);  // both have seen the last scores of the segment before: its queries are no longer read
+      if (!ok) break;
+      load_queries<DK, 16>(sQ, (m * 4 + qtr) * 16, [&](int row) -> const __nv_bfloat16* {
+        if (row >= sg.rows) return nullptr;
+        const int at = sg.tile * TILE_M + row, i = at / R;
+        return p.proj + (long long)members[i] * p.ld + (long long)(sg.g * R + at - i * R) * p.dim;
+      }, p.wq, p.dim, p.eps);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full);
+      const bool row_on = r < sg.rows;
+      const int b = row_on ? members[(sg.tile * TILE_M + r) / R] : 0;
+      const int edge = row_on ? list.edge[b] : 0x7fffffff, lo = row_on ? window_range(p.pos[b], p.window, 0).first : 0;
+      const int warp_edge = __reduce_min_sync(0xffffffffu, edge), warp_first = __reduce_max_sync(0xffffffffu, lo);
+      if (lane == 0) {
+        least_edge[m * 4 + qtr] = warp_edge;
+        last_first[m * 4 + qtr] = warp_first;
+      }
+      ok = warps_meet(&wg_meet[m], met_wg, abort_flag, p.err);
+      int all_edge = least_edge[m * 4], all_first = last_first[m * 4];
+#pragma unroll
+      for (int w = 1; w < 4; ++w) {
+        all_edge = min(all_edge, least_edge[m * 4 + w]);
+        all_first = max(all_first, last_first[m * 4 + w]);
+      }
+      float mx = -INFINITY, l = 0.f;
+      int mine = 0, last = 0;
+      for (int j = sg.block; j < sg.block + sg.count && ok; ++j, ++x) {
+        const int it = x - x0;
+        if ((it & 1) != m) continue;
+        const int key0 = j < keys.kept_blocks ? j * BKV : keys.first + (j - keys.kept_blocks) * BKV;
+        const int end = j < keys.kept_blocks ? keys.kept : keys.end;
+        ok = mbar_wait_warp(&s_full[m], (uint32_t)(it >> 1) & 1u, abort_flag, p.err, ERR_S);
+        if (!ok) break;
+        tcgen05_fence_after();
+        const bool cut = key0 + BKV > end || key0 + BKV > all_edge || (key0 < all_first && key0 + BKV > p.keep_first);
+        if (cut) {  // not every row sees every key: thread r looks at the value of key r
+          const int n = 2 * it + 1;
+          ok = mbar_wait_warp(&full[n % SLOTS], (uint32_t)(n / SLOTS) & 1u, abort_flag, p.err, ERR_KV_FULL);
+          if (!ok) break;
+          uint8_t* tile = ring + n % SLOTS * L::SLOT;
+          bool finite = true;
+#pragma unroll
+          for (int jn = 0; jn < VD / 64; ++jn)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const uint4 v = value_row<VD>(tile, r, jn)[i];
+              const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+              for (int e = 0; e < 4; ++e) finite &= (w[e] & 0x7f80u) != 0x7f80u && (w[e] & 0x7f800000u) != 0x7f800000u;
+            }
+          const bool beyond = key0 + r >= end;  // nobody sees it
+          const unsigned int bits = __ballot_sync(0xffffffffu, !finite && !beyond);
+          if (lane == 0) unknown[m * 4 + qtr] = bits;
+          if (!finite || beyond)
+#pragma unroll
+            for (int jn = 0; jn < VD / 64; ++jn)
+#pragma unroll
+              for (int i = 0; i < 8; ++i) value_row<VD>(tile, r, jn)[i] = make_uint4(0u, 0u, 0u, 0u);
+          fence_proxy_async_smem();
+          ok = warps_meet(&wg_meet[m], met_wg, abort_flag, p.err);
+          if (!ok) break;
+        }
+        float s[BKV];
+        load_scores(tmem_s, s);
+        if (cut) {
+#pragma unroll
+          for (int w = 0; w < BKV / 32; ++w) {
+            const uint32_t not_known = unknown[m * 4 + w];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              const int k = key0 + w * 32 + i;
+              const bool visible = k < end && k < edge && (k >= lo || k < p.keep_first);
+              s[w * 32 + i] = !visible ? -INFINITY : not_known >> i & 1 ? NAN : s[w * 32 + i];
+            }
+          }
+        }
+        const float alpha = weigh(s, mx, l, c);
+        // the scores of a block are only computed after P V of the warpgroup's block before: O is at rest here
+        if (mine && __any_sync(0xffffffffu, alpha != 1.f)) rescale_output<VD>(tmem_o, alpha);
+        store_split_weights<BKV>(tmem_s, s);
+        tmem_st_wait();
+        tcgen05_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[m]);
+        ++mine;
+        last = it >> 1;
+      }
+      // ---- this part's sums ------------------------------------------------------------------------------------------------
+      if (ok && mine) ok = mbar_wait_warp(&pv_done[m], (uint32_t)last & 1u, abort_flag, p.err, ERR_PV);
+      if (!ok) break;
+      const long long at = sg.whole ? ((long long)m * p.G + sg.g) * p.B * R + (long long)list.offset[sg.slot] * R + sg.tile * TILE_M + r
+                                    : ((long long)blockIdx.x * 2 + m) * TILE_M + r;
+      if (row_on) (sg.whole ? a.main_s : a.extra_s)[at] = make_float2(mx * c, l);
+      if (mine) {
+        tcgen05_fence_after();
+        float* o = (sg.whole ? a.main_o : a.extra_o) + at * p.vdim;
+#pragma unroll 1
+        for (int ch = 0; ch < VD / 32; ++ch) {
+          uint32_t raw[32];
+          tmem_ld_32x32b_x32(tmem_o + ch * 32, raw);
+          tmem_ld_wait();
+          if (row_on)
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+              if (ch * 32 + q * 4 < p.vdim)
+                *reinterpret_cast<uint4*>(o + ch * 32 + q * 4) = make_uint4(raw[q * 4], raw[q * 4 + 1], raw[q * 4 + 2], raw[q * 4 + 3]);
+        }
+        tcgen05_fence_before();
+      }
+    }
+  }
+
+  // ---- teardown: every role arrives here, also after an abort --------------------------------------------------------
+  tcgen05_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tcgen05_fence_after();
+    tmem_dealloc(tmem_base, TMEM_COLS);
+  }
+}
+
+// ---- single tokens: each sequence's own keys, and the sum of all parts ----------------------------------------------------------------
+// As window_attn_decode_kernel (attention_window.cu): grid (splits, G * head chunks, B); a CTA takes up to 8 RT query heads of one key / value
+// head and a run of the blocks of keys, each of its 4 warps with a cp.async ring of its own, products on mma.sync. It starts under the
+// prefix kernel's tail: everything but the parts of the shared keys was complete when that kernel let it start. The number of runs
+// goes by the keys that there are: up to 320 one CTA has them all, and no merge of runs.
+constexpr int SD_WARPS = 4;
+constexpr int SD_MAX_SPLITS = 64;
+
+struct SharedDecodeParams {
+  SharedParams p;
+  __nv_bfloat16 *kc, *vc;
+  const float *wk;
+  float* part;             // [units][splits][heads per CTA][vdim], then the same with [2]: maximum, sum
+  unsigned int* counters;  // [units], zero between launches
+  const float *main_o, *extra_o;
+  const float2 *main_s, *extra_s;
+  const PrefixPlan* plan;
+  int stages;
+};
+
+__host__ __device__ constexpr int sd_keys(int kd, int vt) { return 4 * kd + vt <= 16 ? 32 : 16; }
+// bytes of one ring stage of one warp: the keys as KD pieces of 64 B, then the value rows of vdim + 8 elements
+__host__ __device__ constexpr int sd_stage_bytes(int keys, int kd, int vdim) { return keys * kd * 64 + keys * (vdim + 8) * 2; }
+
+// KD: 32-feature steps of a query / key row (dim <= 32 KD); VT: 8-feature tiles of a value row (vdim <= 8 VT)
+template <int KD, int VT, int RT>
+__global__ void __launch_bounds__(SD_WARPS * 32) shared_attn_decode_kernel(const SharedDecodeParams d) {
+  constexpr int KEYS = sd_keys(KD, VT), KT = KEYS / 8;  // keys per block, tiles of eight keys
+  constexpr int HEADS = 8 * RT;
+  const SharedParams& p = d.p;
+  extern __shared__ __align__(16) uint8_t smem[];
+  // normalised queries and their rounding errors; the last row is the new key
+  __shared__ __align__(16) __nv_bfloat16 sq[2][HEADS + 1][KD * 32];
+  __shared__ float sm[SD_WARPS][HEADS], sl[SD_WARPS][HEADS], fw[SD_WARPS][HEADS];
+  __shared__ float2 own[HEADS];  // this CTA's maxima and sums
+  __shared__ unsigned int is_last;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = lane >> 2, j = lane & 3;
+  const int R = p.H / p.G, hchunks = (R + HEADS - 1) / HEADS;
+  const int split = blockIdx.x, g = blockIdx.y / hchunks, b = blockIdx.z;
+  const int h0 = g * R + (blockIdx.y % hchunks) * HEADS;  // first query head of this CTA
+  const int nh = min(HEADS, (g + 1) * R - h0);
+  const int pos = p.pos[b];
+  int lead = b, edge = 0, splits = 0, blocks = 0;
+  WindowRange seen = {0, 0};
+  if (p.count[b] > 0 && window_fits(pos, p.count[b], 1, p.Smax)) {
+    edge = shared_edge(p.prefix, p.pos, b, pos, p.B, lead);
+    seen = window_range(pos, p.window, p.keep_first);
+    seen.first = max(seen.first, edge);
+    seen.kept = max(seen.kept, edge);  // kept tokens of its own: [edge, kept)
+    blocks = (seen.kept - edge + KEYS - 1) / KEYS + (pos - seen.first) / KEYS + 1;
+    splits = blocks * KEYS <= 320 ? 1 : min((int)gridDim.x, (blocks * KEYS + 63) / 64);
+  }
+  if (split >= splits) {
+    xl_grid_dependency_wait();  // no kernel of a chain ends before its predecessor
+    return;
+  }
+  const int kept_blocks = (seen.kept - edge + KEYS - 1) / KEYS;
+  const int blk0 = (int)((long long)split * blocks / splits), blk1 = (int)((long long)(split + 1) * blocks / splits);
+  const __nv_bfloat16* row = p.proj + (long long)b * p.ld;
+  const __nv_bfloat16* kb = d.kc + ((long long)b * p.G + g) * p.Smax * p.dim;
+  const __nv_bfloat16* vb = d.vc + ((long long)b * p.G + g) * p.Smax * p.vdim;
+  auto first_key = [&](int blk) { return blk < kept_blocks ? edge + blk * KEYS : seen.first + (blk - kept_blocks) * KEYS; };
+  // visible keys of a block lie below this; so do those that are in the cache already, except the new one
+  auto end_key = [&](int blk) { return blk < kept_blocks ? seen.kept : pos + 1; };
+
+  // ---- the ring of key / value blocks -------------------------------------------------------------------------------------
+  const int stage_bytes = sd_stage_bytes(KEYS, KD, p.vdim), vld = p.vdim + 8;
+  uint8_t* ring = smem + (long long)warp * d.stages * stage_bytes;
+  const int mine = (blk1 - blk0 - warp + SD_WARPS - 1) / SD_WARPS;  // this warp's blocks: blk0 + warp, + SD_WARPS, ...
+  constexpr int V_ROWS = 32 / VT, V_PASSES = KEYS / V_ROWS;  // value rows that a warp copies at a time, one piece per lane
+  const int v_row = lane / VT, v_col = (lane % VT) * 8;
+  const bool v_on = v_col < p.vdim;
+  auto prefetch = [&](int n) {
+    if (n < mine) {
+      uint8_t* st = ring + (n % d.stages) * stage_bytes;
+      const int blk = blk0 + warp + n * SD_WARPS, key0 = first_key(blk), end = min(end_key(blk), pos);
+      const bool full = key0 + KEYS <= end;  // else rows from `end` on are zero-filled
+#pragma unroll
+      for (int t = 0; t < KT; ++t) {
+        const bool row_on = full || key0 + t * 8 + quad < end;
+        const __nv_bfloat16* src = kb + (row_on ? (long long)(key0 + t * 8 + quad) * p.dim + j * 8 : 0);
+#pragma unroll
+        for (int i = 0; i < KD; ++i) {
+          const bool on = row_on && i * 32 + j * 8 < p.dim;
+          dd_cp16_zfill(st + ((t * KD + i) * 32 + lane) * 16, on ? src + i * 32 : kb, on);
+        }
+      }
+      if (v_on) {
+        uint8_t* dst = st + KEYS * KD * 64 + (v_row * vld + v_col) * 2;
+        const __nv_bfloat16* src = vb + (long long)(key0 + v_row) * p.vdim + v_col;
+#pragma unroll
+        for (int i = 0; i < V_PASSES; ++i) {
+          const bool on = full || key0 + v_row + i * V_ROWS < end;
+          dd_cp16_zfill(dst + i * V_ROWS * vld * 2, on ? src + (long long)i * V_ROWS * p.vdim : vb, on);
+        }
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");  // possibly empty: keeps the group count per block fixed
+  };
+  for (int n = 0; n < d.stages - 1; ++n) prefetch(n);
+  // ---- normalised queries and new key to shared memory; the CTAs with the last keys append (the same data each) ---------------
+  const bool appends = split == splits - 1;
+  const __nv_bfloat16* v_src = row + (long long)(p.H + p.G) * p.dim + (long long)g * p.vdim;
+  uint4 v_new = make_uint4(0, 0, 0, 0);  // lane's piece of the new value, in every warp
+  {
+    constexpr int QUERIES = HEADS / SD_WARPS;  // of a warp
+    uint32_t raw[QUERIES + 1][2];              // dim <= 128; the last one is the new key
+#pragma unroll
+    for (int i = 0; i <= QUERIES; ++i) {
+      const int r = warp + i * SD_WARPS;
+      const __nv_bfloat16* src = row + (long long)(i < QUERIES ? h0 + r : p.H + g) * p.dim;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int e = 2 * lane + 64 * u;
+        raw[i][u] = (r < nh || i == QUERIES) && e < p.dim ? *reinterpret_cast<const uint32_t*>(src + e) : 0u;
+      }
+    }
+    float w[2][4];  // query and key factors
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int e = 2 * lane + 64 * u;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        w[0][2 * u + c] = e < p.dim ? p.wq[e + c] : 0.f;
+        w[1][2 * u + c] = e < p.dim ? d.wk[e + c] : 0.f;
+      }
+    }
+    if (appends && lane < p.vdim / 8) v_new = *reinterpret_cast<const uint4*>(v_src + lane * 8);
+    float sum[QUERIES];
+    double key_sum = 0.0;  // the key's norm is taken in 64 bits, as in every kernel, so that all come to the same number
+#pragma unroll
+    for (int i = 0; i < QUERIES; ++i) {
+      sum[i] = 0.f;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const float y0 = dd_lo(raw[i][u]), y1 = dd_hi(raw[i][u]);
+        sum[i] += y0 * y0 + y1 * y1;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const double y0 = dd_lo(raw[QUERIES][u]), y1 = dd_hi(raw[QUERIES][u]);
+      key_sum += y0 * y0 + y1 * y1;
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {  // the rows' sums side by side
+#pragma unroll
+      for (int i = 0; i < QUERIES; ++i) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], o);
+      key_sum += __shfl_xor_sync(0xffffffffu, key_sum, o);
+    }
+#pragma unroll
+    for (int i = 0; i < QUERIES; ++i) {
+      const int r = warp + i * SD_WARPS;
+      const float f = 1.f / sqrtf(sum[i] / p.dim + p.eps);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int e = 2 * lane + 64 * u;
+        if (e < KD * 32) {  // rows and features that are not in use: zero
+          const float y0 = dd_lo(raw[i][u]) * f * w[0][2 * u], y1 = dd_hi(raw[i][u]) * f * w[0][2 * u + 1];
+          const uint32_t hi = dd_pack(y0, y1);
+          *reinterpret_cast<uint32_t*>(&sq[0][r][e]) = hi;
+          *reinterpret_cast<uint32_t*>(&sq[1][r][e]) = dd_pack(y0 - dd_lo(hi), y1 - dd_hi(hi));
+        }
+      }
+    }
+    if (warp == 0) {
+      const double f = 1.0 / sqrt(key_sum / p.dim + (double)p.eps);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int e = 2 * lane + 64 * u;
+        if (e < KD * 32) {
+          const uint32_t y = dd_pack((float)((double)dd_lo(raw[QUERIES][u]) * f * (double)w[1][2 * u]),
+                                     (float)((double)dd_hi(raw[QUERIES][u]) * f * (double)w[1][2 * u + 1]));
+          *reinterpret_cast<uint32_t*>(&sq[0][HEADS][e]) = y;
+          if (appends && e < p.dim) *reinterpret_cast<uint32_t*>(d.kc + (((long long)b * p.G + g) * p.Smax + pos) * p.dim + e) = y;
+        }
+      }
+    }
+    if (appends && threadIdx.x < p.vdim / 8)
+      *reinterpret_cast<uint4*>(d.vc + (((long long)b * p.G + g) * p.Smax + pos) * p.vdim + threadIdx.x * 8) = v_new;
+  }
+  __syncthreads();
+  uint4 q[2][RT][KD];  // rows quad (and quad + 8)
+#pragma unroll
+  for (int half = 0; half < 2; ++half)
+#pragma unroll
+    for (int m = 0; m < RT; ++m)
+#pragma unroll
+      for (int i = 0; i < KD; ++i) q[half][m][i] = *reinterpret_cast<const uint4*>(&sq[half][quad + 8 * m][i * 32 + j * 8]);
+  float o[VT][2 * RT];
+#pragma unroll
+  for (int t = 0; t < VT; ++t)
+#pragma unroll
+    for (int e = 0; e < 2 * RT; ++e) o[t][e] = 0.f;
+  float mx[RT], l[RT];
+#pragma unroll
+  for (int m = 0; m < RT; ++m) {
+    mx[m] = -INFINITY;
+    l[m] = 0.f;
+  }
+  const float sc = p.scale * 1.4426950408889634f;
+  for (int n = 0; n < mine; ++n) {
+    prefetch(n + d.stages - 1);
+    if (d.stages == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
+    else if (d.stages == 3) asm volatile("cp.async.wait_group 2;" ::: "memory");
+    else asm volatile("cp.async.wait_group 3;" ::: "memory");
+    __syncwarp();
+    uint8_t* st = ring + (n % d.stages) * stage_bytes;
+    const int blk = blk0 + warp + n * SD_WARPS, key0 = first_key(blk), end = end_key(blk);
+    if (blk == blocks - 1) {  // the new key and value take their place
+      const int k = pos - key0;
+      for (int i = lane; i < KD * 4; i += 32)
+        *reinterpret_cast<uint4*>(st + (((k >> 3) * KD + (i >> 2)) * 32 + (k & 7) * 4 + (i & 3)) * 16) =
+            *reinterpret_cast<const uint4*>(&sq[0][HEADS][i * 8]);
+      if (lane < p.vdim / 8) *reinterpret_cast<uint4*>(st + KEYS * KD * 64 + (k * vld + lane * 8) * 2) = v_new;
+      __syncwarp();
+    }
+    float s[KT][2 * RT];
+#pragma unroll
+    for (int t = 0; t < KT; ++t) {
+#pragma unroll
+      for (int e = 0; e < 2 * RT; ++e) s[t][e] = 0.f;
+#pragma unroll
+      for (int i = 0; i < KD; ++i) {
+        const uint4 k = *reinterpret_cast<const uint4*>(st + ((t * KD + i) * 32 + lane) * 16);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const uint4 &lo = q[half][0][i], &hi = q[half][RT - 1][i];
+          wd_mma(s[t], make_uint2(lo.x, lo.y), make_uint2(hi.x, hi.y), k.x, k.y);
+          wd_mma(s[t], make_uint2(lo.z, lo.w), make_uint2(hi.z, hi.w), k.z, k.w);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 2 * RT; ++e)
+        s[t][e] = key0 + t * 8 + 2 * j + (e & 1) < end ? s[t][e] * sc : -INFINITY;
+    }
+    float alpha[RT];
+    uint2 ph[KT / 2][RT], pl[KT / 2][RT];  // weights as operands of the second product, and their rounding errors
+#pragma unroll
+    for (int m = 0; m < RT; ++m) {
+      float v = -INFINITY;
+#pragma unroll
+      for (int t = 0; t < KT; ++t) v = fmaxf(v, fmaxf(s[t][2 * m], s[t][2 * m + 1]));
+      v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
+      v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+      const float m_new = fmaxf(mx[m], v), use = m_new == -INFINITY ? 0.f : m_new;  // (no score is a number: the sum is none either)
+      alpha[m] = exp2f(mx[m] - use);
+      mx[m] = m_new;
+      float sum = 0.f;
+#pragma unroll
+      for (int t = 0; t < KT; ++t) {
+        const float x = exp2f(s[t][2 * m] - use), y = exp2f(s[t][2 * m + 1] - use);
+        sum += x + y;
+        const uint32_t hi = dd_pack(x, y), lo = dd_pack(x - dd_lo(hi), y - dd_hi(hi));
+        uint2 &h = ph[t / 2][m], &r = pl[t / 2][m];
+        (t % 2 ? h.y : h.x) = hi;
+        (t % 2 ? r.y : r.x) = lo;
+      }
+      l[m] = l[m] * alpha[m] + sum;  // this lane's share of the row sum
+    }
+    bool moved = false;
+#pragma unroll
+    for (int m = 0; m < RT; ++m) moved |= alpha[m] != 1.f;
+    if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+      for (int t = 0; t < VT; ++t)
+#pragma unroll
+        for (int e = 0; e < 2 * RT; ++e) o[t][e] *= alpha[e >> 1];
+    }
+    const uint32_t sv = (uint32_t)__cvta_generic_to_shared(st + KEYS * KD * 64);
+    const uint32_t vaddr = sv + (((lane & 7) + ((lane >> 3) & 1) * 8) * vld + (lane >> 4) * 8) * 2;
+#pragma unroll
+    for (int t = 0; t < VT; t += 2) {
+      if (t * 8 < p.vdim) {
+#pragma unroll
+        for (int k = 0; k < KT / 2; ++k) {
+          uint32_t v0, v1, v2, v3;  // 16 keys of value tiles t (v0, v1) and t + 1 (v2, v3)
+          asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                       : "=r"(v0), "=r"(v1), "=r"(v2), "=r"(v3)
+                       : "r"(vaddr + k * 32 * vld + t * 16));
+          wd_mma(o[t], ph[k][0], ph[k][RT - 1], v0, v1);
+          wd_mma(o[t + 1], ph[k][0], ph[k][RT - 1], v2, v3);
+          wd_mma(o[t], pl[k][0], pl[k][RT - 1], v0, v1);
+          wd_mma(o[t + 1], pl[k][0], pl[k][RT - 1], v2, v3);
+        }
+      }
+    }
+    __syncwarp();  // every lane has read the stage before it is refilled
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  // From here on one warp per head; features c of a lane: (lane + 32 u) * 4 .. The gates are asked for before they are needed.
+  constexpr int CH = (VT * 8 + 127) / 128, MINE = HEADS / SD_WARPS;
+  uint2 gates[MINE][CH];
+  {
+    const __nv_bfloat16* gate = row + (long long)(p.H + p.G) * p.dim + (long long)p.G * p.vdim + (long long)h0 * p.vdim;
+#pragma unroll
+    for (int i = 0; i < MINE; ++i)
+#pragma unroll
+      for (int u = 0; u < CH; ++u) {
+        const int r = warp + i * SD_WARPS, c = (lane + 32 * u) * 4;
+        gates[i][u] = p.gated && r < nh && c < p.vdim ? *reinterpret_cast<const uint2*>(gate + (long long)r * p.vdim + c)
+                                                      : make_uint2(0u, 0u);
+      }
+  }
+#pragma unroll
+  for (int m = 0; m < RT; ++m) {
+    l[m] += __shfl_xor_sync(0xffffffffu, l[m], 1);
+    l[m] += __shfl_xor_sync(0xffffffffu, l[m], 2);
+    if (j == 0) {
+      sm[warp][quad + 8 * m] = mx[m];
+      sl[warp][quad + 8 * m] = l[m];
+    }
+  }
+  __syncthreads();  // all rings are idle: their memory holds the warps' outputs from here on
+  float* so = reinterpret_cast<float*>(smem);  // [SD_WARPS][HEADS][vdim + 8]
+  const int old = p.vdim + 8;                  // the padding keeps the quads' stores in different banks
+#pragma unroll
+  for (int t = 0; t < VT; ++t) {
+    if (t * 8 < p.vdim) {
+#pragma unroll
+      for (int m = 0; m < RT; ++m)
+        *reinterpret_cast<float2*>(so + (warp * HEADS + quad + 8 * m) * old + t * 8 + 2 * j) =
+            make_float2(o[t][2 * m], o[t][2 * m + 1]);
+    }
+  }
+  // ---- merge of the warps: their weights, and the sums of the weights --------------------------------------------------------
+  const long long units = (long long)gridDim.z * gridDim.y, unit = (long long)b * gridDim.y + blockIdx.y;
+  float2* stats = reinterpret_cast<float2*>(d.part + units * gridDim.x * HEADS * p.vdim) + unit * gridDim.x * HEADS;
+  float* slices = d.part + unit * gridDim.x * HEADS * p.vdim;
+  if (threadIdx.x < HEADS) {
+    const int r = threadIdx.x;
+    float m = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < SD_WARPS; ++w) m = fmaxf(m, sm[w][r]);
+    float ll = 0.f;
+#pragma unroll
+    for (int w = 0; w < SD_WARPS; ++w) {
+      const float f = sm[w][r] == -INFINITY ? 0.f : exp2f(sm[w][r] - m);
+      fw[w][r] = f;
+      ll += sl[w][r] * f;  // (a sum that is not a number stays none)
+    }
+    own[r] = make_float2(m, ll);
+    if (splits > 1) __stcg(stats + split * HEADS + r, make_float2(m, ll));
+  }
+  __syncthreads();
+  auto merged = [&](int r, int c) {  // head r, features c .. c + 3, over this CTA's warps
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < SD_WARPS; ++w) {
+      const float f = fw[w][r];
+      const float4 x = *reinterpret_cast<const float4*>(so + (w * HEADS + r) * old + c);
+      if (f != 0.f) a = make_float4(a.x + x.x * f, a.y + x.y * f, a.z + x.z * f, a.w + x.w * f);
+    }
+    return a;
+  };
+  if (splits > 1) {
+    for (int r = warp; r < nh; r += SD_WARPS)
+#pragma unroll
+      for (int u = 0; u < CH; ++u) {
+        const int c = (lane + 32 * u) * 4;
+        if (c < p.vdim) __stcg(reinterpret_cast<float4*>(slices + ((long long)split * HEADS + r) * p.vdim + c), merged(r, c));
+      }
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) is_last = atomicAdd(d.counters + unit, 1u) == (unsigned int)splits - 1;
+    __syncthreads();
+    if (!is_last) {
+      xl_grid_dependency_wait();
+      return;
+    }
+    __threadfence();
+    if (threadIdx.x == 0) d.counters[unit] = 0;
+  }
+  // ---- all parts: this sequence's own, then those of the shared keys -------------------------------------------------------------
+  xl_grid_dependency_wait();  // the parts of the prefix kernel
+  xl_grid_launch_dependents();
+  const int4* at = reinterpret_cast<const int4*>(d.plan + b);
+  const int4 pa = __ldcg(at), pb = __ldcg(at + 1);
+  const int n_blocks = pa.y;
+  const XlRanges ranges{n_blocks ? pb.y / pb.z : 1, n_blocks ? pb.y % pb.z : 0};
+  const float sink = p.sink * 1.4426950408889634f;
+#pragma unroll
+  for (int i = 0; i < MINE; ++i) {
+    const int r = warp + i * SD_WARPS;
+    if (r >= nh) break;
+    const int idx = pa.w + h0 - g * R + r;  // row in the group
+    int c0 = 0, parts = 0;
+    if (n_blocks) {
+      const int x = pa.x + (g * pa.z + idx / TILE_M) * n_blocks;
+      c0 = ranges.owner(x);
+      parts = 2 * (ranges.owner(x + n_blocks - 1) - c0 + 1);
+    }
+    const int slices_n = splits > 1 ? splits : 0, all = parts + slices_n;
+    auto stat = [&](int k) {
+      if (k < slices_n) return __ldcg(stats + k * HEADS + r);
+      const int q = k - slices_n, m = q & 1, c = q >> 1;
+      return c == 0 ? __ldcg(d.main_s + ((long long)m * p.G + g) * p.B * R + pb.x + idx)
+                    : __ldcg(d.extra_s + ((long long)(c0 + c) * 2 + m) * TILE_M + idx % TILE_M);
+    };
+    auto sums = [&](int k) -> const float* {
+      if (k < slices_n) return slices + ((long long)k * HEADS + r) * p.vdim;
+      const int q = k - slices_n, m = q & 1, c = q >> 1;
+      return c == 0 ? d.main_o + (((long long)m * p.G + g) * p.B * R + pb.x + idx) * p.vdim
+                    : d.extra_o + (((long long)(c0 + c) * 2 + m) * TILE_M + idx % TILE_M) * p.vdim;
+    };
+    float m = fmaxf(sink, splits > 1 ? -INFINITY : own[r].x);
+    for (int k = lane; k < all; k += 32) m = fmaxf(m, stat(k).x);
+    m = xl_warp_max(m);
+    float4 acc[CH];
+    float total = sink == -INFINITY ? 0.f : exp2f(sink - m);
+#pragma unroll
+    for (int u = 0; u < CH; ++u) acc[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (splits == 1) {
+      const float f = own[r].x == -INFINITY ? 0.f : exp2f(own[r].x - m);
+      total += f * own[r].y;
+#pragma unroll
+      for (int u = 0; u < CH; ++u) {
+        const int c = (lane + 32 * u) * 4;
+        if (c < p.vdim) {
+          const float4 x = merged(r, c);
+          acc[u] = make_float4(x.x * f, x.y * f, x.z * f, x.w * f);
+        }
+      }
+    }
+    for (int k0 = 0; k0 < all; k0 += 32) {
+      float f = 0.f, lk = 0.f;
+      if (k0 + lane < all) {
+        const float2 st = stat(k0 + lane);
+        f = st.x == -INFINITY ? 0.f : exp2f(st.x - m);
+        lk = f * st.y;
+      }
+      total += xl_warp_sum(lk);
+      const int n = min(32, all - k0);
+#pragma unroll 4
+      for (int k = 0; k < n; ++k) {
+        const float fk = __shfl_sync(0xffffffffu, f, k);
+        if (fk == 0.f) continue;
+        const float* src = sums(k0 + k);
+#pragma unroll
+        for (int u = 0; u < CH; ++u) {
+          const int c = (lane + 32 * u) * 4;
+          if (c < p.vdim) {
+            const float4 x = __ldcg(reinterpret_cast<const float4*>(src + c));
+            acc[u] = make_float4(acc[u].x + x.x * fk, acc[u].y + x.y * fk, acc[u].z + x.z * fk, acc[u].w + x.w * fk);
+          }
+        }
+      }
+    }
+    __nv_bfloat16* out = p.out + (long long)b * p.ldo + (long long)(h0 + r) * p.vdim;
+#pragma unroll
+    for (int u = 0; u < CH; ++u) {
+      const int c = (lane + 32 * u) * 4;
+      if (c >= p.vdim) continue;
+      float v[4] = {acc[u].x / total, acc[u].y / total, acc[u].z / total, acc[u].w / total};
+      if (p.gated) {
+        const uint2 gt = gates[i][u];
+        v[0] *= 1.f / (1.f + expf(-dd_lo(gt.x)));
+        v[1] *= 1.f / (1.f + expf(-dd_hi(gt.x)));
+        v[2] *= 1.f / (1.f + expf(-dd_lo(gt.y)));
+        v[3] *= 1.f / (1.f + expf(-dd_hi(gt.y)));
+      }
+      dd_store4(out + c, v[0], v[1], v[2], v[3], ((uintptr_t)out & 3) == 0);
+    }
+  }
+}
+
+constexpr int SD_RING_LIMIT = 104 * 1024;  // two CTAs per SM
+
+template <int KD, int VT, int RT> int launch_decode_rows(SharedDecodeParams d, int splits, cudaStream_t s) {
+  const SharedParams& p = d.p;
+  const int stage = sd_stage_bytes(sd_keys(KD, VT), KD, p.vdim) * SD_WARPS;
+  d.stages = 4 * stage <= SD_RING_LIMIT ? 4 : (3 * stage <= SD_RING_LIMIT ? 3 : 2);
+  int bytes = d.stages * stage;
+  const int merge = SD_WARPS * 8 * RT * (p.vdim + 8) * 4;
+  if (bytes < merge) bytes = merge;
+  static XlPerDevice smem;
+  XL_TRY(xl_allow_smem(shared_attn_decode_kernel<KD, VT, RT>, bytes, smem));
+  const int hchunks = (p.H / p.G + 8 * RT - 1) / (8 * RT);
+  const cudaError_t e = xl_launch_overlapped(shared_attn_decode_kernel<KD, VT, RT>, dim3(splits, p.G * hchunks, p.B), dim3(SD_WARPS * 32),
+                                             (size_t)bytes, s, d);
+  return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
+}
+
+template <int KD, int VT> int launch_decode(const SharedDecodeParams& d, int splits, cudaStream_t s) {
+  return d.p.H / d.p.G <= 8 ? launch_decode_rows<KD, VT, 1>(d, splits, s) : launch_decode_rows<KD, VT, 2>(d, splits, s);
+}
+
+template <int DK, int VD> int launch_prefix(const PrefixParams& a, const void* kc, const void* vc, int ctas, cudaStream_t s) {
+  using L = PrefixSmem<DK, VD>;
+  const SharedParams& p = a.p;
+  CUtensorMap mk, mv;
+  int r = make_map_bf16(&mk, kc, (long long)p.B * p.G * p.Smax, p.dim, p.dim, BKV);
+  if (r) return r;
+  r = make_map_bf16(&mv, vc, (long long)p.B * p.G * p.Smax, p.vdim, p.vdim, 64);
+  if (r) return r;
+  const int bytes = L::total(p.B);
+  static XlPerDevice smem;
+  XL_TRY(xl_allow_smem(shared_attn_prefix_kernel<DK, VD>, bytes, smem));
+  const cudaError_t e = xl_launch_overlapped(shared_attn_prefix_kernel<DK, VD>, dim3(ctas), dim3(SA_THREADS), (size_t)bytes, s, mk, mv, a);
+  return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
+}
+
 // whether the tensor-core kernels take such operands
 bool tensor_sizes(const void* proj, long long ld, const void* kc, const void* vc, const void* out, long long ldo, int B, int T, int H, int G, int dim,
                   int vdim, int Smax, int gated) {
@@ -535,4 +1484,50 @@ XL_API int xl_shared_attn_portion(const void* proj, long long ld, const float* w
   p.window = window; p.keep_first = keep_first; p.gated = gated; p.scale = scale; p.sink = sink; p.eps = eps; p.err = err;
   if (dim <= 64) return vdim <= 64 ? launch_portion<64, 64>(kc, vc, p, s) : launch_portion<64, 128>(kc, vc, p, s);
   return vdim <= 64 ? launch_portion<128, 64>(kc, vc, p, s) : launch_portion<128, 128>(kc, vc, p, s);
+}
+
+// floats of scratch memory for xl_shared_attn_decode: parts of the shared keys by `ctas` CTAs, and of each sequence's own in `splits` runs
+XL_API long long xl_shared_attn_decode_scratch(int B, int H, int G, int vdim, int ctas, int splits) {
+  const long long R = H / G, heads = R <= 8 ? 8 : 16, units = (long long)B * G * ((R + heads - 1) / heads);
+  return B * 8LL + (2LL * B * H + ctas * 2LL * TILE_M) * (vdim + 2) + (splits > 1 ? units * splits * heads * (vdim + 2) : 0);
+}
+
+// One token per sequence (rows of proj = sequences), bf16, in two launches. Sizes and alignment as for portions, at most 1024 sequences. Queries and
+// keys are normalised and keys and values appended here. ctas: CTAs for the shared keys (SMs of the device); splits: runs of a sequence's own keys, at
+// most 64. scratch: xl_shared_attn_decode_scratch floats, 16-byte aligned; counters: B * G * ceil(H/G/8) zero-initialised words (left zeroed).
+// read_ahead: positions, counts, leads and caches were complete before the previous launch of the stream.
+XL_API int xl_shared_attn_decode(const void* proj, long long ld, const float* wq, const float* wk, void* kc, void* vc, void* out, long long ldo,
+                                 const int* pos, const int* count, const int* lead, const int* shared, int B, int H, int G, int dim, int vdim,
+                                 int Smax, int window, int keep_first, int gated, float scale, float sink, float eps, int ctas, int splits,
+                                 float* scratch, unsigned int* counters, int read_ahead, int* err, cudaStream_t s) {
+  if (B < 1 || B > 1024 || G < 1 || H < 1 || H % G || H > 4096 || Smax < 1 || window < 0 || keep_first < 0 || !(scale > 0.f) || !lead || !shared ||
+      !wq || !wk || ctas < 1 || ctas > 4096 || splits < 1 || splits > SD_MAX_SPLITS || !scratch || ((uintptr_t)scratch & 15) || !counters)
+    return -1;
+  if (!tensor_sizes(proj, ld, kc, vc, out, ldo, B, 1, H, G, dim, vdim, Smax, gated)) return -1;
+  SharedParams p = {};
+  p.proj = (const __nv_bfloat16*)proj; p.ld = ld; p.wq = wq; p.pos = pos; p.count = count; p.prefix = {lead, shared};
+  p.out = (__nv_bfloat16*)out; p.ldo = ldo; p.B = B; p.T = 1; p.H = H; p.G = G; p.dim = dim; p.vdim = vdim; p.Smax = Smax;
+  p.window = window; p.keep_first = keep_first; p.gated = gated; p.scale = scale; p.sink = sink; p.eps = eps; p.err = err;
+  PrefixParams a = {};
+  a.p = p;
+  a.plan = (PrefixPlan*)scratch;
+  a.main_o = scratch + 8LL * B;
+  a.extra_o = a.main_o + 2LL * B * H * vdim;
+  a.main_s = (float2*)(a.extra_o + 2LL * ctas * TILE_M * vdim);
+  a.extra_s = a.main_s + 2LL * B * H;
+  a.read_ahead = read_ahead;
+  SharedDecodeParams d = {};
+  d.p = p; d.kc = (__nv_bfloat16*)kc; d.vc = (__nv_bfloat16*)vc; d.wk = wk;
+  d.main_o = a.main_o; d.extra_o = a.extra_o; d.main_s = a.main_s; d.extra_s = a.extra_s; d.plan = a.plan;
+  d.part = (float*)(a.extra_s + 2LL * ctas * TILE_M);
+  d.counters = counters;
+  int r;
+  if (dim <= 64) r = vdim <= 64 ? launch_prefix<64, 64>(a, kc, vc, ctas, s) : launch_prefix<64, 128>(a, kc, vc, ctas, s);
+  else r = vdim <= 64 ? launch_prefix<128, 64>(a, kc, vc, ctas, s) : launch_prefix<128, 128>(a, kc, vc, ctas, s);
+  if (r) return r;
+#define XL_SD(KD) return vdim <= 64 ? launch_decode<KD, 8>(d, splits, s) : launch_decode<KD, 16>(d, splits, s);
+  if (dim <= 32) { XL_SD(1) }
+  if (dim <= 64) { XL_SD(2) }
+  XL_SD(4)
+#undef XL_SD
 }

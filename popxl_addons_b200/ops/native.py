@@ -364,7 +364,8 @@ def check_gemm_errors():
                      103: "attention over shared prefixes: key / value stage was never released",
                      104: "attention over shared prefixes: scores never completed",
                      105: "attention over shared prefixes: weights never arrived",
-                     106: "attention over shared prefixes: output accumulation never completed"}
+                     106: "attention over shared prefixes: output accumulation never completed",
+                     107: "attention over shared prefixes: warps never met"}
             raise RuntimeError(f"tcgen05 GEMM on cuda:{idx} gave up waiting: {names.get(code, code)}")
 
 
