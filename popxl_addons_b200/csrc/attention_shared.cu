@@ -67,8 +67,8 @@ __global__ void __launch_bounds__(256)
 // tiles, which take turns on the tensor cores while the other one's softmax runs:
 //   warp 0       TMA: key and value tiles in turn through one ring
 //   warp 1       MMA: S_m = Q_m K^T into TMEM (both halves of the queries), then O_m += P_m V
-//   warps 2..5   tile 0, warps 6..9 tile 1: norms of the queries, from the projections straight to shared memory; then the softmax, one thread
-//                per row, running maximum and sum in fp32, lazy rescaling of O_m in TMEM
+//   warps 4..7   tile 0, warps 8..11 tile 1: norms of the queries, from the projections straight to shared memory; then the softmax, one thread
+//                per row, running maximum and sum in fp32, lazy rescaling of O_m in TMEM (warps 2, 3: none)
 // P replaces S in TMEM as two bf16 numbers per weight. Keys beyond a range are masked in the scores, and their values are zeroed in shared
 // memory: what lies there belongs to others, and a weight of zero times anything that is not finite would reach the sum.
 //
@@ -77,7 +77,13 @@ __global__ void __launch_bounds__(256)
 constexpr int TILE_M = 128;
 constexpr int BKV = 128;
 constexpr int UMMA_K = 16;
-constexpr int SA_THREADS = 64 + 2 * 128;
+constexpr int SA_THREADS = 128 + 2 * 128;
+// registers of a thread: of the first warpgroup, which only issues, and of the two that hold a row of scores each (together what the
+// launch gives, 384 x 168: with 168 each the softmax spilled, and a block took twice as long)
+constexpr int REGS_CONTROL = 72, REGS_SOFTMAX = 216;
+static_assert(REGS_CONTROL + 2 * REGS_SOFTMAX <= 3 * 168, "more than the launch gives would never be granted");
+template <int N> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 constexpr uint32_t TMEM_COLS = 512;
 
 enum { ERR_Q = 101, ERR_KV_FULL = 102, ERR_KV_EMPTY = 103, ERR_S = 104, ERR_P = 105, ERR_PV = 106, ERR_MEET = 107 };
@@ -105,19 +111,19 @@ template <int DK, int VD> struct SharedTiles {
   static constexpr int SLOT = K_BYTES > V_BYTES ? K_BYTES : V_BYTES;
 };
 
-// COUNT rows of a tile, normalised by one warp, to shared memory as two K-major operands of 128-byte swizzle. `row(r)`: where the projections
-// have the head of row r of the tile, or null.
-template <int DK, int COUNT, typename F>
-__device__ __forceinline__ void load_queries(uint8_t* tile, int first_row, const F& row, const float* wq, int dim, float eps) {
+// Rows first, first + step, ... below `end` (LANES lanes each, as many at a time as a warp has lanes for) of a tile, normalised, to shared memory as
+// two K-major operands of 128-byte swizzle. `row(r)`: where the projections have the head of row r of the tile, or null.
+template <int DK, int UNROLL, typename F>
+__device__ __forceinline__ void load_queries(uint8_t* tile, int first, int step, int end, const F& row, const float* wq, int dim, float eps) {
   constexpr int LANES = DK / 8, ROWS = 32 / LANES;  // lanes of a row, rows at a time
   const int lane = threadIdx.x & 31, chunk = lane % LANES;
   const bool on = chunk * 8 < dim;
   float w[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) w[e] = on ? wq[chunk * 8 + e] : 0.f;
-#pragma unroll 4
-  for (int i = 0; i < COUNT; i += ROWS) {
-    const int r = first_row + i + lane / LANES;
+#pragma unroll UNROLL
+  for (int i = first * ROWS; i < end; i += step * ROWS) {
+    const int r = i + lane / LANES;
     const __nv_bfloat16* src = row(r);
     float x[8], sq = 0.f;
 #pragma unroll
@@ -144,42 +150,73 @@ __device__ __forceinline__ void load_queries(uint8_t* tile, int first_row, const
   }
 }
 
+// Descriptors of a product's steps differ by whole 16 bytes of address, which stay inside the address field. The first one is hidden from the
+// compiler, which would keep those of all steps in registers across the loop over blocks.
+__device__ __forceinline__ uint64_t first_desc(uint32_t addr, uint32_t lbo_bytes) {
+  uint64_t d = make_smem_desc(addr, lbo_bytes);
+  asm volatile("" : "+l"(d));
+  return d;
+}
+
 // S_m = Q K^T, both halves of the queries
 template <int DK> __device__ __forceinline__ void issue_score_product(uint32_t tmem_s, uint32_t q_addr, uint32_t k_addr) {
   // bf16 operands, fp32 accumulator, both K-major, N = BKV
   constexpr uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BKV >> 3) << 17) | ((uint32_t)(TILE_M >> 4) << 24);
+  const uint64_t dq = first_desc(q_addr, 16), dk = first_desc(k_addr, 16);
 #pragma unroll
   for (int half = 0; half < 2; ++half)
 #pragma unroll
     for (int kb = 0; kb < DK / 64; ++kb)
 #pragma unroll
       for (int k = 0; k < 64 / UMMA_K; ++k)
-        tcgen05_mma_f16(tmem_s, make_smem_desc(q_addr + half * (TILE_M * DK * 2) + kb * (TILE_M * 128) + k * (UMMA_K * 2), 16),
-                        make_smem_desc(k_addr + kb * (BKV * 128) + k * (UMMA_K * 2), 16), idesc, (half | kb | k) ? 1u : 0u);
+        tcgen05_mma_f16(tmem_s, dq + ((half * (TILE_M * DK * 2) + kb * (TILE_M * 128) + k * (UMMA_K * 2)) >> 4),
+                        dk + ((kb * (BKV * 128) + k * (UMMA_K * 2)) >> 4), idesc, (half | kb | k) ? 1u : 0u);
 }
 
 // O_m (+)= P V, both halves of the weights
 template <int VD> __device__ __forceinline__ void issue_value_product(uint32_t tmem_o, uint32_t tmem_p, uint32_t v_addr, bool add) {
   // A (P) from TMEM, B (V) MN-major (bit 16), N = VD
   constexpr uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(VD >> 3) << 17) | ((uint32_t)(TILE_M >> 4) << 24);
+  const uint64_t dv = first_desc(v_addr, 8192);
 #pragma unroll
   for (int half = 0; half < 2; ++half)
 #pragma unroll
     for (int k = 0; k < BKV / UMMA_K; ++k)
       tcgen05_mma_f16_ts(tmem_o, tmem_p + half * (BKV / 2) + k * (UMMA_K / 2),
-                         make_smem_desc(v_addr + (k >> 2) * (VD / 64) * 8192 + (k & 3) * (UMMA_K * 128), 8192), idesc,
-                         (add || half || k) ? 1u : 0u);
+                         dv + (((k >> 2) * (VD / 64) * 8192 + (k & 3) * (UMMA_K * 128)) >> 4), idesc, (add || half || k) ? 1u : 0u);
 }
 
+// 64 columns, and the wait for them: nothing may touch the registers in between
+__device__ __forceinline__ void load_scores_64(uint32_t taddr, float* s) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
+      "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, "
+      "%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, "
+      "%48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=f"(s[0]), "=f"(s[1]), "=f"(s[2]), "=f"(s[3]), "=f"(s[4]), "=f"(s[5]), "=f"(s[6]), "=f"(s[7]),
+        "=f"(s[8]), "=f"(s[9]), "=f"(s[10]), "=f"(s[11]), "=f"(s[12]), "=f"(s[13]), "=f"(s[14]), "=f"(s[15]),
+        "=f"(s[16]), "=f"(s[17]), "=f"(s[18]), "=f"(s[19]), "=f"(s[20]), "=f"(s[21]), "=f"(s[22]), "=f"(s[23]),
+        "=f"(s[24]), "=f"(s[25]), "=f"(s[26]), "=f"(s[27]), "=f"(s[28]), "=f"(s[29]), "=f"(s[30]), "=f"(s[31]),
+        "=f"(s[32]), "=f"(s[33]), "=f"(s[34]), "=f"(s[35]), "=f"(s[36]), "=f"(s[37]), "=f"(s[38]), "=f"(s[39]),
+        "=f"(s[40]), "=f"(s[41]), "=f"(s[42]), "=f"(s[43]), "=f"(s[44]), "=f"(s[45]), "=f"(s[46]), "=f"(s[47]),
+        "=f"(s[48]), "=f"(s[49]), "=f"(s[50]), "=f"(s[51]), "=f"(s[52]), "=f"(s[53]), "=f"(s[54]), "=f"(s[55]),
+        "=f"(s[56]), "=f"(s[57]), "=f"(s[58]), "=f"(s[59]), "=f"(s[60]), "=f"(s[61]), "=f"(s[62]), "=f"(s[63])
+      : "r"(taddr)
+      : "memory");
+}
 __device__ __forceinline__ void load_scores(uint32_t tmem_s, float (&s)[BKV]) {
-#pragma unroll
-  for (int ch = 0; ch < BKV / 32; ++ch) {
-    uint32_t raw[32];
-    tmem_ld_32x32b_x32(tmem_s + ch * 32, raw);
-    tmem_ld_wait();
-#pragma unroll
-    for (int i = 0; i < 32; ++i) s[ch * 32 + i] = __uint_as_float(raw[i]);
-  }
+  load_scores_64(tmem_s, s);
+  load_scores_64(tmem_s + 64, s + 64);
+}
+
+// the lowest n bits (n may be anything)
+__device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1; }
+// Keys 32 w .. 32 w + 31 of a block that begins at key0 which a row sees: below `end`, and from `lo` on or below `keep`.
+__device__ __forceinline__ uint32_t visible_bits(int key0, int w, int end, int lo, int keep) {
+  const int k = key0 + 32 * w;
+  return low_bits(end - k) & (~low_bits(lo - k) | low_bits(keep - k));
 }
 
 // Scores of one block (in units of 1 / scale, -inf where masked) become weights; mx, l: running maximum and sum; c = scale * log2(e). Returns the
@@ -317,6 +354,9 @@ __global__ void __launch_bounds__(SA_THREADS, 1)
   const uint32_t tmem_base = *tmem_base_slot;
   const int n_kv = keys.until[3];
 
+  // (the two settings stand at the head of branches that only join again at the end: behind a join the smaller one would hold)
+  if (warp < 4) {
+  fewer_registers<REGS_CONTROL>();
   if (warp == 0) {
     if (lane == 0) {
       xl_grid_dependency_wait();    // the new keys and values; nothing else here depends on the kernel that appends them
@@ -381,13 +421,16 @@ __global__ void __launch_bounds__(SA_THREADS, 1)
         }
       }
     }
-  } else if ((warp < 6 ? 0 : 1) < tiles) {
-    const int m = warp < 6 ? 0 : 1;           // row tile of this warpgroup
+  }
+  } else {
+  more_registers<REGS_SOFTMAX>();
+  if ((warp < 8 ? 0 : 1) < tiles) {
+    const int m = warp < 8 ? 0 : 1;           // row tile of this warpgroup
     const int qtr = warp & 3;                 // TMEM lane quarter this warp may access
     const int r = qtr * 32 + lane;            // row inside the tile
     const long long f = f0 + m * TILE_M + r;  // (token, head of the group)
     const int t = (int)(f / R), hh = (int)(f - (long long)t * R);
-    load_queries<DK, 32>(sQ + m * L::Q_BYTES, qtr * 32, [&](int row) -> const __nv_bfloat16* {
+    load_queries<DK, 4>(sQ + m * L::Q_BYTES, qtr, 4, TILE_M, [&](int row) -> const __nv_bfloat16* {
       const long long at = f0 + m * TILE_M + row;
       if (at >= rows) return nullptr;
       const int tt = (int)(at / R);
@@ -425,8 +468,11 @@ __global__ void __launch_bounds__(SA_THREADS, 1)
       load_scores(tmem_s, s);
       if (col0 + BKV - 1 > hi || (col0 < lo && col0 + BKV > p.keep_first)) {
 #pragma unroll
-        for (int i = 0; i < BKV; ++i)
-          if (col0 + i > hi || (col0 + i < lo && col0 + i >= p.keep_first)) s[i] = -INFINITY;
+        for (int w = 0; w < BKV / 32; ++w) {
+          const uint32_t visible = visible_bits(col0, w, hi + 1, lo, p.keep_first);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) s[w * 32 + i] = visible >> i & 1 ? s[w * 32 + i] : -INFINITY;
+        }
       }
       const float alpha = weigh(s, mx, l, c);
       // the scores of block j are only computed after P V of block j - 1: O is at rest here
@@ -472,6 +518,7 @@ __global__ void __launch_bounds__(SA_THREADS, 1)
     }
   }
 
+  }
   // ---- teardown: every role arrives here, also after an abort --------------------------------------------------------
   tcgen05_fence_before();
   __syncthreads();
@@ -496,41 +543,54 @@ template <int DK, int VD> int launch_portion(const void* kc, const void* vc, con
   return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
 }
 
-// ---- single tokens: the shared positions, once for all that share them -------------------------------------------------------------
+// ---- single tokens: long runs of keys, the shared ones once for all that share them ----------------------------------------------------
 // The query heads of all sequences of a group (those with the same lead) that read one key / value head are the rows of tiles of 128, so a
-// group's shared keys and values are read once per tile and not once per sequence. The blocks of all tiles, groups and heads are one long
-// list, of which every CTA (one per SM) takes an equal run; a tile whose blocks belong to several CTAs leaves as many parts of its sums, and so does
-// each of the two warpgroups, which take a CTA's blocks in turn: one block's softmax runs under the other's products and loads. The kernel behind
-// this one (shared_attn_decode_kernel) adds the parts to what the sequences' own keys give.
+// group's shared keys and values are read once per tile and not once per sequence. Of a sequence's own keys whole blocks of 128 are tiles of
+// R rows, if there are two at least: reading bounds them, and the tensor cores work on empty rows for nothing else. All tiles' blocks, by group and
+// by sequence, are one long list of which every CTA (one per SM) takes an equal run; a tile whose blocks belong to several CTAs leaves as many parts
+// of its sums, and so does each of the two warpgroups, which take a CTA's blocks in turn: one block's softmax runs under the other's products.
+// The kernel behind this one (shared_attn_decode_kernel) adds the parts to what is left of the sequences' own keys.
+//   warp 0       TMA: key and value tiles in turn through one ring
+//   warp 1       MMA: S_m = Q K^T, O_m += P_m V
+//   warps 2, 3   queries of the next tile, normalised, from the projections to shared memory; tiles of up to 64 rows take halves of the room in turn
+//   warps 4..7, 8..11   softmax of every second block; warps without rows only keep step
 //
 // Every CTA makes the list by itself, from positions and leads in shared memory: counts, key ranges and offsets by slot, ranks of the members by
 // votes. CTA 0 leaves a copy for the kernel behind.
 //
 // Keys that only some rows of a tile see are masked; a value that is not finite in a block that some row does not see whole is taken out, and
 // the scores of its key become NaN for the rows that see it: a weight of zero times anything would reach the others.
+constexpr int PF_MAX_BATCH = 512;
 constexpr int PF_SLOTS_LARGE = 4, PF_SLOTS_SMALL = 8;
+constexpr int PF_HALF = TILE_M / 2;
+
+// A sequence's own visible keys before its new one, from `first` on: whole blocks for the prefix kernel (0 or at least two).
+__device__ __forceinline__ int own_blocks(int first, int pos) { return pos - first >= 2 * BKV ? (pos - first) / BKV : 0; }
 
 struct PrefixPlan {  // where a sequence's parts are
-  int first, blocks, tiles, row;      // first block of the group, blocks of a tile, tiles of a head, the sequence's first row in the group
-  int packed, total, ctas, unused;    // rows of the groups before, blocks in all, CTAs that share them
+  int first, blocks, tiles, row;  // first block of the group, blocks of a tile, tiles of a head, the sequence's first row in the group
+  int packed, total, ctas, own_blocks;  // rows of the groups before, blocks in all, CTAs that share them, blocks of a tile of its own keys
+  int own_first, unused[3];       // first block of those
 };
 
 struct PrefixParams {
   SharedParams p;
-  float *main_o, *extra_o;    // parts that begin with a tile's first block: [2][G][B R][vdim]; others, by CTA: [ctas][2][TILE_M][vdim]
+  float *main_o, *extra_o;    // parts that begin with a tile's first block: [groups, own][2][G][B R][vdim]; others, by CTA: [ctas][2][TILE_M][vdim]
   float2 *main_s, *extra_s;   // their maxima (powers of two) and sums
   PrefixPlan* plan;           // [B]
   int read_ahead;             // positions, counts, leads and the caches were complete before the previous launch
 };
 
 struct PrefixLists {  // by slot or by sequence
-  int *edge, *hi, *lo, *begin, *members, *run;
+  int *edge, *hi, *lo, *least, *latest, *members, *run, *own_n, *own_key, *begin;  // begin: of groups, then of sequences
   short *lead, *offset, *rank, *order;
-  __host__ __device__ static int bytes(int B) { return (B + 7) / 8 * 8 * (6 * 4 + 4 * 2); }
+  __host__ __device__ static int padded(int B) { return (B + 7) / 8 * 8; }
+  __host__ __device__ static int bytes(int B) { return padded(B) * (11 * 4 + 4 * 2); }
   __device__ __forceinline__ PrefixLists(void* at, int B) {
-    const int n = (B + 7) / 8 * 8;
-    edge = (int*)at; hi = edge + n; lo = hi + n; begin = lo + n; members = begin + n; run = members + n;
-    lead = (short*)(run + n); offset = lead + n; rank = offset + n; order = rank + n;
+    const int n = padded(B);
+    edge = (int*)at; hi = edge + n; lo = hi + n; least = lo + n; latest = least + n; members = latest + n; run = members + n;
+    own_n = run + n; own_key = own_n + n; begin = own_key + n;
+    lead = (short*)(begin + 2 * n); offset = lead + n; rank = offset + n; order = rank + n;
   }
 };
 
@@ -548,11 +608,13 @@ struct PrefixBlocks {
       total = key_blocks(0, hi);
     }
   }
+  __device__ __forceinline__ int key(int j) const { return j < kept_blocks ? j * BKV : first + (j - kept_blocks) * BKV; }
+  __device__ __forceinline__ int until(int j) const { return j < kept_blocks ? kept : end; }
 };
 
 struct PrefixSegment {  // blocks [block, block + count) of one tile
+  bool own;
   int slot, g, tile, block, count, rows;
-  bool whole;           // begins with the tile's first block
 };
 
 template <int DK, int VD> struct PrefixSmem : SharedTiles<DK, VD> {
@@ -575,6 +637,20 @@ __device__ __forceinline__ bool warps_meet(uint64_t* bar, uint32_t& phase, volat
   return ok;
 }
 
+// Which half of the queries' room a tile takes, and how often it was taken before: the warps that fill it and the one that uses it count alike.
+struct QueryRoom {
+  int next = 0, used[2] = {0, 0};
+  __device__ __forceinline__ int take(int rows) {  // 0 or 1; a tile of more than half takes both, under number 0
+    if (rows > PF_HALF) {
+      next = 0;
+      return 0;
+    }
+    const int h = next;
+    next ^= 1;
+    return h;
+  }
+};
+
 template <int DK, int VD>
 __global__ void __launch_bounds__(SA_THREADS, 1)
     shared_attn_prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const PrefixParams a) {
@@ -586,62 +662,85 @@ __global__ void __launch_bounds__(SA_THREADS, 1)
   uint8_t* sQ = smem;
   uint8_t* ring = smem + L::Q_BYTES;
   uint64_t* bars = (uint64_t*)(smem + L::TILE_BYTES);
-  uint64_t* q_full = bars;
-  uint64_t* s_full = bars + 1;   // [2] per warpgroup
-  uint64_t* p_full = bars + 3;   // [2]
-  uint64_t* pv_done = bars + 5;  // [2]
-  uint64_t* all_meet = bars + 7;  // both warpgroups
-  uint64_t* wg_meet = bars + 8;   // [2]
-  uint64_t* full = bars + 10;     // [SLOTS]
-  uint64_t* empty = bars + 10 + SLOTS;
-  uint32_t* tmem_base_slot = (uint32_t*)(bars + 10 + 2 * SLOTS);
+  uint64_t* q_full = bars;       // [2] by half
+  uint64_t* q_empty = bars + 2;  // [2]
+  uint64_t* s_full = bars + 4;   // [2] per warpgroup
+  uint64_t* p_full = bars + 6;   // [2]
+  uint64_t* pv_done = bars + 8;  // [2]
+  uint64_t* wg_meet = bars + 10;  // [2]
+  uint64_t* full = bars + 12;     // [SLOTS]
+  uint64_t* empty = bars + 12 + SLOTS;
+  uint32_t* tmem_base_slot = (uint32_t*)(bars + 12 + 2 * SLOTS);
   volatile int* abort_flag = (volatile int*)(tmem_base_slot + 1);
-  int* least_edge = (int*)(tmem_base_slot + 2);  // [2][4] by warp: smallest edge and latest window of its rows
-  int* last_first = least_edge + 8;
-  uint32_t* unknown = (uint32_t*)(last_first + 8);  // [2][4] keys whose values are not finite
+  uint32_t* unknown = tmem_base_slot + 2;  // [2][4] keys whose values are not finite
   int* total_blocks = (int*)(unknown + 8);
-  static_assert((10 + 2 * SLOTS) * 8 + 8 + 25 * 4 <= 512, "room behind the tiles");
+  static_assert((12 + 2 * SLOTS) * 8 + 8 + 9 * 4 <= 512, "room behind the tiles");
   const PrefixLists list(smem + L::TILE_BYTES + 512, p.B);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, R = p.H / p.G;
   if (!a.read_ahead) xl_grid_dependency_wait();
   // ---- the list of blocks ------------------------------------------------------------------------------------------------------
   for (int b = tid; b < p.B; b += SA_THREADS) {
-    list.members[b] = list.run[b] = list.hi[b] = 0;
-    list.lo[b] = 0x7fffffff;
+    list.members[b] = list.run[b] = list.hi[b] = list.latest[b] = 0;
+    list.lo[b] = list.least[b] = 0x7fffffff;
+  }
+  if (tid == 0) {
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&q_full[s], 2);
+      mbar_init(&q_empty[s], 1);
+      mbar_init(&s_full[s], 1);
+      mbar_init(&p_full[s], 4);
+      mbar_init(&pv_done[s], 1);
+      mbar_init(&wg_meet[s], 4);
+    }
+    for (int s = 0; s < 2 * SLOTS; ++s) mbar_init(&full[s], 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   __syncthreads();
   for (int b = tid; b < p.B; b += SA_THREADS) {
-    int lead = b, e = 0;
+    int lead = b, e = 0, first = 0, n = 0;
     const int pos = p.pos[b];
-    if (p.count[b] > 0 && window_fits(pos, p.count[b], 1, p.Smax)) e = shared_edge(p.prefix, p.pos, b, pos, p.B, lead);
-    const int first = window_range(pos, p.window, 0).first;
-    const bool sees = e > 0 && (first < e || p.keep_first > 0);
+    bool sees = false;
+    if (p.count[b] > 0 && window_fits(pos, p.count[b], 1, p.Smax)) {
+      e = shared_edge(p.prefix, p.pos, b, pos, p.B, lead);
+      first = window_range(pos, p.window, 0).first;
+      sees = e > 0 && (first < e || p.keep_first > 0);
+      n = own_blocks(max(first, e), pos);
+    }
     list.edge[b] = e;
     list.lead[b] = (short)(sees ? lead : -1);
+    list.own_key[b] = max(first, e);
+    list.own_n[b] = n;
     if (sees) {
       atomicAdd(list.members + lead, 1);
       atomicMax(list.hi + lead, e);
       atomicMin(list.lo + lead, min(first, e));
+      atomicMin(list.least + lead, e);
+      atomicMax(list.latest + lead, first);
     }
   }
   __syncthreads();
-  if (warp == 0) {  // offsets by slot
+  const int n_list = PrefixLists::padded(p.B), own_tiles = (R + TILE_M - 1) / TILE_M;
+  if (warp == 0) {  // offsets by slot, then by sequence
     int rows = 0, blocks = 0;
-    for (int s0 = 0; s0 < p.B; s0 += 32) {
-      const int s = s0 + lane, n = s < p.B ? list.members[s] : 0;
-      int work = 0;
-      if (n) work = (n * R + TILE_M - 1) / TILE_M * p.G * PrefixBlocks(list.lo[s], list.hi[s], p.keep_first).total;
+    for (int s0 = 0; s0 < 2 * n_list; s0 += 32) {
+      const int i = s0 + lane, s = i < n_list ? i : i - n_list;
+      int n = 0, work = 0;
+      if (i < n_list && s < p.B) {
+        n = list.members[s];
+        if (n) work = (n * R + TILE_M - 1) / TILE_M * p.G * PrefixBlocks(list.lo[s], list.hi[s], p.keep_first).total;
+      } else if (i >= n_list && i < 2 * n_list && s < p.B) {
+        work = list.own_n[s] * own_tiles * p.G;
+      }
       int up_n = n, up_w = work;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
         const int x = __shfl_up_sync(0xffffffffu, up_n, d), y = __shfl_up_sync(0xffffffffu, up_w, d);
         if (lane >= d) { up_n += x; up_w += y; }
       }
-      if (s < p.B) {
-        list.offset[s] = (short)(rows + up_n - n);
-        list.begin[s] = blocks + up_w - work;
-      }
+      if (i < n_list) list.offset[i] = (short)(rows + up_n - n);
+      if (i < 2 * n_list) list.begin[i] = blocks + up_w - work;
       rows += __shfl_sync(0xffffffffu, up_n, 31);
       blocks += __shfl_sync(0xffffffffu, up_w, 31);
     }
@@ -665,14 +764,16 @@ __global__ void __launch_bounds__(SA_THREADS, 1)
     if (s >= 0) list.order[list.offset[s] + list.rank[b]] = (short)b;
     if (blockIdx.x == 0) {
       PrefixPlan x = {};
+      x.total = total;
+      x.ctas = ctas;
+      x.own_blocks = list.own_n[b];
+      x.own_first = list.begin[n_list + b];
       if (s >= 0) {
         x.first = list.begin[s];
         x.blocks = PrefixBlocks(list.lo[s], list.hi[s], p.keep_first).total;
         x.tiles = (list.members[s] * R + TILE_M - 1) / TILE_M;
         x.row = list.rank[b] * R;
         x.packed = list.offset[s] * R;
-        x.total = total;
-        x.ctas = ctas;
       }
       a.plan[b] = x;
     }
@@ -685,35 +786,22 @@ __global__ void __launch_bounds__(SA_THREADS, 1)
   const int x0 = ranges.begin(blockIdx.x), x1 = ranges.begin(blockIdx.x + 1);
   // the run of blocks from x on that belong to one tile
   auto segment = [&](int x) {
-    int s = 0;  // the last slot whose blocks begin at x or before
-    for (int step = 512; step; step >>= 1)
-      if (s + step < p.B && list.begin[s + step] <= x) s += step;
-    const int n = PrefixBlocks(list.lo[s], list.hi[s], p.keep_first).total, rows = list.members[s] * R;
-    const int tiles = (rows + TILE_M - 1) / TILE_M, unit = (x - list.begin[s]) / n;
+    int i = 0;  // the last group or sequence whose blocks begin at x or before
+    for (int step = 2 * PF_MAX_BATCH / 2; step; step >>= 1)
+      if (i + step < 2 * n_list && list.begin[i + step] <= x) i += step;
     PrefixSegment g;
-    g.slot = s;
+    g.own = i >= n_list;
+    g.slot = g.own ? i - n_list : i;
+    const int n = g.own ? list.own_n[g.slot] : PrefixBlocks(list.lo[g.slot], list.hi[g.slot], p.keep_first).total;
+    const int rows = g.own ? R : list.members[g.slot] * R, tiles = (rows + TILE_M - 1) / TILE_M, unit = (x - list.begin[i]) / n;
     g.g = unit / tiles;
     g.tile = unit % tiles;
-    g.block = (x - list.begin[s]) % n;
+    g.block = x - list.begin[i] - unit * n;
     g.count = min(n - g.block, x1 - x);
     g.rows = min(TILE_M, rows - g.tile * TILE_M);
-    g.whole = g.block == 0;
     return g;
   };
 
-  if (tid == 0) {
-    mbar_init(q_full, 8);
-    for (int s = 0; s < 2; ++s) {
-      mbar_init(&s_full[s], 1);
-      mbar_init(&p_full[s], 4);
-      mbar_init(&pv_done[s], 1);
-      mbar_init(&wg_meet[s], 4);
-    }
-    mbar_init(all_meet, 8);
-    for (int s = 0; s < 2 * SLOTS; ++s) mbar_init(&full[s], 1);
-    *abort_flag = 0;
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
   if (warp == 1) {
     tmem_alloc(tmem_base_slot, TMEM_COLS);
     tmem_relinquish();
@@ -723,6 +811,9 @@ __global__ void __launch_bounds__(SA_THREADS, 1)
   tcgen05_fence_after();
   const uint32_t tmem_base = *tmem_base_slot;
 
+  // (the two settings stand at the head of branches that only join again at the end: behind a join the smaller one would hold)
+  if (warp < 4) {
+  fewer_registers<REGS_CONTROL>();
   if (warp == 0) {
     if (lane == 0) {
       bool ok = true;
@@ -731,8 +822,7 @@ __global__ void __launch_bounds__(SA_THREADS, 1)
         const PrefixSegment sg = segment(x);
         const PrefixBlocks keys(list.lo[sg.slot], list.hi[sg.slot], p.keep_first);
         for (int j = sg.block; j < sg.block + sg.count && ok; ++j, ++x) {
-          const int key0 = j < keys.kept_blocks ? j * BKV : keys.first + (j - keys.kept_blocks) * BKV;
-          const int row = (sg.slot * p.G + sg.g) * p.Smax + key0;
+          const int row = (sg.slot * p.G + sg.g) * p.Smax + (sg.own ? list.own_key[sg.slot] + j * BKV : keys.key(j));
 #pragma unroll
           for (int kv = 0; kv < 2; ++kv) {
             const int n = 2 * (x - x0) + kv, st = n % SLOTS;
@@ -767,13 +857,13 @@ __global__ void __launch_bounds__(SA_THREADS, 1)
       xl_grid_launch_dependents();  // TMEM is held: a successor that allocates some on this SM cannot come first
       auto wait_full = [&](int n) { return mbar_wait(&full[n % SLOTS], (uint32_t)(n / SLOTS) & 1u, abort_flag, p.err, ERR_KV_FULL); };
       // block `it` of this CTA: warpgroup it & 1, its block it >> 1
-      auto issue_scores = [&](int it) -> bool {
+      auto issue_scores = [&](int it, int half) -> bool {
         const int m = it & 1, st = 2 * it % SLOTS;
         if (!wait_full(2 * it)) return false;
         // the buffer still holds P of the warpgroup's previous block until its product has been taken
         if (it >= 2 && !mbar_wait(&pv_done[m], (uint32_t)((it >> 1) - 1) & 1u, abort_flag, p.err, ERR_PV)) return false;
         tcgen05_fence_after();
-        issue_score_product<DK>(tmem_base + m * BKV, smem_u32(sQ), smem_u32(ring + st * L::SLOT));
+        issue_score_product<DK>(tmem_base + m * BKV, smem_u32(sQ) + half * PF_HALF * 128, smem_u32(ring + st * L::SLOT));
         tcgen05_commit(&empty[st]);
         tcgen05_commit(&s_full[m]);
         return true;
@@ -788,72 +878,84 @@ __global__ void __launch_bounds__(SA_THREADS, 1)
         tcgen05_commit(&pv_done[m]);
         return true;
       };
+      QueryRoom room;
       bool ok = true, add = false;
-      int it = 0, segments = 0;
-      for (int x = x0; x < x1 && ok; ++segments) {
-        const int count = segment(x).count;
-        if (it) ok = issue_values(it - 1, add);  // the last block of the segment before: its warpgroup ends with it
-        ok = ok && mbar_wait(q_full, (uint32_t)segments & 1u, abort_flag, p.err, ERR_Q);
-        for (int j = 0; j < count && ok; ++j, ++it) {
-          ok = issue_scores(it);
-          if (ok && j) ok = issue_values(it - 1, add);
+      int it = 0;
+      for (int x = x0; x < x1 && ok;) {
+        const PrefixSegment sg = segment(x);
+        const int half = room.take(sg.rows);
+        ok = mbar_wait(&q_full[half], (uint32_t)room.used[half] & 1u, abort_flag, p.err, ERR_Q);
+        for (int j = 0; j < sg.count && ok; ++j, ++it) {
+          ok = issue_scores(it, half);
+          if (ok && j + 1 == sg.count) tcgen05_commit(&q_empty[half]);
+          if (ok && it) ok = issue_values(it - 1, add);
           add = j >= 2;  // of this block: the warpgroup has had one of this segment
         }
-        x += count;
+        ++room.used[half];
+        x += sg.count;
       }
       if (ok && it) issue_values(it - 1, add);
     }
   } else {
-    const int m = warp < 6 ? 0 : 1;  // warpgroup
+    xl_grid_dependency_wait();  // the projections
+    QueryRoom room;
+    bool ok = true;
+    for (int x = x0; x < x1 && ok;) {
+      const PrefixSegment sg = segment(x);
+      const int half = room.take(sg.rows);
+      // the products that used the room before: of this half, or of both
+      if (room.used[half]) ok = mbar_wait_warp(&q_empty[half], (uint32_t)(room.used[half] - 1) & 1u, abort_flag, p.err, ERR_Q);
+      if (ok && sg.rows > PF_HALF && room.used[1]) ok = mbar_wait_warp(&q_empty[1], (uint32_t)(room.used[1] - 1) & 1u, abort_flag, p.err, ERR_Q);
+      if (!ok) break;
+      const short* members = list.order + (sg.own ? 0 : list.offset[sg.slot]);
+      load_queries<DK, 2>(sQ + half * PF_HALF * 128, warp - 2, 2, sg.rows, [&](int row) -> const __nv_bfloat16* {
+        if (row >= sg.rows) return nullptr;
+        const int at = sg.tile * TILE_M + row, i = sg.own ? 0 : at / R, b = sg.own ? sg.slot : members[i];
+        return p.proj + (long long)b * p.ld + (long long)(sg.g * R + at - i * R) * p.dim;
+      }, p.wq, p.dim, p.eps);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_full[half]);
+      ++room.used[half];
+      x += sg.count;
+    }
+  }
+  } else {
+    more_registers<REGS_SOFTMAX>();
+    const int m = warp < 8 ? 0 : 1;  // warpgroup
     const int qtr = warp & 3;        // TMEM lane quarter this warp may access
     const int r = qtr * 32 + lane;   // row inside the tile
     const uint32_t lane_base = (uint32_t)(qtr * 32) << 16;
     const uint32_t tmem_s = tmem_base + lane_base + m * BKV;
     const uint32_t tmem_o = tmem_base + lane_base + 2 * BKV + m * VD;
     const float c = p.scale * 1.4426950408889634f;
-    xl_grid_dependency_wait();  // the projections
+    xl_grid_dependency_wait();  // what is written here an earlier attention may still read
     bool ok = true;
-    uint32_t met_all = 0, met_wg = 0;
+    uint32_t met = 0;
     for (int x = x0; x < x1 && ok;) {
       const PrefixSegment sg = segment(x);
       const PrefixBlocks keys(list.lo[sg.slot], list.hi[sg.slot], p.keep_first);
-      const short* members = list.order + list.offset[sg.slot];
-      ok = warps_meet(all_meet, met_all, abort_flag, p.err);  // both have seen the last scores of the segment before: its queries are no longer read
-      if (!ok) break;
-      load_queries<DK, 16>(sQ, (m * 4 + qtr) * 16, [&](int row) -> const __nv_bfloat16* {
-        if (row >= sg.rows) return nullptr;
-        const int at = sg.tile * TILE_M + row, i = at / R;
-        return p.proj + (long long)members[i] * p.ld + (long long)(sg.g * R + at - i * R) * p.dim;
-      }, p.wq, p.dim, p.eps);
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(q_full);
-      const bool row_on = r < sg.rows;
-      const int b = row_on ? members[(sg.tile * TILE_M + r) / R] : 0;
-      const int edge = row_on ? list.edge[b] : 0x7fffffff, lo = row_on ? window_range(p.pos[b], p.window, 0).first : 0;
-      const int warp_edge = __reduce_min_sync(0xffffffffu, edge), warp_first = __reduce_max_sync(0xffffffffu, lo);
-      if (lane == 0) {
-        least_edge[m * 4 + qtr] = warp_edge;
-        last_first[m * 4 + qtr] = warp_first;
-      }
-      ok = warps_meet(&wg_meet[m], met_wg, abort_flag, p.err);
-      int all_edge = least_edge[m * 4], all_first = last_first[m * 4];
-#pragma unroll
-      for (int w = 1; w < 4; ++w) {
-        all_edge = min(all_edge, least_edge[m * 4 + w]);
-        all_first = max(all_first, last_first[m * 4 + w]);
+      const bool row_on = r < sg.rows, warp_on = qtr * 32 < sg.rows;
+      int edge = 0x7fffffff, lo = 0, least = 0x7fffffff, latest = 0;
+      if (!sg.own) {
+        least = list.least[sg.slot];
+        latest = list.latest[sg.slot];
+        if (row_on) {
+          const int b = list.order[list.offset[sg.slot] + (sg.tile * TILE_M + r) / R];
+          edge = list.edge[b];
+          lo = window_range(p.pos[b], p.window, 0).first;
+        }
       }
       float mx = -INFINITY, l = 0.f;
       int mine = 0, last = 0;
       for (int j = sg.block; j < sg.block + sg.count && ok; ++j, ++x) {
         const int it = x - x0;
         if ((it & 1) != m) continue;
-        const int key0 = j < keys.kept_blocks ? j * BKV : keys.first + (j - keys.kept_blocks) * BKV;
-        const int end = j < keys.kept_blocks ? keys.kept : keys.end;
         ok = mbar_wait_warp(&s_full[m], (uint32_t)(it >> 1) & 1u, abort_flag, p.err, ERR_S);
         if (!ok) break;
         tcgen05_fence_after();
-        const bool cut = key0 + BKV > end || key0 + BKV > all_edge || (key0 < all_first && key0 + BKV > p.keep_first);
+        const int key0 = keys.key(j), end = keys.until(j);
+        const bool cut = !sg.own && (key0 + BKV > end || key0 + BKV > least || (key0 < latest && key0 + BKV > p.keep_first));
         if (cut) {  // not every row sees every key: thread r looks at the value of key r
           const int n = 2 * it + 1;
           ok = mbar_wait_warp(&full[n % SLOTS], (uint32_t)(n / SLOTS) & 1u, abort_flag, p.err, ERR_KV_FULL);
@@ -878,28 +980,30 @@ __global__ void __launch_bounds__(SA_THREADS, 1)
 #pragma unroll
               for (int i = 0; i < 8; ++i) value_row<VD>(tile, r, jn)[i] = make_uint4(0u, 0u, 0u, 0u);
           fence_proxy_async_smem();
-          ok = warps_meet(&wg_meet[m], met_wg, abort_flag, p.err);
+          ok = warps_meet(&wg_meet[m], met, abort_flag, p.err);
           if (!ok) break;
         }
-        float s[BKV];
-        load_scores(tmem_s, s);
-        if (cut) {
+        if (warp_on) {
+          float s[BKV];
+          load_scores(tmem_s, s);
+          if (cut) {
 #pragma unroll
-          for (int w = 0; w < BKV / 32; ++w) {
-            const uint32_t not_known = unknown[m * 4 + w];
+            for (int w = 0; w < BKV / 32; ++w) {
+              const uint32_t not_known = unknown[m * 4 + w];
+              const uint32_t visible = visible_bits(key0, w, min(end, edge), lo, p.keep_first);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              const int k = key0 + w * 32 + i;
-              const bool visible = k < end && k < edge && (k >= lo || k < p.keep_first);
-              s[w * 32 + i] = !visible ? -INFINITY : not_known >> i & 1 ? NAN : s[w * 32 + i];
+              for (int i = 0; i < 32; ++i) {
+                s[w * 32 + i] = not_known >> i & 1 ? NAN : s[w * 32 + i];
+                s[w * 32 + i] = visible >> i & 1 ? s[w * 32 + i] : -INFINITY;
+              }
             }
           }
+          const float alpha = weigh(s, mx, l, c);
+          // the scores of a block are only computed after P V of the warpgroup's block before: O is at rest here
+          if (mine && __any_sync(0xffffffffu, alpha != 1.f)) rescale_output<VD>(tmem_o, alpha);
+          store_split_weights<BKV>(tmem_s, s);
+          tmem_st_wait();
         }
-        const float alpha = weigh(s, mx, l, c);
-        // the scores of a block are only computed after P V of the warpgroup's block before: O is at rest here
-        if (mine && __any_sync(0xffffffffu, alpha != 1.f)) rescale_output<VD>(tmem_o, alpha);
-        store_split_weights<BKV>(tmem_s, s);
-        tmem_st_wait();
         tcgen05_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[m]);
@@ -907,14 +1011,17 @@ __global__ void __launch_bounds__(SA_THREADS, 1)
         last = it >> 1;
       }
       // ---- this part's sums ------------------------------------------------------------------------------------------------
-      if (ok && mine) ok = mbar_wait_warp(&pv_done[m], (uint32_t)last & 1u, abort_flag, p.err, ERR_PV);
-      if (!ok) break;
-      const long long at = sg.whole ? ((long long)m * p.G + sg.g) * p.B * R + (long long)list.offset[sg.slot] * R + sg.tile * TILE_M + r
-                                    : ((long long)blockIdx.x * 2 + m) * TILE_M + r;
-      if (row_on) (sg.whole ? a.main_s : a.extra_s)[at] = make_float2(mx * c, l);
+      if (!ok || !warp_on) continue;
+      const bool main = sg.block == 0;
+      const long long at = main ? (((long long)sg.own * 2 + m) * p.G + sg.g) * p.B * R +
+                                      (sg.own ? sg.slot : list.offset[sg.slot]) * (long long)R + sg.tile * TILE_M + r
+                                : ((long long)blockIdx.x * 2 + m) * TILE_M + r;
+      if (row_on) (main ? a.main_s : a.extra_s)[at] = make_float2(mx * c, l);
       if (mine) {
+        ok = mbar_wait_warp(&pv_done[m], (uint32_t)last & 1u, abort_flag, p.err, ERR_PV);
+        if (!ok) break;
         tcgen05_fence_after();
-        float* o = (sg.whole ? a.main_o : a.extra_o) + at * p.vdim;
+        float* o = (main ? a.main_o : a.extra_o) + at * p.vdim;
 #pragma unroll 1
         for (int ch = 0; ch < VD / 32; ++ch) {
           uint32_t raw[32];
@@ -940,20 +1047,16 @@ __global__ void __launch_bounds__(SA_THREADS, 1)
   }
 }
 
-// ---- single tokens: each sequence's own keys, and the sum of all parts ----------------------------------------------------------------
-// As window_attn_decode_kernel (attention_window.cu): grid (splits, G * head chunks, B); a CTA takes up to 8 RT query heads of one key / value
-// head and a run of the blocks of keys, each of its 4 warps with a cp.async ring of its own, products on mma.sync. It starts under the
-// prefix kernel's tail: everything but the parts of the shared keys was complete when that kernel let it start. The number of runs
-// goes by the keys that there are: up to 320 one CTA has them all, and no merge of runs.
+// ---- single tokens: the rest of each sequence's own keys, and the sum of all parts -------------------------------------------------------
+// As window_attn_decode_kernel (attention_window.cu): a CTA takes up to 8 RT query heads of one key / value head, each of its 4 warps every fourth
+// block of keys through a cp.async ring of its own, products on mma.sync. There are fewer than 256 keys besides kept ones: the prefix kernel has the
+// others. It starts under that kernel's tail: everything but its parts was complete when it let this one start.
 constexpr int SD_WARPS = 4;
-constexpr int SD_MAX_SPLITS = 64;
 
 struct SharedDecodeParams {
   SharedParams p;
   __nv_bfloat16 *kc, *vc;
   const float *wk;
-  float* part;             // [units][splits][heads per CTA][vdim], then the same with [2]: maximum, sum
-  unsigned int* counters;  // [units], zero between launches
   const float *main_o, *extra_o;
   const float2 *main_s, *extra_s;
   const PrefixPlan* plan;
@@ -966,7 +1069,7 @@ __host__ __device__ constexpr int sd_stage_bytes(int keys, int kd, int vdim) { r
 
 // KD: 32-feature steps of a query / key row (dim <= 32 KD); VT: 8-feature tiles of a value row (vdim <= 8 VT)
 template <int KD, int VT, int RT>
-__global__ void __launch_bounds__(SD_WARPS * 32) shared_attn_decode_kernel(const SharedDecodeParams d) {
+__global__ void __launch_bounds__(SD_WARPS * 32, RT == 1 ? 3 : 2) shared_attn_decode_kernel(const SharedDecodeParams d) {
   constexpr int KEYS = sd_keys(KD, VT), KT = KEYS / 8;  // keys per block, tiles of eight keys
   constexpr int HEADS = 8 * RT;
   const SharedParams& p = d.p;
@@ -975,29 +1078,24 @@ __global__ void __launch_bounds__(SD_WARPS * 32) shared_attn_decode_kernel(const
   __shared__ __align__(16) __nv_bfloat16 sq[2][HEADS + 1][KD * 32];
   __shared__ float sm[SD_WARPS][HEADS], sl[SD_WARPS][HEADS], fw[SD_WARPS][HEADS];
   __shared__ float2 own[HEADS];  // this CTA's maxima and sums
-  __shared__ unsigned int is_last;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = lane >> 2, j = lane & 3;
   const int R = p.H / p.G, hchunks = (R + HEADS - 1) / HEADS;
-  const int split = blockIdx.x, g = blockIdx.y / hchunks, b = blockIdx.z;
-  const int h0 = g * R + (blockIdx.y % hchunks) * HEADS;  // first query head of this CTA
+  const int g = blockIdx.x / hchunks, b = blockIdx.y;
+  const int h0 = g * R + (blockIdx.x % hchunks) * HEADS;  // first query head of this CTA
   const int nh = min(HEADS, (g + 1) * R - h0);
   const int pos = p.pos[b];
-  int lead = b, edge = 0, splits = 0, blocks = 0;
-  WindowRange seen = {0, 0};
-  if (p.count[b] > 0 && window_fits(pos, p.count[b], 1, p.Smax)) {
-    edge = shared_edge(p.prefix, p.pos, b, pos, p.B, lead);
-    seen = window_range(pos, p.window, p.keep_first);
-    seen.first = max(seen.first, edge);
-    seen.kept = max(seen.kept, edge);  // kept tokens of its own: [edge, kept)
-    blocks = (seen.kept - edge + KEYS - 1) / KEYS + (pos - seen.first) / KEYS + 1;
-    splits = blocks * KEYS <= 320 ? 1 : min((int)gridDim.x, (blocks * KEYS + 63) / 64);
-  }
-  if (split >= splits) {
+  if (p.count[b] <= 0 || !window_fits(pos, p.count[b], 1, p.Smax)) {
     xl_grid_dependency_wait();  // no kernel of a chain ends before its predecessor
     return;
   }
+  int lead;
+  const int edge = shared_edge(p.prefix, p.pos, b, pos, p.B, lead);
+  WindowRange seen = window_range(pos, p.window, p.keep_first);
+  seen.first = max(seen.first, edge);
+  seen.kept = max(seen.kept, edge);  // kept tokens of its own: [edge, kept)
+  seen.first += own_blocks(seen.first, pos) * BKV;
   const int kept_blocks = (seen.kept - edge + KEYS - 1) / KEYS;
-  const int blk0 = (int)((long long)split * blocks / splits), blk1 = (int)((long long)(split + 1) * blocks / splits);
+  const int blocks = kept_blocks + (pos - seen.first) / KEYS + 1;
   const __nv_bfloat16* row = p.proj + (long long)b * p.ld;
   const __nv_bfloat16* kb = d.kc + ((long long)b * p.G + g) * p.Smax * p.dim;
   const __nv_bfloat16* vb = d.vc + ((long long)b * p.G + g) * p.Smax * p.vdim;
@@ -1008,14 +1106,14 @@ __global__ void __launch_bounds__(SD_WARPS * 32) shared_attn_decode_kernel(const
   // ---- the ring of key / value blocks -------------------------------------------------------------------------------------
   const int stage_bytes = sd_stage_bytes(KEYS, KD, p.vdim), vld = p.vdim + 8;
   uint8_t* ring = smem + (long long)warp * d.stages * stage_bytes;
-  const int mine = (blk1 - blk0 - warp + SD_WARPS - 1) / SD_WARPS;  // this warp's blocks: blk0 + warp, + SD_WARPS, ...
+  const int mine = (blocks - warp + SD_WARPS - 1) / SD_WARPS;  // this warp's blocks: warp, warp + SD_WARPS, ...
   constexpr int V_ROWS = 32 / VT, V_PASSES = KEYS / V_ROWS;  // value rows that a warp copies at a time, one piece per lane
   const int v_row = lane / VT, v_col = (lane % VT) * 8;
   const bool v_on = v_col < p.vdim;
   auto prefetch = [&](int n) {
     if (n < mine) {
       uint8_t* st = ring + (n % d.stages) * stage_bytes;
-      const int blk = blk0 + warp + n * SD_WARPS, key0 = first_key(blk), end = min(end_key(blk), pos);
+      const int blk = warp + n * SD_WARPS, key0 = first_key(blk), end = min(end_key(blk), pos);
       const bool full = key0 + KEYS <= end;  // else rows from `end` on are zero-filled
 #pragma unroll
       for (int t = 0; t < KT; ++t) {
@@ -1040,8 +1138,7 @@ __global__ void __launch_bounds__(SD_WARPS * 32) shared_attn_decode_kernel(const
     asm volatile("cp.async.commit_group;" ::: "memory");  // possibly empty: keeps the group count per block fixed
   };
   for (int n = 0; n < d.stages - 1; ++n) prefetch(n);
-  // ---- normalised queries and new key to shared memory; the CTAs with the last keys append (the same data each) ---------------
-  const bool appends = split == splits - 1;
+  // ---- normalised queries and new key to shared memory, new key and value to the caches (the same data from each chunk of heads) -----
   const __nv_bfloat16* v_src = row + (long long)(p.H + p.G) * p.dim + (long long)g * p.vdim;
   uint4 v_new = make_uint4(0, 0, 0, 0);  // lane's piece of the new value, in every warp
   {
@@ -1067,7 +1164,7 @@ __global__ void __launch_bounds__(SD_WARPS * 32) shared_attn_decode_kernel(const
         w[1][2 * u + c] = e < p.dim ? d.wk[e + c] : 0.f;
       }
     }
-    if (appends && lane < p.vdim / 8) v_new = *reinterpret_cast<const uint4*>(v_src + lane * 8);
+    if (lane < p.vdim / 8) v_new = *reinterpret_cast<const uint4*>(v_src + lane * 8);
     float sum[QUERIES];
     double key_sum = 0.0;  // the key's norm is taken in 64 bits, as in every kernel, so that all come to the same number
 #pragma unroll
@@ -1114,11 +1211,11 @@ __global__ void __launch_bounds__(SD_WARPS * 32) shared_attn_decode_kernel(const
           const uint32_t y = dd_pack((float)((double)dd_lo(raw[QUERIES][u]) * f * (double)w[1][2 * u]),
                                      (float)((double)dd_hi(raw[QUERIES][u]) * f * (double)w[1][2 * u + 1]));
           *reinterpret_cast<uint32_t*>(&sq[0][HEADS][e]) = y;
-          if (appends && e < p.dim) *reinterpret_cast<uint32_t*>(d.kc + (((long long)b * p.G + g) * p.Smax + pos) * p.dim + e) = y;
+          if (e < p.dim) *reinterpret_cast<uint32_t*>(d.kc + (((long long)b * p.G + g) * p.Smax + pos) * p.dim + e) = y;
         }
       }
     }
-    if (appends && threadIdx.x < p.vdim / 8)
+    if (threadIdx.x < p.vdim / 8)
       *reinterpret_cast<uint4*>(d.vc + (((long long)b * p.G + g) * p.Smax + pos) * p.vdim + threadIdx.x * 8) = v_new;
   }
   __syncthreads();
@@ -1148,7 +1245,7 @@ __global__ void __launch_bounds__(SD_WARPS * 32) shared_attn_decode_kernel(const
     else asm volatile("cp.async.wait_group 3;" ::: "memory");
     __syncwarp();
     uint8_t* st = ring + (n % d.stages) * stage_bytes;
-    const int blk = blk0 + warp + n * SD_WARPS, key0 = first_key(blk), end = end_key(blk);
+    const int blk = warp + n * SD_WARPS, key0 = first_key(blk), end = end_key(blk);
     if (blk == blocks - 1) {  // the new key and value take their place
       const int k = pos - key0;
       for (int i = lane; i < KD * 4; i += 32)
@@ -1266,9 +1363,6 @@ __global__ void __launch_bounds__(SD_WARPS * 32) shared_attn_decode_kernel(const
     }
   }
   // ---- merge of the warps: their weights, and the sums of the weights --------------------------------------------------------
-  const long long units = (long long)gridDim.z * gridDim.y, unit = (long long)b * gridDim.y + blockIdx.y;
-  float2* stats = reinterpret_cast<float2*>(d.part + units * gridDim.x * HEADS * p.vdim) + unit * gridDim.x * HEADS;
-  float* slices = d.part + unit * gridDim.x * HEADS * p.vdim;
   if (threadIdx.x < HEADS) {
     const int r = threadIdx.x;
     float m = -INFINITY;
@@ -1282,7 +1376,6 @@ __global__ void __launch_bounds__(SD_WARPS * 32) shared_attn_decode_kernel(const
       ll += sl[w][r] * f;  // (a sum that is not a number stays none)
     }
     own[r] = make_float2(m, ll);
-    if (splits > 1) __stcg(stats + split * HEADS + r, make_float2(m, ll));
   }
   __syncthreads();
   auto merged = [&](int r, int c) {  // head r, features c .. c + 3, over this CTA's warps
@@ -1295,89 +1388,70 @@ __global__ void __launch_bounds__(SD_WARPS * 32) shared_attn_decode_kernel(const
     }
     return a;
   };
-  if (splits > 1) {
-    for (int r = warp; r < nh; r += SD_WARPS)
-#pragma unroll
-      for (int u = 0; u < CH; ++u) {
-        const int c = (lane + 32 * u) * 4;
-        if (c < p.vdim) __stcg(reinterpret_cast<float4*>(slices + ((long long)split * HEADS + r) * p.vdim + c), merged(r, c));
-      }
-    __threadfence();
-    __syncthreads();
-    if (threadIdx.x == 0) is_last = atomicAdd(d.counters + unit, 1u) == (unsigned int)splits - 1;
-    __syncthreads();
-    if (!is_last) {
-      xl_grid_dependency_wait();
-      return;
-    }
-    __threadfence();
-    if (threadIdx.x == 0) d.counters[unit] = 0;
-  }
-  // ---- all parts: this sequence's own, then those of the shared keys -------------------------------------------------------------
-  xl_grid_dependency_wait();  // the parts of the prefix kernel
+  // ---- all parts: these keys, then what the prefix kernel has of the shared and of the sequence's own ones ----------------------------------
+  xl_grid_dependency_wait();
   xl_grid_launch_dependents();
   const int4* at = reinterpret_cast<const int4*>(d.plan + b);
-  const int4 pa = __ldcg(at), pb = __ldcg(at + 1);
-  const int n_blocks = pa.y;
-  const XlRanges ranges{n_blocks ? pb.y / pb.z : 1, n_blocks ? pb.y % pb.z : 0};
+  const int4 pa = __ldcg(at), pb = __ldcg(at + 1), pc = __ldcg(at + 2);
+  const XlRanges ranges{pb.z ? pb.y / pb.z : 1, pb.z ? pb.y % pb.z : 0};
   const float sink = p.sink * 1.4426950408889634f;
 #pragma unroll
   for (int i = 0; i < MINE; ++i) {
     const int r = warp + i * SD_WARPS;
     if (r >= nh) break;
-    const int idx = pa.w + h0 - g * R + r;  // row in the group
-    int c0 = 0, parts = 0;
-    if (n_blocks) {
-      const int x = pa.x + (g * pa.z + idx / TILE_M) * n_blocks;
-      c0 = ranges.owner(x);
-      parts = 2 * (ranges.owner(x + n_blocks - 1) - c0 + 1);
-    }
-    const int slices_n = splits > 1 ? splits : 0, all = parts + slices_n;
+    const int hh = h0 - g * R + r;
+    // two sources: the tile of the group and the tile of the sequence; of each one CTA's part for each warpgroup from its first block on, then those of
+    // the CTAs that follow
+    int idx[2] = {pa.w + hh, hh}, c0[2] = {0, 0}, parts[2] = {0, 0};
+    const int n_of[2] = {pa.y, pb.w};
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      if (n_of[k]) {
+        const int x = k ? pc.x + (g * ((R + TILE_M - 1) / TILE_M) + idx[k] / TILE_M) * n_of[k] : pa.x + (g * pa.z + idx[k] / TILE_M) * n_of[k];
+        c0[k] = ranges.owner(x);
+        parts[k] = 2 * (ranges.owner(x + n_of[k] - 1) - c0[k] + 1);
+      }
+    const long long row0[2] = {pb.x + idx[0], (long long)b * R + idx[1]};
+    const int all = parts[0] + parts[1];
+    auto place = [&](int k, bool& main) -> long long {
+      const int q = k < parts[0] ? k : k - parts[0], src = k < parts[0] ? 0 : 1, m = q & 1, c = q >> 1;
+      main = c == 0;
+      return main ? ((long long)(src * 2 + m) * p.G + g) * p.B * R + (src ? row0[1] : row0[0])
+                  : ((long long)((src ? c0[1] : c0[0]) + c) * 2 + m) * TILE_M + (src ? idx[1] : idx[0]) % TILE_M;
+    };
     auto stat = [&](int k) {
-      if (k < slices_n) return __ldcg(stats + k * HEADS + r);
-      const int q = k - slices_n, m = q & 1, c = q >> 1;
-      return c == 0 ? __ldcg(d.main_s + ((long long)m * p.G + g) * p.B * R + pb.x + idx)
-                    : __ldcg(d.extra_s + ((long long)(c0 + c) * 2 + m) * TILE_M + idx % TILE_M);
+      bool main;
+      const long long e = place(k, main);
+      return __ldcg((main ? d.main_s : d.extra_s) + e);
     };
-    auto sums = [&](int k) -> const float* {
-      if (k < slices_n) return slices + ((long long)k * HEADS + r) * p.vdim;
-      const int q = k - slices_n, m = q & 1, c = q >> 1;
-      return c == 0 ? d.main_o + (((long long)m * p.G + g) * p.B * R + pb.x + idx) * p.vdim
-                    : d.extra_o + (((long long)(c0 + c) * 2 + m) * TILE_M + idx % TILE_M) * p.vdim;
-    };
-    float m = fmaxf(sink, splits > 1 ? -INFINITY : own[r].x);
-    for (int k = lane; k < all; k += 32) m = fmaxf(m, stat(k).x);
+    float2 mine_s = lane < all ? stat(lane) : make_float2(-INFINITY, 0.f);  // of the first 32 parts
+    float m = fmaxf(fmaxf(sink, own[r].x), mine_s.x);
+    for (int k = lane + 32; k < all; k += 32) m = fmaxf(m, stat(k).x);
     m = xl_warp_max(m);
     float4 acc[CH];
     float total = sink == -INFINITY ? 0.f : exp2f(sink - m);
-#pragma unroll
-    for (int u = 0; u < CH; ++u) acc[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (splits == 1) {
+    {
       const float f = own[r].x == -INFINITY ? 0.f : exp2f(own[r].x - m);
-      total += f * own[r].y;
+      total += f * own[r].y;  // (a sum that is not a number stays none)
 #pragma unroll
       for (int u = 0; u < CH; ++u) {
         const int c = (lane + 32 * u) * 4;
-        if (c < p.vdim) {
-          const float4 x = merged(r, c);
-          acc[u] = make_float4(x.x * f, x.y * f, x.z * f, x.w * f);
-        }
+        acc[u] = c < p.vdim ? merged(r, c) : make_float4(0.f, 0.f, 0.f, 0.f);
+        acc[u] = make_float4(acc[u].x * f, acc[u].y * f, acc[u].z * f, acc[u].w * f);
       }
     }
     for (int k0 = 0; k0 < all; k0 += 32) {
-      float f = 0.f, lk = 0.f;
-      if (k0 + lane < all) {
-        const float2 st = stat(k0 + lane);
-        f = st.x == -INFINITY ? 0.f : exp2f(st.x - m);
-        lk = f * st.y;
-      }
-      total += xl_warp_sum(lk);
+      if (k0) mine_s = k0 + lane < all ? stat(k0 + lane) : make_float2(-INFINITY, 0.f);
+      const float f = mine_s.x == -INFINITY ? 0.f : exp2f(mine_s.x - m);
+      total += xl_warp_sum(f * mine_s.y);
       const int n = min(32, all - k0);
 #pragma unroll 4
       for (int k = 0; k < n; ++k) {
         const float fk = __shfl_sync(0xffffffffu, f, k);
         if (fk == 0.f) continue;
-        const float* src = sums(k0 + k);
+        bool main;
+        const long long e = place(k0 + k, main);
+        const float* src = (main ? d.main_o : d.extra_o) + e * p.vdim;
 #pragma unroll
         for (int u = 0; u < CH; ++u) {
           const int c = (lane + 32 * u) * 4;
@@ -1406,9 +1480,9 @@ __global__ void __launch_bounds__(SD_WARPS * 32) shared_attn_decode_kernel(const
   }
 }
 
-constexpr int SD_RING_LIMIT = 104 * 1024;  // two CTAs per SM
+constexpr int SD_RING_LIMIT = 68 * 1024;  // three CTAs per SM
 
-template <int KD, int VT, int RT> int launch_decode_rows(SharedDecodeParams d, int splits, cudaStream_t s) {
+template <int KD, int VT, int RT> int launch_decode_rows(SharedDecodeParams d, cudaStream_t s) {
   const SharedParams& p = d.p;
   const int stage = sd_stage_bytes(sd_keys(KD, VT), KD, p.vdim) * SD_WARPS;
   d.stages = 4 * stage <= SD_RING_LIMIT ? 4 : (3 * stage <= SD_RING_LIMIT ? 3 : 2);
@@ -1418,13 +1492,13 @@ template <int KD, int VT, int RT> int launch_decode_rows(SharedDecodeParams d, i
   static XlPerDevice smem;
   XL_TRY(xl_allow_smem(shared_attn_decode_kernel<KD, VT, RT>, bytes, smem));
   const int hchunks = (p.H / p.G + 8 * RT - 1) / (8 * RT);
-  const cudaError_t e = xl_launch_overlapped(shared_attn_decode_kernel<KD, VT, RT>, dim3(splits, p.G * hchunks, p.B), dim3(SD_WARPS * 32),
+  const cudaError_t e = xl_launch_overlapped(shared_attn_decode_kernel<KD, VT, RT>, dim3(p.G * hchunks, p.B), dim3(SD_WARPS * 32),
                                              (size_t)bytes, s, d);
   return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
 }
 
-template <int KD, int VT> int launch_decode(const SharedDecodeParams& d, int splits, cudaStream_t s) {
-  return d.p.H / d.p.G <= 8 ? launch_decode_rows<KD, VT, 1>(d, splits, s) : launch_decode_rows<KD, VT, 2>(d, splits, s);
+template <int KD, int VT> int launch_decode(const SharedDecodeParams& d, cudaStream_t s) {
+  return d.p.H / d.p.G <= 8 ? launch_decode_rows<KD, VT, 1>(d, s) : launch_decode_rows<KD, VT, 2>(d, s);
 }
 
 template <int DK, int VD> int launch_prefix(const PrefixParams& a, const void* kc, const void* vc, int ctas, cudaStream_t s) {
@@ -1486,22 +1560,18 @@ XL_API int xl_shared_attn_portion(const void* proj, long long ld, const float* w
   return vdim <= 64 ? launch_portion<128, 64>(kc, vc, p, s) : launch_portion<128, 128>(kc, vc, p, s);
 }
 
-// floats of scratch memory for xl_shared_attn_decode: parts of the shared keys by `ctas` CTAs, and of each sequence's own in `splits` runs
-XL_API long long xl_shared_attn_decode_scratch(int B, int H, int G, int vdim, int ctas, int splits) {
-  const long long R = H / G, heads = R <= 8 ? 8 : 16, units = (long long)B * G * ((R + heads - 1) / heads);
-  return B * 8LL + (2LL * B * H + ctas * 2LL * TILE_M) * (vdim + 2) + (splits > 1 ? units * splits * heads * (vdim + 2) : 0);
-}
+// floats of scratch memory for xl_shared_attn_decode with `ctas` CTAs for long runs of keys
+XL_API long long xl_shared_attn_decode_scratch(int B, int H, int vdim, int ctas) { return B * 12LL + (4LL * B * H + ctas * 2LL * TILE_M) * (vdim + 2); }
 
-// One token per sequence (rows of proj = sequences), bf16, in two launches. Sizes and alignment as for portions, at most 1024 sequences. Queries and
-// keys are normalised and keys and values appended here. ctas: CTAs for the shared keys (SMs of the device); splits: runs of a sequence's own keys, at
-// most 64. scratch: xl_shared_attn_decode_scratch floats, 16-byte aligned; counters: B * G * ceil(H/G/8) zero-initialised words (left zeroed).
+// One token per sequence (rows of proj = sequences), bf16, in two launches. Sizes and alignment as for portions, at most 512 sequences. Queries and
+// keys are normalised and keys and values appended here. ctas: SMs of the device. scratch: xl_shared_attn_decode_scratch floats, 16-byte aligned.
 // read_ahead: positions, counts, leads and caches were complete before the previous launch of the stream.
 XL_API int xl_shared_attn_decode(const void* proj, long long ld, const float* wq, const float* wk, void* kc, void* vc, void* out, long long ldo,
                                  const int* pos, const int* count, const int* lead, const int* shared, int B, int H, int G, int dim, int vdim,
-                                 int Smax, int window, int keep_first, int gated, float scale, float sink, float eps, int ctas, int splits,
-                                 float* scratch, unsigned int* counters, int read_ahead, int* err, cudaStream_t s) {
-  if (B < 1 || B > 1024 || G < 1 || H < 1 || H % G || H > 4096 || Smax < 1 || window < 0 || keep_first < 0 || !(scale > 0.f) || !lead || !shared ||
-      !wq || !wk || ctas < 1 || ctas > 4096 || splits < 1 || splits > SD_MAX_SPLITS || !scratch || ((uintptr_t)scratch & 15) || !counters)
+                                 int Smax, int window, int keep_first, int gated, float scale, float sink, float eps, int ctas,
+                                 float* scratch, int read_ahead, int* err, cudaStream_t s) {
+  if (B < 1 || B > PF_MAX_BATCH || G < 1 || H < 1 || H % G || H > 4096 || Smax < 1 || window < 0 || keep_first < 0 || !(scale > 0.f) || !lead || !shared ||
+      !wq || !wk || ctas < 1 || ctas > 4096 || !scratch || ((uintptr_t)scratch & 15))
     return -1;
   if (!tensor_sizes(proj, ld, kc, vc, out, ldo, B, 1, H, G, dim, vdim, Smax, gated)) return -1;
   SharedParams p = {};
@@ -1511,21 +1581,20 @@ XL_API int xl_shared_attn_decode(const void* proj, long long ld, const float* wq
   PrefixParams a = {};
   a.p = p;
   a.plan = (PrefixPlan*)scratch;
-  a.main_o = scratch + 8LL * B;
-  a.extra_o = a.main_o + 2LL * B * H * vdim;
+  static_assert(sizeof(PrefixPlan) == 48, "12 floats of scratch memory per sequence");
+  a.main_o = scratch + 12LL * B;
+  a.extra_o = a.main_o + 4LL * B * H * vdim;
   a.main_s = (float2*)(a.extra_o + 2LL * ctas * TILE_M * vdim);
-  a.extra_s = a.main_s + 2LL * B * H;
+  a.extra_s = a.main_s + 4LL * B * H;
   a.read_ahead = read_ahead;
   SharedDecodeParams d = {};
   d.p = p; d.kc = (__nv_bfloat16*)kc; d.vc = (__nv_bfloat16*)vc; d.wk = wk;
   d.main_o = a.main_o; d.extra_o = a.extra_o; d.main_s = a.main_s; d.extra_s = a.extra_s; d.plan = a.plan;
-  d.part = (float*)(a.extra_s + 2LL * ctas * TILE_M);
-  d.counters = counters;
   int r;
   if (dim <= 64) r = vdim <= 64 ? launch_prefix<64, 64>(a, kc, vc, ctas, s) : launch_prefix<64, 128>(a, kc, vc, ctas, s);
   else r = vdim <= 64 ? launch_prefix<128, 64>(a, kc, vc, ctas, s) : launch_prefix<128, 128>(a, kc, vc, ctas, s);
   if (r) return r;
-#define XL_SD(KD) return vdim <= 64 ? launch_decode<KD, 8>(d, splits, s) : launch_decode<KD, 16>(d, splits, s);
+#define XL_SD(KD) return vdim <= 64 ? launch_decode<KD, 8>(d, s) : launch_decode<KD, 16>(d, s);
   if (dim <= 32) { XL_SD(1) }
   if (dim <= 64) { XL_SD(2) }
   XL_SD(4)

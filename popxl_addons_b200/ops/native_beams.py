@@ -5,17 +5,15 @@ import torch
 
 from ..xl import read_ahead
 from ..xl.opdef import native
-from ..xl.ops.beams import MAX_SHARED_BATCH
 from .native import _CODE, _c_f, _c_int, _c_ll, _c_p, _count, _ok, _sig, _sms, _stream, counters, gemm_error_flag, workspace
-from .native_sequence import _decode_slices, _f32, _i32, _ptr
+from .native_sequence import _f32, _i32, _ptr
 from .native_serving import _c_d, _done, _launched, _rows16
 
 _shared_append = _sig("xl_shared_append", _c_p, _c_ll, *[_c_p] * 7, *[_c_int] * 7, _c_f, _c_int, _c_p)
 _shared_general = _sig("xl_shared_attn_general", *[_c_p] * 4, _c_ll, _c_p, _c_ll, *[_c_p] * 4, *[_c_int] * 9, _c_f, _c_f, _c_int, _c_p)
 _shared_portion = _sig("xl_shared_attn_portion", _c_p, _c_ll, *[_c_p] * 4, _c_ll, *[_c_p] * 4, *[_c_int] * 10, *[_c_f] * 3, _c_p, _c_p)
-_shared_decode = _sig("xl_shared_attn_decode", _c_p, _c_ll, *[_c_p] * 5, _c_ll, *[_c_p] * 4, *[_c_int] * 9, *[_c_f] * 3, _c_int, _c_int, _c_p, _c_p,
-                      _c_int, _c_p, _c_p)
-_shared_decode_scratch = _sig("xl_shared_attn_decode_scratch", *[_c_int] * 6, restype=_c_ll)
+_shared_decode = _sig("xl_shared_attn_decode", _c_p, _c_ll, *[_c_p] * 5, _c_ll, *[_c_p] * 4, *[_c_int] * 9, *[_c_f] * 3, _c_int, _c_p, _c_int, _c_p, _c_p)
+_shared_decode_scratch = _sig("xl_shared_attn_decode_scratch", *[_c_int] * 4, restype=_c_ll)
 _take_beams = _sig("xl_take_beams", *[_c_p] * 14, *[_c_int] * 5, _c_d, *[_c_int] * 5, _c_p)
 _take_beams_parts = _sig("xl_take_beams_parts", _c_int, _c_int, _c_int)
 _reorder = _sig("xl_reorder", ctypes.POINTER(_c_ll), _c_int, *[_c_p] * 3, _c_int, _c_int, _c_p)
@@ -46,13 +44,11 @@ def window_attention_shared_cuda(proj, q_norm, k_norm, kc, vc, pos, count, lead,
 
     if (dt == torch.bfloat16 and dim <= 128 and vdim <= 128 and dim % 8 == vdim % 8 == ld % 8 == ldo % 8 == 0
             and all(t.data_ptr() % 16 == 0 for t in (proj, joint, kc, vc))):
-        if T == 1 and B <= MAX_SHARED_BATCH:
-            units = B * G * -(-(heads // G) // 8)
-            splits = _decode_slices(units, min(smax, window + keep_first) if window else smax, 320, dev)
+        if T == 1:
             ctas = _sms(dev)
-            scratch = workspace(_shared_decode_scratch(B, heads, G, vdim, ctas, splits) * 4, dev, "shared attention")
+            scratch = workspace(_shared_decode_scratch(B, heads, vdim, ctas) * 4, dev, "shared attention")
             rc = _shared_decode(proj.data_ptr(), ld, *norms, *caches, joint.data_ptr(), ldo, *where, B, heads, G, dim, vdim, smax, window, keep_first,
-                                int(gated), scale, sink, eps, ctas, splits, scratch.data_ptr(), counters(units, dev, "counters shared").data_ptr(),
+                                int(gated), scale, sink, eps, ctas, scratch.data_ptr(),
                                 int(ahead and read_ahead.allowed(pos, count, lead, shared, kc, vc)), gemm_error_flag(dev).data_ptr(), s)
             if _launched(rc, "shared_attn_prefix"):
                 _count("shared_attn_decode")

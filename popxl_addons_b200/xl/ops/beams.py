@@ -21,7 +21,7 @@ from .sequence import _rms
 from .serving import _expect
 
 MAX_BEAMS = 32          # of a group
-MAX_SHARED_BATCH = 1024  # sequences of one attention over shared prefixes
+MAX_SHARED_BATCH = 512  # sequences of one attention over shared prefixes
 
 
 class BeamState(NamedTuple):
