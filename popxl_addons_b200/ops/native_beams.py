@@ -3,20 +3,25 @@ import ctypes
 
 import torch
 
-from ..xl import read_ahead
 from ..xl.opdef import native
-from .native import _CODE, _c_f, _c_int, _c_ll, _c_p, _count, _ok, _sig, _sms, _stream, counters, gemm_error_flag, workspace
+from .native import _CODE, _c_f, _c_int, _c_ll, _c_p, _count, _sig, _sms, _stream, counters, gemm_error_flag, workspace
 from .native_sequence import _f32, _i32, _ptr
 from .native_serving import _c_d, _done, _launched, _rows16
 
 _shared_append = _sig("xl_shared_append", _c_p, _c_ll, *[_c_p] * 7, *[_c_int] * 7, _c_f, _c_int, _c_p)
 _shared_general = _sig("xl_shared_attn_general", *[_c_p] * 4, _c_ll, _c_p, _c_ll, *[_c_p] * 4, *[_c_int] * 9, _c_f, _c_f, _c_int, _c_p)
 _shared_portion = _sig("xl_shared_attn_portion", _c_p, _c_ll, *[_c_p] * 4, _c_ll, *[_c_p] * 4, *[_c_int] * 10, *[_c_f] * 3, _c_p, _c_p)
-_shared_decode = _sig("xl_shared_attn_decode", _c_p, _c_ll, *[_c_p] * 5, _c_ll, *[_c_p] * 4, *[_c_int] * 9, *[_c_f] * 3, _c_int, _c_p, _c_int, _c_p, _c_p)
-_shared_decode_scratch = _sig("xl_shared_attn_decode_scratch", *[_c_int] * 4, restype=_c_ll)
+_shared_groups = _sig("xl_shared_attn_groups", _c_p, _c_ll, *[_c_p] * 4, _c_ll, *[_c_p] * 4, *[_c_int] * 10, *[_c_f] * 3, _c_int, _c_p, _c_p, _c_p)
+_shared_groups_scratch = _sig("xl_shared_attn_groups_scratch", *[_c_int] * 5, restype=_c_ll)
 _take_beams = _sig("xl_take_beams", *[_c_p] * 14, *[_c_int] * 5, _c_d, *[_c_int] * 5, _c_p)
 _take_beams_parts = _sig("xl_take_beams_parts", _c_int, _c_int, _c_int)
 _reorder = _sig("xl_reorder", ctypes.POINTER(_c_ll), _c_int, *[_c_p] * 3, _c_int, _c_int, _c_p)
+
+
+def _shared_few_rows(B, T, heads, G) -> bool:
+    """Whether a portion of T tokens runs on the kernel that reads shared keys once for a group, and leaves parts of sums in memory, and not on the one
+    that has whole tiles of a sequence's rows and no parts."""
+    return T == 1
 
 
 @native("window_attention_shared_")
@@ -29,7 +34,6 @@ def window_attention_shared_cuda(proj, q_norm, k_norm, kc, vc, pos, count, lead,
         return NotImplemented
     if not (proj.is_cuda and joint.is_cuda and kc.is_cuda and vc.is_cuda and kc.is_contiguous() and vc.is_contiguous()) or joint.stride(1) != 1:
         return NotImplemented
-    ahead = _ok(q_norm, k_norm)  # (a copy of the factors would be a launch of its own, which is not counted)
     q_norm, k_norm = _rows16(q_norm), _rows16(k_norm)
     gated = proj.shape[1] > plain
     code, s, ld, ldo = _CODE[dt], _stream(), proj.stride(0), joint.stride(0)
@@ -44,19 +48,16 @@ def window_attention_shared_cuda(proj, q_norm, k_norm, kc, vc, pos, count, lead,
 
     if (dt == torch.bfloat16 and dim <= 128 and vdim <= 128 and dim % 8 == vdim % 8 == ld % 8 == ldo % 8 == 0
             and all(t.data_ptr() % 16 == 0 for t in (proj, joint, kc, vc))):
-        if T == 1:
-            ctas = _sms(dev)
-            scratch = workspace(_shared_decode_scratch(B, heads, vdim, ctas) * 4, dev, "shared attention")
-            rc = _shared_decode(proj.data_ptr(), ld, *norms, *caches, joint.data_ptr(), ldo, *where, B, heads, G, dim, vdim, smax, window, keep_first,
-                                int(gated), scale, sink, eps, ctas, scratch.data_ptr(),
-                                int(ahead and read_ahead.allowed(pos, count, lead, shared, kc, vc)), gemm_error_flag(dev).data_ptr(), s)
-            if _launched(rc, "shared_attn_prefix"):
-                _count("shared_attn_decode")
-                return joint
         if not _launched(append(None), "shared_append"):
             return NotImplemented
-        rc = _shared_portion(proj.data_ptr(), ld, norms[0], *caches, joint.data_ptr(), ldo, *where, *sizes, window, keep_first, int(gated), scale, sink,
-                             eps, gemm_error_flag(dev).data_ptr(), s)
+        args = (proj.data_ptr(), ld, norms[0], *caches, joint.data_ptr(), ldo, *where, *sizes, window, keep_first, int(gated), scale, sink, eps)
+        flag = gemm_error_flag(dev).data_ptr()
+        if _shared_few_rows(B, T, heads, G):
+            scratch = workspace(_shared_groups_scratch(B, T, heads, vdim, _sms(dev)) * 4, dev, "shared attention")
+            if _launched(_shared_groups(*args, _sms(dev), scratch.data_ptr(), flag, s), "shared_attn_groups"):
+                _count("shared_attn_sum")
+                return joint
+        rc = _shared_portion(*args, flag, s)
         if rc >= 0:
             _done(rc, "shared_attn_portion")
             return joint

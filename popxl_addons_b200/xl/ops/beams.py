@@ -21,7 +21,6 @@ from .sequence import _rms
 from .serving import _expect
 
 MAX_BEAMS = 32          # of a group
-MAX_SHARED_BATCH = 512  # sequences of one attention over shared prefixes
 
 
 class BeamState(NamedTuple):
@@ -176,8 +175,6 @@ def window_attention_shared_(proj: Tensor, q_norm: Tensor, k_norm: Tensor, k_cac
         raise ValueError(f"the attention kernels take dim and vdim up to 512, not {dim} and {vdim}")
     if heads < 1 or heads % G:
         raise ValueError(f"heads ({heads}) must be a multiple of the cache's {G} heads")
-    if B > MAX_SHARED_BATCH:
-        raise ValueError(f"at most {MAX_SHARED_BATCH} sequences, not {B}")
     plain = (heads + G) * dim + G * vdim
     if T < 1 or proj.rank != 2 or proj.shape[0] != B * T or proj.shape[1] not in (plain, plain + heads * vdim):
         raise ValueError(f"projections of {B} sequences x {T} tokens are ({B * T}, {plain}) or, with gates, ({B * T}, "

@@ -167,7 +167,7 @@ def test_refusals_of_attention():
         for bad in (dict(cols=100), dict(heads=3), dict(scale=0.0), dict(window=-1), dict(keep_first=-1), dict(joint=var((3, 90))), dict(joint=var((2, 96))),
                     dict(norm=var((15,))), dict(norm=var((16,), xl.bfloat16)), dict(vcache=var((3, 2, 29, 24))), dict(vcache=var((3, 2, 30, 24), xl.bfloat16)),
                     dict(places=[var((3,), xl.int32)] * 3 + [var((2,), xl.int32)]), dict(places=[var((3,))] * 4), dict(d=520), dict(v=520), dict(T=0),
-                    dict(joint=var((3, 96), xl.bfloat16)), dict(B=513)):
+                    dict(joint=var((3, 96), xl.bfloat16))):
             with pytest.raises(ValueError):
                 call(**bad)
 
