@@ -186,10 +186,13 @@ __device__ __forceinline__ uint64_t first_desc(uint32_t addr, uint32_t lbo_bytes
   return d;
 }
 
-// S_m = Q K^T, both halves of the queries
-template <int DK> __device__ __forceinline__ void issue_score_product(uint32_t tmem_s, uint32_t q_addr, uint32_t k_addr) {
-  // bf16 operands, fp32 accumulator, both K-major, N = BKV
-  constexpr uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BKV >> 3) << 17) | ((uint32_t)(TILE_M >> 4) << 24);
+// steps of 16 keys that a block of `keys` has
+__device__ __forceinline__ int key_steps(int keys) { return (min(keys, BKV) + UMMA_K - 1) / UMMA_K; }
+
+// S_m = Q K^T, both halves of the queries, for `steps` times 16 keys
+template <int DK> __device__ __forceinline__ void issue_score_product(uint32_t tmem_s, uint32_t q_addr, uint32_t k_addr, int steps) {
+  // bf16 operands, fp32 accumulator, both K-major, N = 16 steps
+  const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(2 * steps) << 17) | ((uint32_t)(TILE_M >> 4) << 24);
   const uint64_t dq = first_desc(q_addr, 16), dk = first_desc(k_addr, 16);
 #pragma unroll
   for (int half = 0; half < 2; ++half)
@@ -201,17 +204,19 @@ template <int DK> __device__ __forceinline__ void issue_score_product(uint32_t t
                         dk + ((kb * (BKV * 128) + k * (UMMA_K * 2)) >> 4), idesc, (half | kb | k) ? 1u : 0u);
 }
 
-// O_m (+)= P V, both halves of the weights
-template <int VD> __device__ __forceinline__ void issue_value_product(uint32_t tmem_o, uint32_t tmem_p, uint32_t v_addr, bool add) {
+// O_m (+)= P V, both halves of the weights, over `steps` times 16 keys
+template <int VD> __device__ __forceinline__ void issue_value_product(uint32_t tmem_o, uint32_t tmem_p, uint32_t v_addr, bool add, int steps) {
   // A (P) from TMEM, B (V) MN-major (bit 16), N = VD
   constexpr uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(VD >> 3) << 17) | ((uint32_t)(TILE_M >> 4) << 24);
   const uint64_t dv = first_desc(v_addr, 8192);
 #pragma unroll
-  for (int half = 0; half < 2; ++half)
+  for (int k = 0; k < BKV / UMMA_K; ++k) {
+    if (k == steps) break;
 #pragma unroll
-    for (int k = 0; k < BKV / UMMA_K; ++k)
+    for (int half = 0; half < 2; ++half)
       tcgen05_mma_f16_ts(tmem_o, tmem_p + (k >> 1) * 32 + half * 16 + (k & 1) * (UMMA_K / 2),
                          dv + (((k >> 2) * (VD / 64) * 8192 + (k & 3) * (UMMA_K * 128)) >> 4), idesc, (add || half || k) ? 1u : 0u);
+  }
 }
 
 // the lowest n bits (n may be anything)
@@ -222,9 +227,9 @@ __device__ __forceinline__ uint32_t visible_bits(int key0, int w, int end, int l
   return low_bits(end - k) & (~low_bits(lo - k) | low_bits(keep - k));
 }
 
-// Which keys of a block a row sees, if not all; `unknown`: keys whose scores are not numbers, by 32 of them, or null.
+// Which keys of a block a row sees; `unknown`: keys whose scores are not numbers, by 32 of them, or null.
 struct RowMask {
-  bool cut;
+  bool cut;  // some row of the warp does not see them all: the same for all lanes, which vote where it holds
   int key0, end, lo, keep;
   const uint32_t* unknown;
 };
@@ -237,11 +242,15 @@ __device__ __forceinline__ void masked_scores(uint32_t taddr, const RowMask& mas
 #pragma unroll
   for (int i = 0; i < 32; ++i) s[i] = __uint_as_float(raw[i]);
   if (mask.cut) {
-    const uint32_t visible = visible_bits(mask.key0, w, mask.end, mask.lo, mask.keep), unknown = mask.unknown ? mask.unknown[w] : 0u;
+    const uint32_t visible = visible_bits(mask.key0, w, mask.end, mask.lo, mask.keep);
+    if (mask.unknown) {
+      const uint32_t unknown = mask.unknown[w];
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      s[i] = unknown >> i & 1 ? NAN : s[i];
-      s[i] = visible >> i & 1 ? s[i] : -INFINITY;
+      for (int i = 0; i < 32; ++i) s[i] = unknown >> i & 1 ? NAN : s[i];
+    }
+    if (!__all_sync(0xffffffffu, visible == 0xffffffffu)) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) s[i] = visible >> i & 1 ? s[i] : -INFINITY;
     }
   }
 }
@@ -250,10 +259,10 @@ __device__ __forceinline__ void masked_scores(uint32_t taddr, const RowMask& mas
 // rounding errors. mx, l: running maximum and sum; c = scale * log2(e). Returns the factor of what O holds: the maximum moves only when an exponent
 // would exceed 2^8, as a rule with the first scores of a row, and then what is stored of the block follows. A short loop: a row of 128 scores in
 // registers took 1500 instructions, whose first run cost 6000 cycles.
-__device__ __forceinline__ float weigh(uint32_t tmem_s, const RowMask& mask, float& mx, float& l, float c) {
+__device__ __forceinline__ float weigh(uint32_t tmem_s, const RowMask& mask, int steps, float& mx, float& l, float c) {
   float alpha = 1.f, sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
-  for (int w = 0; w < BKV / 32; ++w) {
+  for (int w = 0; w < (steps + 1) / 2; ++w) {  // (scores behind the steps are those of another block: masked)
     float s[32];
     masked_scores(tmem_s, mask, w, s);
     float top[4] = {s[0], s[1], s[2], s[3]};  // chains of their own
@@ -323,6 +332,15 @@ template <int VD> __device__ __forceinline__ void clear_value_row(uint8_t* tile,
   for (int jn = 0; jn < VD / 64; ++jn)
 #pragma unroll 4
     for (int i = 0; i < 8; ++i) *value_piece<VD>(tile, r, jn, i) = make_uint4(0u, 0u, 0u, 0u);
+}
+// The rows of a block of `keys` keys that the product's last step reads behind them, by the 128 threads of a warpgroup.
+template <int VD> __device__ __forceinline__ void clear_step_rest(uint8_t* tile, int keys, int thread) {
+  const int rows = key_steps(keys) * UMMA_K - keys;
+#pragma unroll 1
+  for (int i = thread; i < rows * (VD / 8); i += 128) {
+    const int r = keys + i / (VD / 8), piece = i % (VD / 8);
+    *value_piece<VD>(tile, r, piece >> 3, piece & 7) = make_uint4(0u, 0u, 0u, 0u);
+  }
 }
 template <int VD> __device__ __forceinline__ bool finite_value_row(uint8_t* tile, int r) {
   bool finite = true;
@@ -478,7 +496,8 @@ __global__ void __launch_bounds__(SA_THREADS, 1)
         if (j > 0 && !bar_wait(&pv_done[m], (uint32_t)(j - 1) & 1u, abort_flag, p.err, ERR_PV)) return false;
         tcgen05_fence_after();
         const int st = 2 * j % SLOTS;
-        issue_score_product<DK>(tmem_base + m * BKV, smem_u32(sQ + m * L::Q_BYTES), smem_u32(ring + st * L::SLOT));
+        const KeyRange x = key_block(keys, j);
+        issue_score_product<DK>(tmem_base + m * BKV, smem_u32(sQ + m * L::Q_BYTES), smem_u32(ring + st * L::SLOT), key_steps(x.end - x.begin));
         if (m == tiles - 1) tcgen05_commit(&empty[st]);
         tcgen05_commit(&s_full[m]);
         return true;
@@ -487,12 +506,14 @@ __global__ void __launch_bounds__(SA_THREADS, 1)
       for (int m = 0; m < tiles && ok; ++m) ok = issue_scores(0, m);
       for (int j = 0; j < n_kv && ok; ++j) {
         const int st = (2 * j + 1) % SLOTS;
+        const KeyRange x = key_block(keys, j);
+        const int steps = key_steps(x.end - x.begin);
         ok = wait_full(2 * j + 1);
         for (int m = 0; m < tiles && ok; ++m) {
           ok = bar_wait(&p_full[m], (uint32_t)j & 1u, abort_flag, p.err, ERR_P);
           if (!ok) break;
           tcgen05_fence_after();
-          issue_value_product<VD>(tmem_base + 2 * BKV + m * VD, tmem_base + m * BKV, smem_u32(ring + st * L::SLOT), j > 0);
+          issue_value_product<VD>(tmem_base + 2 * BKV + m * VD, tmem_base + m * BKV, smem_u32(ring + st * L::SLOT), j > 0, steps);
           if (m == tiles - 1) tcgen05_commit(&empty[st]);
           tcgen05_commit(&pv_done[m]);
           if (j + 1 < n_kv) ok = issue_scores(j + 1, m);
@@ -529,14 +550,15 @@ __global__ void __launch_bounds__(SA_THREADS, 1)
         const int n = 2 * j + 1;
         ok = bar_wait_warp(&full[n % SLOTS], (uint32_t)(n / SLOTS) & 1u, abort_flag, p.err, ERR_KV_FULL);
         if (!ok) break;
-        if (col0 + r >= x.end) clear_value_row<VD>(ring + n % SLOTS * L::SLOT, r);
+        clear_step_rest<VD>(ring + n % SLOTS * L::SLOT, x.end - col0, r);
         fence_proxy_async_smem();
       }
       ok = bar_wait_warp(&s_full[m], (uint32_t)j & 1u, abort_flag, p.err, ERR_S);
       if (!ok) break;
       tcgen05_fence_after();
-      const RowMask mask{col0 + BKV - 1 > hi || (col0 < lo && col0 + BKV > p.keep_first), col0, hi + 1, lo, p.keep_first, nullptr};
-      const float alpha = weigh(tmem_s, mask, mx, l, c);
+      const bool cut = __any_sync(0xffffffffu, col0 + BKV - 1 > hi || (col0 < lo && col0 + BKV > p.keep_first));  // for all lanes alike
+      const RowMask mask{cut, col0, hi + 1, lo, p.keep_first, nullptr};
+      const float alpha = weigh(tmem_s, mask, key_steps(x.end - col0), mx, l, c);
       // the scores of block j are only computed after P V of block j - 1: O is at rest here
       if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) rescale_output<VD>(tmem_o, alpha);
       tmem_st_wait();
@@ -985,49 +1007,52 @@ __global__ void __launch_bounds__(SA_THREADS, 1)
       xl_grid_launch_dependents();  // TMEM is held: a successor that allocates some on this SM cannot come first
       auto wait_full = [&](int n) { return bar_wait(&full[n % SLOTS], (uint32_t)(n / SLOTS) & 1u, abort_flag, p.err, ERR_KV_FULL); };
       // block `it` of this CTA: warpgroup it & 1, its block it >> 1
-      auto issue_scores = [&](int it, int half) -> bool {
+      auto issue_scores = [&](int it, int half, int steps) -> bool {
         const int m = it & 1, st = 2 * it % SLOTS;
         if (!wait_full(2 * it)) return false;
         // the buffer still holds P of the warpgroup's previous block until its product has been taken
         if (it >= 2 && !bar_wait(&pv_done[m], (uint32_t)((it >> 1) - 1) & 1u, abort_flag, p.err, ERR_PV)) return false;
         tcgen05_fence_after();
-        issue_score_product<DK>(tmem_base + m * BKV, smem_u32(sQ) + half * PF_HALF * 128, smem_u32(ring + st * L::SLOT));
+        issue_score_product<DK>(tmem_base + m * BKV, smem_u32(sQ) + half * PF_HALF * 128, smem_u32(ring + st * L::SLOT), steps);
         tcgen05_commit(&empty[st]);
         tcgen05_commit(&s_full[m]);
         return true;
       };
-      auto issue_values = [&](int it, bool add) -> bool {
+      auto issue_values = [&](int it, bool add, int steps) -> bool {
         const int m = it & 1, st = (2 * it + 1) % SLOTS;
         if (!wait_full(2 * it + 1)) return false;
         if (!bar_wait(&p_full[m], (uint32_t)(it >> 1) & 1u, abort_flag, p.err, ERR_P)) return false;
         tcgen05_fence_after();
-        issue_value_product<VD>(tmem_base + 2 * BKV + m * VD, tmem_base + m * BKV, smem_u32(ring + st * L::SLOT), add);
+        issue_value_product<VD>(tmem_base + 2 * BKV + m * VD, tmem_base + m * BKV, smem_u32(ring + st * L::SLOT), add, steps);
         tcgen05_commit(&empty[st]);
         tcgen05_commit(&pv_done[m]);
         return true;
       };
       QueryRoom room;
       bool ok = true, add = false;
-      int it = 0;
+      int it = 0, steps = 0;
 #pragma unroll 1
   #pragma unroll 1
     for (int x = x0, sn = 0; x < x1 && ok; ++sn) {
         const GroupSegment* sg = segment(sn);
         if (!sg) break;
-        const int half = room.take(sg->rows), count = sg->count;
+        const int half = room.take(sg->rows), count = sg->count, block = sg->block;
+        const TileKeys keys = sg->keys;
         *begun = sn;
         ok = sn ? bar_wait(&q_full[half], (uint32_t)room.used(half) & 1u, abort_flag, p.err, ERR_Q) : bar_wait(q_first, 0, abort_flag, p.err, ERR_Q);
 #pragma unroll 1
         for (int j = 0; j < count && ok; ++j, ++it) {
-          ok = issue_scores(it, half);
+          const int now = key_steps(keys.until(block + j) - keys.key(block + j));
+          ok = issue_scores(it, half, now);
           if (ok && j + 1 == count) tcgen05_commit(&q_empty[half]);
-          if (ok && it) ok = issue_values(it - 1, add);
+          if (ok && it) ok = issue_values(it - 1, add, steps);
           add = j >= 2;  // of this block: the warpgroup has had one of this segment
+          steps = now;
         }
         if (sn) room.count(half);
         x += count;
       }
-      if (ok && it) issue_values(it - 1, add);
+      if (ok && it) issue_values(it - 1, add, steps);
     }
   } else if (warp == 2) {  // the first tile's queries are the softmax warps' work
     QueryRoom room;
@@ -1148,14 +1173,14 @@ __global__ void __launch_bounds__(SA_THREADS, 1)
         // not every row sees every key; and, of a group, not all rows see the same ones
         const bool cut = key0 + BKV > end || key0 + BKV > sg.least || (key0 < sg.latest && key0 + BKV > p.keep_first);
         const bool uneven = cut && !sg.own && (min(key0 + BKV, end) > sg.least || (key0 < sg.latest && key0 + BKV > p.keep_first));
-        if (cut && (uneven || key0 + BKV > end)) {  // thread r looks at the value of key r
+        if (uneven || (end - key0 < BKV && (end - key0) % UMMA_K)) {
           const int n = 2 * it + 1;
           ok = bar_wait_warp(&full[n % SLOTS], (uint32_t)(n / SLOTS) & 1u, abort_flag, p.err, ERR_KV_FULL);
           if (!ok) break;
           uint8_t* tile = ring + n % SLOTS * L::SLOT;
-          const bool beyond = key0 + r >= end;  // nobody sees it
-          const bool finite = !uneven || beyond || finite_value_row<VD>(tile, r);
-          if (!finite || beyond) clear_value_row<VD>(tile, r);
+          if (end - key0 < BKV) clear_step_rest<VD>(tile, end - key0, r);
+          const bool finite = !uneven || key0 + r >= end || finite_value_row<VD>(tile, r);  // thread r looks at the value of key r
+          if (!finite) clear_value_row<VD>(tile, r);
           fence_proxy_async_smem();
           if (uneven) {
             const unsigned int bits = __ballot_sync(0xffffffffu, !finite);
@@ -1166,7 +1191,7 @@ __global__ void __launch_bounds__(SA_THREADS, 1)
         }
         if (warp_on) {
           const RowMask mask{cut, key0, min(end, edge), lo, p.keep_first, uneven ? unknown + m * 4 : nullptr};
-          const float alpha = weigh(tmem_s, mask, mx, l, c);
+          const float alpha = weigh(tmem_s, mask, key_steps(end - key0), mx, l, c);
           // the scores of a block are only computed after P V of the warpgroup's block before: O is at rest here
           if (mine && __any_sync(0xffffffffu, alpha != 1.f)) rescale_output<VD>(tmem_o, alpha);
           tmem_st_wait();
