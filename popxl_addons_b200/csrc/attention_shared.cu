@@ -634,8 +634,8 @@ template <int DK, int VD> int launch_portion(const void* kc, const void* vc, con
 // (shared_attn_sum_kernel) adds the parts.
 //   warp 0       TMA: key and value tiles in turn through one ring
 //   warp 1       MMA: S_m = Q K^T, O_m += P_m V
-//   warps 2, 3   queries of the next tile, normalised, from the projections to shared memory; tiles of up to 64 rows take halves of the room in turn
-//   warps 4..7, 8..11   softmax of every second block; warps without rows only keep step
+//   warp 2       queries of the next tile, if they are few, normalised, from the projections to shared memory;  warp 3  the list of this CTA's tiles
+//   warps 4..7, 8..11   queries of large tiles; softmax of every second block (warps without rows only keep step)
 //
 // Every CTA makes the list by itself, from positions and leads in shared memory: counts, key ranges and offsets by slot, ranks of the members by
 // votes. CTA 0 leaves a copy for the kernel behind.
@@ -644,7 +644,7 @@ template <int DK, int VD> int launch_portion(const void* kc, const void* vc, con
 // the scores of its key become NaN for the rows that see it: a weight of zero times anything would reach the others.
 constexpr int PF_MAX_BATCH = 448;
 constexpr int PF_SLOTS_LARGE = 4, PF_SLOTS_SMALL = 8;
-constexpr int PF_HALF = TILE_M / 2;
+constexpr int PF_HALF = 32;  // rows of a tile whose queries one warp makes ready ahead; those of larger tiles are made by the softmax warps
 
 struct GroupPlan {  // where a sequence's parts are
   int first, blocks, tiles, row;        // first block of the group, blocks of a tile, tiles of a head, the sequence's first row in the group
@@ -734,16 +734,23 @@ __device__ __forceinline__ bool warps_meet(uint64_t* bar, uint32_t& phase, volat
   return ok;
 }
 
-// Which half of the queries' room a tile takes, and how often it was taken before: the warps that fill it and the one that uses it count alike.
+// Where a tile's queries are: small tiles take the first rows of the room and the next ones in turn, so that one can be made ready while the other is in
+// use; a large tile takes all of it, under number 0, and so does a CTA's first one. Everybody counts alike.
 struct QueryRoom {
-  int next = 0, first = 0, second = 0;  // how often each was taken
-  __device__ __forceinline__ int take(int rows) {  // 0 or 1; a tile of more than half takes both, under number 0
-    const int h = rows > PF_HALF ? 0 : next;
-    next = rows > PF_HALF ? 0 : next ^ 1;
+  int next = 0, used0 = 0, used1 = 0;           // how often each place was taken
+  int ahead0 = 0, ahead1 = 0, at_once = 0;      // and was filled ahead, or the room at once
+  bool large = false;                           // of the tile that took it last
+  __device__ __forceinline__ int take(int rows, bool first) {
+    large = first || rows > PF_HALF;
+    const int h = large ? 0 : next;
+    next = large ? (rows > PF_HALF ? 0 : 1) : next ^ 1;
     return h;
   }
-  __device__ __forceinline__ int used(int h) const { return h ? second : first; }
-  __device__ __forceinline__ void count(int h) { h ? ++second : ++first; }
+  __device__ __forceinline__ void count(int h) {
+    h ? ++used1 : ++used0;
+    if (large) ++at_once;
+    else h ? ++ahead1 : ++ahead0;
+  }
 };
 
 template <int DK, int VD>
@@ -763,7 +770,7 @@ __global__ void __launch_bounds__(SA_THREADS, 1)
   uint64_t* p_full = bars + 6;   // [2]
   uint64_t* pv_done = bars + 8;  // [2]
   uint64_t* wg_meet = bars + 10;  // [2]
-  uint64_t* q_first = bars + 12;  // the first tile's queries
+  uint64_t* q_large = bars + 12;  // queries of large tiles
   uint64_t* full = bars + 14;     // [SLOTS]
   uint64_t* empty = bars + 14 + SLOTS;
   uint32_t* tmem_base_slot = (uint32_t*)(bars + 14 + 2 * SLOTS);
@@ -798,7 +805,7 @@ __global__ void __launch_bounds__(SA_THREADS, 1)
       mbar_init(&pv_done[s], 1);
       mbar_init(&wg_meet[s], 4);
     }
-    mbar_init(q_first, 8);
+    mbar_init(q_large, 8);
     for (int s = 0; s < 2 * SLOTS; ++s) mbar_init(&full[s], 1);
     *ready = *begun = 0;
     *abort_flag = 0;
@@ -1029,52 +1036,57 @@ __global__ void __launch_bounds__(SA_THREADS, 1)
         return true;
       };
       QueryRoom room;
-      bool ok = true, add = false;
+      bool ok = true, add = false, pending = false;  // pending: block it - 1 has no product with the values yet
       int it = 0, steps = 0;
 #pragma unroll 1
   #pragma unroll 1
     for (int x = x0, sn = 0; x < x1 && ok; ++sn) {
         const GroupSegment* sg = segment(sn);
         if (!sg) break;
-        const int half = room.take(sg->rows), count = sg->count, block = sg->block;
+        const int half = room.take(sg->rows, sn == 0), count = sg->count, block = sg->block;
         const TileKeys keys = sg->keys;
         *begun = sn;
-        ok = sn ? bar_wait(&q_full[half], (uint32_t)room.used(half) & 1u, abort_flag, p.err, ERR_Q) : bar_wait(q_first, 0, abort_flag, p.err, ERR_Q);
+        if (room.large && pending) {  // the warps that make these queries ready end their last tile first
+          ok = issue_values(it - 1, add, steps);
+          pending = false;
+          if (!ok) break;
+        }
+        ok = room.large ? bar_wait(q_large, (uint32_t)room.at_once & 1u, abort_flag, p.err, ERR_Q)
+                        : bar_wait(&q_full[half], (uint32_t)(half ? room.ahead1 : room.ahead0) & 1u, abort_flag, p.err, ERR_Q);
 #pragma unroll 1
         for (int j = 0; j < count && ok; ++j, ++it) {
           const int now = key_steps(keys.until(block + j) - keys.key(block + j));
           ok = issue_scores(it, half, now);
           if (ok && j + 1 == count) tcgen05_commit(&q_empty[half]);
-          if (ok && it) ok = issue_values(it - 1, add, steps);
+          if (ok && pending) ok = issue_values(it - 1, add, steps);
+          pending = true;
           add = j >= 2;  // of this block: the warpgroup has had one of this segment
           steps = now;
         }
-        if (sn) room.count(half);
+        room.count(half);
         x += count;
       }
-      if (ok && it) issue_values(it - 1, add, steps);
+      if (ok && pending) issue_values(it - 1, add, steps);
     }
-  } else if (warp == 2) {  // the first tile's queries are the softmax warps' work
+  } else if (warp == 2) {  // queries of small tiles
     QueryRoom room;
     bool ok = true;
 #pragma unroll 1
     for (int x = x0, sn = 0; x < x1; ++sn) {
       const GroupSegment* sg = segment(sn);
       if (!sg) break;
-      const int half = room.take(sg->rows);
-      if (sn) {
-        // the products that used the room before: of this half, or of both. (The first tile's were the first of half 0. Half 1 comes behind a small tile in
-        // half 0, whose wait was for a large one's products.)
-        if (half == 0) ok = bar_wait_warp(&q_empty[0], (uint32_t)room.first & 1u, abort_flag, p.err, ERR_Q);
-        if (ok && (half == 1 || sg->rows > PF_HALF) && room.second)
-          ok = bar_wait_warp(&q_empty[1], (uint32_t)(room.second - 1) & 1u, abort_flag, p.err, ERR_Q);
+      const int half = room.take(sg->rows, sn == 0);
+      if (!room.large) {
+        // The products that used the place before. (Place 1 comes behind a small tile in place 0, whose wait was for a large one's products.)
+        const int used = half ? room.used1 : room.used0;
+        if (used) ok = bar_wait_warp(&q_empty[half], (uint32_t)(used - 1) & 1u, abort_flag, p.err, ERR_Q);
         if (!ok) break;
         fill_queries(*sg, half, 0, 1);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&q_full[half]);
-        room.count(half);
       }
+      room.count(half);
       x += sg->count;
     }
   } else if (warp == 3) {  // the table of this CTA's segments
@@ -1136,18 +1148,24 @@ __global__ void __launch_bounds__(SA_THREADS, 1)
     const float c = p.scale * 1.4426950408889634f;
     bool ok = true;
     uint32_t met = 0;
-    if (const GroupSegment* sg = segment(0)) {
-      fill_queries(*sg, 0, warp - 4, 8);
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(q_first);
-    }
+    QueryRoom room;
 #pragma unroll 1
     for (int x = x0, sn = 0; x < x1 && ok; ++sn) {
       const GroupSegment* at_table = segment(sn);
       if (!at_table) break;
       const GroupSegment sg = *at_table;
       const TileKeys& keys = sg.keys;
+      const int half = room.take(sg.rows, sn == 0);
+      if (room.large) {
+        if (room.used0) ok = bar_wait_warp(&q_empty[0], (uint32_t)(room.used0 - 1) & 1u, abort_flag, p.err, ERR_Q);
+        if (ok && room.used1) ok = bar_wait_warp(&q_empty[1], (uint32_t)(room.used1 - 1) & 1u, abort_flag, p.err, ERR_Q);
+        if (!ok) break;
+        fill_queries(sg, 0, warp - 4, 8);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(q_large);
+      }
+      room.count(half);
       // row r: its sequence and position; the keys that it sees end at `edge` and begin with its window at `lo`
       const int at_row = sg.tile * TILE_M + r, member = sg.own ? 0 : small_quotient(at_row, M);
       bool row_on = r < sg.rows;
@@ -1259,7 +1277,12 @@ __global__ void __launch_bounds__(128) shared_attn_sum_kernel(const GroupParams 
     gate = *reinterpret_cast<const uint2*>(p.proj + (long long)row * p.ld + (long long)(p.H + p.G) * p.dim + (long long)p.G * p.vdim +
                                            (long long)h * p.vdim + c);
   if (t >= n || !window_fits(pos, n, p.T, p.Smax)) return;
-  const XlRanges ranges{pb.y / pb.z, pb.y % pb.z};  // (there are blocks: the row's own key is among them)
+  const int per = pb.y / pb.z;  // (there are blocks: the row's own key is among them)
+  const XlRanges ranges{per, pb.y - per * pb.z};
+  auto owner = [&](int x) {  // ranges.owner(x)
+    const int head = ranges.rem * (per + 1);
+    return x < head ? small_quotient(x, per + 1) : ranges.rem + small_quotient(x - head, per);
+  };
   const float sink = p.sink * 1.4426950408889634f;
   // two sources: the tile of the group and the tile of the sequence; of each one CTA's part for each warpgroup from its first block on, then those of
   // the CTAs that follow
@@ -1270,8 +1293,8 @@ __global__ void __launch_bounds__(128) shared_attn_sum_kernel(const GroupParams 
   for (int k = 0; k < 2; ++k)
     if (blocks[k]) {
       const int tiles = k ? (M + TILE_M - 1) / TILE_M : pa.z, x = (k ? pc.x : pa.x) + (g * tiles + idx[k] / TILE_M) * blocks[k];
-      c0[k] = ranges.owner(x);
-      parts[k] = 2 * (ranges.owner(x + blocks[k] - 1) - c0[k] + 1);
+      c0[k] = owner(x);
+      parts[k] = 2 * (owner(x + blocks[k] - 1) - c0[k] + 1);
     }
   const int all = parts[0] + parts[1];
   auto place = [&](int k, bool& main) -> long long {
@@ -1287,10 +1310,12 @@ __global__ void __launch_bounds__(128) shared_attn_sum_kernel(const GroupParams 
   };
   float2 mine = lane < all ? stat(lane) : make_float2(-INFINITY, 0.f);  // of the first 32 parts
   float m = fmaxf(sink, mine.x);
+#pragma unroll 1
   for (int k = lane + 32; k < all; k += 32) m = fmaxf(m, stat(k).x);
   m = xl_warp_max(m);
   float total = sink == -INFINITY ? 0.f : exp2f(sink - m);
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
   for (int k0 = 0; k0 < all; k0 += 32) {
     if (k0) mine = k0 + lane < all ? stat(k0 + lane) : make_float2(-INFINITY, 0.f);
     const float f = mine.x == -INFINITY ? 0.f : exp2f(mine.x - m);
