@@ -252,6 +252,10 @@ class Dunelix:
                 out[f"run{r}.v"] = ((batch, m.kv_heads, max_seq, m.vdim), self.dtype)
         return out
 
+    def state_positions(self) -> Dict[str, Tuple[Optional[int], int]]:
+        """By name of a state: its axis of positions (None: it has none) and how many of them an entry stands for."""
+        return {name: ({"k": 3, "v": 2}.get(name.rsplit(".", 1)[1]), 1) for name in self.state(1, 1)}
+
     def tables(self, max_seq: int) -> Dict[str, Any]:
         """Constant fp32 tables: cosine and sine of every rotary setting in use."""
         out = {}

@@ -12,6 +12,10 @@ and does not know the architecture:
 * **decoding**: tokens, positions and the output buffer stay on the device, so a decoding step is one graph replay.
 * **requests of their own kind**: a request may bring an adapter of the model (`load_adapter`), and what shapes its logits before a token
   is chosen (`LogitShaping`). Both are looked up by slot on the device: a batch of unlike requests is one step like any other.
+* **a beginning in common**: a request may take the first positions of another one (`admit(prefix_of=)`, of a model with `shared_prefixes`):
+  they stay where they are, and attention reads them once for all that share them.
+* **beams**: `generate_beams` keeps the best continuations of every prompt, in groups of consecutive slots. The choice and the states that
+  follow it stay on the device; what a prompt's beams have in common is shared where the model can, else copied once.
 """
 import math
 from dataclasses import dataclass
@@ -23,7 +27,14 @@ import torch
 from .. import xl
 from ..xl import ops
 
-__all__ = ["LogitShaping", "SequenceGenerator", "portion_size"]
+__all__ = ["Beam", "LogitShaping", "SequenceGenerator", "portion_size"]
+
+
+@dataclass(frozen=True)
+class Beam:
+    """A continuation of a prompt: its tokens (with the end, if it has come to it) and the sum of the logarithms of their probabilities."""
+    tokens: np.ndarray
+    score: float
 
 
 @dataclass(frozen=True)
@@ -72,15 +83,19 @@ def portion_size(n: int) -> int:
 class SequenceGenerator:
     def __init__(self, model, batch: int = 1, max_seq: int = 2048, max_portion: int = 4096, max_new_tokens: int = 256,
                  device: str = "auto", cuda_graphs: bool = True, use_native: Optional[bool] = None, shaping: bool = False,
-                 max_biases: int = 64):
+                 max_biases: int = 64, beams: int = 0):
         """`max_seq`: positions a slot can hold; `max_portion`: tokens per sequence of one step's graph (longer portions are
         run in several); `max_new_tokens`: rows of the device buffer that collects generated tokens. `shaping`: requests may bring a
-        `LogitShaping` with up to `max_biases` biases; the slots' tokens are then kept on the device."""
+        `LogitShaping` with up to `max_biases` biases; the slots' tokens are then kept on the device. `beams`: how many `generate_beams`
+        keeps of every prompt (0: none); `batch` slots are those of `batch // beams` prompts."""
         if batch < 1 or max_seq < 1:
             raise ValueError("batch and max_seq must be positive")
         if shaping and not (1 <= max_biases <= ops.MAX_BIASES and max_seq <= ops.MAX_HISTORY):
             raise ValueError(f"shaping takes between 1 and {ops.MAX_BIASES} biases and max_seq up to {ops.MAX_HISTORY}")
-        self.shaping, self.max_biases = shaping, max_biases
+        if beams and not (1 <= beams <= ops.MAX_BEAMS and batch % beams == 0):
+            raise ValueError(f"{batch} slots are not groups of {beams} beams (1 to {ops.MAX_BEAMS})")
+        self.shaping, self.max_biases, self.beams = shaping, max_biases, beams
+        self.shares = bool(getattr(model, "shared_prefixes", False))
         self.adapters = getattr(model, "adapters", 0)
         self.model, self.batch, self.max_seq = model, batch, max_seq
         self.max_portion = portion_size(min(max_portion, max_seq))
@@ -104,6 +119,11 @@ class SequenceGenerator:
                 state.update(history=((batch, max_seq), xl.int32), start=((batch,), xl.int32), penalties=((batch, 3), xl.float32),
                              bias_tokens=((batch, max_biases), xl.int32), bias_values=((batch, max_biases), xl.float32),
                              allowed=((batch, -(-model.vocab // 32)), xl.int32))
+            if self.shares:
+                state.update(lead=((batch,), xl.int32), shared=((batch,), xl.int32))
+            if beams:
+                rows = ((batch,), xl.int32)
+                state.update(scores=((batch,), xl.float32), ended=rows, length=rows, parent=rows, begin=rows, parents=((max_new_tokens, batch), xl.int32))
             for name, (shape, dt) in state.items():
                 self._vars[name] = xl.variable(xl.LazyInit(shape, np.float32, "zeros"), dt, name)
                 self._mutable.add(name)
@@ -114,6 +134,9 @@ class SequenceGenerator:
         self.lengths = [0] * batch          # positions held by every slot (host mirror of the device-side `pos`)
         self.slots: Dict[object, int] = {}  # live request -> slot
         self._free = list(range(batch))[::-1]
+        self._prefix = [(slot, 0) for slot in range(batch)]  # whose slot holds a sequence's first positions, and how many
+        self._kept: set = set()             # slots of released requests whose positions others share
+        self._adapter_of: Dict[int, Optional[int]] = {}
         if self.adapters:
             self._set_device("adapter", -1)
         if shaping:
@@ -151,9 +174,12 @@ class SequenceGenerator:
         return self
 
     # -- slots ---------------------------------------------------------------------------------------------------------
-    def admit(self, request, adapter: Optional[int] = None, shaping: Optional[LogitShaping] = None, prompt: int = 0) -> int:
+    def admit(self, request, adapter: Optional[int] = None, shaping: Optional[LogitShaping] = None, prompt: int = 0, prefix_of=None,
+              prefix: Optional[int] = None) -> int:
         """Give a request a slot; its first token will be at position 0. `adapter`: which adapter it uses (None: the model alone);
-        `shaping`: what changes its logits, of which the first `prompt` tokens count as its prompt."""
+        `shaping`: what changes its logits, of which the first `prompt` tokens count as its prompt. `prefix_of`: a live request whose first
+        `prefix` positions (None: all that it holds) are also this one's, which goes on behind them; the model must have been made with
+        `shared_prefixes`, and both have to use the same adapter."""
         if request in self.slots:
             raise ValueError(f"request {request!r} already holds a slot")
         if not self._free:
@@ -162,20 +188,56 @@ class SequenceGenerator:
             raise ValueError(f"request {request!r} asks for adapter {adapter} of {self.adapters}")
         if shaping is not None and not self.shaping:
             raise ValueError("this program was made without shaping=True")
+        lead, shared = self._lead_of(prefix_of, prefix, adapter) if prefix_of is not None else (None, 0)
         slot = self._free[-1]
         if self.shaping:
             self._write_shaping(slot, shaping or LogitShaping(), prompt)
         if self.adapters:
             self.session.device_tensor(self._vars["adapter"])[slot] = -1 if adapter is None else adapter
+        if self.adapters:
+            self._adapter_of[slot] = adapter
+        if self.shares:
+            self._share(slot, lead if shared else slot, shared)
+            if shared and self.shaping:
+                history = self.session.device_tensor(self._vars["history"])
+                history[slot, :shared].copy_(history[self.slots[prefix_of], :shared])
         self._free.pop()
         self.slots[request] = slot
-        self.lengths[slot] = 0
+        self.lengths[slot] = shared
         return slot
 
+    def _lead_of(self, request, n: Optional[int], adapter: Optional[int]):
+        """The slot that holds the first `n` positions of a live request, and `n`."""
+        if not self.shares:
+            raise ValueError("the model was made without shared prefixes")
+        if request not in self.slots:
+            raise ValueError(f"no live request {request!r} to share positions of")
+        slot = self.slots[request]
+        n = self.lengths[slot] if n is None else n
+        if not 0 <= n <= self.lengths[slot]:
+            raise ValueError(f"request {request!r} holds {self.lengths[slot]} positions, not {n}")
+        if self.adapters and self._adapter_of.get(slot) != adapter:
+            raise ValueError(f"request {request!r} uses another adapter")
+        lead, held = self._prefix[slot]
+        if held and n > held:
+            raise ValueError(f"request {request!r} shares its first {held} positions itself: no more than those can be shared on")
+        return (lead if held else slot), n
+
+    def _share(self, slot: int, lead: int, shared: int) -> None:
+        self._prefix[slot] = (lead, shared)
+        for name, value in (("lead", lead), ("shared", shared)):
+            self.session.device_tensor(self._vars[name])[slot] = value
+
     def release(self, request) -> None:
+        """Give a request's slot back; positions that others share stay until these are released too."""
         slot = self.slots.pop(request)
-        self.lengths[slot] = 0
-        self._free.append(slot)
+        self._kept.add(slot)
+        for s in (slot, self._prefix[slot][0]):
+            live = set(self.slots.values())
+            if s in self._kept and not any(lead == s and n and o in live and o != s for o, (lead, n) in enumerate(self._prefix)):
+                self._kept.discard(s)
+                self.lengths[s] = 0
+                self._free.append(s)
 
     def _write_shaping(self, slot: int, s: LogitShaping, prompt: int) -> None:
         biases = dict(s.biases or {})
@@ -216,11 +278,29 @@ class SequenceGenerator:
         else:
             ops.take_greedy_(t("current"), self.model.logits(t, h), t("generated"), t("step"), self.model.vocab)
 
+    def _choose_beams(self, t, h, first: bool, end: Optional[int], length_penalty: float):
+        """The next beams of every group become the current tokens, and their states follow. Positions have moved on already. `first`: the prompt is one
+        beam's so far, and what its other beams cannot share is copied."""
+        logits = self.model.logits(t, h)
+        if self.shaping:
+            logits = ops.shape_logits(logits, xl.constant(np.arange(self.batch), xl.int32, "slots"), t("pos"), self._rules(t))
+        ops.take_beams_(t("current"), t("parent"), logits, t("generated"), t("parents"), t("step"),
+                        ops.BeamState(t("scores"), t("ended"), t("length")), self.beams, end, self.model.vocab, length_penalty)
+        begin = xl.constant(np.zeros(self.batch), xl.int32, "begin") if first else t("begin")
+        rows = [ops.StateRows(t(name), *where) for name, where in self.model.state_positions().items()
+                if not (first and self.shares and where[0] is not None)]
+        if self.shaping:
+            rows.append(ops.StateRows(t("history"), 1))
+        ops.reorder_(rows, t("parent"), begin, t("pos"), self.beams)
+        if self.shaping:
+            ops.append_tokens_(t("history"), t("current"), t("pos"), t("count"), 1)
+
     @staticmethod
     def _rules(t) -> ops.LogitRules:
         return ops.LogitRules(*(t(k) for k in ops.LogitRules._fields))
 
-    def _portion_program(self, T: int, sample: bool):
+    def _portion_program(self, T: int, sample):
+        """`sample`: whether the portion ends in a choice; or the arguments of a first choice of beams."""
         def build(entry, t):
             entry["tokens"] = xl.h2d_stream((self.batch * T,), xl.int32, f"tokens_{T}")
             ctrl = ops.host_load(self._ctrl_in)
@@ -230,13 +310,26 @@ class SequenceGenerator:
             self.model.portion(T, t, tokens, t("pos"), t("count"), final_norm=False)
             if self.shaping:
                 ops.append_tokens_(t("history"), tokens, t("pos"), t("count"), T)
+            if self.shaping or isinstance(sample, tuple):
                 ops.advance_by_(t("pos"), t("count"))
-            if sample:
+            if isinstance(sample, tuple):
+                h = self.model.select(t, t("count"), stride=T, offset=1)
+                ops.var_updates.copy_var_update_(t("count"), xl.constant(np.ones(self.batch), xl.int32, "each"))  # from here on every beam goes on
+                self._choose_beams(t, h, True, *sample)
+            elif sample:
                 self._sample(t, self.model.select(t, t("count"), stride=T, offset=1))
-            if not self.shaping:
+            if not self.shaping and not isinstance(sample, tuple):
                 ops.advance_by_(t("pos"), t("count"))
 
-        return self._program(("portion", T, "sample") if sample else ("portion", T), build)
+        return self._program(("portion", T, "sample", *(sample if isinstance(sample, tuple) else ())) if sample else ("portion", T), build)
+
+    def _beams_program(self, end: Optional[int], length_penalty: float):
+        def build(entry, t):
+            h = self.model.portion(1, t, t("current"), t("pos"), t("count"), final_norm=True)
+            ops.advance_by_(t("pos"), t("count"))
+            self._choose_beams(t, h, False, end, length_penalty)
+
+        return self._program(("beams", end, length_penalty), build)
 
     def _decode_program(self):
         def build(entry, t):
@@ -260,7 +353,7 @@ class SequenceGenerator:
         return self._program(("logits", n, "shaped") if shaped else ("logits", n), build)
 
     # -- steps -----------------------------------------------------------------------------------------------------------
-    def _run_portion(self, part: Mapping[int, Sequence[int]], sample: bool = False) -> int:
+    def _run_portion(self, part: Mapping[int, Sequence[int]], sample=False) -> int:
         """`part`: slot -> its next tokens (at most `max_portion`). Returns the rows per sequence of the program."""
         T = portion_size(max(len(v) for v in part.values()))
         entry = self._portion_program(T, sample)
@@ -365,6 +458,89 @@ class SequenceGenerator:
             for r in slot:
                 self.release(r)
         return [np.array(got[:n_new, slot[r]], np.int32) for r in reqs]
+
+    def generate_beams(self, prompts: Sequence[Sequence[int]], max_new_tokens: int, end: Optional[int] = None, length_penalty: float = 0.0,
+                       shaping: Union[None, LogitShaping, Sequence[Optional[LogitShaping]]] = None,
+                       adapters: Optional[Sequence[Optional[int]]] = None) -> List[List[Beam]]:
+        """The best continuations of every prompt by beam search, at most `beams` of them, the best first: by the sum of the logarithms of their
+        tokens' probabilities, divided by their number to the power of `length_penalty`. A continuation ends with the token `end` (None: at
+        `max_new_tokens`). `shaping` and `adapters` as for `generate`; probabilities are those of the shaped logits."""
+        if not self.beams:
+            raise ValueError("this program was made without beams")
+        if max_new_tokens < 1 or max_new_tokens > self.max_new:
+            raise ValueError(f"max_new_tokens must be in [1, {self.max_new}]")
+        if self.slots:
+            raise RuntimeError("generate_beams() needs all slots: release the live requests first")
+        if end is not None and not 0 <= end < self.model.vocab:
+            raise ValueError(f"the end is a token below {self.model.vocab}, not {end}")
+        if any(len(p) < 1 or len(p) + max_new_tokens - 1 > self.max_seq for p in prompts):
+            raise ValueError(f"prompts must hold between 1 and {self.max_seq - max_new_tokens + 1} tokens")
+        shaping = [shaping] * len(prompts) if shaping is None or isinstance(shaping, LogitShaping) else list(shaping)
+        adapters = [None] * len(prompts) if adapters is None else list(adapters)
+        if not len(shaping) == len(adapters) == len(prompts):
+            raise ValueError(f"{len(prompts)} prompts need as many shapings and adapters")
+        out: List[List[Beam]] = []
+        groups = self.batch // self.beams
+        for lo in range(0, len(prompts), groups):
+            hi = lo + groups
+            out += self._beams_of_batch(prompts[lo:hi], max_new_tokens, end, float(length_penalty), shaping[lo:hi], adapters[lo:hi])
+        return out
+
+    def _beams_of_batch(self, prompts, n_new: int, end, length_penalty: float, shaping, adapters) -> List[List[Beam]]:
+        K, n = self.beams, len(prompts)
+        self._free = list(range(self.batch))[::-1]  # groups are consecutive slots
+        try:
+            for g in range(n):
+                for k in range(K):
+                    self.admit((g, k), adapters[g], shaping[g], len(prompts[g]))
+            # the prompt is read by the first beam of its group
+            last = {g: prompts[g][(len(prompts[g]) - 1) // self.max_portion * self.max_portion:] for g in range(n)}
+            self.step({(g, 0): prompts[g][:len(prompts[g]) - len(last[g])] for g in range(n) if len(last[g]) < len(prompts[g])})
+            for g in range(n):
+                for k in range(1, K):
+                    self.lengths[g * K + k] = len(prompts[g])
+                    if self.shares:
+                        self._share(g * K + k, g * K, len(prompts[g]))
+            self._set_device("step", 0)
+            for name, value in (("ended", 0), ("length", 0), ("scores", [0.0 if s % K == 0 and s < n * K else -math.inf for s in range(self.batch)]),
+                                ("begin", [len(prompts[s // K]) if s < n * K else 0 for s in range(self.batch)])):
+                self._set_device(name, value)
+            self.session.record_timestamp("start")
+            self._run_portion({g * K: last[g] for g in range(n)}, sample=(end, length_penalty))
+            self.session.record_timestamp("prefill_done")
+            self._set_device("count", [1 if s < n * K else 0 for s in range(self.batch)])
+            program, steps = self._beams_program(end, length_penalty)["program"], 1
+            while steps < n_new:
+                self.session.run_program(program, fetch=False)
+                steps += 1
+                if end is not None and steps % 16 == 0 and self._all_ended(n * K):
+                    break
+            self.session.record_timestamp("decode_done")
+            tokens, parents, scores, lengths = (self.session.get_tensor_data(self._vars[k]) for k in ("generated", "parents", "scores", "length"))
+            if self.session.use_native:
+                from ..ops import native
+
+                native.check_gemm_errors()
+        finally:
+            for request in [r for r in self.slots if isinstance(r, tuple)][::-1]:
+                self.release(request)
+        out = []
+        for g in range(n):
+            found = []
+            for s in range(g * K, (g + 1) * K):
+                if not math.isfinite(scores[s]):
+                    continue
+                row, at = [], s
+                for i in range(steps - 1, -1, -1):
+                    row.append(int(tokens[i, at]))
+                    at = int(parents[i, at])
+                found.append(Beam(np.array(row[::-1][:int(lengths[s])], np.int32), float(scores[s])))
+            out.append(sorted(found, key=lambda b: -b.score / max(1, len(b.tokens)) ** length_penalty))
+        return out
+
+    def _all_ended(self, rows: int) -> bool:
+        ended, scores = (self.session.device_tensor(self._vars[k])[:rows] for k in ("ended", "scores"))
+        return bool(((ended != 0) | ~torch.isfinite(scores)).all())
 
     def _set_device(self, name: str, value):
         v = self.session._vars[self._vars[name]][0]

@@ -11,8 +11,9 @@ Both sublayers read the same h and end in the same sum, so a layer is two produc
 `[o | down]` on the attention's and the feed-forward's results side by side.
 
 `Zirunex` describes the model to `SequenceGenerator`: which tensors it needs, how they are made from a checkpoint, what state
-a sequence has, and the ops of one portion of tokens. Two of its properties belong to a deployment and not to a checkpoint: whether
-caches are held in the model's type or in 8 bits, and how many low-rank adapters stand beside the projections of every layer.
+a sequence has, and the ops of one portion of tokens. Three of its properties belong to a deployment and not to a checkpoint: whether
+caches are held in the model's type or in 8 bits, how many low-rank adapters stand beside the projections of every layer, and whether
+sequences may share their first positions.
 """
 from dataclasses import dataclass
 from typing import Any, Callable, Dict, List, Mapping, Optional, Tuple
@@ -150,15 +151,20 @@ class Zirunex:
     """Weights, state and step of the model for `SequenceGenerator`."""
 
     config_class = ZirunexConfig
-    options = ("cache", "adapters", "adapter_rank")
+    options = ("cache", "adapters", "adapter_rank", "shared_prefixes")
 
-    def __init__(self, cfg: ZirunexConfig, dtype: str = "bfloat16", cache: str = "model", adapters: int = 0, adapter_rank: int = 16):
+    def __init__(self, cfg: ZirunexConfig, dtype: str = "bfloat16", cache: str = "model", adapters: int = 0, adapter_rank: int = 16,
+                 shared_prefixes: bool = False):
         """`cache`: "model" (keys and values in the model's type) or "int8" (codes of 8 bits with a scale per block of 64 tokens and
-        head). `adapters`: how many low-rank adapters the program holds, each of `adapter_rank` numbers per joint matrix of a layer."""
+        head). `adapters`: how many low-rank adapters the program holds, each of `adapter_rank` numbers per joint matrix of a layer.
+        `shared_prefixes`: sequences may have their first positions in another one's cache (of the model's type)."""
         if cache not in ("model", "int8"):
             raise ValueError(f"a cache is held as 'model' or 'int8', not {cache!r}")
         if adapters < 0 or not 1 <= adapter_rank <= ops.MAX_RANK:
             raise ValueError(f"cannot hold {adapters} adapters of rank {adapter_rank}")
+        if shared_prefixes and cache != "model":
+            raise ValueError("positions can be shared in a cache of the model's type only")
+        self.shared_prefixes = shared_prefixes
         self.cfg = cfg
         self.dtype = xl.dtype.as_dtype(dtype)
         self.vocab, self.width = cfg.vocab, cfg.width
@@ -285,6 +291,11 @@ class Zirunex:
             out[f"l{i}.v"] = ((batch, m.kv_heads, max_seq, m.vdim), self.dtype)
         return out
 
+    def state_positions(self) -> Dict[str, Tuple[Optional[int], int]]:
+        """By name of a state: its axis of positions (None: it has none) and how many of them an entry stands for."""
+        per = ops.CACHE8_BLOCK if self.cache == "int8" else 1
+        return {name: (None if name.endswith("_tail") else 2, per) for name in self.state(1, 1)}
+
     def tables(self, max_seq: int) -> Dict[str, Any]:
         return {}
 
@@ -318,6 +329,9 @@ class Zirunex:
                 cache = ops.Cache8(*(t(f"l{i}.{field}") for field in ops.Cache8._fields))
                 joint = ops.window_attention_q8_(proj, t(w + "q_norm"), t(w + "k_norm"), cache, pos, count, joint, T, m.heads, m.scale,
                                                  m.window, m.keep_first, SINK_SCORE, c.eps)
+            elif self.shared_prefixes:
+                joint = ops.window_attention_shared_(proj, t(w + "q_norm"), t(w + "k_norm"), t(f"l{i}.k"), t(f"l{i}.v"), pos, count, t("lead"),
+                                                     t("shared"), joint, T, m.heads, m.scale, m.window, m.keep_first, SINK_SCORE, c.eps)
             else:
                 joint = ops.window_attention_(proj, t(w + "q_norm"), t(w + "k_norm"), t(f"l{i}.k"), t(f"l{i}.v"), pos, count, joint,
                                               T, m.heads, m.scale, m.window, m.keep_first, SINK_SCORE, c.eps)
