@@ -26,6 +26,7 @@ constexpr int BM_MAX_BEAMS = 32;
 constexpr int BM_MAX_PARTS = 128;
 constexpr int BM_KEEP = 512;                      // a longer list is cut to its best between two chunks
 constexpr int BM_MERGED = 2048;                   // entries that the parts of a group leave, at most
+constexpr int BM_GROUP = 4;                       // threads whose largest entry counts as one for the bound
 
 template <typename V> __device__ __forceinline__ bool better(V a, int i, V b, int j) { return a > b || (a == b && i < j); }
 
@@ -38,7 +39,7 @@ template <typename V> __device__ int best_of_list(const V* v, const int* id, int
       const V mine = v[e];
       const int at = id[e];
       int rank = 0;
-#pragma unroll 4
+#pragma unroll 2
       for (int o = 0; o < n; ++o) rank += better(v[o], id[o], mine, at) ? 1 : 0;
       if (rank < most) {
         best_v[rank] = mine;
@@ -75,17 +76,40 @@ template <typename V> __device__ int best_of_list(const V* v, const int* id, int
   return most;
 }
 
-// A bound that at least `most` of the threads' values reach (-inf where fewer than that are finite).
+// A bound that at least `most` (up to 64) of the threads' values reach (-inf where fewer than that are finite): the `most`-th largest of the maxima of
+// BM_GROUP threads each. (Of all threads: 1.1 us of every CTA instead of 0.2, for a list that is hardly shorter.)
 template <typename V> __device__ V bound_of(V mine, int most, V* room, V* result) {
+  constexpr int GROUPS = BM_THREADS / BM_GROUP;
   const int tid = threadIdx.x;
-  room[tid] = mine;
+#pragma unroll
+  for (int d = 1; d < BM_GROUP; d <<= 1) {
+    const V other = __shfl_xor_sync(0xffffffffu, mine, d);
+    mine = other > mine ? other : mine;
+  }
+  if (tid % BM_GROUP == 0) room[tid / BM_GROUP] = mine;
   __syncthreads();
-  int rank = 0;
-#pragma unroll 8
-  for (int o = 0; o < BM_THREADS; ++o) rank += better(room[o], o, mine, tid) ? 1 : 0;
-  if (rank == most - 1) *result = mine;
+  if (tid < GROUPS) {
+    const V own = room[tid];
+    int rank = 0;
+#pragma unroll 4
+    for (int o = 0; o < GROUPS; ++o) rank += better(room[o], o, own, tid) ? 1 : 0;
+    if (rank == most - 1) *result = own;
+  }
   __syncthreads();
   return *result;
+}
+
+// the next lower number (of what is finite)
+__device__ __forceinline__ float below(float x) {
+  const int i = __float_as_int(x);
+  return !isfinite(x) ? x : x > 0.f ? __int_as_float(i - 1) : x < 0.f ? __int_as_float(i + 1) : __int_as_float((int)0x80000001u);
+}
+// e^d for d <= 0 (or d = -inf): the rounding of d * log2(e) is made good, the rest is the special-function unit's (2^-22 relative)
+__device__ __forceinline__ float exp_below(float d) {
+  constexpr float HI = 1.44269502f, LO = 1.92596299e-8f;  // of log2(e)
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(fmaf(d, HI, d * LO)));
+  return y;
 }
 
 struct BeamArgs {
@@ -123,58 +147,84 @@ template <typename T> __global__ void __launch_bounds__(BM_THREADS) take_beams_k
     const int phase = (int)(((uintptr_t)p & 15) / sizeof(T));  // places are counted from the 16-byte boundary before the row
     const int u0 = max(part * a.per_part, phase), u1 = min((part + 1) * a.per_part, a.valid + phase);
     p -= phase;
-    float m = -INFINITY, hi = 0.f, lo = 0.f, tau = -INFINITY;  // m: of the warp
+    float m = -INFINITY, hi = 0.f, lo = 0.f, tau = -INFINITY;  // m: of the warp; tau: entries above it go to the list
     auto add = [&](float e) {
       const float h = __fsub_rn(__fadd_rn(e, 512.f), 512.f);  // steps of 2^-14
       hi = __fadd_rn(hi, h);
       lo = __fadd_rn(lo, __fsub_rn(e, h));
     };
+    constexpr int LOADS = BM_EACH / N;
+    uint4 raw[LOADS];
+    auto fetch = [&](int c0) {
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        const int u = c0 + (i * BM_THREADS + tid) * N;
+        if (u >= u0 && u + N <= u1) raw[i] = __ldcs(reinterpret_cast<const uint4*>(p + u));
+      }
+    };
     bool first = true;
-    for (int c0 = part * a.per_part; c0 < u1; c0 += BM_CHUNK) {
+    const int begin = part * a.per_part;
+    if (begin < u1) fetch(begin);
+#pragma unroll 1
+    for (int c0 = begin; c0 < u1; c0 += BM_CHUNK) {
       float x[BM_EACH];
 #pragma unroll
-      for (int i = 0; i < BM_EACH / N; ++i) {
+      for (int i = 0; i < LOADS; ++i) {
         const int u = c0 + (i * BM_THREADS + tid) * N;
-        float y[N];
-        if (u >= u0 && u + N <= u1) {
-          xl_load16(p + u, y);
-        } else {  // the first and the last group of the part
+        const T* e = reinterpret_cast<const T*>(&raw[i]);
+        const bool whole = u >= u0 && u + N <= u1;  // else the first or the last group of the part, or none of it
 #pragma unroll
-          for (int e = 0; e < N; ++e) y[e] = u + e >= u0 && u + e < u1 ? xl_to_float(p[u + e]) : -INFINITY;
+        for (int k = 0; k < N; ++k) {
+          x[i * N + k] = -INFINITY;
+          if (whole) x[i * N + k] = fmaxf(xl_to_float(e[k]), -INFINITY);  // NaN: minus infinity
         }
+        if (!whole && u + N > u0 && u < u1)
 #pragma unroll
-        for (int e = 0; e < N; ++e) x[i * N + e] = y[e] == y[e] ? y[e] : -INFINITY;
+          for (int k = 0; k < N; ++k)
+            if (u + k >= u0 && u + k < u1) x[i * N + k] = fmaxf(xl_to_float(p[u + k]), -INFINITY);
       }
+      if (c0 + BM_CHUNK < u1) fetch(c0 + BM_CHUNK);  // under way while these are looked at
       float top = x[0];
 #pragma unroll
       for (int i = 1; i < BM_EACH; ++i) top = fmaxf(top, x[i]);
       const float now = fmaxf(m, xl_warp_max(top));
       if (now > m) {
-        const float f = expf(m - now), h = hi * f, l = lo * f;
+        const float f = m > -INFINITY ? expf(m - now) : 0.f, h = hi * f, l = lo * f;
         hi = lo = 0.f;
         m = now;
         add(h);
         add(l);
       }
       if (m > -INFINITY) {
+        float e[BM_EACH];
 #pragma unroll
-        for (int i = 0; i < BM_EACH; ++i) add(expf(x[i] - m));
+        for (int i = 0; i < BM_EACH; ++i) e[i] = exp_below(x[i] - m);
+#pragma unroll
+        for (int w = BM_EACH / 2; w; w >>= 1)
+#pragma unroll
+          for (int i = 0; i < w; ++i) e[i] += e[i + w];
+        add(e[0]);
       }
-      if (first) tau = bound_of(top, K, list_v, &tau_s);  // (the list is empty)
-      __syncthreads();
-      // entries of the first chunk that reach the bound, those of later ones that pass it: equal ones have K before them
-#pragma unroll
-      for (int i = 0; i < BM_EACH; ++i)
-        if (x[i] > tau || (first && x[i] == tau && x[i] > -INFINITY)) {
-          const int at = atomicAdd(&listed, 1);
-          list_v[at] = x[i];
-          list_i[at] = c0 + (i / N * BM_THREADS + tid) * N + i % N - phase;
-        }
+      // of the first chunk entries that reach the bound, of later ones those that pass it: equal ones have K before them
+      float bound = tau;
+      if (first) {
+        tau = bound_of(top, K, list_v, &tau_s);  // (the list is empty)
+        bound = below(tau);
+      }
       first = false;
-      __syncthreads();
-      if (listed > BM_KEEP && c0 + BM_CHUNK < u1) {
-        best_of_list(list_v, list_i, listed, K, best_v, best_i);
-        if (tid < K) {
+      int places = 0;
+      if (top > bound) {
+#pragma unroll
+        for (int i = 0; i < BM_EACH; ++i)
+          if (x[i] > bound) {
+            places = atomicAdd(&listed, 1);
+            list_v[places] = x[i];
+            list_i[places] = c0 + (i / N * BM_THREADS + tid) * N + i % N - phase;
+          }
+      }
+      if (__syncthreads_or(places >= BM_KEEP) && c0 + BM_CHUNK < u1) {  // (the same for all threads, and nobody adds before all are here)
+        const int kept = best_of_list(list_v, list_i, listed, K, best_v, best_i);
+        if (tid < kept) {
           list_v[tid] = best_v[tid];
           list_i[tid] = best_i[tid];
         }
@@ -219,8 +269,8 @@ template <typename T> __global__ void __launch_bounds__(BM_THREADS) take_beams_k
   __shared__ double top[BM_MAX_BEAMS], log_sum[BM_MAX_BEAMS], divisor[BM_MAX_BEAMS], score[BM_MAX_BEAMS], chosen_rank[BM_MAX_BEAMS], tau_d;
   __shared__ int chosen[BM_MAX_BEAMS], state[BM_MAX_BEAMS], after[BM_MAX_BEAMS], slot_of[BM_MAX_BEAMS];  // state 0: no beam, 1: live, 2: ended
   const int row0 = group * K;
-  double* merged_r = reinterpret_cast<double*>(smem);  // [BM_MERGED]
-  int* merged_i = reinterpret_cast<int*>(merged_r + BM_MERGED);
+  double* merged_r = reinterpret_cast<double*>(smem);
+  int* merged_i;
   if (tid < K) {
     const float f = a.scores[row0 + tid];
     const bool ended = a.end >= 0 && a.ended[row0 + tid] != 0;
@@ -229,7 +279,6 @@ template <typename T> __global__ void __launch_bounds__(BM_THREADS) take_beams_k
     after[tid] = a.length[row0 + tid] + (ended ? 0 : 1);
     divisor[tid] = a.penalty == 0.0 ? 1.0 : pow((double)max(after[tid], 1), a.penalty);
   }
-  if (tid == 0) listed = 0;
   __syncthreads();
   for (int k = tid >> 5; k < K; k += BM_THREADS / 32) {  // a warp for every row: its maximum and sum
     if (state[k] != 1) continue;
@@ -252,40 +301,55 @@ template <typename T> __global__ void __launch_bounds__(BM_THREADS) take_beams_k
   __syncthreads();
   // the sum that beam k has with an entry x; where its row has no finite largest entry: not a number, or minus infinity
   auto with = [&](int k, float x) { return score[k] + (((double)x - top[k]) - log_sum[k]); };
-  const int each = a.parts * K, total = each * K;  // entries of a row, of the group: a thread looks at tid, tid + 256, ...
-  constexpr int MINE = BM_MERGED / BM_THREADS;
-  double mine[MINE], most = -INFINITY;
-  int flat[MINE];
-#pragma unroll
-  for (int i = 0; i < MINE; ++i) {
-    const int e = tid + i * BM_THREADS, k = e / each, q = (e - k * each) / K, at = e - k * each - q * K;
-    mine[i] = -INFINITY;
-    flat[i] = 0;
-    if (e < total) {
-      if (state[k] == 1) {
-        const long long from = (long long)(row0 + k) * a.parts + q;
-        if (at < __float_as_int(__ldcg(&a.stats[from].w))) {
-          mine[i] = with(k, __ldcg(a.part_v + from * K + at)) / divisor[k];
-          flat[i] = k * a.valid + __ldcg(a.part_i + from * K + at);
-        }
-      } else if (state[k] == 2 && q == 0 && at == 0) {
-        mine[i] = score[k] / divisor[k];
-        flat[i] = k * a.valid + a.end;
+  // a thread for each of the rows' parts in turn
+  const int parts_all = a.parts * K;
+  double* all_r = merged_r + BM_THREADS;  // [BM_MERGED] ranks, behind room for the bound; then [BM_MERGED] entries
+  int* all_i = reinterpret_cast<int*>(all_r + BM_MERGED);
+  double most = -INFINITY;
+#pragma unroll 1
+  for (int e = tid; e < parts_all * K; e += BM_THREADS) {
+    const int from = e / K, at = e - from * K, k = from / a.parts, q = from - k * a.parts;
+    double r = -INFINITY;
+    int flat = 0;
+    if (state[k] == 1) {
+      const long long place = (long long)(row0 + k) * a.parts + q;
+      const float4 st = __ldcg(&a.stats[place]);
+      const float x = __ldcg(a.part_v + place * K + at);
+      const int v = __ldcg(a.part_i + place * K + at);
+      if (at < __float_as_int(st.w)) {
+        r = with(k, x) / divisor[k];
+        flat = k * a.valid + v;
       }
-      if (!isfinite(mine[i])) mine[i] = -INFINITY;
+    } else if (state[k] == 2 && q == 0 && at == 0) {
+      r = score[k] / divisor[k];
+      flat = k * a.valid + a.end;
     }
-    if (mine[i] > most) most = mine[i];
+    if (!isfinite(r)) r = -INFINITY;
+    all_r[e] = r;
+    all_i[e] = flat;
+    most = r > most ? r : most;
   }
-  const double tau = bound_of(most, K, merged_r, &tau_d);  // (the list is empty)
-#pragma unroll
-  for (int i = 0; i < MINE; ++i)
-    if (mine[i] >= tau && mine[i] > -INFINITY) {
-      const int at = atomicAdd(&listed, 1);
-      merged_r[at] = mine[i];
-      merged_i[at] = flat[i];
-    }
+  const double tau = bound_of(most, K, merged_r, &tau_d);
+  // The list takes the place of the ranks that have been looked at: no more entries are before an entry than in front of it.
+  __shared__ int at_list;
+  if (tid == 0) at_list = 0;
   __syncthreads();
-  const int found = best_of_list(merged_r, merged_i, listed, K, chosen_rank, chosen);
+  merged_i = all_i;
+  merged_r = all_r;
+#pragma unroll 1
+  for (int e0 = 0; e0 < parts_all * K; e0 += BM_THREADS) {
+    const int e = e0 + tid;
+    const double r = e < parts_all * K ? all_r[e] : -INFINITY;
+    const int flat = e < parts_all * K ? all_i[e] : 0;
+    __syncthreads();
+    if (r >= tau && r > -INFINITY) {
+      const int at = atomicAdd(&at_list, 1);
+      merged_r[at] = r;
+      merged_i[at] = flat;
+    }
+    __syncthreads();
+  }
+  const int found = best_of_list(merged_r, merged_i, at_list, K, chosen_rank, chosen);
   bool any = false;
   for (int k = 0; k < K; ++k) any |= state[k] != 0;
   if (any) {
@@ -339,7 +403,7 @@ template <typename T> __global__ void __launch_bounds__(BM_THREADS) take_beams_k
 
 template <typename T> int launch_take(const void* logits, const BeamArgs& a, cudaStream_t s) {
   const int bytes = (BM_CHUNK + BM_KEEP) * 8;
-  static_assert(BM_MERGED * 12 <= (BM_CHUNK + BM_KEEP) * 8, "the merge has room in the list");
+  static_assert(BM_THREADS * 8 + BM_MERGED * 12 <= (BM_CHUNK + BM_KEEP) * 8, "the merge has room in the list");
   const cudaError_t e = xl_launch_overlapped(take_beams_kernel<T>, dim3(a.parts, a.rows), dim3(BM_THREADS), (size_t)bytes, s, (const T*)logits, a);
   return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
 }
