@@ -23,7 +23,7 @@ constexpr int BM_THREADS = 256;
 constexpr int BM_EACH = 16;                       // entries of a thread in a chunk
 constexpr int BM_CHUNK = BM_THREADS * BM_EACH;
 constexpr int BM_MAX_BEAMS = 32;
-constexpr int BM_MAX_PARTS = 128;
+constexpr int BM_MAX_PARTS = 16;                  // each part costs the merge its loads
 constexpr int BM_KEEP = 512;                      // a longer list is cut to its best between two chunks
 constexpr int BM_MERGED = 2048;                   // entries that the parts of a group leave, at most
 constexpr int BM_GROUP = 4;                       // threads whose largest entry counts as one for the bound
@@ -126,7 +126,7 @@ struct BeamArgs {
   double penalty;
 };
 
-template <typename T> __global__ void __launch_bounds__(BM_THREADS) take_beams_kernel(const T* logits, const BeamArgs a) {
+template <typename T> __global__ void __launch_bounds__(BM_THREADS, 5) take_beams_kernel(const T* logits, const BeamArgs a) {
   constexpr int N = XlVec<T>::N;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ float best_v[BM_MAX_BEAMS];
@@ -214,15 +214,20 @@ template <typename T> __global__ void __launch_bounds__(BM_THREADS) take_beams_k
       first = false;
       int places = 0;
       if (top > bound) {
+        unsigned int hits = 0;
+#pragma unroll
+        for (int i = 0; i < BM_EACH; ++i) hits |= x[i] > bound ? 1u << i : 0u;
+        places = atomicAdd(&listed, __popc(hits));
+        int at = places;
 #pragma unroll
         for (int i = 0; i < BM_EACH; ++i)
-          if (x[i] > bound) {
-            places = atomicAdd(&listed, 1);
-            list_v[places] = x[i];
-            list_i[places] = c0 + (i / N * BM_THREADS + tid) * N + i % N - phase;
+          if (hits >> i & 1) {
+            list_v[at] = x[i];
+            list_i[at++] = c0 + (i / N * BM_THREADS + tid) * N + i % N - phase;
           }
+        places = at;
       }
-      if (__syncthreads_or(places >= BM_KEEP) && c0 + BM_CHUNK < u1) {  // (the same for all threads, and nobody adds before all are here)
+      if (__syncthreads_or(places > BM_KEEP) && c0 + BM_CHUNK < u1) {  // (the same for all threads, and nobody adds before all are here)
         const int kept = best_of_list(list_v, list_i, listed, K, best_v, best_i);
         if (tid < kept) {
           list_v[tid] = best_v[tid];
@@ -280,20 +285,21 @@ template <typename T> __global__ void __launch_bounds__(BM_THREADS) take_beams_k
     divisor[tid] = a.penalty == 0.0 ? 1.0 : pow((double)max(after[tid], 1), a.penalty);
   }
   __syncthreads();
-  for (int k = tid >> 5; k < K; k += BM_THREADS / 32) {  // a warp for every row: its maximum and sum
-    if (state[k] != 1) continue;
-    const int lane = tid & 31;
+  {  // maxima and sums of all rows side by side
+    const int lanes = K <= 8 ? 32 : K <= 16 ? 16 : 8, k = tid / lanes, lane = tid & (lanes - 1);
+    const bool on = k < K && state[min(k, K - 1)] == 1;
+    const float4* st = a.stats + (long long)(row0 + k) * a.parts;
     float m = -INFINITY;
-    for (int q = lane; q < a.parts; q += 32) m = fmaxf(m, __ldcg(&a.stats[(long long)(row0 + k) * a.parts + q]).x);
-    m = xl_warp_max(m);
+    for (int q = lane; on && q < a.parts; q += lanes) m = fmaxf(m, __ldcg(&st[q]).x);
+    for (int d = lanes / 2; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
     double sum = 0.0;
-    for (int q = lane; q < a.parts; q += 32) {
-      const float4 st = __ldcg(&a.stats[(long long)(row0 + k) * a.parts + q]);
-      if (st.x > -INFINITY) sum += ((double)st.y + (double)st.z) * exp((double)st.x - (double)m);
+#pragma unroll 1
+    for (int q = lane; on && q < a.parts; q += lanes) {
+      const float4 x = __ldcg(&st[q]);
+      if (x.x > -INFINITY) sum += ((double)x.y + (double)x.z) * (x.x == m ? 1.0 : exp((double)x.x - (double)m));
     }
-#pragma unroll
-    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    if (lane == 0) {
+    for (int d = lanes / 2; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    if (on && lane == 0) {
       top[k] = (double)m;
       log_sum[k] = log(sum);
     }
@@ -301,33 +307,41 @@ template <typename T> __global__ void __launch_bounds__(BM_THREADS) take_beams_k
   __syncthreads();
   // the sum that beam k has with an entry x; where its row has no finite largest entry: not a number, or minus infinity
   auto with = [&](int k, float x) { return score[k] + (((double)x - top[k]) - log_sum[k]); };
-  // a thread for each of the rows' parts in turn
+  // 2^n lanes for the entries of one row and part, several of these for a warp at a time
   const int parts_all = a.parts * K;
   double* all_r = merged_r + BM_THREADS;  // [BM_MERGED] ranks, behind room for the bound; then [BM_MERGED] entries
   int* all_i = reinterpret_cast<int*>(all_r + BM_MERGED);
   double most = -INFINITY;
-#pragma unroll 1
-  for (int e = tid; e < parts_all * K; e += BM_THREADS) {
-    const int from = e / K, at = e - from * K, k = from / a.parts, q = from - k * a.parts;
-    double r = -INFINITY;
-    int flat = 0;
-    if (state[k] == 1) {
-      const long long place = (long long)(row0 + k) * a.parts + q;
-      const float4 st = __ldcg(&a.stats[place]);
-      const float x = __ldcg(a.part_v + place * K + at);
-      const int v = __ldcg(a.part_i + place * K + at);
-      if (at < __float_as_int(st.w)) {
-        r = with(k, x) / divisor[k];
-        flat = k * a.valid + v;
+  {
+    int lanes = 1;
+    while (lanes < K) lanes *= 2;
+    const int at = tid & (lanes - 1), stride = BM_THREADS / lanes;
+    int from = tid / lanes, k = from / a.parts, q = from - k * a.parts;
+#pragma unroll 2
+    for (; from < parts_all; from += stride) {
+      if (at < K) {
+        double r = -INFINITY;
+        int flat = 0;
+        if (state[k] == 1) {
+          const long long place = (long long)(row0 + k) * a.parts + q;
+          const float kept = __ldcg(&a.stats[place].w), x = __ldcg(a.part_v + place * K + at);
+          const int v = __ldcg(a.part_i + place * K + at);
+          if (at < __float_as_int(kept)) {
+            r = with(k, x);
+            if (a.penalty != 0.0) r /= divisor[k];
+            flat = k * a.valid + v;
+          }
+        } else if (state[k] == 2 && q == 0 && at == 0) {
+          r = score[k] / divisor[k];
+          flat = k * a.valid + a.end;
+        }
+        if (!isfinite(r)) r = -INFINITY;
+        all_r[from * K + at] = r;
+        all_i[from * K + at] = flat;
+        most = r > most ? r : most;
       }
-    } else if (state[k] == 2 && q == 0 && at == 0) {
-      r = score[k] / divisor[k];
-      flat = k * a.valid + a.end;
+      for (q += stride; q >= a.parts; q -= a.parts) ++k;
     }
-    if (!isfinite(r)) r = -INFINITY;
-    all_r[e] = r;
-    all_i[e] = flat;
-    most = r > most ? r : most;
   }
   const double tau = bound_of(most, K, merged_r, &tau_d);
   // The list takes the place of the ranks that have been looked at: no more entries are before an entry than in front of it.
@@ -353,25 +367,23 @@ template <typename T> __global__ void __launch_bounds__(BM_THREADS) take_beams_k
   bool any = false;
   for (int k = 0; k < K; ++k) any |= state[k] != 0;
   if (any) {
-    if (tid == 0) {
-      for (int n = found, i = 0; n < K; ++i) {  // too few: those at minus infinity follow, the lowest first
-        bool in = false;
-        for (int j = 0; j < found; ++j) in |= chosen[j] == i;
-        if (!in) chosen[n++] = i;
-      }
-      unsigned int continued = 0, taken = 0;  // slots whose beams go on, slots that are given away
-      for (int r = 0; r < K; ++r) continued |= 1u << (chosen[r] / a.valid);
-      unsigned int spare = ~continued & (K == 32 ? ~0u : (1u << K) - 1);
-      for (int r = 0; r < K; ++r) {
-        int to = chosen[r] / a.valid;
-        const unsigned int bit = 1u << to;
-        if (taken & bit) {
-          to = __ffs(spare) - 1;
-          spare &= spare - 1;
+    if (found < K) {
+      if (tid == 0)
+        for (int n = found, i = 0; n < K; ++i) {  // too few: those at minus infinity follow, the lowest first
+          bool in = false;
+          for (int j = 0; j < found; ++j) in |= chosen[j] == i;
+          if (!in) chosen[n++] = i;
         }
-        taken |= bit;
-        slot_of[r] = to;
-      }
+      __syncthreads();
+    }
+    if (tid < 32) {  // slots by rank: the beam's own for its best continuation, the spare ones in order for others
+      const unsigned int all = K == 32 ? ~0u : (1u << K) - 1, mine = 1u << tid;
+      const int k = tid < K ? chosen[tid] / a.valid : -1;
+      const unsigned int same = __match_any_sync(0xffffffffu, k);
+      const unsigned int spare = ~__reduce_or_sync(0xffffffffu, k >= 0 ? 1u << k : 0u) & all;
+      const bool again = k >= 0 && (same & (mine - 1));
+      const unsigned int others = __ballot_sync(0xffffffffu, again);
+      if (k >= 0) slot_of[tid] = again ? (int)__fns(spare, 0, __popc(others & (mine - 1)) + 1) : k;
     }
     __syncthreads();
     if (tid < K) {
@@ -408,10 +420,10 @@ template <typename T> int launch_take(const void* logits, const BeamArgs& a, cud
   return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
 }
 
-// Into how many parts a row is cut.
+// Into how many parts a row is cut: about six CTAs for every SM, of which five run at a time (384 rows of 50400 entries: 1 part 50 us, 2 parts 43).
 int parts_of(int rows, int beams, int valid) {
-  int parts = 888 / rows < 1 ? 1 : 888 / rows;
-  if (parts > (valid + 1023) / 1024) parts = (valid + 1023) / 1024;
+  int parts = 6 * 148 / rows < 1 ? 1 : 6 * 148 / rows;
+  if (parts > (valid + 2047) / 2048) parts = (valid + 2047) / 2048;
   if (parts > BM_MERGED / (beams * beams)) parts = BM_MERGED / (beams * beams);
   return parts < BM_MAX_PARTS ? parts : BM_MAX_PARTS;
 }
