@@ -106,8 +106,15 @@ constexpr int BKV = 128;
 constexpr int UMMA_K = 16;
 constexpr int SA_THREADS = 128 + 2 * 128;
 constexpr uint32_t TMEM_COLS = 512;
+// Registers of a thread of a kernel that holds rows of scores: of the first warpgroup, which only issues, and of the two others (together what the
+// launch gives, 384 x 168: with 168 each the rows spilled). The settings stand at the head of branches that only join again at the end: behind a join the
+// smaller one would hold.
+constexpr int REGS_CONTROL = 72, REGS_SOFTMAX = 216;
+static_assert(REGS_CONTROL + 2 * REGS_SOFTMAX <= 3 * 168, "more than the launch gives would never be granted");
+template <int N> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 
-enum { ERR_Q = 101, ERR_KV_FULL = 102, ERR_KV_EMPTY = 103, ERR_S = 104, ERR_P = 105, ERR_PV = 106, ERR_MEET = 107 };
+enum { ERR_Q = 101, ERR_KV_FULL = 102, ERR_KV_EMPTY = 103, ERR_S = 104, ERR_P = 105, ERR_PV = 106, ERR_MEET = 107, ERR_TABLE = 108, ERR_ROOM = 109 };
 
 struct SharedParams {
   const __nv_bfloat16* proj;
@@ -311,6 +318,46 @@ __device__ __forceinline__ float weigh(uint32_t tmem_s, const RowMask& mask, int
   return alpha;
 }
 
+// The same with the whole row in registers: more code, and less time for each block where there are many (16 x 250 tokens behind 4000: 630 -> 570 us).
+// What the maximum was before serves for all of the row.
+__device__ __forceinline__ float weigh_row(uint32_t tmem_s, const RowMask& mask, float& mx, float& l, float c) {
+  float s[BKV];
+#pragma unroll
+  for (int w = 0; w < BKV / 32; ++w) {
+    float part[32];
+    masked_scores(tmem_s, mask, w, part);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) s[w * 32 + i] = part[i];
+  }
+  float top[4] = {s[0], s[1], s[2], s[3]}, sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 4; i < BKV; ++i) top[i & 3] = fmaxf(top[i & 3], s[i]);
+  const float m_blk = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+  const bool move = m_blk > -INFINITY && (mx == -INFINITY || (m_blk - mx) * c > 8.f);
+  const float alpha = move && mx != -INFINITY ? fast_exp2((mx - m_blk) * c) : 1.f;
+  if (move) mx = m_blk;
+  const float mc = mx == -INFINITY ? 0.f : mx * c;
+#pragma unroll
+  for (int w = 0; w < BKV / 32; ++w) {
+    uint32_t pairs[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      float& x = s[w * 32 + i];
+      x = fast_exp2(fmaf(x, c, -mc));
+      sum[i & 3] += x;
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float x = s[w * 32 + 2 * i], y = s[w * 32 + 2 * i + 1];
+      pairs[i] = dd_pack(x, y);
+      pairs[16 + i] = dd_pack(x - dd_lo(pairs[i]), y - dd_hi(pairs[i]));
+    }
+    tmem_st_32x32b_x32(tmem_s + w * 32, pairs);
+  }
+  l = l * alpha + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+  return alpha;
+}
+
 template <int VD> __device__ __forceinline__ void rescale_output(uint32_t tmem_o, float alpha) {
 #pragma unroll 1
   for (int ch = 0; ch < VD / 32; ++ch) {
@@ -452,8 +499,9 @@ __global__ void __launch_bounds__(SA_THREADS, 1)
   const uint32_t tmem_base = *tmem_base_slot;
   const int n_kv = keys.until[3];
 
-  if (warp == 0) {
-    if (lane == 0) {
+  if (warp < 4) {
+    fewer_registers<REGS_CONTROL>();
+    if (warp == 0 && lane == 0) {
       xl_grid_dependency_wait();    // the new keys and values; nothing else here depends on the kernel that appends them
       xl_grid_launch_dependents();  // TMEM is held: a successor that allocates some on this SM cannot come first
       bool ok = true;
@@ -485,9 +533,7 @@ __global__ void __launch_bounds__(SA_THREADS, 1)
 #pragma unroll 1
           for (uint32_t i = 0; i < MBAR_SPIN_LIMIT && !mbar_try_wait(&full[n % SLOTS], (uint32_t)(n / SLOTS) & 1u); ++i) {}
       }
-    }
-  } else if (warp == 1) {
-    if (elect_one()) {
+    } else if (warp == 1 && elect_one()) {
       auto wait_full = [&](int n) { return bar_wait(&full[n % SLOTS], (uint32_t)(n / SLOTS) & 1u, abort_flag, p.err, ERR_KV_FULL); };
       auto issue_scores = [&](int j, int m) -> bool {
         if (j == 0 && !bar_wait(&q_full[m], 0, abort_flag, p.err, ERR_Q)) return false;
@@ -520,7 +566,9 @@ __global__ void __launch_bounds__(SA_THREADS, 1)
         }
       }
     }
-  } else if (warp >= 4 && (warp < 8 ? 0 : 1) < tiles) {
+  } else {
+    more_registers<REGS_SOFTMAX>();
+    if ((warp < 8 ? 0 : 1) < tiles) {
     const int m = warp < 8 ? 0 : 1;           // row tile of this warpgroup
     const int qtr = warp & 3;                 // TMEM lane quarter this warp may access
     const int r = qtr * 32 + lane;            // row inside the tile
@@ -558,7 +606,7 @@ __global__ void __launch_bounds__(SA_THREADS, 1)
       tcgen05_fence_after();
       const bool cut = __any_sync(0xffffffffu, col0 + BKV - 1 > hi || (col0 < lo && col0 + BKV > p.keep_first));  // for all lanes alike
       const RowMask mask{cut, col0, hi + 1, lo, p.keep_first, nullptr};
-      const float alpha = weigh(tmem_s, mask, key_steps(x.end - col0), mx, l, c);
+      const float alpha = weigh_row(tmem_s, mask, mx, l, c);
       // the scores of block j are only computed after P V of block j - 1: O is at rest here
       if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) rescale_output<VD>(tmem_o, alpha);
       tmem_st_wait();
@@ -600,7 +648,7 @@ __global__ void __launch_bounds__(SA_THREADS, 1)
       }
     }
   }
-
+  }
   // ---- teardown: every role arrives here, also after an abort --------------------------------------------------------
   tcgen05_fence_before();
   __syncthreads();
@@ -931,12 +979,14 @@ __global__ void __launch_bounds__(SA_THREADS, 1)
   // segment number n of this CTA, when it is in the table; null: the wait for it gave up
   auto segment = [&](int n) -> const GroupSegment* {
 #pragma unroll 1
-    for (uint32_t i = 0; *ready <= n; ++i)
+    for (uint32_t i = 0; *ready <= n; ++i) {
       if (i == MBAR_SPIN_LIMIT || *abort_flag) {
         *abort_flag = 1;
-        atomicCAS(p.err, 0, (int)ERR_MEET);
+        atomicCAS(p.err, 0, (int)ERR_TABLE);
         return nullptr;
       }
+      if (i > 64) __nanosleep(200);  // (a wait that gives up does so behind the barriers' waits, which have the reason)
+    }
     __threadfence_block();
     return table + n % PF_SEGMENTS;
   };
@@ -1076,11 +1126,12 @@ __global__ void __launch_bounds__(SA_THREADS, 1)
       const GroupSegment* sg = segment(sn);
       if (!sg) break;
       const int half = room.take(sg->rows, sn == 0);
+      // The products that used the place before. (Place 1 comes behind a small tile in place 0, whose wait was for a large one's products.) Every use is
+      // waited for, in order, those of large tiles too: a barrier only tells apart the phase that runs and the one before.
+      const int used = half ? room.used1 : room.used0;
+      if (used) ok = bar_wait_warp(&q_empty[half], (uint32_t)(used - 1) & 1u, abort_flag, p.err, ERR_Q);
+      if (!ok) break;
       if (!room.large) {
-        // The products that used the place before. (Place 1 comes behind a small tile in place 0, whose wait was for a large one's products.)
-        const int used = half ? room.used1 : room.used0;
-        if (used) ok = bar_wait_warp(&q_empty[half], (uint32_t)(used - 1) & 1u, abort_flag, p.err, ERR_Q);
-        if (!ok) break;
         fill_queries(*sg, half, 0, 1);
         fence_proxy_async_smem();
         __syncwarp();
@@ -1117,10 +1168,10 @@ __global__ void __launch_bounds__(SA_THREADS, 1)
         for (; x < min(end, x1); ++sn) {
           // the other warps are a few blocks apart from each other: half a table is more than that
 #pragma unroll 1
-          for (uint32_t k = 0; sn - *begun >= PF_SEGMENTS / 2 && k < MBAR_SPIN_LIMIT && !*abort_flag; ++k) {}
+          for (uint32_t k = 0; sn - *begun >= PF_SEGMENTS / 2 && k < MBAR_SPIN_LIMIT && !*abort_flag; ++k) __nanosleep(200);
           if (sn - *begun >= PF_SEGMENTS / 2) {
             *abort_flag = 1;
-            atomicCAS(p.err, 0, (int)ERR_MEET);
+            atomicCAS(p.err, 0, (int)ERR_ROOM);
             x = x1;
             break;
           }
@@ -1417,7 +1468,7 @@ XL_API long long xl_shared_attn_groups_scratch(int B, int T, int H, int vdim, in
 }
 
 // The same for few rows per sequence, whose shared keys are read once for all that share them: two launches behind xl_shared_append, which has to be the
-// launch before. At most 512 sequences. ctas: SMs of the device. scratch: xl_shared_attn_groups_scratch floats, 16-byte aligned.
+// launch before. At most 448 sequences. ctas: SMs of the device. scratch: xl_shared_attn_groups_scratch floats, 16-byte aligned.
 XL_API int xl_shared_attn_groups(const void* proj, long long ld, const float* wq, const void* kc, const void* vc, void* out, long long ldo,
                                  const int* pos, const int* count, const int* lead, const int* shared, int B, int T, int H, int G, int dim,
                                  int vdim, int Smax, int window, int keep_first, int gated, float scale, float sink, float eps, int ctas,

@@ -365,7 +365,9 @@ def check_gemm_errors():
                      104: "attention over shared prefixes: scores never completed",
                      105: "attention over shared prefixes: weights never arrived",
                      106: "attention over shared prefixes: output accumulation never completed",
-                     107: "attention over shared prefixes: warps never met"}
+                     107: "attention over shared prefixes: warps never met",
+                     108: "attention over shared prefixes: a tile never came into the list",
+                     109: "attention over shared prefixes: the list of tiles never emptied"}
             raise RuntimeError(f"tcgen05 GEMM on cuda:{idx} gave up waiting: {names.get(code, code)}")
 
 

@@ -19,9 +19,11 @@ _reorder = _sig("xl_reorder", ctypes.POINTER(_c_ll), _c_int, *[_c_p] * 3, _c_int
 
 
 def _shared_few_rows(B, T, heads, G) -> bool:
-    """Whether a portion of T tokens runs on the kernel that reads shared keys once for a group, and leaves parts of sums in memory, and not on the one
-    that has whole tiles of a sequence's rows and no parts."""
-    return T == 1
+    """Whether a portion runs on the kernel that reads shared keys once for a group and leaves parts of sums in memory, and not on the one that has
+    whole tiles of a sequence's rows and no parts. Measured with 32 heads on 8 and 4 rows per token, groups against portion: 16 sequences behind 4000
+    positions 1 token 42 and 106 us, 8 tokens 76 and 111, 16 tokens 136 and 114; 16 x 8 behind 2000 8 tokens 297 and 422, 16 tokens 567 and 441; 64
+    behind 8000 8 tokens 204 and 800, 32 tokens 1004 and 855. The parts of 2^16 rows of 128 features are 136 MB."""
+    return B <= 448 and (T == 1 or T * (heads // G) <= 32) and B * T * heads <= 1 << 16
 
 
 @native("window_attention_shared_")
