@@ -101,6 +101,10 @@ __global__ void __launch_bounds__(256)
 //
 // TMEM columns: [0, 128) S_0 / P_0, [128, 256) S_1 / P_1, [256, 256 + VD) O_0, [256 + VD, 256 + 2 VD) O_1. One CTA per SM. Every wait is
 // bounded (see tcgen05.cuh).
+//
+// The chain of a tile bounds this: scores, softmax, product. 16 x 250 tokens behind 4000, 32 heads on 8 of 128: 583 us with the append, 437 TFLOP/s (of
+// 255 GFLOP; the two numbers of queries and weights make it 874 in the tensor cores). 7700 clocks for a block of both tiles, 4096 of them products.
+// Two tiles, since a tile's softmax then has the other's products to run under, and keys are read half as often.
 constexpr int TILE_M = 128;
 constexpr int BKV = 128;
 constexpr int UMMA_K = 16;
@@ -114,7 +118,7 @@ static_assert(REGS_CONTROL + 2 * REGS_SOFTMAX <= 3 * 168, "more than the launch 
 template <int N> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 
-enum { ERR_Q = 101, ERR_KV_FULL = 102, ERR_KV_EMPTY = 103, ERR_S = 104, ERR_P = 105, ERR_PV = 106, ERR_MEET = 107, ERR_TABLE = 108, ERR_ROOM = 109 };
+enum { ERR_Q = 111, ERR_KV_FULL = 112, ERR_KV_EMPTY = 113, ERR_S = 114, ERR_P = 115, ERR_PV = 116, ERR_MEET = 117, ERR_TABLE = 118, ERR_ROOM = 119 };
 
 struct SharedParams {
   const __nv_bfloat16* proj;
@@ -318,8 +322,8 @@ __device__ __forceinline__ float weigh(uint32_t tmem_s, const RowMask& mask, int
   return alpha;
 }
 
-// The same with the whole row in registers: more code, and less time for each block where there are many (16 x 250 tokens behind 4000: 630 -> 570 us).
-// What the maximum was before serves for all of the row.
+// The same with the whole row in registers: more code, and less time for each block where there are many (16 x 250 tokens behind 4000: 630 -> 583 us).
+// The maximum from before the block serves for all of the row.
 __device__ __forceinline__ float weigh_row(uint32_t tmem_s, const RowMask& mask, float& mx, float& l, float c) {
   float s[BKV];
 #pragma unroll
@@ -685,6 +689,10 @@ template <int DK, int VD> int launch_portion(const void* kc, const void* vc, con
 //   warp 2       queries of the next tile, if they are few, normalised, from the projections to shared memory;  warp 3  the list of this CTA's tiles
 //   warps 4..7, 8..11   queries of large tiles; softmax of every second block (warps without rows only keep step)
 //
+// 16 x 8 beams behind 2000, up to 130 own positions, 32 heads on 8 of 128: 81 us with the append and the sum (176 MB, 2.2 TB/s); 64 requests behind 8000,
+// up to 700 own: 88 us (183 MB). About 9 us pass before a CTA's first product; from then on about 2900 clocks per block, while loads alone take 2800.
+// Equal runs and not a CTA per tile and slice: groups and own parts are of unlike lengths, and one wave has to end together.
+//
 // Every CTA makes the list by itself, from positions and leads in shared memory: counts, key ranges and offsets by slot, ranks of the members by
 // votes. CTA 0 leaves a copy for the kernel behind.
 //
@@ -1015,8 +1023,7 @@ __global__ void __launch_bounds__(SA_THREADS, 1)
       bool ok = true;
       int issued = 0;
 #pragma unroll 1
-  #pragma unroll 1
-    for (int x = x0, sn = 0; x < x1 && ok; ++sn) {
+      for (int x = x0, sn = 0; x < x1 && ok; ++sn) {
         const GroupSegment* sg = segment(sn);
         if (!sg) break;
         const TileKeys keys = sg->keys;
@@ -1089,8 +1096,7 @@ __global__ void __launch_bounds__(SA_THREADS, 1)
       bool ok = true, add = false, pending = false;  // pending: block it - 1 has no product with the values yet
       int it = 0, steps = 0;
 #pragma unroll 1
-  #pragma unroll 1
-    for (int x = x0, sn = 0; x < x1 && ok; ++sn) {
+      for (int x = x0, sn = 0; x < x1 && ok; ++sn) {
         const GroupSegment* sg = segment(sn);
         if (!sg) break;
         const int half = room.take(sg->rows, sn == 0), count = sg->count, block = sg->block;

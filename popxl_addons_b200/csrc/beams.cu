@@ -10,6 +10,9 @@
 // is a bound that K entries reach; the few entries that reach it go to a list, those of later chunks if they pass it, and the list is
 // ranked at the end. A list that grows long (sorted or equal logits) is cut to its K best between two chunks.
 //
+// 48 x 8 beams of 50400 entries: 38 us (77 MB, 2.0 TB/s; about 26 instructions per entry, most of them for the exponential and its two sums), 16 x 16 of
+// 32000 in bf16: 27 us; one prompt's 4 beams of 32000: 14 us, dependent loads and barriers.
+//
 // Two beams are compared by sums over 50000 entries each, so those have to be better than a sum in 32 bits: an exponential is cut at 2^-14,
 // upper parts add up exactly (up to 2^10 of a warp's maximum), lower ones lose 2^-24 of 2^-15 each; a warp's sums are joined in 64 bits, and c is
 // formed and compared in 64 bits.
@@ -430,7 +433,8 @@ int parts_of(int rows, int beams, int valid) {
 
 // ---- reordering of states ---------------------------------------------------------------------------------------------------
 // A CTA takes a span of one state, group and outer index. A thread takes the same 16 bytes of all rows of the group that move: it
-// has them all before it writes the first, so that rows may be read and written in any pattern, without a copy elsewhere.
+// has them all before it writes the first, so that rows may be read and written in any pattern, without a copy elsewhere. Bytes bound it: each
+// distinct source once, each moved row once. 32 x 8 beams, 8 layers of 8 heads of 128, up to 230 positions: 944 MB in 163 to 172 us (5.5 to 5.8 TB/s).
 constexpr int RO_MAX_STATES = 64;
 constexpr int RO_THREADS = 256;
 

@@ -359,15 +359,15 @@ def check_gemm_errors():
                      95: "attention over an 8-bit cache: scores never completed",
                      96: "attention over an 8-bit cache: weights never arrived",
                      97: "attention over an 8-bit cache: output accumulation never completed",
-                     101: "attention over shared prefixes: query tiles never arrived",
-                     102: "attention over shared prefixes: key / value tile never arrived",
-                     103: "attention over shared prefixes: key / value stage was never released",
-                     104: "attention over shared prefixes: scores never completed",
-                     105: "attention over shared prefixes: weights never arrived",
-                     106: "attention over shared prefixes: output accumulation never completed",
-                     107: "attention over shared prefixes: warps never met",
-                     108: "attention over shared prefixes: a tile never came into the list",
-                     109: "attention over shared prefixes: the list of tiles never emptied"}
+                     111: "attention over shared prefixes: query tiles never arrived",
+                     112: "attention over shared prefixes: key / value tile never arrived",
+                     113: "attention over shared prefixes: key / value stage was never released",
+                     114: "attention over shared prefixes: scores never completed",
+                     115: "attention over shared prefixes: weights never arrived",
+                     116: "attention over shared prefixes: output accumulation never completed",
+                     117: "attention over shared prefixes: warps never met",
+                     118: "attention over shared prefixes: a tile never came into the list",
+                     119: "attention over shared prefixes: the list of tiles never emptied"}
             raise RuntimeError(f"tcgen05 GEMM on cuda:{idx} gave up waiting: {names.get(code, code)}")
 
 
