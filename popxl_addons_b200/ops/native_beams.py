@@ -1,5 +1,6 @@
 """CUDA implementations of the ops of sequences with a common beginning (`xl/ops/beams.py`)."""
 import ctypes
+import functools
 
 import torch
 
@@ -18,6 +19,21 @@ _take_beams_parts = _sig("xl_take_beams_parts", _c_int, _c_int, _c_int)
 _reorder = _sig("xl_reorder", ctypes.POINTER(_c_ll), _c_int, *[_c_p] * 3, _c_int, _c_int, _c_p)
 
 
+def _on_their_device(fn):
+    """A launch goes to the device of its tensors, whatever the current one is."""
+    @functools.wraps(fn)
+    def launch(*args, **kw):
+        devices = {a.device for a in args if isinstance(a, torch.Tensor)}
+        if len(devices) != 1:
+            raise ValueError(f"the tensors of one call lie on {sorted(map(str, devices))}")
+        dev = devices.pop()
+        if dev.type != "cuda" or dev.index == torch.cuda.current_device():
+            return fn(*args, **kw)
+        with torch.cuda.device(dev):
+            return fn(*args, **kw)
+    return launch
+
+
 def _shared_few_rows(B, T, heads, G) -> bool:
     """Whether a portion runs on the kernel that reads shared keys once for a group and leaves parts of sums in memory, and not on the one that has
     whole tiles of a sequence's rows and no parts. Measured with 32 heads on 8 and 4 rows per token, groups against portion: 16 sequences behind 4000
@@ -27,6 +43,7 @@ def _shared_few_rows(B, T, heads, G) -> bool:
 
 
 @native("window_attention_shared_")
+@_on_their_device
 def window_attention_shared_cuda(proj, q_norm, k_norm, kc, vc, pos, count, lead, shared, joint, T, heads, window, keep_first, scale, sink, eps):
     B, G, smax, dim = kc.shape
     vdim, dt, dev = vc.shape[-1], proj.dtype, proj.device
@@ -72,6 +89,7 @@ def window_attention_shared_cuda(proj, q_norm, k_norm, kc, vc, pos, count, lead,
 
 
 @native("take_beams_")
+@_on_their_device
 def take_beams_cuda(current, parent, logits, buf, parents, step, scores, ended, length, *into, beams, end, valid, length_penalty, base, ahead,
                     advance):
     to = into or (scores, ended, length)
@@ -103,6 +121,7 @@ def _rows_of(t, axis, per):
 
 
 @native("reorder_")
+@_on_their_device
 def reorder_cuda(parent, begin, end, *states, beams, axes, per):
     if not _i32(parent, begin, end) or any(not (t.is_cuda and t.is_contiguous()) for t in states):
         return NotImplemented

@@ -171,6 +171,8 @@ def window_attention_shared_(proj: Tensor, q_norm: Tensor, k_norm: Tensor, k_cac
     vdim = v_cache.shape[-1]
     _expect("k_cache", k_cache, (B, G, smax, dim), proj.dtype)
     _expect("v_cache", v_cache, (B, G, smax, vdim), proj.dtype)
+    if k_cache is v_cache:
+        raise ValueError("keys and values cannot be held in one tensor")
     if max(dim, vdim) > 512:
         raise ValueError(f"the attention kernels take dim and vdim up to 512, not {dim} and {vdim}")
     if heads < 1 or heads % G:
@@ -222,6 +224,9 @@ def take_beams_(current: Tensor, parent: Tensor, logits: Tensor, buf: Tensor, pa
         _expect(what, t, (rows,), int32)
     if any(t.rank != 2 or t.shape[1] != rows or t.dtype != int32 for t in (buf, parents)) or buf.shape != parents.shape:
         raise ValueError(f"the choices of {rows} beams are kept in rows of two int32 buffers, not {tuple(buf.shape)} and {tuple(parents.shape)}")
+    written = [current, parent, buf, parents, *(into or state)]
+    if len({id(t) for t in written}) < len(written):
+        raise ValueError("the results of a choice go to tensors of their own")
     if step.dtype != int32 or step.nelms != 1:
         raise ValueError(f"the choices of a step have one position in int32, not {tuple(step.shape)} {step.dtype}")
     return emit1("take_beams_", [current, parent, logits, buf, parents, step, *state, *(into or ())],

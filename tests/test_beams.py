@@ -1,6 +1,5 @@
 """Beam search and shared prefixes through `SequenceGenerator`, against plain float64 models. CPU backend, and marked `gpu` the kernels in
 32 bits and bf16."""
-import math
 
 import numpy as np
 import pytest
@@ -185,4 +184,4 @@ def test_refusals():
     gen.step({"y": [4, 5]})
     with pytest.raises(ValueError, match="itself"):
         gen.admit("z", prefix_of="y")
-    assert len(gen._free) == 2 and math.isinf(math.inf)
+    assert len(gen._free) == 2

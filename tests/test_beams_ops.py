@@ -146,7 +146,6 @@ def test_what_is_not_finite_reaches_those_who_see_it(backend, T):
                     assert not torch.isfinite(got[b, t, h, 3])
                 elif what != what:  # (an infinite key may come to a score of minus infinity)
                     assert not torch.isfinite(got[b, t, h]).any()
-        assert count[3] and count[0] and count[5]
 
 
 def test_refusals_of_attention():
@@ -170,6 +169,18 @@ def test_refusals_of_attention():
                     dict(joint=var((3, 96), xl.bfloat16))):
             with pytest.raises(ValueError):
                 call(**bad)
+        with pytest.raises(ValueError, match="one tensor"):
+            cache = var((3, 2, 30, 16))
+            ops.window_attention_shared_(var((3, 160)), var((16,)), var((16,)), cache, cache, *(var((3,), xl.int32) for _ in range(4)), var((3, 64)), 1, 4, 0.5)
+
+
+
+def test_one_device_per_call():
+    from popxl_addons_b200.ops.native_beams import _on_their_device
+    call = _on_their_device(lambda *a: len(a))
+    assert call(torch.zeros(1), 2, torch.zeros(1)) == 3
+    with pytest.raises(ValueError, match="lie on"):
+        call(torch.zeros(1), torch.zeros(1, device="meta"))
 
 
 # ---- selection ------------------------------------------------------------------------------------------------------
@@ -323,6 +334,10 @@ def test_refusals_of_choices():
                     dict(step=var((2,))), dict(step=var((1,), xl.float32)), dict(s=state(7)), dict(s=state(dts=(xl.int32,) * 3)), dict(into=state(4)),
                     dict(length_penalty=NAN), dict(length_penalty=1e9)):
             with pytest.raises(ValueError):
+                call(**bad)
+        one, two = var((8,)), var((5, 8))
+        for bad in (dict(current=one, parent=one), dict(buf=two, parents=two), dict(s=ops.BeamState(var((8,), xl.float32), one, one))):
+            with pytest.raises(ValueError, match="of their own"):
                 call(**bad)
 
 
