@@ -46,44 +46,63 @@ __device__ __forceinline__ bool bar_wait_warp(uint64_t* bar, uint32_t parity, vo
 
 // ---- new keys and values ------------------------------------------------------------------------------------------------------
 // One CTA per row, a warp per head. What it reads and the kernels behind it write was complete or is no longer read when it lets them start: they
-// may do all but look at the new keys and values at once.
-template <typename T>
+// may do all but look at the new keys and values at once. Latency bounds it, so a head's key, weights and value are all under way before position and
+// count are looked at, V features at a time (4 where sizes and addresses allow, else 1).
+template <typename T, int V>
+struct alignas(sizeof(T) * V) Features {
+  T v[V];
+};
+
+template <typename T, int V>
 __global__ void __launch_bounds__(256)
     shared_append_kernel(const T* proj, long long ld, const float* wq, const float* wk, float* qn, T* kc, T* vc, const int* pos, const int* count,
                          int T_len, int H, int G, int dim, int vdim, int Smax, float eps) {
+  using Raw = Features<T, V>;
+  using Real = Features<float, V>;
   xl_grid_dependency_wait();
   xl_grid_launch_dependents();
-  const int b = blockIdx.y, t = blockIdx.x, p = pos[b] + t;
-  if (t >= count[b] || !window_fits(pos[b], count[b], T_len, Smax)) return;
+  const int b = blockIdx.y, t = blockIdx.x, at = pos[b], n = count[b];
   const T* row = proj + ((long long)b * T_len + t) * ld;
   const int R = H / G, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  constexpr int NP = SA_MAX_DIM / 32;
-  const T* src = row + (long long)(H + G) * dim;
-  for (int i = threadIdx.x; i < G * vdim; i += blockDim.x) {
-    const int g = i / vdim, c = i - g * vdim;
-    vc[(((long long)b * G + g) * Smax + p) * vdim + c] = src[i];
-  }
-  for (int h = qn ? warp : H + warp; h < H + G; h += 8) {
-    float x[NP];
-    double sq = 0.0;
+  constexpr int NP = SA_MAX_DIM / (32 * V);
+  for (int h = qn ? warp : H + warp; h < H + G; h += blockDim.x >> 5) {
+    const T* head = row + (long long)h * dim;
+    const T* value = row + (long long)(H + G) * dim + (long long)(h - H) * vdim;
+    const float* weight = h < H ? wq : wk;
+    Raw x[NP], val[NP];
+    Real w[NP];
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
-      const int c = lane + 32 * i;
-      x[i] = c < dim ? xl_to_float(row[(long long)h * dim + c]) : 0.f;
+      const int c = (lane + 32 * i) * V;
+      if (c < dim) x[i] = *(const Raw*)(head + c), w[i] = *(const Real*)(weight + c);
+      if (h >= H && c < vdim) val[i] = *(const Raw*)(value + c);
     }
+    if (t >= n || !window_fits(at, n, T_len, Smax)) return;
+    double sq = 0.0;
 #pragma unroll
     for (int i = 0; i < NP; ++i)
-      if (32 * i < dim) sq += (double)x[i] * (double)x[i];
+      if ((lane + 32 * i) * V < dim)
+#pragma unroll
+        for (int e = 0; e < V; ++e) sq += (double)xl_to_float(x[i].v[e]) * (double)xl_to_float(x[i].v[e]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
     const double f = 1.0 / sqrt(sq / dim + (double)eps);
+    const long long entry = h < H ? (((long long)b * G + h / R) * T_len + t) * R + h % R : ((long long)b * G + (h - H)) * Smax + at + t;
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
-      const int c = lane + 32 * i;
-      if (c >= dim) break;
-      const float y = (float)((double)x[i] * f * (double)(h < H ? wq : wk)[c]);
-      if (h < H) qn[((((long long)b * G + h / R) * T_len + t) * R + h % R) * dim + c] = y;
-      else kc[(((long long)b * G + (h - H)) * Smax + p) * dim + c] = xl_from_float<T>(y);
+      const int c = (lane + 32 * i) * V;
+      Real y;
+      Raw r;
+      if (c < dim) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          y.v[e] = (float)((double)xl_to_float(x[i].v[e]) * f * (double)w[i].v[e]);
+          r.v[e] = xl_from_float<T>(y.v[e]);
+        }
+        if (h < H) *(Real*)(qn + entry * dim + c) = y;
+        else *(Raw*)(kc + entry * dim + c) = r;
+      }
+      if (h >= H && c < vdim) *(Raw*)(vc + entry * vdim + c) = val[i];
     }
   }
 }
@@ -1439,15 +1458,20 @@ bool tensor_sizes(const void* proj, long long ld, const void* kc, const void* vc
 }  // namespace
 
 // proj: (B*T, ld) as in attention_window.cu; wq, wk (dim) fp32. New keys and values go to the caches, of sequences whose rows all fit; with qn (B, G,
-// T, H/G, dim) the queries go there. dim <= 512.
+// T, H/G, dim) the queries go there. dim, vdim <= 512.
 XL_API int xl_shared_append(const void* proj, long long ld, const float* wq, const float* wk, float* qn, void* kc, void* vc, const int* pos,
                             const int* count, int B, int T, int H, int G, int dim, int vdim, int Smax, float eps, int dtype, cudaStream_t s) {
-  if (B < 1 || B > 65535 || T < 1 || G < 1 || H < 1 || H % G || dim < 1 || dim > SA_MAX_DIM || vdim < 1 || Smax < 1 ||
+  if (B < 1 || B > 65535 || T < 1 || G < 1 || H < 1 || H % G || dim < 1 || dim > SA_MAX_DIM || vdim < 1 || vdim > SA_MAX_DIM || Smax < 1 ||
       ld < (long long)(H + G) * dim + (long long)G * vdim || !wq || !wk)
     return -1;
+  const int warps = min(8, qn ? H + G : G);
   XL_DISPATCH_DTYPE(dtype, X, {
-    XL_TRY(xl_launch_overlapped(shared_append_kernel<X>, dim3(T, B), dim3(256), (size_t)0, s, (const X*)proj, ld, wq, wk, qn, (X*)kc, (X*)vc, pos, count, T, H,
-                                G, dim, vdim, Smax, eps));
+    const auto all = (uintptr_t)proj | (uintptr_t)kc | (uintptr_t)vc;
+    const auto real = (uintptr_t)wq | (uintptr_t)wk | (uintptr_t)qn;
+    const bool wide = dim % 4 == 0 && vdim % 4 == 0 && ld % 4 == 0 && all % (4 * sizeof(X)) == 0 && real % 16 == 0;
+    const auto kernel = wide ? shared_append_kernel<X, 4> : shared_append_kernel<X, 1>;
+    XL_TRY(xl_launch_overlapped(kernel, dim3(T, B), dim3(32 * warps), (size_t)0, s, (const X*)proj, ld, wq, wk, qn, (X*)kc, (X*)vc, pos, count, T, H, G, dim,
+                                vdim, Smax, eps));
   });
   return (int)cudaGetLastError();
 }
