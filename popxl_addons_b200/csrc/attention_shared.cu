@@ -1397,14 +1397,22 @@ __global__ void __launch_bounds__(128) shared_attn_sum_kernel(const GroupParams 
     const float f = mine.x == -INFINITY ? 0.f : exp2f(mine.x - m);
     total += xl_warp_sum(f * mine.y);  // (a sum that is not a number stays none)
     const int now = min(32, all - k0);
-#pragma unroll 4
-    for (int k = 0; k < now; ++k) {
-      const float fk = __shfl_sync(0xffffffffu, f, k);
-      if (fk == 0.f || c >= p.vdim) continue;
-      bool main;
-      const long long e = place(k0 + k, main);
-      const float4 x = __ldcg(reinterpret_cast<const float4*>((main ? a.main_o : a.extra_o) + e * p.vdim + c));
-      acc = make_float4(acc.x + x.x * fk, acc.y + x.y * fk, acc.z + x.z * fk, acc.w + x.w * fk);
+#pragma unroll 1
+    for (int k = 0; k < now; k += 4) {  // four parts under way together, those that hold nothing among them
+      float fk[4];
+      float4 x[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int q = min(k + u, now - 1);
+        const float fq = __shfl_sync(0xffffffffu, f, q);
+        fk[u] = k + u < now ? fq : 0.f;
+        bool main;
+        const long long e = place(k0 + q, main);
+        if (c < p.vdim) x[u] = __ldcg(reinterpret_cast<const float4*>((main ? a.main_o : a.extra_o) + e * p.vdim + c));
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (fk[u] != 0.f) acc = make_float4(acc.x + x[u].x * fk[u], acc.y + x[u].y * fk[u], acc.z + x[u].z * fk[u], acc.w + x[u].w * fk[u]);
     }
   }
   if (c >= p.vdim) return;
