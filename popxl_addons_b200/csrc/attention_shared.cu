@@ -47,7 +47,8 @@ __device__ __forceinline__ bool bar_wait_warp(uint64_t* bar, uint32_t parity, vo
 // ---- new keys and values ------------------------------------------------------------------------------------------------------
 // One CTA per row, a warp per head. What it reads and the kernels behind it write was complete or is no longer read when it lets them start: they
 // may do all but look at the new keys and values at once. Latency bounds it, so a head's key, weights and value are all under way before position and
-// count are looked at, V features at a time (4 where sizes and addresses allow, else 1).
+// count are looked at, V features at a time (4 where sizes and addresses allow, else 1). 4 us for 128 rows of 8 heads, 20 us for 4000 rows (33 MB;
+// 33 us with one feature at a time and values before keys).
 template <typename T, int V>
 struct alignas(sizeof(T) * V) Features {
   T v[V];
@@ -121,8 +122,8 @@ __global__ void __launch_bounds__(256)
 // TMEM columns: [0, 128) S_0 / P_0, [128, 256) S_1 / P_1, [256, 256 + VD) O_0, [256 + VD, 256 + 2 VD) O_1. One CTA per SM. Every wait is
 // bounded (see tcgen05.cuh).
 //
-// The chain of a tile bounds this: scores, softmax, product. 16 x 250 tokens behind 4000, 32 heads on 8 of 128: 583 us with the append, 437 TFLOP/s (of
-// 255 GFLOP; the two numbers of queries and weights make it 874 in the tensor cores). 7700 clocks for a block of both tiles, 4096 of them products.
+// The chain of a tile bounds this: scores, softmax, product. 16 x 250 tokens behind 4000, 32 heads on 8 of 128: 519 us, and 572 with the append (446 TFLOP/s
+// of 255 GFLOP; the two numbers of queries and weights make it twice that in the tensor cores). 7700 clocks for a block of both tiles, 4096 of them products.
 // Two tiles, since a tile's softmax then has the other's products to run under, and keys are read half as often.
 constexpr int TILE_M = 128;
 constexpr int BKV = 128;
@@ -708,8 +709,8 @@ template <int DK, int VD> int launch_portion(const void* kc, const void* vc, con
 //   warp 2       queries of the next tile, if they are few, normalised, from the projections to shared memory;  warp 3  the list of this CTA's tiles
 //   warps 4..7, 8..11   queries of large tiles; softmax of every second block (warps without rows only keep step)
 //
-// 16 x 8 beams behind 2000, up to 130 own positions, 32 heads on 8 of 128: 81 us with the append and the sum (176 MB, 2.2 TB/s); 64 requests behind 8000,
-// up to 700 own: 88 us (183 MB). About 9 us pass before a CTA's first product; from then on about 2900 clocks per block, while loads alone take 2800.
+// 16 x 8 beams behind 2000, up to 130 own positions, 32 heads on 8 of 128: 70 us, 77 with the append and the sum (176 MB, 2.3 TB/s); 64 requests
+// behind 8000, up to 700 own: 75 and 86 us (183 MB). About 9 us pass before a CTA's first product; from then on about 2900 clocks per block, while loads alone take 2800.
 // Equal runs and not a CTA per tile and slice: groups and own parts are of unlike lengths, and one wave has to end together.
 //
 // Every CTA makes the list by itself, from positions and leads in shared memory: counts, key ranges and offsets by slot, ranks of the members by
@@ -1335,7 +1336,7 @@ __global__ void __launch_bounds__(SA_THREADS, 1)
 
 // ---- the sum of all parts -----------------------------------------------------------------------------------------------------------
 // A warp per row and head, four features per lane. Reading bounds it: 2 + 2 parts of a row, and two more for every further CTA that had blocks of its
-// tiles.
+// tiles. 9 us for 64 rows of 32 heads with about 20 parts (12.6 with one part after the other).
 __global__ void __launch_bounds__(128) shared_attn_sum_kernel(const GroupParams a) {
   const SharedParams& p = a.p;
   const int R = p.H / p.G, M = p.T * R, lane = threadIdx.x & 31;

@@ -434,7 +434,7 @@ int parts_of(int rows, int beams, int valid) {
 // ---- reordering of states ---------------------------------------------------------------------------------------------------
 // A CTA takes a span of one state, group and outer index. A thread takes the same 16 bytes of all rows of the group that move: it
 // has them all before it writes the first, so that rows may be read and written in any pattern, without a copy elsewhere. Bytes bound it: each
-// distinct source once, each moved row once. 32 x 8 beams, 8 layers of 8 heads of 128, up to 230 positions: 944 MB in 163 to 172 us (5.5 to 5.8 TB/s).
+// distinct source once, each moved row once. 32 x 8 beams, 8 layers of 8 heads of 128, up to 230 positions: 944 MB in 156 to 172 us (5.5 to 6.1 TB/s).
 constexpr int RO_MAX_STATES = 64;
 constexpr int RO_THREADS = 256;
 
