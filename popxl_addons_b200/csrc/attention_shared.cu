@@ -847,6 +847,7 @@ __global__ void __launch_bounds__(SA_THREADS, 1)
   uint64_t* pv_done = bars + 8;  // [2]
   uint64_t* wg_meet = bars + 10;  // [2]
   uint64_t* q_large = bars + 12;  // queries of large tiles
+  uint64_t* q_free = bars + 13;   // no product needs the queries' room any more, for the next large tile
   uint64_t* full = bars + 14;     // [SLOTS]
   uint64_t* empty = bars + 14 + SLOTS;
   uint32_t* tmem_base_slot = (uint32_t*)(bars + 14 + 2 * SLOTS);
@@ -882,6 +883,7 @@ __global__ void __launch_bounds__(SA_THREADS, 1)
       mbar_init(&wg_meet[s], 4);
     }
     mbar_init(q_large, 8);
+    mbar_init(q_free, 1);
     for (int s = 0; s < 2 * SLOTS; ++s) mbar_init(&full[s], 1);
     *ready = *begun = 0;
     *abort_flag = 0;
@@ -1123,6 +1125,9 @@ __global__ void __launch_bounds__(SA_THREADS, 1)
         const TileKeys keys = sg->keys;
         *begun = sn;
         if (room.large && pending) {  // the warps that make these queries ready end their last tile first
+          ok = bar_wait(&s_full[(it - 1) & 1], (uint32_t)((it - 1) >> 1) & 1u, abort_flag, p.err, ERR_S);  // and with it all products before
+          if (!ok) break;
+          mbar_arrive(q_free);
           ok = issue_values(it - 1, add, steps);
           pending = false;
           if (!ok) break;
@@ -1234,8 +1239,9 @@ __global__ void __launch_bounds__(SA_THREADS, 1)
       const TileKeys& keys = sg.keys;
       const int half = room.take(sg.rows, sn == 0);
       if (room.large) {
-        if (room.used0) ok = bar_wait_warp(&q_empty[0], (uint32_t)(room.used0 - 1) & 1u, abort_flag, p.err, ERR_Q);
-        if (ok && room.used1) ok = bar_wait_warp(&q_empty[1], (uint32_t)(room.used1 - 1) & 1u, abort_flag, p.err, ERR_Q);
+        // The MMA warp says when the room is free, once for every large tile. (The products' own barriers cannot: who skips the uses of small tiles may
+        // come here two uses ahead of one, and a barrier only tells apart the phase that runs and the one before.)
+        if (sn) ok = bar_wait_warp(q_free, (uint32_t)(room.at_once - 1) & 1u, abort_flag, p.err, ERR_Q);
         if (!ok) break;
         fill_queries(sg, 0, warp - 4, 8);
         fence_proxy_async_smem();
