@@ -10,12 +10,14 @@
 // is a bound that K entries reach; the few entries that reach it go to a list, those of later chunks if they pass it, and the list is
 // ranked at the end. A list that grows long (sorted or equal logits) is cut to its K best between two chunks.
 //
-// 48 x 8 beams of 50400 entries: 38 us (77 MB, 2.0 TB/s; about 26 instructions per entry, most of them for the exponential and its two sums), 16 x 16 of
-// 32000 in bf16: 27 us; one prompt's 4 beams of 32000: 14 us, dependent loads and barriers.
+// 48 x 8 beams of 50400 entries: 42 us (77 MB, 1.8 TB/s), 16 x 16 of 32000 in bf16: 30 us; one prompt's 4 beams of 32000: 15 us, dependent loads and
+// barriers.
 //
-// Two beams are compared by sums over 50000 entries each, so those have to be better than a sum in 32 bits: an exponential is cut at 2^-14,
-// upper parts add up exactly (up to 2^10 of a warp's maximum), lower ones lose 2^-24 of 2^-15 each; a warp's sums are joined in 64 bits, and c is
-// formed and compared in 64 bits.
+// Continuations are compared in 64 bits. Within a row that takes no more than the logits; between rows it takes the logarithms of sums over 50000
+// entries each. Those are first formed from exponentials in 32 bits, 16 of them added in 32 bits and the rest in 64 (off by 2e-6 at most,
+// 5e-8 as a rule). Where the choice hangs on less than that, the last CTA forms the sums of the rows concerned again with exponentials in 64
+// bits, in an order that does not depend on where a row lies, and merges once more: equal rows are equal.
+// That is rare, and takes 35 us for a row of 50400 entries.
 #include "common.cuh"
 
 #include <math.h>
@@ -127,7 +129,33 @@ struct BeamArgs {
   unsigned int* counters;  // [groups + 1], zero between launches
   int rows, V, valid, beams, parts, per_part, end, buf_rows, base, ahead, advance;
   double penalty;
+  double slack;  // how far the logarithm of a row's sum may be off, see xl_take_beams
 };
+
+// A sum of exponentials relative to `m` as one relative to `now`, the larger one: rare, and out of the way of the loop's registers.
+__device__ __noinline__ double rescaled(double sum, float m, float now) { return m > -INFINITY ? sum * exp((double)m - (double)now) : 0.0; }
+
+// The sum over a row of e^(x - top), in 64 bits and in an order that only depends on the number of entries, for all threads.
+template <typename T> __device__ __noinline__ double exact_sum(const T* row, int valid, double top, double* room) {
+  constexpr int AHEAD = 8;
+  double sum = 0.0;
+#pragma unroll 1
+  for (long long v = threadIdx.x; v < valid; v += AHEAD * BM_THREADS) {
+    float x[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) x[i] = v + i * BM_THREADS < valid ? fmaxf(xl_to_float(row[v + i * BM_THREADS]), -INFINITY) : -INFINITY;
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) sum += exp((double)x[i] - top);
+  }
+#pragma unroll
+  for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) room[threadIdx.x >> 5] = sum;
+  __syncthreads();
+  sum = 0.0;
+  for (int w = 0; w < BM_THREADS / 32; ++w) sum += room[w];
+  return sum;
+}
 
 template <typename T> __global__ void __launch_bounds__(BM_THREADS, 5) take_beams_kernel(const T* logits, const BeamArgs a) {
   constexpr int N = XlVec<T>::N;
@@ -150,12 +178,8 @@ template <typename T> __global__ void __launch_bounds__(BM_THREADS, 5) take_beam
     const int phase = (int)(((uintptr_t)p & 15) / sizeof(T));  // places are counted from the 16-byte boundary before the row
     const int u0 = max(part * a.per_part, phase), u1 = min((part + 1) * a.per_part, a.valid + phase);
     p -= phase;
-    float m = -INFINITY, hi = 0.f, lo = 0.f, tau = -INFINITY;  // m: of the warp; tau: entries above it go to the list
-    auto add = [&](float e) {
-      const float h = __fsub_rn(__fadd_rn(e, 512.f), 512.f);  // steps of 2^-14
-      hi = __fadd_rn(hi, h);
-      lo = __fadd_rn(lo, __fsub_rn(e, h));
-    };
+    float m = -INFINITY, tau = -INFINITY;  // m: of the warp; tau: entries above it go to the list
+    double sum = 0.0;
     constexpr int LOADS = BM_EACH / N;
     uint4 raw[LOADS];
     auto fetch = [&](int c0) {
@@ -192,11 +216,8 @@ template <typename T> __global__ void __launch_bounds__(BM_THREADS, 5) take_beam
       for (int i = 1; i < BM_EACH; ++i) top = fmaxf(top, x[i]);
       const float now = fmaxf(m, xl_warp_max(top));
       if (now > m) {
-        const float f = m > -INFINITY ? expf(m - now) : 0.f, h = hi * f, l = lo * f;
-        hi = lo = 0.f;
+        sum = rescaled(sum, m, now);
         m = now;
-        add(h);
-        add(l);
       }
       if (m > -INFINITY) {
         float e[BM_EACH];
@@ -206,7 +227,7 @@ template <typename T> __global__ void __launch_bounds__(BM_THREADS, 5) take_beam
         for (int w = BM_EACH / 2; w; w >>= 1)
 #pragma unroll
           for (int i = 0; i < w; ++i) e[i] += e[i + w];
-        add(e[0]);
+        sum += (double)e[0];
       }
       // of the first chunk entries that reach the bound, of later ones those that pass it: equal ones have K before them
       float bound = tau;
@@ -243,7 +264,6 @@ template <typename T> __global__ void __launch_bounds__(BM_THREADS, 5) take_beam
     }
     // ---- the part's maximum and sum, and its best entries -----------------------------------------------------------------------
     const int kept = best_of_list(list_v, list_i, listed, K, best_v, best_i);
-    double sum = (double)hi + (double)lo;
 #pragma unroll
     for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
     if ((tid & 31) == 0) {
@@ -275,10 +295,11 @@ template <typename T> __global__ void __launch_bounds__(BM_THREADS, 5) take_beam
 
   // ---- the group's last CTA: continuations of all its beams ---------------------------------------------------------------------------
   __shared__ double top[BM_MAX_BEAMS], log_sum[BM_MAX_BEAMS], divisor[BM_MAX_BEAMS], score[BM_MAX_BEAMS], chosen_rank[BM_MAX_BEAMS], tau_d;
-  __shared__ int chosen[BM_MAX_BEAMS], state[BM_MAX_BEAMS], after[BM_MAX_BEAMS], slot_of[BM_MAX_BEAMS];  // state 0: no beam, 1: live, 2: ended
+  __shared__ double slack[BM_MAX_BEAMS];
+  __shared__ unsigned int doubt;  // rows whose sums have to be better than they are
+  __shared__ int chosen[BM_MAX_BEAMS], state[BM_MAX_BEAMS], after[BM_MAX_BEAMS], slot_of[BM_MAX_BEAMS], row_of[BM_MAX_BEAMS];  // state 0: no beam, 1: live, 2: ended
   const int row0 = group * K;
-  double* merged_r = reinterpret_cast<double*>(smem);
-  int* merged_i;
+  double* room = reinterpret_cast<double*>(smem);  // [BM_THREADS] for the bound
   if (tid < K) {
     const float f = a.scores[row0 + tid];
     const bool ended = a.end >= 0 && a.ended[row0 + tid] != 0;
@@ -286,7 +307,9 @@ template <typename T> __global__ void __launch_bounds__(BM_THREADS, 5) take_beam
     score[tid] = (double)f;
     after[tid] = a.length[row0 + tid] + (ended ? 0 : 1);
     divisor[tid] = a.penalty == 0.0 ? 1.0 : pow((double)max(after[tid], 1), a.penalty);
+    slack[tid] = state[tid] == 1 ? a.slack / divisor[tid] : 0.0;  // (the only continuation of an ended beam has the sum that the beam has)
   }
+  if (tid == 0) doubt = 0;
   __syncthreads();
   {  // maxima and sums of all rows side by side
     const int lanes = K <= 8 ? 32 : K <= 16 ? 16 : 8, k = tid / lanes, lane = tid & (lanes - 1);
@@ -312,61 +335,92 @@ template <typename T> __global__ void __launch_bounds__(BM_THREADS, 5) take_beam
   auto with = [&](int k, float x) { return score[k] + (((double)x - top[k]) - log_sum[k]); };
   // 2^n lanes for the entries of one row and part, several of these for a warp at a time
   const int parts_all = a.parts * K;
-  double* all_r = merged_r + BM_THREADS;  // [BM_MERGED] ranks, behind room for the bound; then [BM_MERGED] entries
+  double* all_r = room + BM_THREADS;  // [BM_MERGED] ranks, then [BM_MERGED] entries
   int* all_i = reinterpret_cast<int*>(all_r + BM_MERGED);
-  double most = -INFINITY;
-  {
-    int lanes = 1;
-    while (lanes < K) lanes *= 2;
-    const int at = tid & (lanes - 1), stride = BM_THREADS / lanes;
-    int from = tid / lanes, k = from / a.parts, q = from - k * a.parts;
-#pragma unroll 2
-    for (; from < parts_all; from += stride) {
-      if (at < K) {
-        double r = -INFINITY;
-        int flat = 0;
-        if (state[k] == 1) {
-          const long long place = (long long)(row0 + k) * a.parts + q;
-          const float kept = __ldcg(&a.stats[place].w), x = __ldcg(a.part_v + place * K + at);
-          const int v = __ldcg(a.part_i + place * K + at);
-          if (at < __float_as_int(kept)) {
-            r = with(k, x);
-            if (a.penalty != 0.0) r /= divisor[k];
-            flat = k * a.valid + v;
-          }
-        } else if (state[k] == 2 && q == 0 && at == 0) {
-          r = score[k] / divisor[k];
-          flat = k * a.valid + a.end;
-        }
-        if (!isfinite(r)) r = -INFINITY;
-        all_r[from * K + at] = r;
-        all_i[from * K + at] = flat;
-        most = r > most ? r : most;
-      }
-      for (q += stride; q >= a.parts; q -= a.parts) ++k;
-    }
-  }
-  const double tau = bound_of(most, K, merged_r, &tau_d);
-  // The list takes the place of the ranks that have been looked at: no more entries are before an entry than in front of it.
   __shared__ int at_list;
-  if (tid == 0) at_list = 0;
-  __syncthreads();
-  merged_i = all_i;
-  merged_r = all_r;
+  double widest = 0.0;
+  for (int k = 0; k < K; ++k) widest = fmax(widest, slack[k]);
+  int found;
 #pragma unroll 1
-  for (int e0 = 0; e0 < parts_all * K; e0 += BM_THREADS) {
-    const int e = e0 + tid;
-    const double r = e < parts_all * K ? all_r[e] : -INFINITY;
-    const int flat = e < parts_all * K ? all_i[e] : 0;
+  for (bool again = false;; again = true) {
+    double most = -INFINITY;
+    {
+      int lanes = 1;
+      while (lanes < K) lanes *= 2;
+      const int at = tid & (lanes - 1), stride = BM_THREADS / lanes;
+      int from = tid / lanes, k = from / a.parts, q = from - k * a.parts;
+#pragma unroll 2
+      for (; from < parts_all; from += stride) {
+        if (at < K) {
+          double r = -INFINITY;
+          int flat = 0;
+          if (state[k] == 1) {
+            const long long place = (long long)(row0 + k) * a.parts + q;
+            const float kept = __ldcg(&a.stats[place].w), x = __ldcg(a.part_v + place * K + at);
+            const int v = __ldcg(a.part_i + place * K + at);
+            if (at < __float_as_int(kept)) {
+              r = with(k, x);
+              if (a.penalty != 0.0) r /= divisor[k];
+              flat = k * a.valid + v;
+            }
+          } else if (state[k] == 2 && q == 0 && at == 0) {
+            r = score[k] / divisor[k];
+            flat = k * a.valid + a.end;
+          }
+          if (!isfinite(r)) r = -INFINITY;
+          all_r[from * K + at] = r;
+          all_i[from * K + at] = flat;
+          most = r > most ? r : most;
+        }
+        for (q += stride; q >= a.parts; q -= a.parts) ++k;
+      }
+    }
+    const double tau = bound_of(most, K, room, &tau_d);
+    // The list takes the place of the ranks that have been looked at: no more entries are before an entry than in front of it.
+    if (tid == 0) at_list = 0;
     __syncthreads();
-    if (r >= tau && r > -INFINITY) {
-      const int at = atomicAdd(&at_list, 1);
-      merged_r[at] = r;
-      merged_i[at] = flat;
+#pragma unroll 1
+    for (int e0 = 0; e0 < parts_all * K; e0 += BM_THREADS) {
+      const int e = e0 + tid;
+      const double r = e < parts_all * K ? all_r[e] : -INFINITY;
+      const int flat = e < parts_all * K ? all_i[e] : 0;
+      __syncthreads();
+      if (r >= tau - 2.0 * widest && r > -INFINITY) {
+        const int at = atomicAdd(&at_list, 1);
+        all_r[at] = r;
+        all_i[at] = flat;
+      }
+      __syncthreads();
+    }
+    found = best_of_list(all_r, all_i, at_list, K, chosen_rank, chosen);
+    if (again) break;
+    // Continuations of different rows, one of them chosen, that are closer than the logarithms of their sums are known. (Two that are neither chosen
+    // nor as close as that to one that is need no order.)
+    if (tid < found) row_of[tid] = chosen[tid] / a.valid;
+    __syncthreads();
+#pragma unroll 1
+    for (int e = tid; e < at_list; e += BM_THREADS) {
+      const int k = all_i[e] / a.valid;
+      const double r = all_r[e];
+      unsigned int rows = 0;
+      for (int j = 0; j < found; ++j) {
+        const int o = row_of[j];
+        if (o != k && fabs(r - chosen_rank[j]) <= slack[k] + slack[o]) rows |= 1u << k | 1u << o;
+      }
+      if (rows) atomicOr(&doubt, rows);
     }
     __syncthreads();
+    bool better_sums = false;
+    for (unsigned int rows = doubt; rows; rows &= rows - 1) {
+      const int k = __ffs(rows) - 1;
+      if (state[k] != 1) continue;
+      const double sum = exact_sum(logits + (long long)(row0 + k) * a.V, a.valid, top[k], chosen_rank);
+      if (tid == 0) log_sum[k] = log(sum);
+      better_sums = true;
+    }
+    if (!better_sums) break;
+    __syncthreads();
   }
-  const int found = best_of_list(merged_r, merged_i, at_list, K, chosen_rank, chosen);
   bool any = false;
   for (int k = 0; k < K; ++k) any |= state[k] != 0;
   if (any) {
@@ -548,6 +602,9 @@ XL_API int xl_take_beams(const void* logits, const float* scores, const int* end
   a.current = current; a.parent = parent; a.buf = buf; a.parents = parents; a.step = step; a.counters = counters;
   a.rows = rows; a.V = V; a.valid = valid; a.beams = beams; a.end = end; a.buf_rows = buf_rows; a.base = base; a.ahead = ahead;
   a.advance = advance; a.penalty = penalty;
+  // What a sum's logarithm may be off, relative errors of the sum: a difference x - m and its product with log2(e) are rounded to 2^-24 of themselves,
+  // together 2^-23 |x - m| of the exponential, on average over the sum at most 2^-23 log(entries); the exponential itself 2^-22, four sums in 32 bits 2^-22.
+  a.slack = ldexp(4.0 + log((double)valid), -23);
   a.parts = parts_of(rows, beams, valid);
   a.per_part = ((valid + 8 + a.parts - 1) / a.parts + 31) / 32 * 32;  // whole 16 bytes of any type, with room for a row that starts off a boundary
   a.stats = (float4*)scratch;
