@@ -116,8 +116,8 @@ __global__ void __launch_bounds__(256)
 //   warp 1       MMA: S_m = Q_m K^T into TMEM (both halves of the queries), then O_m += P_m V
 //   warps 4..7   tile 0, warps 8..11 tile 1: norms of the queries, from the projections straight to shared memory; then the softmax, one thread
 //                per row, running maximum and sum in fp32, lazy rescaling of O_m in TMEM (warps 2, 3: none)
-// P replaces S in TMEM as two bf16 numbers per weight. Keys beyond a range are masked in the scores, and their values are zeroed in shared
-// memory: what lies there belongs to others, and a weight of zero times anything that is not finite would reach the sum.
+// P replaces S in TMEM as two bf16 numbers per weight. Keys beyond a range, and those that no row of the tiles sees, are masked in the scores, and their
+// values are zeroed in shared memory: they belong to others, and a weight of zero times anything that is not finite would reach the sum.
 //
 // TMEM columns: [0, 128) S_0 / P_0, [128, 256) S_1 / P_1, [256, 256 + VD) O_0, [256 + VD, 256 + 2 VD) O_1. One CTA per SM. Every wait is
 // bounded (see tcgen05.cuh).
@@ -434,6 +434,7 @@ struct KeyRange {
 struct KeyRanges {  // in shared memory
   KeyRange r[4];
   int until[4];  // blocks of the ranges up to and with this one
+  int kept, first;  // the keys from `kept` to `first` are seen by no row, though blocks may have them
 };
 __device__ __forceinline__ int key_blocks(int begin, int end) { return begin < end ? (end - begin + BKV - 1) / BKV : 0; }
 __device__ __forceinline__ void set_ranges(KeyRanges& k, int b, int lead, int edge, int p_first, int p_last, int window, int keep_first) {
@@ -441,6 +442,8 @@ __device__ __forceinline__ void set_ranges(KeyRanges& k, int b, int lead, int ed
   const int all = key_blocks(0, edge) + key_blocks(edge, p_last + 1);
   const int visible = key_blocks(0, min(seen.kept, edge)) + key_blocks(seen.first, edge) + key_blocks(edge, seen.kept) +
                       key_blocks(max(seen.first, edge), p_last + 1);
+  k.kept = seen.kept;
+  k.first = seen.first;
   if (visible >= all) seen = {0, 0};  // leaving keys out saves no block
   k.r[0] = {lead, 0, min(seen.kept, edge)};
   k.r[1] = {lead, seen.first, edge};
@@ -449,6 +452,8 @@ __device__ __forceinline__ void set_ranges(KeyRanges& k, int b, int lead, int ed
   int n = 0;
   for (int i = 0; i < 4; ++i) k.until[i] = n += key_blocks(k.r[i].begin, k.r[i].end);
 }
+// whether a block of keys from `begin` on has some that no row sees
+__device__ __forceinline__ bool has_unseen(int begin, int end, int kept, int first) { return begin < first && end > kept; }
 // slot, first key, and end of the range, of block j
 __device__ __forceinline__ KeyRange key_block(const KeyRanges& k, int j) {
   int i = 0;
@@ -618,11 +623,14 @@ __global__ void __launch_bounds__(SA_THREADS, 1)
     for (int j = 0; j < n_kv && ok; ++j) {
       const KeyRange x = key_block(keys, j);
       const int col0 = x.begin, hi = min(qpos, x.end - 1);
-      if (m == 0 && col0 + BKV > x.end) {  // the values beyond the range
+      const bool unseen = has_unseen(col0, min(col0 + BKV, x.end), keys.kept, keys.first);
+      if (m == 0 && (col0 + BKV > x.end || unseen)) {  // the values beyond the range, and those that no row sees
         const int n = 2 * j + 1;
         ok = bar_wait_warp(&full[n % SLOTS], (uint32_t)(n / SLOTS) & 1u, abort_flag, p.err, ERR_KV_FULL);
         if (!ok) break;
-        clear_step_rest<VD>(ring + n % SLOTS * L::SLOT, x.end - col0, r);
+        uint8_t* tile = ring + n % SLOTS * L::SLOT;
+        if (col0 + BKV > x.end) clear_step_rest<VD>(tile, x.end - col0, r);
+        if (unseen && col0 + r >= keys.kept && col0 + r < keys.first) clear_value_row<VD>(tile, r);
         fence_proxy_async_smem();
       }
       ok = bar_wait_warp(&s_full[m], (uint32_t)j & 1u, abort_flag, p.err, ERR_S);
@@ -716,7 +724,7 @@ template <int DK, int VD> int launch_portion(const void* kc, const void* vc, con
 // Every CTA makes the list by itself, from positions and leads in shared memory: counts, key ranges and offsets by slot, ranks of the members by
 // votes. CTA 0 leaves a copy for the kernel behind.
 //
-// Keys that only some rows of a tile see are masked; a value that is not finite in a block that some row does not see whole is taken out, and
+// Keys that only some rows of a tile see are masked, and values that none sees zeroed; a value that is not finite in a block that some row does not see whole is taken out, and
 // the scores of its key become NaN for the rows that see it: a weight of zero times anything would reach the others.
 constexpr int PF_MAX_BATCH = 448;
 constexpr int PF_SLOTS_LARGE = 4, PF_SLOTS_SMALL = 8;
@@ -785,6 +793,7 @@ __device__ __forceinline__ int small_quotient(int a, int n) {
 struct alignas(16) GroupSegment {  // blocks [block, block + count) of one tile
   int own, slot, g, tile, block, count, rows;
   int least, latest;  // every row of the tile sees the keys below `least` and from `latest` on
+  int first;          // own keys below this one that are not kept are seen by no row, though blocks may have them
   TileKeys keys;
   __device__ __forceinline__ GroupSegment() : keys(0, 0, 0) {}
 };
@@ -1190,6 +1199,7 @@ __global__ void __launch_bounds__(SA_THREADS, 1)
                      : TileKeys(list.lo[slot], list.hi[slot], p.keep_first);
         g.least = own ? list.pos[slot] + 1 : list.least[slot];
         g.latest = own ? window_range(list.pos[slot] + list.tokens[slot] - 1, p.window, 0).first : list.latest[slot];
+        g.first = own ? list.own_key[slot] : 0;
         const int n = g.keys.total, rows = own ? M : list.members[slot] * M, tiles = (rows + TILE_M - 1) / TILE_M;
         int unit = small_quotient(x - list.begin[i], n);  // tiles by head
         g.g = small_quotient(unit, tiles);
@@ -1274,14 +1284,15 @@ __global__ void __launch_bounds__(SA_THREADS, 1)
         // not every row sees every key; and, of a group, not all rows see the same ones
         const bool cut = key0 + BKV > end || key0 + BKV > sg.least || (key0 < sg.latest && key0 + BKV > p.keep_first);
         const bool uneven = cut && !sg.own && (min(key0 + BKV, end) > sg.least || (key0 < sg.latest && key0 + BKV > p.keep_first));
-        if (uneven || (end - key0 < BKV && (end - key0) % UMMA_K)) {
+        const bool unseen = has_unseen(key0, min(key0 + BKV, end), p.keep_first, sg.first);
+        if (uneven || unseen || (end - key0 < BKV && (end - key0) % UMMA_K)) {
           const int n = 2 * it + 1;
           ok = bar_wait_warp(&full[n % SLOTS], (uint32_t)(n / SLOTS) & 1u, abort_flag, p.err, ERR_KV_FULL);
           if (!ok) break;
           uint8_t* tile = ring + n % SLOTS * L::SLOT;
           if (end - key0 < BKV) clear_step_rest<VD>(tile, end - key0, r);
           const bool finite = !uneven || key0 + r >= end || finite_value_row<VD>(tile, r);  // thread r looks at the value of key r
-          if (!finite) clear_value_row<VD>(tile, r);
+          if (!finite || (unseen && key0 + r >= p.keep_first && key0 + r < sg.first)) clear_value_row<VD>(tile, r);
           fence_proxy_async_smem();
           if (uneven) {
             const unsigned int bits = __ballot_sync(0xffffffffu, !finite);

@@ -162,7 +162,8 @@ def window_attention_shared_(proj: Tensor, q_norm: Tensor, k_norm: Tensor, k_cac
     positions, which have to be in the lead's own cache. New keys and values go to the sequence's own; norms of keys are taken in 64 bits and rounded
     once, queries are not rounded to the model's type. A sequence that would not fit the cache is
     left out, rows past `count[b]` are left as they are. A value that is not finite makes those results non-finite (at least in the feature
-    concerned) that read its position, and may do so for the other results of its own sequence's portion; no other sequence is touched.
+    concerned) that read its position, and may do so for the other results of a sequence's portion of which some read it; portions that do not are
+    not touched.
     On the GPU bf16 models of features up to 128 in multiples of 8 run on the tensor cores, where the keys that a group of sequences shares
     are read once for all of it; all others on the CUDA cores, many times slower."""
     if k_cache.rank != 4 or v_cache.rank != 4:

@@ -62,3 +62,28 @@ def test_large_and_small_tiles_in_turn(members, heads):
     args, kw = case("cuda", torch.bfloat16, B, 1, heads, 1, 64, 64, 120, 100 + place % 7, 1, lead, 100)
     for _ in range(3):
         assert_close(*outputs([a.clone() for a in args], kw))
+
+
+# tokens, position, shared, window, kept first ones, and positions (of the lead: 0, or its own: 1) that no row of sequence 1 sees
+UNSEEN = {"lead's, portion": (64, 120, 100, 64, 0, [(0, 10), (0, 56)]), "lead's behind kept ones, portion": (40, 120, 100, 64, 7, [(0, 7), (0, 56)]),
+          "own, portion": (40, 90, 0, 64, 0, [(1, 3), (1, 26)]), "own behind kept ones, portion": (40, 90, 10, 64, 12, [(1, 12), (1, 26)]),
+          "lead's and own, portion": (40, 110, 20, 64, 2, [(0, 3), (1, 21), (1, 46)]), "several blocks, portion": (40, 300, 10, 160, 100, [(1, 100), (1, 140)]),
+          "lead's, one token": (1, 120, 100, 64, 3, [(0, 3), (0, 56)]), "own, one token": (1, 100, 0, 64, 0, [(1, 3), (1, 36)]),
+          "own behind kept ones, one token": (1, 100, 10, 64, 12, [(1, 12), (1, 36)]), "several blocks, one token": (1, 300, 0, 100, 130, [(1, 130), (1, 200)]),
+          "lead's and own, some tokens": (5, 100, 10, 64, 3, [(0, 3), (1, 12), (1, 36)])}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("junk", [NAN, math.inf])
+@pytest.mark.parametrize("name", list(UNSEEN))
+def test_values_that_no_row_sees_reach_nobody(dt, junk, name):
+    """Not even where leaving their positions out would save no block of keys."""
+    T, pos, shared, window, keep, unseen = UNSEEN[name]
+    assert all(keep <= p <= pos - window and (p < shared) == (b == 0) for b, p in unseen)
+    args, kw = case("cuda", dt, 2, T, 8, 2, 128, 128, 400, pos, T, [7, 0], [0, shared], window=window, keep_first=keep)
+    args[6][0] = 0  # the lead only holds its positions
+    for b, p in unseen:
+        args[4][b, :, p] = junk
+        args[3][b, :, p] = NAN
+    assert_close(*outputs(args, kw))
