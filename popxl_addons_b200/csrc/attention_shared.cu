@@ -618,7 +618,7 @@ __global__ void __launch_bounds__(SA_THREADS, 1)
     const uint32_t tmem_s = tmem_base + lane_base + m * BKV;
     const uint32_t tmem_o = tmem_base + lane_base + 2 * BKV + m * VD;
     const float c = p.scale * 1.4426950408889634f;
-    float mx = p.sink / p.scale, l = p.sink == -INFINITY ? 0.f : 1.f;
+    float mx = p.sink / p.scale, l = mx == -INFINITY ? 0.f : 1.f;  // (in units of the scores a sink far below them all is none)
     bool ok = true;
     for (int j = 0; j < n_kv && ok; ++j) {
       const KeyRange x = key_block(keys, j);
@@ -1377,7 +1377,8 @@ __global__ void __launch_bounds__(128) shared_attn_sum_kernel(const GroupParams 
     const int head = ranges.rem * (per + 1);
     return x < head ? small_quotient(x, per + 1) : ranges.rem + small_quotient(x - head, per);
   };
-  const float sink = p.sink * 1.4426950408889634f;
+  float sink = p.sink * 1.4426950408889634f;
+  if (sink > 3.4e38f) sink = 3.4e38f;  // (infinite in these units, it would leave no number in the difference below)
   // two sources: the tile of the group and the tile of the sequence; of each one CTA's part for each warpgroup from its first block on, then those of
   // the CTAs that follow
   const int own = t * R + h - g * R;  // row in the sequence's tiles

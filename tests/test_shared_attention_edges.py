@@ -87,3 +87,19 @@ def test_values_that_no_row_sees_reach_nobody(dt, junk, name):
         args[4][b, :, p] = junk
         args[3][b, :, p] = NAN
     assert_close(*outputs(args, kw))
+
+
+BACKENDS = [("cuda", torch.bfloat16, 1), ("cuda", torch.bfloat16, 40), ("cuda", torch.float32, 1), ("cuda", torch.float32, 40), ("cuda", torch.float16, 3)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dev,dt,T", BACKENDS)
+@pytest.mark.parametrize("sink", [torch.finfo(torch.float32).min, -1e38, -1e30, 1e38, torch.finfo(torch.float32).max])
+def test_sinks_of_any_size(dev, dt, T, sink):
+    """A sink far below all scores is none, one far above them leaves nothing of the values; neither overflows where scores are counted in other units."""
+    args, kw = case(dev, dt, 3, T, 8, 2, 128, 128, 400, 200, T, 0, 150, sink=sink)
+    got, want = outputs(args, kw)
+    if sink > 0:
+        assert (got == 0).all()
+    else:
+        assert_close(got, want)
