@@ -1415,6 +1415,7 @@ __global__ void __launch_bounds__(128) shared_attn_sum_kernel(const GroupParams 
     if (k0) mine = k0 + lane < all ? stat(k0 + lane) : make_float2(-INFINITY, 0.f);
     const float f = mine.x == -INFINITY ? 0.f : exp2f(mine.x - m);
     total += xl_warp_sum(f * mine.y);  // (a sum that is not a number stays none)
+    const unsigned int holds = __ballot_sync(0xffffffffu, mine.x > -INFINITY);  // parts that had a score (others were not written, or l is no number)
     const int now = min(32, all - k0);
 #pragma unroll 1
     for (int k = 0; k < now; k += 4) {  // four parts under way together, those that hold nothing among them
@@ -1431,7 +1432,8 @@ __global__ void __launch_bounds__(128) shared_attn_sum_kernel(const GroupParams 
       }
 #pragma unroll
       for (int u = 0; u < 4; ++u)
-        if (fk[u] != 0.f) acc = make_float4(acc.x + x[u].x * fk[u], acc.y + x[u].y * fk[u], acc.z + x[u].z * fk[u], acc.w + x[u].w * fk[u]);
+        if (k + u < now && holds >> (k + u) & 1)  // (with a factor of zero too: what is not finite stays so)
+          acc = make_float4(acc.x + x[u].x * fk[u], acc.y + x[u].y * fk[u], acc.z + x[u].z * fk[u], acc.w + x[u].w * fk[u]);
     }
   }
   if (c >= p.vdim) return;

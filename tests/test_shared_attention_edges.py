@@ -103,3 +103,21 @@ def test_sinks_of_any_size(dev, dt, T, sink):
         assert (got == 0).all()
     else:
         assert_close(got, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dev,dt,T", BACKENDS)
+@pytest.mark.parametrize("junk", [NAN, -math.inf])
+def test_values_that_are_not_finite_reach_those_who_see_them_with_any_weight(dev, dt, T, junk):
+    """Scores of -113 and 113: the first block's weights are zero in 32 bits, and in another part than the others."""
+    d, G = 128, 2
+    args, kw = case(dev, dt, 2, T, 4, G, d, d, 1200, 1000, T, [7, 0], [0, 960], wq=10.0, scale=d ** -0.5)
+    args[0][:, :4 * d] = 1.0
+    args[3][:] = 1.0
+    args[3][:, :, :128] = -1.0
+    args[4][0, 1, 10, 3] = junk
+    args[6][0] = 0
+    got, want = outputs(args, kw)
+    got = got.reshape(2, T, 4, d)[1]
+    assert not torch.isfinite(got[:, 2:, 3]).any()
+    assert torch.isfinite(got[:, :2]).all()
