@@ -208,7 +208,7 @@ def take_beams_(current: Tensor, parent: Tensor, logits: Tensor, buf: Tensor, pa
     ends, whatever `ended` holds. NaN among logits counts as minus infinity; where too few continuations are finite those at minus infinity
     follow. A group without a finite score is left as it is, and its rows, like those of beams that have ended, are not read. With
     `advance`, `step` moves on by one."""
-    rows, valid = (logits.shape[0] if logits.rank == 2 else 0), int(valid or logits.shape[-1])
+    rows, valid = (logits.shape[0] if logits.rank == 2 else 0), int(logits.shape[-1] if valid is None else valid)
     if logits.rank != 2 or logits.dtype not in (float32, float16, bfloat16):
         raise ValueError(f"logits are rows of floating-point numbers, not {tuple(logits.shape)} {logits.dtype}")
     if not 1 <= beams <= MAX_BEAMS or rows < 1 or rows % beams:

@@ -1,0 +1,29 @@
+"""What the ops and the generator of sequences with a common beginning refuse, beside what the tests of each of them have."""
+import pytest
+
+from popxl_addons_b200 import xl
+from popxl_addons_b200.xl import ops
+
+
+def var(shape, dt=xl.int32):
+    return xl.variable(xl.LazyInit(shape, kind="zeros"), dt)
+
+
+@pytest.fixture
+def graph():
+    ir = xl.Ir()
+    with ir.main_graph:
+        yield ir
+
+
+def choose(n=8, **kw):
+    """A call of `take_beams_` with tensors of its own, but for those given."""
+    kw = dict(current=var((n,)), parent=var((n,)), logits=var((n, 50), xl.float32), buf=var((5, n)), parents=var((5, n)), step=var((1,)),
+              state=ops.BeamState(var((n,), xl.float32), var((n,)), var((n,))), beams=min(n, 4)) | kw
+    return ops.take_beams_(**kw)
+
+
+def test_a_choice_among_no_entries(graph):
+    choose(valid=50)
+    with pytest.raises(ValueError, match="choice among 0 entries"):
+        choose(valid=0)
