@@ -226,7 +226,7 @@ def take_beams_(current: Tensor, parent: Tensor, logits: Tensor, buf: Tensor, pa
         _expect(what, t, (rows,), int32)
     if any(t.rank != 2 or t.shape[1] != rows or t.dtype != int32 for t in (buf, parents)) or buf.shape != parents.shape:
         raise ValueError(f"the choices of {rows} beams are kept in rows of two int32 buffers, not {tuple(buf.shape)} and {tuple(parents.shape)}")
-    written = [current, parent, buf, parents, *(into or state)]
+    written = [current, parent, buf, parents, step, *(into or state)]
     if len({id(t) for t in written}) < len(written):
         raise ValueError("the results of a choice go to tensors of their own")
     if step.dtype != int32 or step.nelms != 1:

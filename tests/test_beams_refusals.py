@@ -27,3 +27,12 @@ def test_a_choice_among_no_entries(graph):
     choose(valid=50)
     with pytest.raises(ValueError, match="choice among 0 entries"):
         choose(valid=0)
+
+
+def test_results_on_top_of_the_step(graph):
+    """One beam: its token and the number of the step have the same shape, and whether the step is read first is up to the kernel."""
+    choose(1)
+    for name in ("current", "parent", "buf", "parents"):
+        step = var((1, 1)) if name.startswith("b") or name == "parents" else var((1,))
+        with pytest.raises(ValueError, match="of their own"):
+            choose(1, **{"step": step, name: step}, **({"parents": var((1, 1))} if name == "buf" else {"buf": var((1, 1))} if name == "parents" else {}))
