@@ -174,6 +174,8 @@ def window_attention_shared_(proj: Tensor, q_norm: Tensor, k_norm: Tensor, k_cac
     _expect("v_cache", v_cache, (B, G, smax, vdim), proj.dtype)
     if k_cache is v_cache:
         raise ValueError("keys and values cannot be held in one tensor")
+    if joint is proj:
+        raise ValueError("the results cannot lie on top of the projections, which are read until the last one is written")
     if max(dim, vdim) > 512:
         raise ValueError(f"the attention kernels take dim and vdim up to 512, not {dim} and {vdim}")
     if heads < 1 or heads % G:

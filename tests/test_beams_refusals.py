@@ -36,3 +36,14 @@ def test_results_on_top_of_the_step(graph):
         step = var((1, 1)) if name.startswith("b") or name == "parents" else var((1,))
         with pytest.raises(ValueError, match="of their own"):
             choose(1, **{"step": step, name: step}, **({"parents": var((1, 1))} if name == "buf" else {"buf": var((1, 1))} if name == "parents" else {}))
+
+
+def test_attention_on_top_of_its_projections(graph):
+    def call(proj, joint):
+        k, v = var((3, 2, 30, 16), xl.float32), var((3, 2, 30, 24), xl.float32)
+        return ops.window_attention_shared_(proj, var((16,), xl.float32), var((16,), xl.float32), k, v, *(var((3,)) for _ in range(4)), joint, 1, 4, 0.5)
+
+    proj = var((3, 240), xl.float32)
+    call(proj, var((3, 240), xl.float32))
+    with pytest.raises(ValueError, match="on top of the projections"):
+        call(proj, proj)
