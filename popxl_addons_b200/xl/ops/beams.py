@@ -21,6 +21,7 @@ from .sequence import _rms
 from .serving import _expect
 
 MAX_BEAMS = 32          # of a group
+MAX_PENALTY = 32        # any number of tokens to this power, 2^992 at most, is a number in 64 bits, and sums divided by it are still unlike each other
 
 
 class BeamState(NamedTuple):
@@ -219,8 +220,8 @@ def take_beams_(current: Tensor, parent: Tensor, logits: Tensor, buf: Tensor, pa
         raise ValueError(f"a choice among {valid} entries from rows of {logits.shape[1]}")
     if end is not None and not 0 <= end < valid:
         raise ValueError(f"the end is a token below {valid}, not {end}")
-    if not abs(length_penalty) <= 100:
-        raise ValueError(f"a length penalty is a number up to 100, not {length_penalty}")
+    if not abs(length_penalty) <= MAX_PENALTY:
+        raise ValueError(f"a length penalty is a number up to {MAX_PENALTY}, not {length_penalty}")
     for what, s in (("state", state), ("into", into)):
         for field, t, dt in zip(BeamState._fields, s or (), (float32, int32, int32)):
             _expect(f"{what}.{field}", t, (rows,), dt)

@@ -1,8 +1,12 @@
 """What the ops and the generator of sequences with a common beginning refuse, beside what the tests of each of them have."""
+import math
+
 import pytest
+import torch
 
 from popxl_addons_b200 import xl
 from popxl_addons_b200.xl import ops
+from test_beams_ops import backend, check_beams  # noqa: F401  (fixture and helper)
 
 
 def var(shape, dt=xl.int32):
@@ -47,3 +51,21 @@ def test_attention_on_top_of_its_projections(graph):
     call(proj, var((3, 240), xl.float32))
     with pytest.raises(ValueError, match="on top of the projections"):
         call(proj, proj)
+
+
+@pytest.mark.parametrize("penalty", [ops.MAX_PENALTY, -ops.MAX_PENALTY])
+def test_the_largest_length_penalties(backend, penalty):  # noqa: F811
+    """Sums of unlike beams stay unlike when divided by the largest number of tokens to the largest power."""
+    g = torch.Generator().manual_seed(1)
+    logits = torch.randn(4, 200, generator=g).to(backend[1])
+    for tokens in (1, 1500, 0x7ffffff0):
+        length = torch.full((4,), tokens, dtype=torch.int32)
+        assert math.isfinite(float(tokens + 1) ** penalty)
+        check_beams(backend, logits, torch.tensor([-1.0, -1.25, -2.0, -0.5]), torch.zeros(4, dtype=torch.int32), length, 4, 3, 200, float(penalty))
+
+
+def test_length_penalties_whose_powers_overflow(graph):
+    choose(length_penalty=float(ops.MAX_PENALTY))
+    for penalty in (100.0, -100.0, 32.5):  # 2000 tokens to the power of 100 are infinite, and all sums divided by it zero
+        with pytest.raises(ValueError, match="length penalty"):
+            choose(length_penalty=penalty)
