@@ -188,6 +188,8 @@ class SequenceGenerator:
             raise ValueError(f"request {request!r} asks for adapter {adapter} of {self.adapters}")
         if shaping is not None and not self.shaping:
             raise ValueError("this program was made without shaping=True")
+        if prefix is not None and prefix_of is None:
+            raise ValueError(f"{prefix} positions are to be shared, and no request to share them with is named")
         lead, shared = self._lead_of(prefix_of, prefix, adapter) if prefix_of is not None else (None, 0)
         slot = self._free[-1]
         if self.shaping:

@@ -69,3 +69,15 @@ def test_length_penalties_whose_powers_overflow(graph):
     for penalty in (100.0, -100.0, 32.5):  # 2000 tokens to the power of 100 are infinite, and all sums divided by it zero
         with pytest.raises(ValueError, match="length penalty"):
             choose(length_penalty=penalty)
+
+
+def test_a_prefix_of_nobody():
+    import zirunex_cases as C
+    from test_beams import MODEL, generator
+
+    gen = generator(("cpu", "float32"), C.checkpoint(MODEL, 1), options={"shared_prefixes": True})
+    gen.admit("x")
+    gen.step({"x": [1, 2, 3]})
+    with pytest.raises(ValueError, match="no request"):
+        gen.admit("y", prefix=2)
+    assert gen.slots == {"x": 0} and len(gen._free) == 2
