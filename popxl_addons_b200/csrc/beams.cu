@@ -28,6 +28,7 @@ constexpr int BM_THREADS = 256;
 constexpr int BM_EACH = 16;                       // entries of a thread in a chunk
 constexpr int BM_CHUNK = BM_THREADS * BM_EACH;
 constexpr int BM_MAX_BEAMS = 32;
+constexpr double BM_MAX_PENALTY = 32.0;           // any number of tokens to this power is finite
 constexpr int BM_MAX_PARTS = 16;                  // each part costs the merge its loads
 constexpr int BM_KEEP = 512;                      // a longer list is cut to its best between two chunks
 constexpr int BM_MERGED = 2048;                   // entries that the parts of a group leave, at most
@@ -120,6 +121,8 @@ __device__ __forceinline__ float exp_below(float d) {
 struct BeamArgs {
   const float* scores;
   const int *ended, *length;
+  const int* rule_end;          // what `end` and `penalty` are, if the device holds them, else null
+  const double* rule_penalty;
   float* to_scores;
   int *to_ended, *to_length;
   int *current, *parent, *buf, *parents, *step;
@@ -131,6 +134,13 @@ struct BeamArgs {
   double penalty;
   double slack;  // how far the logarithm of a row's sum may be off, see xl_take_beams
 };
+
+// the token that ends a beam, or a negative number
+__device__ __forceinline__ int end_of(const BeamArgs& a) {
+  int end = a.end;
+  if (a.rule_end) end = *a.rule_end;
+  return end < a.valid ? end : -1;
+}
 
 // A sum of exponentials relative to `m` as one relative to `now`, the larger one: rare, and out of the way of the loop's registers.
 __device__ __noinline__ double rescaled(double sum, float m, float now) { return m > -INFINITY ? sum * exp((double)m - (double)now) : 0.0; }
@@ -171,7 +181,7 @@ template <typename T> __global__ void __launch_bounds__(BM_THREADS, 5) take_beam
   if (tid == 0) listed = 0;
   xl_grid_dependency_wait();
   xl_grid_launch_dependents();
-  const bool live = isfinite(a.scores[row]) && !(a.end >= 0 && a.ended[row] != 0);
+  const bool live = isfinite(a.scores[row]) && !(end_of(a) >= 0 && a.ended[row] != 0);
   __syncthreads();
   if (live) {
     const T* p = logits + (long long)row * a.V;
@@ -300,13 +310,17 @@ template <typename T> __global__ void __launch_bounds__(BM_THREADS, 5) take_beam
   __shared__ int chosen[BM_MAX_BEAMS], state[BM_MAX_BEAMS], after[BM_MAX_BEAMS], slot_of[BM_MAX_BEAMS], row_of[BM_MAX_BEAMS];  // state 0: no beam, 1: live, 2: ended
   const int row0 = group * K;
   double* room = reinterpret_cast<double*>(smem);  // [BM_THREADS] for the bound
+  const int end = end_of(a);
+  double penalty = a.penalty;
+  if (a.rule_penalty) penalty = *a.rule_penalty;
+  if (!(fabs(penalty) <= BM_MAX_PENALTY)) penalty = 0.0;
   if (tid < K) {
     const float f = a.scores[row0 + tid];
-    const bool ended = a.end >= 0 && a.ended[row0 + tid] != 0;
+    const bool ended = end >= 0 && a.ended[row0 + tid] != 0;
     state[tid] = !isfinite(f) ? 0 : ended ? 2 : 1;
     score[tid] = (double)f;
     after[tid] = a.length[row0 + tid] + (ended ? 0 : 1);
-    divisor[tid] = a.penalty == 0.0 ? 1.0 : pow((double)max(after[tid], 1), a.penalty);
+    divisor[tid] = penalty == 0.0 ? 1.0 : pow((double)max(after[tid], 1), penalty);
     slack[tid] = state[tid] == 1 ? a.slack / divisor[tid] : 0.0;  // (the only continuation of an ended beam has the sum that the beam has)
   }
   if (tid == 0) doubt = 0;
@@ -360,12 +374,12 @@ template <typename T> __global__ void __launch_bounds__(BM_THREADS, 5) take_beam
             const int v = __ldcg(a.part_i + place * K + at);
             if (at < __float_as_int(kept)) {
               r = with(k, x);
-              if (a.penalty != 0.0) r /= divisor[k];
+              if (penalty != 0.0) r /= divisor[k];
               flat = k * a.valid + v;
             }
           } else if (state[k] == 2 && q == 0 && at == 0) {
             r = score[k] / divisor[k];
-            flat = k * a.valid + a.end;
+            flat = k * a.valid + end;
           }
           if (!isfinite(r)) r = -INFINITY;
           all_r[from * K + at] = r;
@@ -448,7 +462,7 @@ template <typename T> __global__ void __launch_bounds__(BM_THREADS, 5) take_beam
       double c = -INFINITY;
       if (tid < found) c = state[k] == 2 ? score[k] : with(k, xl_to_float(logits[(long long)(row0 + k) * a.V + token]));
       a.to_scores[to] = (float)c;
-      a.to_ended[to] = state[k] == 2 || token == a.end;
+      a.to_ended[to] = state[k] == 2 || token == end;
       a.to_length[to] = after[k];
       a.current[to] = token;
       a.parent[to] = row0 + k;
@@ -588,18 +602,19 @@ XL_API int xl_take_beams_parts(int rows, int beams, int valid) {
 // logits (rows, V), of which the first `valid` entries count; rows are groups of `beams`. scores, ended, length (rows) -> to_* (rows, may be the same).
 // The choices become current, parent (rows) and row *step + ahead - base of buf, parents (buf_rows, rows); with `advance` *step moves on. end < 0: no beam
 // ends. scratch: rows * parts * (16 + 8 beams) bytes, 16-byte aligned, with parts = xl_take_beams_parts; counters: rows / beams + 1 zero-initialised
-// words (left zeroed).
+// words (left zeroed). rule_end, rule_penalty: both null, or one number each that is read instead of `end` and `penalty`.
 XL_API int xl_take_beams(const void* logits, const float* scores, const int* ended, const int* length, float* to_scores, int* to_ended,
                          int* to_length, int* current, int* parent, int* buf, int* parents, int* step, void* scratch, unsigned int* counters,
-                         int rows, int V, int valid, int beams, int end, double penalty, int buf_rows, int base, int ahead, int advance, int dtype,
+                         const int* rule_end, const double* rule_penalty, int rows, int V, int valid, int beams, int end, double penalty, int buf_rows, int base, int ahead, int advance, int dtype,
                          cudaStream_t s) {
   if (rows < 1 || rows > 65535 || beams < 1 || beams > BM_MAX_BEAMS || rows % beams || valid < 1 || valid > V || V > 0x7fff0000 ||
       (long long)valid * beams > 0x7fffffffLL || end >= valid || !scores || !ended || !length || !to_scores || !to_ended || !to_length ||
-      !current || !parent || !buf || !parents || !step || !scratch || ((uintptr_t)scratch & 15) || !counters)
+      !current || !parent || !buf || !parents || !step || !scratch || !rule_end != !rule_penalty || ((uintptr_t)rule_penalty & 7) || ((uintptr_t)scratch & 15) || !counters)
     return -1;
   BeamArgs a = {};
   a.scores = scores; a.ended = ended; a.length = length; a.to_scores = to_scores; a.to_ended = to_ended; a.to_length = to_length;
   a.current = current; a.parent = parent; a.buf = buf; a.parents = parents; a.step = step; a.counters = counters;
+  a.rule_end = rule_end; a.rule_penalty = rule_penalty;
   a.rows = rows; a.V = V; a.valid = valid; a.beams = beams; a.end = end; a.buf_rows = buf_rows; a.base = base; a.ahead = ahead;
   a.advance = advance; a.penalty = penalty;
   // What a sum's logarithm may be off, relative errors of the sum: a difference x - m and its product with log2(e) are rounded to 2^-24 of themselves,

@@ -123,7 +123,8 @@ class SequenceGenerator:
                 state.update(lead=((batch,), xl.int32), shared=((batch,), xl.int32))
             if beams:
                 rows = ((batch,), xl.int32)
-                state.update(scores=((batch,), xl.float32), ended=rows, length=rows, parent=rows, begin=rows, parents=((max_new_tokens, batch), xl.int32))
+                state.update(scores=((batch,), xl.float32), ended=rows, length=rows, parent=rows, begin=rows, parents=((max_new_tokens, batch), xl.int32),
+                             end=((1,), xl.int32), length_penalty=((1,), xl.float64))
             for name, (shape, dt) in state.items():
                 self._vars[name] = xl.variable(xl.LazyInit(shape, np.float32, "zeros"), dt, name)
                 self._mutable.add(name)
@@ -280,14 +281,15 @@ class SequenceGenerator:
         else:
             ops.take_greedy_(t("current"), self.model.logits(t, h), t("generated"), t("step"), self.model.vocab)
 
-    def _choose_beams(self, t, h, first: bool, end: Optional[int], length_penalty: float):
+    def _choose_beams(self, t, h, first: bool):
         """The next beams of every group become the current tokens, and their states follow. Positions have moved on already. `first`: the prompt is one
         beam's so far, and what its other beams cannot share is copied."""
         logits = self.model.logits(t, h)
         if self.shaping:
             logits = ops.shape_logits(logits, xl.constant(np.arange(self.batch), xl.int32, "slots"), t("pos"), self._rules(t))
         ops.take_beams_(t("current"), t("parent"), logits, t("generated"), t("parents"), t("step"),
-                        ops.BeamState(t("scores"), t("ended"), t("length")), self.beams, end, self.model.vocab, length_penalty)
+                        ops.BeamState(t("scores"), t("ended"), t("length")), self.beams, valid=self.model.vocab,
+                        rule=ops.BeamRule(t("end"), t("length_penalty")))
         begin = xl.constant(np.zeros(self.batch), xl.int32, "begin") if first else t("begin")
         rows = [ops.StateRows(t(name), *where) for name, where in self.model.state_positions().items()
                 if not (first and self.shares and where[0] is not None)]
@@ -301,8 +303,8 @@ class SequenceGenerator:
     def _rules(t) -> ops.LogitRules:
         return ops.LogitRules(*(t(k) for k in ops.LogitRules._fields))
 
-    def _portion_program(self, T: int, sample):
-        """`sample`: whether the portion ends in a choice; or the arguments of a first choice of beams."""
+    def _portion_program(self, T: int, choice: Optional[str] = None):
+        """`choice`: what the portion ends in, a "sample" of every slot or the first choice of "beams" (None: in neither)."""
         def build(entry, t):
             entry["tokens"] = xl.h2d_stream((self.batch * T,), xl.int32, f"tokens_{T}")
             ctrl = ops.host_load(self._ctrl_in)
@@ -312,26 +314,26 @@ class SequenceGenerator:
             self.model.portion(T, t, tokens, t("pos"), t("count"), final_norm=False)
             if self.shaping:
                 ops.append_tokens_(t("history"), tokens, t("pos"), t("count"), T)
-            if self.shaping or isinstance(sample, tuple):
+            if self.shaping or choice == "beams":
                 ops.advance_by_(t("pos"), t("count"))
-            if isinstance(sample, tuple):
+            if choice == "beams":
                 h = self.model.select(t, t("count"), stride=T, offset=1)
                 ops.var_updates.copy_var_update_(t("count"), xl.constant(np.ones(self.batch), xl.int32, "each"))  # from here on every beam goes on
-                self._choose_beams(t, h, True, *sample)
-            elif sample:
+                self._choose_beams(t, h, True)
+            elif choice:
                 self._sample(t, self.model.select(t, t("count"), stride=T, offset=1))
-            if not self.shaping and not isinstance(sample, tuple):
+            if not self.shaping and choice != "beams":
                 ops.advance_by_(t("pos"), t("count"))
 
-        return self._program(("portion", T, "sample", *(sample if isinstance(sample, tuple) else ())) if sample else ("portion", T), build)
+        return self._program(("portion", T, choice) if choice else ("portion", T), build)
 
-    def _beams_program(self, end: Optional[int], length_penalty: float):
+    def _beams_program(self):
         def build(entry, t):
             h = self.model.portion(1, t, t("current"), t("pos"), t("count"), final_norm=True)
             ops.advance_by_(t("pos"), t("count"))
-            self._choose_beams(t, h, False, end, length_penalty)
+            self._choose_beams(t, h, False)
 
-        return self._program(("beams", end, length_penalty), build)
+        return self._program(("beams",), build)
 
     def _decode_program(self):
         def build(entry, t):
@@ -355,10 +357,10 @@ class SequenceGenerator:
         return self._program(("logits", n, "shaped") if shaped else ("logits", n), build)
 
     # -- steps -----------------------------------------------------------------------------------------------------------
-    def _run_portion(self, part: Mapping[int, Sequence[int]], sample=False) -> int:
-        """`part`: slot -> its next tokens (at most `max_portion`). Returns the rows per sequence of the program."""
+    def _run_portion(self, part: Mapping[int, Sequence[int]], choice: Optional[str] = None) -> int:
+        """`part`: slot -> its next tokens (at most `max_portion`); `choice`: see `_portion_program`. Returns the rows per sequence of the program."""
         T = portion_size(max(len(v) for v in part.values()))
-        entry = self._portion_program(T, sample)
+        entry = self._portion_program(T, choice)
         tokens = np.zeros((self.batch, T), np.int32)
         ctrl = np.zeros((2, self.batch), np.int32)
         ctrl[0] = self.lengths
@@ -444,7 +446,7 @@ class SequenceGenerator:
             self.step({r: h for r, h in head.items() if len(h)})
             self._set_device("step", 0)
             self.session.record_timestamp("start")
-            self._run_portion({slot[r]: last[r] for r in reqs}, sample=True)
+            self._run_portion({slot[r]: last[r] for r in reqs}, choice="sample")
             self.session.record_timestamp("prefill_done")
             self._set_device("count", [1 if s in slot.values() else 0 for s in range(self.batch)])
             decode = self._decode_program()["program"]
@@ -475,6 +477,8 @@ class SequenceGenerator:
             raise RuntimeError("generate_beams() needs all slots: release the live requests first")
         if end is not None and not 0 <= end < self.model.vocab:
             raise ValueError(f"the end is a token below {self.model.vocab}, not {end}")
+        if not abs(length_penalty) <= ops.MAX_PENALTY:
+            raise ValueError(f"a length penalty is a number up to {ops.MAX_PENALTY}, not {length_penalty}")
         if any(len(p) < 1 or len(p) + max_new_tokens - 1 > self.max_seq for p in prompts):
             raise ValueError(f"prompts must hold between 1 and {self.max_seq - max_new_tokens + 1} tokens")
         shaping = [shaping] * len(prompts) if shaping is None or isinstance(shaping, LogitShaping) else list(shaping)
@@ -504,14 +508,14 @@ class SequenceGenerator:
                     if self.shares:
                         self._share(g * K + k, g * K, len(prompts[g]))
             self._set_device("step", 0)
-            for name, value in (("ended", 0), ("length", 0), ("scores", [0.0 if s % K == 0 and s < n * K else -math.inf for s in range(self.batch)]),
+            for name, value in (("end", -1 if end is None else end), ("length_penalty", length_penalty), ("ended", 0), ("length", 0), ("scores", [0.0 if s % K == 0 and s < n * K else -math.inf for s in range(self.batch)]),
                                 ("begin", [len(prompts[s // K]) if s < n * K else 0 for s in range(self.batch)])):
                 self._set_device(name, value)
             self.session.record_timestamp("start")
-            self._run_portion({g * K: last[g] for g in range(n)}, sample=(end, length_penalty))
+            self._run_portion({g * K: last[g] for g in range(n)}, choice="beams")
             self.session.record_timestamp("prefill_done")
             self._set_device("count", [1 if s < n * K else 0 for s in range(self.batch)])
-            program, steps = self._beams_program(end, length_penalty)["program"], 1
+            program, steps = self._beams_program()["program"], 1
             while steps < n_new:
                 self.session.run_program(program, fetch=False)
                 steps += 1

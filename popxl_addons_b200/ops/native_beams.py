@@ -5,6 +5,7 @@ import functools
 import torch
 
 from ..xl.opdef import native
+from ..xl.ops.beams import into_and_rule
 from .native import _CODE, _c_f, _c_int, _c_ll, _c_p, _count, _sig, _sms, _stream, counters, gemm_error_flag, workspace
 from .native_sequence import _f32, _i32, _ptr
 from .native_serving import _c_d, _done, _launched, _rows16
@@ -14,7 +15,7 @@ _shared_general = _sig("xl_shared_attn_general", *[_c_p] * 4, _c_ll, _c_p, _c_ll
 _shared_portion = _sig("xl_shared_attn_portion", _c_p, _c_ll, *[_c_p] * 4, _c_ll, *[_c_p] * 4, *[_c_int] * 10, *[_c_f] * 3, _c_p, _c_p)
 _shared_groups = _sig("xl_shared_attn_groups", _c_p, _c_ll, *[_c_p] * 4, _c_ll, *[_c_p] * 4, *[_c_int] * 10, *[_c_f] * 3, _c_int, _c_p, _c_p, _c_p)
 _shared_groups_scratch = _sig("xl_shared_attn_groups_scratch", *[_c_int] * 5, restype=_c_ll)
-_take_beams = _sig("xl_take_beams", *[_c_p] * 14, *[_c_int] * 5, _c_d, *[_c_int] * 5, _c_p)
+_take_beams = _sig("xl_take_beams", *[_c_p] * 16, *[_c_int] * 5, _c_d, *[_c_int] * 5, _c_p)
 _take_beams_parts = _sig("xl_take_beams_parts", _c_int, _c_int, _c_int)
 _reorder = _sig("xl_reorder", ctypes.POINTER(_c_ll), _c_int, *[_c_p] * 3, _c_int, _c_int, _c_p)
 
@@ -90,9 +91,12 @@ def window_attention_shared_cuda(proj, q_norm, k_norm, kc, vc, pos, count, lead,
 
 @native("take_beams_")
 @_on_their_device
-def take_beams_cuda(current, parent, logits, buf, parents, step, scores, ended, length, *into, beams, end, valid, length_penalty, base, ahead,
+def take_beams_cuda(current, parent, logits, buf, parents, step, scores, ended, length, *more, beams, end, valid, length_penalty, base, ahead,
                     advance):
+    into, rule = into_and_rule(more)
     to = into or (scores, ended, length)
+    if rule and not (_i32(rule[0]) and rule[1].is_cuda and rule[1].dtype == torch.float64):
+        return NotImplemented
     rows = logits.shape[0]
     if not logits.is_cuda or logits.dtype not in _CODE or not _i32(current, parent, buf, parents, step, ended, length, to[1], to[2]):
         return NotImplemented
@@ -103,8 +107,8 @@ def take_beams_cuda(current, parent, logits, buf, parents, step, scores, ended, 
     scratch = workspace(rows * parts * (16 + 8 * beams), dev, "beams")
     done = counters(rows // beams + 1, dev, "counters beams")
     rc = _take_beams(logits.data_ptr(), scores.data_ptr(), ended.data_ptr(), length.data_ptr(), *map(_ptr, to), current.data_ptr(), parent.data_ptr(),
-                     buf.data_ptr(), parents.data_ptr(), step.data_ptr(), scratch.data_ptr(), done.data_ptr(), rows, logits.shape[1], valid, beams,
-                     end, length_penalty, buf.shape[0], base, ahead, int(advance), _CODE[logits.dtype], _stream())
+                     buf.data_ptr(), parents.data_ptr(), step.data_ptr(), scratch.data_ptr(), done.data_ptr(), *(map(_ptr, rule or (None, None))),
+                     rows, logits.shape[1], valid, beams, end, length_penalty, buf.shape[0], base, ahead, int(advance), _CODE[logits.dtype], _stream())
     return current if _launched(rc, "take_beams") else NotImplemented
 
 

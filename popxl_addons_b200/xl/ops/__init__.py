@@ -1403,7 +1403,7 @@ from .sequence import (embed_dyt_, linear_residual_dyt_, select_dyt, linear_rows
                        window_attention_)
 from .serving import (Adapters, Cache8, LogitRules, CACHE8_BLOCK, MAX_BIASES, MAX_HISTORY, MAX_RANK, append_tokens_, cache8_spec, linear_adapted, residual_rms_,  # noqa: E402
                       shape_logits, split_glu, take_shaped_, window_attention_q8_)
-from .beams import BeamState, MAX_BEAMS, MAX_PENALTY, StateRows, reorder_, take_beams_, window_attention_shared_  # noqa: E402
+from .beams import BeamRule, BeamState, MAX_BEAMS, MAX_PENALTY, StateRows, reorder_, take_beams_, window_attention_shared_  # noqa: E402
 from .extra import *  # noqa: E402,F401,F403
 # module paths of popxl (`ops.call`, `ops.utils`): loaded here so that a later `from ...ops.call import CallSiteInfo`
 # finds the submodule already imported and the name `call` stays bound to the function

@@ -14,7 +14,7 @@ from typing import NamedTuple, Optional, Sequence
 import torch
 
 from ..core import Tensor
-from ..dtypes import bfloat16, float16, float32, int32
+from ..dtypes import bfloat16, float16, float32, float64, int32
 from ..opdef import OpDef, emit, emit1
 from .decode import _store_row_ref
 from .sequence import _rms
@@ -30,6 +30,13 @@ class BeamState(NamedTuple):
     scores: Tensor
     ended: Tensor
     length: Tensor
+
+
+class BeamRule(NamedTuple):
+    """What a choice of beams goes by, held on the device, so that one program serves any: `end (1,)` int32 (a number that is no token: no
+    beam ends) and `length_penalty (1,)` float64 (not a number up to `MAX_PENALTY`: none)."""
+    end: Tensor
+    length_penalty: Tensor
 
 
 class StateRows(NamedTuple):
@@ -92,11 +99,21 @@ def place_beams(parents: Sequence[int]) -> list:
     return out
 
 
-def _take_beams_ref(current, parent, logits, buf, parents, step, scores, ended, length, *into, beams, end, valid, length_penalty, base, ahead,
+def into_and_rule(more) -> tuple:
+    """The optional tensors of `take_beams_`: those that results go to, three or none, and the rule's, two or none."""
+    n = len(more) // 3 * 3
+    return more[:n], more[n:]
+
+
+def _take_beams_ref(current, parent, logits, buf, parents, step, scores, ended, length, *more, beams, end, valid, length_penalty, base, ahead,
                     advance):
     if logits.device.type == "meta":
         return current
+    into, rule = into_and_rule(more)
     to_scores, to_ended, to_length = into or (scores, ended, length)
+    if rule:
+        end, length_penalty = int(rule[0].reshape(-1)[0]), float(rule[1].reshape(-1)[0])
+        end, length_penalty = end if 0 <= end < valid else -1, length_penalty if abs(length_penalty) <= MAX_PENALTY else 0.0
     at, dev = int(step.reshape(-1)[0]) + ahead - base, logits.device
     rows = [(t, t[at].clone() if 0 <= at < t.shape[0] else t.new_zeros(t.shape[1])) for t in (buf, parents)]
     for g in range(logits.shape[0] // beams):
@@ -200,7 +217,7 @@ def window_attention_shared_(proj: Tensor, q_norm: Tensor, k_norm: Tensor, k_cac
 
 def take_beams_(current: Tensor, parent: Tensor, logits: Tensor, buf: Tensor, parents: Tensor, step: Tensor, state: BeamState, beams: int,
                 end: Optional[int] = None, valid: Optional[int] = None, length_penalty: float = 0.0, into: Optional[BeamState] = None,
-                base: int = 0, ahead: int = 0, advance: bool = True) -> Tensor:
+                base: int = 0, ahead: int = 0, advance: bool = True, rule: Optional[BeamRule] = None) -> Tensor:
     """One step of beam search. Row `i` of `logits (rows, vocab)` continues beam `i` of group `i // beams` by every token below `valid`, at
     the sum `scores[i] + log_softmax(logits[i])`; a beam that has ended only by `end`, at the sum that it has. The `beams` continuations of
     a group with the largest `sum / tokens ** length_penalty` are its next beams: token `current[s]` of slot `s` continues slot
@@ -208,7 +225,7 @@ def take_beams_(current: Tensor, parent: Tensor, logits: Tensor, buf: Tensor, pa
     lowest slot and then the lowest token is taken. The best continuation of a beam keeps its slot, the others take the free ones, in
     order of rank. Sums are compared in 64 bits (on the GPU those of a row are formed from exponentials in 32, and again in 64 where the choice hangs
     on it) and kept in 32, in `into` (default: `state` itself). Without `end` no beam
-    ends, whatever `ended` holds. NaN among logits counts as minus infinity; where too few continuations are finite those at minus infinity
+    ends, whatever `ended` holds. `rule`: `end` and `length_penalty` are those that the device holds. NaN among logits counts as minus infinity; where too few continuations are finite those at minus infinity
     follow. A group without a finite score is left as it is, and its rows, like those of beams that have ended, are not read. With
     `advance`, `step` moves on by one."""
     rows, valid = (logits.shape[0] if logits.rank == 2 else 0), int(logits.shape[-1] if valid is None else valid)
@@ -222,6 +239,11 @@ def take_beams_(current: Tensor, parent: Tensor, logits: Tensor, buf: Tensor, pa
         raise ValueError(f"the end is a token below {valid}, not {end}")
     if not abs(length_penalty) <= MAX_PENALTY:
         raise ValueError(f"a length penalty is a number up to {MAX_PENALTY}, not {length_penalty}")
+    if rule is not None:
+        if end is not None or length_penalty:
+            raise ValueError("a choice goes by a rule that the device holds, or by an end and a length penalty given here")
+        _expect("rule.end", rule.end, (1,), int32)
+        _expect("rule.length_penalty", rule.length_penalty, (1,), float64)
     for what, s in (("state", state), ("into", into)):
         for field, t, dt in zip(BeamState._fields, s or (), (float32, int32, int32)):
             _expect(f"{what}.{field}", t, (rows,), dt)
@@ -229,12 +251,12 @@ def take_beams_(current: Tensor, parent: Tensor, logits: Tensor, buf: Tensor, pa
         _expect(what, t, (rows,), int32)
     if any(t.rank != 2 or t.shape[1] != rows or t.dtype != int32 for t in (buf, parents)) or buf.shape != parents.shape:
         raise ValueError(f"the choices of {rows} beams are kept in rows of two int32 buffers, not {tuple(buf.shape)} and {tuple(parents.shape)}")
-    written = [current, parent, buf, parents, step, *(into or state)]
+    written = [current, parent, buf, parents, step, *(into or state), *(rule or ())[:1]]
     if len({id(t) for t in written}) < len(written):
         raise ValueError("the results of a choice go to tensors of their own")
     if step.dtype != int32 or step.nelms != 1:
         raise ValueError(f"the choices of a step have one position in int32, not {tuple(step.shape)} {step.dtype}")
-    return emit1("take_beams_", [current, parent, logits, buf, parents, step, *state, *(into or ())],
+    return emit1("take_beams_", [current, parent, logits, buf, parents, step, *state, *(into or ()), *(rule or ())],
                  dict(beams=int(beams), end=-1 if end is None else int(end), valid=valid, length_penalty=float(length_penalty), base=int(base),
                       ahead=int(ahead), advance=bool(advance)))
 
