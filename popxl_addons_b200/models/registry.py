@@ -15,6 +15,7 @@ class Architecture:
     config: Callable[[Dict[str, Any]], Any]   # entries of config.json -> configuration object
     model: Optional[Callable[..., Any]] = None  # (configuration, dtype, **options) -> model description for SequenceGenerator
     dtypes: tuple = ("bfloat16", "float32")
+    options: Callable[[], tuple] = tuple      # names of what `model` leaves to a deployment
 
 
 ARCHITECTURES: Dict[str, Architecture] = {}
@@ -51,7 +52,7 @@ def _served(name: str, module: str) -> Architecture:
             raise ValueError(f"{name} has no options {sorted(set(options) - set(getattr(cls, 'options', ())))}")
         return cls(cfg, dtype, **options)
 
-    return Architecture(name, config, model)
+    return Architecture(name, config, model, options=lambda: tuple(getattr(getattr(import_module(f"{__package__}.{module}"), name), "options", ())))
 
 
 # trained / generated with DecoderTrainer and DecoderGenerator, which take the configuration object
