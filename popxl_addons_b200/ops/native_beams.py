@@ -6,7 +6,7 @@ import torch
 
 from ..xl.opdef import native
 from ..xl.ops.beams import into_and_rule
-from .native import _CODE, _c_f, _c_int, _c_ll, _c_p, _count, _sig, _sms, _stream, counters, gemm_error_flag, workspace
+from .native import _CODE, _c_f, _c_int, _c_ll, _c_p, _count, _sig, _sms, _stream, counters, gemm_error_flag, large_scratch, workspace
 from .native_sequence import _f32, _i32, _ptr
 from .native_serving import _c_d, _done, _launched, _rows16
 
@@ -33,6 +33,9 @@ def _on_their_device(fn):
         with torch.cuda.device(dev):
             return fn(*args, **kw)
     return launch
+
+
+_GROUPS_PARTS = 160 << 20  # bytes that the parts of 2^16 rows of 128 features come to
 
 
 def _shared_few_rows(B, T, heads, G) -> bool:
@@ -73,7 +76,7 @@ def window_attention_shared_cuda(proj, q_norm, k_norm, kc, vc, pos, count, lead,
         args = (proj.data_ptr(), ld, norms[0], *caches, joint.data_ptr(), ldo, *where, *sizes, window, keep_first, int(gated), scale, sink, eps)
         flag = gemm_error_flag(dev).data_ptr()
         if _shared_few_rows(B, T, heads, G):
-            scratch = workspace(_shared_groups_scratch(B, T, heads, vdim, _sms(dev)) * 4, dev, "shared attention")
+            scratch = large_scratch(_shared_groups_scratch(B, T, heads, vdim, _sms(dev)) * 4, dev, "shared attention", _GROUPS_PARTS)
             if _launched(_shared_groups(*args, _sms(dev), scratch.data_ptr(), flag, s), "shared_attn_groups"):
                 _count("shared_attn_sum")
                 return joint
@@ -81,7 +84,7 @@ def window_attention_shared_cuda(proj, q_norm, k_norm, kc, vc, pos, count, lead,
         if rc >= 0:
             _done(rc, "shared_attn_portion")
             return joint
-    qn = torch.empty((B, G, T, heads // G, dim), dtype=torch.float32, device=dev)
+    qn = large_scratch(B * T * heads * dim * 4, dev, "shared queries", 1 << 30)
     if not _launched(append(qn), "shared_append"):
         return NotImplemented
     _done(_shared_general(qn.data_ptr(), *caches, proj.data_ptr() + plain * proj.element_size() if gated else None, ld, joint.data_ptr(), ldo, *where,
