@@ -42,7 +42,8 @@ def _shared_few_rows(B, T, heads, G) -> bool:
     """Whether a portion runs on the kernel that reads shared keys once for a group and leaves parts of sums in memory, and not on the one that has
     whole tiles of a sequence's rows and no parts. Measured with 32 heads on 8 and 4 rows per token, groups against portion: 16 sequences behind 4000
     positions 1 token 42 and 106 us, 8 tokens 76 and 111, 16 tokens 136 and 114; 16 x 8 behind 2000 8 tokens 297 and 422, 16 tokens 567 and 441; 64
-    behind 8000 8 tokens 204 and 800, 32 tokens 1004 and 855. The parts of 2^16 rows of 128 features are 136 MB."""
+    behind 8000 8 tokens 204 and 800, 32 tokens 1004 and 855. Where the two cross depends on how many share how much, which only the device knows: between 9
+    and 32 tokens of four rows each there are cases for either. The parts of 2^16 rows of 128 features are 136 MB."""
     return B <= 448 and (T == 1 or T * (heads // G) <= 32) and B * T * heads <= 1 << 16
 
 
@@ -71,12 +72,14 @@ def window_attention_shared_cuda(proj, q_norm, k_norm, kc, vc, pos, count, lead,
 
     if (dt == torch.bfloat16 and dim <= 128 and vdim <= 128 and dim % 8 == vdim % 8 == ld % 8 == ldo % 8 == 0
             and all(t.data_ptr() % 16 == 0 for t in (proj, joint, kc, vc))):
+        few = _shared_few_rows(B, T, heads, G)
+        # before the first launch: nothing, not even a wait for another stream, may come between that of the append and that of the groups
+        scratch = large_scratch(_shared_groups_scratch(B, T, heads, vdim, _sms(dev)) * 4, dev, "shared attention", _GROUPS_PARTS) if few else None
         if not _launched(append(None), "shared_append"):
             return NotImplemented
         args = (proj.data_ptr(), ld, norms[0], *caches, joint.data_ptr(), ldo, *where, *sizes, window, keep_first, int(gated), scale, sink, eps)
         flag = gemm_error_flag(dev).data_ptr()
-        if _shared_few_rows(B, T, heads, G):
-            scratch = large_scratch(_shared_groups_scratch(B, T, heads, vdim, _sms(dev)) * 4, dev, "shared attention", _GROUPS_PARTS)
+        if few:
             if _launched(_shared_groups(*args, _sms(dev), scratch.data_ptr(), flag, s), "shared_attn_groups"):
                 _count("shared_attn_sum")
                 return joint

@@ -52,3 +52,16 @@ def test_programs_share_parts_of_sums_and_queries(kind):
             assert (got - want).abs().max() <= bound * want.abs().max()
     kept = [{t.data_ptr() for tag, t in session._programs[p]["scratch"].items() if tag.startswith("shared")} for p, *_ in programs]
     assert all(len(k) == 1 and k == kept[0] for k in kept)
+
+
+@pytest.mark.gpu
+def test_nothing_comes_between_the_append_and_the_groups(monkeypatch):
+    """Taking memory may make the stream wait for another one, and the groups read what came before the append without waiting for it."""
+    from popxl_addons_b200.ops import native_beams
+    from test_shared_attention_edges import case, outputs
+
+    order = []
+    for name in ("large_scratch", "_shared_append", "_shared_groups"):
+        monkeypatch.setattr(native_beams, name, lambda *a, f=getattr(native_beams, name), n=name, **kw: order.append(n) or f(*a, **kw))
+    outputs(*case("cuda", torch.bfloat16, 4, 1, 8, 2, 64, 64, 300, 200, 1, 0, 150))
+    assert order == ["large_scratch", "_shared_append", "_shared_groups"]
