@@ -1,7 +1,7 @@
 // Sliding-window attention where the first positions of a sequence lie in the cache of another slot (attention_window.cuh): beams of one
 // prompt, requests behind one system prompt. Same mathematics and layouts as attention_window.cu.
 //
-//   xl_shared_append           new keys (norms in 64 bits, rounded once) and values into the caches; for the general kernel queries in fp32
+//   xl_shared_append           new keys (norms in 64 bits, rounded to 32 and then to the type) and values into the caches; for the general kernel queries in fp32
 //   xl_shared_attn_groups      few rows per sequence, bf16: the keys that a group of sequences shares, once for the group, on the tensor cores
 //                              (tcgen05), and behind it the sum of its parts
 //   xl_shared_attn_portion     portions of many rows per sequence on the tensor cores, bf16
@@ -122,7 +122,7 @@ __global__ void __launch_bounds__(256)
 // TMEM columns: [0, 128) S_0 / P_0, [128, 256) S_1 / P_1, [256, 256 + VD) O_0, [256 + VD, 256 + 2 VD) O_1. One CTA per SM. Every wait is
 // bounded (see tcgen05.cuh).
 //
-// The chain of a tile bounds this: scores, softmax, product. 16 x 250 tokens behind 4000, 32 heads on 8 of 128: 519 us, and 572 with the append (446 TFLOP/s
+// The chain of a tile bounds this: scores, softmax, product. 16 x 250 tokens behind 4000, 32 heads on 8 of 128: 562 us by itself, 569 with the append (448 TFLOP/s
 // of 255 GFLOP; the two numbers of queries and weights make it twice that in the tensor cores). 7700 clocks for a block of both tiles, 4096 of them products.
 // Two tiles, since a tile's softmax then has the other's products to run under, and keys are read half as often.
 constexpr int TILE_M = 128;
@@ -717,8 +717,9 @@ template <int DK, int VD> int launch_portion(const void* kc, const void* vc, con
 //   warp 2       queries of the next tile, if they are few, normalised, from the projections to shared memory;  warp 3  the list of this CTA's tiles
 //   warps 4..7, 8..11   queries of large tiles; softmax of every second block (warps without rows only keep step)
 //
-// 16 x 8 beams behind 2000, up to 130 own positions, 32 heads on 8 of 128: 70 us, 77 with the append and the sum (176 MB, 2.3 TB/s); 64 requests
-// behind 8000, up to 700 own: 75 and 86 us (183 MB). About 9 us pass before a CTA's first product; from then on about 2900 clocks per block, while loads alone take 2800.
+// 16 x 8 beams behind 2000, up to 130 own positions, 32 heads on 8 of 128: 73 us by itself, 79 with the append and the sum (176 MB, 2.2 TB/s); 64 requests
+// behind 8000, up to 700 own: 80 and 86 us (183 MB). About 9 us pass before a CTA's first product; then about 2900 clocks per block, and what it takes to
+// change from tile to tile.
 // Equal runs and not a CTA per tile and slice: groups and own parts are of unlike lengths, and one wave has to end together.
 //
 // Every CTA makes the list by itself, from positions and leads in shared memory: counts, key ranges and offsets by slot, ranks of the members by

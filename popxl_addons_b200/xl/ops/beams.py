@@ -178,7 +178,7 @@ def window_attention_shared_(proj: Tensor, q_norm: Tensor, k_norm: Tensor, k_cac
     """`window_attention_` where the first `shared[b]` positions of sequence `b` are those of slot `lead[b]` (both int32; a lead that is not
     there: none), and the others its own. Nobody shares more than both hold before the op: `min(shared[b], pos[b], pos[lead[b]])`
     positions, which have to be in the lead's own cache. New keys and values go to the sequence's own; norms of keys are taken in 64 bits and rounded
-    once, queries are not rounded to the model's type. A sequence that would not fit the cache is
+    to 32 and then to the model's type, queries are not rounded to the model's type. A sequence that would not fit the cache is
     left out, rows past `count[b]` are left as they are. A value that is not finite makes those results non-finite (at least in the feature
     concerned) that read its position, and may do so for the other results of a sequence's portion of which some read it; portions that do not are
     not touched.
