@@ -307,7 +307,7 @@ template <typename T> __global__ void __launch_bounds__(BM_THREADS, 5) take_beam
   __shared__ double top[BM_MAX_BEAMS], log_sum[BM_MAX_BEAMS], divisor[BM_MAX_BEAMS], score[BM_MAX_BEAMS], chosen_rank[BM_MAX_BEAMS], tau_d;
   __shared__ double slack[BM_MAX_BEAMS];
   __shared__ unsigned int doubt;  // rows whose sums have to be better than they are
-  __shared__ int chosen[BM_MAX_BEAMS], state[BM_MAX_BEAMS], after[BM_MAX_BEAMS], slot_of[BM_MAX_BEAMS], row_of[BM_MAX_BEAMS];  // state 0: no beam, 1: live, 2: ended
+  __shared__ int chosen[BM_MAX_BEAMS], state[BM_MAX_BEAMS], after[BM_MAX_BEAMS], slot_of[BM_MAX_BEAMS], row_of[BM_MAX_BEAMS];  // state 0: no beam, 1: live, 2: ended, 3: no beam, but marked as ended
   const int row0 = group * K;
   double* room = reinterpret_cast<double*>(smem);  // [BM_THREADS] for the bound
   const int end = end_of(a);
@@ -317,7 +317,7 @@ template <typename T> __global__ void __launch_bounds__(BM_THREADS, 5) take_beam
   if (tid < K) {
     const float f = a.scores[row0 + tid];
     const bool ended = end >= 0 && a.ended[row0 + tid] != 0;
-    state[tid] = !isfinite(f) ? 0 : ended ? 2 : 1;
+    state[tid] = !isfinite(f) ? (ended ? 3 : 0) : ended ? 2 : 1;
     score[tid] = (double)f;
     after[tid] = a.length[row0 + tid] + (ended ? 0 : 1);
     divisor[tid] = penalty == 0.0 ? 1.0 : pow((double)max(after[tid], 1), penalty);
@@ -436,7 +436,7 @@ template <typename T> __global__ void __launch_bounds__(BM_THREADS, 5) take_beam
     __syncthreads();
   }
   bool any = false;
-  for (int k = 0; k < K; ++k) any |= state[k] != 0;
+  for (int k = 0; k < K; ++k) any |= state[k] == 1 || state[k] == 2;
   if (any) {
     if (found < K) {
       if (tid == 0)
@@ -462,7 +462,7 @@ template <typename T> __global__ void __launch_bounds__(BM_THREADS, 5) take_beam
       double c = -INFINITY;
       if (tid < found) c = state[k] == 2 ? score[k] : with(k, xl_to_float(logits[(long long)(row0 + k) * a.V + token]));
       a.to_scores[to] = (float)c;
-      a.to_ended[to] = state[k] == 2 || token == end;
+      a.to_ended[to] = state[k] >= 2 || token == end;
       a.to_length[to] = after[k];
       a.current[to] = token;
       a.parent[to] = row0 + k;

@@ -79,3 +79,13 @@ def test_many_rows_that_are_alike(backend):  # noqa: F811
     check_beams(backend, rows, torch.full((groups * K,), -2.0), ended, length, K, None, V, 0.5)
     scores = -torch.arange(groups * K).float() * 2.0 ** -20  # and sums that differ by a few steps
     check_beams(backend, rows, scores, ended, length, K, None, V, 0.0)
+
+
+def test_slots_without_a_beam_that_are_marked_as_ended(backend):  # noqa: F811
+    """They fill up a group whose beams have all ended, at minus infinity, and keep their mark and their number of tokens."""
+    V, K = 40, 4
+    logits = torch.randn(3 * K, V, generator=torch.Generator().manual_seed(1)).to(backend[1])
+    scores = torch.tensor([-math.inf, -3.0, -1.5, -2.0, math.nan, -1.0, math.inf, -math.inf, -2.5, -math.inf, -math.inf, -4.0])
+    ended, length = torch.tensor([1, 1, 1, 1, 1, 1, 0, 1, 1, 0, 1, 1]).int(), torch.arange(3 * K).int() + 5
+    for end, penalty in ((3, 0.0), (0, 0.8), (None, 0.0)):
+        check_beams(backend, logits, scores, ended, length, K, end, V, penalty)
