@@ -223,10 +223,10 @@ def take_beams_(current: Tensor, parent: Tensor, logits: Tensor, buf: Tensor, pa
     a group with the largest `sum / tokens ** length_penalty` are its next beams: token `current[s]` of slot `s` continues slot
     `parent[s]`, and both become row `step + ahead - base` of `buf` and `parents (n, rows)` (ignored when out of range). Of equal ones the
     lowest slot and then the lowest token is taken. The best continuation of a beam keeps its slot, the others take the free ones, in
-    order of rank. Sums are compared in 64 bits (on the GPU those of a row are formed from exponentials in 32, and again in 64 where the choice hangs
-    on it) and kept in 32, in `into` (default: `state` itself). Without `end` no beam
-    ends, whatever `ended` holds. `rule`: `end` and `length_penalty` are those that the device holds. NaN among logits counts as minus infinity; where too few continuations are finite those at minus infinity
-    follow. A group without a finite score is left as it is, and its rows, like those of beams that have ended, are not read. With
+    order of rank. Sums are compared in 64 bits (on the GPU those of a row are formed from exponentials in 32, and again in 64 where the choice
+    hangs on it) and kept in 32, in `into` (default: `state` itself). Without `end` no beam ends, whatever `ended` holds. `rule`: `end` and
+    `length_penalty` are those that the device holds. NaN among logits counts as minus infinity; where too few continuations are finite those
+    at minus infinity follow. A group without a finite score is left as it is, and its rows, like those of beams that have ended, are not read. With
     `advance`, `step` moves on by one."""
     rows, valid = (logits.shape[0] if logits.rank == 2 else 0), int(logits.shape[-1] if valid is None else valid)
     if logits.rank != 2 or logits.dtype not in (float32, float16, bfloat16):
