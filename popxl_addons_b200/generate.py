@@ -55,7 +55,7 @@ def main(argv=None) -> int:
                      device=a.device, shaping=shaping != LogitShaping(), beams=a.beams, model_options=options)
     shaping = shaping if gen.shaping else None
     if a.beams:
-        out = [beams[0].tokens for beams in gen.generate_beams(prompts, a.max_new_tokens, a.end, a.length_penalty, shaping)]
+        out = [beams[0].tokens if beams else () for beams in gen.generate_beams(prompts, a.max_new_tokens, a.end, a.length_penalty, shaping)]
     else:
         out = gen.generate(prompts, a.max_new_tokens, shaping)
     for row in out:

@@ -55,3 +55,10 @@ def test_refusals(folder):
             generate.main(["--model", folder, "--prompt", "5", *more])
     with pytest.raises(ValueError, match="shared"):
         generate.main(["--model", folder, "--prompt", "5", "--device", "cpu", "--beams", "2", "--prefixes", "shared", "--cache", "int8"])
+
+
+def test_prompts_without_a_continuation(tmp_path, capsys):
+    """A model whose logits are no numbers leaves no beam: an empty line for each prompt."""
+    ckpt = {k: v * float("nan") if k.endswith("mix.o") else v for k, v in C.checkpoint(MODEL, 8).items()}
+    C.write_model(tmp_path, MODEL, ckpt)
+    assert lines(capsys, str(tmp_path), "--beams", "3") == [[], []]
